@@ -26,6 +26,10 @@
  *   ww_cost_stem3d            generalised 3-input CostStem3D (Cin -> Cout)
  *   ww_corr_cost_stem3d       fused CorrVolume -> CostStem3D ("CorrCostStem3D")
  *   ww_corr_cost_stem3d_band  the same over a band of image rows (multi-GPU sharding)
+ * and the attention operators of a matching network on those features:
+ *   ww_qk_norm_rope           per-head norm and rotation of queries and keys, and its gradient
+ *   ww_cross_attention        attention to states of another length with a bucketed relative
+ *                             position bias, and its gradient
  *
  * Status codes: 0 on success.  The plugin-level ww_plugin_*_enqueue calls
  * return exactly what IPluginV3OneRuntime::enqueue returns in the reference
@@ -57,8 +61,8 @@ typedef enum ww_status {
     WW_ERR_DEVICE = 7         /* no usable sm_100 device is current              */
 } ww_status_t;
 
-/* Same numeric values as nvinfer1::DataType::kFLOAT / kHALF / kINT8. */
-typedef enum ww_dtype { WW_DTYPE_FLOAT = 0, WW_DTYPE_HALF = 1, WW_DTYPE_INT8 = 2 } ww_dtype_t;
+/* Same numeric values as nvinfer1::DataType::kFLOAT / kHALF / kINT8 / kBF16. */
+typedef enum ww_dtype { WW_DTYPE_FLOAT = 0, WW_DTYPE_HALF = 1, WW_DTYPE_INT8 = 2, WW_DTYPE_BF16 = 7 } ww_dtype_t;
 
 /* Activation of the generalised / fused stem. */
 typedef enum ww_act { WW_ACT_RELU = 0, WW_ACT_RELU6 = 1 } ww_act_t;
@@ -264,6 +268,108 @@ int ww_nv12_decode(const void* nv12, void* out, int dtype, int B, int H_IN, int 
  * ------------------------------------------------------------------------- */
 int ww_disparity_regression(const void* cost, void* out, int in_dtype, int out_dtype, int B, int D, int H, int W,
                             int mode, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention operators (extensions; the reference library has no such ops, the
+ * formulas below are their specification).
+ *
+ * Tensors of vectors are [B, L, H, D] with unit stride along D and the other
+ * strides given in elements ({b, l, h}; multiples of 16 bytes; 0 = broadcast
+ * along b or h).  Outputs and gradients are contiguous.  Pointers to vectors
+ * are 16-byte aligned.  Pointers of tensors without elements may be NULL.
+ * dtypes WW_DTYPE_HALF, WW_DTYPE_BF16 and, for ww_qk_norm_rope,
+ * WW_DTYPE_FLOAT; fp32 arithmetic, one rounding to the output's type.
+ * Some calls need device scratch memory: the *_workspace functions return the
+ * bytes (0: none) for the same parameters, the caller passes a 16-byte
+ * aligned buffer of at least that size in `workspace` (else
+ * WW_ERR_UNSUPPORTED).  Results do not depend on what it holds, and the same
+ * call gives the same bits again.
+ * ------------------------------------------------------------------------- */
+
+/* Per-head RMS norm and position rotation of queries and keys in one pass.
+ *   y = x * rsqrt(mean_d x^2 + eps) * weight
+ *   (y1, y2) -> (y1 cos - y2 sin, y2 cos + y1 sin) over the first R of D dims,
+ * pairs (i, i + R/2), or (2i, 2i + 1) with interleaved != 0; the angle of
+ * pair i at position p is row p of cos / sin.  Positions default to 0, 1, ...
+ * and are clamped to [0, P).
+ * Backward: from dq_out, dk_out the gradients of q, k and of the weights
+ * (sums over all rows in fp32, joined in a fixed order). */
+typedef struct ww_qk_norm_rope {
+    const void* q;        /* [B, Lq, Hq, D] */
+    const void* k;        /* [B, Lk, Hk, D] */
+    const void* q_weight; /* [D], the type of q */
+    const void* k_weight;
+    const float* cos; /* [P, R / 2] fp32, contiguous */
+    const float* sin;
+    const int32_t* q_pos; /* [Lq] or [B, Lq] or NULL */
+    const int32_t* k_pos;
+    void* q_out;
+    void* k_out;
+    const void* dq_out; /* backward: incoming gradients */
+    const void* dk_out;
+    void* dq; /* backward: outgoing gradients */
+    void* dk;
+    void* dq_weight;
+    void* dk_weight;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t q_strides[3], k_strides[3], dq_out_strides[3], dk_out_strides[3];
+    int32_t q_pos_stride, k_pos_stride; /* elements between batch items: 0 or L */
+    int32_t dtype, B, Lq, Lk, Hq, Hk, D, R, P, interleaved;
+    float eps;
+} ww_qk_norm_rope_t;
+
+int ww_qk_norm_rope(const ww_qk_norm_rope_t* p, void* stream);
+int ww_qk_norm_rope_backward(const ww_qk_norm_rope_t* p, void* stream);
+int64_t ww_qk_norm_rope_backward_workspace(const ww_qk_norm_rope_t* p);
+
+/* Attention of queries to an encoder's states of another length.
+ *   S[b, h, i, j] = scale * q[b, i, h] . k[b, j, h / (Hq / Hk)] + table[h, bucket(j - i - q_offset)]
+ *   P = softmax of S over the valid keys j:  j < k_lens[b] and key_mask[b, j] != 0
+ *   out[b, i, h] = sum_j P v[b, j, h / (Hq / Hk)],   lse[b, h, i] = log sum_j exp S
+ * A row without a valid key gives out = 0, lse = -inf and no gradient.  What
+ * masked places of k and v hold does not matter (NaN included); their
+ * gradients are 0.  P is rounded to the inputs' 16-bit type before the second
+ * product (as are P and dS in the backward pass); sums are fp32.
+ * bucket(r): with n = num_buckets (half of them, the upper half for r > 0, if
+ * bidirectional), d = |r| (max(0, -r) if not), e = n / 2: d below e is its own
+ * bucket, the others are spaced logarithmically from e up to max_distance and
+ * the last takes everything beyond:
+ *   min(n - 1, e + floor(ln(d / e) / ln(max_distance / e) * (n - e))).
+ * A table value of -inf or the type's lowest finite value forbids its pairs.
+ * Backward: out and lse of the forward call and dout give dq, dk, dv and
+ * (with a table) dbias_table.
+ * Limits: D <= 128, D % 8 == 0; num_buckets <= 128. */
+typedef struct ww_attention {
+    const void* q; /* [B, Lq, Hq, D] */
+    const void* k; /* [B, Lk, Hk, D], Hk divides Hq */
+    const void* v;
+    void* out;               /* [B, Lq, Hq, D] contiguous (backward: read) */
+    float* lse;              /* [B, Hq, Lq] or NULL (backward: read) */
+    const int32_t* k_lens;   /* [B] (clamped to [0, Lk]) or NULL */
+    const uint8_t* key_mask; /* [B, Lk] contiguous or NULL */
+    const void* bias_table;  /* [Hq, num_buckets], the type of q, or NULL */
+    const void* dout;
+    void* dq; /* contiguous */
+    void* dk;
+    void* dv;
+    void* dbias_table;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t q_strides[3], k_strides[3], v_strides[3], dout_strides[3];
+    int32_t dtype, B, Lq, Lk, Hq, Hk, D;
+    int32_t num_buckets, max_distance, bidirectional, q_offset;
+    float scale;
+} ww_attention_t;
+
+int ww_cross_attention(const ww_attention_t* p, void* stream);
+int64_t ww_cross_attention_workspace(const ww_attention_t* p);
+int ww_cross_attention_backward(const ww_attention_t* p, void* stream);
+int64_t ww_cross_attention_backward_workspace(const ww_attention_t* p);
+
+/* Bucket of one relative position, or a negative ww_status_t for arguments
+ * that the operators reject (host only). */
+int ww_relative_position_bucket(int rel, int num_buckets, int max_distance, int bidirectional);
 
 /* BatchNorm folding on the host: w16[o, :] = fp16(w[o, :] * scale[o]) computed in
  * fp32, b16[o] = fp16(bias[o]); k = Cin * 27.  Host memory only. */

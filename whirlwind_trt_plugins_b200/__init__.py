@@ -24,6 +24,9 @@ reference project):
   (``src/plugins/nv12_decode/nv12_decode_kernel.hpp:20-28``)
 * ``disparity_regression(cost, mode, dtype)``          -- soft-argmax / soft-argmin
   after the 3-D aggregation (no reference counterpart; specified by its formula)
+* ``qk_norm_rope(...)``, ``cross_attention(...)`` and their gradients -- attention
+  of a matching network on the features (``whirlwind_trt_plugins_b200.attention``;
+  no reference counterpart)
 
 The plugin-level classes mirroring the reference's IPluginV3 plugins live in
 ``whirlwind_trt_plugins_b200.plugins``; row-band sharding over several GPUs in
@@ -39,7 +42,9 @@ __all__ = [
     "corr_cost_stem3d", "corr_cost_stem3d_band", "nv12_decode", "disparity_regression", "fold_bn", "device_error",
     "clear_device_error", "ACT_RELU", "ACT_RELU6", "DTYPE_FLOAT", "DTYPE_HALF", "DISP_SOFTARGMAX", "DISP_SOFTARGMIN",
     "MULTI_BATCH", "MULTI_ROWS", "multi_split", "corr_cost_stem3d_multi", "CORR_ENGINE_TENSOR",
-    "CORR_ENGINE_CUDA_CORES", "set_fused_corr_engine", "fused_corr_engine",
+    "CORR_ENGINE_CUDA_CORES", "set_fused_corr_engine", "fused_corr_engine", "DTYPE_BF16", "qk_norm_rope",
+    "qk_norm_rope_backward", "cross_attention", "cross_attention_backward", "qk_norm_rope_autograd",
+    "cross_attention_autograd", "relative_position_bucket",
 ]
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libww_trt_plugins.so")
@@ -433,3 +438,7 @@ def device_error() -> int:
 
 def clear_device_error() -> None:
     _check("ww_clear_device_error", _lib.ww_clear_device_error())
+
+
+from .attention import (DTYPE_BF16, cross_attention, cross_attention_autograd, cross_attention_backward,  # noqa: E402
+                        qk_norm_rope, qk_norm_rope_autograd, qk_norm_rope_backward, relative_position_bucket)

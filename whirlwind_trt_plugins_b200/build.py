@@ -37,6 +37,9 @@ SOURCES = [
     "tensor_map.cu",
     "nv12_decode.cu",
     "disparity_regression.cu",
+    "attention_host.cu",
+    "qk_norm_rope.cu",
+    "cross_attention.cu",
     "multi.cu",
     "plugin_core.cpp",
 ]

@@ -1,0 +1,97 @@
+// attention.cuh -- what the attention kernels share: 16-bit type helpers, the
+// relative-position buckets and the argument checks.
+#pragma once
+
+#include "ww_common.cuh"
+
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+namespace ww {
+
+constexpr float kLog2eF = 1.4426950408889634f;
+constexpr float kLn2F = 0.6931471805599453f;
+constexpr int kMaxBuckets = 128;
+
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(float x) { return x; }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Relative-position buckets.  Distance d >= exact is in bucket
+// exact + #{t : least[t] <= d}: least[t] is the smallest whole distance of
+// logarithmic bucket t + 1, found once per call on the host, so that the
+// kernels compare whole numbers and no logarithm is rounded at an edge.
+struct RelBuckets {
+    int32_t per_side = 0;  // buckets of one direction; 0: no bias
+    int32_t exact = 0;
+    int32_t bidirectional = 0;
+    int32_t q_offset = 0;
+    int32_t total = 0;
+    int32_t max_distance = 0;  // |rel| >= this: last bucket of its side
+    int32_t n_least = 0;
+    int32_t least[kMaxBuckets / 2];
+};
+
+__host__ __device__ __forceinline__ int rel_bucket(const RelBuckets& r, int rel)
+{
+    int first = 0, d;
+    if (r.bidirectional) {
+        d = rel < 0 ? -rel : rel;
+        if (rel > 0) first = r.per_side;
+    } else {
+        d = rel < 0 ? -rel : 0;
+    }
+    if (d < r.exact) return first + d;
+    int lo = 0, hi = r.n_least;  // first t with least[t] > d
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (r.least[mid] <= d) lo = mid + 1;
+        else hi = mid;
+    }
+    return first + r.exact + lo;
+}
+
+// A bias at the type's lowest finite value forbids the pair like -inf: a row
+// of such biases alone is empty instead of a softmax of rounding errors.
+template <typename T>
+__device__ __forceinline__ float bias_value(T b);
+template <>
+__device__ __forceinline__ float bias_value<__half>(__half b)
+{
+    const float f = __half2float(b);
+    return f <= -65504.0f ? -INFINITY : f;
+}
+template <>
+__device__ __forceinline__ float bias_value<__nv_bfloat16>(__nv_bfloat16 b)
+{
+    const float f = __bfloat162float(b);
+    return f <= -0x1.fep127f ? -INFINITY : f;
+}
+
+// Fills `out`; WW_SUCCESS or the status of rejected arguments (attention_host.cu).
+int make_buckets(int num_buckets, int max_distance, int bidirectional, int q_offset, RelBuckets* out) noexcept;
+
+// Checks the arguments that both directions of ww_cross_attention share.
+int check_attention(const ww_attention_t& p) noexcept;
+// What only the gradient needs: its pointers and `need` bytes of workspace.
+int check_attention_backward(const ww_attention_t& p, int64_t need) noexcept;
+bool vectors_ok(const void* ptr, const int64_t (&strides)[3], int B, int L, int H, int elem_bytes) noexcept;
+
+}  // namespace ww
