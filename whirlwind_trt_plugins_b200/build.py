@@ -39,7 +39,8 @@ SOURCES = [
     "disparity_regression.cu",
     "attention_host.cu",
     "qk_norm_rope.cu",
-    "cross_attention.cu",
+    "attention_forward.cu",
+    "attention_backward.cu",
     "multi.cu",
     "plugin_core.cpp",
 ]

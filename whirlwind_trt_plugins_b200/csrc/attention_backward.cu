@@ -1,7 +1,6 @@
-// cross_attention.cu -- attention of queries to an encoder's states of another
-// length, with a learned relative position bias by buckets, and its gradient.
+// attention_backward.cu -- ww_cross_attention_backward.
 //
-// One warp per query row (forward, dq) or key row (dk, dv): 32 scores at a
+// One warp per query row (dq) or key row (dk, dv): 32 scores at a
 // time, one per lane, with the running maximum and sum of the softmax; the
 // second product runs over the 32 rows with the lanes across the head's dims.
 #include "attention.cuh"
@@ -53,51 +52,6 @@ __device__ __forceinline__ float bias_of(const AttnParams& p, int h, int i, int 
 {
     if (p.rel.per_side == 0) return 0.0f;
     return bias_value<T>(static_cast<const T*>(p.a.bias_table)[h * p.rel.total + rel_bucket(p.rel, j - i - p.rel.q_offset)]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) forward_kernel(const __grid_constant__ AttnParams p)
-{
-    __shared__ float qs[kWarps][128];
-    const ww_attention_t& a = p.a;
-    const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int rb = blockIdx.x % p.row_blocks, bh = blockIdx.x / p.row_blocks;
-    const int b = bh / a.Hq, h = bh % a.Hq, g = h / (a.Hq / a.Hk);
-    const int i = rb * kWarps + w;
-    if (i >= a.Lq) return;
-    const T* q = row<T>(a.q, a.q_strides, b, i, h);
-    for (int d = lane; d < a.D; d += 32) qs[w][d] = to_float(q[d]);
-    __syncwarp();
-    float m = -INFINITY, sum = 0.0f, acc[4] = {};
-    const int len = key_count(a, b);
-    for (int j0 = 0; j0 < len; j0 += 32) {
-        const int j = j0 + lane;
-        float s = -INFINITY;
-        const bool ok = valid_key(a, b, j, len);
-        if (ok) s = dot(row<T>(a.k, a.k_strides, b, j, g), qs[w], a.D) * a.scale + bias_of<T>(p, h, i, j);
-        float mc = s;
-        for (int o = 16; o > 0; o >>= 1) mc = fmaxf(mc, __shfl_xor_sync(~0u, mc, o));
-        const float mn = fmaxf(m, mc), ms = mn == -INFINITY ? 0.0f : mn;
-        const float pr = ok ? exp2_approx((s - ms) * kLog2eF) : 0.0f;
-        const float f = exp2_approx((m - ms) * kLog2eF);
-        m = mn;
-        sum = sum * f + pr;
-        for (int t = 0; t < 4; ++t) acc[t] *= f;
-        for (int n = 0; n < 32; ++n) {
-            const float pn = __shfl_sync(~0u, pr, n);
-            if (pn == 0.0f) continue;
-            const T* v = row<T>(a.v, a.v_strides, b, j0 + n, g);
-            for (int t = 0; t < 4; ++t)
-                if (lane + 32 * t < a.D) acc[t] += pn * to_float(v[lane + 32 * t]);
-        }
-    }
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.Lq + i) * a.Hq + h) * a.D;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int t = 0; t < 4; ++t)
-        if (lane + 32 * t < a.D) out[lane + 32 * t] = from_float<T>(acc[t] * inv);
-    if (a.lse != nullptr && lane == 0)
-        a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Lq + i] = sum == 0.0f ? -INFINITY : m + logf(sum);
 }
 
 template <typename T>
@@ -241,15 +195,6 @@ void fill(const ww_attention_t& p, AttnParams* out)
 }
 
 template <typename T>
-int forward(const ww_attention_t& p, cudaStream_t s)
-{
-    AttnParams r;
-    fill(p, &r);
-    forward_kernel<T><<<r.row_blocks * p.B * p.Hq, 32 * kWarps, 0, s>>>(r);
-    return launch_status("cross_attention");
-}
-
-template <typename T>
 int backward(const ww_attention_t& p, cudaStream_t s)
 {
     AttnParams r;
@@ -265,19 +210,6 @@ int backward(const ww_attention_t& p, cudaStream_t s)
 }  // namespace ww
 
 extern "C" {
-
-int64_t ww_cross_attention_workspace(const ww_attention_t*) { return 0; }
-
-int ww_cross_attention(const ww_attention_t* p, void* stream)
-{
-    if (p == nullptr) return WW_ERR_NULL_POINTER;
-    int st = ww::check_attention(*p);
-    if (st != WW_SUCCESS || p->B == 0 || p->Lq == 0) return st;
-    ww::DeviceInfo d;
-    if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return p->dtype == WW_DTYPE_HALF ? ww::forward<__half>(*p, s) : ww::forward<__nv_bfloat16>(*p, s);
-}
 
 int64_t ww_cross_attention_backward_workspace(const ww_attention_t* p)
 {

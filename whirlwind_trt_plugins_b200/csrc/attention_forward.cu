@@ -1,0 +1,578 @@
+// attention_forward.cu -- ww_cross_attention: softmax(scale Q K^T + bias) V on
+// the 5th-generation tensor cores, one pass over the keys.
+//
+// For a tile of 128 query rows and 128 keys at a time, with x = scale log2(e) s
+// + bias log2(e) the scores in log2 units:
+//
+//   S = Q K^T                       tcgen05.mma, operands staged by TMA, S in TMEM
+//   m' = max(m, max_j x_j)          one thread per row: its 128 scores from TMEM
+//   P_j = 2^(x_j - m'), l = l 2^(m - m') + sum_j P_j
+//   O = O 2^(m - m') + P V          P goes back to TMEM as the A operand
+//   out = O / l, lse = ln 2 (m + log2 l)
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the
+// last time (P then stays below 2^8, exact in 16 bits' range): after the first
+// tiles that hardly happens, and no tile needs the read-multiply-write of O.
+//
+// Roles: 4 warps per query tile turn scores into P; one thread issues every
+// MMA; one thread every TMA load.  P overwrites the first half of its scores'
+// columns, and the next S of a tile is issued behind the product that reads
+// that P (MMAs of a CTA run in issue order).  What hides the round trip of a
+// tile is a second one: NT = 2 query tiles of one CTA against the same keys, or
+// two CTAs of one tile on an SM.
+//
+// Bound: the exponential, 16 per clock and SM: 1024 clocks for a tile of
+// 128 x 128, against 2 x 8 D clocks for its products (8192 fp16 FMA per clock):
+// 512 clocks at D = 32, equal at D = 64 ... 128.
+//
+// Masked keys get P = 0 and their rows of V are zeroed in shared memory (0 times
+// a NaN would not be 0); tiles without a masked key skip all of it.
+// The relative bias of a tile depends on j - i alone: its 255 values are put
+// into shared memory per tile (the bucket search runs twice per thread), a row
+// reads them at a fixed offset from its own start; tiles whose distances all
+// lie in one bucket add a constant.
+//
+// Few rows against many keys: the keys are split over CTAs, each writes its
+// normalised fp32 rows and log sums, a second kernel joins them in order.
+#include "attention.cuh"
+#include "tensor_map.cuh"
+#include "umma.cuh"
+
+#include <algorithm>
+
+namespace ww {
+namespace {
+
+constexpr int kTile = 128;       // query rows and keys of a tile
+constexpr float kRescale = 8.0f; // log2 growth of the maximum that is left in P
+
+struct FwdParams {
+    CUtensorMap q, k, v;
+    void* out;
+    float* lse;
+    const int32_t* k_lens;
+    const uint8_t* key_mask;
+    const void* table;
+    float* part_o;    // [splits][B * Lq * Hq][D], splits > 1
+    float* part_lse;  // [splits][B * Lq * Hq], log2
+    RelBuckets rel;
+    int32_t B, Lq, Lk, Hq, group, D;
+    int32_t q_blocks, splits;
+    int32_t q_b, q_h, k_b, k_h, v_b, v_h;  // 0 where the tensor is broadcast
+    float scale2;                          // scale * log2(e)
+    int* err;
+};
+
+template <int DP, int NT>
+struct Layout {
+    static constexpr int kRow = DP == 32 ? 64 : 128;       // bytes of an operand row
+    static constexpr int kCols = kRow / 2;                 // values in it
+    static constexpr int kChunks = DP * 2 / kRow;          // rows of one token
+    static constexpr int kChunkBytes = kTile * kRow;
+    static constexpr int kTileBytes = kTile * DP * 2;
+    static constexpr int kStages = DP == 128 ? 2 : (NT == 2 ? 3 : 2);
+    static constexpr int kQ = 0;
+    static constexpr int kK = NT * kTileBytes;
+    static constexpr int kV = kK + kStages * kTileBytes;
+    static constexpr int kWin = kV + kStages * kTileBytes;         // NT x 2 windows of 256 floats
+    static constexpr int kBar = kWin + NT * 2 * 256 * 4;
+    static constexpr int kBytes = kBar + 256 + 1024;               // + alignment of the base
+    static constexpr int kColumns = NT * (kTile + DP) <= 256 ? 256 : 512;
+    static constexpr int kThreads = NT * 128 + 64;
+};
+
+template <int DP, int NT>
+struct Bars {
+    static constexpr int kStages = Layout<DP, NT>::kStages;
+    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], p_ready[NT],
+        o_full[NT];
+    uint32_t tmem;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ float f32(uint32_t u) { return __uint_as_float(u); }
+
+// Barrier of the 128 threads of query tile t.
+__device__ __forceinline__ void tile_sync(int t)
+{
+    if (t == 0) asm volatile("bar.sync 1, 128;" : : : "memory");
+    else asm volatile("bar.sync 2, 128;" : : : "memory");
+}
+
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) attention_forward_kernel(const __grid_constant__ FwdParams p)
+{
+    using L = Layout<DP, NT>;
+    using Bar = Bars<DP, NT>;
+    constexpr int S = L::kStages;
+    extern __shared__ uint8_t raw[];
+    uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
+    const uint32_t sm = umma::smem_addr(base);
+    Bar* bar = reinterpret_cast<Bar*>(base + L::kBar);
+    const auto at = [](const uint64_t& b) { return umma::smem_addr(&b); };
+
+    const int split = blockIdx.x % p.splits;
+    int rest = blockIdx.x / p.splits;
+    const int qb = rest % p.q_blocks;
+    rest /= p.q_blocks;
+    const int h = rest % p.Hq, b = rest / p.Hq;
+    const int q0 = qb * (NT * kTile);
+    const int tiles = NT == 1 || q0 + kTile >= p.Lq ? 1 : 2;  // query tiles with rows
+    const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
+    const int n_all = (len + kTile - 1) / kTile;
+    const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / p.splits);
+    const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / p.splits) - first;
+
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x == 0) {
+        umma::mbar_init(at(bar->q_full), 1);
+        for (int s = 0; s < S; ++s) {
+            umma::mbar_init(at(bar->k_full[s]), 1);
+            umma::mbar_init(at(bar->k_empty[s]), 1);
+            umma::mbar_init(at(bar->v_full[s]), 1);
+            umma::mbar_init(at(bar->v_empty[s]), 1);
+        }
+        for (int t = 0; t < NT; ++t) {
+            umma::mbar_init(at(bar->s_full[t]), 1);
+            umma::mbar_init(at(bar->p_ready[t]), 128);
+            umma::mbar_init(at(bar->o_full[t]), 1);
+        }
+        umma::mbar_fence_init();
+    }
+    if (warp == NT * 4) umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = bar->tmem;
+    // columns: S (then P) of each tile, then O of each tile
+    const auto s_col = [&](int t) { return tmem + t * kTile; };
+    const auto o_col = [&](int t) { return tmem + NT * kTile + t * DP; };
+    // columns of key tile n-th that hold keys
+    const auto cols_of = [&](int kt) { return min(kTile, len - (first + kt) * kTile); };
+
+    if (warp == NT * 4 + 1) {
+        if ((threadIdx.x & 31) == 0 && n > 0) {
+            umma::tma_prefetch_desc(&p.q);
+            umma::tma_prefetch_desc(&p.k);
+            umma::tma_prefetch_desc(&p.v);
+            umma::mbar_arrive_expect_tx(at(bar->q_full), tiles * L::kTileBytes);
+            for (int t = 0; t < tiles; ++t)
+                for (int c = 0; c < L::kChunks; ++c)
+                    umma::tma_load_4d(sm + L::kQ + t * L::kTileBytes + c * L::kChunkBytes, &p.q, c * L::kCols,
+                                      h * p.q_h, q0 + t * kTile, b * p.q_b, at(bar->q_full));
+            const int g = h / p.group;
+            bool ok = true;
+            for (int kt = 0; kt < n && ok; ++kt) {
+                const int s = kt % S;
+                const uint32_t ph = (kt / S + 1) & 1;
+                const int l0 = (first + kt) * kTile;
+                ok = umma::mbar_wait(at(bar->k_empty[s]), ph);
+                if (!ok) break;
+                umma::mbar_arrive_expect_tx(at(bar->k_full[s]), L::kTileBytes);
+                for (int c = 0; c < L::kChunks; ++c)
+                    umma::tma_load_4d(sm + L::kK + s * L::kTileBytes + c * L::kChunkBytes, &p.k, c * L::kCols,
+                                      g * p.k_h, l0, b * p.k_b, at(bar->k_full[s]));
+                ok = umma::mbar_wait(at(bar->v_empty[s]), ph);
+                if (!ok) break;
+                umma::mbar_arrive_expect_tx(at(bar->v_full[s]), L::kTileBytes);
+                for (int c = 0; c < L::kChunks; ++c)
+                    umma::tma_load_4d(sm + L::kV + s * L::kTileBytes + c * L::kChunkBytes, &p.v, c * L::kCols,
+                                      g * p.v_h, l0, b * p.v_b, at(bar->v_full[s]));
+            }
+            if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x20);
+        }
+    } else if (warp == NT * 4) {
+        if ((threadIdx.x & 31) == 0 && n > 0) {
+            constexpr bool bf = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+            const int steps = (p.D + 15) / 16;
+            const auto qk = [&](int t, int kt) {
+                const int s = kt % S;
+                const uint32_t id = umma::idesc_16bit(bf, kTile, (cols_of(kt) + 15) / 16 * 16, false);
+                for (int i = 0; i < steps; ++i) {
+                    const uint32_t off = (i * 16 / L::kCols) * L::kChunkBytes + (i * 16 % L::kCols) * 2;
+                    umma::mma_f16_ss(s_col(t),
+                                     umma::smem_desc_swizzled<L::kRow>(sm + L::kQ + t * L::kTileBytes + off, 16),
+                                     umma::smem_desc_swizzled<L::kRow>(sm + L::kK + s * L::kTileBytes + off, 16), id,
+                                     i > 0);
+                }
+                umma::mma_commit(at(bar->s_full[t]));
+            };
+            bool ok = umma::mbar_wait(at(bar->q_full), 0) && umma::mbar_wait(at(bar->k_full[0]), 0);
+            if (ok) {
+                for (int t = 0; t < tiles; ++t) qk(t, 0);
+                umma::mma_commit(at(bar->k_empty[0]));
+            }
+            for (int kt = 0; kt < n && ok; ++kt) {
+                const int s = kt % S, s1 = (kt + 1) % S;
+                const uint32_t id = umma::idesc_16bit(bf, kTile, DP, true);
+                const int ksteps = (cols_of(kt) + 15) / 16;
+                for (int t = 0; t < tiles && ok; ++t) {
+                    if (t == 0) ok = umma::mbar_wait(at(bar->v_full[s]), (kt / S) & 1);
+                    ok = ok && umma::mbar_wait(at(bar->p_ready[t]), kt & 1);
+                    if (!ok) break;
+                    umma::fence_after_sync();
+                    for (int i = 0; i < ksteps; ++i)
+                        umma::mma_f16_ts(o_col(t), s_col(t) + i * 8,
+                                         umma::smem_desc_swizzled<L::kRow>(
+                                             sm + L::kV + s * L::kTileBytes + i * 16 * L::kRow, L::kChunkBytes),
+                                         id, kt > 0 || i > 0);
+                    if (t == tiles - 1) umma::mma_commit(at(bar->v_empty[s]));
+                    if (kt + 1 < n) {
+                        if (t == 0) ok = umma::mbar_wait(at(bar->k_full[s1]), ((kt + 1) / S) & 1);
+                        if (!ok) break;
+                        qk(t, kt + 1);
+                        if (t == tiles - 1) umma::mma_commit(at(bar->k_empty[s1]));
+                    } else {
+                        umma::mma_commit(at(bar->o_full[t]));
+                    }
+                }
+            }
+            if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x21);
+        }
+    } else if (warp / 4 < tiles) {
+        const int t = warp / 4, r = threadIdx.x % 128, lane = threadIdx.x % 32;
+        const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;  // TMEM lane of this warp's first row
+        const int i = q0 + t * kTile + r;
+        float* win = reinterpret_cast<float*>(base + L::kWin) + t * 512;
+        float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        bool ok = true;  // once a wait has run out: no more waits, but every barrier of the tile is kept
+        uint32_t x[kTile];
+        for (int kt = 0; kt < n; ++kt) {
+            const int k0 = (first + kt) * kTile, cols = cols_of(kt);
+            // which of the 128 keys count
+            uint32_t keep[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int left = cols - 32 * c;
+                keep[c] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+                if (p.key_mask != nullptr)
+                    keep[c] &= __ballot_sync(~0u, 32 * c + lane < cols &&
+                                             __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + k0 + 32 * c + lane) != 0);
+            }
+            const bool whole = (keep[0] & keep[1] & keep[2] & keep[3]) == ~0u;
+            // the bias: one value for the tile, or a window over j - i
+            float flat = 0.0f;
+            const float* mine = nullptr;
+            if (p.rel.per_side != 0) {
+                const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
+                const int rel0 = k0 - (q0 + t * kTile) - p.rel.q_offset;
+                const int lo = rel_bucket(p.rel, rel0 - 127);
+                if (lo == rel_bucket(p.rel, rel0 + 127)) {
+                    flat = bias_value<T>(table[lo]) * kLog2eF;
+                } else {
+                    float* w = win + (kt & 1) * 256;
+                    w[r] = bias_value<T>(table[rel_bucket(p.rel, rel0 - 127 + r)]) * kLog2eF;
+                    w[r + 128] = bias_value<T>(table[rel_bucket(p.rel, rel0 + 1 + r)]) * kLog2eF;
+                    tile_sync(t);
+                    mine = w + 127 - r;
+                }
+            }
+            ok = ok && umma::mbar_wait(at(bar->s_full[t]), kt & 1);
+            umma::fence_after_sync();
+            const int chunks = (cols + 31) / 32;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < chunks) umma::tmem_ld32(s_col(t) + lanes + c * 32, x + c * 32);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < chunks) umma::tmem_wait_ld32(x + c * 32);
+
+            const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f;
+            float top = -INFINITY;
+            if (plain) {
+                float top1 = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < kTile; j += 2) {
+                    top = fmaxf(top, f32(x[j]));
+                    top1 = fmaxf(top1, f32(x[j + 1]));
+                }
+                top = fmaf(fmaxf(top, top1), p.scale2, flat);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c >= chunks) continue;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float y = fmaf(f32(x[32 * c + j]), p.scale2, mine != nullptr ? mine[32 * c + j] : flat);
+                        y = (keep[c] >> j) & 1 ? y : -INFINITY;
+                        top = fmaxf(top, y);
+                        x[32 * c + j] = __float_as_uint(y);
+                    }
+                }
+            }
+            // grow the maximum: always on the first tile, then only past kRescale
+            const bool grow = kt == 0 || top > m + kRescale;
+            if (__any_sync(~0u, grow)) {
+                const float mn = fmaxf(m, top);
+                if (kt > 0) {
+                    const float f = exp2_approx(m == -INFINITY ? -INFINITY : m - mn);
+                    l0 *= f;
+                    l1 *= f;
+#pragma unroll
+                    for (int c = 0; c < DP; c += 16) {
+                        uint32_t o[16];
+                        umma::tmem_ld16(o_col(t) + lanes + c, o);
+                        umma::tmem_wait_ld16(o);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(f32(o[j]) * f);
+                        umma::tmem_st16(o_col(t) + lanes + c, o);
+                    }
+                }
+                m = mn;
+            }
+            const float ms = m == -INFINITY ? 0.0f : m;
+            const float mul = plain ? p.scale2 : 1.0f, add = (plain ? flat : 0.0f) - ms;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (c >= chunks) continue;
+                uint32_t pk[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float a = exp2_approx(fmaf(f32(x[32 * c + 2 * j]), mul, add));
+                    const float e = exp2_approx(fmaf(f32(x[32 * c + 2 * j + 1]), mul, add));
+                    l0 += a;
+                    l1 += e;
+                    pk[j] = pack2<T>(a, e);
+                }
+                umma::tmem_st16(s_col(t) + lanes + c * 16, pk);
+            }
+            if (!whole) {
+                // rows of V behind masked keys: 0 in place of whatever they hold
+                const int s = kt % S;
+                ok = ok && umma::mbar_wait(at(bar->v_full[s]), (kt / S) & 1);
+                if (!((keep[warp % 4] >> lane) & 1)) {
+                    for (int c = 0; c < L::kChunks; ++c)
+#pragma unroll
+                        for (int j = 0; j < L::kRow; j += 16)
+                            umma::st_shared_v4(sm + L::kV + s * L::kTileBytes + c * L::kChunkBytes + r * L::kRow + j, 0, 0,
+                                               0, 0);
+                }
+                umma::fence_proxy_async_smem();
+            }
+            umma::tmem_wait_st();
+            umma::fence_before_sync();
+            umma::mbar_arrive(at(bar->p_ready[t]));
+        }
+        if (ok && n > 0) ok = umma::mbar_wait(at(bar->o_full[t]), 0);
+        umma::fence_after_sync();
+        if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x22);
+        const float sum = l0 + l1;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
+        const int64_t rows = static_cast<int64_t>(p.B) * p.Lq * p.Hq;
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            if (n > 0) {
+                umma::tmem_ld32(o_col(t) + lanes + c, o);
+                umma::tmem_wait_ld32(o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = 0;
+            }
+            if (i >= p.Lq) continue;
+            if (p.splits > 1) {
+                float* to = p.part_o + (split * rows + row) * p.D + c;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    if (c + j < p.D)
+                        *reinterpret_cast<float4*>(to + j) =
+                            make_float4(f32(o[j]) * inv, f32(o[j + 1]) * inv, f32(o[j + 2]) * inv, f32(o[j + 3]) * inv);
+            } else {
+                T* to = static_cast<T*>(p.out) + row * p.D + c;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8)
+                    if (c + j < p.D)
+                        *reinterpret_cast<uint4*>(to + j) = make_uint4(
+                            pack2<T>(f32(o[j]) * inv, f32(o[j + 1]) * inv), pack2<T>(f32(o[j + 2]) * inv, f32(o[j + 3]) * inv),
+                            pack2<T>(f32(o[j + 4]) * inv, f32(o[j + 5]) * inv),
+                            pack2<T>(f32(o[j + 6]) * inv, f32(o[j + 7]) * inv));
+            }
+        }
+        if (i < p.Lq) {
+            const float lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
+            if (p.splits > 1) p.part_lse[split * rows + row] = lse2;
+            else if (p.lse != nullptr) p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Lq + i] = lse2 * kLn2F;
+        }
+        umma::fence_before_sync();
+    }
+    __syncthreads();
+    if (warp == NT * 4) {
+        umma::fence_after_sync();
+        umma::tmem_dealloc(tmem, L::kColumns);
+    }
+}
+
+// Joins the splits of a row: out = sum_s 2^(lse_s - top) out_s / sum_s 2^(lse_s - top).
+// One warp per row, 4 values per lane.
+template <typename T>
+__global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o, const float* part_lse, void* out,
+                                                             float* lse, int splits, int64_t rows, int Lq, int Hq, int D)
+{
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    if (row >= rows) return;
+    float top = -INFINITY;
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + row]);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    float4 acc = make_float4(0, 0, 0, 0);
+    for (int s = 0; s < splits; ++s) {
+        const float w = exp2_approx(part_lse[s * rows + row] - base);
+        sum += w;
+        if (w != 0.0f && lane * 4 < D) {
+            const float4 v = *reinterpret_cast<const float4*>(part_o + (s * rows + row) * D + lane * 4);
+            acc.x += w * v.x;
+            acc.y += w * v.y;
+            acc.z += w * v.z;
+            acc.w += w * v.w;
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (lane * 4 < D)
+        *reinterpret_cast<uint2*>(static_cast<T*>(out) + row * D + lane * 4) =
+            make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    if (lse != nullptr && lane == 0) {
+        const int h = static_cast<int>(row % Hq);
+        const int64_t bi = row / Hq, b = bi / Lq, i = bi % Lq;
+        lse[(b * Hq + h) * Lq + i] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * kLn2F;
+    }
+}
+
+// How a call runs: query tiles per CTA, CTAs over the keys.
+struct Plan {
+    int nt, q_blocks, splits;
+    int64_t part_bytes;
+};
+
+Plan make_plan(const ww_attention_t& p, int sms) noexcept
+{
+    Plan r;
+    r.nt = p.Lq > 1024 ? 2 : 1;
+    r.q_blocks = (p.Lq + r.nt * kTile - 1) / (r.nt * kTile);
+    const int64_t ctas = i64(r.q_blocks) * p.B * p.Hq;
+    const int key_tiles = (p.Lk + kTile - 1) / kTile;
+    r.splits = 1;
+    if (ctas > 0 && ctas < sms && key_tiles >= 4)
+        r.splits = static_cast<int>(std::min<int64_t>({2 * i64(sms) / ctas, key_tiles / 2, 64}));
+    const int64_t rows = i64(p.B) * p.Lq * p.Hq;
+    r.part_bytes = r.splits > 1 ? r.splits * rows * (p.D + 1) * 4 : 0;
+    return r;
+}
+
+template <typename T, int DP, int NT>
+int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
+{
+    using L = Layout<DP, NT>;
+    const auto kernel = attention_forward_kernel<T, DP, NT>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
+        return launch_status("cross_attention");
+    kernel<<<static_cast<unsigned>(ctas), L::kThreads, L::kBytes, stream>>>(f);
+    return launch_status("cross_attention");
+}
+
+template <typename T>
+int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noexcept
+{
+    FwdParams f;
+    const int dp = p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128;
+    constexpr bool bf = !std::is_same<T, __half>::value;
+    const int nq[3] = {p.B, p.Lq, p.Hq}, nk[3] = {p.B, p.Lk, p.Hk};
+    const int cols = dp == 32 ? 32 : 64;
+    if (!encode_vectors_map(&f.q, bf, p.q, p.D, nq, p.q_strides, cols, kTile)) return WW_ERR_UNSUPPORTED;
+    if (p.Lk > 0) {
+        if (!encode_vectors_map(&f.k, bf, p.k, p.D, nk, p.k_strides, cols, kTile) ||
+            !encode_vectors_map(&f.v, bf, p.v, p.D, nk, p.v_strides, cols, kTile))
+            return WW_ERR_UNSUPPORTED;
+    }
+    f.out = p.out;
+    f.lse = p.lse;
+    f.k_lens = p.k_lens;
+    f.key_mask = p.key_mask;
+    f.table = p.bias_table;
+    if (p.bias_table != nullptr)
+        make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
+    const int64_t rows = i64(p.B) * p.Lq * p.Hq;
+    f.part_o = static_cast<float*>(p.workspace);
+    f.part_lse = f.part_o + plan.splits * rows * p.D;
+    f.B = p.B;
+    f.Lq = p.Lq;
+    f.Lk = p.Lk;
+    f.Hq = p.Hq;
+    f.group = p.Hq / p.Hk;
+    f.D = p.D;
+    f.q_blocks = plan.q_blocks;
+    f.splits = plan.splits;
+    f.q_b = p.q_strides[0] != 0;
+    f.q_h = p.q_strides[2] != 0;
+    f.k_b = p.k_strides[0] != 0;
+    f.k_h = p.k_strides[2] != 0;
+    f.v_b = p.v_strides[0] != 0;
+    f.v_h = p.v_strides[2] != 0;
+    f.scale2 = p.scale * kLog2eF;
+    f.err = device_error_slot();
+    const int64_t ctas = i64(plan.q_blocks) * p.B * p.Hq * plan.splits;
+    if (f.err == nullptr) return WW_ERR_DEVICE;
+    if (ctas > 0x7fffffff) return WW_ERR_UNSUPPORTED;
+    int st;
+    if (plan.nt == 1)
+        st = dp == 32 ? launch<T, 32, 1>(f, ctas, stream)
+           : dp == 64 ? launch<T, 64, 1>(f, ctas, stream) : launch<T, 128, 1>(f, ctas, stream);
+    else
+        st = dp == 32 ? launch<T, 32, 2>(f, ctas, stream)
+           : dp == 64 ? launch<T, 64, 2>(f, ctas, stream) : launch<T, 128, 2>(f, ctas, stream);
+    if (st != WW_SUCCESS || plan.splits == 1) return st;
+    attention_join_kernel<T><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
+        f.part_o, f.part_lse, p.out, p.lse, plan.splits, rows, p.Lq, p.Hq, p.D);
+    return launch_status("cross_attention");
+}
+
+int sm_count() noexcept
+{
+    DeviceInfo d;
+    return current_device_info(&d) == WW_SUCCESS ? d.sm_count : 148;
+}
+
+}  // namespace
+}  // namespace ww
+
+extern "C" {
+
+int64_t ww_cross_attention_workspace(const ww_attention_t* p)
+{
+    if (p == nullptr || ww::check_attention(*p) != WW_SUCCESS) return 0;
+    return ww::make_plan(*p, ww::sm_count()).part_bytes;
+}
+
+int ww_cross_attention(const ww_attention_t* p, void* stream)
+{
+    if (p == nullptr) return WW_ERR_NULL_POINTER;
+    int st = ww::check_attention(*p);
+    if (st != WW_SUCCESS || p->B == 0 || p->Lq == 0) return st;
+    ww::DeviceInfo d;
+    if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
+    const ww::Plan plan = ww::make_plan(*p, d.sm_count);
+    if (plan.part_bytes > 0 && p->workspace == nullptr) return WW_ERR_NULL_POINTER;
+    if (plan.part_bytes > p->workspace_bytes) return WW_ERR_UNSUPPORTED;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return p->dtype == WW_DTYPE_HALF ? ww::forward<__half>(*p, plan, s) : ww::forward<__nv_bfloat16>(*p, plan, s);
+}
+
+}  // extern "C"

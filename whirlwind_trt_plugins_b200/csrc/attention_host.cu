@@ -38,7 +38,7 @@ bool vectors_ok(const void* ptr, const int64_t (&strides)[3], int B, int L, int 
     const int n[3] = {B, L, H};
     for (int i = 0; i < 3; ++i)
         if (n[i] > 1 && (strides[i] < 0 || (strides[i] * elem_bytes) % 16 != 0)) return false;
-    return true;
+    return L <= 1 || strides[1] != 0;  // broadcast along b and h only
 }
 
 int check_attention(const ww_attention_t& p) noexcept

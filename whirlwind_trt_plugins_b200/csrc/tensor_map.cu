@@ -73,4 +73,33 @@ bool encode_volume_map(CUtensorMap* out, const void* base, int B, int G, int D, 
     return r == CUDA_SUCCESS;
 }
 
+bool encode_vectors_map(CUtensorMap* out, bool bf16, const void* base, int D, const int (&n)[3],
+                        const int64_t (&strides)[3], int box_cols, int box_rows) noexcept
+{
+    if (out == nullptr || base == nullptr || reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+    if (D <= 0 || (box_cols != 32 && box_cols != 64) || box_rows <= 0 || box_rows > 256) return false;
+    const EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    // n and strides are {b, l, h}; the map's dims are innermost first: D, h, l, b.
+    // A dim without a stride of its own (one element, or broadcast) gets extent 1.
+    cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), 1, 1, 1};
+    cuuint64_t st[3] = {16, 16, 16};
+    constexpr int from[3] = {2, 1, 0};
+    for (int i = 0; i < 3; ++i) {
+        const int a = from[i];
+        if (n[a] <= 0) return false;
+        if (n[a] == 1 || strides[a] == 0) continue;
+        if (strides[a] < 0 || (strides[a] * 2) % 16 != 0 || strides[a] * 2 >= (int64_t{1} << 40)) return false;
+        dims[i + 1] = static_cast<cuuint64_t>(n[a]);
+        st[i] = static_cast<cuuint64_t>(strides[a]) * 2;
+    }
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(box_cols), 1u, static_cast<cuuint32_t>(box_rows), 1u};
+    const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                          const_cast<void*>(base), dims, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS;
+}
+
 }  // namespace ww

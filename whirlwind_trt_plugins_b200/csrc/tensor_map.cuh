@@ -24,4 +24,11 @@ bool encode_feature_map(CUtensorMap* out, const void* base, int B, int C, int ro
 bool encode_volume_map(CUtensorMap* out, const void* base, int B, int G, int D, int H, int W, int box_x, int box_d,
                        int box_g) noexcept;
 
+// [B, L, H, D] 16-bit vectors (n, strides in elements: {b, l, h}); box = box_rows
+// tokens x box_cols (32 or 64) values of one head, rows swizzled over their 64
+// or 128 bytes.  Places outside the tensor read 0.  Extents of 1 and strides of
+// 0 make a dim of extent 1: its coordinate must be 0.
+bool encode_vectors_map(CUtensorMap* out, bool bf16, const void* base, int D, const int (&n)[3],
+                        const int64_t (&strides)[3], int box_cols, int box_rows) noexcept;
+
 }  // namespace ww
