@@ -339,7 +339,7 @@ int64_t ww_qk_norm_rope_backward_workspace(const ww_qk_norm_rope_t* p);
  * A table value of -inf or the type's lowest finite value forbids its pairs.
  * Backward: out and lse of the forward call and dout give dq, dk, dv and
  * (with a table) dbias_table.
- * Limits: D <= 128, D % 8 == 0; num_buckets <= 128. */
+ * Limits: D <= 128, D % 8 == 0; num_buckets <= 128, max_distance <= 1024. */
 typedef struct ww_attention {
     const void* q; /* [B, Lq, Hq, D] */
     const void* k; /* [B, Lk, Hk, D], Hk divides Hq */

@@ -85,6 +85,65 @@ __device__ __forceinline__ float bias_value<__nv_bfloat16>(__nv_bfloat16 b)
     return f <= -0x1.fep127f ? -INFINITY : f;
 }
 
+// What one CTA needs of a head's bias: buckets of the relative positions
+// [lo, hi] of its tiles, of which those further than max_distance + kRelMargin
+// are left out -- a tile that reaches beyond holds one bucket only (a tile
+// spans fewer than kRelMargin positions).  Built once per CTA into shared
+// memory; entry e stands for rel = lo + e.
+constexpr int kRelMargin = 256;
+constexpr int kMaxDistance = 1024;  // what fits beside the operands of the widest heads
+
+struct RelRange {
+    int lo = 0, hi = -1;
+    __host__ __device__ int count() const { return hi - lo + 1; }
+};
+
+__host__ __device__ __forceinline__ RelRange rel_range(const RelBuckets& r, int lo, int hi)
+{
+    const int far = r.max_distance + kRelMargin;
+    RelRange g;
+    g.lo = lo < -far ? -far : lo > far ? far : lo;
+    g.hi = hi > far ? far : hi < -far ? -far : hi;
+    return g;
+}
+
+// Buckets of a range.  Ends without a barrier.
+__device__ __forceinline__ void build_buckets(const RelBuckets& r, const RelRange& g, uint8_t* to, int thread, int threads)
+{
+    for (int e = thread; e < g.count(); e += threads) to[e] = static_cast<uint8_t>(rel_bucket(r, g.lo + e));
+}
+
+__device__ __forceinline__ int bucket_at(const RelRange& g, const uint8_t* buckets, int rel)
+{
+    return buckets[min(max(rel, g.lo), g.hi) - g.lo];
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ float f32(uint32_t u) { return __uint_as_float(u); }
+
+// Barrier of the 128 threads of warpgroup w (0 or 1).
+__device__ __forceinline__ void warpgroup_sync(int w)
+{
+    if (w == 0) asm volatile("bar.sync 1, 128;" : : : "memory");
+    else asm volatile("bar.sync 2, 128;" : : : "memory");
+}
+
 // Fills `out`; WW_SUCCESS or the status of rejected arguments (attention_host.cu).
 int make_buckets(int num_buckets, int max_distance, int bidirectional, int q_offset, RelBuckets* out) noexcept;
 

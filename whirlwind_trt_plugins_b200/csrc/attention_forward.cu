@@ -27,10 +27,10 @@
 //
 // Masked keys get P = 0 and their rows of V are zeroed in shared memory (0 times
 // a NaN would not be 0); tiles without a masked key skip all of it.
-// The relative bias of a tile depends on j - i alone: its 255 values are put
-// into shared memory per tile (the bucket search runs twice per thread), a row
-// reads them at a fixed offset from its own start; tiles whose distances all
-// lie in one bucket add a constant.
+// The relative bias of a head depends on j - i alone: a CTA puts its values by
+// position into shared memory once, a row reads a tile's 128 at fixed offsets
+// from its own start (neighbouring rows one apart: no bank conflicts); tiles
+// whose positions all lie in one bucket add a constant.
 //
 // Few rows against many keys: the keys are split over CTAs, each writes its
 // normalised fp32 rows and log sums, a second kernel joins them in order.
@@ -59,6 +59,7 @@ struct FwdParams {
     int32_t B, Lq, Lk, Hq, group, D;
     int32_t q_blocks, splits;
     int32_t q_b, q_h, k_b, k_h, v_b, v_h;  // 0 where the tensor is broadcast
+    int32_t max_entries;                   // relative positions a CTA keeps
     float scale2;                          // scale * log2(e)
     int* err;
 };
@@ -74,9 +75,9 @@ struct Layout {
     static constexpr int kQ = 0;
     static constexpr int kK = NT * kTileBytes;
     static constexpr int kV = kK + kStages * kTileBytes;
-    static constexpr int kWin = kV + kStages * kTileBytes;         // NT x 2 windows of 256 floats
-    static constexpr int kBar = kWin + NT * 2 * 256 * 4;
-    static constexpr int kBytes = kBar + 256 + 1024;               // + alignment of the base
+    static constexpr int kBar = kV + kStages * kTileBytes;
+    static constexpr int kBias = kBar + 256;                       // [entries] values, [entries] buckets
+    static constexpr int kBytes = kBias + 1024;                    // + alignment of the base, + the bias
     static constexpr int kColumns = NT * (kTile + DP) <= 256 ? 256 : 512;
     static constexpr int kThreads = NT * 128 + 64;
 };
@@ -88,32 +89,6 @@ struct Bars {
         o_full[NT];
     uint32_t tmem;
 };
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-__device__ __forceinline__ float f32(uint32_t u) { return __uint_as_float(u); }
-
-// Barrier of the 128 threads of query tile t.
-__device__ __forceinline__ void tile_sync(int t)
-{
-    if (t == 0) asm volatile("bar.sync 1, 128;" : : : "memory");
-    else asm volatile("bar.sync 2, 128;" : : : "memory");
-}
 
 template <typename T, int DP, int NT>
 __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) attention_forward_kernel(const __grid_constant__ FwdParams p)
@@ -140,6 +115,19 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
     const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / p.splits) - first;
 
     const int warp = threadIdx.x / 32;
+    RelRange range;  // positions j - i - q_offset of the tiles, padded rows and columns included
+    float* values = reinterpret_cast<float*>(base + L::kBias);
+    uint8_t* buckets = base + L::kBias + 4 * p.max_entries;
+    if (p.rel.per_side != 0 && n > 0) {
+        range = rel_range(p.rel, first * kTile - (q0 + NT * kTile - 1) - p.rel.q_offset,
+                          (first + n) * kTile - 1 - q0 - p.rel.q_offset);
+        const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
+        for (int e = threadIdx.x; e < range.count(); e += L::kThreads) {
+            const int bu = rel_bucket(p.rel, range.lo + e);
+            buckets[e] = static_cast<uint8_t>(bu);
+            values[e] = bias_value<T>(table[bu]) * kLog2eF;
+        }
+    }
     if (threadIdx.x == 0) {
         umma::mbar_init(at(bar->q_full), 1);
         for (int s = 0; s < S; ++s) {
@@ -249,7 +237,6 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
         const int t = warp / 4, r = threadIdx.x % 128, lane = threadIdx.x % 32;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;  // TMEM lane of this warp's first row
         const int i = q0 + t * kTile + r;
-        float* win = reinterpret_cast<float*>(base + L::kWin) + t * 512;
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         bool ok = true;  // once a wait has run out: no more waits, but every barrier of the tile is kept
         uint32_t x[kTile];
@@ -266,22 +253,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
                                              __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + k0 + 32 * c + lane) != 0);
             }
             const bool whole = (keep[0] & keep[1] & keep[2] & keep[3]) == ~0u;
-            // the bias: one value for the tile, or a window over j - i
+            // the bias: one value for the tile, or by j - i from this row's start
             float flat = 0.0f;
             const float* mine = nullptr;
             if (p.rel.per_side != 0) {
-                const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
-                const int rel0 = k0 - (q0 + t * kTile) - p.rel.q_offset;
-                const int lo = rel_bucket(p.rel, rel0 - 127);
-                if (lo == rel_bucket(p.rel, rel0 + 127)) {
-                    flat = bias_value<T>(table[lo]) * kLog2eF;
-                } else {
-                    float* w = win + (kt & 1) * 256;
-                    w[r] = bias_value<T>(table[rel_bucket(p.rel, rel0 - 127 + r)]) * kLog2eF;
-                    w[r + 128] = bias_value<T>(table[rel_bucket(p.rel, rel0 + 1 + r)]) * kLog2eF;
-                    tile_sync(t);
-                    mine = w + 127 - r;
-                }
+                const int lo = k0 - (q0 + t * kTile + 127) - p.rel.q_offset;
+                if (bucket_at(range, buckets, lo) == bucket_at(range, buckets, lo + 254))
+                    flat = values[min(max(lo, range.lo), range.hi) - range.lo];
+                else
+                    mine = values + k0 - i - p.rel.q_offset - range.lo;
             }
             ok = ok && umma::mbar_wait(at(bar->s_full[t]), kt & 1);
             umma::fence_after_sync();
@@ -482,9 +462,10 @@ int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, NT>;
     const auto kernel = attention_forward_kernel<T, DP, NT>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
+    const int bytes = L::kBytes + 5 * f.max_entries;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
         return launch_status("cross_attention");
-    kernel<<<static_cast<unsigned>(ctas), L::kThreads, L::kBytes, stream>>>(f);
+    kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
     return launch_status("cross_attention");
 }
 
@@ -507,8 +488,12 @@ int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noex
     f.k_lens = p.k_lens;
     f.key_mask = p.key_mask;
     f.table = p.bias_table;
-    if (p.bias_table != nullptr)
+    f.max_entries = 0;
+    if (p.bias_table != nullptr) {
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
+        const int all = (p.Lk + kTile - 1) / kTile * kTile + plan.nt * kTile;
+        f.max_entries = (std::min(2 * (p.max_distance + kRelMargin) + 1, all) + 15) / 16 * 16;
+    }
     const int64_t rows = i64(p.B) * p.Lq * p.Hq;
     f.part_o = static_cast<float*>(p.workspace);
     f.part_lse = f.part_o + plan.splits * rows * p.D;

@@ -56,6 +56,7 @@ int check_attention(const ww_attention_t& p) noexcept
         RelBuckets r;
         const int st = make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &r);
         if (st != WW_SUCCESS) return st;
+        if (p.max_distance > kMaxDistance) return WW_ERR_UNSUPPORTED;
     }
     if (has_q && (!vectors_ok(p.q, p.q_strides, p.B, p.Lq, p.Hq, 2) || reinterpret_cast<uintptr_t>(p.out) % 16 != 0))
         return WW_ERR_MISALIGNED;
