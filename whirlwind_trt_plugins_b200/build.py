@@ -40,6 +40,7 @@ SOURCES = [
     "attention_host.cu",
     "qk_norm_rope.cu",
     "attention_forward.cu",
+    "attention_token.cu",
     "attention_backward.cu",
     "multi.cu",
     "plugin_core.cpp",

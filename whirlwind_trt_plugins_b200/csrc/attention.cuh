@@ -59,13 +59,11 @@ __host__ __device__ __forceinline__ int rel_bucket(const RelBuckets& r, int rel)
         d = rel < 0 ? -rel : 0;
     }
     if (d < r.exact) return first + d;
-    int lo = 0, hi = r.n_least;  // first t with least[t] > d
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (r.least[mid] <= d) lo = mid + 1;
-        else hi = mid;
-    }
-    return first + r.exact + lo;
+    // counted, not searched: every thread reads the same edges in the same
+    // order (a search's constant-memory reads differ by thread and serialise)
+    int n = 0;
+    for (int t = 0; t < r.n_least; ++t) n += r.least[t] <= d;
+    return first + r.exact + n;
 }
 
 // A bias at the type's lowest finite value forbids the pair like -inf: a row

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / p.splits);
     const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / p.splits) - first;
 
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // warp-uniform: roles branch as warps
     RelRange range;
     uint8_t* buckets = base + L::kBias;
     float* values = nullptr;  // bias of [range]: KEYS: of this warpgroup's current head
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             bool ok = true;
             for (int i = 0; i < n && ok; ++i) {
                 const int s = i % S;
-                ok = umma::mbar_wait(at(bar->c_empty[s]), (i / S + 1) & 1);
+                ok = umma::mbar_poll(at(bar->c_empty[s]), (i / S + 1) & 1);
                 if (!ok) break;
                 int ch = h / group, l = (first + i) * kCols;
                 if (KEYS) {
@@ -217,51 +217,63 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x30);
         }
     } else if (warp == 8) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
+            // one lane issues, the warp runs as a whole with everything in uniform registers
+            // (see attention_forward.cu)
+            const uint32_t tm = __reduce_or_sync(~0u, tmem);
+            const auto s_col = [&](int st) { return tm + st * kCols; };
+            const auto dp_col = [&](int st) { return tm + 2 * kCols + st * kCols; };
+            const uint32_t acc1 = tm + 4 * kCols, acc2 = acc1 + DP;
             constexpr bool bf = !kHalf;
-            const int steps = (p.D + 15) / 16;
-            const uint32_t id_s = umma::idesc_16bit(bf, kRows, kCols, false);
-            const uint32_t id_a = umma::idesc_16bit(bf, kRows, DP, true);
+            constexpr uint32_t id_s = umma::idesc_16bit(bf, kRows, kCols, false), id_a = umma::idesc_16bit(bf, kRows, DP, true);
+            const uint64_t r_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kR1, 16);
+            const uint64_t c_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kC, 16);
+            const uint64_t a_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kC, L::kColChunk);
             const auto scores = [&](int i) {
-                const uint32_t cs = sm + L::kC + (i % S) * 2 * L::kColBytes;
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t r = sm + (x ? L::kR2 : L::kR1), c = cs + x * L::kColBytes;
-                    const uint32_t to = x ? dp_col(i & 1) : s_col(i & 1);
-                    for (int j = 0; j < steps; ++j) {
-                        const int chunk = j * 16 / L::kVals, in = j * 16 % L::kVals * 2;
-                        umma::mma_f16_ss(to, umma::smem_desc_swizzled<L::kRow>(r + chunk * L::kRowChunk + in, 16),
-                                         umma::smem_desc_swizzled<L::kRow>(c + chunk * L::kColChunk + in, 16), id_s, j > 0);
-                    }
-                }
+                const uint64_t cd = umma::desc_advance(c_desc, i % S * 2 * L::kColBytes);
+                const uint32_t to = s_col(i & 1), to2 = dp_col(i & 1);
+                if (!umma::elect_one()) return;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < DP / 16; ++j)
+                        umma::mma_f16_ss(x ? to2 : to,
+                                         umma::desc_advance(r_desc, x * L::kRowBytes + j * 16 / L::kVals * L::kRowChunk +
+                                                                        j * 16 % L::kVals * 2),
+                                         umma::desc_advance(cd, x * L::kColBytes + j * 16 / L::kVals * L::kColChunk +
+                                                                    j * 16 % L::kVals * 2),
+                                         id_s, j > 0);
                 umma::mma_commit(at(bar->s_full[i & 1]));
             };
-            bool ok = umma::mbar_wait(at(bar->r_full), 0);
+            bool ok = umma::mbar_poll(at(bar->r_full), 0);
             for (int i = 0; i < 2 && i < n && ok; ++i) {
-                ok = umma::mbar_wait(at(bar->c_full[i]), 0);
+                ok = umma::mbar_poll(at(bar->c_full[i]), 0);
                 if (ok) scores(i);
             }
             for (int i = 0; i < n && ok; ++i) {
-                ok = umma::mbar_wait(at(bar->p_ready[i & 1]), (i >> 1) & 1);
+                ok = umma::mbar_poll(at(bar->p_ready[i & 1]), (i >> 1) & 1);
                 if (!ok) break;
                 umma::fence_after_sync();
-                const uint32_t cs = sm + L::kC + (i % S) * 2 * L::kColBytes;
+                const uint64_t ad = umma::desc_advance(a_desc, i % S * 2 * L::kColBytes);
+                const uint32_t from = s_col(i & 1), from2 = dp_col(i & 1);
+                if (umma::elect_one()) {
+#pragma unroll
                 for (int j = 0; j < kCols / 16; ++j) {
-                    const uint32_t rows = j * 16 * L::kRow;
-                    umma::mma_f16_ts(acc1, dp_col(i & 1) + j * 8,
-                                     umma::smem_desc_swizzled<L::kRow>(cs + rows, L::kColChunk), id_a, i > 0 || j > 0);
+                    umma::mma_f16_ts(acc1, from2 + j * 8, umma::desc_advance(ad, j * 16 * L::kRow), id_a, i > 0 || j > 0);
                     if (KEYS)
-                        umma::mma_f16_ts(acc2, s_col(i & 1) + j * 8,
-                                         umma::smem_desc_swizzled<L::kRow>(cs + L::kColBytes + rows, L::kColChunk), id_a,
+                        umma::mma_f16_ts(acc2, from + j * 8, umma::desc_advance(ad, L::kColBytes + j * 16 * L::kRow), id_a,
                                          i > 0 || j > 0);
                 }
                 umma::mma_commit(at(bar->c_empty[i % S]));
+                }
+                __syncwarp();
                 if (i + 2 < n) {
-                    ok = umma::mbar_wait(at(bar->c_full[(i + 2) % S]), ((i + 2) / S) & 1);
+                    ok = umma::mbar_poll(at(bar->c_full[(i + 2) % S]), ((i + 2) / S) & 1);
                     if (ok) scores(i + 2);
                 }
             }
-            if (ok) umma::mma_commit(at(bar->done));
-            else record_device_error(p.err, kErrMbarTimeout | 0x31);
+            if (ok && umma::elect_one()) umma::mma_commit(at(bar->done));
+            if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x31);
         }
     } else {
         const int wg = warp / 4, r = threadIdx.x % 128;
@@ -284,10 +296,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             my_delta = __ldg(p.delta + i) * f;
         }
         const bool rows_ok = __all_sync(~0u, row_ok);
+        const bool any_row = row0 + warp % 4 * 32 < (KEYS ? len : p.Lq);  // else this warp keeps the barriers only
         int built = -1;  // KEYS: head of `values`
         float* diag = values + entries + wg * entries;
         float* plain = values + 3 * entries + warp * kMaxBuckets;
         float* tile = values + 3 * entries + 8 * kMaxBuckets + wg * kRows * kPitch;
+        if (BIAS && !KEYS && !any_row)
+            for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;
         for (int i = wg; i < n; i += 2) {
             const int col0 = KEYS ? (first + i) % p.q_tiles * kCols : (first + i) * kCols;
             uint32_t keep[2] = {~0u, ~0u};
@@ -323,15 +338,42 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                 else
                     mine = values + (KEYS ? row - col0 : col0 - row) - p.rel.q_offset - range.lo;
             }
-            ok = ok && umma::mbar_wait(at(bar->s_full[wg]), (i >> 1) & 1);
+            ok = ok && umma::mbar_poll(at(bar->s_full[wg]), (i >> 1) & 1);
             umma::fence_after_sync();
             const float* vec = reinterpret_cast<const float*>(base + L::kVec + (i % S) * 2 * kCols * 4);
-            if (KEYS) ok = ok && umma::mbar_wait(at(bar->c_full[i % S]), (i / S) & 1);
+            if (KEYS) ok = ok && umma::mbar_poll(at(bar->c_full[i % S]), (i / S) & 1);
             const float row_add = (BIAS ? flat : 0.0f) - (KEYS ? 0.0f : my_lse);
-            float total = 0.0f, run = 0.0f, done_diag = 0.0f;
+            float total = 0.0f;
+            // sums of a half tile's dS along j - i: each thread a diagonal, column
+            // j of row (j + 127 - r) mod 128: diagonal r - 127 until column r, r + 1
+            // (r < 31) from there on
+            const auto diagonals = [&](int c) {
+                warpgroup_sync(wg);
+                float run = 0.0f, left = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    if (j == r + 1) {
+                        left = run;
+                        run = 0.0f;
+                    }
+                    run += tile[((j + 127 - r) & 127) * kPitch + j];
+                }
+                float* to = diag + col0 + 32 * c - row0 - p.rel.q_offset - range.lo;
+                to[r - 127] += r < 31 ? left : run;
+                if (r < 31) to[r + 1] += run;
+            };
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t s[32], d[32];
+                if (!any_row) {
+                    if (!KEYS && BIAS) {
+                        if (mine != nullptr) {
+                            warpgroup_sync(wg);
+                            diagonals(c);
+                        }
+                    }
+                    continue;
+                }
                 umma::tmem_ld32(s_col(wg) + lanes + c * 32, s);
                 umma::tmem_ld32(dp_col(wg) + lanes + c * 32, d);
                 umma::tmem_wait_ld32(s);
@@ -368,29 +410,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
 #pragma unroll
                         for (int j = 0; j < 32; ++j) total += f32(d[j]);
                     } else {
-                        // each thread a diagonal: column j of row (j + 127 - r) mod 128
                         float* to = tile + r * kPitch;
                         warpgroup_sync(wg);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) to[j] = f32(d[j]);
-                        warpgroup_sync(wg);
-                        run = done_diag = 0.0f;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (j == r + 1) {
-                                done_diag = run;
-                                run = 0.0f;
-                            }
-                            run += tile[((j + 127 - r) & 127) * kPitch + j];
-                        }
-                        // r <= 31 held diagonal r - 127 until column r and r + 1 from there on
-                        float* dg = diag + col0 + 32 * c - row0 - p.rel.q_offset - range.lo;
-                        if (r < 31) {
-                            dg[r - 127] += done_diag;
-                            dg[r + 1] += run;
-                        } else {
-                            dg[r - 127] += run;
-                        }
+                        diagonals(c);
                     }
                 }
 #pragma unroll
@@ -407,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             }
             if (!KEYS && !whole) {
                 // rows of K behind masked keys: 0 in place of whatever they hold
-                ok = ok && umma::mbar_wait(at(bar->c_full[i % S]), (i / S) & 1);
+                ok = ok && umma::mbar_poll(at(bar->c_full[i % S]), (i / S) & 1);
                 if (r < kCols && !((keep[(r >> 5) & 1] >> lane) & 1)) {
                     const uint32_t to = sm + L::kC + (i % S) * 2 * L::kColBytes + r * L::kRow;
                     for (int c = 0; c < L::kChunks; ++c)
@@ -420,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             umma::fence_before_sync();
             umma::mbar_arrive(at(bar->p_ready[wg]));
         }
-        if (n > 0) ok = ok && umma::mbar_wait(at(bar->done), 0);
+        if (n > 0) ok = ok && umma::mbar_poll(at(bar->done), 0);
         umma::fence_after_sync();
         if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x32);
         // keys: warpgroup 0 writes dk, 1 dv; queries: each half of dq
@@ -444,6 +468,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                 for (int j = 0; j < 16; ++j) o[j] = 0;
             }
             if (row >= L_) continue;
+            if (KEYS && !row_ok) {  // a masked key: 0, whatever a skipped warp left in its lanes
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = 0;
+            }
             if (p.splits > 1) {
                 float* to = p.part + (static_cast<int64_t>(split) * (KEYS ? 2 : 1) + second) * size + at_row + d0;
 #pragma unroll
@@ -495,14 +523,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
 
 // delta = rowsum(dO * O) and lse in log2 units, both laid out [B * Hq][Lq_pad]
 // with rows of no gradient (lse -inf, padding) at lse2 = +inf; for fp16 also
-// max |dO| (an integer maximum of non-negative floats: no order).  D / 8 lanes
-// of a group of 16 per row.
-template <typename T>
+// max |dO| (an integer maximum of non-negative floats: no order).  kLanes >= D / 8
+// lanes per row, 8 values each.
+template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ ww_attention_t a, float* lse2,
                                                               float* delta, uint32_t* top, int Lq_pad)
 {
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
-    const int lane = threadIdx.x % 16;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+    const int lane = threadIdx.x % kLanes;
     const int64_t rows = static_cast<int64_t>(a.B) * Lq_pad * a.Hq;
     const int h = static_cast<int>(item % a.Hq);
     const int64_t bi = item / a.Hq;
@@ -523,7 +551,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
         }
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     if (item < rows && lane == 0) {
         const int64_t to = (static_cast<int64_t>(b) * a.Hq + h) * Lq_pad + i;
         const float l = live ? a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Lq + i] : -INFINITY;
@@ -558,22 +586,25 @@ __global__ void __launch_bounds__(256) attention_sum_kernel(const float* part, i
     *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
 }
 
-// Table gradient of one head: the CTAs' buckets in order.  Each warp takes
-// every 8th CTA, 32 buckets at a time, then the warps' sums in order.
+// Table gradient of one head: the CTAs' buckets in order.  Each of 32 warps takes
+// every 32nd CTA (four loads in flight), 32 buckets at a time, then the warps'
+// sums in order.
 template <typename T>
-__global__ void __launch_bounds__(256) attention_table_kernel(const float* part, T* out, int B, int Hq, int per_head, int total)
+__global__ void __launch_bounds__(1024) attention_table_kernel(const float* part, T* out, int B, int Hq, int per_head, int total)
 {
-    __shared__ float sums[8][32];
+    __shared__ float sums[32][33];
     const int h = blockIdx.x, t = blockIdx.y * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
     float s = 0.0f;
-    if (t < total)
-        for (int n = w; n < B * per_head; n += 8)
+    if (t < total) {
+#pragma unroll 4
+        for (int n = w; n < B * per_head; n += 32)
             s += part[((static_cast<int64_t>(n / per_head) * Hq + h) * per_head + n % per_head) * total + t];
+    }
     sums[w][threadIdx.x % 32] = s;
     __syncthreads();
     if (w == 0 && t < total) {
         s = 0.0f;
-        for (int n = 0; n < 8; ++n) s += sums[n][threadIdx.x];
+        for (int n = 0; n < 32; ++n) s += sums[n][threadIdx.x];
         out[h * total + t] = from_float<T>(s);
     }
 }
@@ -693,9 +724,13 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     if (has_q) {
         if (!bf && cudaMemsetAsync(ws, 0, 4, stream) != cudaSuccess) return launch_status("cross_attention_backward");
         const int64_t rows = i64(p.B) * plan.Lq_pad * p.Hq;
-        if ((rows + 15) / 16 > 0x7fffffff) return WW_ERR_UNSUPPORTED;
-        attention_delta_kernel<T><<<static_cast<unsigned>((rows + 15) / 16), 256, 0, stream>>>(
-            p, const_cast<float*>(f.lse2), const_cast<float*>(f.delta), reinterpret_cast<uint32_t*>(ws), plan.Lq_pad);
+        const int per = p.D <= 32 ? 64 : p.D <= 64 ? 32 : 16;  // rows of a block
+        const int64_t blocks = (rows + per - 1) / per;
+        if (blocks > 0x7fffffff) return WW_ERR_UNSUPPORTED;
+        const auto kernel = per == 64 ? attention_delta_kernel<T, 4> : per == 32 ? attention_delta_kernel<T, 8>
+                                                                                 : attention_delta_kernel<T, 16>;
+        kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, const_cast<float*>(f.lse2), const_cast<float*>(f.delta),
+                                                                  reinterpret_cast<uint32_t*>(ws), plan.Lq_pad);
         st = launch_status("cross_attention_backward");
     }
     const int far = 2 * (p.max_distance + kRelMargin) + 1;
@@ -720,7 +755,7 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
         if (st == WW_SUCCESS && plan.q_splits > 1) st = sum_parts<T>(f.part, plan.q_splits, n, p.dq, n, stream);
     }
     if (st == WW_SUCCESS && p.bias_table != nullptr) {
-        attention_table_kernel<T><<<dim3(p.Hq, (p.num_buckets + 31) / 32), 256, 0, stream>>>(
+        attention_table_kernel<T><<<dim3(p.Hq, (p.num_buckets + 31) / 32), 1024, 0, stream>>>(
             f.table_part, static_cast<T*>(p.dbias_table), has_q ? p.B : 0, p.Hq, plan.q_blocks * plan.q_splits, p.num_buckets);
         st = launch_status("cross_attention_backward");
     }

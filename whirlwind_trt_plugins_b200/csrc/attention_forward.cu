@@ -1,11 +1,11 @@
 // attention_forward.cu -- ww_cross_attention: softmax(scale Q K^T + bias) V on
 // the 5th-generation tensor cores, one pass over the keys.
 //
-// For a tile of 128 query rows and 128 keys at a time, with x = scale log2(e) s
+// For a tile of 128 query rows and KT keys at a time, with x = scale log2(e) s
 // + bias log2(e) the scores in log2 units:
 //
 //   S = Q K^T                       tcgen05.mma, operands staged by TMA, S in TMEM
-//   m' = max(m, max_j x_j)          one thread per row: its 128 scores from TMEM
+//   m' = max(m, max_j x_j)          one thread per row: its KT scores from TMEM
 //   P_j = 2^(x_j - m'), l = l 2^(m - m') + sum_j P_j
 //   O = O 2^(m - m') + P V          P goes back to TMEM as the A operand
 //   out = O / l, lse = ln 2 (m + log2 l)
@@ -15,26 +15,33 @@
 // tiles that hardly happens, and no tile needs the read-multiply-write of O.
 //
 // Roles: 4 warps per query tile turn scores into P; one thread issues every
-// MMA; one thread every TMA load.  P overwrites the first half of its scores'
-// columns, and the next S of a tile is issued behind the product that reads
-// that P (MMAs of a CTA run in issue order).  What hides the round trip of a
-// tile is a second one: NT = 2 query tiles of one CTA against the same keys, or
-// two CTAs of one tile on an SM.
+// MMA; one warp every TMA load and the limits of masked keys.
 //
-// Bound: the exponential, 16 per clock and SM: 1024 clocks for a tile of
-// 128 x 128, against 2 x 8 D clocks for its products (8192 fp16 FMA per clock):
-// 512 clocks at D = 32, equal at D = 64 ... 128.
+// Bound: the exponential, 16 per clock and SM: 1024 clocks for 128 x 128
+// scores, against 16 D clocks for their products (8192 fp16 FMA per clock):
+// 512 at D = 32, equal at D = 64.  Two forms keep it busy:
+//   short rows (NT = 1)  one query tile, 64 keys at a time, three CTAs on an SM
+//                        (two at D = 128): the CTAs hide one another's round
+//                        trips, starts and ends.  P overwrites its scores and
+//                        the next S is issued behind the product that reads it
+//                        (MMAs of a CTA run in issue order).
+//   long rows (NT = 2)   two query tiles of one CTA against the same keys, which
+//                        halves what each SM reads of them from L2; P has its
+//                        own columns, so that the next S is formed as soon as
+//                        the scores have been read.
 //
-// Masked keys get P = 0 and their rows of V are zeroed in shared memory (0 times
-// a NaN would not be 0); tiles without a masked key skip all of it.
+// Masked keys: their scores meet a limit of -inf (a minimum, which also takes
+// a NaN) and their rows of V are zeroed in shared memory (0 times a NaN would
+// not be 0); tiles without a masked key skip both.
 // The relative bias of a head depends on j - i alone: a CTA puts its values by
-// position into shared memory once, a row reads a tile's 128 at fixed offsets
-// from its own start (neighbouring rows one apart: no bank conflicts); tiles
-// whose positions all lie in one bucket add a constant.
+// position into shared memory once, a row reads a tile's at fixed offsets from
+// its own start (neighbouring rows one apart: no bank conflicts); tiles whose
+// positions all lie in one bucket add a constant.
 //
 // Few rows against many keys: the keys are split over CTAs, each writes its
 // normalised fp32 rows and log sums, a second kernel joins them in order.
 #include "attention.cuh"
+#include "attention_token.cuh"
 #include "tensor_map.cuh"
 #include "umma.cuh"
 
@@ -43,7 +50,8 @@
 namespace ww {
 namespace {
 
-constexpr int kTile = 128;       // query rows and keys of a tile
+constexpr int kTile = 128;       // query rows of a tile
+constexpr int kBox = 64;         // tokens of a TMA box
 constexpr float kRescale = 8.0f; // log2 growth of the maximum that is left in P
 
 struct FwdParams {
@@ -66,36 +74,64 @@ struct FwdParams {
 
 template <int DP, int NT>
 struct Layout {
+    static constexpr bool kOwnP = NT == 2;                 // P beside its scores instead of over them
+    static constexpr int kKeys = NT == 2 && DP <= 64 ? 128 : 64;
     static constexpr int kRow = DP == 32 ? 64 : 128;       // bytes of an operand row
     static constexpr int kCols = kRow / 2;                 // values in it
     static constexpr int kChunks = DP * 2 / kRow;          // rows of one token
-    static constexpr int kChunkBytes = kTile * kRow;
-    static constexpr int kTileBytes = kTile * DP * 2;
-    static constexpr int kStages = DP == 128 ? 2 : (NT == 2 ? 3 : 2);
-    static constexpr int kQ = 0;
-    static constexpr int kK = NT * kTileBytes;
-    static constexpr int kV = kK + kStages * kTileBytes;
-    static constexpr int kBar = kV + kStages * kTileBytes;
-    static constexpr int kBias = kBar + 256;                       // [entries] values, [entries] buckets
-    static constexpr int kBytes = kBias + 1024;                    // + alignment of the base, + the bias
-    static constexpr int kColumns = NT * (kTile + DP) <= 256 ? 256 : 512;
+    static constexpr int kQChunk = kTile * kRow;
+    static constexpr int kQBytes = kTile * DP * 2;
+    static constexpr int kChunk = kKeys * kRow;            // of a tile of K or V
+    static constexpr int kBytes = kKeys * DP * 2;
+    static constexpr int kStages = NT == 2 ? 3 : 2;
+    static constexpr int kK = NT * kQBytes;
+    static constexpr int kV = kK + kStages * kBytes;
+    static constexpr int kLim = kV + kStages * kBytes;     // [stages][keys] limits, [stages] flags
+    static constexpr int kBar = kLim + kStages * (kKeys + 4) * 4;
+    static constexpr int kBias = kBar + 256;               // [entries] values, [entries] buckets
+    static constexpr int kTotal = kBias + 1024;            // + alignment of the base, + the bias
+    static constexpr int kPCols = kOwnP ? kKeys / 2 : 0;
+    static constexpr int kNeed = NT * (kKeys + kPCols + DP);
+    static constexpr int kColumns = kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
     static constexpr int kThreads = NT * 128 + 64;
+    static constexpr int kCtas = NT == 2 ? 1 : DP == 128 ? 2 : 3;
 };
 
 template <int DP, int NT>
 struct Bars {
     static constexpr int kStages = Layout<DP, NT>::kStages;
-    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], p_ready[NT],
-        o_full[NT];
+    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], s_free[NT],
+        p_ready[NT], pv_done[NT];
     uint32_t tmem;
 };
 
+// Scores of N columns in log2 units with bias and limits, and their maximum.
+template <int N, bool BIAS, bool LIMIT>
+__device__ __forceinline__ float score_pass(uint32_t* x, float scale2, float flat, const float* bias, const float* limit)
+{
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        float4 lim;
+        if (LIMIT) lim = *reinterpret_cast<const float4*>(limit + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float y = fmaf(f32(x[j + i]), scale2, BIAS ? bias[j + i] : flat);
+            if (LIMIT) y = fminf(y, i == 0 ? lim.x : i == 1 ? lim.y : i == 2 ? lim.z : lim.w);
+            top[i & 1] = fmaxf(top[i & 1], y);
+            x[j + i] = __float_as_uint(y);
+        }
+    }
+    return fmaxf(top[0], top[1]);
+}
+
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) attention_forward_kernel(const __grid_constant__ FwdParams p)
+__global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCtas)
+    attention_forward_kernel(const __grid_constant__ FwdParams p)
 {
     using L = Layout<DP, NT>;
     using Bar = Bars<DP, NT>;
-    constexpr int S = L::kStages;
+    constexpr int S = L::kStages, KT = L::kKeys;
     extern __shared__ uint8_t raw[];
     uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
     const uint32_t sm = umma::smem_addr(base);
@@ -106,29 +142,29 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
     int rest = blockIdx.x / p.splits;
     const int qb = rest % p.q_blocks;
     rest /= p.q_blocks;
-    const int h = rest % p.Hq, b = rest / p.Hq;
+    const int h = rest % p.Hq, b = rest / p.Hq, g = h / p.group;
     const int q0 = qb * (NT * kTile);
     const int tiles = NT == 1 || q0 + kTile >= p.Lq ? 1 : 2;  // query tiles with rows
     const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
-    const int n_all = (len + kTile - 1) / kTile;
+    const int n_all = (len + KT - 1) / KT;
     const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / p.splits);
     const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / p.splits) - first;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // warp-uniform: roles branch as warps
+    // keys of a tile
+    const auto cols_of = [&](int kt) { return min(KT, len - (first + kt) * KT); };
+    float* limits = reinterpret_cast<float*>(base + L::kLim);
+    uint32_t* wholes = reinterpret_cast<uint32_t*>(limits + S * KT);  // tile without a masked key
 
-    const int warp = threadIdx.x / 32;
-    RelRange range;  // positions j - i - q_offset of the tiles, padded rows and columns included
-    float* values = reinterpret_cast<float*>(base + L::kBias);
-    uint8_t* buckets = base + L::kBias + 4 * p.max_entries;
-    if (p.rel.per_side != 0 && n > 0) {
-        range = rel_range(p.rel, first * kTile - (q0 + NT * kTile - 1) - p.rel.q_offset,
-                          (first + n) * kTile - 1 - q0 - p.rel.q_offset);
-        const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
-        for (int e = threadIdx.x; e < range.count(); e += L::kThreads) {
-            const int bu = rel_bucket(p.rel, range.lo + e);
-            buckets[e] = static_cast<uint8_t>(bu);
-            values[e] = bias_value<T>(table[bu]) * kLog2eF;
-        }
-    }
-    if (threadIdx.x == 0) {
+    const auto load_k = [&](int kt) {
+        const int s = kt % S;
+        umma::mbar_arrive_expect_tx(at(bar->k_full[s]), L::kBytes);
+        for (int c = 0; c < L::kChunks; ++c)
+            for (int x = 0; x < KT; x += kBox)
+                umma::tma_load_4d(sm + L::kK + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.k, c * L::kCols, g * p.k_h,
+                                  (first + kt) * KT + x, b * p.k_b, at(bar->k_full[s]));
+    };
+    if (warp == NT * 4 + 1 && lane == 0) {
+        // this thread alone uses the barriers until the block's first barrier below
         umma::mbar_init(at(bar->q_full), 1);
         for (int s = 0; s < S; ++s) {
             umma::mbar_init(at(bar->k_full[s]), 1);
@@ -138,167 +174,217 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
         }
         for (int t = 0; t < NT; ++t) {
             umma::mbar_init(at(bar->s_full[t]), 1);
+            umma::mbar_init(at(bar->s_free[t]), 128);
             umma::mbar_init(at(bar->p_ready[t]), 128);
-            umma::mbar_init(at(bar->o_full[t]), 1);
+            umma::mbar_init(at(bar->pv_done[t]), 1);
         }
         umma::mbar_fence_init();
+        umma::fence_proxy_async_smem();
+        if (n > 0) {
+            umma::mbar_arrive_expect_tx(at(bar->q_full), tiles * L::kQBytes);
+            for (int t = 0; t < tiles; ++t)
+                for (int c = 0; c < L::kChunks; ++c)
+                    for (int x = 0; x < kTile; x += kBox)  // a box beyond the last row reads zeros
+                        umma::tma_load_4d(sm + t * L::kQBytes + c * L::kQChunk + x * L::kRow, &p.q, c * L::kCols, h * p.q_h,
+                                          min(q0 + t * kTile + x, p.Lq), b * p.q_b, at(bar->q_full));
+            load_k(0);
+        }
+    }
+    RelRange range;  // positions j - i - q_offset of the tiles, padded rows and columns included
+    float* values = reinterpret_cast<float*>(base + L::kBias);
+    uint8_t* buckets = base + L::kBias + 4 * p.max_entries;
+    if (p.rel.per_side != 0 && n > 0) {
+        range = rel_range(p.rel, first * KT - (q0 + NT * kTile - 1) - p.rel.q_offset,
+                          (first + n) * KT - 1 - q0 - p.rel.q_offset);
+        const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
+        for (int e = threadIdx.x; e < range.count(); e += L::kThreads) {
+            const int bu = rel_bucket(p.rel, range.lo + e);
+            buckets[e] = static_cast<uint8_t>(bu);
+            values[e] = bias_value<T>(table[bu]) * kLog2eF;
+        }
     }
     if (warp == NT * 4) umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = bar->tmem;
-    // columns: S (then P) of each tile, then O of each tile
-    const auto s_col = [&](int t) { return tmem + t * kTile; };
-    const auto o_col = [&](int t) { return tmem + NT * kTile + t * DP; };
-    // columns of key tile n-th that hold keys
-    const auto cols_of = [&](int kt) { return min(kTile, len - (first + kt) * kTile); };
+    // columns: S of each tile, P of each tile, O of each tile
+    const auto s_col = [&](int t) { return tmem + t * KT; };
+    const auto p_col = [&](int t) { return L::kOwnP ? tmem + NT * KT + t * L::kPCols : s_col(t); };
+    const auto o_col = [&](int t) { return tmem + NT * (KT + L::kPCols) + t * DP; };
 
     if (warp == NT * 4 + 1) {
-        if ((threadIdx.x & 31) == 0 && n > 0) {
-            umma::tma_prefetch_desc(&p.q);
-            umma::tma_prefetch_desc(&p.k);
-            umma::tma_prefetch_desc(&p.v);
-            umma::mbar_arrive_expect_tx(at(bar->q_full), tiles * L::kTileBytes);
-            for (int t = 0; t < tiles; ++t)
-                for (int c = 0; c < L::kChunks; ++c)
-                    umma::tma_load_4d(sm + L::kQ + t * L::kTileBytes + c * L::kChunkBytes, &p.q, c * L::kCols,
-                                      h * p.q_h, q0 + t * kTile, b * p.q_b, at(bar->q_full));
-            const int g = h / p.group;
-            bool ok = true;
-            for (int kt = 0; kt < n && ok; ++kt) {
-                const int s = kt % S;
-                const uint32_t ph = (kt / S + 1) & 1;
-                const int l0 = (first + kt) * kTile;
-                ok = umma::mbar_wait(at(bar->k_empty[s]), ph);
-                if (!ok) break;
-                umma::mbar_arrive_expect_tx(at(bar->k_full[s]), L::kTileBytes);
-                for (int c = 0; c < L::kChunks; ++c)
-                    umma::tma_load_4d(sm + L::kK + s * L::kTileBytes + c * L::kChunkBytes, &p.k, c * L::kCols,
-                                      g * p.k_h, l0, b * p.k_b, at(bar->k_full[s]));
-                ok = umma::mbar_wait(at(bar->v_empty[s]), ph);
-                if (!ok) break;
-                umma::mbar_arrive_expect_tx(at(bar->v_full[s]), L::kTileBytes);
-                for (int c = 0; c < L::kChunks; ++c)
-                    umma::tma_load_4d(sm + L::kV + s * L::kTileBytes + c * L::kChunkBytes, &p.v, c * L::kCols,
-                                      g * p.v_h, l0, b * p.v_b, at(bar->v_full[s]));
+        bool ok = true;
+        for (int kt = 0; kt < n; ++kt) {
+            const int s = kt % S;
+            const uint32_t ph = (kt / S + 1) & 1;
+            if (kt > 0 && lane == 0) {
+                ok = ok && umma::mbar_poll(at(bar->k_empty[s]), ph);
+                if (ok) load_k(kt);
             }
-            if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x20);
-        }
-    } else if (warp == NT * 4) {
-        if ((threadIdx.x & 31) == 0 && n > 0) {
-            constexpr bool bf = sizeof(T) == 2 && !std::is_same<T, __half>::value;
-            const int steps = (p.D + 15) / 16;
-            const auto qk = [&](int t, int kt) {
-                const int s = kt % S;
-                const uint32_t id = umma::idesc_16bit(bf, kTile, (cols_of(kt) + 15) / 16 * 16, false);
-                for (int i = 0; i < steps; ++i) {
-                    const uint32_t off = (i * 16 / L::kCols) * L::kChunkBytes + (i * 16 % L::kCols) * 2;
-                    umma::mma_f16_ss(s_col(t),
-                                     umma::smem_desc_swizzled<L::kRow>(sm + L::kQ + t * L::kTileBytes + off, 16),
-                                     umma::smem_desc_swizzled<L::kRow>(sm + L::kK + s * L::kTileBytes + off, 16), id,
-                                     i > 0);
+            if (lane == 0) ok = ok && umma::mbar_poll(at(bar->v_empty[s]), ph);
+            __syncwarp();
+            // limits of the tile's keys (read until its P V is done, as V is)
+            const int cols = cols_of(kt), k0 = (first + kt) * KT;
+            if (p.key_mask != nullptr || cols < KT) {
+                bool all = true;
+#pragma unroll
+                for (int c = 0; c < KT; c += 32) {
+                    const bool in = c + lane < cols &&
+                                    (p.key_mask == nullptr ||
+                                     __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + k0 + c + lane) != 0);
+                    limits[s * KT + c + lane] = in ? INFINITY : -INFINITY;
+                    all = all && in;
                 }
-                umma::mma_commit(at(bar->s_full[t]));
-            };
-            bool ok = umma::mbar_wait(at(bar->q_full), 0) && umma::mbar_wait(at(bar->k_full[0]), 0);
-            if (ok) {
-                for (int t = 0; t < tiles; ++t) qk(t, 0);
-                umma::mma_commit(at(bar->k_empty[0]));
+                all = __all_sync(~0u, all);
+                if (lane == 0) wholes[s] = all;
+                __syncwarp();
             }
-            for (int kt = 0; kt < n && ok; ++kt) {
-                const int s = kt % S, s1 = (kt + 1) % S;
-                const uint32_t id = umma::idesc_16bit(bf, kTile, DP, true);
-                const int ksteps = (cols_of(kt) + 15) / 16;
+            if (lane == 0 && ok) {
+                umma::mbar_arrive_expect_tx(at(bar->v_full[s]), L::kBytes);
+                for (int c = 0; c < L::kChunks; ++c)
+                    for (int x = 0; x < KT; x += kBox)
+                        umma::tma_load_4d(sm + L::kV + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.v, c * L::kCols,
+                                          g * p.v_h, k0 + x, b * p.v_b, at(bar->v_full[s]));
+            }
+            if (!__shfl_sync(~0u, ok, 0)) break;
+        }
+        if (lane == 0 && !ok) record_device_error(p.err, kErrMbarTimeout | 0x20);
+    } else if (warp == NT * 4) {
+        if (n > 0) {
+            // One lane issues every product of the CTA.  The warp runs the loop as a
+            // whole, descriptors are formed once and advanced by constants and loops are
+            // unrolled: everything a product needs is in uniform registers (forming it per
+            // product, in one thread, took 100 clocks each and was what the kernel waited for).
+            const uint32_t tm = __reduce_or_sync(~0u, tmem);  // uniform
+            const auto s_col = [&](int t) { return tm + t * KT; };
+            const auto p_col = [&](int t) { return L::kOwnP ? tm + NT * KT + t * L::kPCols : s_col(t); };
+            const auto o_col = [&](int t) { return tm + NT * (KT + L::kPCols) + t * DP; };
+            constexpr bool bf = !std::is_same<T, __half>::value;
+            constexpr uint32_t id_full = umma::idesc_16bit(bf, kTile, KT, false), id_o = umma::idesc_16bit(bf, kTile, DP, true);
+            const uint64_t q_desc = umma::smem_desc_swizzled<L::kRow>(sm, 16);
+            const uint64_t k_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kK, 16);
+            const uint64_t v_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kV, L::kChunk);
+            const auto qk = [&](int t, int kt) {
+                const int s = kt % S, cols = cols_of(kt);
+                const uint32_t id = cols >= KT ? id_full : umma::idesc_16bit(bf, kTile, (cols + 15) / 16 * 16, false);
+                const uint64_t qd = umma::desc_advance(q_desc, t * L::kQBytes), kd = umma::desc_advance(k_desc, s * L::kBytes);
+                const uint32_t to = s_col(t);
+                if (!umma::elect_one()) return;
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i)
+                    umma::mma_f16_ss(to, umma::desc_advance(qd, i * 16 / L::kCols * L::kQChunk + i * 16 % L::kCols * 2),
+                                     umma::desc_advance(kd, i * 16 / L::kCols * L::kChunk + i * 16 % L::kCols * 2), id, i > 0);
+                umma::mma_commit(at(bar->s_full[t]));
+                if (t == tiles - 1) umma::mma_commit(at(bar->k_empty[s]));
+            };
+            const auto pv = [&](int t, int kt) {
+                const int s = kt % S, cols = cols_of(kt);
+                const uint64_t vd = umma::desc_advance(v_desc, s * L::kBytes);
+                const uint32_t from = p_col(t), to = o_col(t);
+                if (!umma::elect_one()) return;
+#pragma unroll
+                for (int i = 0; i < KT / 16; ++i)
+                    if (i * 16 < cols)
+                        umma::mma_f16_ts(to, from + i * 8, umma::desc_advance(vd, i * 16 * L::kRow), id_o, kt > 0 || i > 0);
+                if (L::kOwnP || kt == n - 1) umma::mma_commit(at(bar->pv_done[t]));
+                if (t == tiles - 1) umma::mma_commit(at(bar->v_empty[s]));
+            };
+            bool ok = umma::mbar_poll(at(bar->q_full), 0) && umma::mbar_poll(at(bar->k_full[0]), 0);
+            for (int t = 0; t < tiles && ok; ++t) qk(t, 0);
+            for (int kt = 0; kt < n && ok; ++kt)
                 for (int t = 0; t < tiles && ok; ++t) {
-                    if (t == 0) ok = umma::mbar_wait(at(bar->v_full[s]), (kt / S) & 1);
-                    ok = ok && umma::mbar_wait(at(bar->p_ready[t]), kt & 1);
+                    const bool next = kt + 1 < n;
+                    if (next && t == 0) ok = umma::mbar_poll(at(bar->k_full[(kt + 1) % S]), ((kt + 1) / S) & 1);
+                    if (L::kOwnP && next && ok) {
+                        ok = umma::mbar_poll(at(bar->s_free[t]), kt & 1);
+                        umma::fence_after_sync();
+                        if (ok) qk(t, kt + 1);
+                    }
+                    if (t == 0) ok = ok && umma::mbar_poll(at(bar->v_full[kt % S]), (kt / S) & 1);
+                    ok = ok && umma::mbar_poll(at(bar->p_ready[t]), kt & 1);
                     if (!ok) break;
                     umma::fence_after_sync();
-                    for (int i = 0; i < ksteps; ++i)
-                        umma::mma_f16_ts(o_col(t), s_col(t) + i * 8,
-                                         umma::smem_desc_swizzled<L::kRow>(
-                                             sm + L::kV + s * L::kTileBytes + i * 16 * L::kRow, L::kChunkBytes),
-                                         id, kt > 0 || i > 0);
-                    if (t == tiles - 1) umma::mma_commit(at(bar->v_empty[s]));
-                    if (kt + 1 < n) {
-                        if (t == 0) ok = umma::mbar_wait(at(bar->k_full[s1]), ((kt + 1) / S) & 1);
-                        if (!ok) break;
-                        qk(t, kt + 1);
-                        if (t == tiles - 1) umma::mma_commit(at(bar->k_empty[s1]));
-                    } else {
-                        umma::mma_commit(at(bar->o_full[t]));
-                    }
+                    pv(t, kt);
+                    if (!L::kOwnP && next) qk(t, kt + 1);
                 }
-            }
-            if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x21);
+            if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x21);
         }
     } else if (warp / 4 < tiles) {
-        const int t = warp / 4, r = threadIdx.x % 128, lane = threadIdx.x % 32;
+        const int t = warp / 4, r = threadIdx.x % 128;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;  // TMEM lane of this warp's first row
         const int i = q0 + t * kTile + r;
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-        bool ok = true;  // once a wait has run out: no more waits, but every barrier of the tile is kept
-        uint32_t x[kTile];
+        bool ok = true;  // once a wait has run out: no more waits, everything else goes on
+        const bool any_row = q0 + t * kTile + warp % 4 * 32 < p.Lq;  // else this warp keeps the barriers only
+        uint32_t x[KT];
         for (int kt = 0; kt < n; ++kt) {
-            const int k0 = (first + kt) * kTile, cols = cols_of(kt);
-            // which of the 128 keys count
-            uint32_t keep[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int left = cols - 32 * c;
-                keep[c] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-                if (p.key_mask != nullptr)
-                    keep[c] &= __ballot_sync(~0u, 32 * c + lane < cols &&
-                                             __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + k0 + 32 * c + lane) != 0);
-            }
-            const bool whole = (keep[0] & keep[1] & keep[2] & keep[3]) == ~0u;
+            const int s = kt % S, k0 = (first + kt) * KT, cols = cols_of(kt);
             // the bias: one value for the tile, or by j - i from this row's start
             float flat = 0.0f;
             const float* mine = nullptr;
             if (p.rel.per_side != 0) {
-                const int lo = k0 - (q0 + t * kTile + 127) - p.rel.q_offset;
-                if (bucket_at(range, buckets, lo) == bucket_at(range, buckets, lo + 254))
+                const int lo = k0 - (q0 + t * kTile + kTile - 1) - p.rel.q_offset;
+                if (bucket_at(range, buckets, lo) == bucket_at(range, buckets, lo + kTile + KT - 2))
                     flat = values[min(max(lo, range.lo), range.hi) - range.lo];
                 else
                     mine = values + k0 - i - p.rel.q_offset - range.lo;
             }
-            ok = ok && umma::mbar_wait(at(bar->s_full[t]), kt & 1);
+            bool whole = cols == KT;
+            if (!whole || p.key_mask != nullptr) {
+                ok = ok && umma::mbar_poll(at(bar->v_full[s]), (kt / S) & 1);
+                whole = wholes[s] != 0;
+            }
+            ok = ok && umma::mbar_poll(at(bar->s_full[t]), kt & 1);
             umma::fence_after_sync();
-            const int chunks = (cols + 31) / 32;
+            const int chunks = any_row ? (cols + 31) / 32 : 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < KT / 32; ++c)
                 if (c < chunks) umma::tmem_ld32(s_col(t) + lanes + c * 32, x + c * 32);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < KT / 32; ++c)
                 if (c < chunks) umma::tmem_wait_ld32(x + c * 32);
-
-            const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f;
-            float top = -INFINITY;
-            if (plain) {
-                float top1 = -INFINITY;
+            if (L::kOwnP) {
+                umma::fence_before_sync();
+                umma::mbar_arrive(at(bar->s_free[t]));
+            }
+            float top = -INFINITY, mul = 1.0f, add = 0.0f;
+            if (whole && mine == nullptr && p.scale2 >= 0.0f) {
+                // raw scores: scale and constant join the exponential's argument
+                if (any_row) {
+                    float top1 = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < kTile; j += 2) {
-                    top = fmaxf(top, f32(x[j]));
-                    top1 = fmaxf(top1, f32(x[j + 1]));
-                }
-                top = fmaf(fmaxf(top, top1), p.scale2, flat);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c >= chunks) continue;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        float y = fmaf(f32(x[32 * c + j]), p.scale2, mine != nullptr ? mine[32 * c + j] : flat);
-                        y = (keep[c] >> j) & 1 ? y : -INFINITY;
-                        top = fmaxf(top, y);
-                        x[32 * c + j] = __float_as_uint(y);
+                    for (int j = 0; j < KT; j += 2) {
+                        top = fmaxf(top, f32(x[j]));
+                        top1 = fmaxf(top1, f32(x[j + 1]));
                     }
+                    mul = p.scale2;
+                    add = flat;
+                    top = fmaf(fmaxf(top, top1), mul, add);
+                }
+            } else {
+                const float* lim = limits + s * KT;
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) {
+                    if (c >= chunks) continue;
+                    uint32_t* y = x + 32 * c;
+                    float tc;
+                    if (mine == nullptr)
+                        tc = whole ? score_pass<32, false, false>(y, p.scale2, flat, nullptr, nullptr)
+                                   : score_pass<32, false, true>(y, p.scale2, flat, nullptr, lim + 32 * c);
+                    else
+                        tc = whole ? score_pass<32, true, false>(y, p.scale2, 0.0f, mine + 32 * c, nullptr)
+                                   : score_pass<32, true, true>(y, p.scale2, 0.0f, mine + 32 * c, lim + 32 * c);
+                    top = fmaxf(top, tc);
                 }
             }
+            // P and O of the tile before are this thread's again
+            if (L::kOwnP && kt > 0) {
+                ok = ok && umma::mbar_poll(at(bar->pv_done[t]), (kt - 1) & 1);
+                umma::fence_after_sync();
+            }
             // grow the maximum: always on the first tile, then only past kRescale
-            const bool grow = kt == 0 || top > m + kRescale;
-            if (__any_sync(~0u, grow)) {
+            if (__any_sync(~0u, kt == 0 || top > m + kRescale)) {
                 const float mn = fmaxf(m, top);
                 if (kt > 0) {
                     const float f = exp2_approx(m == -INFINITY ? -INFINITY : m - mn);
@@ -316,10 +402,9 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
                 }
                 m = mn;
             }
-            const float ms = m == -INFINITY ? 0.0f : m;
-            const float mul = plain ? p.scale2 : 1.0f, add = (plain ? flat : 0.0f) - ms;
+            add -= m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < KT / 32; ++c) {
                 if (c >= chunks) continue;
                 uint32_t pk[16];
 #pragma unroll
@@ -330,18 +415,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
                     l1 += e;
                     pk[j] = pack2<T>(a, e);
                 }
-                umma::tmem_st16(s_col(t) + lanes + c * 16, pk);
+                umma::tmem_st16(p_col(t) + lanes + c * 16, pk);
             }
             if (!whole) {
                 // rows of V behind masked keys: 0 in place of whatever they hold
-                const int s = kt % S;
-                ok = ok && umma::mbar_wait(at(bar->v_full[s]), (kt / S) & 1);
-                if (!((keep[warp % 4] >> lane) & 1)) {
+                if (r < KT && limits[s * KT + r] < 0.0f) {
                     for (int c = 0; c < L::kChunks; ++c)
 #pragma unroll
                         for (int j = 0; j < L::kRow; j += 16)
-                            umma::st_shared_v4(sm + L::kV + s * L::kTileBytes + c * L::kChunkBytes + r * L::kRow + j, 0, 0,
-                                               0, 0);
+                            umma::st_shared_v4(sm + L::kV + s * L::kBytes + c * L::kChunk + r * L::kRow + j, 0, 0, 0, 0);
                 }
                 umma::fence_proxy_async_smem();
             }
@@ -349,7 +431,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, NT == 1 ? 2 : 1) att
             umma::fence_before_sync();
             umma::mbar_arrive(at(bar->p_ready[t]));
         }
-        if (ok && n > 0) ok = umma::mbar_wait(at(bar->o_full[t]), 0);
+        if (n > 0) ok = ok && umma::mbar_poll(at(bar->pv_done[t]), L::kOwnP ? (n - 1) & 1 : 0);
         umma::fence_after_sync();
         if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x22);
         const float sum = l0 + l1;
@@ -436,8 +518,10 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o
     }
 }
 
-// How a call runs: query tiles per CTA, CTAs over the keys.
+// How a call runs: few rows per key (attention_token.cu) or query tiles per
+// CTA, and CTAs over the keys.
 struct Plan {
+    bool token;
     int nt, q_blocks, splits;
     int64_t part_bytes;
 };
@@ -445,13 +529,15 @@ struct Plan {
 Plan make_plan(const ww_attention_t& p, int sms) noexcept
 {
     Plan r;
+    r.token = token_form(p);
     r.nt = p.Lq > 1024 ? 2 : 1;
     r.q_blocks = (p.Lq + r.nt * kTile - 1) / (r.nt * kTile);
     const int64_t ctas = i64(r.q_blocks) * p.B * p.Hq;
-    const int key_tiles = (p.Lk + kTile - 1) / kTile;
+    const int key_tiles = (p.Lk + 63) / 64;
     r.splits = 1;
-    if (ctas > 0 && ctas < sms && key_tiles >= 4)
-        r.splits = static_cast<int>(std::min<int64_t>({2 * i64(sms) / ctas, key_tiles / 2, 64}));
+    if (r.token) r.splits = token_splits(p, sms);
+    else if (ctas > 0 && ctas < sms && key_tiles >= 8)
+        r.splits = static_cast<int>(std::min<int64_t>({2 * i64(sms) / ctas, key_tiles / 4, 64}));
     const int64_t rows = i64(p.B) * p.Lq * p.Hq;
     r.part_bytes = r.splits > 1 ? r.splits * rows * (p.D + 1) * 4 : 0;
     return r;
@@ -462,7 +548,7 @@ int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, NT>;
     const auto kernel = attention_forward_kernel<T, DP, NT>;
-    const int bytes = L::kBytes + 5 * f.max_entries;
+    const int bytes = L::kTotal + 5 * f.max_entries;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
         return launch_status("cross_attention");
     kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
@@ -470,17 +556,17 @@ int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 }
 
 template <typename T>
-int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noexcept
+int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_lse, cudaStream_t stream) noexcept
 {
     FwdParams f;
     const int dp = p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128;
     constexpr bool bf = !std::is_same<T, __half>::value;
     const int nq[3] = {p.B, p.Lq, p.Hq}, nk[3] = {p.B, p.Lk, p.Hk};
     const int cols = dp == 32 ? 32 : 64;
-    if (!encode_vectors_map(&f.q, bf, p.q, p.D, nq, p.q_strides, cols, kTile)) return WW_ERR_UNSUPPORTED;
+    if (!encode_vectors_map(&f.q, bf, p.q, p.D, nq, p.q_strides, cols, kBox)) return WW_ERR_UNSUPPORTED;
     if (p.Lk > 0) {
-        if (!encode_vectors_map(&f.k, bf, p.k, p.D, nk, p.k_strides, cols, kTile) ||
-            !encode_vectors_map(&f.v, bf, p.v, p.D, nk, p.v_strides, cols, kTile))
+        if (!encode_vectors_map(&f.k, bf, p.k, p.D, nk, p.k_strides, cols, kBox) ||
+            !encode_vectors_map(&f.v, bf, p.v, p.D, nk, p.v_strides, cols, kBox))
             return WW_ERR_UNSUPPORTED;
     }
     f.out = p.out;
@@ -491,12 +577,11 @@ int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noex
     f.max_entries = 0;
     if (p.bias_table != nullptr) {
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
-        const int all = (p.Lk + kTile - 1) / kTile * kTile + plan.nt * kTile;
+        const int all = (p.Lk + 127) / 128 * 128 + plan.nt * kTile;
         f.max_entries = (std::min(2 * (p.max_distance + kRelMargin) + 1, all) + 15) / 16 * 16;
     }
-    const int64_t rows = i64(p.B) * p.Lq * p.Hq;
-    f.part_o = static_cast<float*>(p.workspace);
-    f.part_lse = f.part_o + plan.splits * rows * p.D;
+    f.part_o = part_o;
+    f.part_lse = part_lse;
     f.B = p.B;
     f.Lq = p.Lq;
     f.Lk = p.Lk;
@@ -516,16 +601,24 @@ int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noex
     const int64_t ctas = i64(plan.q_blocks) * p.B * p.Hq * plan.splits;
     if (f.err == nullptr) return WW_ERR_DEVICE;
     if (ctas > 0x7fffffff) return WW_ERR_UNSUPPORTED;
-    int st;
     if (plan.nt == 1)
-        st = dp == 32 ? launch<T, 32, 1>(f, ctas, stream)
-           : dp == 64 ? launch<T, 64, 1>(f, ctas, stream) : launch<T, 128, 1>(f, ctas, stream);
-    else
-        st = dp == 32 ? launch<T, 32, 2>(f, ctas, stream)
-           : dp == 64 ? launch<T, 64, 2>(f, ctas, stream) : launch<T, 128, 2>(f, ctas, stream);
+        return dp == 32 ? launch<T, 32, 1>(f, ctas, stream)
+             : dp == 64 ? launch<T, 64, 1>(f, ctas, stream) : launch<T, 128, 1>(f, ctas, stream);
+    return dp == 32 ? launch<T, 32, 2>(f, ctas, stream)
+         : dp == 64 ? launch<T, 64, 2>(f, ctas, stream) : launch<T, 128, 2>(f, ctas, stream);
+}
+
+template <typename T>
+int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noexcept
+{
+    const int64_t rows = i64(p.B) * p.Lq * p.Hq;
+    float* part_o = static_cast<float*>(p.workspace);
+    float* part_lse = part_o + plan.splits * rows * p.D;
+    const int st = plan.token ? attention_token_launch(p, plan.splits, part_o, part_lse, stream)
+                              : tiles<T>(p, plan, part_o, part_lse, stream);
     if (st != WW_SUCCESS || plan.splits == 1) return st;
     attention_join_kernel<T><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
-        f.part_o, f.part_lse, p.out, p.lse, plan.splits, rows, p.Lq, p.Hq, p.D);
+        part_o, part_lse, p.out, p.lse, plan.splits, rows, p.Lq, p.Hq, p.D);
     return launch_status("cross_attention");
 }
 

@@ -1,0 +1,21 @@
+// attention_token.cuh -- the form of ww_cross_attention for a few query rows
+// per key head (attention_token.cu).
+#pragma once
+
+#include "attention.cuh"
+
+namespace ww {
+
+// Whether a call takes this form: at most 32 rows (query heads of a key head x
+// tokens) share each key.
+bool token_form(const ww_attention_t& p) noexcept;
+
+// CTAs that share the keys of one batch item and key head.
+int token_splits(const ww_attention_t& p, int sms) noexcept;
+
+// splits > 1: writes part_o [splits][B * Lq * Hq][D] (each normalised) and
+// part_lse [splits][B * Lq * Hq] (log2) instead of out and lse.
+int attention_token_launch(const ww_attention_t& p, int splits, float* part_o, float* part_lse,
+                           cudaStream_t stream) noexcept;
+
+}  // namespace ww

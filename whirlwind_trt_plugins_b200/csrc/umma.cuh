@@ -266,6 +266,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t saddr, uint32_t parity)
     return false;
 }
 
+// The same bound by count of non-blocking polls, for waits of a few hundred
+// clocks between warps that all have work.
+constexpr uint32_t kPollRounds = 1u << 26;
+__device__ __forceinline__ bool mbar_poll(uint32_t saddr, uint32_t parity)
+{
+    for (uint32_t i = 0; i < kPollRounds; ++i)
+        if (mbar_try_wait(saddr, parity)) return true;
+    return false;
+}
+
 // ---------------------------------------------------------------------------
 // Bulk copies (TMA engine, untiled) global -> shared and shared -> global
 // ---------------------------------------------------------------------------
@@ -438,6 +448,19 @@ __host__ __device__ constexpr uint32_t idesc_16bit(bool bf16, int M, int N, bool
 {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
            (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// True in one lane of a converged warp.  A warp that runs its loop as a whole and
+// issues MMAs under this keeps their descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(r));
+    return r != 0;
 }
 
 // D[tmem] (+)= A[tmem] * B[smem]: A's rows on the lanes, two consecutive
