@@ -34,6 +34,79 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 
+// ---- pairs of floats: one instruction for two values ----
+
+struct Pair {
+    uint64_t v;
+};
+
+__device__ __forceinline__ Pair pair(float lo, float hi)
+{
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ void unpair(Pair p, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v));
+}
+
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
+{
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+__device__ __forceinline__ Pair add2(Pair a, Pair b)
+{
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+__device__ __forceinline__ Pair mul2(Pair a, Pair b)
+{
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of two values on the FMA pipe, for x <= 2^8: x = n + f with n the nearest
+// whole number (read off the low bits after adding 1.5 * 2^23), 2^f on
+// [-1/2, 1/2] by a polynomial of degree 4 fitted to its relative error (2.6e-6,
+// a hundredth of what rounding P to 16 bits costs), n added to the exponent.
+// Below 2^-126: 2^-126.  The exponential unit does 16 values per clock and SM
+// against 128 here, so a share of a tile's exponentials is done this way.
+__device__ __forceinline__ Pair exp2_poly(Pair x)
+{
+    float a, b;
+    unpair(x, a, b);
+    x = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    constexpr float kMagic = 12582912.0f;
+    const Pair t = add2(x, pair(kMagic, kMagic));
+    const Pair n = add2(t, pair(-kMagic, -kMagic));
+    const Pair f = fma2(n, pair(-1.0f, -1.0f), x);
+    Pair p = pair(0.009570102f, 0.009570102f);
+    p = fma2(p, f, pair(0.05591786f, 0.05591786f));
+    p = fma2(p, f, pair(0.24024744f, 0.24024744f));
+    p = fma2(p, f, pair(0.6931218f, 0.6931218f));
+    p = fma2(p, f, pair(0.9999993f, 0.9999993f));
+    float ta, tb;
+    unpair(t, ta, tb);
+    unpair(p, a, b);
+    return pair(__int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23)),
+                __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23)));
+}
+
 // Relative-position buckets.  Distance d >= exact is in bucket
 // exact + #{t : least[t] <= d}: least[t] is the smallest whole distance of
 // logarithmic bucket t + 1, found once per call on the host, so that the

@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         }
         for (int s = 0; s < 2; ++s) {
             umma::mbar_init(at(bar->s_full[s]), 1);
-            umma::mbar_init(at(bar->p_ready[s]), 128);
+            umma::mbar_init(at(bar->p_ready[s]), 4);  // one arrival per warp
         }
         umma::mbar_init(at(bar->done), 1);
         umma::mbar_fence_init();
@@ -442,7 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             }
             umma::tmem_wait_st();
             umma::fence_before_sync();
-            umma::mbar_arrive(at(bar->p_ready[wg]));
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(at(bar->p_ready[wg]));
         }
         if (n > 0) ok = ok && umma::mbar_poll(at(bar->done), 0);
         umma::fence_after_sync();

@@ -52,6 +52,7 @@ namespace {
 
 constexpr int kTile = 128;       // query rows of a tile
 constexpr int kBox = 64;         // tokens of a TMA box
+constexpr int kPolyOf = 4;       // one pair of exponentials in so many on the FMA pipe
 constexpr float kRescale = 8.0f; // log2 growth of the maximum that is left in P
 
 struct FwdParams {
@@ -110,19 +111,50 @@ template <int N, bool BIAS, bool LIMIT>
 __device__ __forceinline__ float score_pass(uint32_t* x, float scale2, float flat, const float* bias, const float* limit)
 {
     float top[2] = {-INFINITY, -INFINITY};
+    const Pair scale_2 = pair(scale2, scale2), flat_2 = pair(flat, flat);
 #pragma unroll
     for (int j = 0; j < N; j += 4) {
-        float4 lim;
-        if (LIMIT) lim = *reinterpret_cast<const float4*>(limit + j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float y = fmaf(f32(x[j + i]), scale2, BIAS ? bias[j + i] : flat);
-            if (LIMIT) y = fminf(y, i == 0 ? lim.x : i == 1 ? lim.y : i == 2 ? lim.z : lim.w);
-            top[i & 1] = fmaxf(top[i & 1], y);
-            x[j + i] = __float_as_uint(y);
+        float y[4];
+        unpair(fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, BIAS ? pair(bias[j], bias[j + 1]) : flat_2), y[0], y[1]);
+        unpair(fma2(pair(f32(x[j + 2]), f32(x[j + 3])), scale_2, BIAS ? pair(bias[j + 2], bias[j + 3]) : flat_2), y[2], y[3]);
+        if (LIMIT) {
+            const float4 lim = *reinterpret_cast<const float4*>(limit + j);
+            y[0] = fminf(y[0], lim.x);
+            y[1] = fminf(y[1], lim.y);
+            y[2] = fminf(y[2], lim.z);
+            y[3] = fminf(y[3], lim.w);
         }
+        top[0] = max3(top[0], y[0], y[1]);
+        top[1] = max3(top[1], y[2], y[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[j + i] = __float_as_uint(y[i]);
     }
     return fmaxf(top[0], top[1]);
+}
+
+// P = 2^(mul x + add) of 32 columns: summed, rounded and put into 16 columns of
+// TMEM.  POLY: one pair in kPolyOf on the FMA pipe (whole tiles without a bias
+// of their own: there no argument is -inf).
+template <typename T, bool POLY>
+__device__ __forceinline__ void exp_pass(const uint32_t* x, float mul, float add, Pair& sum, uint32_t to)
+{
+    uint32_t pk[16];
+    const Pair mul_2 = pair(mul, mul), add_2 = pair(add, add);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const Pair arg = fma2(pair(f32(x[2 * j]), f32(x[2 * j + 1])), mul_2, add_2);
+        float a, b;
+        if (POLY && j % kPolyOf == kPolyOf - 1) {
+            unpair(exp2_poly(arg), a, b);
+        } else {
+            unpair(arg, a, b);
+            a = exp2_approx(a);
+            b = exp2_approx(b);
+        }
+        sum = add2(sum, pair(a, b));
+        pk[j] = pack2<T>(a, b);
+    }
+    umma::tmem_st16(to, pk);
 }
 
 template <typename T, int DP, int NT>
@@ -174,8 +206,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         }
         for (int t = 0; t < NT; ++t) {
             umma::mbar_init(at(bar->s_full[t]), 1);
-            umma::mbar_init(at(bar->s_free[t]), 128);
-            umma::mbar_init(at(bar->p_ready[t]), 128);
+            umma::mbar_init(at(bar->s_free[t]), 4);  // one arrival per warp
+            umma::mbar_init(at(bar->p_ready[t]), 4);
             umma::mbar_init(at(bar->pv_done[t]), 1);
         }
         umma::mbar_fence_init();
@@ -314,7 +346,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         const int t = warp / 4, r = threadIdx.x % 128;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;  // TMEM lane of this warp's first row
         const int i = q0 + t * kTile + r;
-        float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        float m = -INFINITY;
+        Pair l2 = pair(0.0f, 0.0f);  // sums of the even and of the odd columns
         bool ok = true;  // once a wait has run out: no more waits, everything else goes on
         const bool any_row = q0 + t * kTile + warp % 4 * 32 < p.Lq;  // else this warp keeps the barriers only
         uint32_t x[KT];
@@ -346,17 +379,19 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 if (c < chunks) umma::tmem_wait_ld32(x + c * 32);
             if (L::kOwnP) {
                 umma::fence_before_sync();
-                umma::mbar_arrive(at(bar->s_free[t]));
+                __syncwarp();
+                if (lane == 0) umma::mbar_arrive(at(bar->s_free[t]));
             }
             float top = -INFINITY, mul = 1.0f, add = 0.0f;
-            if (whole && mine == nullptr && p.scale2 >= 0.0f) {
+            const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f && flat > -INFINITY;
+            if (plain) {
                 // raw scores: scale and constant join the exponential's argument
                 if (any_row) {
                     float top1 = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < KT; j += 2) {
-                        top = fmaxf(top, f32(x[j]));
-                        top1 = fmaxf(top1, f32(x[j + 1]));
+                    for (int j = 0; j < KT; j += 4) {
+                        top = max3(top, f32(x[j]), f32(x[j + 1]));
+                        top1 = max3(top1, f32(x[j + 2]), f32(x[j + 3]));
                     }
                     mul = p.scale2;
                     add = flat;
@@ -388,8 +423,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 const float mn = fmaxf(m, top);
                 if (kt > 0) {
                     const float f = exp2_approx(m == -INFINITY ? -INFINITY : m - mn);
-                    l0 *= f;
-                    l1 *= f;
+                    l2 = mul2(l2, pair(f, f));
 #pragma unroll
                     for (int c = 0; c < DP; c += 16) {
                         uint32_t o[16];
@@ -403,19 +437,14 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 m = mn;
             }
             add -= m == -INFINITY ? 0.0f : m;
+            if (plain) {
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) {
-                if (c >= chunks) continue;
-                uint32_t pk[16];
+                for (int c = 0; c < KT / 32; ++c)
+                    if (any_row) exp_pass<T, true>(x + 32 * c, mul, add, l2, p_col(t) + lanes + c * 16);
+            } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float a = exp2_approx(fmaf(f32(x[32 * c + 2 * j]), mul, add));
-                    const float e = exp2_approx(fmaf(f32(x[32 * c + 2 * j + 1]), mul, add));
-                    l0 += a;
-                    l1 += e;
-                    pk[j] = pack2<T>(a, e);
-                }
-                umma::tmem_st16(p_col(t) + lanes + c * 16, pk);
+                for (int c = 0; c < KT / 32; ++c)
+                    if (c < chunks) exp_pass<T, false>(x + 32 * c, 1.0f, add, l2, p_col(t) + lanes + c * 16);
             }
             if (!whole) {
                 // rows of V behind masked keys: 0 in place of whatever they hold
@@ -429,12 +458,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             }
             umma::tmem_wait_st();
             umma::fence_before_sync();
-            umma::mbar_arrive(at(bar->p_ready[t]));
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(at(bar->p_ready[t]));
         }
         if (n > 0) ok = ok && umma::mbar_poll(at(bar->pv_done[t]), L::kOwnP ? (n - 1) & 1 : 0);
         umma::fence_after_sync();
         if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x22);
-        const float sum = l0 + l1;
+        float l_even, l_odd;
+        unpair(l2, l_even, l_odd);
+        const float sum = l_even + l_odd;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
         const int64_t rows = static_cast<int64_t>(p.B) * p.Lq * p.Hq;
