@@ -14,21 +14,22 @@
 // last time (P then stays below 2^8, exact in 16 bits' range): after the first
 // tiles that hardly happens, and no tile needs the read-multiply-write of O.
 //
-// Roles: 4 warps per query tile turn scores into P; one thread issues every
-// MMA; one warp every TMA load and the limits of masked keys.
+// Roles: per query tile 4 warps that turn scores into P and one that issues its
+// MMAs; one warp for every TMA load and the limits of masked keys.
 //
 // Bound: the exponential, 16 per clock and SM: 1024 clocks for 128 x 128
 // scores, against 16 D clocks for their products (8192 fp16 FMA per clock):
-// 512 at D = 32, equal at D = 64.  Two forms keep it busy:
-//   short rows (NT = 1)  one query tile, 64 keys at a time, three CTAs on an SM
-//                        (two at D = 128): the CTAs hide one another's round
-//                        trips, starts and ends.  P overwrites its scores and
-//                        the next S is issued behind the product that reads it
-//                        (MMAs of a CTA run in issue order).
-//   long rows (NT = 2)   two query tiles of one CTA against the same keys, which
-//                        halves what each SM reads of them from L2; P has its
-//                        own columns, so that the next S is formed as soon as
-//                        the scores have been read.
+// 512 at D = 32, equal at D = 64.  A round trip (scores, maximum, P, product) is
+// a chain of latencies several times its exponentials, so what counts is how
+// many tiles of an SM are under way: 64 keys at a time keep a tile's TMEM at
+// 64 + D columns (P overwrites its scores, the next S is issued behind the
+// product that reads them: MMAs of one thread run in issue order), and scores
+// are read 32 columns at a time in a loop that fits 80 registers -- four tiles on
+// an SM, 16 warps of elementwise work (two tiles at D = 128, where S, P and O of
+// a tile take 192 columns).
+//   NT = 1  four CTAs of one query tile: starts and ends overlap as well
+//   NT = 2  two CTAs of two query tiles against the same keys: half the reads of
+//           K and V from L2, for long rows
 //
 // Masked keys: their scores meet a limit of -inf (a minimum, which also takes
 // a NaN) and their rows of V are zeroed in shared memory (0 times a NaN would
@@ -75,8 +76,7 @@ struct FwdParams {
 
 template <int DP, int NT>
 struct Layout {
-    static constexpr bool kOwnP = NT == 2;                 // P beside its scores instead of over them
-    static constexpr int kKeys = NT == 2 && DP <= 64 ? 128 : 64;
+    static constexpr int kKeys = 64;                       // keys of a tile
     static constexpr int kRow = DP == 32 ? 64 : 128;       // bytes of an operand row
     static constexpr int kCols = kRow / 2;                 // values in it
     static constexpr int kChunks = DP * 2 / kRow;          // rows of one token
@@ -91,29 +91,29 @@ struct Layout {
     static constexpr int kBar = kLim + kStages * (kKeys + 4) * 4;
     static constexpr int kBias = kBar + 256;               // [entries] values, [entries] buckets
     static constexpr int kTotal = kBias + 1024;            // + alignment of the base, + the bias
-    static constexpr int kPCols = kOwnP ? kKeys / 2 : 0;
-    static constexpr int kNeed = NT * (kKeys + kPCols + DP);
+    static constexpr int kNeed = NT * (kKeys + DP);
     static constexpr int kColumns = kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
-    static constexpr int kThreads = NT * 128 + 64;
-    static constexpr int kCtas = NT == 2 ? 1 : DP == 128 ? 2 : 3;
+    static constexpr int kThreads = NT * 160 + 32;         // softmax warps, MMA warps, TMA warp
+    static constexpr int kCtas = 512 / kColumns;
 };
 
 template <int DP, int NT>
 struct Bars {
     static constexpr int kStages = Layout<DP, NT>::kStages;
-    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], s_free[NT],
-        p_ready[NT], pv_done[NT];
+    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], p_ready[NT],
+        o_full[NT];
     uint32_t tmem;
 };
 
-// Scores of N columns in log2 units with bias and limits, and their maximum.
-template <int N, bool BIAS, bool LIMIT>
-__device__ __forceinline__ float score_pass(uint32_t* x, float scale2, float flat, const float* bias, const float* limit)
+// 32 scores in log2 units with bias and limits, and their maximum.
+template <bool BIAS, bool LIMIT>
+__device__ __forceinline__ float score_pass(uint32_t (&x)[32], float scale2, float flat, const float* bias,
+                                            const float* limit)
 {
     float top[2] = {-INFINITY, -INFINITY};
     const Pair scale_2 = pair(scale2, scale2), flat_2 = pair(flat, flat);
 #pragma unroll
-    for (int j = 0; j < N; j += 4) {
+    for (int j = 0; j < 32; j += 4) {
         float y[4];
         unpair(fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, BIAS ? pair(bias[j], bias[j + 1]) : flat_2), y[0], y[1]);
         unpair(fma2(pair(f32(x[j + 2]), f32(x[j + 3])), scale_2, BIAS ? pair(bias[j + 2], bias[j + 3]) : flat_2), y[2], y[3]);
@@ -136,7 +136,7 @@ __device__ __forceinline__ float score_pass(uint32_t* x, float scale2, float fla
 // TMEM.  POLY: one pair in kPolyOf on the FMA pipe (whole tiles without a bias
 // of their own: there no argument is -inf).
 template <typename T, bool POLY>
-__device__ __forceinline__ void exp_pass(const uint32_t* x, float mul, float add, Pair& sum, uint32_t to)
+__device__ __forceinline__ void exp_pass(const uint32_t (&x)[32], float mul, float add, Pair& sum, uint32_t to)
 {
     uint32_t pk[16];
     const Pair mul_2 = pair(mul, mul), add_2 = pair(add, add);
@@ -195,20 +195,19 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 umma::tma_load_4d(sm + L::kK + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.k, c * L::kCols, g * p.k_h,
                                   (first + kt) * KT + x, b * p.k_b, at(bar->k_full[s]));
     };
-    if (warp == NT * 4 + 1 && lane == 0) {
+    if (warp == NT * 5 && lane == 0) {
         // this thread alone uses the barriers until the block's first barrier below
         umma::mbar_init(at(bar->q_full), 1);
         for (int s = 0; s < S; ++s) {
             umma::mbar_init(at(bar->k_full[s]), 1);
-            umma::mbar_init(at(bar->k_empty[s]), 1);
+            umma::mbar_init(at(bar->k_empty[s]), tiles);  // one MMA warp per tile
             umma::mbar_init(at(bar->v_full[s]), 1);
-            umma::mbar_init(at(bar->v_empty[s]), 1);
+            umma::mbar_init(at(bar->v_empty[s]), tiles);
         }
         for (int t = 0; t < NT; ++t) {
             umma::mbar_init(at(bar->s_full[t]), 1);
-            umma::mbar_init(at(bar->s_free[t]), 4);  // one arrival per warp
-            umma::mbar_init(at(bar->p_ready[t]), 4);
-            umma::mbar_init(at(bar->pv_done[t]), 1);
+            umma::mbar_init(at(bar->p_ready[t]), 4);  // one arrival per warp
+            umma::mbar_init(at(bar->o_full[t]), 1);
         }
         umma::mbar_fence_init();
         umma::fence_proxy_async_smem();
@@ -240,12 +239,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = bar->tmem;
-    // columns: S of each tile, P of each tile, O of each tile
-    const auto s_col = [&](int t) { return tmem + t * KT; };
-    const auto p_col = [&](int t) { return L::kOwnP ? tmem + NT * KT + t * L::kPCols : s_col(t); };
-    const auto o_col = [&](int t) { return tmem + NT * (KT + L::kPCols) + t * DP; };
 
-    if (warp == NT * 4 + 1) {
+    if (warp == NT * 5) {
         bool ok = true;
         for (int kt = 0; kt < n; ++kt) {
             const int s = kt % S;
@@ -282,75 +277,66 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             if (!__shfl_sync(~0u, ok, 0)) break;
         }
         if (lane == 0 && !ok) record_device_error(p.err, kErrMbarTimeout | 0x20);
-    } else if (warp == NT * 4) {
-        if (n > 0) {
-            // One lane issues every product of the CTA.  The warp runs the loop as a
-            // whole, descriptors are formed once and advanced by constants and loops are
-            // unrolled: everything a product needs is in uniform registers (forming it per
-            // product, in one thread, took 100 clocks each and was what the kernel waited for).
-            const uint32_t tm = __reduce_or_sync(~0u, tmem);  // uniform
-            const auto s_col = [&](int t) { return tm + t * KT; };
-            const auto p_col = [&](int t) { return L::kOwnP ? tm + NT * KT + t * L::kPCols : s_col(t); };
-            const auto o_col = [&](int t) { return tm + NT * (KT + L::kPCols) + t * DP; };
+    } else if (warp >= NT * 4) {
+        const int t = warp - NT * 4;
+        if (n > 0 && t < tiles) {
+            // The warp runs the loop as a whole, one elected lane issues; descriptors are
+            // formed once and advanced by constants and loops are unrolled, so that all a
+            // product needs is in uniform registers (formed per product in one thread
+            // they took 100 clocks each, more than the products).
             constexpr bool bf = !std::is_same<T, __half>::value;
             constexpr uint32_t id_full = umma::idesc_16bit(bf, kTile, KT, false), id_o = umma::idesc_16bit(bf, kTile, DP, true);
-            const uint64_t q_desc = umma::smem_desc_swizzled<L::kRow>(sm, 16);
+            const uint32_t s_col = __reduce_or_sync(~0u, tmem) + t * KT, o_col = s_col + (NT - t) * KT + t * DP;
+            const uint64_t q_desc = umma::smem_desc_swizzled<L::kRow>(sm + t * L::kQBytes, 16);
             const uint64_t k_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kK, 16);
             const uint64_t v_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kV, L::kChunk);
-            const auto qk = [&](int t, int kt) {
+            const auto qk = [&](int kt) {
                 const int s = kt % S, cols = cols_of(kt);
                 const uint32_t id = cols >= KT ? id_full : umma::idesc_16bit(bf, kTile, (cols + 15) / 16 * 16, false);
-                const uint64_t qd = umma::desc_advance(q_desc, t * L::kQBytes), kd = umma::desc_advance(k_desc, s * L::kBytes);
-                const uint32_t to = s_col(t);
-                if (!umma::elect_one()) return;
+                const uint64_t kd = umma::desc_advance(k_desc, s * L::kBytes);
+                if (umma::elect_one()) {
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i)
-                    umma::mma_f16_ss(to, umma::desc_advance(qd, i * 16 / L::kCols * L::kQChunk + i * 16 % L::kCols * 2),
-                                     umma::desc_advance(kd, i * 16 / L::kCols * L::kChunk + i * 16 % L::kCols * 2), id, i > 0);
-                umma::mma_commit(at(bar->s_full[t]));
-                if (t == tiles - 1) umma::mma_commit(at(bar->k_empty[s]));
-            };
-            const auto pv = [&](int t, int kt) {
-                const int s = kt % S, cols = cols_of(kt);
-                const uint64_t vd = umma::desc_advance(v_desc, s * L::kBytes);
-                const uint32_t from = p_col(t), to = o_col(t);
-                if (!umma::elect_one()) return;
-#pragma unroll
-                for (int i = 0; i < KT / 16; ++i)
-                    if (i * 16 < cols)
-                        umma::mma_f16_ts(to, from + i * 8, umma::desc_advance(vd, i * 16 * L::kRow), id_o, kt > 0 || i > 0);
-                if (L::kOwnP || kt == n - 1) umma::mma_commit(at(bar->pv_done[t]));
-                if (t == tiles - 1) umma::mma_commit(at(bar->v_empty[s]));
+                    for (int i = 0; i < DP / 16; ++i)
+                        umma::mma_f16_ss(s_col, umma::desc_advance(q_desc, i * 16 / L::kCols * L::kQChunk + i * 16 % L::kCols * 2),
+                                         umma::desc_advance(kd, i * 16 / L::kCols * L::kChunk + i * 16 % L::kCols * 2), id, i > 0);
+                    umma::mma_commit(at(bar->s_full[t]));
+                    umma::mma_commit(at(bar->k_empty[s]));
+                }
+                __syncwarp();
             };
             bool ok = umma::mbar_poll(at(bar->q_full), 0) && umma::mbar_poll(at(bar->k_full[0]), 0);
-            for (int t = 0; t < tiles && ok; ++t) qk(t, 0);
-            for (int kt = 0; kt < n && ok; ++kt)
-                for (int t = 0; t < tiles && ok; ++t) {
-                    const bool next = kt + 1 < n;
-                    if (next && t == 0) ok = umma::mbar_poll(at(bar->k_full[(kt + 1) % S]), ((kt + 1) / S) & 1);
-                    if (L::kOwnP && next && ok) {
-                        ok = umma::mbar_poll(at(bar->s_free[t]), kt & 1);
-                        umma::fence_after_sync();
-                        if (ok) qk(t, kt + 1);
-                    }
-                    if (t == 0) ok = ok && umma::mbar_poll(at(bar->v_full[kt % S]), (kt / S) & 1);
-                    ok = ok && umma::mbar_poll(at(bar->p_ready[t]), kt & 1);
-                    if (!ok) break;
-                    umma::fence_after_sync();
-                    pv(t, kt);
-                    if (!L::kOwnP && next) qk(t, kt + 1);
+            if (ok) qk(0);
+            for (int kt = 0; kt < n && ok; ++kt) {
+                const int s = kt % S, cols = cols_of(kt);
+                ok = umma::mbar_poll(at(bar->v_full[s]), (kt / S) & 1) && umma::mbar_poll(at(bar->p_ready[t]), kt & 1);
+                if (!ok) break;
+                umma::fence_after_sync();
+                const uint64_t vd = umma::desc_advance(v_desc, s * L::kBytes);
+                if (umma::elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < KT / 16; ++i)
+                        if (i * 16 < cols)
+                            umma::mma_f16_ts(o_col, s_col + i * 8, umma::desc_advance(vd, i * 16 * L::kRow), id_o, kt > 0 || i > 0);
+                    umma::mma_commit(at(bar->v_empty[s]));
+                    if (kt == n - 1) umma::mma_commit(at(bar->o_full[t]));
                 }
+                __syncwarp();
+                if (kt + 1 < n) {
+                    ok = umma::mbar_poll(at(bar->k_full[(kt + 1) % S]), ((kt + 1) / S) & 1);
+                    if (ok) qk(kt + 1);
+                }
+            }
             if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x21);
         }
     } else if (warp / 4 < tiles) {
         const int t = warp / 4, r = threadIdx.x % 128;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;  // TMEM lane of this warp's first row
+        const uint32_t s_col = tmem + lanes + t * KT, o_col = tmem + lanes + NT * KT + t * DP;
         const int i = q0 + t * kTile + r;
         float m = -INFINITY;
         Pair l2 = pair(0.0f, 0.0f);  // sums of the even and of the odd columns
         bool ok = true;  // once a wait has run out: no more waits, everything else goes on
         const bool any_row = q0 + t * kTile + warp % 4 * 32 < p.Lq;  // else this warp keeps the barriers only
-        uint32_t x[KT];
         for (int kt = 0; kt < n; ++kt) {
             const int s = kt % S, k0 = (first + kt) * KT, cols = cols_of(kt);
             // the bias: one value for the tile, or by j - i from this row's start
@@ -371,84 +357,68 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             ok = ok && umma::mbar_poll(at(bar->s_full[t]), kt & 1);
             umma::fence_after_sync();
             const int chunks = any_row ? (cols + 31) / 32 : 0;
-#pragma unroll
-            for (int c = 0; c < KT / 32; ++c)
-                if (c < chunks) umma::tmem_ld32(s_col(t) + lanes + c * 32, x + c * 32);
-#pragma unroll
-            for (int c = 0; c < KT / 32; ++c)
-                if (c < chunks) umma::tmem_wait_ld32(x + c * 32);
-            if (L::kOwnP) {
-                umma::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) umma::mbar_arrive(at(bar->s_free[t]));
-            }
-            float top = -INFINITY, mul = 1.0f, add = 0.0f;
+            // raw scores: scale and constant join the exponential's argument
             const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f && flat > -INFINITY;
-            if (plain) {
-                // raw scores: scale and constant join the exponential's argument
-                if (any_row) {
+            float top = -INFINITY;
+            const float* lim = limits + s * KT;
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                uint32_t x[32];
+                umma::tmem_ld32(s_col + c * 32, x);
+                umma::tmem_wait_ld32(x);
+                if (plain) {
                     float top1 = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < KT; j += 4) {
+                    for (int j = 0; j < 32; j += 4) {
                         top = max3(top, f32(x[j]), f32(x[j + 1]));
                         top1 = max3(top1, f32(x[j + 2]), f32(x[j + 3]));
                     }
-                    mul = p.scale2;
-                    add = flat;
-                    top = fmaf(fmaxf(top, top1), mul, add);
-                }
-            } else {
-                const float* lim = limits + s * KT;
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
-                    if (c >= chunks) continue;
-                    uint32_t* y = x + 32 * c;
+                    top = fmaxf(top, top1);
+                } else {
                     float tc;
                     if (mine == nullptr)
-                        tc = whole ? score_pass<32, false, false>(y, p.scale2, flat, nullptr, nullptr)
-                                   : score_pass<32, false, true>(y, p.scale2, flat, nullptr, lim + 32 * c);
+                        tc = whole ? score_pass<false, false>(x, p.scale2, flat, nullptr, nullptr)
+                                   : score_pass<false, true>(x, p.scale2, flat, nullptr, lim + 32 * c);
                     else
-                        tc = whole ? score_pass<32, true, false>(y, p.scale2, 0.0f, mine + 32 * c, nullptr)
-                                   : score_pass<32, true, true>(y, p.scale2, 0.0f, mine + 32 * c, lim + 32 * c);
+                        tc = whole ? score_pass<true, false>(x, p.scale2, 0.0f, mine + 32 * c, nullptr)
+                                   : score_pass<true, true>(x, p.scale2, 0.0f, mine + 32 * c, lim + 32 * c);
                     top = fmaxf(top, tc);
+                    umma::tmem_st32(s_col + c * 32, x);
                 }
             }
-            // P and O of the tile before are this thread's again
-            if (L::kOwnP && kt > 0) {
-                ok = ok && umma::mbar_poll(at(bar->pv_done[t]), (kt - 1) & 1);
-                umma::fence_after_sync();
-            }
+            if (plain) top = fmaf(top, p.scale2, flat);
+            else umma::tmem_wait_st();
             // grow the maximum: always on the first tile, then only past kRescale
             if (__any_sync(~0u, kt == 0 || top > m + kRescale)) {
                 const float mn = fmaxf(m, top);
-                if (kt > 0) {
+                if (kt > 0) {  // the product before is done: its commit came before that of these scores
                     const float f = exp2_approx(m == -INFINITY ? -INFINITY : m - mn);
                     l2 = mul2(l2, pair(f, f));
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < DP; c += 16) {
                         uint32_t o[16];
-                        umma::tmem_ld16(o_col(t) + lanes + c, o);
+                        umma::tmem_ld16(o_col + c, o);
                         umma::tmem_wait_ld16(o);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(f32(o[j]) * f);
-                        umma::tmem_st16(o_col(t) + lanes + c, o);
+                        umma::tmem_st16(o_col + c, o);
                     }
                 }
                 m = mn;
             }
-            add -= m == -INFINITY ? 0.0f : m;
-            if (plain) {
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
-                    if (any_row) exp_pass<T, true>(x + 32 * c, mul, add, l2, p_col(t) + lanes + c * 16);
-            } else {
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
-                    if (c < chunks) exp_pass<T, false>(x + 32 * c, 1.0f, add, l2, p_col(t) + lanes + c * 16);
+            const float add = (plain ? flat : 0.0f) - (m == -INFINITY ? 0.0f : m);
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                uint32_t x[32];
+                umma::tmem_ld32(s_col + c * 32, x);
+                umma::tmem_wait_ld32(x);
+                // 16 columns of P over scores that have been read
+                if (plain) exp_pass<T, true>(x, p.scale2, add, l2, s_col + c * 16);
+                else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c * 16);
             }
             if (!whole) {
                 // rows of V behind masked keys: 0 in place of whatever they hold
-                if (r < KT && limits[s * KT + r] < 0.0f) {
+                if (r < KT && lim[r] < 0.0f) {
                     for (int c = 0; c < L::kChunks; ++c)
 #pragma unroll
                         for (int j = 0; j < L::kRow; j += 16)
@@ -461,7 +431,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             __syncwarp();
             if (lane == 0) umma::mbar_arrive(at(bar->p_ready[t]));
         }
-        if (n > 0) ok = ok && umma::mbar_poll(at(bar->pv_done[t]), L::kOwnP ? (n - 1) & 1 : 0);
+        if (n > 0) ok = ok && umma::mbar_poll(at(bar->o_full[t]), 0);
         umma::fence_after_sync();
         if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x22);
         float l_even, l_odd;
@@ -474,7 +444,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
             if (n > 0) {
-                umma::tmem_ld32(o_col(t) + lanes + c, o);
+                umma::tmem_ld32(o_col + c, o);
                 umma::tmem_wait_ld32(o);
             } else {
 #pragma unroll
