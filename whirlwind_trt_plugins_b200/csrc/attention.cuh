@@ -208,11 +208,13 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
 
 __device__ __forceinline__ float f32(uint32_t u) { return __uint_as_float(u); }
 
-// Barrier of the 128 threads of warpgroup w (0 or 1).
+// Barrier of the 128 threads of warpgroup w < 4.
 __device__ __forceinline__ void warpgroup_sync(int w)
 {
     if (w == 0) asm volatile("bar.sync 1, 128;" : : : "memory");
-    else asm volatile("bar.sync 2, 128;" : : : "memory");
+    else if (w == 1) asm volatile("bar.sync 2, 128;" : : : "memory");
+    else if (w == 2) asm volatile("bar.sync 3, 128;" : : : "memory");
+    else asm volatile("bar.sync 4, 128;" : : : "memory");
 }
 
 // Fills `out`; WW_SUCCESS or the status of rejected arguments (attention_host.cu).

@@ -11,11 +11,13 @@
 //   keys:     128 keys on the rows (S^T, dP^T), streaming 64 queries at a time
 //             over all query heads of the key head; dV and dK in TMEM
 //   queries:  128 queries on the rows, streaming 64 keys at a time; dQ in TMEM
-// The row operands stay in shared memory; each streamed tile is the K-major B
-// operand of the two score products and, unchanged, the MN-major B operand of
-// the accumulating ones; P and dS return to TMEM as their A operands.  Two
-// tiles are in flight (S and dP of 64 columns each: 256 of 512 columns), one
-// per warpgroup, so that products and elementwise work overlap.
+// The row operands are A operands in TMEM (in shared memory where the widest
+// accumulators leave no room: keys at D = 128), which keeps their re-reading for
+// every tile off the shared memory; each streamed tile is the K-major B operand
+// of the two score products and, unchanged, the MN-major B operand of the
+// accumulating ones; P and dS return to TMEM over S and dP as A operands.  Two
+// tiles are under way, each with two warpgroups of elementwise work (32 of its 64
+// columns each).
 //
 // 16-bit ranges: P is kept as 2^6 P, and in fp16 dS is formed from dO 2^e with
 // 2^e max|dO| in [1, 2): gradients as small as a mean over a batch leaves
@@ -41,23 +43,28 @@ constexpr int kRows = 128;
 constexpr int kCols = 64;
 constexpr int kShift = 6;         // P is kept times 2^kShift
 constexpr int kPitch = 33;        // floats of a dS row in shared memory
-constexpr int kThreads = 2 * 128 + 64;
+constexpr int kGroups = 4;        // warpgroups: two per streamed tile
+constexpr int kThreads = kGroups * 128 + 64;
+constexpr int kMmaWarp = kGroups * 4, kLoadWarp = kMmaWarp + 1;
 
 struct BwdParams {
     CUtensorMap q, k, v, dout;  // boxes of 64 tokens
+    const void* r1;             // row operands: keys: k, v; queries: q, dout
+    const void* r2;
     const int32_t* k_lens;
     const uint8_t* key_mask;
     const void* table;
-    const float* lse2;    // [B * Hq][Lq_pad] log2 units minus kShift; +inf: no gradient
-    const float* delta;   // [B * Hq][Lq_pad]
+    const float* nlse2;   // [B * Hq][Lq_pad] kShift - log2 units; -inf: no gradient
+    const float* ndelta;  // [B * Hq][Lq_pad]
     const uint32_t* top;  // bits of max |dO| (fp16)
     void* d1;             // keys: dk; queries: dq
     void* d2;             // keys: dv
-    float* part;          // splits > 1: [splits][values of d1, then of d2] fp32
-    float* table_part;    // queries: [B * Hq * blocks * splits][buckets]
+    float* part;          // split items: [item][split][d1, d2][128][D] fp32
+    float* table_part;    // queries: [CTA][buckets]
     RelBuckets rel;
+    int64_t r1_strides[3], r2_strides[3];
     int32_t B, Lq, Lk, Hq, Hk, D, Lq_pad;
-    int32_t blocks, splits, q_tiles;
+    int32_t blocks, whole_items, splits, q_tiles;
     int32_t q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h;
     int32_t max_entries;  // relative positions a CTA keeps
     float scale, scale2;
@@ -66,6 +73,7 @@ struct BwdParams {
 
 template <int DP, bool KEYS>
 struct Layout {
+    static constexpr bool kRowsInTmem = !(KEYS && DP == 128);
     static constexpr int kRow = DP == 32 ? 64 : 128;   // bytes of an operand row
     static constexpr int kVals = kRow / 2;
     static constexpr int kChunks = DP * 2 / kRow;
@@ -74,12 +82,14 @@ struct Layout {
     static constexpr int kColChunk = kCols * kRow;     // streamed operand
     static constexpr int kColBytes = kCols * DP * 2;
     static constexpr int kStages = DP == 128 ? 2 : 4;
-    static constexpr int kR1 = 0;
-    static constexpr int kR2 = kRowBytes;
-    static constexpr int kC = 2 * kRowBytes;                       // stages of C1, C2
-    static constexpr int kVec = kC + kStages * 2 * kColBytes;      // KEYS: lse2, delta of 64 queries per stage
+    static constexpr int kC = kRowsInTmem ? 0 : 2 * kRowBytes;     // stages of C1, C2
+    static constexpr int kVec = kC + kStages * 2 * kColBytes;      // KEYS: nlse2, ndelta of 64 queries per stage
     static constexpr int kBar = kVec + (KEYS ? kStages * 2 * kCols * 4 : 0);
     static constexpr int kBias = kBar + 256;                       // bias tables, see below
+    // TMEM columns: S of both tiles, dP of both, accumulators, row operands
+    static constexpr int kDp = 2 * kCols, kAcc1 = 4 * kCols, kAcc2 = kAcc1 + DP, kR1 = kAcc1 + (KEYS ? 2 : 1) * DP,
+                         kR2 = kR1 + DP / 2;
+    static_assert(!kRowsInTmem || kR2 + DP / 2 <= 512, "TMEM");
 };
 
 template <int DP, bool KEYS>
@@ -89,15 +99,16 @@ struct Bars {
     uint32_t tmem;
 };
 
-// Shared memory after the barriers, with a bias:
-//   buckets  [entries] bytes
-//   KEYS:    values [2 warpgroups][entries] floats, rebuilt when the head changes
-//   queries: values [entries], with a gradient also the diagonals
-//            [2][entries], plain sums [8 warps][kMaxBuckets] and dS [2][128][33]
+// Shared memory after the barriers, with a bias (E = entries):
+//   buckets  [E] bytes
+//   KEYS:    values [4 warpgroups][E] floats, rebuilt when the head changes
+//   queries: values [E], with the gradient's diagonals [4 warpgroups][E], plain
+//            sums [16 warps][kMaxBuckets] and dS [4][128][33]
 __host__ __device__ inline int bias_bytes(bool keys, int entries)
 {
     const int e = (entries + 15) / 16 * 16;
-    return keys ? e + 2 * e * 4 : e + 3 * e * 4 + 8 * kMaxBuckets * 4 + 2 * kRows * kPitch * 4;
+    return keys ? e + kGroups * e * 4
+                : e + (1 + kGroups) * e * 4 + kGroups * 4 * kMaxBuckets * 4 + kGroups * kRows * kPitch * 4;
 }
 
 template <typename T, int DP, bool KEYS, bool BIAS>
@@ -113,95 +124,91 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     Bar* bar = reinterpret_cast<Bar*>(base + L::kBar);
     const auto at = [](const uint64_t& b) { return umma::smem_addr(&b); };
 
-    const int split = blockIdx.x % p.splits;
-    int rest = blockIdx.x / p.splits;
-    const int block = rest % p.blocks;
-    rest /= p.blocks;
+    // items (row block, head, batch item); the last ones are split over their streamed tiles
+    const int blk = blockIdx.x;
+    const bool in_parts = blk >= p.whole_items;
+    const int split = in_parts ? (blk - p.whole_items) % p.splits : 0, splits = in_parts ? p.splits : 1;
+    const int item = in_parts ? p.whole_items + (blk - p.whole_items) / p.splits : blk;
     const int heads = KEYS ? p.Hk : p.Hq, group = p.Hq / p.Hk;
-    const int h = rest % heads, b = rest / heads;
+    const int block = item % p.blocks, h = item / p.blocks % heads, b = item / p.blocks / heads;
     const int row0 = block * kRows;
     const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
     // streamed tiles of this CTA
     const int n_all = KEYS ? (row0 < len ? group * p.q_tiles : 0) : (len + kCols - 1) / kCols;
-    const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / p.splits);
-    const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / p.splits) - first;
+    const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / splits);
+    const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / splits) - first;
 
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // warp-uniform: roles branch as warps
+    const int wg = warp / 4;
     RelRange range;
     uint8_t* buckets = base + L::kBias;
-    float* values = nullptr;  // bias of [range]: KEYS: of this warpgroup's current head
+    float* values = nullptr;  // bias of [range]; KEYS: of this warpgroup's current head
     const int entries = (p.max_entries + 15) / 16 * 16;
     if (BIAS) {
         // positions j - i - offset of the CTA's tiles, padded rows and columns included
         range = KEYS ? rel_range(p.rel, row0 - (p.q_tiles * kCols - 1) - p.rel.q_offset, row0 + kRows - 1 - p.rel.q_offset)
                      : rel_range(p.rel, first * kCols - (row0 + kRows - 1) - p.rel.q_offset,
                                  (first + n) * kCols - 1 - row0 - p.rel.q_offset);
-        if (n > 0) build_buckets(p.rel, range, buckets, threadIdx.x, kThreads);
-        values = reinterpret_cast<float*>(base + L::kBias + entries) + (KEYS && warp >= 4 ? entries : 0);
-        if (!KEYS) {
-            const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
-            if (n > 0)
-                for (int e = threadIdx.x; e < range.count(); e += kThreads)
-                    values[e] = bias_value<T>(table[rel_bucket(p.rel, range.lo + e)]) * kLog2eF;
-            float* diag = values + entries;  // diagonals, then plain sums
-            for (int e = threadIdx.x; e < 2 * entries + 8 * kMaxBuckets; e += kThreads) diag[e] = 0.0f;
-        }
+        values = reinterpret_cast<float*>(base + L::kBias + entries) + (KEYS ? min(wg, kGroups - 1) * entries : 0);
+        const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
+        if (n > 0)
+            for (int e = threadIdx.x; e < range.count(); e += kThreads) {
+                const int bu = rel_bucket(p.rel, range.lo + e);
+                buckets[e] = static_cast<uint8_t>(bu);
+                if (!KEYS) values[e] = bias_value<T>(table[bu]) * kLog2eF;
+            }
+        if (!KEYS)  // diagonals, then plain sums
+            for (int e = threadIdx.x; e < kGroups * entries + kGroups * 4 * kMaxBuckets; e += kThreads)
+                values[entries + e] = 0.0f;
     }
-    if (threadIdx.x == 0) {
-        umma::mbar_init(at(bar->r_full), 1);
+    if (warp == kLoadWarp && lane == 0) {
+        umma::mbar_init(at(bar->r_full), L::kRowsInTmem ? 8 : 1);
         for (int s = 0; s < S; ++s) {
             umma::mbar_init(at(bar->c_full[s]), 1);
             umma::mbar_init(at(bar->c_empty[s]), 1);
         }
         for (int s = 0; s < 2; ++s) {
             umma::mbar_init(at(bar->s_full[s]), 1);
-            umma::mbar_init(at(bar->p_ready[s]), 4);  // one arrival per warp
+            umma::mbar_init(at(bar->p_ready[s]), 8);  // one arrival per warp
         }
         umma::mbar_init(at(bar->done), 1);
         umma::mbar_fence_init();
+        umma::fence_proxy_async_smem();
     }
-    if (warp == 8) umma::tmem_alloc(umma::smem_addr(&bar->tmem), 512);
+    if (warp == kMmaWarp) umma::tmem_alloc(umma::smem_addr(&bar->tmem), 512);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = bar->tmem;
-    // columns: S of both stages, dP of both stages, then the accumulators
-    const auto s_col = [&](int st) { return tmem + st * kCols; };
-    const auto dp_col = [&](int st) { return tmem + 2 * kCols + st * kCols; };
-    const uint32_t acc1 = tmem + 4 * kCols, acc2 = acc1 + DP;
 
-    if (warp == 9) {
+    if (warp == kLoadWarp) {
         if (lane == 0 && n > 0) {
-            const CUtensorMap* r1 = KEYS ? &p.k : &p.q;
-            const CUtensorMap* r2 = KEYS ? &p.v : &p.dout;
             const CUtensorMap* c1 = KEYS ? &p.q : &p.k;
             const CUtensorMap* c2 = KEYS ? &p.dout : &p.v;
-            const int r1b = KEYS ? p.k_b : p.q_b, r1h = KEYS ? p.k_h : p.q_h, r2b = KEYS ? p.v_b : p.g_b,
-                      r2h = KEYS ? p.v_h : p.g_h;
             const int c1b = KEYS ? p.q_b : p.k_b, c1h = KEYS ? p.q_h : p.k_h, c2b = KEYS ? p.g_b : p.v_b,
                       c2h = KEYS ? p.g_h : p.v_h;
-            const int rows_end = KEYS ? p.Lk : p.Lq;
-            // a half of the row tile that lies beyond the tensor reads as zeros like any other place outside
-            umma::mbar_arrive_expect_tx(at(bar->r_full), 2 * L::kRowBytes);
-            for (int half = 0; half < 2; ++half)
-                for (int c = 0; c < L::kChunks; ++c) {
-                    const uint32_t off = c * L::kRowChunk + half * L::kColChunk;
-                    const int l = min(row0 + half * kCols, rows_end);
-                    umma::tma_load_4d(sm + L::kR1 + off, r1, c * L::kVals, h * r1h, l, b * r1b, at(bar->r_full));
-                    umma::tma_load_4d(sm + L::kR2 + off, r2, c * L::kVals, h * r2h, l, b * r2b, at(bar->r_full));
-                }
+            if (!L::kRowsInTmem) {
+                // a half of the row tile that lies beyond the tensor reads as zeros like any other place outside
+                umma::mbar_arrive_expect_tx(at(bar->r_full), 2 * L::kRowBytes);
+                for (int half = 0; half < 2; ++half)
+                    for (int c = 0; c < L::kChunks; ++c) {
+                        const uint32_t off = c * L::kRowChunk + half * L::kColChunk;
+                        const int l = min(row0 + half * kCols, p.Lk);
+                        umma::tma_load_4d(sm + off, &p.k, c * L::kVals, h * p.k_h, l, b * p.k_b, at(bar->r_full));
+                        umma::tma_load_4d(sm + L::kRowBytes + off, &p.v, c * L::kVals, h * p.v_h, l, b * p.v_b,
+                                          at(bar->r_full));
+                    }
+            }
+            int ch = KEYS ? h * group + first / p.q_tiles : h / group, qt = KEYS ? first % p.q_tiles : first;
             bool ok = true;
-            for (int i = 0; i < n && ok; ++i) {
+            for (int i = 0; i < n; ++i) {
                 const int s = i % S;
                 ok = umma::mbar_poll(at(bar->c_empty[s]), (i / S + 1) & 1);
                 if (!ok) break;
-                int ch = h / group, l = (first + i) * kCols;
-                if (KEYS) {
-                    ch = h * group + (first + i) / p.q_tiles;
-                    l = (first + i) % p.q_tiles * kCols;
-                }
                 umma::mbar_arrive_expect_tx(at(bar->c_full[s]), 2 * L::kColBytes + (KEYS ? 2 * kCols * 4 : 0));
                 const uint32_t to = sm + L::kC + s * 2 * L::kColBytes;
+                const int l = qt * kCols;
+#pragma unroll
                 for (int c = 0; c < L::kChunks; ++c) {
                     umma::tma_load_4d(to + c * L::kColChunk, c1, c * L::kVals, ch * c1h, l, b * c1b, at(bar->c_full[s]));
                     umma::tma_load_4d(to + L::kColBytes + c * L::kColChunk, c2, c * L::kVals, ch * c2h, l, b * c2b,
@@ -210,42 +217,51 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                 if (KEYS) {
                     const int64_t row = (static_cast<int64_t>(b) * p.Hq + ch) * p.Lq_pad + l;
                     const uint32_t vec = sm + L::kVec + s * 2 * kCols * 4;
-                    umma::bulk_g2s(vec, p.lse2 + row, kCols * 4, at(bar->c_full[s]));
-                    umma::bulk_g2s(vec + kCols * 4, p.delta + row, kCols * 4, at(bar->c_full[s]));
+                    umma::bulk_g2s(vec, p.nlse2 + row, kCols * 4, at(bar->c_full[s]));
+                    umma::bulk_g2s(vec + kCols * 4, p.ndelta + row, kCols * 4, at(bar->c_full[s]));
+                }
+                ++qt;
+                if (KEYS && qt == p.q_tiles) {
+                    qt = 0;
+                    ++ch;
                 }
             }
             if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x30);
         }
-    } else if (warp == 8) {
+    } else if (warp == kMmaWarp) {
         if (n > 0) {
-            // one lane issues, the warp runs as a whole with everything in uniform registers
-            // (see attention_forward.cu)
-            const uint32_t tm = __reduce_or_sync(~0u, tmem);
-            const auto s_col = [&](int st) { return tm + st * kCols; };
-            const auto dp_col = [&](int st) { return tm + 2 * kCols + st * kCols; };
-            const uint32_t acc1 = tm + 4 * kCols, acc2 = acc1 + DP;
+            // the warp runs as a whole, one elected lane issues, everything in uniform
+            // registers (see attention_forward.cu)
             constexpr bool bf = !kHalf;
             constexpr uint32_t id_s = umma::idesc_16bit(bf, kRows, kCols, false), id_a = umma::idesc_16bit(bf, kRows, DP, true);
-            const uint64_t r_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kR1, 16);
+            const uint32_t tm = __reduce_or_sync(~0u, tmem);
+            const uint64_t r_desc = umma::smem_desc_swizzled<L::kRow>(sm, 16);
             const uint64_t c_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kC, 16);
             const uint64_t a_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kC, L::kColChunk);
             const auto scores = [&](int i) {
                 const uint64_t cd = umma::desc_advance(c_desc, i % S * 2 * L::kColBytes);
-                const uint32_t to = s_col(i & 1), to2 = dp_col(i & 1);
-                if (!umma::elect_one()) return;
+                const uint32_t to = tm + (i & 1) * kCols;
+                if (umma::elect_one()) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int j = 0; j < DP / 16; ++j)
-                        umma::mma_f16_ss(x ? to2 : to,
-                                         umma::desc_advance(r_desc, x * L::kRowBytes + j * 16 / L::kVals * L::kRowChunk +
-                                                                        j * 16 % L::kVals * 2),
-                                         umma::desc_advance(cd, x * L::kColBytes + j * 16 / L::kVals * L::kColChunk +
-                                                                    j * 16 % L::kVals * 2),
-                                         id_s, j > 0);
-                umma::mma_commit(at(bar->s_full[i & 1]));
+                        for (int j = 0; j < DP / 16; ++j) {
+                            const uint64_t bd = umma::desc_advance(cd, x * L::kColBytes + j * 16 / L::kVals * L::kColChunk +
+                                                                           j * 16 % L::kVals * 2);
+                            if (L::kRowsInTmem)
+                                umma::mma_f16_ts(to + x * L::kDp, tm + (x ? L::kR2 : L::kR1) + j * 8, bd, id_s, j > 0);
+                            else
+                                umma::mma_f16_ss(to + x * L::kDp,
+                                                 umma::desc_advance(r_desc, x * L::kRowBytes + j * 16 / L::kVals * L::kRowChunk +
+                                                                                j * 16 % L::kVals * 2),
+                                                 bd, id_s, j > 0);
+                        }
+                    umma::mma_commit(at(bar->s_full[i & 1]));
+                }
+                __syncwarp();
             };
             bool ok = umma::mbar_poll(at(bar->r_full), 0);
+            umma::fence_after_sync();
             for (int i = 0; i < 2 && i < n && ok; ++i) {
                 ok = umma::mbar_poll(at(bar->c_full[i]), 0);
                 if (ok) scores(i);
@@ -255,16 +271,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                 if (!ok) break;
                 umma::fence_after_sync();
                 const uint64_t ad = umma::desc_advance(a_desc, i % S * 2 * L::kColBytes);
-                const uint32_t from = s_col(i & 1), from2 = dp_col(i & 1);
+                const uint32_t from = tm + (i & 1) * kCols;
                 if (umma::elect_one()) {
 #pragma unroll
-                for (int j = 0; j < kCols / 16; ++j) {
-                    umma::mma_f16_ts(acc1, from2 + j * 8, umma::desc_advance(ad, j * 16 * L::kRow), id_a, i > 0 || j > 0);
-                    if (KEYS)
-                        umma::mma_f16_ts(acc2, from + j * 8, umma::desc_advance(ad, L::kColBytes + j * 16 * L::kRow), id_a,
+                    for (int j = 0; j < kCols / 16; ++j) {
+                        const uint32_t a = from + j / 2 * 32 + j % 2 * 8;  // each warpgroup's 32 values over its own 32 scores
+                        umma::mma_f16_ts(tm + L::kAcc1, a + L::kDp, umma::desc_advance(ad, j * 16 * L::kRow), id_a,
                                          i > 0 || j > 0);
-                }
-                umma::mma_commit(at(bar->c_empty[i % S]));
+                        if (KEYS)
+                            umma::mma_f16_ts(tm + L::kAcc2, a,
+                                             umma::desc_advance(ad, L::kColBytes + j * 16 * L::kRow), id_a, i > 0 || j > 0);
+                    }
+                    umma::mma_commit(at(bar->c_empty[i % S]));
+                    if (i == n - 1) umma::mma_commit(at(bar->done));
                 }
                 __syncwarp();
                 if (i + 2 < n) {
@@ -272,56 +291,80 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                     if (ok) scores(i + 2);
                 }
             }
-            if (ok && umma::elect_one()) umma::mma_commit(at(bar->done));
             if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x31);
         }
     } else {
-        const int wg = warp / 4, r = threadIdx.x % 128;
+        const int st = wg >> 1, half = wg & 1;  // tile of the pair, columns of it
+        const int r = threadIdx.x % 128, row = row0 + r;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
-        const int row = row0 + r;
+        const uint32_t s_col = tmem + lanes + st * kCols, dp_col = s_col + L::kDp;
         bool ok = true;  // once a wait has run out: no more waits, but every barrier is kept
+        if (L::kRowsInTmem && wg < 2 && n > 0) {
+            // warpgroup 0 brings the first row operand to TMEM, 1 the second: two values a column
+            const int64_t* stride = wg == 0 ? p.r1_strides : p.r2_strides;
+            const T* from = static_cast<const T*>(wg == 0 ? p.r1 : p.r2) + b * stride[0] + row * stride[1] + h * stride[2];
+            const bool live = row < (KEYS ? p.Lk : p.Lq);
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t x[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (live && c + j * 8 < p.D) u = __ldg(reinterpret_cast<const uint4*>(from + c + j * 8));
+                    x[4 * j] = u.x;
+                    x[4 * j + 1] = u.y;
+                    x[4 * j + 2] = u.z;
+                    x[4 * j + 3] = u.w;
+                }
+                umma::tmem_st16(tmem + lanes + (wg == 0 ? L::kR1 : L::kR2) + c / 2, x);
+            }
+            umma::tmem_wait_st();
+            umma::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(at(bar->r_full));
+        }
         // fp16: f = 2^e, e = 127 - the biased exponent of max |dO|
         float f = 1.0f;
         if (kHalf) {
-            const int top = static_cast<int>(__ldg(p.top) >> 23);  // biased exponent
+            const int top = static_cast<int>(__ldg(p.top) >> 23);
             if (top > 0 && top < 255) f = __int_as_float((254 - top) << 23);
         }
         bool row_ok = row < (KEYS ? len : p.Lq);
-        float my_lse = INFINITY, my_delta = 0.0f;
+        float my_nlse = -INFINITY, my_ndelta = 0.0f;
         if (KEYS) {
             if (row_ok && p.key_mask != nullptr) row_ok = __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + row) != 0;
         } else if (row_ok) {
             const int64_t i = (static_cast<int64_t>(b) * p.Hq + h) * p.Lq_pad + row;
-            my_lse = __ldg(p.lse2 + i);
-            my_delta = __ldg(p.delta + i) * f;
+            my_nlse = __ldg(p.nlse2 + i);
+            my_ndelta = __ldg(p.ndelta + i) * f;
         }
         const bool rows_ok = __all_sync(~0u, row_ok);
         const bool any_row = row0 + warp % 4 * 32 < (KEYS ? len : p.Lq);  // else this warp keeps the barriers only
+        const Pair scale_2 = pair(p.scale2, p.scale2), f_2 = pair(f, f), ndelta_2 = pair(my_ndelta, my_ndelta);
         int built = -1;  // KEYS: head of `values`
-        float* diag = values + entries + wg * entries;
-        float* plain = values + 3 * entries + warp * kMaxBuckets;
-        float* tile = values + 3 * entries + 8 * kMaxBuckets + wg * kRows * kPitch;
+        float* diag = values + (1 + wg) * entries;
+        float* plain = values + (1 + kGroups) * entries + warp * kMaxBuckets;
+        float* tile = values + (1 + kGroups) * entries + kGroups * 4 * kMaxBuckets + wg * kRows * kPitch;
         if (BIAS && !KEYS && !any_row)
             for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;
-        for (int i = wg; i < n; i += 2) {
-            const int col0 = KEYS ? (first + i) % p.q_tiles * kCols : (first + i) * kCols;
-            uint32_t keep[2] = {~0u, ~0u};
+        int ch = h, qt = first + st;  // tile i's head (KEYS) and its place along the streamed axis
+        if (KEYS) {
+            ch = h * group + (first + st) / p.q_tiles;
+            qt = (first + st) % p.q_tiles;
+        }
+        for (int i = st; i < n; i += 2) {
+            const int s = i % S, col0 = qt * kCols + half * 32;
+            uint32_t keep = ~0u;
             if (!KEYS) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int left = len - col0 - 32 * c;
-                    keep[c] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-                    if (p.key_mask != nullptr)
-                        keep[c] &= __ballot_sync(~0u, lane < left && __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk +
-                                                                          col0 + 32 * c + lane) != 0);
-                }
+                const int left = len - col0;
+                keep = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+                if (p.key_mask != nullptr)
+                    keep &= __ballot_sync(~0u, lane < left && __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + col0 + lane) != 0);
             }
-            const bool whole = (keep[0] & keep[1]) == ~0u;
             float flat = 0.0f;
-            const float* mine = nullptr;  // bias of column 0 of this row
+            const float* mine = nullptr;  // bias of this row's first column
             int flat_bucket = 0;
             if (BIAS) {
-                const int ch = KEYS ? h * group + (first + i) / p.q_tiles : h;
                 const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(ch) * p.rel.total;
                 if (KEYS && built != ch) {
                     warpgroup_sync(wg);
@@ -329,111 +372,89 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                     warpgroup_sync(wg);
                     built = ch;
                 }
-                // j - i - offset over the tile
-                const int lo = KEYS ? row0 - (col0 + kCols - 1) - p.rel.q_offset : col0 - (row0 + kRows - 1) - p.rel.q_offset;
-                const int hi = lo + kRows + kCols - 2;
+                // j - i - offset over these 128 x 32
+                const int lo = KEYS ? row0 - (col0 + 31) - p.rel.q_offset : col0 - (row0 + kRows - 1) - p.rel.q_offset;
                 flat_bucket = bucket_at(range, buckets, lo);
-                if (flat_bucket == bucket_at(range, buckets, hi))
-                    flat = bias_value<T>(table[flat_bucket]) * kLog2eF;
+                if (flat_bucket == bucket_at(range, buckets, lo + kRows + 30))
+                    flat = values[min(max(lo, range.lo), range.hi) - range.lo];
                 else
                     mine = values + (KEYS ? row - col0 : col0 - row) - p.rel.q_offset - range.lo;
             }
-            ok = ok && umma::mbar_poll(at(bar->s_full[wg]), (i >> 1) & 1);
+            if (KEYS) ok = ok && umma::mbar_poll(at(bar->c_full[s]), (i / S) & 1);
+            ok = ok && umma::mbar_poll(at(bar->s_full[st]), (i >> 1) & 1);
             umma::fence_after_sync();
-            const float* vec = reinterpret_cast<const float*>(base + L::kVec + (i % S) * 2 * kCols * 4);
-            if (KEYS) ok = ok && umma::mbar_poll(at(bar->c_full[i % S]), (i / S) & 1);
-            const float row_add = (BIAS ? flat : 0.0f) - (KEYS ? 0.0f : my_lse);
-            float total = 0.0f;
-            // sums of a half tile's dS along j - i: each thread a diagonal, column
-            // j of row (j + 127 - r) mod 128: diagonal r - 127 until column r, r + 1
-            // (r < 31) from there on
-            const auto diagonals = [&](int c) {
-                warpgroup_sync(wg);
-                float run = 0.0f, left = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    if (j == r + 1) {
-                        left = run;
-                        run = 0.0f;
-                    }
-                    run += tile[((j + 127 - r) & 127) * kPitch + j];
-                }
-                float* to = diag + col0 + 32 * c - row0 - p.rel.q_offset - range.lo;
-                to[r - 127] += r < 31 ? left : run;
-                if (r < 31) to[r + 1] += run;
-            };
+            const float4* nlse = reinterpret_cast<const float4*>(base + L::kVec + s * 2 * kCols * 4) + half * 8;
+            const float row_add = flat + (KEYS ? 0.0f : my_nlse);
+            Pair total = pair(0.0f, 0.0f);
+            const bool sums = BIAS && !KEYS;
+            if (sums && mine != nullptr) warpgroup_sync(wg);  // the diagonals before have been read
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t s[32], d[32];
-                if (!any_row) {
-                    if (!KEYS && BIAS) {
+                if (!any_row) continue;
+                uint32_t x[16], d[16];
+                umma::tmem_ld16(s_col + half * 32 + c * 16, x);
+                umma::tmem_ld16(dp_col + half * 32 + c * 16, d);
+                umma::tmem_wait_ld16(x);
+                umma::tmem_wait_ld16(d);
+                uint32_t pk[8], dk[8];
+                const Pair add_2 = pair(row_add, row_add);
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    Pair arg = fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, add_2);
+                    Pair nd = ndelta_2;
+                    if (KEYS) {
+                        const float4 a = nlse[c * 4 + j / 4], e = nlse[kCols / 4 + c * 4 + j / 4];
+                        arg = add2(arg, j % 4 == 0 ? pair(a.x, a.y) : pair(a.z, a.w));
+                        nd = j % 4 == 0 ? pair(e.x, e.y) : pair(e.z, e.w);
+                    }
+                    if (BIAS) {
                         if (mine != nullptr) {
-                            warpgroup_sync(wg);
-                            diagonals(c);
+                            const int at0 = c * 16 + j;
+                            arg = add2(arg, KEYS ? pair(mine[-at0], mine[-at0 - 1]) : pair(mine[at0], mine[at0 + 1]));
                         }
                     }
-                    continue;
-                }
-                umma::tmem_ld32(s_col(wg) + lanes + c * 32, s);
-                umma::tmem_ld32(dp_col(wg) + lanes + c * 32, d);
-                umma::tmem_wait_ld32(s);
-                umma::tmem_wait_ld32(d);
-                uint32_t pk[16], dk[16];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float add = row_add;
-                    if (KEYS) add -= vec[32 * c + j];
-                    if (BIAS) {
-                        if (mine != nullptr) add += KEYS ? mine[-(32 * c + j)] : mine[32 * c + j];
-                    }
-                    float pr = exp2_approx(fmaf(f32(s[j]), p.scale2, add));
-                    float ds;
-                    if (KEYS) {
-                        const float del = vec[kCols + 32 * c + j];
-                        ds = kHalf ? pr * ((f32(d[j]) - del) * f) : pr * (f32(d[j]) - del);
+                    float p0, p1;
+                    if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe, where no argument is -inf
+                        unpair(exp2_poly(arg), p0, p1);
                     } else {
-                        ds = kHalf ? pr * fmaf(f32(d[j]), f, -my_delta) : pr * (f32(d[j]) - my_delta);
+                        unpair(arg, p0, p1);
+                        p0 = exp2_approx(p0);
+                        p1 = exp2_approx(p1);
                     }
-                    s[j] = __float_as_uint(pr);
-                    d[j] = __float_as_uint(ds);
-                }
-                if (KEYS ? !rows_ok : !whole) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const bool in = KEYS ? row_ok : ((keep[c] >> j) & 1);
-                        s[j] = in ? s[j] : 0u;
-                        d[j] = in ? d[j] : 0u;
+                    const Pair dp = pair(f32(d[j]), f32(d[j + 1]));
+                    Pair ds;
+                    if (!kHalf) ds = mul2(pair(p0, p1), add2(dp, nd));
+                    else if (KEYS) ds = mul2(pair(p0, p1), mul2(add2(dp, nd), f_2));
+                    else ds = mul2(pair(p0, p1), fma2(dp, f_2, nd));
+                    float d0, d1;
+                    unpair(ds, d0, d1);
+                    if (KEYS ? !rows_ok : keep != ~0u) {
+                        const bool in0 = KEYS ? row_ok : (keep >> (c * 16 + j)) & 1, in1 = KEYS ? row_ok : (keep >> (c * 16 + j + 1)) & 1;
+                        p0 = in0 ? p0 : 0.0f;
+                        p1 = in1 ? p1 : 0.0f;
+                        d0 = in0 ? d0 : 0.0f;
+                        d1 = in1 ? d1 : 0.0f;
                     }
-                }
-                if (!KEYS && BIAS) {
-                    if (mine == nullptr) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) total += f32(d[j]);
-                    } else {
-                        float* to = tile + r * kPitch;
-                        warpgroup_sync(wg);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) to[j] = f32(d[j]);
-                        diagonals(c);
+                    if (sums) {
+                        if (mine == nullptr) {
+                            total = add2(total, pair(d0, d1));
+                        } else {
+                            tile[r * kPitch + c * 16 + j] = d0;
+                            tile[r * kPitch + c * 16 + j + 1] = d1;
+                        }
                     }
+                    if (KEYS) pk[j / 2] = pack2<T>(p0, p1);
+                    dk[j / 2] = pack2<T>(d0, d1);
                 }
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if (KEYS) pk[j] = pack2<T>(f32(s[2 * j]), f32(s[2 * j + 1]));
-                    dk[j] = pack2<T>(f32(d[2 * j]), f32(d[2 * j + 1]));
-                }
-                if (KEYS) umma::tmem_st16(s_col(wg) + lanes + c * 16, pk);
-                umma::tmem_st16(dp_col(wg) + lanes + c * 16, dk);
+                // over columns of this half of the tile only: the other half may not have been read
+                if (KEYS) umma::tmem_st8(s_col + half * 32 + c * 8, pk);
+                umma::tmem_st8(dp_col + half * 32 + c * 8, dk);
             }
-            if (!KEYS && BIAS && mine == nullptr) {
-                for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-                if (lane == 0) plain[flat_bucket] += total;
-            }
-            if (!KEYS && !whole) {
+            if (!KEYS && keep != ~0u) {
                 // rows of K behind masked keys: 0 in place of whatever they hold
-                ok = ok && umma::mbar_poll(at(bar->c_full[i % S]), (i / S) & 1);
-                if (r < kCols && !((keep[(r >> 5) & 1] >> lane) & 1)) {
-                    const uint32_t to = sm + L::kC + (i % S) * 2 * L::kColBytes + r * L::kRow;
+                ok = ok && umma::mbar_poll(at(bar->c_full[s]), (i / S) & 1);
+                if (r < 32 && !((keep >> lane) & 1)) {
+                    const uint32_t to = sm + L::kC + s * 2 * L::kColBytes + (half * 32 + r) * L::kRow;
                     for (int c = 0; c < L::kChunks; ++c)
 #pragma unroll
                         for (int j = 0; j < L::kRow; j += 16) umma::st_shared_v4(to + c * L::kColChunk + j, 0, 0, 0, 0);
@@ -443,92 +464,116 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             umma::tmem_wait_st();
             umma::fence_before_sync();
             __syncwarp();
-            if (lane == 0) umma::mbar_arrive(at(bar->p_ready[wg]));
+            if (lane == 0) umma::mbar_arrive(at(bar->p_ready[st]));
+            if (sums) {
+                if (mine == nullptr) {
+                    float t0, t1;
+                    unpair(total, t0, t1);
+                    t0 += t1;
+                    for (int o = 16; o > 0; o >>= 1) t0 += __shfl_xor_sync(~0u, t0, o);
+                    if (lane == 0) plain[flat_bucket] += t0;
+                } else {
+                    // sums along j - i: each thread a diagonal, column j of row
+                    // (j + 127 - r) mod 128: diagonal r - 127 until column r, r + 1
+                    // (r < 31) from there on
+                    warpgroup_sync(wg);
+                    float run = 0.0f, first_part = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (j == r + 1) {
+                            first_part = run;
+                            run = 0.0f;
+                        }
+                        run += tile[((j + 127 - r) & 127) * kPitch + j];
+                    }
+                    float* to = diag + col0 - row0 - p.rel.q_offset - range.lo;
+                    to[r - 127] += r < 31 ? first_part : run;
+                    if (r < 31) to[r + 1] += run;
+                }
+            }
+            qt += 2;
+            if (KEYS)
+                while (qt >= p.q_tiles) {
+                    qt -= p.q_tiles;
+                    ++ch;
+                }
         }
         if (n > 0) ok = ok && umma::mbar_poll(at(bar->done), 0);
         umma::fence_after_sync();
         if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x32);
-        // keys: warpgroup 0 writes dk, 1 dv; queries: each half of dq
-        const int L_ = KEYS ? p.Lk : p.Lq;
-        const int64_t at_row = ((static_cast<int64_t>(b) * L_ + row) * heads + h) * p.D;
-        const int64_t size = static_cast<int64_t>(p.B) * L_ * heads * p.D;
-        const bool second = KEYS && wg == 1;
+        // keys: warpgroups 0, 1 write the halves of dk, 2, 3 of dv; queries: each a quarter of dq
+        const int rows_of = KEYS ? p.Lk : p.Lq;
+        const bool second = KEYS && wg >= 2;
         const float mul = second ? 1.0f / (1 << kShift) : p.scale / (1 << kShift) / f;
-        const uint32_t acc = second ? acc2 : acc1;
-        constexpr int kSpan = KEYS ? DP : DP / 2;
-        const int begin = KEYS ? 0 : wg * kSpan;
+        constexpr int kSpan = KEYS ? DP / 2 : DP / 4;
+        const int begin = (KEYS ? half : wg) * kSpan;
+        const uint32_t acc = tmem + lanes + (second ? L::kAcc2 : L::kAcc1) + begin;
+        T* to = static_cast<T*>(second ? p.d2 : p.d1) + ((static_cast<int64_t>(b) * rows_of + row) * heads + h) * p.D;
+        float* part = p.part + (((static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (KEYS ? 2 : 1) + second) * kRows + r) * p.D;
 #pragma unroll
-        for (int c = 0; c < kSpan; c += 16) {
-            uint32_t o[16];
+        for (int c = 0; c < kSpan; c += 8) {
+            uint32_t o[8];
             const int d0 = begin + c;
             if (n > 0) {
-                umma::tmem_ld16(acc + lanes + d0, o);
-                umma::tmem_wait_ld16(o);
+                umma::tmem_ld8(acc + c, o);
+                umma::tmem_wait_ld8(o);
             } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = 0;
+                for (int j = 0; j < 8; ++j) o[j] = 0;
             }
-            if (row >= L_) continue;
+            if (row >= rows_of || d0 >= p.D) continue;
             if (KEYS && !row_ok) {  // a masked key: 0, whatever a skipped warp left in its lanes
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = 0;
+                for (int j = 0; j < 8; ++j) o[j] = 0;
             }
-            if (p.splits > 1) {
-                float* to = p.part + (static_cast<int64_t>(split) * (KEYS ? 2 : 1) + second) * size + at_row + d0;
-#pragma unroll
-                for (int j = 0; j < 16; j += 4)
-                    if (d0 + j < p.D)
-                        *reinterpret_cast<float4*>(to + j) =
-                            make_float4(f32(o[j]) * mul, f32(o[j + 1]) * mul, f32(o[j + 2]) * mul, f32(o[j + 3]) * mul);
+            if (in_parts) {
+                *reinterpret_cast<float4*>(part + d0) =
+                    make_float4(f32(o[0]) * mul, f32(o[1]) * mul, f32(o[2]) * mul, f32(o[3]) * mul);
+                *reinterpret_cast<float4*>(part + d0 + 4) =
+                    make_float4(f32(o[4]) * mul, f32(o[5]) * mul, f32(o[6]) * mul, f32(o[7]) * mul);
             } else {
-                T* to = static_cast<T*>(second ? p.d2 : p.d1) + at_row + d0;
-#pragma unroll
-                for (int j = 0; j < 16; j += 8)
-                    if (d0 + j < p.D)
-                        *reinterpret_cast<uint4*>(to + j) = make_uint4(
-                            pack2<T>(f32(o[j]) * mul, f32(o[j + 1]) * mul), pack2<T>(f32(o[j + 2]) * mul, f32(o[j + 3]) * mul),
-                            pack2<T>(f32(o[j + 4]) * mul, f32(o[j + 5]) * mul),
-                            pack2<T>(f32(o[j + 6]) * mul, f32(o[j + 7]) * mul));
+                *reinterpret_cast<uint4*>(to + d0) =
+                    make_uint4(pack2<T>(f32(o[0]) * mul, f32(o[1]) * mul), pack2<T>(f32(o[2]) * mul, f32(o[3]) * mul),
+                               pack2<T>(f32(o[4]) * mul, f32(o[5]) * mul), pack2<T>(f32(o[6]) * mul, f32(o[7]) * mul));
             }
         }
         umma::fence_before_sync();
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         umma::fence_after_sync();
         umma::tmem_dealloc(tmem, 512);
     }
     if (BIAS && !KEYS) {
-        // buckets of this CTA: each warp every 8th bucket, its lanes over the entries
+        // buckets of this CTA: each warp every 18th bucket, its lanes over the entries
         const float* diag = values + entries;
-        const float* plain = values + 3 * entries;
+        const float* plain = values + (1 + kGroups) * entries;
         float f = 1.0f;
         if (kHalf) {
             const int top = static_cast<int>(__ldg(p.top) >> 23);
             if (top > 0 && top < 255) f = __int_as_float((254 - top) << 23);
         }
-        float* to = p.table_part + static_cast<int64_t>(blockIdx.x) * p.rel.total;
+        float* to = p.table_part + static_cast<int64_t>(blk) * p.rel.total;
         for (int t = warp; t < p.rel.total; t += kThreads / 32) {
             float sum = 0.0f;
             if (n > 0)
                 for (int e = lane; e < range.count(); e += 32)
-                    if (buckets[e] == t) sum += diag[e] + diag[entries + e];
+                    if (buckets[e] == t)
+                        for (int w = 0; w < kGroups; ++w) sum += diag[w * entries + e];
+            if (lane < kGroups * 4) sum += plain[lane * kMaxBuckets + t];
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            if (lane == 0) {
-                for (int w = 0; w < 8; ++w) sum += plain[w * kMaxBuckets + t];
-                to[t] = sum / (1 << kShift) / f;
-            }
+            if (lane == 0) to[t] = sum / (1 << kShift) / f;
         }
     }
 }
 
-// delta = rowsum(dO * O) and lse in log2 units, both laid out [B * Hq][Lq_pad]
-// with rows of no gradient (lse -inf, padding) at lse2 = +inf; for fp16 also
+// -delta = -rowsum(dO * O) and kShift - lse in log2 units, both laid out
+// [B * Hq][Lq_pad] with rows of no gradient (lse -inf, padding) at nlse2 = -inf; for fp16 also
 // max |dO| (an integer maximum of non-negative floats: no order).  kLanes >= D / 8
 // lanes per row, 8 values each.
 template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ ww_attention_t a, float* lse2,
-                                                              float* delta, uint32_t* top, int Lq_pad)
+__global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ ww_attention_t a, float* nlse2,
+                                                              float* ndelta, uint32_t* top, int Lq_pad)
 {
     const int64_t item = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
     const int lane = threadIdx.x % kLanes;
@@ -556,8 +601,8 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
     if (item < rows && lane == 0) {
         const int64_t to = (static_cast<int64_t>(b) * a.Hq + h) * Lq_pad + i;
         const float l = live ? a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Lq + i] : -INFINITY;
-        lse2[to] = l == -INFINITY ? INFINITY : l * kLog2eF - kShift;
-        delta[to] = sum;
+        nlse2[to] = l == -INFINITY ? -INFINITY : kShift - l * kLog2eF;
+        ndelta[to] = -sum;
     }
     if (std::is_same<T, __half>::value) {
         __shared__ uint32_t block_top;
@@ -570,36 +615,63 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
     }
 }
 
-// Sums of the splits in order; 4 values per thread.
+// Joins the parts of the split items in order: kSumRows rows of an item and
+// output per CTA, 4 values per thread and step.
+constexpr int kSumRows = 8;
 template <typename T>
-__global__ void __launch_bounds__(256) attention_sum_kernel(const float* part, int splits, int64_t stride, T* out, int64_t n)
+__global__ void __launch_bounds__(256) attention_sum_kernel(const float* part, int whole_items, int splits, int outputs,
+                                                            T* d1, T* d2, int blocks, int heads, int L, int D)
 {
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
-    float4 s = make_float4(0, 0, 0, 0);
-    for (int k = 0; k < splits; ++k) {
-        const float4 v = *reinterpret_cast<const float4*>(part + k * stride + i);
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+    const int k = blockIdx.x / outputs, which = blockIdx.x % outputs, item = whole_items + k;
+    const int row0 = item % blocks * kRows, h = item / blocks % heads;
+    const int64_t b = item / blocks / heads;
+    T* out = which == 0 ? d1 : d2;
+    const int begin = blockIdx.y * kSumRows * D;
+    for (int e = begin + threadIdx.x * 4; e < begin + kSumRows * D; e += 256 * 4) {
+        const int r = e / D, d = e - r * D;
+        if (row0 + r >= L) break;
+        float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+        for (int n = 0; n < splits; ++n) {
+            const float4 v = *reinterpret_cast<const float4*>(
+                part + ((static_cast<int64_t>(k) * splits + n) * outputs + which) * kRows * D + e);
+            s.x += v.x;
+            s.y += v.y;
+            s.z += v.z;
+            s.w += v.w;
+        }
+        *reinterpret_cast<uint2*>(out + ((b * L + row0 + r) * heads + h) * D + d) =
+            make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
     }
-    *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
 }
 
-// Table gradient of one head: the CTAs' buckets in order.  Each of 32 warps takes
-// every 32nd CTA (four loads in flight), 32 buckets at a time, then the warps'
-// sums in order.
+// Table gradient of one head: the CTAs' buckets in order.  Items are numbered
+// (batch item, head, block); those from whole_items on have `splits` CTAs each.
+// Each of 32 warps takes every 32nd item of the head (item numbers grow with n),
+// 32 buckets at a time, then the warps' sums in order.
 template <typename T>
-__global__ void __launch_bounds__(1024) attention_table_kernel(const float* part, T* out, int B, int Hq, int per_head, int total)
+__global__ void __launch_bounds__(1024) attention_table_kernel(const float* part, T* out, int B, int Hq, int blocks,
+                                                               int whole_items, int splits, int total)
 {
     __shared__ float sums[32][33];
     const int h = blockIdx.x, t = blockIdx.y * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
     float s = 0.0f;
     if (t < total) {
-#pragma unroll 4
-        for (int n = w; n < B * per_head; n += 32)
-            s += part[((static_cast<int64_t>(n / per_head) * Hq + h) * per_head + n % per_head) * total + t];
+        const auto item_of = [&](int n) { return (static_cast<int64_t>(n / blocks) * Hq + h) * blocks + n % blocks; };
+        int n = w;
+        for (; n + 7 * 32 < B * blocks && item_of(n + 7 * 32) < whole_items; n += 8 * 32) {  // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = part[item_of(n + k * 32) * total + t];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
+        for (; n < B * blocks; n += 32) {
+            const int64_t item = item_of(n);
+            const bool one = item < whole_items;
+            const int64_t at = one ? item : whole_items + (item - whole_items) * splits;
+            for (int k = 0; k < (one ? 1 : splits); ++k) s += part[(at + k) * total + t];
+        }
     }
     sums[w][threadIdx.x % 32] = s;
     __syncthreads();
@@ -610,36 +682,48 @@ __global__ void __launch_bounds__(1024) attention_table_kernel(const float* part
     }
 }
 
-// How a call runs and where its workspace is.
-struct Plan {
-    int q_blocks, k_blocks, q_splits, k_splits, Lq_pad;
-    int64_t lse2, delta, part, table, bytes;  // byte offsets; the maximum of |dO| stands first
+// How one of the two kernels runs: one CTA per SM, and the items that do not
+// fill a round of all SMs are split over their streamed tiles.
+struct Half {
+    int blocks, whole, rest, splits;
+    int64_t ctas() const { return i64(whole) + i64(rest) * splits; }
 };
 
-int splits_for(int64_t ctas, int64_t tiles, int sms)
+Half make_half(int blocks, int64_t items, int64_t tiles, int sms) noexcept
 {
-    if (ctas <= 0 || ctas >= sms || tiles < 8) return 1;
-    return static_cast<int>(std::min<int64_t>({sms / ctas, tiles / 4, 64}));
+    Half r;
+    r.blocks = blocks;
+    r.rest = static_cast<int>(items % sms);
+    r.splits = r.rest == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms / r.rest, tiles / 4, 64})));
+    if (r.splits == 1) r.rest = 0;
+    r.whole = static_cast<int>(items - r.rest);
+    return r;
 }
 
-Plan make_plan(const ww_attention_t& p, int sms) noexcept
+// Both, and where the workspace's parts are.
+struct Plan {
+    Half q, k;
+    int Lq_pad;
+    int64_t nlse2, ndelta, part, table, bytes;  // byte offsets; the maximum of |dO| stands first
+};
+
+bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
 {
-    Plan r;
-    r.q_blocks = (p.Lq + kRows - 1) / kRows;
-    r.k_blocks = (p.Lk + kRows - 1) / kRows;
+    Plan& r = *plan;
+    const int q_blocks = (p.Lq + kRows - 1) / kRows, k_blocks = (p.Lk + kRows - 1) / kRows;
     r.Lq_pad = (p.Lq + kCols - 1) / kCols * kCols;
-    const int64_t q_ctas = i64(r.q_blocks) * p.B * p.Hq, k_ctas = i64(r.k_blocks) * p.B * p.Hk;
-    r.q_splits = splits_for(q_ctas, (p.Lk + kCols - 1) / kCols, sms);
-    r.k_splits = splits_for(k_ctas, i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), sms);
+    const int64_t q_items = i64(q_blocks) * p.B * p.Hq, k_items = i64(k_blocks) * p.B * p.Hk;
+    if (q_items > (1 << 30) || k_items > (1 << 30)) return false;
+    r.q = make_half(q_blocks, q_items, (p.Lk + kCols - 1) / kCols, sms);
+    r.k = make_half(k_blocks, k_items, i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), sms);
     const int64_t rows = i64(p.B) * p.Hq * r.Lq_pad;
-    const int64_t q_part = r.q_splits > 1 ? r.q_splits * i64(p.B) * p.Lq * p.Hq * p.D * 4 : 0;
-    const int64_t k_part = r.k_splits > 1 ? 2 * r.k_splits * i64(p.B) * p.Lk * p.Hk * p.D * 4 : 0;
-    r.lse2 = 256;
-    r.delta = r.lse2 + rows * 4;
-    r.part = r.delta + rows * 4;  // one after the other: both kernels use the same place
+    const int64_t q_part = i64(r.q.rest) * r.q.splits * kRows * p.D * 4, k_part = i64(r.k.rest) * r.k.splits * 2 * kRows * p.D * 4;
+    r.nlse2 = 256;
+    r.ndelta = r.nlse2 + rows * 4;
+    r.part = r.ndelta + rows * 4;  // one after the other: both kernels use the same place
     r.table = r.part + std::max(q_part, k_part);
-    r.bytes = r.table + (p.bias_table != nullptr ? q_ctas * r.q_splits * p.num_buckets * 4 : 0);
-    return r;
+    r.bytes = r.table + (p.bias_table != nullptr ? r.q.ctas() * p.num_buckets * 4 : 0);
+    return true;
 }
 
 template <typename T, int DP, bool KEYS, bool BIAS>
@@ -658,7 +742,6 @@ template <typename T, bool KEYS>
 int launch(const BwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     if (ctas == 0) return WW_SUCCESS;
-    if (ctas > 0x7fffffff) return WW_ERR_UNSUPPORTED;
     const int dp = f.D <= 32 ? 32 : f.D <= 64 ? 64 : 128;
     if (f.table != nullptr)
         return dp == 32 ? launch_one<T, 32, KEYS, true>(f, ctas, stream)
@@ -667,11 +750,18 @@ int launch(const BwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
          : dp == 64 ? launch_one<T, 64, KEYS, false>(f, ctas, stream) : launch_one<T, 128, KEYS, false>(f, ctas, stream);
 }
 
-template <typename T>
-int sum_parts(const float* part, int splits, int64_t stride, void* out, int64_t n, cudaStream_t stream) noexcept
+template <typename T, bool KEYS>
+int run_half(BwdParams& f, const Half& half, cudaStream_t stream) noexcept
 {
-    attention_sum_kernel<T><<<static_cast<unsigned>((n / 4 + 255) / 256), 256, 0, stream>>>(part, splits, stride,
-                                                                                           static_cast<T*>(out), n);
+    f.blocks = half.blocks;
+    f.whole_items = half.whole;
+    f.splits = half.splits;
+    const int st = launch<T, KEYS>(f, half.ctas(), stream);
+    if (st != WW_SUCCESS || half.rest == 0) return st;
+    constexpr int outputs = KEYS ? 2 : 1;
+    attention_sum_kernel<T><<<dim3(half.rest * outputs, kRows / kSumRows), 256, 0, stream>>>(f.part, half.whole, half.splits, outputs,
+                                                                     static_cast<T*>(f.d1), static_cast<T*>(f.d2), half.blocks,
+                                                                     KEYS ? f.Hk : f.Hq, KEYS ? f.Lk : f.Lq, f.D);
     return launch_status("cross_attention_backward");
 }
 
@@ -694,8 +784,8 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     f.key_mask = p.key_mask;
     f.table = p.bias_table;
     f.top = reinterpret_cast<uint32_t*>(ws);
-    f.lse2 = reinterpret_cast<float*>(ws + plan.lse2);
-    f.delta = reinterpret_cast<float*>(ws + plan.delta);
+    f.nlse2 = reinterpret_cast<float*>(ws + plan.nlse2);
+    f.ndelta = reinterpret_cast<float*>(ws + plan.ndelta);
     f.part = reinterpret_cast<float*>(ws + plan.part);
     f.table_part = reinterpret_cast<float*>(ws + plan.table);
     if (p.bias_table != nullptr)
@@ -730,7 +820,7 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
         if (blocks > 0x7fffffff) return WW_ERR_UNSUPPORTED;
         const auto kernel = per == 64 ? attention_delta_kernel<T, 4> : per == 32 ? attention_delta_kernel<T, 8>
                                                                                  : attention_delta_kernel<T, 16>;
-        kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, const_cast<float*>(f.lse2), const_cast<float*>(f.delta),
+        kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, const_cast<float*>(f.nlse2), const_cast<float*>(f.ndelta),
                                                                   reinterpret_cast<uint32_t*>(ws), plan.Lq_pad);
         st = launch_status("cross_attention_backward");
     }
@@ -738,26 +828,27 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     if (st == WW_SUCCESS && has_k) {
         f.d1 = p.dk;
         f.d2 = p.dv;
-        f.blocks = plan.k_blocks;
-        f.splits = plan.k_splits;
+        f.r1 = p.k;
+        f.r2 = p.v;
+        std::copy(p.k_strides, p.k_strides + 3, f.r1_strides);
+        std::copy(p.v_strides, p.v_strides + 3, f.r2_strides);
         f.max_entries = std::min(far, plan.Lq_pad + kRows);
-        st = launch<T, true>(f, i64(plan.k_blocks) * p.B * p.Hk * plan.k_splits, stream);
-        const int64_t n = i64(p.B) * p.Lk * p.Hk * p.D;
-        if (st == WW_SUCCESS && plan.k_splits > 1) st = sum_parts<T>(f.part, plan.k_splits, 2 * n, p.dk, n, stream);
-        if (st == WW_SUCCESS && plan.k_splits > 1) st = sum_parts<T>(f.part + n, plan.k_splits, 2 * n, p.dv, n, stream);
+        st = run_half<T, true>(f, plan.k, stream);
     }
     if (st == WW_SUCCESS && has_q) {
         f.d1 = p.dq;
-        f.blocks = plan.q_blocks;
-        f.splits = plan.q_splits;
+        f.d2 = nullptr;
+        f.r1 = p.q;
+        f.r2 = p.dout;
+        std::copy(p.q_strides, p.q_strides + 3, f.r1_strides);
+        std::copy(p.dout_strides, p.dout_strides + 3, f.r2_strides);
         f.max_entries = std::min(far, (p.Lk + kCols - 1) / kCols * kCols + kRows);
-        st = launch<T, false>(f, i64(plan.q_blocks) * p.B * p.Hq * plan.q_splits, stream);
-        const int64_t n = i64(p.B) * p.Lq * p.Hq * p.D;
-        if (st == WW_SUCCESS && plan.q_splits > 1) st = sum_parts<T>(f.part, plan.q_splits, n, p.dq, n, stream);
+        st = run_half<T, false>(f, plan.q, stream);
     }
     if (st == WW_SUCCESS && p.bias_table != nullptr) {
         attention_table_kernel<T><<<dim3(p.Hq, (p.num_buckets + 31) / 32), 1024, 0, stream>>>(
-            f.table_part, static_cast<T*>(p.dbias_table), has_q ? p.B : 0, p.Hq, plan.q_blocks * plan.q_splits, p.num_buckets);
+            f.table_part, static_cast<T*>(p.dbias_table), has_q ? p.B : 0, p.Hq, plan.q.blocks, plan.q.whole, plan.q.splits,
+            p.num_buckets);
         st = launch_status("cross_attention_backward");
     }
     return st;
@@ -776,19 +867,21 @@ extern "C" {
 
 int64_t ww_cross_attention_backward_workspace(const ww_attention_t* p)
 {
-    if (p == nullptr || ww::check_attention(*p) != WW_SUCCESS) return 0;
-    return ww::make_plan(*p, ww::sm_count()).bytes;
+    ww::Plan plan;
+    if (p == nullptr || ww::check_attention(*p) != WW_SUCCESS || !ww::make_plan(*p, ww::sm_count(), &plan)) return 0;
+    return plan.bytes;
 }
 
 int ww_cross_attention_backward(const ww_attention_t* p, void* stream)
 {
     if (p == nullptr) return WW_ERR_NULL_POINTER;
+    ww::Plan plan;
     int st = ww::check_attention(*p);
-    if (st == WW_SUCCESS) st = ww::check_attention_backward(*p, ww::make_plan(*p, ww::sm_count()).bytes);
+    if (st == WW_SUCCESS && !ww::make_plan(*p, ww::sm_count(), &plan)) st = WW_ERR_UNSUPPORTED;
+    if (st == WW_SUCCESS) st = ww::check_attention_backward(*p, plan.bytes);
     if (st != WW_SUCCESS) return st;
     ww::DeviceInfo d;
     if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
-    const ww::Plan plan = ww::make_plan(*p, d.sm_count);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return p->dtype == WW_DTYPE_HALF ? ww::backward<__half>(*p, plan, s) : ww::backward<__nv_bfloat16>(*p, plan, s);
 }

@@ -63,11 +63,11 @@ struct FwdParams {
     const int32_t* k_lens;
     const uint8_t* key_mask;
     const void* table;
-    float* part_o;    // [splits][B * Lq * Hq][D], splits > 1
-    float* part_lse;  // [splits][B * Lq * Hq], log2
+    float* part_o;    // split items: [item][split][NT * 128][D], normalised
+    float* part_lse;  // [item][split][NT * 128], log2
     RelBuckets rel;
     int32_t B, Lq, Lk, Hq, group, D;
-    int32_t q_blocks, splits;
+    int32_t q_blocks, whole_items, splits;
     int32_t q_b, q_h, k_b, k_h, v_b, v_h;  // 0 where the tensor is broadcast
     int32_t max_entries;                   // relative positions a CTA keeps
     float scale2;                          // scale * log2(e)
@@ -170,17 +170,18 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     Bar* bar = reinterpret_cast<Bar*>(base + L::kBar);
     const auto at = [](const uint64_t& b) { return umma::smem_addr(&b); };
 
-    const int split = blockIdx.x % p.splits;
-    int rest = blockIdx.x / p.splits;
-    const int qb = rest % p.q_blocks;
-    rest /= p.q_blocks;
-    const int h = rest % p.Hq, b = rest / p.Hq, g = h / p.group;
+    // items (query block, head, batch item); the last ones are split over their keys
+    const int blk = blockIdx.x;
+    const bool in_parts = blk >= p.whole_items;
+    const int split = in_parts ? (blk - p.whole_items) % p.splits : 0, splits = in_parts ? p.splits : 1;
+    const int item = in_parts ? p.whole_items + (blk - p.whole_items) / p.splits : blk;
+    const int qb = item % p.q_blocks, h = item / p.q_blocks % p.Hq, b = item / p.q_blocks / p.Hq, g = h / p.group;
     const int q0 = qb * (NT * kTile);
     const int tiles = NT == 1 || q0 + kTile >= p.Lq ? 1 : 2;  // query tiles with rows
     const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
     const int n_all = (len + KT - 1) / KT;
-    const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / p.splits);
-    const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / p.splits) - first;
+    const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / splits);
+    const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / splits) - first;
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // warp-uniform: roles branch as warps
     // keys of a tile
     const auto cols_of = [&](int kt) { return min(KT, len - (first + kt) * KT); };
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         const float sum = l_even + l_odd;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
-        const int64_t rows = static_cast<int64_t>(p.B) * p.Lq * p.Hq;
+        const int64_t part = (static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (NT * kTile) + t * kTile + r;
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
@@ -451,8 +452,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 for (int j = 0; j < 32; ++j) o[j] = 0;
             }
             if (i >= p.Lq) continue;
-            if (p.splits > 1) {
-                float* to = p.part_o + (split * rows + row) * p.D + c;
+            if (in_parts) {
+                float* to = p.part_o + part * p.D + c;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4)
                     if (c + j < p.D)
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         }
         if (i < p.Lq) {
             const float lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
-            if (p.splits > 1) p.part_lse[split * rows + row] = lse2;
+            if (in_parts) p.part_lse[part] = lse2;
             else if (p.lse != nullptr) p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Lq + i] = lse2 * kLn2F;
         }
         umma::fence_before_sync();
@@ -483,26 +484,43 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     }
 }
 
-// Joins the splits of a row: out = sum_s 2^(lse_s - top) out_s / sum_s 2^(lse_s - top).
-// One warp per row, 4 values per lane.
+// Joins the parts of a row: out = sum_s 2^(lse_s - top) out_s / sum_s 2^(lse_s - top),
+// in order.  One warp per row, 4 values per lane; items as numbered by the kernel
+// that wrote the parts: (query block, head, batch item) with `rows` query rows, or
+// for the token form (key head, batch item) with rows (shared head, token).
 template <typename T>
 __global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o, const float* part_lse, void* out,
-                                                             float* lse, int splits, int64_t rows, int Lq, int Hq, int D)
+                                                             float* lse, int whole_items, int splits, int rows, int q_blocks,
+                                                             int Lq, int Hq, int Hk, int D)
 {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32;
-    if (row >= rows) return;
+    const int k = blockIdx.x, r = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int item = whole_items + k;
+    int64_t b;
+    int h, i;
+    if (q_blocks == 0) {
+        b = item / Hk;
+        h = item % Hk * (Hq / Hk) + r / Lq;
+        i = r % Lq;
+    } else {
+        b = item / q_blocks / Hq;
+        h = item / q_blocks % Hq;
+        i = item % q_blocks * rows + r;
+    }
+    if (r >= rows || i >= Lq) return;
+    const int64_t first = static_cast<int64_t>(k) * splits * rows + r;  // + s * rows
     float top = -INFINITY;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + row]);
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[first + static_cast<int64_t>(s) * rows]);
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-        const float w = exp2_approx(part_lse[s * rows + row] - base);
+        const int64_t at = first + static_cast<int64_t>(s) * rows;
+        const float w = exp2_approx(part_lse[at] - base);
         sum += w;
-        if (w != 0.0f && lane * 4 < D) {
-            const float4 v = *reinterpret_cast<const float4*>(part_o + (s * rows + row) * D + lane * 4);
+        if (lane * 4 < D) {  // a part without keys is written as zeros
+            const float4 v = *reinterpret_cast<const float4*>(part_o + at * D + lane * 4);
             acc.x += w * v.x;
             acc.y += w * v.y;
             acc.z += w * v.z;
@@ -511,38 +529,46 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (lane * 4 < D)
-        *reinterpret_cast<uint2*>(static_cast<T*>(out) + row * D + lane * 4) =
+        *reinterpret_cast<uint2*>(static_cast<T*>(out) + ((b * Lq + i) * Hq + h) * D + lane * 4) =
             make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-    if (lse != nullptr && lane == 0) {
-        const int h = static_cast<int>(row % Hq);
-        const int64_t bi = row / Hq, b = bi / Lq, i = bi % Lq;
-        lse[(b * Hq + h) * Lq + i] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * kLn2F;
-    }
+    if (lse != nullptr && lane == 0) lse[(b * Hq + h) * Lq + i] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * kLn2F;
 }
 
-// How a call runs: few rows per key (attention_token.cu) or query tiles per
-// CTA, and CTAs over the keys.
+// How a call runs: few rows per key (attention_token.cu) or tiles of query rows,
+// and which items are split over their keys: those that do not fill a round of
+// the GPU's CTAs (all of them, where there are few).
 struct Plan {
     bool token;
-    int nt, q_blocks, splits;
-    int64_t part_bytes;
+    int nt, q_blocks, whole, rest, splits, rows;
+    int64_t part_rows() const { return i64(rest) * splits * rows; }
+    int64_t part_bytes(int D) const { return part_rows() * (D + 1) * 4; }
 };
 
-Plan make_plan(const ww_attention_t& p, int sms) noexcept
+bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
 {
-    Plan r;
+    Plan& r = *plan;
     r.token = token_form(p);
+    if (r.token) {
+        r.q_blocks = 0;
+        r.nt = 0;
+        r.rows = p.Hq / p.Hk * p.Lq;
+        r.splits = token_splits(p, sms);
+        if (i64(p.B) * p.Hk * r.splits > (1 << 30)) return false;
+        r.whole = 0;
+        r.rest = r.splits > 1 ? p.B * p.Hk : 0;
+        return true;
+    }
     r.nt = p.Lq > 1024 ? 2 : 1;
-    r.q_blocks = (p.Lq + r.nt * kTile - 1) / (r.nt * kTile);
-    const int64_t ctas = i64(r.q_blocks) * p.B * p.Hq;
-    const int key_tiles = (p.Lk + 63) / 64;
-    r.splits = 1;
-    if (r.token) r.splits = token_splits(p, sms);
-    else if (ctas > 0 && ctas < sms && key_tiles >= 8)
-        r.splits = static_cast<int>(std::min<int64_t>({2 * i64(sms) / ctas, key_tiles / 4, 64}));
-    const int64_t rows = i64(p.B) * p.Lq * p.Hq;
-    r.part_bytes = r.splits > 1 ? r.splits * rows * (p.D + 1) * 4 : 0;
-    return r;
+    r.rows = r.nt * kTile;
+    r.q_blocks = (p.Lq + r.rows - 1) / r.rows;
+    const int64_t items = i64(r.q_blocks) * p.B * p.Hq, tiles = (p.Lk + 63) / 64;
+    if (items > (1 << 30)) return false;
+    const int slots = sms * (p.D > 64 ? 2 : 4) / r.nt;
+    r.rest = static_cast<int>(items % slots);
+    r.splits = r.rest == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({slots / r.rest, tiles / 4, 64})));
+    if (r.splits == 1) r.rest = 0;
+    r.whole = static_cast<int>(items - r.rest);
+    return true;
 }
 
 template <typename T, int DP, int NT>
@@ -591,6 +617,7 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.group = p.Hq / p.Hk;
     f.D = p.D;
     f.q_blocks = plan.q_blocks;
+    f.whole_items = plan.whole;
     f.splits = plan.splits;
     f.q_b = p.q_strides[0] != 0;
     f.q_h = p.q_strides[2] != 0;
@@ -600,9 +627,8 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.v_h = p.v_strides[2] != 0;
     f.scale2 = p.scale * kLog2eF;
     f.err = device_error_slot();
-    const int64_t ctas = i64(plan.q_blocks) * p.B * p.Hq * plan.splits;
+    const int64_t ctas = plan.whole + i64(plan.rest) * plan.splits;
     if (f.err == nullptr) return WW_ERR_DEVICE;
-    if (ctas > 0x7fffffff) return WW_ERR_UNSUPPORTED;
     if (plan.nt == 1)
         return dp == 32 ? launch<T, 32, 1>(f, ctas, stream)
              : dp == 64 ? launch<T, 64, 1>(f, ctas, stream) : launch<T, 128, 1>(f, ctas, stream);
@@ -613,14 +639,13 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
 template <typename T>
 int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noexcept
 {
-    const int64_t rows = i64(p.B) * p.Lq * p.Hq;
     float* part_o = static_cast<float*>(p.workspace);
-    float* part_lse = part_o + plan.splits * rows * p.D;
+    float* part_lse = part_o + plan.part_rows() * p.D;
     const int st = plan.token ? attention_token_launch(p, plan.splits, part_o, part_lse, stream)
                               : tiles<T>(p, plan, part_o, part_lse, stream);
-    if (st != WW_SUCCESS || plan.splits == 1) return st;
-    attention_join_kernel<T><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
-        part_o, part_lse, p.out, p.lse, plan.splits, rows, p.Lq, p.Hq, p.D);
+    if (st != WW_SUCCESS || plan.rest == 0) return st;
+    attention_join_kernel<T><<<dim3(plan.rest, (plan.rows + 3) / 4), 128, 0, stream>>>(
+        part_o, part_lse, p.out, p.lse, plan.whole, plan.splits, plan.rows, plan.q_blocks, p.Lq, p.Hq, p.Hk, p.D);
     return launch_status("cross_attention");
 }
 
@@ -637,8 +662,9 @@ extern "C" {
 
 int64_t ww_cross_attention_workspace(const ww_attention_t* p)
 {
-    if (p == nullptr || ww::check_attention(*p) != WW_SUCCESS) return 0;
-    return ww::make_plan(*p, ww::sm_count()).part_bytes;
+    ww::Plan plan;
+    if (p == nullptr || ww::check_attention(*p) != WW_SUCCESS || !ww::make_plan(*p, ww::sm_count(), &plan)) return 0;
+    return plan.part_bytes(p->D);
 }
 
 int ww_cross_attention(const ww_attention_t* p, void* stream)
@@ -648,9 +674,10 @@ int ww_cross_attention(const ww_attention_t* p, void* stream)
     if (st != WW_SUCCESS || p->B == 0 || p->Lq == 0) return st;
     ww::DeviceInfo d;
     if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
-    const ww::Plan plan = ww::make_plan(*p, d.sm_count);
-    if (plan.part_bytes > 0 && p->workspace == nullptr) return WW_ERR_NULL_POINTER;
-    if (plan.part_bytes > p->workspace_bytes) return WW_ERR_UNSUPPORTED;
+    ww::Plan plan;
+    if (!ww::make_plan(*p, d.sm_count, &plan)) return WW_ERR_UNSUPPORTED;
+    if (plan.part_rows() > 0 && p->workspace == nullptr) return WW_ERR_NULL_POINTER;
+    if (plan.part_bytes(p->D) > p->workspace_bytes) return WW_ERR_UNSUPPORTED;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return p->dtype == WW_DTYPE_HALF ? ww::forward<__half>(*p, plan, s) : ww::forward<__nv_bfloat16>(*p, plan, s);
 }

@@ -294,7 +294,6 @@ __global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __gr
                     make_float2(o[x][e][2 * y], o[x][e][2 * y + 1]);
         }
     __syncthreads();
-    const int64_t total = static_cast<int64_t>(p.B) * p.Lq * p.Hq;
     for (int e = threadIdx.x; e < p.rows * (p.D / 8); e += kWarps * 32) {
         const int r = e / (p.D / 8), d = e % (p.D / 8) * 8;
         float top = -INFINITY;
@@ -313,10 +312,11 @@ __global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __gr
         const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
         const float lse2 = sum == 0.0f ? -INFINITY : ms + log2f(sum);
         if (p.splits > 1) {
-            float* to = p.part_o + (split * total + row) * p.D + d;
+            const int64_t part = static_cast<int64_t>(blockIdx.x) * p.rows + r;  // [item][split][row]
+            float* to = p.part_o + part * p.D + d;
             *reinterpret_cast<float4*>(to) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
             *reinterpret_cast<float4*>(to + 4) = make_float4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-            if (d == 0) p.part_lse[split * total + row] = lse2;
+            if (d == 0) p.part_lse[part] = lse2;
         } else {
             *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.D + d) =
                 make_uint4(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv),
@@ -374,7 +374,6 @@ int tokens(const ww_attention_t& p, int splits, float* part_o, float* part_lse, 
     f.err = device_error_slot();
     if (f.err == nullptr) return WW_ERR_DEVICE;
     const int64_t ctas = i64(p.B) * p.Hk * splits;
-    if (ctas > 0x7fffffff) return WW_ERR_UNSUPPORTED;
     if (f.rows <= 16)
         return dp == 32 ? launch<T, 32, 1>(f, ctas, stream)
              : dp == 64 ? launch<T, 64, 1>(f, ctas, stream) : launch<T, 128, 1>(f, ctas, stream);

@@ -13,8 +13,9 @@ bool token_form(const ww_attention_t& p) noexcept;
 // CTAs that share the keys of one batch item and key head.
 int token_splits(const ww_attention_t& p, int sms) noexcept;
 
-// splits > 1: writes part_o [splits][B * Lq * Hq][D] (each normalised) and
-// part_lse [splits][B * Lq * Hq] (log2) instead of out and lse.
+// splits > 1: writes part_o [B * Hk][splits][rows][D] (each normalised) and
+// part_lse [B * Hk][splits][rows] (log2), rows = (shared head, token), instead of
+// out and lse.
 int attention_token_launch(const ww_attention_t& p, int splits, float* part_o, float* part_lse,
                            cudaStream_t stream) noexcept;
 

@@ -542,5 +542,13 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16])
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_wait_ld8(uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+        :
+        : "memory");
+}
+
 }  // namespace umma
 }  // namespace ww
