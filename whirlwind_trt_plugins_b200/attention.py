@@ -23,7 +23,7 @@ import functools
 import math
 import struct
 
-from . import DTYPE_FLOAT, DTYPE_HALF, _check, _lib, _out, _stream_ptr, _torch
+from . import DTYPE_FLOAT, DTYPE_HALF, _check, _lib, _out, _torch
 
 __all__ = ["DTYPE_BF16", "qk_norm_rope", "qk_norm_rope_backward", "cross_attention", "cross_attention_backward",
            "qk_norm_rope_autograd", "cross_attention_autograd", "relative_position_bucket"]
@@ -44,10 +44,24 @@ _ROPE = struct.Struct("@17Pq12q12if0P")
 _ATTN = struct.Struct("@14Pq12q11if0P")
 
 
-@functools.cache
-def _dtypes():
-    torch = _torch()
-    return {torch.float16: DTYPE_HALF, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_FLOAT}
+class _Torch:
+    """torch's pieces that every call needs, looked up once (importing this module does not import torch)."""
+    ready = False
+
+    @classmethod
+    def get(cls):
+        if not cls.ready:
+            torch = _torch()
+            cls.torch, cls.Tensor, cls.empty, cls.empty_like = torch, torch.Tensor, torch.empty, torch.empty_like
+            cls.half, cls.bf16, cls.f32 = torch.float16, torch.bfloat16, torch.float32
+            cls.int32, cls.bool, cls.uint8 = torch.int32, torch.bool, torch.uint8
+            cls.dtypes = {torch.float16: DTYPE_HALF, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_FLOAT}
+            # the current device and stream as plain numbers; the public forms build objects on every call
+            cls.device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            cls.stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+            cls.ready = True
+        return cls
 
 
 def _is_device(t) -> bool:
@@ -55,13 +69,13 @@ def _is_device(t) -> bool:
 
 
 def _tensor(t, name: str, like=None, dtype=None, shape=None, contiguous=True):
-    if not isinstance(t, _torch().Tensor) or not _is_device(t):
+    if not isinstance(t, _Torch.Tensor) or not _is_device(t):
         raise TypeError(f"{name} must be a CUDA tensor")
-    if like is not None and t.device != like.device:
+    if like is not None and t.get_device() != like.get_device():
         raise ValueError(f"{name} must be on {like.device}, got {t.device}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -70,17 +84,24 @@ def _tensor(t, name: str, like=None, dtype=None, shape=None, contiguous=True):
 
 def _vectors(t, name: str, like=None, shape=None):
     """A [B, L, H, D] tensor with strides the kernels take; returns its (b, l, h) strides in elements."""
-    _tensor(t, name, like, None if like is None else like.dtype, shape, contiguous=False)
+    _tensor(t, name, like, None if like is None else like.dtype, shape, False)
     if t.dim() != 4:
         raise ValueError(f"{name} must be [B, L, H, D]")
     st = t.stride()
-    if t.numel() and not t.is_contiguous():
+    if not t.is_contiguous() and t.numel():
         step = 16 // t.element_size()
         if st[3] != 1 or any(n > 1 and s % step for n, s in zip(t.shape[:3], st[:3])):
             raise ValueError(f"{name} needs unit stride along D and other strides of whole 16 bytes, got {st}")
         if t.shape[1] > 1 and st[1] == 0:
             raise ValueError(f"{name} may be broadcast along B and H, not along L")
     return st[:3]
+
+
+def _new(t, out, name: str):
+    """The contiguous output like t: a new one, or the caller's after its checks."""
+    if out is not None:
+        return _out(out, t.shape, t.dtype, t.device, name)
+    return _Torch.empty_like(t) if t.is_contiguous() else _Torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 @contextlib.contextmanager
@@ -97,7 +118,11 @@ def _place(t, stream):
 
 
 def _here(t, stream) -> bool:
-    return stream is None and t.device.index == _torch().cuda.current_device()
+    return stream is None and t.get_device() == _Torch.device()
+
+
+def _workspace(n: int, like):
+    return _Torch.empty(n, dtype=_Torch.uint8, device=like.device)
 
 
 def _ptr(t) -> int:
@@ -105,9 +130,9 @@ def _ptr(t) -> int:
 
 
 def _rope_args(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos):
-    torch = _torch()
+    T = _Torch.get()
     qs = _vectors(q, "q")
-    dt = _dtypes().get(q.dtype)
+    dt = T.dtypes.get(q.dtype)
     if dt is None:
         raise TypeError("q must be float16, bfloat16 or float32")
     B, Lq, Hq, D = q.shape
@@ -116,21 +141,25 @@ def _rope_args(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos):
         raise ValueError(f"k must be [{B}, Lk, Hk, {D}], got {tuple(k.shape)}")
     _tensor(q_weight, "q_weight", q, q.dtype, (D,))
     _tensor(k_weight, "k_weight", q, q.dtype, (D,))
-    _tensor(cos, "cos", q, torch.float32)
-    _tensor(sin, "sin", q, torch.float32, cos.shape)
+    _tensor(cos, "cos", q, T.f32)
+    _tensor(sin, "sin", q, T.f32, cos.shape)
     if cos.dim() != 2 or 2 * cos.shape[1] > D:
         raise ValueError("cos and sin must be [positions, R / 2] with R <= D")
-    steps = []
-    for pos, name, L in ((q_pos, "q_pos", Lq), (k_pos, "k_pos", k.shape[1])):
-        if pos is None:
-            steps.append(0)
-            continue
-        _tensor(pos, name, q, torch.int32)
-        if tuple(pos.shape) not in ((L,), (B, L)):
-            raise ValueError(f"{name} must be [{L}] or [{B}, {L}]")
-        steps.append(L if pos.dim() == 2 else 0)
-    sizes = (*steps, dt, B, Lq, k.shape[1], Hq, k.shape[2], D, 2 * cos.shape[1], cos.shape[0])
+    sizes = (_pos_step(q_pos, "q_pos", q, B, Lq), _pos_step(k_pos, "k_pos", q, B, k.shape[1]), dt, B, Lq, k.shape[1], Hq,
+             k.shape[2], D, 2 * cos.shape[1], cos.shape[0])
     return qs, ks, sizes
+
+
+def _pos_step(pos, name: str, like, B: int, L: int) -> int:
+    """Elements between the batch items of a position tensor."""
+    if pos is None:
+        return 0
+    _tensor(pos, name, like, _Torch.int32)
+    if pos.shape == (L,):
+        return 0
+    if pos.shape != (B, L):
+        raise ValueError(f"{name} must be [{L}] or [{B}, {L}]")
+    return L
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_pos=None, k_pos=None, eps: float = 1e-6,
@@ -148,12 +177,11 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_pos=None, k_pos=None, eps
     if not _here(q, stream):
         with _place(q, stream):
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved, q_out, k_out)
-    q_out = _out(q_out, q.shape, q.dtype, q.device, "q_out")
-    k_out = _out(k_out, k.shape, q.dtype, q.device, "k_out")
+    q_out, k_out = _new(q, q_out, "q_out"), _new(k, k_out, "k_out")
     a = _ROPE.pack(q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
                    sin.data_ptr(), _ptr(q_pos), _ptr(k_pos), q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0,
                    0, *qs, *ks, 0, 0, 0, 0, 0, 0, *sizes, bool(interleaved), eps)
-    _check("ww_qk_norm_rope", _lib.ww_qk_norm_rope(a, _stream_ptr(None)))
+    _check("ww_qk_norm_rope", _lib.ww_qk_norm_rope(a, _Torch.stream(q.get_device())))
     return q_out, k_out
 
 
@@ -168,27 +196,24 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, q_
         with _place(q, stream):
             return qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps,
                                          interleaved)
-    torch = _torch()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
-
-    def pack(ws, n):
-        return _ROPE.pack(q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
-                          sin.data_ptr(), _ptr(q_pos), _ptr(k_pos), 0, 0, dq_out.data_ptr(), dk_out.data_ptr(),
-                          dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), ws, n, *qs, *ks, *gqs, *gks,
-                          *sizes, bool(interleaved), eps)
-
-    n = _lib.ww_qk_norm_rope_backward_workspace(pack(0, 0))
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    _check("ww_qk_norm_rope_backward", _lib.ww_qk_norm_rope_backward(pack(ws.data_ptr(), n), _stream_ptr(None)))
+    dq, dk = _new(q, None, "dq"), _new(k, None, "dk")
+    dqw, dkw = _Torch.empty_like(q_weight), _Torch.empty_like(k_weight)
+    ptrs = (q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+            _ptr(q_pos), _ptr(k_pos), 0, 0, dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            dqw.data_ptr(), dkw.data_ptr())
+    rest = (*qs, *ks, *gqs, *gks, *sizes, bool(interleaved), eps)
+    n = _lib.ww_qk_norm_rope_backward_workspace(_ROPE.pack(*ptrs, 0, 0, *rest))
+    ws = _workspace(n, q)
+    _check("ww_qk_norm_rope_backward", _lib.ww_qk_norm_rope_backward(_ROPE.pack(*ptrs, ws.data_ptr(), n, *rest),
+                                                                     _Torch.stream(q.get_device())))
     return dq, dk, dqw, dkw
 
 
 def _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional, q_offset):
-    torch = _torch()
+    T = _Torch.get()
     qs = _vectors(q, "q")
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    dt = T.dtypes.get(q.dtype)
+    if dt is None or dt == DTYPE_FLOAT:
         raise TypeError("q must be float16 or bfloat16")
     B, Lq, Hq, D = q.shape
     ks = _vectors(k, "k", q)
@@ -199,9 +224,9 @@ def _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidir
         raise ValueError(f"{Hq} query heads cannot share {Hk} key heads evenly")
     vs = _vectors(v, "v", q, k.shape)
     if k_lens is not None:
-        _tensor(k_lens, "k_lens", q, torch.int32, (B,))
+        _tensor(k_lens, "k_lens", q, T.int32, (B,))
     if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8):
+        if key_mask.dtype != T.bool and key_mask.dtype != T.uint8:
             raise TypeError(f"key_mask must be bool or uint8, got {key_mask.dtype}")
         _tensor(key_mask, "key_mask", q, None, (B, Lk))
     buckets = 0
@@ -212,7 +237,7 @@ def _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidir
         buckets = bias_table.shape[1]
     if scale is None:
         scale = 1.0 / math.sqrt(D) if D else 1.0
-    sizes = (_dtypes()[q.dtype], B, Lq, Lk, Hq, Hk, D, buckets, max_distance, bool(bidirectional), q_offset, scale)
+    sizes = (dt, B, Lq, Lk, Hq, Hk, D, buckets, max_distance, bool(bidirectional), q_offset, scale)
     return qs, ks, vs, sizes
 
 
@@ -236,19 +261,17 @@ def cross_attention(q, k, v, scale: float | None = None, k_lens=None, key_mask=N
         with _place(q, stream):
             return cross_attention(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional,
                                    q_offset, return_lse, out)
-    torch = _torch()
-    out = _out(out, q.shape, q.dtype, q.device)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) \
-        if return_lse else None
+    out = _new(q, out, "out")
+    lse = _Torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=_Torch.f32, device=q.device) if return_lse else None
     ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(k_lens), _ptr(key_mask),
             _ptr(bias_table), 0, 0, 0, 0, 0)
     strides = (*qs, *ks, *vs, 0, 0, 0)
     a = _ATTN.pack(*ptrs, 0, 0, *strides, *sizes)
     n = _lib.ww_cross_attention_workspace(a)
     if n:
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        ws = _workspace(n, q)
         a = _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes)
-    _check("ww_cross_attention", _lib.ww_cross_attention(a, _stream_ptr(None)))
+    _check("ww_cross_attention", _lib.ww_cross_attention(a, _Torch.stream(q.get_device())))
     return (out, lse) if return_lse else out
 
 
@@ -261,24 +284,21 @@ def cross_attention_backward(dout, q, k, v, out, lse, scale: float | None = None
     them, in fp32 and in a fixed order."""
     qs, ks, vs, sizes = _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional, q_offset)
     gs = _vectors(dout, "dout", q, q.shape)
-    torch = _torch()
     _tensor(out, "out", q, q.dtype, q.shape)
-    _tensor(lse, "lse", q, torch.float32, (q.shape[0], q.shape[2], q.shape[1]))
+    _tensor(lse, "lse", q, _Torch.f32, (q.shape[0], q.shape[2], q.shape[1]))
     if not _here(q, stream):
         with _place(q, stream):
             return cross_attention_backward(dout, q, k, v, out, lse, scale, k_lens, key_mask, bias_table,
                                             max_distance, bidirectional, q_offset)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dtable = None if bias_table is None else torch.empty_like(bias_table)
+    dq, dk, dv = _new(q, None, "dq"), _new(k, None, "dk"), _new(v, None, "dv")
+    dtable = None if bias_table is None else _Torch.empty_like(bias_table)
     ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(k_lens), _ptr(key_mask),
             _ptr(bias_table), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable))
     strides = (*qs, *ks, *vs, *gs)
     n = _lib.ww_cross_attention_backward_workspace(_ATTN.pack(*ptrs, 0, 0, *strides, *sizes))
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    ws = _workspace(n, q)
     _check("ww_cross_attention_backward", _lib.ww_cross_attention_backward(
-        _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes), _stream_ptr(None)))
+        _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes), _Torch.stream(q.get_device())))
     return dq, dk, dv, dtable
 
 

@@ -217,6 +217,30 @@ __device__ __forceinline__ void warpgroup_sync(int w)
     else asm volatile("bar.sync 4, 128;" : : : "memory");
 }
 
+// Launch of a kernel that follows another one of the same call: it may be set up
+// while that one still runs, and waits for it (wait_for_launches_before) before
+// it reads anything.
+template <typename... P, typename... A>
+inline cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) noexcept
+{
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+__device__ __forceinline__ void wait_for_launches_before()
+{
+    asm volatile("griddepcontrol.wait;" : : : "memory");
+}
+
 // Fills `out`; WW_SUCCESS or the status of rejected arguments (attention_host.cu).
 int make_buckets(int num_buckets, int max_distance, int bidirectional, int q_offset, RelBuckets* out) noexcept;
 

@@ -507,6 +507,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o
         i = item % q_blocks * rows + r;
     }
     if (r >= rows || i >= Lq) return;
+    wait_for_launches_before();
     const int64_t first = static_cast<int64_t>(k) * splits * rows + r;  // + s * rows
     float top = -INFINITY;
     for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[first + static_cast<int64_t>(s) * rows]);
@@ -644,8 +645,8 @@ int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noex
     const int st = plan.token ? attention_token_launch(p, plan.splits, part_o, part_lse, stream)
                               : tiles<T>(p, plan, part_o, part_lse, stream);
     if (st != WW_SUCCESS || plan.rest == 0) return st;
-    attention_join_kernel<T><<<dim3(plan.rest, (plan.rows + 3) / 4), 128, 0, stream>>>(
-        part_o, part_lse, p.out, p.lse, plan.whole, plan.splits, plan.rows, plan.q_blocks, p.Lq, p.Hq, p.Hk, p.D);
+    launch_behind(attention_join_kernel<T>, dim3(plan.rest, (plan.rows + 3) / 4), dim3(128), 0, stream, part_o, part_lse, p.out,
+                  p.lse, plan.whole, plan.splits, plan.rows, plan.q_blocks, p.Lq, p.Hq, p.Hk, p.D);
     return launch_status("cross_attention");
 }
 

@@ -6,10 +6,11 @@
 // The rows of a key head (query heads x tokens, up to 16 or 32) are one M tile
 // of mma.sync m16n8k16, so that shared heads read their keys once; tcgen05's
 // 128 rows would be almost all padding.
-// Each warp runs alone over every kWarps-th tile of 32 keys of its CTA's share:
-// one lane keeps a ring of TMA loads in flight (swizzled rows, read back by
-// ldmatrix without conflicts), the warp computes scores, the running maximum
-// and sum and O in registers, and no barrier joins the warps before the end.
+// Each of 8 warps runs alone over every 8th tile of 16 or 32 keys of its CTA's
+// share: one lane keeps a ring of TMA loads in flight (swizzled rows, read back
+// by ldmatrix without conflicts; up to 128 KB per SM), the warp computes scores,
+// the running maximum and sum and O in registers, and no barrier joins the warps
+// before the end.  O is rescaled only when a maximum has grown by 2^8.
 // The keys are split over CTAs until the GPU is full; the partial rows are
 // joined by attention_join_kernel (attention_forward.cu) in order.
 #include "attention_token.cuh"
@@ -21,8 +22,11 @@
 namespace ww {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kKeys = 32;  // keys of a warp's tile
+constexpr int kWarps = 8;
+constexpr float kRescale = 8.0f;  // log2 growth of a maximum that is left in P
+
+// Keys of a warp's tile: 8 KB of keys and values at D = 64 and 128.
+constexpr int tile_keys(int dp) { return dp == 128 ? 16 : 32; }
 
 struct TokenParams {
     CUtensorMap k, v;
@@ -39,23 +43,26 @@ struct TokenParams {
     int32_t B, Lq, Lk, Hq, Hk, D, rows;
     int32_t splits;
     int32_t k_b, k_h, v_b, v_h;
+    int32_t max_entries;
     float scale2;
     int* err;
 };
 
 template <int DP, int MB>
 struct Layout {
+    static constexpr int kKeys = tile_keys(DP);
     static constexpr int kRow = DP == 32 ? 64 : 128;
     static constexpr int kChunks = DP * 2 / kRow;
     static constexpr int kChunkBytes = kKeys * kRow;
     static constexpr int kTileBytes = kKeys * DP * 2;
-    static constexpr int kStages = DP == 128 ? 3 : DP == 64 ? 5 : 8;
+    static constexpr int kStages = DP == 32 ? 4 : 3;
     static constexpr int kRing = kStages * 2 * kTileBytes;            // of a warp
     static constexpr int kQPitch = DP * 2 + 16;                       // bytes, ldmatrix without conflicts
     static constexpr int kQ = kWarps * kRing;
     static constexpr int kBar = kQ + MB * 16 * kQPitch;
     static constexpr int kMl = kBar + kWarps * kStages * 8;           // maximum and sum of [warp][row]
-    static constexpr int kBytes = kMl + kWarps * MB * 16 * 8 + 1024;
+    static constexpr int kBias = kMl + kWarps * MB * 16 * 8;          // [heads][buckets] values, [entries] buckets
+    static constexpr int kBytes = kBias + 1024;
     static_assert(MB * 16 * DP * 4 <= kRing, "a warp's rows replace its ring at the end");
 };
 
@@ -91,10 +98,10 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
 }
 
 template <typename T, int DP, int MB>
-__global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __grid_constant__ TokenParams p)
+__global__ void __launch_bounds__(kWarps * 32, 1) attention_token_kernel(const __grid_constant__ TokenParams p)
 {
     using L = Layout<DP, MB>;
-    constexpr int S = L::kStages;
+    constexpr int S = L::kStages, kKeys = L::kKeys;
     constexpr int kRows = MB * 16;
     extern __shared__ uint8_t raw[];
     uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
@@ -136,6 +143,17 @@ __global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __gr
                                                 (r % p.Lq) * p.q_strides[1] + (g * group + r / p.Lq) * p.q_strides[2] + d);
         *reinterpret_cast<uint4*>(base + L::kQ + r * L::kQPitch + d * 2) = u;
     }
+    // bias: the heads' values by bucket, buckets by position over this CTA's keys
+    const bool biased = p.rel.per_side != 0;
+    float* values = reinterpret_cast<float*>(base + L::kBias);
+    uint8_t* buckets = base + L::kBias + (biased ? group * p.rel.total * 4 : 0);
+    RelRange range;
+    if (biased) {
+        for (int e = threadIdx.x; e < group * p.rel.total; e += kWarps * 32)
+            values[e] = bias_value<T>(static_cast<const T*>(p.table)[static_cast<int64_t>(g) * group * p.rel.total + e]) * kLog2eF;
+        range = rel_range(p.rel, first * kKeys - (p.Lq - 1) - p.rel.q_offset, last * kKeys - 1 - p.rel.q_offset);
+        if (last > first) build_buckets(p.rel, range, buckets, threadIdx.x, kWarps * 32);
+    }
     __syncthreads();
     const uint32_t q_at = sm + L::kQ + (lane % 16) * L::kQPitch + (lane / 16) * 16;
 
@@ -148,41 +166,60 @@ __global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __gr
         m[x][0] = m[x][1] = -INFINITY;
         l[x][0] = l[x][1] = 0.0f;
     }
+    // query fragments of a single M tile stay in registers
+    uint32_t qf[MB == 1 ? DP / 16 : 1][4];
+    if (MB == 1)
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) ldmatrix_x4(q_at + d * 32, qf[d]);
+    uint8_t byte = 0;  // of the key mask, for the tile to come
+    const auto mask_byte = [&](int i) {
+        const int key = (first + warp + kWarps * i) * kKeys + lane;
+        byte = lane < kKeys && key < len ? __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + key) : 0;
+    };
+    if (p.key_mask != nullptr && n > 0) mask_byte(0);
+    constexpr uint32_t kAll = kKeys == 32 ? ~0u : (1u << (kKeys & 31)) - 1;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
         const int s = i % S, key0 = (first + warp + kWarps * i) * kKeys;
         const uint32_t kt = ring + s * 2 * L::kTileBytes, vt = kt + L::kTileBytes;
-        uint32_t keep = len - key0 >= kKeys ? ~0u : (1u << (len - key0)) - 1;
-        if (p.key_mask != nullptr)
-            keep &= __ballot_sync(~0u, key0 + lane < len &&
-                                           __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + key0 + lane) != 0);
+        uint32_t keep = len - key0 >= kKeys ? kAll : (1u << (len - key0)) - 1;
+        if (p.key_mask != nullptr) {
+            keep &= __ballot_sync(~0u, byte != 0);
+            if (i + 1 < n) mask_byte(i + 1);
+        }
         ok = ok && umma::mbar_poll(bars + s * 8, (i / S) & 1);
-        if (keep != ~0u) {
+        if (keep != kAll) {
             // rows of V behind masked keys: 0 in place of whatever they hold
             __syncwarp();
-            if (!((keep >> lane) & 1))
+            if (lane < kKeys && !((keep >> lane) & 1))
                 for (int c = 0; c < L::kChunks; ++c)
 #pragma unroll
                     for (int j = 0; j < L::kRow; j += 16)
                         umma::st_shared_v4(vt + c * L::kChunkBytes + lane * L::kRow + j, 0, 0, 0, 0);
             __syncwarp();
         }
-        float sc[MB][4][4];
+        float sc[MB][kKeys / 8][4];
 #pragma unroll
         for (int x = 0; x < MB; ++x)
 #pragma unroll
-            for (int nb = 0; nb < 4; ++nb) sc[x][nb][0] = sc[x][nb][1] = sc[x][nb][2] = sc[x][nb][3] = 0.0f;
+            for (int nb = 0; nb < kKeys / 8; ++nb) sc[x][nb][0] = sc[x][nb][1] = sc[x][nb][2] = sc[x][nb][3] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DP; d += 32) {
             uint32_t a[MB][2][4];
 #pragma unroll
-            for (int x = 0; x < MB; ++x) {
-                ldmatrix_x4(q_at + x * 16 * L::kQPitch + d * 2, a[x][0]);
-                ldmatrix_x4(q_at + x * 16 * L::kQPitch + d * 2 + 32, a[x][1]);
-            }
+            for (int x = 0; x < MB; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    if (MB == 1) {
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) a[x][y][z] = qf[MB == 1 ? d / 16 + y : 0][z];
+                    } else {
+                        ldmatrix_x4(q_at + x * 16 * L::kQPitch + d * 2 + y * 32, a[x][y]);
+                    }
+                }
             const uint32_t chunk = kt + d * 2 / L::kRow * L::kChunkBytes;
 #pragma unroll
-            for (int nb = 0; nb < 4; ++nb) {
+            for (int nb = 0; nb < kKeys / 8; ++nb) {
                 uint32_t kb[4];  // 8 keys x 32 dims
                 ldmatrix_x4(piece<L::kRow>(chunk, nb * 8 + lane % 8, d * 2 % L::kRow / 16 + lane / 8), kb);
 #pragma unroll
@@ -193,34 +230,28 @@ __global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __gr
             }
         }
         // scores in log2 units; this lane: rows lane / 4 (+ 8), keys 2 (lane % 4) + {0, 1} of each 8
-        const bool biased = p.rel.per_side != 0;
-        bool one = true;  // the tile's positions lie in one bucket for every token
         int bucket = 0;
+        bool one = true;  // the tile's positions lie in one bucket for every token
+        const int rel0 = key0 - p.rel.q_offset;
         if (biased) {
-            const int lo = key0 - (p.Lq - 1) - p.rel.q_offset, hi = key0 + kKeys - 1 - p.rel.q_offset;
-            bucket = rel_bucket(p.rel, lo);
-            one = bucket == rel_bucket(p.rel, hi);
+            bucket = bucket_at(range, buckets, rel0 - (p.Lq - 1));
+            one = bucket == bucket_at(range, buckets, rel0 + kKeys - 1);
         }
 #pragma unroll
         for (int x = 0; x < MB; ++x)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 const int r = x * 16 + y * 8 + lane / 4;
-                const T* table = nullptr;
-                float flat = 0.0f;
-                if (biased && r < p.rows) {
-                    table = static_cast<const T*>(p.table) + static_cast<int64_t>(g * group + r / p.Lq) * p.rel.total;
-                    if (one) flat = bias_value<T>(table[bucket]) * kLog2eF;
-                }
+                const float* table = biased && r < p.rows ? values + r / p.Lq * p.rel.total : nullptr;
+                const uint8_t* by = buckets + rel0 - (r % p.Lq) - range.lo;
+                const float flat = table != nullptr ? table[bucket] : 0.0f;
                 float top = -INFINITY;
 #pragma unroll
-                for (int nb = 0; nb < 4; ++nb)
+                for (int nb = 0; nb < kKeys / 8; ++nb)
 #pragma unroll
                     for (int z = 0; z < 2; ++z) {
                         const int c = nb * 8 + 2 * (lane % 4) + z;
-                        float bias = flat;
-                        if (!one && table != nullptr)
-                            bias = bias_value<T>(table[rel_bucket(p.rel, key0 + c - r % p.Lq - p.rel.q_offset)]) * kLog2eF;
+                        const float bias = !one && table != nullptr ? table[by[c]] : flat;
                         float v = fmaf(sc[x][nb][2 * y + z], p.scale2, bias);
                         v = (keep >> c) & 1 ? v : -INFINITY;
                         sc[x][nb][2 * y + z] = v;
@@ -228,17 +259,20 @@ __global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __gr
                     }
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                const float mn = fmaxf(m[x][y], top), ms = mn == -INFINITY ? 0.0f : mn;
-                const float f = exp2_approx(m[x][y] - ms);
-                m[x][y] = mn;
-                l[x][y] *= f;
+                if (__any_sync(~0u, top > m[x][y] + kRescale || i == 0)) {
+                    const float mn = fmaxf(m[x][y], top);
+                    const float f = m[x][y] == -INFINITY ? 0.0f : exp2_approx(m[x][y] - mn);
+                    m[x][y] = mn;
+                    l[x][y] *= f;
 #pragma unroll
-                for (int e = 0; e < DP / 8; ++e) {
-                    o[x][e][2 * y] *= f;
-                    o[x][e][2 * y + 1] *= f;
+                    for (int e = 0; e < DP / 8; ++e) {
+                        o[x][e][2 * y] *= f;
+                        o[x][e][2 * y + 1] *= f;
+                    }
                 }
+                const float ms = m[x][y] == -INFINITY ? 0.0f : m[x][y];
 #pragma unroll
-                for (int nb = 0; nb < 4; ++nb)
+                for (int nb = 0; nb < kKeys / 8; ++nb)
 #pragma unroll
                     for (int z = 0; z < 2; ++z) {
                         const float pr = exp2_approx(sc[x][nb][2 * y + z] - ms);
@@ -247,7 +281,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_token_kernel(const __gr
                     }
             }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 16 keys each
+        for (int h = 0; h < kKeys / 16; ++h) {  // 16 keys each
             uint32_t a[MB][4];
 #pragma unroll
             for (int x = 0; x < MB; ++x) {
@@ -331,9 +365,10 @@ int launch(const TokenParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, MB>;
     const auto kernel = attention_token_kernel<T, DP, MB>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
+    const int bytes = L::kBytes + (f.table != nullptr ? f.Hq / f.Hk * f.rel.total * 4 + f.max_entries : 0);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
         return launch_status("cross_attention");
-    kernel<<<static_cast<unsigned>(ctas), kWarps * 32, L::kBytes, stream>>>(f);
+    kernel<<<static_cast<unsigned>(ctas), kWarps * 32, bytes, stream>>>(f);
     return launch_status("cross_attention");
 }
 
@@ -344,8 +379,8 @@ int tokens(const ww_attention_t& p, int splits, float* part_o, float* part_lse, 
     const int dp = p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128;
     constexpr bool bf = !std::is_same<T, __half>::value;
     const int nk[3] = {p.B, p.Lk, p.Hk};
-    if (p.Lk > 0 && (!encode_vectors_map(&f.k, bf, p.k, p.D, nk, p.k_strides, dp == 32 ? 32 : 64, kKeys) ||
-                     !encode_vectors_map(&f.v, bf, p.v, p.D, nk, p.v_strides, dp == 32 ? 32 : 64, kKeys)))
+    if (p.Lk > 0 && (!encode_vectors_map(&f.k, bf, p.k, p.D, nk, p.k_strides, dp == 32 ? 32 : 64, tile_keys(dp)) ||
+                     !encode_vectors_map(&f.v, bf, p.v, p.D, nk, p.v_strides, dp == 32 ? 32 : 64, tile_keys(dp))))
         return WW_ERR_UNSUPPORTED;
     f.q = p.q;
     f.out = p.out;
@@ -355,6 +390,9 @@ int tokens(const ww_attention_t& p, int splits, float* part_o, float* part_lse, 
     f.table = p.bias_table;
     if (p.bias_table != nullptr)
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
+    f.max_entries = 0;
+    if (p.bias_table != nullptr)
+        f.max_entries = static_cast<int>(std::min<int64_t>(2 * (p.max_distance + kRelMargin) + 1, i64(p.Lk) + 64 + p.Lq));
     f.part_o = part_o;
     f.part_lse = part_lse;
     for (int i = 0; i < 3; ++i) f.q_strides[i] = p.q_strides[i];
@@ -387,9 +425,10 @@ bool token_form(const ww_attention_t& p) noexcept { return i64(p.Hq / p.Hk) * p.
 
 int token_splits(const ww_attention_t& p, int sms) noexcept
 {
-    const int64_t ctas = i64(p.B) * p.Hk, tiles = (p.Lk + kKeys - 1) / kKeys;
+    const int keys = tile_keys(p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128);
+    const int64_t ctas = i64(p.B) * p.Hk, tiles = (p.Lk + keys - 1) / keys;
     if (ctas <= 0 || ctas >= sms) return 1;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms / ctas, tiles / (2 * kWarps), 128})));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms / ctas, tiles / kWarps, 128})));
 }
 
 int attention_token_launch(const ww_attention_t& p, int splits, float* part_o, float* part_lse,

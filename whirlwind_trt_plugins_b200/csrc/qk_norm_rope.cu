@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(kBlock) weight_gradient_kernel(const __grid_co
     __shared__ float sums[kBlock / 32][32];
     const Side& s = p.side[blockIdx.y];
     const int d = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
+    wait_for_launches_before();
     float sum = 0.0f;
     if (d < p.D)
         for (int n = w; n < s.blocks; n += kBlock / 32) sum += s.part[static_cast<int64_t>(n) * p.D + d];
@@ -426,7 +427,7 @@ int launch(const RopeParams& r, bool inter, bool backward, cudaStream_t stream) 
             else qk_norm_rope_backward_kernel<T, V, GROUP, false><<<blocks, kBlock, 0, stream>>>(r);
         }
     }
-    if (backward) weight_gradient_kernel<T><<<dim3((r.D + 31) / 32, 2), kBlock, 0, stream>>>(r);
+    if (backward) launch_behind(weight_gradient_kernel<T>, dim3((r.D + 31) / 32, 2), dim3(kBlock), 0, stream, r);
     return launch_status(backward ? "qk_norm_rope_backward" : "qk_norm_rope");
 }
 
