@@ -276,7 +276,7 @@ int ww_disparity_regression(const void* cost, void* out, int in_dtype, int out_d
  * Tensors of vectors are [B, L, H, D] with unit stride along D and the other
  * strides given in elements ({b, l, h}; multiples of 16 bytes; 0 = broadcast
  * along b or h).  Outputs and gradients are contiguous.  Pointers to vectors
- * are 16-byte aligned.  Pointers of tensors without elements may be NULL.
+ * and to the cos and sin tables are 16-byte aligned.  Pointers of tensors without elements may be NULL.
  * dtypes WW_DTYPE_HALF, WW_DTYPE_BF16 and, for ww_qk_norm_rope,
  * WW_DTYPE_FLOAT; fp32 arithmetic, one rounding to the output's type.
  * Some calls need device scratch memory: the *_workspace functions return the

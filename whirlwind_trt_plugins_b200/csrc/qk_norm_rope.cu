@@ -9,26 +9,54 @@
 //   dw = sum over rows of g xh,   u = g w,   dx = r (u - xh mean_d(u xh)).
 //
 // Bound: HBM (forward 2 values per element moved, backward 3; ~10 flops).
-// Layout: a group of lanes owns a token's head; each lane holds two chunks of
-// V consecutive dims whose members are rotation partners of one another
-// (chunk a of the first half, chunk b of the second; for interleaved pairs
-// each chunk holds its own pairs), so the rotation needs no exchange and the
-// only shuffles are the group's sums.  A group takes kHeads heads of one token
-// at once: their loads are in flight together and the token's cos and sin are
-// read once.  Queries and keys are one grid: one launch.
-// The weight gradients stay in registers over all tokens of a group, are
-// joined per block through shared memory and over blocks by a second small
-// kernel, both in a fixed order: the same inputs give the same bits.
+// That leaves about 16 instructions per value and lane, so the layout saves them:
+// all (token, head) rows are one sequence, a row is a group of lanes, and a lane
+// holds two pieces of V values that are each other's rotation partners (piece a of
+// the first half, piece b of the second; for interleaved pairs each its own
+// pairs): the rotation needs no exchange and both pieces share their angles.
+// Neighbouring groups hold neighbouring rows, so that a warp's loads lie side by
+// side; divisions by H and L are multiplies;
+// arithmetic is two values an instruction.  cos and sin come from L1 (a token's
+// heads are neighbours).  Queries and keys are one grid: one launch.
+// The weight gradients stay in registers over all rows of a lane, are joined per
+// block through shared memory and over blocks by a second small kernel, both in a
+// fixed order: the same inputs give the same bits.
 #include "attention.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace ww {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kHeads = 4;
-constexpr int kMaxPartBlocks = 296;  // backward: two blocks of each of 148 SMs per side
+// Resident blocks asked of the compiler, one row of a lane in flight: more rows
+// per lane cost registers and with them warps (rows of 16 pairs 94 x 312, fp16,
+// 961 MB: 158 us; two rows and 4 blocks 180 us, four and 3 207 us, one and 8,
+// which spills, 304 us).
+constexpr int kForwardBlocks = 6;
+constexpr int backward_blocks(int V) { return V == 8 ? 3 : 4; }
+constexpr int kSms = 148;
+
+// Division of n < 2^31 by d, prepared on the host.
+struct Divisor {
+    uint32_t mul = 1;
+    int32_t shift = 0;
+    int32_t d = 1;
+    __device__ __forceinline__ int div(int n) const
+    {
+        return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+    }
+};
+
+Divisor make_divisor(int d)
+{
+    Divisor r;
+    r.d = d;
+    while ((int64_t{1} << r.shift) < d) ++r.shift;
+    r.mul = static_cast<uint32_t>(((((uint64_t{1} << r.shift) - d) << 32) / d) + 1);
+    return r;
+}
 
 struct Side {
     const void* x;
@@ -39,11 +67,11 @@ struct Side {
     void* dw;
     float* part;  // backward: [blocks][D] partial weight gradients
     int64_t sb, sl, sh, gb, gl, gh;
+    Divisor L, H;
+    int32_t x_linear, g_linear;  // rows follow one another without a gap
     int32_t pos_stride;
-    int32_t L, H;
-    int32_t chunks;   // head chunks of kHeads per token
-    int32_t items;    // B * L * chunks
-    int32_t blocks;   // grid blocks of this side
+    int32_t rows;    // B * L * H
+    int32_t blocks;  // grid blocks of this side
 };
 
 struct RopeParams {
@@ -51,99 +79,139 @@ struct RopeParams {
     const float* cos;
     const float* sin;
     int32_t D, R, P;
-    int32_t lanes;  // lanes with work in a group
-    float eps;
+    int32_t lanes;  // lanes of a group with pieces
+    float eps, inv_d;
 };
 
+// V values of T as V / 2 pairs of fp32.
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T v[V];
-};
-
-template <typename T, int V>
-__device__ __forceinline__ void load(const T* p, float (&f)[V])
+__device__ __forceinline__ void load(const T* p, Pair (&f)[V / 2])
 {
-    const Vec<T, V> u = *reinterpret_cast<const Vec<T, V>*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = to_float(u.v[i]);
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void store(T* p, const float (&f)[V])
-{
-    Vec<T, V> u;
-#pragma unroll
-    for (int i = 0; i < V; ++i) u.v[i] = from_float<T>(f[i]);
-    *reinterpret_cast<Vec<T, V>*>(p) = u;
-}
-
-// The two chunks of lane l: dims [a, a + V) and [b, b + V), and whether they rotate.
-template <int V>
-__device__ __forceinline__ void chunk_dims(int l, int D, int R, int& a, int& b, bool& rot)
-{
-    const int nr = R / (2 * V);
-    rot = l < nr;
-    if (rot) {
-        a = l * V;
-        b = R / 2 + a;
+    constexpr int kN = V * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[kN];
+    if constexpr (kN == 4) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = u.x;
+        w[1] = u.y;
+        w[2] = u.z;
+        w[3] = u.w;
     } else {
-        a = R + (l - nr) * V;
-        b = a + (D - R) / 2;
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = u.x;
+        w[1] = u.y;
+    }
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            f[i] = pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[i] = pair(v.x, v.y);
+        } else {
+            f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        }
     }
 }
 
-// Angles of one lane: V per chunk.  Pairs (i, i + R/2): both chunks share the
-// V angles from a; interleaved: V/2 angles for each chunk.
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const Pair (&f)[V / 2])
+{
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) unpair(f[i], v[2 * i], v[2 * i + 1]);
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else if constexpr (V == 8)
+        *reinterpret_cast<uint4*>(p) =
+            make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    else
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+}
+
+// The two pieces of a lane: dims [a, a + V) and [b, b + V), and whether they
+// rotate.  Lanes beyond the row hold its last pieces.
+struct Pieces {
+    int a, b;
+    bool rotates;
+};
+
+template <int V>
+__device__ __forceinline__ Pieces pieces_of(int lane, const RopeParams& p)
+{
+    Pieces r;
+    const int l = min(lane, p.lanes - 1), n = p.R / (2 * V);
+    r.rotates = l < n;
+    r.a = r.rotates ? l * V : p.R + (l - n) * V;
+    r.b = r.a + (r.rotates ? p.R / 2 : (p.D - p.R) / 2);
+    return r;
+}
+
+// cos and sin of the two pieces: V angles that both share, or (interleaved) V / 2
+// for each, a's first; as pairs (INTER: as values).
 template <int V, bool INTER>
 struct Angles {
-    float ca[V], sa[V];  // INTER: first V/2 for chunk a, the others for chunk b
-    __device__ __forceinline__ void get(const float* cos, const float* sin, int64_t row, int a, int b)
+    float c[V], s[V];
+    __device__ __forceinline__ void get(const RopeParams& p, int pos, const Pieces& x)
     {
-        if (INTER) {
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                ca[i] = __ldg(cos + row + a / 2 + i);
-                sa[i] = __ldg(sin + row + a / 2 + i);
-                ca[V / 2 + i] = __ldg(cos + row + b / 2 + i);
-                sa[V / 2 + i] = __ldg(sin + row + b / 2 + i);
-            }
-        } else {
+        if (!x.rotates) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                ca[i] = __ldg(cos + row + a + i);
-                sa[i] = __ldg(sin + row + a + i);
+                c[i] = 1.0f;
+                s[i] = 0.0f;
             }
+            return;
+        }
+        const int64_t row = static_cast<int64_t>(pos) * (p.R / 2);
+        if (INTER) {
+            part(p, row + x.a / 2, 0);
+            part(p, row + x.b / 2, V / 2);
+        } else {
+            part(p, row + x.a, 0);
+            part(p, row + x.a + V / 2, V / 2);
         }
     }
-    __device__ __forceinline__ void none()
+    // V / 2 angles from `at` to place i
+    __device__ __forceinline__ void part(const RopeParams& p, int64_t at, int i)
     {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            ca[i] = 1.0f;
-            sa[i] = 0.0f;
+        if constexpr (V == 8) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos + at)), b = __ldg(reinterpret_cast<const float4*>(p.sin + at));
+            c[i] = a.x;
+            c[i + 1] = a.y;
+            c[i + 2] = a.z;
+            c[i + 3] = a.w;
+            s[i] = b.x;
+            s[i + 1] = b.y;
+            s[i + 2] = b.z;
+            s[i + 3] = b.w;
+        } else {
+            const float2 a = __ldg(reinterpret_cast<const float2*>(p.cos + at)), b = __ldg(reinterpret_cast<const float2*>(p.sin + at));
+            c[i] = a.x;
+            c[i + 1] = a.y;
+            s[i] = b.x;
+            s[i + 1] = b.y;
         }
     }
-    // turn by the angle (dir = 1) or back (dir = -1)
+    // both pieces turned by the angle (DIR 1) or back (-1)
     template <int DIR>
-    __device__ __forceinline__ void turn(float (&x)[V], float (&y)[V]) const
+    __device__ __forceinline__ void turn(Pair (&x)[V / 2], Pair (&y)[V / 2]) const
     {
         if (INTER) {
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
-                const float s0 = DIR * sa[i], s1 = DIR * sa[V / 2 + i];
-                const float p = x[2 * i], q = x[2 * i + 1];
-                x[2 * i] = p * ca[i] - q * s0;
-                x[2 * i + 1] = q * ca[i] + p * s0;
-                const float u = y[2 * i], v = y[2 * i + 1];
-                y[2 * i] = u * ca[V / 2 + i] - v * s1;
-                y[2 * i + 1] = v * ca[V / 2 + i] + u * s1;
+                float u, v;
+                unpair(x[i], u, v);
+                x[i] = pair(u * c[i] - v * (DIR * s[i]), v * c[i] + u * (DIR * s[i]));
+                unpair(y[i], u, v);
+                y[i] = pair(u * c[V / 2 + i] - v * (DIR * s[V / 2 + i]), v * c[V / 2 + i] + u * (DIR * s[V / 2 + i]));
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float p = x[i], q = y[i], s = DIR * sa[i];
-                x[i] = p * ca[i] - q * s;
-                y[i] = q * ca[i] + p * s;
+            for (int i = 0; i < V / 2; ++i) {
+                const Pair cc = pair(c[2 * i], c[2 * i + 1]), ss = pair(DIR * s[2 * i], DIR * s[2 * i + 1]),
+                           ns = pair(-DIR * s[2 * i], -DIR * s[2 * i + 1]);
+                const Pair u = x[i];
+                x[i] = fma2(y[i], ns, mul2(u, cc));
+                y[i] = fma2(u, ss, mul2(y[i], cc));
             }
         }
     }
@@ -153,176 +221,173 @@ template <int GROUP>
 __device__ __forceinline__ float group_sum(float v)
 {
 #pragma unroll
-    for (int o = GROUP / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = GROUP / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     return v;
 }
 
-__device__ __forceinline__ int position(const RopeParams& p, const Side& s, int b, int l)
+__device__ __forceinline__ float both(Pair p)
 {
-    const int at = s.pos != nullptr ? __ldg(s.pos + static_cast<int64_t>(b) * s.pos_stride + l) : l;
-    return min(max(at, 0), p.P - 1);
+    float a, b;
+    unpair(p, a, b);
+    return a + b;
+}
+
+// Batch item, token and head of a row.
+struct RowAt {
+    int b, l, h;
+    __device__ __forceinline__ RowAt(const Side& s, int row)
+    {
+        const int token = s.H.div(row);
+        h = row - token * s.H.d;
+        b = s.L.div(token);
+        l = token - b * s.L.d;
+    }
+};
+
+__device__ __forceinline__ int position(const RopeParams& p, const Side& s, const RowAt& at)
+{
+    const int pos = s.pos != nullptr ? __ldg(s.pos + static_cast<int64_t>(at.b) * s.pos_stride + at.l) : at.l;
+    return min(max(pos, 0), p.P - 1);
+}
+
+__device__ __forceinline__ int64_t offset(bool linear, int D, int row, const RowAt& at, int64_t sb, int64_t sl, int64_t sh)
+{
+    return linear ? static_cast<int64_t>(row) * D : at.b * sb + at.l * sl + at.h * sh;
 }
 
 template <typename T, int V, int GROUP, bool INTER>
-__global__ void __launch_bounds__(kBlock) qk_norm_rope_kernel(const __grid_constant__ RopeParams p)
+__global__ void __launch_bounds__(kBlock, kForwardBlocks) qk_norm_rope_kernel(const __grid_constant__ RopeParams p)
 {
     const bool second = static_cast<int>(blockIdx.x) >= p.side[0].blocks;
     const Side& s = p.side[second ? 1 : 0];
     const int block = blockIdx.x - (second ? p.side[0].blocks : 0);
-    const int item = block * (kBlock / GROUP) + threadIdx.x / GROUP;
     const int lane = threadIdx.x % GROUP;
-    const bool live = item < s.items && lane < p.lanes;
-    const int it = min(item, s.items - 1);
-    const int token = it / s.chunks;
-    const int h0 = (it - token * s.chunks) * kHeads;
-    const int b = token / s.L, l = token - b * s.L;
-    int a, c;
-    bool rot;
-    chunk_dims<V>(min(lane, p.lanes - 1), p.D, p.R, a, c, rot);
-
-    const T* x = static_cast<const T*>(s.x) + b * s.sb + l * s.sl;
-    T* y = static_cast<T*>(s.y) + (static_cast<int64_t>(token) * s.H) * p.D;
-    float xa[kHeads][V], xc[kHeads][V];
+    constexpr int kStep = kBlock / GROUP;  // rows of a block at a time
+    const int row = block * kStep + threadIdx.x / GROUP;
+    const Pieces pc = pieces_of<V>(lane, p);
+    const int known = min(row, s.rows - 1);
+    const RowAt at(s, known);
+    const T* x = static_cast<const T*>(s.x) + offset(s.x_linear, p.D, known, at, s.sb, s.sl, s.sh);
+    Pair xa[V / 2], xb[V / 2], wa[V / 2], wb[V / 2];
+    load<T, V>(x + pc.a, xa);
+    load<T, V>(x + pc.b, xb);
+    load<T, V>(static_cast<const T*>(s.w) + pc.a, wa);
+    load<T, V>(static_cast<const T*>(s.w) + pc.b, wb);
+    Pair sq = mul2(xa[0], xa[0]);
 #pragma unroll
-    for (int j = 0; j < kHeads; ++j) {
-        const int h = min(h0 + j, s.H - 1);
-        load<T, V>(x + h * s.sh + a, xa[j]);
-        load<T, V>(x + h * s.sh + c, xc[j]);
+    for (int i = 1; i < V / 2; ++i) sq = fma2(xa[i], xa[i], sq);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) sq = fma2(xb[i], xb[i], sq);
+    const float r = rsqrtf(fmaf(group_sum<GROUP>(lane < p.lanes ? both(sq) : 0.0f), p.inv_d, p.eps));
+    const Pair r2 = pair(r, r);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        xa[i] = mul2(xa[i], mul2(r2, wa[i]));
+        xb[i] = mul2(xb[i], mul2(r2, wb[i]));
     }
     Angles<V, INTER> ang;
-    if (rot) ang.get(p.cos, p.sin, static_cast<int64_t>(position(p, s, b, l)) * (p.R / 2), a, c);
-    else ang.none();
-    float wa[V], wc[V];
-    load<T, V>(static_cast<const T*>(s.w) + a, wa);
-    load<T, V>(static_cast<const T*>(s.w) + c, wc);
-#pragma unroll
-    for (int j = 0; j < kHeads; ++j) {
-        float sq = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) sq += xa[j][i] * xa[j][i] + xc[j][i] * xc[j][i];
-        sq = group_sum<GROUP>(lane < p.lanes ? sq : 0.0f);
-        const float r = rsqrtf(sq / p.D + p.eps);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            xa[j][i] *= r * wa[i];
-            xc[j][i] *= r * wc[i];
-        }
-        ang.template turn<1>(xa[j], xc[j]);
-        if (live && h0 + j < s.H) {
-            store<T, V>(y + static_cast<int64_t>(h0 + j) * p.D + a, xa[j]);
-            store<T, V>(y + static_cast<int64_t>(h0 + j) * p.D + c, xc[j]);
-        }
+    ang.get(p, p.R > 0 ? position(p, s, at) : 0, pc);
+    ang.template turn<1>(xa, xb);
+    if (row < s.rows && lane < p.lanes) {
+        T* y = static_cast<T*>(s.y) + static_cast<int64_t>(row) * p.D;
+        store<T, V>(y + pc.a, xa);
+        store<T, V>(y + pc.b, xb);
     }
 }
 
 template <typename T, int V, int GROUP, bool INTER>
-__global__ void __launch_bounds__(kBlock) qk_norm_rope_backward_kernel(const __grid_constant__ RopeParams p)
+__global__ void __launch_bounds__(kBlock, backward_blocks(V)) qk_norm_rope_backward_kernel(const __grid_constant__ RopeParams p)
 {
     __shared__ float joined[kBlock * 2 * V];
     const bool second = static_cast<int>(blockIdx.x) >= p.side[0].blocks;
     const Side& s = p.side[second ? 1 : 0];
     const int block = blockIdx.x - (second ? p.side[0].blocks : 0);
     const int lane = threadIdx.x % GROUP;
-    int a, c;
-    bool rot;
-    chunk_dims<V>(min(lane, p.lanes - 1), p.D, p.R, a, c, rot);
-    float wa[V], wc[V], da[V], dc[V];
-    load<T, V>(static_cast<const T*>(s.w) + a, wa);
-    load<T, V>(static_cast<const T*>(s.w) + c, wc);
+    constexpr int kStep = kBlock / GROUP;
+    const Pieces pc = pieces_of<V>(lane, p);
+    Pair wa[V / 2], wb[V / 2], da[V / 2], db[V / 2];
+    load<T, V>(static_cast<const T*>(s.w) + pc.a, wa);
+    load<T, V>(static_cast<const T*>(s.w) + pc.b, wb);
 #pragma unroll
-    for (int i = 0; i < V; ++i) da[i] = dc[i] = 0.0f;
-
-    const int step = s.blocks * (kBlock / GROUP);
-    // every group of a warp makes the same number of rounds (the sums are warp-wide shuffles)
-    const int first = block * (kBlock / GROUP) + threadIdx.x / GROUP;
-    const int rounds = (s.items + step - 1) / step;
-    for (int n = 0; n < rounds; ++n) {
-        const int item = first + n * step;
-        const int it = min(item, s.items - 1);
-        const int token = it / s.chunks;
-        const int h0 = (it - token * s.chunks) * kHeads;
-        const int b = token / s.L, l = token - b * s.L;
-        const T* x = static_cast<const T*>(s.x) + b * s.sb + l * s.sl;
-        const T* g = static_cast<const T*>(s.dout) + b * s.gb + l * s.gl;
-        T* y = static_cast<T*>(s.y) + (static_cast<int64_t>(token) * s.H) * p.D;
+    for (int i = 0; i < V / 2; ++i) da[i] = db[i] = pair(0.0f, 0.0f);
+    // every lane makes the same number of rounds (the sums are warp-wide shuffles)
+    const int stride = s.blocks * kStep;
+    for (int base = 0; base < s.rows; base += stride) {
+        const int row = base + block * kStep + threadIdx.x / GROUP, known = min(row, s.rows - 1);
+        const RowAt at(s, known);
+        const T* x = static_cast<const T*>(s.x) + offset(s.x_linear, p.D, known, at, s.sb, s.sl, s.sh);
+        const T* g = static_cast<const T*>(s.dout) + offset(s.g_linear, p.D, known, at, s.gb, s.gl, s.gh);
+        Pair xa[V / 2], xb[V / 2], ga[V / 2], gb[V / 2];
+        load<T, V>(x + pc.a, xa);
+        load<T, V>(x + pc.b, xb);
+        load<T, V>(g + pc.a, ga);
+        load<T, V>(g + pc.b, gb);
         Angles<V, INTER> ang;
-        if (rot) ang.get(p.cos, p.sin, static_cast<int64_t>(position(p, s, b, l)) * (p.R / 2), a, c);
-        else ang.none();
-        constexpr int kPair = 2;  // heads in flight
-        for (int j0 = 0; j0 < kHeads; j0 += kPair) {
-            float xa[kPair][V], xc[kPair][V], ga[kPair][V], gc[kPair][V];
+        ang.get(p, p.R > 0 ? position(p, s, at) : 0, pc);
+        ang.template turn<-1>(ga, gb);
+        Pair sq = mul2(xa[0], xa[0]), dot = mul2(mul2(ga[0], wa[0]), xa[0]);
 #pragma unroll
-            for (int j = 0; j < kPair; ++j) {
-                const int h = min(h0 + j0 + j, s.H - 1);
-                load<T, V>(x + h * s.sh + a, xa[j]);
-                load<T, V>(x + h * s.sh + c, xc[j]);
-                load<T, V>(g + h * s.gh + a, ga[j]);
-                load<T, V>(g + h * s.gh + c, gc[j]);
+        for (int i = 1; i < V / 2; ++i) {
+            sq = fma2(xa[i], xa[i], sq);
+            dot = fma2(mul2(ga[i], wa[i]), xa[i], dot);
+        }
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            sq = fma2(xb[i], xb[i], sq);
+            dot = fma2(mul2(gb[i], wb[i]), xb[i], dot);
+        }
+        const float r = rsqrtf(fmaf(group_sum<GROUP>(lane < p.lanes ? both(sq) : 0.0f), p.inv_d, p.eps));
+        const float m = group_sum<GROUP>(lane < p.lanes ? both(dot) : 0.0f) * r * r * p.inv_d;  // mean(u xh) r, applied to x
+        if (row < s.rows && lane < p.lanes) {
+            const Pair r2 = pair(r, r), nm = pair(-m, -m);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                da[i] = fma2(ga[i], mul2(xa[i], r2), da[i]);
+                db[i] = fma2(gb[i], mul2(xb[i], r2), db[i]);
+                ga[i] = mul2(r2, fma2(xa[i], nm, mul2(ga[i], wa[i])));
+                gb[i] = mul2(r2, fma2(xb[i], nm, mul2(gb[i], wb[i])));
             }
-#pragma unroll
-            for (int j = 0; j < kPair; ++j) {
-                const bool live = item < s.items && lane < p.lanes && h0 + j0 + j < s.H;
-                ang.template turn<-1>(ga[j], gc[j]);
-                float sq = 0.0f, dot = 0.0f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    sq += xa[j][i] * xa[j][i] + xc[j][i] * xc[j][i];
-                    dot += ga[j][i] * wa[i] * xa[j][i] + gc[j][i] * wc[i] * xc[j][i];
-                }
-                sq = group_sum<GROUP>(lane < p.lanes ? sq : 0.0f);
-                dot = group_sum<GROUP>(lane < p.lanes ? dot : 0.0f);
-                const float r = rsqrtf(sq / p.D + p.eps);
-                const float m = dot * r * r / p.D;  // mean(u xh) r, applied to x
-                if (live) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        da[i] += ga[j][i] * (xa[j][i] * r);
-                        dc[i] += gc[j][i] * (xc[j][i] * r);
-                        ga[j][i] = r * (ga[j][i] * wa[i] - xa[j][i] * m);
-                        gc[j][i] = r * (gc[j][i] * wc[i] - xc[j][i] * m);
-                    }
-                    store<T, V>(y + static_cast<int64_t>(h0 + j0 + j) * p.D + a, ga[j]);
-                    store<T, V>(y + static_cast<int64_t>(h0 + j0 + j) * p.D + c, gc[j]);
-                }
-            }
+            T* y = static_cast<T*>(s.y) + static_cast<int64_t>(row) * p.D;
+            store<T, V>(y + pc.a, ga);
+            store<T, V>(y + pc.b, gb);
         }
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        joined[threadIdx.x * 2 * V + i] = da[i];
-        joined[threadIdx.x * 2 * V + V + i] = dc[i];
+    for (int i = 0; i < V / 2; ++i) {
+        unpair(da[i], joined[threadIdx.x * 2 * V + 2 * i], joined[threadIdx.x * 2 * V + 2 * i + 1]);
+        unpair(db[i], joined[threadIdx.x * 2 * V + V + 2 * i], joined[threadIdx.x * 2 * V + V + 2 * i + 1]);
     }
     __syncthreads();
-    // one thread per (lane, value): the groups' partials in order
+    // one thread per value of the lanes: the groups' sums in order
     for (int t = threadIdx.x; t < p.lanes * 2 * V; t += kBlock) {
         const int ln = t / (2 * V), i = t - ln * 2 * V;
         float sum = 0.0f;
-        for (int gidx = 0; gidx < kBlock / GROUP; ++gidx) sum += joined[(gidx * GROUP + ln) * 2 * V + i];
-        int la, lc;
-        bool lrot;
-        chunk_dims<V>(ln, p.D, p.R, la, lc, lrot);
-        s.part[static_cast<int64_t>(block) * p.D + (i < V ? la + i : lc + i - V)] = sum;
+        for (int n = 0; n < kStep; ++n) sum += joined[(n * GROUP + ln) * 2 * V + i];
+        const Pieces x = pieces_of<V>(ln, p);
+        s.part[static_cast<int64_t>(block) * p.D + (i < V ? x.a + i : x.b + i - V)] = sum;
     }
 }
 
-// Joins the blocks' weight gradients: one block per side, kBlock / 32 warps
-// each take every 8th block's row, then the warps' sums in order.
+// Joins the blocks' weight gradients: 32 dims per CTA, each of 32 warps takes
+// every 32nd block's row (eight loads in flight), then the warps' sums in order.
 template <typename T>
-__global__ void __launch_bounds__(kBlock) weight_gradient_kernel(const __grid_constant__ RopeParams p)
+__global__ void __launch_bounds__(1024) weight_gradient_kernel(const __grid_constant__ RopeParams p)
 {
-    __shared__ float sums[kBlock / 32][32];
+    __shared__ float sums[32][33];
     const Side& s = p.side[blockIdx.y];
     const int d = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
     wait_for_launches_before();
     float sum = 0.0f;
-    if (d < p.D)
-        for (int n = w; n < s.blocks; n += kBlock / 32) sum += s.part[static_cast<int64_t>(n) * p.D + d];
+    if (d < p.D) {
+#pragma unroll 8
+        for (int n = w; n < s.blocks; n += 32) sum += s.part[static_cast<int64_t>(n) * p.D + d];
+    }
     sums[w][threadIdx.x % 32] = sum;
     __syncthreads();
     if (w == 0 && d < p.D) {
         sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < kBlock / 32; ++n) sum += sums[n][threadIdx.x];
+        for (int n = 0; n < 32; ++n) sum += sums[n][threadIdx.x];
         static_cast<T*>(s.dw)[d] = from_float<T>(sum);
     }
 }
@@ -336,15 +401,16 @@ int check(const ww_qk_norm_rope_t& p, bool backward) noexcept
     if (p.R < 0 || p.R > p.D || p.R % 2 != 0 || p.P < 0 || !(p.eps >= 0.0f)) return WW_ERR_INVALID_SHAPE;
     if (p.q_pos_stride < 0 || p.k_pos_stride < 0) return WW_ERR_INVALID_SHAPE;
     if (p.D % 8 != 0 || p.R % 8 != 0 || p.D > 256) return WW_ERR_UNSUPPORTED;
-    const int64_t lim = int64_t{1} << 30;  // items and one grid step beyond them in 32 bits
+    const int64_t lim = int64_t{1} << 30;  // rows and one grid step beyond them in 32 bits
     const int64_t nq = i64(p.B) * p.Lq, nk = i64(p.B) * p.Lk;
-    if (nq > lim || nk > lim || nq * ((p.Hq + kHeads - 1) / kHeads) > lim || nk * ((p.Hk + kHeads - 1) / kHeads) > lim)
+    if (nq > lim || nk > lim || nq * (p.Hq) > lim || nk * (p.Hk) > lim)
         return WW_ERR_UNSUPPORTED;
     const bool any = nq > 0 || nk > 0;
     if (p.R > 0 && any && (p.P == 0 || p.cos == nullptr || p.sin == nullptr))
         return p.P == 0 ? WW_ERR_INVALID_SHAPE : WW_ERR_NULL_POINTER;
     const int es = elem_size(p.dtype);
     const auto off = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 != 0; };
+    if (any && (off(p.cos) || off(p.sin))) return WW_ERR_MISALIGNED;
     if (nq > 0) {
         if (p.q == nullptr || p.q_weight == nullptr || (backward ? p.dq == nullptr || p.dq_out == nullptr : p.q_out == nullptr))
             return WW_ERR_NULL_POINTER;
@@ -363,17 +429,17 @@ int check(const ww_qk_norm_rope_t& p, bool backward) noexcept
     return WW_SUCCESS;
 }
 
-// Dims per lane and chunk: 16-byte loads where both halves split into them,
-// else 4 values.  Lanes per head are then D / (2 V).
-int chunk_values(const ww_qk_norm_rope_t& p)
+// Values of a lane's piece: 16 bytes where both halves split into them, else 4.
+int piece_values(const ww_qk_norm_rope_t& p)
 {
     if (p.dtype == WW_DTYPE_FLOAT) return 4;
     return p.R % 16 == 0 && p.D % 16 == 0 ? 8 : 4;
 }
 
+// Lanes of a row: the power of two that holds its pieces, two a lane.
 int group_lanes(const ww_qk_norm_rope_t& p)
 {
-    const int lanes = p.D / (2 * chunk_values(p));
+    const int lanes = p.D / (2 * piece_values(p));
     int g = 1;
     while (g < lanes) g *= 2;
     return g;
@@ -388,7 +454,8 @@ void fill(const ww_qk_norm_rope_t& p, bool backward, RopeParams* out) noexcept
     r.R = p.R;
     r.P = p.P;
     r.eps = p.eps;
-    r.lanes = p.D / (2 * chunk_values(p));
+    r.inv_d = 1.0f / p.D;
+    r.lanes = p.D / (2 * piece_values(p));
     const int per_block = kBlock / group_lanes(p);
     for (int i = 0; i < 2; ++i) {
         Side& s = r.side[i];
@@ -403,12 +470,25 @@ void fill(const ww_qk_norm_rope_t& p, bool backward, RopeParams* out) noexcept
         s.sb = st[0]; s.sl = st[1]; s.sh = st[2];
         s.gb = gs[0]; s.gl = gs[1]; s.gh = gs[2];
         s.pos_stride = i ? p.k_pos_stride : p.q_pos_stride;
-        s.L = i ? p.Lk : p.Lq;
-        s.H = i ? p.Hk : p.Hq;
-        s.chunks = (s.H + kHeads - 1) / kHeads;
-        s.items = static_cast<int32_t>(i64(p.B) * s.L * s.chunks);
-        const int need = (s.items + per_block - 1) / per_block;
-        s.blocks = backward ? (need < kMaxPartBlocks ? need : kMaxPartBlocks) : need;
+        const int L = i ? p.Lk : p.Lq, H = i ? p.Hk : p.Hq;
+        s.L = make_divisor(L > 0 ? L : 1);
+        s.H = make_divisor(H);
+        // strides of dims with one element do not matter
+        const auto linear = [&](int64_t sb, int64_t sl, int64_t sh) {
+            return (H == 1 || sh == p.D) && (L == 1 || sl == i64(H) * p.D) && (p.B == 1 || sb == i64(L) * H * p.D);
+        };
+        s.x_linear = linear(s.sb, s.sl, s.sh);
+        s.g_linear = linear(s.gb, s.gl, s.gh);
+        s.rows = static_cast<int32_t>(i64(p.B) * L * H);
+        s.blocks = (s.rows + per_block - 1) / per_block;
+    }
+    if (backward) {
+        // one round of resident blocks, shared between the sides by their rows
+        const int all = kSms * backward_blocks(piece_values(p));
+        const int64_t total = i64(r.side[0].rows) + r.side[1].rows;
+        for (Side& s : r.side)
+            if (s.rows > 0)
+                s.blocks = static_cast<int>(std::min<int64_t>(s.blocks, std::max<int64_t>(1, all * i64(s.rows) / total)));
     }
     r.side[0].part = static_cast<float*>(p.workspace);
     r.side[1].part = r.side[0].part + static_cast<int64_t>(r.side[0].blocks) * p.D;
@@ -427,7 +507,7 @@ int launch(const RopeParams& r, bool inter, bool backward, cudaStream_t stream) 
             else qk_norm_rope_backward_kernel<T, V, GROUP, false><<<blocks, kBlock, 0, stream>>>(r);
         }
     }
-    if (backward) launch_behind(weight_gradient_kernel<T>, dim3((r.D + 31) / 32, 2), dim3(kBlock), 0, stream, r);
+    if (backward) launch_behind(weight_gradient_kernel<T>, dim3((r.D + 31) / 32, 2), dim3(1024), 0, stream, r);
     return launch_status(backward ? "qk_norm_rope_backward" : "qk_norm_rope");
 }
 
@@ -451,7 +531,7 @@ int launch_type(const ww_qk_norm_rope_t& p, bool backward, cudaStream_t stream) 
     fill(p, backward, &r);
     const int group = group_lanes(p);
     if constexpr (sizeof(T) == 2)
-        if (chunk_values(p) == 8) return launch_group<T, 8>(r, group, p.interleaved != 0, backward, stream);
+        if (piece_values(p) == 8) return launch_group<T, 8>(r, group, p.interleaved != 0, backward, stream);
     return launch_group<T, 4>(r, group, p.interleaved != 0, backward, stream);
 }
 
