@@ -244,6 +244,10 @@ __device__ __forceinline__ void wait_for_launches_before()
 // Fills `out`; WW_SUCCESS or the status of rejected arguments (attention_host.cu).
 int make_buckets(int num_buckets, int max_distance, int bidirectional, int q_offset, RelBuckets* out) noexcept;
 
+// Parts for each of `rest` items that do not fill a round of `slots` CTAs, of
+// `tiles` steps each: the count whose rounds end soonest.
+int tail_splits(int rest, int slots, int64_t tiles) noexcept;
+
 // Checks the arguments that both directions of ww_cross_attention share.
 int check_attention(const ww_attention_t& p) noexcept;
 // What only the gradient needs: its pointers and `need` bytes of workspace.

@@ -11,13 +11,14 @@
 //   keys:     128 keys on the rows (S^T, dP^T), streaming 64 queries at a time
 //             over all query heads of the key head; dV and dK in TMEM
 //   queries:  128 queries on the rows, streaming 64 keys at a time; dQ in TMEM
-// The row operands are A operands in TMEM (in shared memory where the widest
-// accumulators leave no room: keys at D = 128), which keeps their re-reading for
+// The row operands are A operands in TMEM (in shared memory where the accumulators
+// leave no room: keys at D = 128), which keeps their re-reading for
 // every tile off the shared memory; each streamed tile is the K-major B operand
 // of the two score products and, unchanged, the MN-major B operand of the
 // accumulating ones; P and dS return to TMEM over S and dP as A operands.  Two
-// tiles are under way, each with two warpgroups of elementwise work (32 of its 64
-// columns each).
+// tiles are under way on an SM, each with two warpgroups of elementwise work (32 of
+// its 64 columns each): of two CTAs, whose starts and ends overlap as well, or of
+// one where the accumulators take half of TMEM.
 //
 // 16-bit ranges: P is kept as 2^6 P, and in fp16 dS is formed from dO 2^e with
 // 2^e max|dO| in [1, 2): gradients as small as a mean over a batch leaves
@@ -43,9 +44,6 @@ constexpr int kRows = 128;
 constexpr int kCols = 64;
 constexpr int kShift = 6;         // P is kept times 2^kShift
 constexpr int kPitch = 33;        // floats of a dS row in shared memory
-constexpr int kGroups = 4;        // warpgroups: two per streamed tile
-constexpr int kThreads = kGroups * 128 + 64;
-constexpr int kMmaWarp = kGroups * 4, kLoadWarp = kMmaWarp + 1;
 
 struct BwdParams {
     CUtensorMap q, k, v, dout;  // boxes of 64 tokens
@@ -73,6 +71,15 @@ struct BwdParams {
 
 template <int DP, bool KEYS>
 struct Layout {
+    // tiles under way: two in one CTA of an SM, or one in each of two.  Two CTAs need
+    // TMEM for their accumulators and, to be fast, for their row operands twice:
+    // keys at D = 64, 1200 x 1777 tokens, 4 x 16 heads: one CTA 61 us, two with the row
+    // operands in shared memory 112 us; rows of 320, 3 heads of 32: 195 and 143 us.
+    static constexpr int kTiles = DP >= (KEYS ? 64 : 128) ? 2 : 1;
+    static constexpr int kCtas = 2 / kTiles;
+    static constexpr int kGroups = 2 * kTiles;         // warpgroups: two per tile
+    static constexpr int kThreads = kGroups * 128 + 64;
+    static constexpr int kMmaWarp = kGroups * 4, kLoadWarp = kMmaWarp + 1;
     static constexpr bool kRowsInTmem = !(KEYS && DP == 128);
     static constexpr int kRow = DP == 32 ? 64 : 128;   // bytes of an operand row
     static constexpr int kVals = kRow / 2;
@@ -81,42 +88,44 @@ struct Layout {
     static constexpr int kRowBytes = kRows * DP * 2;
     static constexpr int kColChunk = kCols * kRow;     // streamed operand
     static constexpr int kColBytes = kCols * DP * 2;
-    static constexpr int kStages = DP == 128 ? 2 : 4;
+    static constexpr int kStages = DP == 128 ? 2 : 3;
     static constexpr int kC = kRowsInTmem ? 0 : 2 * kRowBytes;     // stages of C1, C2
     static constexpr int kVec = kC + kStages * 2 * kColBytes;      // KEYS: nlse2, ndelta of 64 queries per stage
     static constexpr int kBar = kVec + (KEYS ? kStages * 2 * kCols * 4 : 0);
     static constexpr int kBias = kBar + 256;                       // bias tables, see below
-    // TMEM columns: S of both tiles, dP of both, accumulators, row operands
-    static constexpr int kDp = 2 * kCols, kAcc1 = 4 * kCols, kAcc2 = kAcc1 + DP, kR1 = kAcc1 + (KEYS ? 2 : 1) * DP,
-                         kR2 = kR1 + DP / 2;
-    static_assert(!kRowsInTmem || kR2 + DP / 2 <= 512, "TMEM");
+    // TMEM columns: S of the tiles, dP of the tiles, accumulators, row operands
+    static constexpr int kDp = kTiles * kCols, kAcc1 = 2 * kDp, kAcc2 = kAcc1 + DP, kR1 = kAcc1 + (KEYS ? 2 : 1) * DP,
+                         kR2 = kR1 + DP / 2, kColumns = 512 / kCtas;
+    static_assert(kR1 + (kRowsInTmem ? DP : 0) <= kColumns, "TMEM");
 };
 
 template <int DP, bool KEYS>
 struct Bars {
     static constexpr int kStages = Layout<DP, KEYS>::kStages;
-    uint64_t r_full, c_full[kStages], c_empty[kStages], s_full[2], p_ready[2], done;
+    uint64_t r_full, c_full[kStages], c_empty[kStages], s_full[Layout<DP, KEYS>::kTiles],
+        p_ready[Layout<DP, KEYS>::kTiles], done;
     uint32_t tmem;
 };
 
-// Shared memory after the barriers, with a bias (E = entries):
+// Shared memory after the barriers, with a bias (E = entries, W warpgroups):
 //   buckets  [E] bytes
-//   KEYS:    values [4 warpgroups][E] floats, rebuilt when the head changes
-//   queries: values [E], with the gradient's diagonals [4 warpgroups][E], plain
-//            sums [16 warps][kMaxBuckets] and dS [4][128][33]
-__host__ __device__ inline int bias_bytes(bool keys, int entries)
+//   KEYS:    values [W][E] floats, rebuilt when the head changes
+//   queries: values [E], with the gradient's diagonals [W][E], plain sums
+//            [4 W warps][buckets] and dS [W][128][33]
+__host__ __device__ inline int bias_bytes(bool keys, int groups, int entries, int buckets)
 {
     const int e = (entries + 15) / 16 * 16;
-    return keys ? e + kGroups * e * 4
-                : e + (1 + kGroups) * e * 4 + kGroups * 4 * kMaxBuckets * 4 + kGroups * kRows * kPitch * 4;
+    return keys ? e + groups * e * 4 : e + (1 + groups) * e * 4 + groups * 4 * buckets * 4 + groups * kRows * kPitch * 4;
 }
 
 template <typename T, int DP, bool KEYS, bool BIAS>
-__global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const __grid_constant__ BwdParams p)
+__global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::kCtas)
+    attention_backward_kernel(const __grid_constant__ BwdParams p)
 {
     using L = Layout<DP, KEYS>;
     using Bar = Bars<DP, KEYS>;
-    constexpr int S = L::kStages;
+    constexpr int S = L::kStages, NT = L::kTiles, kGroups = L::kGroups, kThreads = L::kThreads, kMmaWarp = L::kMmaWarp,
+                  kLoadWarp = L::kLoadWarp;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     extern __shared__ uint8_t raw[];
     uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
@@ -158,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                 if (!KEYS) values[e] = bias_value<T>(table[bu]) * kLog2eF;
             }
         if (!KEYS)  // diagonals, then plain sums
-            for (int e = threadIdx.x; e < kGroups * entries + kGroups * 4 * kMaxBuckets; e += kThreads)
+            for (int e = threadIdx.x; e < kGroups * entries + kGroups * 4 * p.rel.total; e += kThreads)
                 values[entries + e] = 0.0f;
     }
     if (warp == kLoadWarp && lane == 0) {
@@ -167,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             umma::mbar_init(at(bar->c_full[s]), 1);
             umma::mbar_init(at(bar->c_empty[s]), 1);
         }
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < NT; ++s) {
             umma::mbar_init(at(bar->s_full[s]), 1);
             umma::mbar_init(at(bar->p_ready[s]), 8);  // one arrival per warp
         }
@@ -175,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         umma::mbar_fence_init();
         umma::fence_proxy_async_smem();
     }
-    if (warp == kMmaWarp) umma::tmem_alloc(umma::smem_addr(&bar->tmem), 512);
+    if (warp == kMmaWarp) umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
@@ -240,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             const uint64_t a_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kC, L::kColChunk);
             const auto scores = [&](int i) {
                 const uint64_t cd = umma::desc_advance(c_desc, i % S * 2 * L::kColBytes);
-                const uint32_t to = tm + (i & 1) * kCols;
+                const uint32_t to = tm + i % NT * kCols;
                 if (umma::elect_one()) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
@@ -256,22 +265,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                                                                                 j * 16 % L::kVals * 2),
                                                  bd, id_s, j > 0);
                         }
-                    umma::mma_commit(at(bar->s_full[i & 1]));
+                    umma::mma_commit(at(bar->s_full[i % NT]));
                 }
                 __syncwarp();
             };
             bool ok = umma::mbar_poll(at(bar->r_full), 0);
             umma::fence_after_sync();
-            for (int i = 0; i < 2 && i < n && ok; ++i) {
+            for (int i = 0; i < NT && i < n && ok; ++i) {
                 ok = umma::mbar_poll(at(bar->c_full[i]), 0);
                 if (ok) scores(i);
             }
             for (int i = 0; i < n && ok; ++i) {
-                ok = umma::mbar_poll(at(bar->p_ready[i & 1]), (i >> 1) & 1);
+                ok = umma::mbar_poll(at(bar->p_ready[i % NT]), (i / NT) & 1);
                 if (!ok) break;
                 umma::fence_after_sync();
                 const uint64_t ad = umma::desc_advance(a_desc, i % S * 2 * L::kColBytes);
-                const uint32_t from = tm + (i & 1) * kCols;
+                const uint32_t from = tm + i % NT * kCols;
                 if (umma::elect_one()) {
 #pragma unroll
                     for (int j = 0; j < kCols / 16; ++j) {
@@ -286,15 +295,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                     if (i == n - 1) umma::mma_commit(at(bar->done));
                 }
                 __syncwarp();
-                if (i + 2 < n) {
-                    ok = umma::mbar_poll(at(bar->c_full[(i + 2) % S]), ((i + 2) / S) & 1);
-                    if (ok) scores(i + 2);
+                if (i + NT < n) {
+                    ok = umma::mbar_poll(at(bar->c_full[(i + NT) % S]), ((i + NT) / S) & 1);
+                    if (ok) scores(i + NT);
                 }
             }
             if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x31);
         }
     } else {
-        const int st = wg >> 1, half = wg & 1;  // tile of the pair, columns of it
+        const int st = wg >> 1, half = wg & 1;  // tile of those under way, columns of it
         const int r = threadIdx.x % 128, row = row0 + r;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;
         const uint32_t s_col = tmem + lanes + st * kCols, dp_col = s_col + L::kDp;
@@ -343,8 +352,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         const Pair scale_2 = pair(p.scale2, p.scale2), f_2 = pair(f, f), ndelta_2 = pair(my_ndelta, my_ndelta);
         int built = -1;  // KEYS: head of `values`
         float* diag = values + (1 + wg) * entries;
-        float* plain = values + (1 + kGroups) * entries + warp * kMaxBuckets;
-        float* tile = values + (1 + kGroups) * entries + kGroups * 4 * kMaxBuckets + wg * kRows * kPitch;
+        float* plain = values + (1 + kGroups) * entries + warp * p.rel.total;
+        float* tile = values + (1 + kGroups) * entries + kGroups * 4 * p.rel.total + wg * kRows * kPitch;
         if (BIAS && !KEYS && !any_row)
             for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;
         int ch = h, qt = first + st;  // tile i's head (KEYS) and its place along the streamed axis
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
             ch = h * group + (first + st) / p.q_tiles;
             qt = (first + st) % p.q_tiles;
         }
-        for (int i = st; i < n; i += 2) {
+        for (int i = st; i < n; i += NT) {
             const int s = i % S, col0 = qt * kCols + half * 32;
             uint32_t keep = ~0u;
             if (!KEYS) {
@@ -381,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                     mine = values + (KEYS ? row - col0 : col0 - row) - p.rel.q_offset - range.lo;
             }
             if (KEYS) ok = ok && umma::mbar_poll(at(bar->c_full[s]), (i / S) & 1);
-            ok = ok && umma::mbar_poll(at(bar->s_full[st]), (i >> 1) & 1);
+            ok = ok && umma::mbar_poll(at(bar->s_full[st]), (i / NT) & 1);
             umma::fence_after_sync();
             const float4* nlse = reinterpret_cast<const float4*>(base + L::kVec + s * 2 * kCols * 4) + half * 8;
             const float row_add = flat + (KEYS ? 0.0f : my_nlse);
@@ -491,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                     if (r < 31) to[r + 1] += run;
                 }
             }
-            qt += 2;
+            qt += NT;
             if (KEYS)
                 while (qt >= p.q_tiles) {
                     qt -= p.q_tiles;
@@ -501,12 +510,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
         if (n > 0) ok = ok && umma::mbar_poll(at(bar->done), 0);
         umma::fence_after_sync();
         if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x32);
-        // keys: warpgroups 0, 1 write the halves of dk, 2, 3 of dv; queries: each a quarter of dq
+        // the warpgroups share the accumulators' columns (keys: dk, then dv)
         const int rows_of = KEYS ? p.Lk : p.Lq;
-        const bool second = KEYS && wg >= 2;
+        constexpr int kSpan = (KEYS ? 2 : 1) * DP / kGroups;
+        const bool second = KEYS && wg >= kGroups / 2;
         const float mul = second ? 1.0f / (1 << kShift) : p.scale / (1 << kShift) / f;
-        constexpr int kSpan = KEYS ? DP / 2 : DP / 4;
-        const int begin = (KEYS ? half : wg) * kSpan;
+        const int begin = (KEYS ? wg % (kGroups / 2) : wg) * kSpan;
         const uint32_t acc = tmem + lanes + (second ? L::kAcc2 : L::kAcc1) + begin;
         T* to = static_cast<T*>(second ? p.d2 : p.d1) + ((static_cast<int64_t>(b) * rows_of + row) * heads + h) * p.D;
         float* part = p.part + (((static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (KEYS ? 2 : 1) + second) * kRows + r) * p.D;
@@ -542,10 +551,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
     __syncthreads();
     if (warp == kMmaWarp) {
         umma::fence_after_sync();
-        umma::tmem_dealloc(tmem, 512);
+        umma::tmem_dealloc(tmem, L::kColumns);
     }
     if (BIAS && !KEYS) {
-        // buckets of this CTA: each warp every 18th bucket, its lanes over the entries
+        // buckets of this CTA: warps take turns, their lanes run over the entries
         const float* diag = values + entries;
         const float* plain = values + (1 + kGroups) * entries;
         float f = 1.0f;
@@ -560,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_backward_kernel(const _
                 for (int e = lane; e < range.count(); e += 32)
                     if (buckets[e] == t)
                         for (int w = 0; w < kGroups; ++w) sum += diag[w * entries + e];
-            if (lane < kGroups * 4) sum += plain[lane * kMaxBuckets + t];
+            if (lane < kGroups * 4) sum += plain[lane * p.rel.total + t];
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
             if (lane == 0) to[t] = sum / (1 << kShift) / f;
         }
@@ -682,19 +691,19 @@ __global__ void __launch_bounds__(1024) attention_table_kernel(const float* part
     }
 }
 
-// How one of the two kernels runs: one CTA per SM, and the items that do not
-// fill a round of all SMs are split over their streamed tiles.
+// How one of the two kernels runs: the items that do not fill a round of the
+// GPU's CTAs (slots) are split over their streamed tiles.
 struct Half {
     int blocks, whole, rest, splits;
     int64_t ctas() const { return i64(whole) + i64(rest) * splits; }
 };
 
-Half make_half(int blocks, int64_t items, int64_t tiles, int sms) noexcept
+Half make_half(int blocks, int64_t items, int64_t tiles, int slots) noexcept
 {
     Half r;
     r.blocks = blocks;
-    r.rest = static_cast<int>(items % sms);
-    r.splits = r.rest == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms / r.rest, tiles / 4, 64})));
+    r.rest = static_cast<int>(items % slots);
+    r.splits = tail_splits(r.rest, slots, tiles);
     if (r.splits == 1) r.rest = 0;
     r.whole = static_cast<int>(items - r.rest);
     return r;
@@ -714,8 +723,9 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     r.Lq_pad = (p.Lq + kCols - 1) / kCols * kCols;
     const int64_t q_items = i64(q_blocks) * p.B * p.Hq, k_items = i64(k_blocks) * p.B * p.Hk;
     if (q_items > (1 << 30) || k_items > (1 << 30)) return false;
-    r.q = make_half(q_blocks, q_items, (p.Lk + kCols - 1) / kCols, sms);
-    r.k = make_half(k_blocks, k_items, i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), sms);
+    const int q_slots = sms * (p.D > 64 ? 1 : 2), k_slots = sms * (p.D > 32 ? 1 : 2);  // Layout::kCtas
+    r.q = make_half(q_blocks, q_items, (p.Lk + kCols - 1) / kCols, q_slots);
+    r.k = make_half(k_blocks, k_items, i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), k_slots);
     const int64_t rows = i64(p.B) * p.Hq * r.Lq_pad;
     const int64_t q_part = i64(r.q.rest) * r.q.splits * kRows * p.D * 4, k_part = i64(r.k.rest) * r.k.splits * 2 * kRows * p.D * 4;
     r.nlse2 = 256;
@@ -731,10 +741,10 @@ int launch_one(const BwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, KEYS>;
     const auto kernel = attention_backward_kernel<T, DP, KEYS, BIAS>;
-    const int bytes = 1024 + L::kBias + (BIAS ? bias_bytes(KEYS, f.max_entries) : 0);
+    const int bytes = 1024 + L::kBias + (BIAS ? bias_bytes(KEYS, L::kGroups, f.max_entries, f.rel.total) : 0);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
         return launch_status("cross_attention_backward");
-    kernel<<<static_cast<unsigned>(ctas), kThreads, bytes, stream>>>(f);
+    kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
     return launch_status("cross_attention_backward");
 }
 

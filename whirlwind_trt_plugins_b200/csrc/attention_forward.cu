@@ -566,7 +566,7 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     if (items > (1 << 30)) return false;
     const int slots = sms * (p.D > 64 ? 2 : 4) / r.nt;
     r.rest = static_cast<int>(items % slots);
-    r.splits = r.rest == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({slots / r.rest, tiles / 4, 64})));
+    r.splits = tail_splits(r.rest, slots, tiles);
     if (r.splits == 1) r.rest = 0;
     r.whole = static_cast<int>(items - r.rest);
     return true;

@@ -32,6 +32,23 @@ int make_buckets(int num_buckets, int max_distance, int bidirectional, int q_off
     return WW_SUCCESS;
 }
 
+int tail_splits(int rest, int slots, int64_t tiles) noexcept
+{
+    if (rest == 0) return 1;
+    // a CTA's start and end cost about 8 steps, joining parts about 6
+    constexpr double kStart = 8.0, kJoin = 6.0;
+    int best = 1;
+    double least = tiles + kStart;
+    for (int s = 2; s <= 64 && s * 4 <= tiles; ++s) {
+        const double time = static_cast<double>((i64(rest) * s + slots - 1) / slots) * (static_cast<double>(tiles) / s + kStart) + kJoin;
+        if (time < least) {
+            least = time;
+            best = s;
+        }
+    }
+    return best;
+}
+
 bool vectors_ok(const void* ptr, const int64_t (&strides)[3], int B, int L, int H, int elem_bytes) noexcept
 {
     if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return false;
