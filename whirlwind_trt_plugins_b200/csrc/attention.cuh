@@ -178,6 +178,21 @@ __host__ __device__ __forceinline__ RelRange rel_range(const RelBuckets& r, int 
     return g;
 }
 
+// Positions [lo, hi] of bucket t (empty where two edges coincide).
+__device__ __forceinline__ RelRange bucket_positions(const RelBuckets& r, int t)
+{
+    constexpr int kFar = 1 << 30;
+    const bool right = r.bidirectional && t >= r.per_side;
+    const int i = right ? t - r.per_side : t;
+    // distances [d0, d1]
+    const int d0 = i <= r.exact ? i : r.least[i - r.exact - 1];
+    const int d1 = i < r.exact ? i : i - r.exact < r.n_least ? r.least[i - r.exact] - 1 : kFar;
+    RelRange x;
+    x.lo = right ? max(d0, 1) : -d1;  // position 0 is on the left
+    x.hi = right ? d1 : !r.bidirectional && i == 0 ? kFar : -d0;
+    return x;
+}
+
 // Buckets of a range.  Ends without a barrier.
 __device__ __forceinline__ void build_buckets(const RelBuckets& r, const RelRange& g, uint8_t* to, int thread, int threads)
 {

@@ -44,6 +44,7 @@ constexpr int kRows = 128;
 constexpr int kCols = 64;
 constexpr int kShift = 6;         // P is kept times 2^kShift
 constexpr int kPitch = 33;        // floats of a dS row in shared memory
+constexpr int kTileRows = 160;    // 128, and copies of the first 32
 
 struct BwdParams {
     CUtensorMap q, k, v, dout;  // boxes of 64 tokens
@@ -91,7 +92,8 @@ struct Layout {
     static constexpr int kStages = DP == 128 ? 2 : 3;
     static constexpr int kC = kRowsInTmem ? 0 : 2 * kRowBytes;     // stages of C1, C2
     static constexpr int kVec = kC + kStages * 2 * kColBytes;      // KEYS: nlse2, ndelta of 64 queries per stage
-    static constexpr int kBar = kVec + (KEYS ? kStages * 2 * kCols * 4 : 0);
+    // queries: limits of 64 keys per stage, then flags
+    static constexpr int kBar = kVec + (KEYS ? kStages * 2 * kCols * 4 : kStages * (kCols + 4) * 4);
     static constexpr int kBias = kBar + 256;                       // bias tables, see below
     // TMEM columns: S of the tiles, dP of the tiles, accumulators, row operands
     static constexpr int kDp = kTiles * kCols, kAcc1 = 2 * kDp, kAcc2 = kAcc1 + DP, kR1 = kAcc1 + (KEYS ? 2 : 1) * DP,
@@ -102,7 +104,7 @@ struct Layout {
 template <int DP, bool KEYS>
 struct Bars {
     static constexpr int kStages = Layout<DP, KEYS>::kStages;
-    uint64_t r_full, c_full[kStages], c_empty[kStages], s_full[Layout<DP, KEYS>::kTiles],
+    uint64_t r_full, c_full[kStages], c_ready[kStages], c_empty[kStages], s_full[Layout<DP, KEYS>::kTiles],
         p_ready[Layout<DP, KEYS>::kTiles], done;
     uint32_t tmem;
 };
@@ -111,11 +113,11 @@ struct Bars {
 //   buckets  [E] bytes
 //   KEYS:    values [W][E] floats, rebuilt when the head changes
 //   queries: values [E], with the gradient's diagonals [W][E], plain sums
-//            [4 W warps][buckets] and dS [W][128][33]
+//            [4 W warps][buckets] and dS [W][160][33]
 __host__ __device__ inline int bias_bytes(bool keys, int groups, int entries, int buckets)
 {
     const int e = (entries + 15) / 16 * 16;
-    return keys ? e + groups * e * 4 : e + (1 + groups) * e * 4 + groups * 4 * buckets * 4 + groups * kRows * kPitch * 4;
+    return keys ? e + groups * e * 4 : e + (1 + groups) * e * 4 + groups * 4 * buckets * 4 + groups * kTileRows * kPitch * 4;
 }
 
 template <typename T, int DP, bool KEYS, bool BIAS>
@@ -174,6 +176,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         umma::mbar_init(at(bar->r_full), L::kRowsInTmem ? 8 : 1);
         for (int s = 0; s < S; ++s) {
             umma::mbar_init(at(bar->c_full[s]), 1);
+            umma::mbar_init(at(bar->c_ready[s]), 1);
             umma::mbar_init(at(bar->c_empty[s]), 1);
         }
         for (int s = 0; s < NT; ++s) {
@@ -189,14 +192,21 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = bar->tmem;
+    // queries with masked keys: the load warp clears their rows of K and V before a
+    // tile is used (its products then see zeros, whatever the places held) and
+    // leaves limits (0 or -inf) that join the scores
+    const bool masks = !KEYS && (p.key_mask != nullptr || len % kCols != 0);
+    float* limits = reinterpret_cast<float*>(base + L::kVec);
+    uint32_t* wholes = reinterpret_cast<uint32_t*>(limits + S * kCols);
+    const auto tile_bar = [&](int s) { return masks ? at(bar->c_ready[s]) : at(bar->c_full[s]); };
 
     if (warp == kLoadWarp) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             const CUtensorMap* c1 = KEYS ? &p.q : &p.k;
             const CUtensorMap* c2 = KEYS ? &p.dout : &p.v;
             const int c1b = KEYS ? p.q_b : p.k_b, c1h = KEYS ? p.q_h : p.k_h, c2b = KEYS ? p.g_b : p.v_b,
                       c2h = KEYS ? p.g_h : p.v_h;
-            if (!L::kRowsInTmem) {
+            if (!L::kRowsInTmem && lane == 0) {
                 // a half of the row tile that lies beyond the tensor reads as zeros like any other place outside
                 umma::mbar_arrive_expect_tx(at(bar->r_full), 2 * L::kRowBytes);
                 for (int half = 0; half < 2; ++half)
@@ -210,10 +220,10 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             }
             int ch = KEYS ? h * group + first / p.q_tiles : h / group, qt = KEYS ? first % p.q_tiles : first;
             bool ok = true;
-            for (int i = 0; i < n; ++i) {
+            const auto load = [&](int i) {  // lane 0
                 const int s = i % S;
-                ok = umma::mbar_poll(at(bar->c_empty[s]), (i / S + 1) & 1);
-                if (!ok) break;
+                ok = ok && umma::mbar_poll(at(bar->c_empty[s]), (i / S + 1) & 1);
+                if (!ok) return;
                 umma::mbar_arrive_expect_tx(at(bar->c_full[s]), 2 * L::kColBytes + (KEYS ? 2 * kCols * 4 : 0));
                 const uint32_t to = sm + L::kC + s * 2 * L::kColBytes;
                 const int l = qt * kCols;
@@ -234,8 +244,47 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                     qt = 0;
                     ++ch;
                 }
+            };
+            if (lane == 0)
+                for (int i = 0; i < S && i < n; ++i) load(i);
+            for (int i = 0; i < n; ++i) {
+                // the place of tile i - 1 is free once its products are done, which wait for
+                // tiles up to i - 1 + NT - 1 only: cleared below before this asks for it
+                if (lane == 0 && i > 0 && i - 1 + S < n && !masks) load(i - 1 + S);
+                if (!masks) continue;
+                const int s = i % S, k0 = (first + i) * kCols;
+                uint32_t in_mask = 0;
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    const int key = k0 + c + lane;
+                    if (key < len && (p.key_mask == nullptr || __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + key) != 0))
+                        in_mask |= 1u << (c / 32);
+                }
+                ok = __shfl_sync(~0u, ok, 0) && umma::mbar_poll(at(bar->c_full[s]), (i / S) & 1);
+                bool all = true;
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    const bool in = (in_mask >> (c / 32)) & 1;
+                    all = all && in;
+                    limits[s * kCols + c + lane] = in ? 0.0f : -INFINITY;
+                    if (!in) {
+                        const uint32_t to = sm + L::kC + s * 2 * L::kColBytes + (c + lane) * L::kRow;
+                        for (int x = 0; x < 2 * L::kChunks; ++x)
+#pragma unroll
+                            for (int j = 0; j < L::kRow; j += 16) umma::st_shared_v4(to + x * L::kColChunk + j, 0, 0, 0, 0);
+                    }
+                }
+                all = __all_sync(~0u, all);
+                if (lane == 0) wholes[s] = all;
+                umma::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    umma::mbar_arrive(at(bar->c_ready[s]));
+                    if (i > 0 && i - 1 + S < n) load(i - 1 + S);
+                }
+                __syncwarp();
             }
-            if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x30);
+            if (lane == 0 && !ok) record_device_error(p.err, kErrMbarTimeout | 0x30);
         }
     } else if (warp == kMmaWarp) {
         if (n > 0) {
@@ -272,7 +321,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             bool ok = umma::mbar_poll(at(bar->r_full), 0);
             umma::fence_after_sync();
             for (int i = 0; i < NT && i < n && ok; ++i) {
-                ok = umma::mbar_poll(at(bar->c_full[i]), 0);
+                ok = umma::mbar_poll(tile_bar(i), 0);
                 if (ok) scores(i);
             }
             for (int i = 0; i < n && ok; ++i) {
@@ -296,7 +345,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                 }
                 __syncwarp();
                 if (i + NT < n) {
-                    ok = umma::mbar_poll(at(bar->c_full[(i + NT) % S]), ((i + NT) / S) & 1);
+                    ok = umma::mbar_poll(tile_bar((i + NT) % S), ((i + NT) / S) & 1);
                     if (ok) scores(i + NT);
                 }
             }
@@ -347,15 +396,14 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             my_nlse = __ldg(p.nlse2 + i);
             my_ndelta = __ldg(p.ndelta + i) * f;
         }
-        const bool rows_ok = __all_sync(~0u, row_ok);
         const bool any_row = row0 + warp % 4 * 32 < (KEYS ? len : p.Lq);  // else this warp keeps the barriers only
         const Pair scale_2 = pair(p.scale2, p.scale2), f_2 = pair(f, f), ndelta_2 = pair(my_ndelta, my_ndelta);
         int built = -1;  // KEYS: head of `values`
         float* diag = values + (1 + wg) * entries;
         float* plain = values + (1 + kGroups) * entries + warp * p.rel.total;
-        float* tile = values + (1 + kGroups) * entries + kGroups * 4 * p.rel.total + wg * kRows * kPitch;
+        float* tile = values + (1 + kGroups) * entries + kGroups * 4 * p.rel.total + wg * kTileRows * kPitch;
         if (BIAS && !KEYS && !any_row)
-            for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;
+            for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;  // (never warp 0: its rows exist)
         int ch = h, qt = first + st;  // tile i's head (KEYS) and its place along the streamed axis
         if (KEYS) {
             ch = h * group + (first + st) / p.q_tiles;
@@ -363,13 +411,6 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         }
         for (int i = st; i < n; i += NT) {
             const int s = i % S, col0 = qt * kCols + half * 32;
-            uint32_t keep = ~0u;
-            if (!KEYS) {
-                const int left = len - col0;
-                keep = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-                if (p.key_mask != nullptr)
-                    keep &= __ballot_sync(~0u, lane < left && __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + col0 + lane) != 0);
-            }
             float flat = 0.0f;
             const float* mine = nullptr;  // bias of this row's first column
             int flat_bucket = 0;
@@ -389,7 +430,9 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                 else
                     mine = values + (KEYS ? row - col0 : col0 - row) - p.rel.q_offset - range.lo;
             }
-            if (KEYS) ok = ok && umma::mbar_poll(at(bar->c_full[s]), (i / S) & 1);
+            if (KEYS || masks) ok = ok && umma::mbar_poll(tile_bar(s), (i / S) & 1);  // its vectors or limits
+            const bool limited = masks && wholes[s] == 0;
+            const float4* lim = reinterpret_cast<const float4*>(limits + s * kCols) + half * 8;
             ok = ok && umma::mbar_poll(at(bar->s_full[st]), (i / NT) & 1);
             umma::fence_after_sync();
             const float4* nlse = reinterpret_cast<const float4*>(base + L::kVec + s * 2 * kCols * 4) + half * 8;
@@ -416,6 +459,12 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                         arg = add2(arg, j % 4 == 0 ? pair(a.x, a.y) : pair(a.z, a.w));
                         nd = j % 4 == 0 ? pair(e.x, e.y) : pair(e.z, e.w);
                     }
+                    if (!KEYS) {
+                        if (limited) {
+                            const float4 a = lim[c * 4 + j / 4];
+                            arg = add2(arg, j % 4 == 0 ? pair(a.x, a.y) : pair(a.z, a.w));
+                        }
+                    }
                     if (BIAS) {
                         if (mine != nullptr) {
                             const int at0 = c * 16 + j;
@@ -423,7 +472,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                         }
                     }
                     float p0, p1;
-                    if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe, where no argument is -inf
+                    if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe: 2^-126 for -inf, times rows of zeros
                         unpair(exp2_poly(arg), p0, p1);
                     } else {
                         unpair(arg, p0, p1);
@@ -437,19 +486,16 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                     else ds = mul2(pair(p0, p1), fma2(dp, f_2, nd));
                     float d0, d1;
                     unpair(ds, d0, d1);
-                    if (KEYS ? !rows_ok : keep != ~0u) {
-                        const bool in0 = KEYS ? row_ok : (keep >> (c * 16 + j)) & 1, in1 = KEYS ? row_ok : (keep >> (c * 16 + j + 1)) & 1;
-                        p0 = in0 ? p0 : 0.0f;
-                        p1 = in1 ? p1 : 0.0f;
-                        d0 = in0 ? d0 : 0.0f;
-                        d1 = in1 ? d1 : 0.0f;
-                    }
                     if (sums) {
                         if (mine == nullptr) {
                             total = add2(total, pair(d0, d1));
                         } else {
                             tile[r * kPitch + c * 16 + j] = d0;
                             tile[r * kPitch + c * 16 + j + 1] = d1;
+                            if (warp % 4 == 0) {
+                                tile[(128 + r) * kPitch + c * 16 + j] = d0;
+                                tile[(128 + r) * kPitch + c * 16 + j + 1] = d1;
+                            }
                         }
                     }
                     if (KEYS) pk[j / 2] = pack2<T>(p0, p1);
@@ -458,17 +504,6 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                 // over columns of this half of the tile only: the other half may not have been read
                 if (KEYS) umma::tmem_st8(s_col + half * 32 + c * 8, pk);
                 umma::tmem_st8(dp_col + half * 32 + c * 8, dk);
-            }
-            if (!KEYS && keep != ~0u) {
-                // rows of K behind masked keys: 0 in place of whatever they hold
-                ok = ok && umma::mbar_poll(at(bar->c_full[s]), (i / S) & 1);
-                if (r < 32 && !((keep >> lane) & 1)) {
-                    const uint32_t to = sm + L::kC + s * 2 * L::kColBytes + (half * 32 + r) * L::kRow;
-                    for (int c = 0; c < L::kChunks; ++c)
-#pragma unroll
-                        for (int j = 0; j < L::kRow; j += 16) umma::st_shared_v4(to + c * L::kColChunk + j, 0, 0, 0, 0);
-                }
-                umma::fence_proxy_async_smem();
             }
             umma::tmem_wait_st();
             umma::fence_before_sync();
@@ -483,21 +518,27 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                     if (lane == 0) plain[flat_bucket] += t0;
                 } else {
                     // sums along j - i: each thread a diagonal, column j of row
-                    // (j + 127 - r) mod 128: diagonal r - 127 until column r, r + 1
-                    // (r < 31) from there on
+                    // j + 127 - r; rows from 128 on are copies of rows 0 ..., so that
+                    // warp 0's threads pass from diagonal r - 127 to r + 1 (r < 31)
                     warpgroup_sync(wg);
-                    float run = 0.0f, first_part = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (j == r + 1) {
-                            first_part = run;
-                            run = 0.0f;
-                        }
-                        run += tile[((j + 127 - r) & 127) * kPitch + j];
-                    }
+                    const float* at0 = tile + (127 - r) * kPitch;
                     float* to = diag + col0 - row0 - p.rel.q_offset - range.lo;
-                    to[r - 127] += r < 31 ? first_part : run;
-                    if (r < 31) to[r + 1] += run;
+                    if (warp % 4 != 0) {
+                        float run[2] = {0.0f, 0.0f};
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) run[j & 1] += at0[j * (kPitch + 1)];
+                        to[r - 127] += run[0] + run[1];
+                    } else {
+                        float before = 0.0f, after = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float v = at0[j * (kPitch + 1)];
+                            before += j <= r ? v : 0.0f;
+                            after += j <= r ? 0.0f : v;
+                        }
+                        to[r - 127] += before;
+                        if (r < 31) to[r + 1] += after;
+                    }
                 }
             }
             qt += NT;
@@ -531,7 +572,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                 for (int j = 0; j < 8; ++j) o[j] = 0;
             }
             if (row >= rows_of || d0 >= p.D) continue;
-            if (KEYS && !row_ok) {  // a masked key: 0, whatever a skipped warp left in its lanes
+            if (KEYS && !row_ok) {  // a masked key: 0, whatever its rows held (rows do not mix)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = 0;
             }
@@ -554,7 +595,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         umma::tmem_dealloc(tmem, L::kColumns);
     }
     if (BIAS && !KEYS) {
-        // buckets of this CTA: warps take turns, their lanes run over the entries
+        // buckets of this CTA: warps take turns, their lanes run over a bucket's positions
         const float* diag = values + entries;
         const float* plain = values + (1 + kGroups) * entries;
         float f = 1.0f;
@@ -565,10 +606,11 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         float* to = p.table_part + static_cast<int64_t>(blk) * p.rel.total;
         for (int t = warp; t < p.rel.total; t += kThreads / 32) {
             float sum = 0.0f;
-            if (n > 0)
-                for (int e = lane; e < range.count(); e += 32)
-                    if (buckets[e] == t)
-                        for (int w = 0; w < kGroups; ++w) sum += diag[w * entries + e];
+            if (n > 0) {
+                const RelRange x = bucket_positions(p.rel, t);
+                for (int rel = max(x.lo, range.lo) + lane; rel <= min(x.hi, range.hi); rel += 32)
+                    for (int w = 0; w < kGroups; ++w) sum += diag[w * entries + rel - range.lo];
+            }
             if (lane < kGroups * 4) sum += plain[lane * p.rel.total + t];
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
             if (lane == 0) to[t] = sum / (1 << kShift) / f;
