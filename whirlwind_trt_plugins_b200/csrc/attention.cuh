@@ -178,6 +178,31 @@ __host__ __device__ __forceinline__ RelRange rel_range(const RelBuckets& r, int 
     return g;
 }
 
+// One head's table, spread over the lanes of a warp in log2 units: loaded early,
+// looked up by shuffles (all lanes together) instead of dependent loads.
+template <typename T>
+struct TableRow {
+    float v[kMaxBuckets / 32];
+    __device__ __forceinline__ void load(const RelBuckets& r, const void* table, int h, int lane)
+    {
+        const T* row = static_cast<const T*>(table) + static_cast<int64_t>(h) * r.total;
+#pragma unroll
+        for (int k = 0; k < kMaxBuckets / 32; ++k)
+            v[k] = lane + 32 * k < r.total ? bias_value<T>(row[lane + 32 * k]) * kLog2eF : 0.0f;
+    }
+    __device__ __forceinline__ float get(const RelBuckets& r, int bucket) const
+    {
+        float x = __shfl_sync(~0u, v[0], bucket & 31);
+#pragma unroll
+        for (int k = 1; k < kMaxBuckets / 32; ++k) {
+            if (32 * k >= r.total) break;  // the same for all
+            const float y = __shfl_sync(~0u, v[k], bucket & 31);
+            if (bucket >> 5 == k) x = y;
+        }
+        return x;
+    }
+};
+
 // Positions [lo, hi] of bucket t (empty where two edges coincide).
 __device__ __forceinline__ RelRange bucket_positions(const RelBuckets& r, int t)
 {

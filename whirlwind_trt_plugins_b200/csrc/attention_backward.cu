@@ -151,27 +151,32 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
 
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // warp-uniform: roles branch as warps
     const int wg = warp / 4;
-    RelRange range;
-    uint8_t* buckets = base + L::kBias;
-    float* values = nullptr;  // bias of [range]; KEYS: of this warpgroup's current head
-    const int entries = (p.max_entries + 15) / 16 * 16;
-    if (BIAS) {
-        // positions j - i - offset of the CTA's tiles, padded rows and columns included
-        range = KEYS ? rel_range(p.rel, row0 - (p.q_tiles * kCols - 1) - p.rel.q_offset, row0 + kRows - 1 - p.rel.q_offset)
-                     : rel_range(p.rel, first * kCols - (row0 + kRows - 1) - p.rel.q_offset,
-                                 (first + n) * kCols - 1 - row0 - p.rel.q_offset);
-        values = reinterpret_cast<float*>(base + L::kBias + entries) + (KEYS ? min(wg, kGroups - 1) * entries : 0);
-        const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
-        if (n > 0)
-            for (int e = threadIdx.x; e < range.count(); e += kThreads) {
-                const int bu = rel_bucket(p.rel, range.lo + e);
-                buckets[e] = static_cast<uint8_t>(bu);
-                if (!KEYS) values[e] = bias_value<T>(table[bu]) * kLog2eF;
-            }
-        if (!KEYS)  // diagonals, then plain sums
-            for (int e = threadIdx.x; e < kGroups * entries + kGroups * 4 * p.rel.total; e += kThreads)
-                values[entries + e] = 0.0f;
-    }
+    // the streamed tiles' next load: head (KEYS) and place along the streamed axis
+    int load_h = KEYS ? h * group + first / max(p.q_tiles, 1) : h / group, load_at = KEYS ? first % max(p.q_tiles, 1) : first;
+    const auto load = [&](int i) {  // one thread of the load warp
+        const int s = i % S;
+        umma::mbar_arrive_expect_tx(at(bar->c_full[s]), 2 * L::kColBytes + (KEYS ? 2 * kCols * 4 : 0));
+        const uint32_t to = sm + L::kC + s * 2 * L::kColBytes;
+        const int l = load_at * kCols;
+#pragma unroll
+        for (int c = 0; c < L::kChunks; ++c) {
+            umma::tma_load_4d(to + c * L::kColChunk, KEYS ? &p.q : &p.k, c * L::kVals, load_h * (KEYS ? p.q_h : p.k_h), l,
+                              b * (KEYS ? p.q_b : p.k_b), at(bar->c_full[s]));
+            umma::tma_load_4d(to + L::kColBytes + c * L::kColChunk, KEYS ? &p.dout : &p.v, c * L::kVals,
+                              load_h * (KEYS ? p.g_h : p.v_h), l, b * (KEYS ? p.g_b : p.v_b), at(bar->c_full[s]));
+        }
+        if (KEYS) {
+            const int64_t row = (static_cast<int64_t>(b) * p.Hq + load_h) * p.Lq_pad + l;
+            const uint32_t vec = sm + L::kVec + s * 2 * kCols * 4;
+            umma::bulk_g2s(vec, p.nlse2 + row, kCols * 4, at(bar->c_full[s]));
+            umma::bulk_g2s(vec + kCols * 4, p.ndelta + row, kCols * 4, at(bar->c_full[s]));
+        }
+        ++load_at;
+        if (KEYS && load_at == p.q_tiles) {
+            load_at = 0;
+            ++load_h;
+        }
+    };
     if (warp == kLoadWarp && lane == 0) {
         umma::mbar_init(at(bar->r_full), L::kRowsInTmem ? 8 : 1);
         for (int s = 0; s < S; ++s) {
@@ -186,6 +191,63 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         umma::mbar_init(at(bar->done), 1);
         umma::mbar_fence_init();
         umma::fence_proxy_async_smem();
+            if (n > 0) {
+            if (!L::kRowsInTmem) {
+                // a half of the row tile that lies beyond the tensor reads as zeros like any other place outside
+                umma::mbar_arrive_expect_tx(at(bar->r_full), 2 * L::kRowBytes);
+                for (int half = 0; half < 2; ++half)
+                    for (int c = 0; c < L::kChunks; ++c) {
+                        const uint32_t off = c * L::kRowChunk + half * L::kColChunk;
+                        const int l = min(row0 + half * kCols, p.Lk);
+                        umma::tma_load_4d(sm + off, &p.k, c * L::kVals, h * p.k_h, l, b * p.k_b, at(bar->r_full));
+                        umma::tma_load_4d(sm + L::kRowBytes + off, &p.v, c * L::kVals, h * p.v_h, l, b * p.v_b, at(bar->r_full));
+                    }
+            }
+            for (int i = 0; i < S && i < n; ++i) load(i);
+        }
+    }
+    // row operands: warpgroup 0 takes the first, 1 the second, a row per thread; on their way
+    // while the rest is set up
+    uint32_t rows[L::kRowsInTmem ? DP / 2 : 1];
+    if (L::kRowsInTmem && wg < 2 && n > 0) {
+        const int row = row0 + threadIdx.x % 128;
+        const int64_t* stride = wg == 0 ? p.r1_strides : p.r2_strides;
+        const T* from = static_cast<const T*>(wg == 0 ? p.r1 : p.r2) + b * stride[0] + row * stride[1] + h * stride[2];
+        const bool live = row < (KEYS ? p.Lk : p.Lq);
+#pragma unroll
+        for (int c = 0; c < DP; c += 8) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (live && c < p.D) u = __ldg(reinterpret_cast<const uint4*>(from + c));
+            if (L::kRowsInTmem) {
+                rows[c / 2] = u.x;
+                rows[c / 2 + 1] = u.y;
+                rows[c / 2 + 2] = u.z;
+                rows[c / 2 + 3] = u.w;
+            }
+        }
+    }
+    RelRange range;
+    uint8_t* buckets = base + L::kBias;
+    float* values = nullptr;  // bias of [range]; KEYS: of this warpgroup's current head
+    const int entries = (p.max_entries + 15) / 16 * 16;
+    if (BIAS) {
+        // positions j - i - offset of the CTA's tiles, padded rows and columns included
+        range = KEYS ? rel_range(p.rel, row0 - (p.q_tiles * kCols - 1) - p.rel.q_offset, row0 + kRows - 1 - p.rel.q_offset)
+                     : rel_range(p.rel, first * kCols - (row0 + kRows - 1) - p.rel.q_offset,
+                                 (first + n) * kCols - 1 - row0 - p.rel.q_offset);
+        values = reinterpret_cast<float*>(base + L::kBias + entries) + (KEYS ? min(wg, kGroups - 1) * entries : 0);
+        if (n > 0) {
+            TableRow<T> table;
+            if (!KEYS) table.load(p.rel, p.table, h, lane);
+            for (int e0 = warp * 32; e0 < range.count(); e0 += kThreads) {
+                const int e = min(e0 + lane, range.count() - 1), bu = rel_bucket(p.rel, range.lo + e);
+                buckets[e] = static_cast<uint8_t>(bu);
+                if (!KEYS) values[e] = table.get(p.rel, bu);
+            }
+        }
+        if (!KEYS)  // diagonals, then plain sums
+            for (int e = threadIdx.x; e < kGroups * entries + kGroups * 4 * p.rel.total; e += kThreads)
+                values[entries + e] = 0.0f;
     }
     if (warp == kMmaWarp) umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
     umma::fence_before_sync();
@@ -202,55 +264,16 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
 
     if (warp == kLoadWarp) {
         if (n > 0) {
-            const CUtensorMap* c1 = KEYS ? &p.q : &p.k;
-            const CUtensorMap* c2 = KEYS ? &p.dout : &p.v;
-            const int c1b = KEYS ? p.q_b : p.k_b, c1h = KEYS ? p.q_h : p.k_h, c2b = KEYS ? p.g_b : p.v_b,
-                      c2h = KEYS ? p.g_h : p.v_h;
-            if (!L::kRowsInTmem && lane == 0) {
-                // a half of the row tile that lies beyond the tensor reads as zeros like any other place outside
-                umma::mbar_arrive_expect_tx(at(bar->r_full), 2 * L::kRowBytes);
-                for (int half = 0; half < 2; ++half)
-                    for (int c = 0; c < L::kChunks; ++c) {
-                        const uint32_t off = c * L::kRowChunk + half * L::kColChunk;
-                        const int l = min(row0 + half * kCols, p.Lk);
-                        umma::tma_load_4d(sm + off, &p.k, c * L::kVals, h * p.k_h, l, b * p.k_b, at(bar->r_full));
-                        umma::tma_load_4d(sm + L::kRowBytes + off, &p.v, c * L::kVals, h * p.v_h, l, b * p.v_b,
-                                          at(bar->r_full));
-                    }
-            }
-            int ch = KEYS ? h * group + first / p.q_tiles : h / group, qt = KEYS ? first % p.q_tiles : first;
             bool ok = true;
-            const auto load = [&](int i) {  // lane 0
-                const int s = i % S;
-                ok = ok && umma::mbar_poll(at(bar->c_empty[s]), (i / S + 1) & 1);
-                if (!ok) return;
-                umma::mbar_arrive_expect_tx(at(bar->c_full[s]), 2 * L::kColBytes + (KEYS ? 2 * kCols * 4 : 0));
-                const uint32_t to = sm + L::kC + s * 2 * L::kColBytes;
-                const int l = qt * kCols;
-#pragma unroll
-                for (int c = 0; c < L::kChunks; ++c) {
-                    umma::tma_load_4d(to + c * L::kColChunk, c1, c * L::kVals, ch * c1h, l, b * c1b, at(bar->c_full[s]));
-                    umma::tma_load_4d(to + L::kColBytes + c * L::kColChunk, c2, c * L::kVals, ch * c2h, l, b * c2b,
-                                      at(bar->c_full[s]));
-                }
-                if (KEYS) {
-                    const int64_t row = (static_cast<int64_t>(b) * p.Hq + ch) * p.Lq_pad + l;
-                    const uint32_t vec = sm + L::kVec + s * 2 * kCols * 4;
-                    umma::bulk_g2s(vec, p.nlse2 + row, kCols * 4, at(bar->c_full[s]));
-                    umma::bulk_g2s(vec + kCols * 4, p.ndelta + row, kCols * 4, at(bar->c_full[s]));
-                }
-                ++qt;
-                if (KEYS && qt == p.q_tiles) {
-                    qt = 0;
-                    ++ch;
-                }
+            // tile i's place is free once its products are done, which wait for the tiles
+            // up to i + NT - 1: all of them loaded (and cleared) before this waits for it
+            const auto next = [&](int i) {
+                if (lane != 0 || i < 0 || i + S >= n || !ok) return;
+                ok = umma::mbar_poll(at(bar->c_empty[i % S]), (i / S) & 1);
+                if (ok) load(i + S);
             };
-            if (lane == 0)
-                for (int i = 0; i < S && i < n; ++i) load(i);
             for (int i = 0; i < n; ++i) {
-                // the place of tile i - 1 is free once its products are done, which wait for
-                // tiles up to i - 1 + NT - 1 only: cleared below before this asks for it
-                if (lane == 0 && i > 0 && i - 1 + S < n && !masks) load(i - 1 + S);
+                if (!masks) next(i - 1);
                 if (!masks) continue;
                 const int s = i % S, k0 = (first + i) * kCols;
                 uint32_t in_mask = 0;
@@ -278,10 +301,8 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                 if (lane == 0) wholes[s] = all;
                 umma::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) {
-                    umma::mbar_arrive(at(bar->c_ready[s]));
-                    if (i > 0 && i - 1 + S < n) load(i - 1 + S);
-                }
+                if (lane == 0) umma::mbar_arrive(at(bar->c_ready[s]));
+                next(i - 1);
                 __syncwarp();
             }
             if (lane == 0 && !ok) record_device_error(p.err, kErrMbarTimeout | 0x30);
@@ -358,24 +379,9 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         const uint32_t s_col = tmem + lanes + st * kCols, dp_col = s_col + L::kDp;
         bool ok = true;  // once a wait has run out: no more waits, but every barrier is kept
         if (L::kRowsInTmem && wg < 2 && n > 0) {
-            // warpgroup 0 brings the first row operand to TMEM, 1 the second: two values a column
-            const int64_t* stride = wg == 0 ? p.r1_strides : p.r2_strides;
-            const T* from = static_cast<const T*>(wg == 0 ? p.r1 : p.r2) + b * stride[0] + row * stride[1] + h * stride[2];
-            const bool live = row < (KEYS ? p.Lk : p.Lq);
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-                uint32_t x[16];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (live && c + j * 8 < p.D) u = __ldg(reinterpret_cast<const uint4*>(from + c + j * 8));
-                    x[4 * j] = u.x;
-                    x[4 * j + 1] = u.y;
-                    x[4 * j + 2] = u.z;
-                    x[4 * j + 3] = u.w;
-                }
-                umma::tmem_st16(tmem + lanes + (wg == 0 ? L::kR1 : L::kR2) + c / 2, x);
-            }
+            for (int c = 0; c < (L::kRowsInTmem ? DP / 2 : 0); c += 16)
+                umma::tmem_st16(tmem + lanes + (wg == 0 ? L::kR1 : L::kR2) + c, rows + c);  // two values a column
             umma::tmem_wait_st();
             umma::fence_before_sync();
             __syncwarp();
@@ -415,10 +421,14 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             const float* mine = nullptr;  // bias of this row's first column
             int flat_bucket = 0;
             if (BIAS) {
-                const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(ch) * p.rel.total;
                 if (KEYS && built != ch) {
                     warpgroup_sync(wg);
-                    for (int e = r; e < range.count(); e += 128) values[e] = bias_value<T>(table[buckets[e]]) * kLog2eF;
+                    TableRow<T> table;
+                    table.load(p.rel, p.table, ch, lane);
+                    for (int e0 = warp % 4 * 32; e0 < range.count(); e0 += 128) {
+                        const int e = min(e0 + lane, range.count() - 1);
+                        values[e] = table.get(p.rel, buckets[e]);
+                    }
                     warpgroup_sync(wg);
                     built = ch;
                 }
@@ -595,25 +605,29 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         umma::tmem_dealloc(tmem, L::kColumns);
     }
     if (BIAS && !KEYS) {
-        // buckets of this CTA: warps take turns, their lanes run over a bucket's positions
+        // buckets of this CTA: 8 lanes run over a bucket's positions
         const float* diag = values + entries;
         const float* plain = values + (1 + kGroups) * entries;
-        float f = 1.0f;
+        float back = 1.0f / (1 << kShift);
         if (kHalf) {
             const int top = static_cast<int>(__ldg(p.top) >> 23);
-            if (top > 0 && top < 255) f = __int_as_float((254 - top) << 23);
+            if (top > 0 && top < 255) back *= __int_as_float(top << 23);  // 1 / f
         }
-        float* to = p.table_part + static_cast<int64_t>(blk) * p.rel.total;
-        for (int t = warp; t < p.rel.total; t += kThreads / 32) {
+        const int sub = lane % 8;
+        for (int t0 = warp * 4; t0 < p.rel.total; t0 += kThreads / 8) {
+            const int t = min(t0 + lane / 8, p.rel.total - 1);
             float sum = 0.0f;
             if (n > 0) {
                 const RelRange x = bucket_positions(p.rel, t);
-                for (int rel = max(x.lo, range.lo) + lane; rel <= min(x.hi, range.hi); rel += 32)
-                    for (int w = 0; w < kGroups; ++w) sum += diag[w * entries + rel - range.lo];
+                const int lo = max(x.lo, range.lo) - range.lo, hi = min(x.hi, range.hi) - range.lo;
+                for (int e = lo + sub; e <= hi; e += 8)
+#pragma unroll
+                    for (int w = 0; w < kGroups; ++w) sum += diag[w * entries + e];
             }
-            if (lane < kGroups * 4) sum += plain[lane * p.rel.total + t];
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            if (lane == 0) to[t] = sum / (1 << kShift) / f;
+#pragma unroll
+            for (int w = 0; w < kGroups * 4; w += 8) sum += plain[(w + sub) * p.rel.total + t];
+            for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            if (sub == 0 && t0 + lane / 8 < p.rel.total) p.table_part[static_cast<int64_t>(blk) * p.rel.total + t] = sum * back;
         }
     }
 }

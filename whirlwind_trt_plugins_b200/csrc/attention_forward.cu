@@ -228,11 +228,12 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     if (p.rel.per_side != 0 && n > 0) {
         range = rel_range(p.rel, first * KT - (q0 + NT * kTile - 1) - p.rel.q_offset,
                           (first + n) * KT - 1 - q0 - p.rel.q_offset);
-        const T* table = static_cast<const T*>(p.table) + static_cast<int64_t>(h) * p.rel.total;
-        for (int e = threadIdx.x; e < range.count(); e += L::kThreads) {
-            const int bu = rel_bucket(p.rel, range.lo + e);
+        TableRow<T> table;
+        table.load(p.rel, p.table, h, lane);
+        for (int e0 = warp * 32; e0 < range.count(); e0 += L::kThreads) {
+            const int e = min(e0 + lane, range.count() - 1), bu = rel_bucket(p.rel, range.lo + e);
             buckets[e] = static_cast<uint8_t>(bu);
-            values[e] = bias_value<T>(table[bu]) * kLog2eF;
+            values[e] = table.get(p.rel, bu);
         }
     }
     if (warp == NT * 4) umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
