@@ -28,7 +28,7 @@
 // each kernel against 8 D (dK, dV) and 6 D (dQ) clocks of products.
 //
 // dtable: a tile whose positions all lie in one bucket adds its plain sum.
-// Otherwise dS goes through shared memory 32 columns at a time; a thread sums
+// Otherwise dS goes through shared memory, rounded as for its product, 32 columns at a time; a thread sums
 // one diagonal j - i (one read and one add per value, no conflicts), diagonals
 // are collected per CTA and joined to buckets, CTAs and warpgroups in order.
 #include "attention.cuh"
@@ -43,7 +43,7 @@ namespace {
 constexpr int kRows = 128;
 constexpr int kCols = 64;
 constexpr int kShift = 6;         // P is kept times 2^kShift
-constexpr int kPitch = 33;        // floats of a dS row in shared memory
+constexpr int kPitch = 17;        // words (two 16-bit values) of a dS row in shared memory
 constexpr int kTileRows = 160;    // 128, and copies of the first 32
 
 struct BwdParams {
@@ -89,7 +89,8 @@ struct Layout {
     static constexpr int kRowBytes = kRows * DP * 2;
     static constexpr int kColChunk = kCols * kRow;     // streamed operand
     static constexpr int kColBytes = kCols * DP * 2;
-    static constexpr int kStages = DP == 128 ? 2 : 3;
+    // a place is free only when its tile's products are done: one more than tiles under way
+    static constexpr int kStages = KEYS && DP == 64 ? 4 : 3;
     static constexpr int kC = kRowsInTmem ? 0 : 2 * kRowBytes;     // stages of C1, C2
     static constexpr int kVec = kC + kStages * 2 * kColBytes;      // KEYS: nlse2, ndelta of 64 queries per stage
     // queries: limits of 64 keys per stage, then flags
@@ -113,7 +114,7 @@ struct Bars {
 //   buckets  [E] bytes
 //   KEYS:    values [W][E] floats, rebuilt when the head changes
 //   queries: values [E], with the gradient's diagonals [W][E], plain sums
-//            [4 W warps][buckets] and dS [W][160][33]
+//            [4 W warps][buckets] and dS [W][160][17] words
 __host__ __device__ inline int bias_bytes(bool keys, int groups, int entries, int buckets)
 {
     const int e = (entries + 15) / 16 * 16;
@@ -407,9 +408,10 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         int built = -1;  // KEYS: head of `values`
         float* diag = values + (1 + wg) * entries;
         float* plain = values + (1 + kGroups) * entries + warp * p.rel.total;
-        float* tile = values + (1 + kGroups) * entries + kGroups * 4 * p.rel.total + wg * kTileRows * kPitch;
+        uint32_t* tile = reinterpret_cast<uint32_t*>(values + (1 + kGroups) * entries + kGroups * 4 * p.rel.total) +
+                         wg * kTileRows * kPitch;
         if (BIAS && !KEYS && !any_row)
-            for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;  // (never warp 0: its rows exist)
+            for (int j = 0; j < 16; ++j) tile[r * kPitch + j] = 0;  // (never warp 0: its rows exist)
         int ch = h, qt = first + st;  // tile i's head (KEYS) and its place along the streamed axis
         if (KEYS) {
             ch = h * group + (first + st) / p.q_tiles;
@@ -496,20 +498,13 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                     else ds = mul2(pair(p0, p1), fma2(dp, f_2, nd));
                     float d0, d1;
                     unpair(ds, d0, d1);
-                    if (sums) {
-                        if (mine == nullptr) {
-                            total = add2(total, pair(d0, d1));
-                        } else {
-                            tile[r * kPitch + c * 16 + j] = d0;
-                            tile[r * kPitch + c * 16 + j + 1] = d1;
-                            if (warp % 4 == 0) {
-                                tile[(128 + r) * kPitch + c * 16 + j] = d0;
-                                tile[(128 + r) * kPitch + c * 16 + j + 1] = d1;
-                            }
-                        }
-                    }
+                    if (sums && mine == nullptr) total = add2(total, ds);
                     if (KEYS) pk[j / 2] = pack2<T>(p0, p1);
                     dk[j / 2] = pack2<T>(d0, d1);
+                    if (sums && mine != nullptr) {
+                        tile[r * kPitch + c * 8 + j / 2] = dk[j / 2];
+                        if (warp % 4 == 0) tile[(128 + r) * kPitch + c * 8 + j / 2] = dk[j / 2];
+                    }
                 }
                 // over columns of this half of the tile only: the other half may not have been read
                 if (KEYS) umma::tmem_st8(s_col + half * 32 + c * 8, pk);
@@ -531,18 +526,18 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                     // j + 127 - r; rows from 128 on are copies of rows 0 ..., so that
                     // warp 0's threads pass from diagonal r - 127 to r + 1 (r < 31)
                     warpgroup_sync(wg);
-                    const float* at0 = tile + (127 - r) * kPitch;
+                    const T* at0 = reinterpret_cast<const T*>(tile + (127 - r) * kPitch);
                     float* to = diag + col0 - row0 - p.rel.q_offset - range.lo;
                     if (warp % 4 != 0) {
                         float run[2] = {0.0f, 0.0f};
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) run[j & 1] += at0[j * (kPitch + 1)];
+                        for (int j = 0; j < 32; ++j) run[j & 1] += to_float(at0[j * (2 * kPitch + 1)]);
                         to[r - 127] += run[0] + run[1];
                     } else {
                         float before = 0.0f, after = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float v = at0[j * (kPitch + 1)];
+                            const float v = to_float(at0[j * (2 * kPitch + 1)]);
                             before += j <= r ? v : 0.0f;
                             after += j <= r ? 0.0f : v;
                         }
