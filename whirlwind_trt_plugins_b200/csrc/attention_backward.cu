@@ -36,6 +36,7 @@
 #include "umma.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ww {
 namespace {
@@ -452,63 +453,75 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             Pair total = pair(0.0f, 0.0f);
             const bool sums = BIAS && !KEYS;
             if (sums && mine != nullptr) warpgroup_sync(wg);  // the diagonals before have been read
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (!any_row) continue;
-                uint32_t x[16], d[16];
-                umma::tmem_ld16(s_col + half * 32 + c * 16, x);
-                umma::tmem_ld16(dp_col + half * 32 + c * 16, d);
-                umma::tmem_wait_ld16(x);
-                umma::tmem_wait_ld16(d);
-                uint32_t pk[8], dk[8];
+            // W: bias by position, M: limits; resolved outside the unrolled columns
+            const auto columns = [&](auto w, auto l) {
+                constexpr bool W = decltype(w)::value, M = decltype(l)::value;
                 const Pair add_2 = pair(row_add, row_add);
 #pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    Pair arg = fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, add_2);
-                    Pair nd = ndelta_2;
-                    if (KEYS) {
-                        const float4 a = nlse[c * 4 + j / 4], e = nlse[kCols / 4 + c * 4 + j / 4];
-                        arg = add2(arg, j % 4 == 0 ? pair(a.x, a.y) : pair(a.z, a.w));
-                        nd = j % 4 == 0 ? pair(e.x, e.y) : pair(e.z, e.w);
-                    }
-                    if (!KEYS) {
-                        if (limited) {
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t x[16], d[16], pk[8], dk[8];
+                    umma::tmem_ld16(s_col + half * 32 + c * 16, x);
+                    umma::tmem_ld16(dp_col + half * 32 + c * 16, d);
+                    umma::tmem_wait_ld16(x);
+                    umma::tmem_wait_ld16(d);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        Pair arg = fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, add_2);
+                        Pair nd = ndelta_2;
+                        if (KEYS) {
+                            const float4 a = nlse[c * 4 + j / 4], e = nlse[kCols / 4 + c * 4 + j / 4];
+                            arg = add2(arg, j % 4 == 0 ? pair(a.x, a.y) : pair(a.z, a.w));
+                            nd = j % 4 == 0 ? pair(e.x, e.y) : pair(e.z, e.w);
+                        }
+                        if (M) {
                             const float4 a = lim[c * 4 + j / 4];
                             arg = add2(arg, j % 4 == 0 ? pair(a.x, a.y) : pair(a.z, a.w));
                         }
-                    }
-                    if (BIAS) {
-                        if (mine != nullptr) {
-                            const int at0 = c * 16 + j;
-                            arg = add2(arg, KEYS ? pair(mine[-at0], mine[-at0 - 1]) : pair(mine[at0], mine[at0 + 1]));
+                        if (W) {
+                            const int k = c * 16 + j;
+                            arg = add2(arg, KEYS ? pair(mine[-k], mine[-k - 1]) : pair(mine[k], mine[k + 1]));
                         }
+                        float p0, p1;
+                        if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe: 2^-126 for -inf, times rows of zeros
+                            unpair(exp2_poly(arg), p0, p1);
+                        } else {
+                            unpair(arg, p0, p1);
+                            p0 = exp2_approx(p0);
+                            p1 = exp2_approx(p1);
+                        }
+                        const Pair dp = pair(f32(d[j]), f32(d[j + 1]));
+                        Pair ds;
+                        if (!kHalf) ds = mul2(pair(p0, p1), add2(dp, nd));
+                        else if (KEYS) ds = mul2(pair(p0, p1), mul2(add2(dp, nd), f_2));
+                        else ds = mul2(pair(p0, p1), fma2(dp, f_2, nd));
+                        if (BIAS && !KEYS && !W) total = add2(total, ds);
+                        float d0, d1;
+                        unpair(ds, d0, d1);
+                        if (KEYS) pk[j / 2] = pack2<T>(p0, p1);
+                        dk[j / 2] = pack2<T>(d0, d1);
                     }
-                    float p0, p1;
-                    if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe: 2^-126 for -inf, times rows of zeros
-                        unpair(exp2_poly(arg), p0, p1);
-                    } else {
-                        unpair(arg, p0, p1);
-                        p0 = exp2_approx(p0);
-                        p1 = exp2_approx(p1);
-                    }
-                    const Pair dp = pair(f32(d[j]), f32(d[j + 1]));
-                    Pair ds;
-                    if (!kHalf) ds = mul2(pair(p0, p1), add2(dp, nd));
-                    else if (KEYS) ds = mul2(pair(p0, p1), mul2(add2(dp, nd), f_2));
-                    else ds = mul2(pair(p0, p1), fma2(dp, f_2, nd));
-                    float d0, d1;
-                    unpair(ds, d0, d1);
-                    if (sums && mine == nullptr) total = add2(total, ds);
-                    if (KEYS) pk[j / 2] = pack2<T>(p0, p1);
-                    dk[j / 2] = pack2<T>(d0, d1);
-                    if (sums && mine != nullptr) {
-                        tile[r * kPitch + c * 8 + j / 2] = dk[j / 2];
-                        if (warp % 4 == 0) tile[(128 + r) * kPitch + c * 8 + j / 2] = dk[j / 2];
+                    // over columns of this half of the tile only: the other half may not have been read
+                    if (KEYS) umma::tmem_st8(s_col + half * 32 + c * 8, pk);
+                    umma::tmem_st8(dp_col + half * 32 + c * 8, dk);
+                    if (W && !KEYS) {
+                        uint32_t* to = tile + r * kPitch + c * 8;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) to[j] = dk[j];
+                        if (warp % 4 == 0)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) to[128 * kPitch + j] = dk[j];
                     }
                 }
-                // over columns of this half of the tile only: the other half may not have been read
-                if (KEYS) umma::tmem_st8(s_col + half * 32 + c * 8, pk);
-                umma::tmem_st8(dp_col + half * 32 + c * 8, dk);
+            };
+            if (any_row) {
+                using No = std::false_type;
+                if (!KEYS && limited) {
+                    if (BIAS && mine != nullptr) columns(std::integral_constant<bool, BIAS>{}, std::integral_constant<bool, !KEYS>{});
+                    else columns(No{}, std::integral_constant<bool, !KEYS>{});
+                } else {
+                    if (BIAS && mine != nullptr) columns(std::integral_constant<bool, BIAS>{}, No{});
+                    else columns(No{}, No{});
+                }
             }
             umma::tmem_wait_st();
             umma::fence_before_sync();
