@@ -34,6 +34,26 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 
+// Division of n < 2^31 by d, prepared on the host.
+struct Divisor {
+    uint32_t mul = 1;
+    int32_t shift = 0;
+    int32_t d = 1;
+    __device__ __forceinline__ int div(int n) const
+    {
+        return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+    }
+};
+
+inline Divisor make_divisor(int d)
+{
+    Divisor r;
+    r.d = d;
+    while ((int64_t{1} << r.shift) < d) ++r.shift;
+    r.mul = static_cast<uint32_t>(((((uint64_t{1} << r.shift) - d) << 32) / d) + 1);
+    return r;
+}
+
 // ---- pairs of floats: one instruction for two values ----
 
 struct Pair {
@@ -135,6 +155,7 @@ __host__ __device__ __forceinline__ int rel_bucket(const RelBuckets& r, int rel)
     // counted, not searched: every thread reads the same edges in the same
     // order (a search's constant-memory reads differ by thread and serialise)
     int n = 0;
+#pragma unroll 8
     for (int t = 0; t < r.n_least; ++t) n += r.least[t] <= d;
     return first + r.exact + n;
 }
@@ -279,6 +300,18 @@ inline cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, si
 __device__ __forceinline__ void wait_for_launches_before()
 {
     asm volatile("griddepcontrol.wait;" : : : "memory");
+}
+
+// Share [first, first + n) of part `split` of `splits` in `all` steps (a 64-bit
+// division is worth avoiding where there is one part).
+__device__ __forceinline__ void part_of(int all, int split, int splits, int& first, int& n)
+{
+    first = 0;
+    n = all;
+    if (splits > 1) {
+        first = static_cast<int>(static_cast<int64_t>(all) * split / splits);
+        n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - first;
+    }
 }
 
 // Fills `out`; WW_SUCCESS or the status of rejected arguments (attention_host.cu).

@@ -65,6 +65,7 @@ struct BwdParams {
     int64_t r1_strides[3], r2_strides[3];
     int32_t B, Lq, Lk, Hq, Hk, D, Lq_pad;
     int32_t blocks, whole_items, splits, q_tiles;
+    Divisor by_block, by_head;
     int32_t q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h;
     int32_t max_entries;  // relative positions a CTA keeps
     float scale, scale2;
@@ -143,13 +144,13 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
     const int split = in_parts ? (blk - p.whole_items) % p.splits : 0, splits = in_parts ? p.splits : 1;
     const int item = in_parts ? p.whole_items + (blk - p.whole_items) / p.splits : blk;
     const int heads = KEYS ? p.Hk : p.Hq, group = p.Hq / p.Hk;
-    const int block = item % p.blocks, h = item / p.blocks % heads, b = item / p.blocks / heads;
+    const int bh = p.by_block.div(item), block = item - bh * p.blocks, b = p.by_head.div(bh), h = bh - b * heads;
     const int row0 = block * kRows;
     const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
     // streamed tiles of this CTA
     const int n_all = KEYS ? (row0 < len ? group * p.q_tiles : 0) : (len + kCols - 1) / kCols;
-    const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / splits);
-    const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / splits) - first;
+    int first, n;
+    part_of(n_all, split, splits, first, n);
 
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // warp-uniform: roles branch as warps
     const int wg = warp / 4;
@@ -241,14 +242,14 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         if (n > 0) {
             TableRow<T> table;
             if (!KEYS) table.load(p.rel, p.table, h, lane);
-            for (int e0 = warp * 32; e0 < range.count(); e0 += kThreads) {
+            for (int e0 = warp * 32; warp < kGroups * 4 && e0 < range.count(); e0 += kGroups * 128) {  // the others have their own starts
                 const int e = min(e0 + lane, range.count() - 1), bu = rel_bucket(p.rel, range.lo + e);
                 buckets[e] = static_cast<uint8_t>(bu);
                 if (!KEYS) values[e] = table.get(p.rel, bu);
             }
         }
         if (!KEYS)  // diagonals, then plain sums
-            for (int e = threadIdx.x; e < kGroups * entries + kGroups * 4 * p.rel.total; e += kThreads)
+            for (int e = threadIdx.x; wg < kGroups && e < kGroups * entries + kGroups * 4 * p.rel.total; e += kGroups * 128)
                 values[entries + e] = 0.0f;
     }
     if (warp == kMmaWarp) umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
@@ -828,6 +829,8 @@ template <typename T, bool KEYS>
 int run_half(BwdParams& f, const Half& half, cudaStream_t stream) noexcept
 {
     f.blocks = half.blocks;
+    f.by_block = make_divisor(half.blocks > 0 ? half.blocks : 1);
+    f.by_head = make_divisor(KEYS ? f.Hk : f.Hq);
     f.whole_items = half.whole;
     f.splits = half.splits;
     const int st = launch<T, KEYS>(f, half.ctas(), stream);

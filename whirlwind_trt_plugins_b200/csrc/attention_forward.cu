@@ -68,6 +68,7 @@ struct FwdParams {
     RelBuckets rel;
     int32_t B, Lq, Lk, Hq, group, D;
     int32_t q_blocks, whole_items, splits;
+    Divisor by_block, by_head, by_group;
     int32_t q_b, q_h, k_b, k_h, v_b, v_h;  // 0 where the tensor is broadcast
     int32_t max_entries;                   // relative positions a CTA keeps
     float scale2;                          // scale * log2(e)
@@ -175,13 +176,14 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     const bool in_parts = blk >= p.whole_items;
     const int split = in_parts ? (blk - p.whole_items) % p.splits : 0, splits = in_parts ? p.splits : 1;
     const int item = in_parts ? p.whole_items + (blk - p.whole_items) / p.splits : blk;
-    const int qb = item % p.q_blocks, h = item / p.q_blocks % p.Hq, b = item / p.q_blocks / p.Hq, g = h / p.group;
+    const int bh = p.by_block.div(item), qb = item - bh * p.q_blocks, b = p.by_head.div(bh), h = bh - b * p.Hq,
+              g = p.by_group.div(h);
     const int q0 = qb * (NT * kTile);
     const int tiles = NT == 1 || q0 + kTile >= p.Lq ? 1 : 2;  // query tiles with rows
     const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
     const int n_all = (len + KT - 1) / KT;
-    const int first = static_cast<int>(static_cast<int64_t>(n_all) * split / splits);
-    const int n = static_cast<int>(static_cast<int64_t>(n_all) * (split + 1) / splits) - first;
+    int first, n;
+    part_of(n_all, split, splits, first, n);
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;  // warp-uniform: roles branch as warps
     // keys of a tile
     const auto cols_of = [&](int kt) { return min(KT, len - (first + kt) * KT); };
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                           (first + n) * KT - 1 - q0 - p.rel.q_offset);
         TableRow<T> table;
         table.load(p.rel, p.table, h, lane);
-        for (int e0 = warp * 32; e0 < range.count(); e0 += L::kThreads) {
+        for (int e0 = warp * 32; warp < NT * 4 && e0 < range.count(); e0 += NT * 128) {  // the other warps have their own starts
             const int e = min(e0 + lane, range.count() - 1), bu = rel_bucket(p.rel, range.lo + e);
             buckets[e] = static_cast<uint8_t>(bu);
             values[e] = table.get(p.rel, bu);
@@ -619,6 +621,9 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.group = p.Hq / p.Hk;
     f.D = p.D;
     f.q_blocks = plan.q_blocks;
+    f.by_block = make_divisor(plan.q_blocks);
+    f.by_head = make_divisor(p.Hq);
+    f.by_group = make_divisor(p.Hq / p.Hk);
     f.whole_items = plan.whole;
     f.splits = plan.splits;
     f.q_b = p.q_strides[0] != 0;

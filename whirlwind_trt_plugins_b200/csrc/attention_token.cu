@@ -113,8 +113,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attention_token_kernel(const _
     const int g = blockIdx.x / p.splits % p.Hk, b = blockIdx.x / p.splits / p.Hk;
     const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
     const int all = (len + kKeys - 1) / kKeys;
-    const int first = static_cast<int>(static_cast<int64_t>(all) * split / p.splits);
-    const int last = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits);
+    int first, count;
+    part_of(all, split, p.splits, first, count);
+    const int last = first + count;
     const int n = (last - first - warp + kWarps - 1) / kWarps;  // tiles of this warp: first + warp + kWarps i
     const int group = p.Hq / p.Hk;
 

@@ -38,26 +38,6 @@ constexpr int kForwardBlocks = 6;
 constexpr int backward_blocks(int V) { return V == 8 ? 3 : 4; }
 constexpr int kSms = 148;
 
-// Division of n < 2^31 by d, prepared on the host.
-struct Divisor {
-    uint32_t mul = 1;
-    int32_t shift = 0;
-    int32_t d = 1;
-    __device__ __forceinline__ int div(int n) const
-    {
-        return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
-    }
-};
-
-Divisor make_divisor(int d)
-{
-    Divisor r;
-    r.d = d;
-    while ((int64_t{1} << r.shift) < d) ++r.shift;
-    r.mul = static_cast<uint32_t>(((((uint64_t{1} << r.shift) - d) << 32) / d) + 1);
-    return r;
-}
-
 struct Side {
     const void* x;
     const void* w;
