@@ -61,8 +61,16 @@ typedef enum ww_status {
     WW_ERR_DEVICE = 7         /* no usable sm_100 device is current              */
 } ww_status_t;
 
-/* Same numeric values as nvinfer1::DataType::kFLOAT / kHALF / kINT8 / kBF16. */
-typedef enum ww_dtype { WW_DTYPE_FLOAT = 0, WW_DTYPE_HALF = 1, WW_DTYPE_INT8 = 2, WW_DTYPE_BF16 = 7 } ww_dtype_t;
+/* Same numeric values as nvinfer1::DataType's. */
+typedef enum ww_dtype {
+    WW_DTYPE_FLOAT = 0,
+    WW_DTYPE_HALF = 1,
+    WW_DTYPE_INT8 = 2,
+    WW_DTYPE_INT32 = 3,
+    WW_DTYPE_BOOL = 4,
+    WW_DTYPE_UINT8 = 5,
+    WW_DTYPE_BF16 = 7
+} ww_dtype_t;
 
 /* Activation of the generalised / fused stem. */
 typedef enum ww_act { WW_ACT_RELU = 0, WW_ACT_RELU6 = 1 } ww_act_t;
@@ -282,7 +290,8 @@ int ww_disparity_regression(const void* cost, void* out, int in_dtype, int out_d
  * Some calls need device scratch memory: the *_workspace functions return the
  * bytes (0: none) for the same parameters, the caller passes a 16-byte
  * aligned buffer of at least that size in `workspace` (else
- * WW_ERR_UNSUPPORTED).  Results do not depend on what it holds, and the same
+ * WW_ERR_UNSUPPORTED; ww_cross_attention alone also runs with NULL, without
+ * splitting its keys, which is slower for few rows against many keys).  Results do not depend on what it holds, and the same
  * call gives the same bits again.
  * ------------------------------------------------------------------------- */
 
@@ -460,6 +469,37 @@ int ww_plugin_disparity_regression_supports_format(int pos, const ww_tensor_desc
 int ww_plugin_disparity_regression_enqueue(int mode, const ww_tensor_desc_t* in_desc,
                                            const ww_tensor_desc_t* out_desc, const void* const* inputs,
                                            void* const* outputs, void* stream);
+
+/* "CrossAttention" v"1" (extension): ww_cross_attention with scale 1 / sqrt(D).
+ * Inputs q [B, Lq, Hq, D], k, v [B, Lk, Hk, D] (fp16 or bf16), then those that
+ * `flags` names, in this order: k_lens [B] int32, key_mask [B, Lk] bool or uint8,
+ * bias_table [Hq, num_buckets] (the type of q); output like q.  Fields
+ * use_lens, use_mask, use_bias (0), max_distance (128), bidirectional (1),
+ * q_offset (0).  `workspace` is NULL or WW_PLUGIN_ATTENTION_WORKSPACE bytes,
+ * whatever the shapes: a call that would need more runs without it. */
+#define WW_PLUGIN_ATTENTION_LENS 1
+#define WW_PLUGIN_ATTENTION_MASK 2
+#define WW_PLUGIN_ATTENTION_BIAS 4
+#define WW_PLUGIN_ATTENTION_WORKSPACE (64 << 20)
+int ww_plugin_cross_attention_output_dims(int flags, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                          ww_tensor_desc_t* out);
+int ww_plugin_cross_attention_supports_format(int flags, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                              int nb_outputs);
+int ww_plugin_cross_attention_enqueue(int flags, int max_distance, int bidirectional, int q_offset,
+                                      const ww_tensor_desc_t* in_desc, const void* const* inputs,
+                                      void* const* outputs, void* workspace, void* stream);
+
+/* "QkNormRope" v"1" (extension): ww_qk_norm_rope.  Inputs q [B, Lq, Hq, D],
+ * k [B, Lk, Hk, D], q_weight [D], k_weight [D] (one type: fp16, bf16 or fp32),
+ * cos, sin [P, R / 2] fp32 and with use_positions q_pos, k_pos int32 ([L] or
+ * [B, L]); two outputs like q and k.  Fields use_positions (0), interleaved (0),
+ * eps_nano (eps in 1e-9, default 1000). */
+int ww_plugin_qk_norm_rope_output_dims(int use_positions, int which, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                       ww_tensor_desc_t* out);
+int ww_plugin_qk_norm_rope_supports_format(int use_positions, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                           int nb_outputs);
+int ww_plugin_qk_norm_rope_enqueue(int use_positions, int eps_nano, int interleaved, const ww_tensor_desc_t* in_desc,
+                                   const void* const* inputs, void* const* outputs, void* stream);
 
 /* Device error word written by bounded waits inside the tensor-core kernels
  * (0 = none).  There is ONE word per device, shared by every call, stream and

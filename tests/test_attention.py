@@ -143,3 +143,42 @@ def test_wrappers_refuse_host_tensors():
         ww.cross_attention(x, x, x)
     with pytest.raises(TypeError):
         ww.qk_norm_rope(x, x, x[0, 0, 0], x[0, 0, 0], torch.zeros(2, 16), torch.zeros(2, 16))
+
+
+def test_plugins_shapes_formats_fields():
+    from whirlwind_trt_plugins_b200 import plugins as pl
+    T = pl.TensorDesc
+    cr = pl.get_plugin_creator("CrossAttention", "1")
+    p = cr.create_plugin({"use_lens": 1, "use_bias": 1, "q_offset": 3})
+    assert p.clone().get_fields_to_serialize() == {"use_lens": 1, "use_mask": 0, "use_bias": 1, "max_distance": 128,
+                                                   "bidirectional": 1, "q_offset": 3}
+    q, k, lens, table = T((2, 5, 8, 64)), T((2, 7, 4, 64)), T((2,), 3), T((8, 32))
+    assert p.get_output_shapes([q, k, k, lens, table]) == [(2, 5, 8, 64)]
+    for bad in ([q, k, k, lens], [q, k, T((2, 6, 4, 64)), lens, table], [q, T((2, 7, 3, 64))] + [T((2, 7, 3, 64)), lens, table],
+                [q, k, k, T((3,), 3), table], [q, k, k, lens, T((4, 32))]):
+        with pytest.raises(ValueError):
+            p.get_output_shapes(bad)
+    io = [q, k, k, lens, table, q]
+    assert all(p.supports_format_combination(i, io, 5, 1) for i in range(6))
+    assert not p.supports_format_combination(3, [q, k, k, T((2,), 1), table, q], 5, 1)
+    assert not p.supports_format_combination(0, [T((2, 5, 8, 64), 0)] + io[1:], 5, 1)
+    m = cr.create_plugin({"use_mask": 1})
+    assert m.supports_format_combination(3, [q, k, k, T((2, 7), 4), q], 4, 1)
+    assert m.get_workspace_size() == 64 << 20 and m.get_nb_outputs() == 1
+    # refused before any GPU work
+    assert p.enqueue([q, k, k, lens, T((4, 32))], [0] * 5, [0], stream=0) == 1
+    assert p.enqueue([q, k, k, lens, table], [0] * 5, [0], stream=0) == 1
+
+    cr = pl.get_plugin_creator("QkNormRope", "1")
+    r = cr.create_plugin({"use_positions": 1})
+    assert r.get_nb_outputs() == 2 and r.get_output_data_types([7] * 8) == [7, 7]
+    w, c = T((64,)), T((100, 16), 0)
+    ins = [q, k, w, w, c, c, T((5,), 3), T((2, 7), 3)]
+    assert r.get_output_shapes(ins) == [(2, 5, 8, 64), (2, 7, 4, 64)]
+    assert all(r.supports_format_combination(i, ins + [q, k], 8, 2) for i in range(10))
+    assert not r.supports_format_combination(4, [q, k, w, w, T((100, 16), 1)] + ins[5:] + [q, k], 8, 2)
+    with pytest.raises(ValueError):
+        r.get_output_shapes(ins[:6])
+    with pytest.raises(ValueError):
+        r.get_output_shapes(ins[:6] + [T((6,), 3), T((2, 7), 3)])
+    assert r.enqueue(ins, [0] * 8, [0, 0], stream=0) == 1

@@ -495,3 +495,50 @@ def test_refusals(env):
         ww.qk_norm_rope(q, k, w, w, cos, cos, q_pos=torch.zeros(3, device="cuda", dtype=torch.int32))
     with pytest.raises(ww.WWError):  # 12 rotated dims
         ww.qk_norm_rope(q, k, w, w, cos[:, :6].contiguous(), cos[:, :6].contiguous())
+
+
+def test_plugin_enqueue_and_calls_without_workspace(env):
+    """The plugins give the functions' bits; without a workspace the keys are not
+    split, which rounds differently but stays within the bounds."""
+    torch, ww = env
+    from whirlwind_trt_plugins_b200 import plugins as pl
+    T = pl.TensorDesc.of
+    a, kw, keep = _attention_case(torch, ww, 2, 3, 900, 8, 2, 64, "bf16", "lens keys", (32, 64, True, 5), 70)
+    p = pl.get_plugin_creator("CrossAttention").create_plugin(
+        {"use_lens": 1, "use_mask": 1, "use_bias": 1, "max_distance": 64, "q_offset": 5})
+    ins = [a["q"], a["k"], a["v"], kw["k_lens"], kw["key_mask"], kw["bias_table"]]
+    want = ww.cross_attention(a["q"], a["k"], a["v"], **kw)
+    ws = torch.empty(p.get_workspace_size(), dtype=torch.uint8, device="cuda")
+    out, plain = torch.empty_like(want), torch.empty_like(want)
+    assert p.enqueue([T(x) for x in ins], ins, [out], ws) == 0
+    assert p.enqueue([T(x) for x in ins], ins, [plain]) == 0
+    assert torch.equal(out, want)
+    ref, bounds = _attention_ref(torch, ww, a, kw, keep, 1 / 8)
+    _within(plain, ref["out"], bounds(U["bf16"], 0.0)["out"], "without workspace")
+    w = torch.ones(64, device="cuda", dtype=torch.bfloat16)
+    ang = torch.arange(900, device="cuda").float()[:, None] * torch.rand(32, device="cuda")
+    cos, sin = ang.cos(), ang.sin()
+    pos = torch.arange(3, device="cuda", dtype=torch.int32) + 5, torch.arange(900, device="cuda", dtype=torch.int32)
+    k = torch.randn((2, 900, 2, 64), device="cuda").bfloat16()
+    want = ww.qk_norm_rope(a["q"], k, w, w, cos, sin, *pos, eps=1e-6)
+    r = pl.get_plugin_creator("QkNormRope").create_plugin({"use_positions": 1})
+    ins = [a["q"], k, w, w, cos, sin, *pos]
+    outs = [torch.empty_like(x) for x in want]
+    assert r.enqueue([T(x) for x in ins], ins, outs) == 0
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_example_trains_and_matches():
+    """The matching layer of examples/: training lowers its loss, its features
+    give the rows' disparities through the volume and the regression."""
+    import importlib.util
+    import os
+
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("example", os.path.join(ROOT, "examples", "stereo_cross_attention.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    losses, error = m.main(steps=60, verbose=False)
+    assert all(map(math.isfinite, losses))
+    assert sum(losses[-5:]) < 0.9 * sum(losses[:5])
+    assert error < 2.0

@@ -546,6 +546,12 @@ struct Plan {
     int nt, q_blocks, whole, rest, splits, rows;
     int64_t part_rows() const { return i64(rest) * splits * rows; }
     int64_t part_bytes(int D) const { return part_rows() * (D + 1) * 4; }
+    void without_parts(const ww_attention_t& p)
+    {
+        splits = 1;
+        rest = 0;
+        whole = token ? 0 : static_cast<int>(i64(q_blocks) * p.B * p.Hq);
+    }
 };
 
 bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
@@ -683,8 +689,8 @@ int ww_cross_attention(const ww_attention_t* p, void* stream)
     if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
     ww::Plan plan;
     if (!ww::make_plan(*p, d.sm_count, &plan)) return WW_ERR_UNSUPPORTED;
-    if (plan.part_rows() > 0 && p->workspace == nullptr) return WW_ERR_NULL_POINTER;
-    if (plan.part_bytes(p->D) > p->workspace_bytes) return WW_ERR_UNSUPPORTED;
+    if (p->workspace == nullptr) plan.without_parts(*p);
+    else if (plan.part_bytes(p->D) > p->workspace_bytes) return WW_ERR_UNSUPPORTED;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return p->dtype == WW_DTYPE_HALF ? ww::forward<__half>(*p, plan, s) : ww::forward<__nv_bfloat16>(*p, plan, s);
 }

@@ -6,6 +6,7 @@
 // functions, and those only after every check has passed.
 #include "../../include/ww_trt_plugins.h"
 
+#include <cmath>
 #include <cstring>
 
 namespace {
@@ -35,6 +36,28 @@ int64_t numel(const ww_tensor_desc_t& d)
         n *= d.dims[i];
     }
     return n;
+}
+
+// Inputs of CrossAttention with these flags, and what input i >= 3 is.
+int attention_inputs(int flags)
+{
+    return 3 + ((flags & WW_PLUGIN_ATTENTION_LENS) != 0) + ((flags & WW_PLUGIN_ATTENTION_MASK) != 0) +
+           ((flags & WW_PLUGIN_ATTENTION_BIAS) != 0);
+}
+
+int attention_role(int flags, int i)
+{
+    for (int role = WW_PLUGIN_ATTENTION_LENS; role <= WW_PLUGIN_ATTENTION_BIAS; role <<= 1)
+        if ((flags & role) != 0 && i-- == 3) return role;
+    return 0;
+}
+
+// {b, l, h} strides of a contiguous [B, L, H, D].
+void contiguous_strides(const ww_tensor_desc_t& d, int64_t (&s)[3])
+{
+    s[2] = d.dims[3];
+    s[1] = s[2] * d.dims[2];
+    s[0] = s[1] * d.dims[1];
 }
 
 }  // namespace
@@ -371,6 +394,181 @@ int ww_plugin_disparity_regression_enqueue(int mode, const ww_tensor_desc_t* in_
                                            static_cast<int>(d.dims[n - 2]), static_cast<int>(d.dims[n - 1]), mode,
                                            stream);
     return st == WW_SUCCESS ? 0 : 1;
+}
+
+// ---------------------------------------------------------- CrossAttention
+// No reference counterpart; LINEAR only, the type of q decides the others'.
+
+int ww_plugin_cross_attention_output_dims(int flags, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                          ww_tensor_desc_t* out)
+{
+    if (inputs == nullptr || out == nullptr || nb_inputs != attention_inputs(flags)) return 1;
+    const ww_tensor_desc_t &q = inputs[0], &k = inputs[1], &v = inputs[2];
+    if (q.nb_dims != 4 || k.nb_dims != 4 || !same_shape(k, v)) return 1;
+    if (k.dims[0] != q.dims[0] || k.dims[3] != q.dims[3]) return 1;
+    if (q.dims[3] <= 0 || q.dims[3] % 8 != 0 || q.dims[3] > 128) return 1;
+    if (k.dims[2] <= 0 || q.dims[2] <= 0 || q.dims[2] % k.dims[2] != 0) return 1;
+    const int n = attention_inputs(flags);
+    for (int i = 3; i < n; ++i) {
+        const ww_tensor_desc_t& d = inputs[i];
+        switch (attention_role(flags, i)) {
+            case WW_PLUGIN_ATTENTION_LENS:
+                if (d.nb_dims != 1 || d.dims[0] != q.dims[0]) return 1;
+                break;
+            case WW_PLUGIN_ATTENTION_MASK:
+                if (d.nb_dims != 2 || d.dims[0] != q.dims[0] || d.dims[1] != k.dims[1]) return 1;
+                break;
+            default:
+                if (d.nb_dims != 2 || d.dims[0] != q.dims[2]) return 1;
+        }
+    }
+    *out = q;
+    return 0;
+}
+
+int ww_plugin_cross_attention_supports_format(int flags, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                              int nb_outputs)
+{
+    if (in_out == nullptr || nb_outputs != 1 || nb_inputs != attention_inputs(flags)) return 0;
+    if (pos < 0 || pos >= nb_inputs + nb_outputs) return 0;
+    const ww_tensor_desc_t& d = in_out[pos];
+    if (d.format != WW_FORMAT_LINEAR) return 0;
+    if (pos == 0) return d.dtype == WW_DTYPE_HALF || d.dtype == WW_DTYPE_BF16;
+    if (pos >= 3 && pos < nb_inputs) {
+        const int role = attention_role(flags, pos);
+        if (role == WW_PLUGIN_ATTENTION_LENS) return d.dtype == WW_DTYPE_INT32;
+        if (role == WW_PLUGIN_ATTENTION_MASK) return d.dtype == WW_DTYPE_BOOL || d.dtype == WW_DTYPE_UINT8;
+    }
+    return d.dtype == in_out[0].dtype;
+}
+
+int ww_plugin_cross_attention_enqueue(int flags, int max_distance, int bidirectional, int q_offset,
+                                      const ww_tensor_desc_t* in_desc, const void* const* inputs,
+                                      void* const* outputs, void* workspace, void* stream)
+{
+    if (in_desc == nullptr || inputs == nullptr || outputs == nullptr) return 1;
+    ww_tensor_desc_t out;
+    const int n = attention_inputs(flags);
+    if (ww_plugin_cross_attention_output_dims(flags, n, in_desc, &out) != 0) return 1;
+    for (int i = 0; i < n; ++i) {
+        if (!ww_plugin_cross_attention_supports_format(flags, i, in_desc, n, 1)) return 1;
+        for (int j = 0; j < in_desc[i].nb_dims; ++j)
+            if (!fits_int(in_desc[i].dims[j])) return 1;
+    }
+    ww_attention_t p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = inputs[0];
+    p.k = inputs[1];
+    p.v = inputs[2];
+    p.out = outputs[0];
+    for (int i = 3; i < n; ++i) {
+        switch (attention_role(flags, i)) {
+            case WW_PLUGIN_ATTENTION_LENS: p.k_lens = static_cast<const int32_t*>(inputs[i]); break;
+            case WW_PLUGIN_ATTENTION_MASK: p.key_mask = static_cast<const uint8_t*>(inputs[i]); break;
+            default:
+                p.bias_table = inputs[i];
+                p.num_buckets = static_cast<int32_t>(in_desc[i].dims[1]);
+        }
+        if (inputs[i] == nullptr && numel(in_desc[i]) != 0) return 1;
+    }
+    const ww_tensor_desc_t &q = in_desc[0], &k = in_desc[1];
+    p.dtype = q.dtype;
+    p.B = static_cast<int32_t>(q.dims[0]);
+    p.Lq = static_cast<int32_t>(q.dims[1]);
+    p.Hq = static_cast<int32_t>(q.dims[2]);
+    p.D = static_cast<int32_t>(q.dims[3]);
+    p.Lk = static_cast<int32_t>(k.dims[1]);
+    p.Hk = static_cast<int32_t>(k.dims[2]);
+    contiguous_strides(q, p.q_strides);
+    contiguous_strides(k, p.k_strides);
+    contiguous_strides(k, p.v_strides);
+    p.max_distance = max_distance;
+    p.bidirectional = bidirectional;
+    p.q_offset = q_offset;
+    p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(p.D)));
+    if (workspace != nullptr && ww_cross_attention_workspace(&p) <= WW_PLUGIN_ATTENTION_WORKSPACE) {
+        p.workspace = workspace;
+        p.workspace_bytes = WW_PLUGIN_ATTENTION_WORKSPACE;
+    }
+    return ww_cross_attention(&p, stream) == WW_SUCCESS ? 0 : 1;
+}
+
+// --------------------------------------------------------------- QkNormRope
+
+int ww_plugin_qk_norm_rope_output_dims(int use_positions, int which, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                       ww_tensor_desc_t* out)
+{
+    if (inputs == nullptr || out == nullptr || nb_inputs != (use_positions ? 8 : 6) || which < 0 || which > 1) return 1;
+    const ww_tensor_desc_t &q = inputs[0], &k = inputs[1], &cs = inputs[4];
+    if (q.nb_dims != 4 || k.nb_dims != 4 || q.dims[0] != k.dims[0] || q.dims[3] != k.dims[3]) return 1;
+    for (int i = 2; i < 4; ++i)
+        if (inputs[i].nb_dims != 1 || inputs[i].dims[0] != q.dims[3]) return 1;
+    if (cs.nb_dims != 2 || !same_shape(cs, inputs[5]) || 2 * cs.dims[1] > q.dims[3]) return 1;
+    for (int i = 6; i < nb_inputs; ++i) {  // [L] or [B, L]
+        const ww_tensor_desc_t& d = inputs[i];
+        const int64_t L = inputs[i - 6].dims[1];
+        if (!(d.nb_dims == 1 && d.dims[0] == L) && !(d.nb_dims == 2 && d.dims[0] == q.dims[0] && d.dims[1] == L)) return 1;
+    }
+    *out = inputs[which];
+    return 0;
+}
+
+int ww_plugin_qk_norm_rope_supports_format(int use_positions, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                           int nb_outputs)
+{
+    if (in_out == nullptr || nb_outputs != 2 || nb_inputs != (use_positions ? 8 : 6)) return 0;
+    if (pos < 0 || pos >= nb_inputs + nb_outputs) return 0;
+    const ww_tensor_desc_t& d = in_out[pos];
+    if (d.format != WW_FORMAT_LINEAR) return 0;
+    if (pos == 0) return d.dtype == WW_DTYPE_HALF || d.dtype == WW_DTYPE_BF16 || d.dtype == WW_DTYPE_FLOAT;
+    if (pos == 4 || pos == 5) return d.dtype == WW_DTYPE_FLOAT;
+    if (pos >= 6 && pos < nb_inputs) return d.dtype == WW_DTYPE_INT32;
+    return d.dtype == in_out[0].dtype;
+}
+
+int ww_plugin_qk_norm_rope_enqueue(int use_positions, int eps_nano, int interleaved, const ww_tensor_desc_t* in_desc,
+                                   const void* const* inputs, void* const* outputs, void* stream)
+{
+    if (in_desc == nullptr || inputs == nullptr || outputs == nullptr) return 1;
+    const int n = use_positions ? 8 : 6;
+    ww_tensor_desc_t out;
+    if (ww_plugin_qk_norm_rope_output_dims(use_positions, 0, n, in_desc, &out) != 0) return 1;
+    for (int i = 0; i < n; ++i) {
+        if (!ww_plugin_qk_norm_rope_supports_format(use_positions, i, in_desc, n, 2)) return 1;
+        for (int j = 0; j < in_desc[i].nb_dims; ++j)
+            if (!fits_int(in_desc[i].dims[j])) return 1;
+    }
+    ww_qk_norm_rope_t p;
+    std::memset(&p, 0, sizeof(p));
+    p.q = inputs[0];
+    p.k = inputs[1];
+    p.q_weight = inputs[2];
+    p.k_weight = inputs[3];
+    p.cos = static_cast<const float*>(inputs[4]);
+    p.sin = static_cast<const float*>(inputs[5]);
+    p.q_out = outputs[0];
+    p.k_out = outputs[1];
+    const ww_tensor_desc_t &q = in_desc[0], &k = in_desc[1];
+    if (use_positions) {
+        p.q_pos = static_cast<const int32_t*>(inputs[6]);
+        p.k_pos = static_cast<const int32_t*>(inputs[7]);
+        p.q_pos_stride = in_desc[6].nb_dims == 2 ? static_cast<int32_t>(q.dims[1]) : 0;
+        p.k_pos_stride = in_desc[7].nb_dims == 2 ? static_cast<int32_t>(k.dims[1]) : 0;
+    }
+    contiguous_strides(q, p.q_strides);
+    contiguous_strides(k, p.k_strides);
+    p.dtype = q.dtype;
+    p.B = static_cast<int32_t>(q.dims[0]);
+    p.Lq = static_cast<int32_t>(q.dims[1]);
+    p.Lk = static_cast<int32_t>(k.dims[1]);
+    p.Hq = static_cast<int32_t>(q.dims[2]);
+    p.Hk = static_cast<int32_t>(k.dims[2]);
+    p.D = static_cast<int32_t>(q.dims[3]);
+    p.R = static_cast<int32_t>(2 * in_desc[4].dims[1]);
+    p.P = static_cast<int32_t>(in_desc[4].dims[0]);
+    p.interleaved = interleaved;
+    p.eps = static_cast<float>(eps_nano * 1e-9);
+    return ww_qk_norm_rope(&p, stream) == WW_SUCCESS ? 0 : 1;
 }
 
 }  // extern "C"

@@ -10,7 +10,8 @@
 // under the same names and version -- "CorrVolume" v"1" with field max_disp
 // (default 48), "CostStem3D" v"1" with no required field, "Nv12Decode" v"1"
 // with fields out_h / out_w (224 / 288) -- plus the fused "CorrCostStem3D" and
-// "DisparityRegression" (field mode), which have no reference counterpart.  Every method is
+// "DisparityRegression" (field mode), "CrossAttention" and "QkNormRope", which have
+// no reference counterpart.  Every method is
 // a thin forwarder to the ww_plugin_* functions of the C ABI (plugin_core.cpp),
 // which carry the logic of the reference's IPluginV3 methods
 // (src/plugins/corr_volume/corr_volume.cpp:23-139,
@@ -33,7 +34,15 @@ namespace ww_trt {
 
 using namespace nvinfer1;
 
-enum class Op { kCorrVolume, kCostStem3D, kCorrCostStem3D, kNv12Decode, kDisparityRegression };
+enum class Op {
+    kCorrVolume,
+    kCostStem3D,
+    kCorrCostStem3D,
+    kNv12Decode,
+    kDisparityRegression,
+    kCrossAttention,
+    kQkNormRope
+};
 
 // Integer fields an op carries; every op stores all three, serialises its own.
 struct Fields {
@@ -43,6 +52,21 @@ struct Fields {
     int32_t out_h = 224;
     int32_t out_w = 288;
     int32_t mode = WW_DISP_SOFTARGMAX;
+    int32_t use_lens = 0;
+    int32_t use_mask = 0;
+    int32_t use_bias = 0;
+    int32_t max_distance = 128;
+    int32_t bidirectional = 1;
+    int32_t q_offset = 0;
+    int32_t use_positions = 0;
+    int32_t interleaved = 0;
+    int32_t eps_nano = 1000;
+
+    int attention_flags() const noexcept
+    {
+        return (use_lens != 0 ? WW_PLUGIN_ATTENTION_LENS : 0) | (use_mask != 0 ? WW_PLUGIN_ATTENTION_MASK : 0) |
+               (use_bias != 0 ? WW_PLUGIN_ATTENTION_BIAS : 0);
+    }
 };
 
 constexpr char const* kVersion = "1";
@@ -55,6 +79,8 @@ char const* op_name(Op op) noexcept
         case Op::kCorrCostStem3D: return "CorrCostStem3D";
         case Op::kNv12Decode: return "Nv12Decode";
         case Op::kDisparityRegression: return "DisparityRegression";
+        case Op::kCrossAttention: return "CrossAttention";
+        case Op::kQkNormRope: return "QkNormRope";
     }
     return "";
 }
@@ -68,6 +94,9 @@ std::vector<char const*> op_fields(Op op)
         case Op::kCorrCostStem3D: return {"max_disp", "num_groups", "act"};
         case Op::kNv12Decode: return {"out_h", "out_w"};
         case Op::kDisparityRegression: return {"mode"};
+        case Op::kCrossAttention:
+            return {"use_lens", "use_mask", "use_bias", "max_distance", "bidirectional", "q_offset"};
+        case Op::kQkNormRope: return {"use_positions", "interleaved", "eps_nano"};
     }
     return {};
 }
@@ -80,6 +109,15 @@ int32_t* field_slot(Fields& f, char const* name) noexcept
     if (std::strcmp(name, "out_h") == 0) return &f.out_h;
     if (std::strcmp(name, "out_w") == 0) return &f.out_w;
     if (std::strcmp(name, "mode") == 0) return &f.mode;
+    if (std::strcmp(name, "use_lens") == 0) return &f.use_lens;
+    if (std::strcmp(name, "use_mask") == 0) return &f.use_mask;
+    if (std::strcmp(name, "use_bias") == 0) return &f.use_bias;
+    if (std::strcmp(name, "max_distance") == 0) return &f.max_distance;
+    if (std::strcmp(name, "bidirectional") == 0) return &f.bidirectional;
+    if (std::strcmp(name, "q_offset") == 0) return &f.q_offset;
+    if (std::strcmp(name, "use_positions") == 0) return &f.use_positions;
+    if (std::strcmp(name, "interleaved") == 0) return &f.interleaved;
+    if (std::strcmp(name, "eps_nano") == 0) return &f.eps_nano;
     return nullptr;
 }
 
@@ -122,7 +160,7 @@ public:
     AsciiChar const* getPluginNamespace() const noexcept override { return mNamespace.c_str(); }
 
     // IPluginV3OneBuild
-    int32_t getNbOutputs() const noexcept override { return 1; }
+    int32_t getNbOutputs() const noexcept override { return mOp == Op::kQkNormRope ? 2 : 1; }
 
     int32_t configurePlugin(DynamicPluginTensorDesc const*, int32_t nbInputs, DynamicPluginTensorDesc const*,
                             int32_t) noexcept override
@@ -137,14 +175,14 @@ public:
         if (nbOutputs < 1 || nbInputs < 1) return 1;
         // Nv12Decode declares fp32 and lets the format choice pick fp16 or
         // fp32 (nv12_decode.cpp:26-39); the others follow input 0.
-        out[0] = mOp == Op::kNv12Decode ? DataType::kFLOAT : in[0];
+        for (int32_t i = 0; i < nbOutputs; ++i) out[i] = mOp == Op::kNv12Decode ? DataType::kFLOAT : in[0];
         return 0;
     }
 
     int32_t getOutputShapes(DimsExprs const* in, int32_t nbInputs, DimsExprs const*, int32_t, DimsExprs* out,
                             int32_t nbOutputs, IExprBuilder& eb) noexcept override
     {
-        if (nbOutputs != 1) return 1;
+        if (nbOutputs != getNbOutputs()) return 1;
         switch (mOp) {
             case Op::kCorrVolume:  // [B, D, H, W] or [B, G, D, H, W]
                 if (nbInputs != 2 || in[0].nbDims != 4) return 1;
@@ -188,6 +226,15 @@ public:
                 out[0].d[2] = in[0].d[in[0].nbDims - 2];
                 out[0].d[3] = in[0].d[in[0].nbDims - 1];
                 return 0;
+            case Op::kCrossAttention:  // like q
+                if (nbInputs < 3 || in[0].nbDims != 4 || in[1].nbDims != 4) return 1;
+                out[0] = in[0];
+                return 0;
+            case Op::kQkNormRope:  // like q and k
+                if (nbInputs < 6 || in[0].nbDims != 4 || in[1].nbDims != 4) return 1;
+                out[0] = in[0];
+                out[1] = in[1];
+                return 0;
             case Op::kCorrCostStem3D:  // [B, Cout, D, H, W]; 8 inputs (3-stage stem): Cout = 1
                 if ((nbInputs != 4 && nbInputs != 8) || in[0].nbDims != 4) return 1;
                 if (nbInputs == 4 && in[2].nbDims != 5) return 1;
@@ -206,8 +253,8 @@ public:
                                    int32_t nbOutputs) noexcept override
     {
         const int n = nbInputs + nbOutputs;
-        if (n <= 0 || n > 9) return false;  // up to 8 inputs + 1 output
-        std::array<ww_tensor_desc_t, 9> d{};
+        if (n <= 0 || n > 10) return false;  // up to 8 inputs + 2 outputs
+        std::array<ww_tensor_desc_t, 10> d{};
         for (int i = 0; i < n; ++i) d[i] = to_ww(inOut[i].desc);
         switch (mOp) {
             case Op::kCorrVolume:
@@ -220,6 +267,12 @@ public:
                 return ww_plugin_nv12_decode_supports_format(pos, d.data(), nbInputs, nbOutputs) != 0;
             case Op::kDisparityRegression:
                 return ww_plugin_disparity_regression_supports_format(pos, d.data(), nbInputs, nbOutputs) != 0;
+            case Op::kCrossAttention:
+                return ww_plugin_cross_attention_supports_format(mFields.attention_flags(), pos, d.data(), nbInputs,
+                                                                 nbOutputs) != 0;
+            case Op::kQkNormRope:
+                return ww_plugin_qk_norm_rope_supports_format(mFields.use_positions, pos, d.data(), nbInputs,
+                                                              nbOutputs) != 0;
         }
         return false;
     }
@@ -227,7 +280,8 @@ public:
     size_t getWorkspaceSize(DynamicPluginTensorDesc const*, int32_t, DynamicPluginTensorDesc const*,
                             int32_t) const noexcept override
     {
-        return 0;  // no kernel of this library uses scratch memory
+        // the others use no scratch memory
+        return mOp == Op::kCrossAttention ? WW_PLUGIN_ATTENTION_WORKSPACE : 0;
     }
 
     // IPluginV3OneRuntime
@@ -239,9 +293,10 @@ public:
     }
 
     int32_t enqueue(PluginTensorDesc const* inDesc, PluginTensorDesc const* outDesc, void const* const* inputs,
-                    void* const* outputs, void*, cudaStream_t stream) noexcept override
+                    void* const* outputs, void* workspace, cudaStream_t stream) noexcept override
     {
-        // Descriptors of the inputs: 2 (CorrVolume), 7 or 3 (CostStem3D), 4 or 8 (fused).
+        // Descriptors of the inputs: 2 (CorrVolume), 7 or 3 (CostStem3D), 4 or 8 (fused),
+        // 3 to 6 (CrossAttention), 6 or 8 (QkNormRope).
         std::array<ww_tensor_desc_t, 8> d{};
         const int nin = mNbInputs;
         if (nin < 1 || nin > 8) return 1;
@@ -266,6 +321,13 @@ public:
                 const ww_tensor_desc_t od = to_ww(outDesc[0]);
                 return ww_plugin_disparity_regression_enqueue(mFields.mode, d.data(), &od, inputs, outputs, stream);
             }
+            case Op::kCrossAttention:
+                return ww_plugin_cross_attention_enqueue(mFields.attention_flags(), mFields.max_distance,
+                                                         mFields.bidirectional, mFields.q_offset, d.data(), inputs,
+                                                         outputs, workspace, stream);
+            case Op::kQkNormRope:
+                return ww_plugin_qk_norm_rope_enqueue(mFields.use_positions, mFields.eps_nano, mFields.interleaved,
+                                                      d.data(), inputs, outputs, stream);
         }
         return 1;
     }
@@ -355,6 +417,12 @@ struct Nv12DecodeCreator final : WwCreator {
 struct DisparityRegressionCreator final : WwCreator {
     DisparityRegressionCreator() : WwCreator(Op::kDisparityRegression) {}
 };
+struct CrossAttentionCreator final : WwCreator {
+    CrossAttentionCreator() : WwCreator(Op::kCrossAttention) {}
+};
+struct QkNormRopeCreator final : WwCreator {
+    QkNormRopeCreator() : WwCreator(Op::kQkNormRope) {}
+};
 
 }  // namespace ww_trt
 
@@ -363,11 +431,15 @@ struct DisparityRegressionCreator final : WwCreator {
 using ww_trt::CorrCostStem3DCreator;
 using ww_trt::CorrVolumeCreator;
 using ww_trt::CostStem3DCreator;
+using ww_trt::CrossAttentionCreator;
 using ww_trt::DisparityRegressionCreator;
 using ww_trt::Nv12DecodeCreator;
+using ww_trt::QkNormRopeCreator;
 
 REGISTER_TENSORRT_PLUGIN(CorrVolumeCreator);
 REGISTER_TENSORRT_PLUGIN(CostStem3DCreator);
 REGISTER_TENSORRT_PLUGIN(CorrCostStem3DCreator);
 REGISTER_TENSORRT_PLUGIN(Nv12DecodeCreator);
 REGISTER_TENSORRT_PLUGIN(DisparityRegressionCreator);
+REGISTER_TENSORRT_PLUGIN(CrossAttentionCreator);
+REGISTER_TENSORRT_PLUGIN(QkNormRopeCreator);

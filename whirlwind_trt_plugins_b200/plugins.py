@@ -25,8 +25,14 @@ Reference plugins (paths relative to the reference project):
 * ``DisparityRegression`` v1 (extension, no reference counterpart): field
   ``mode`` (0 soft-argmax, 1 soft-argmin).
 
+* ``CrossAttention`` v1 (extension): fields ``use_lens``, ``use_mask``,
+  ``use_bias`` (which optional inputs follow q, k, v), ``max_distance`` (128),
+  ``bidirectional`` (1), ``q_offset`` (0).
+* ``QkNormRope`` v1 (extension, two outputs): fields ``use_positions``,
+  ``interleaved``, ``eps_nano`` (eps in 1e-9, 1000).
+
 Descriptors are :class:`TensorDesc` (dims, dtype, format); dtypes use
-TensorRT's numbering (0 = kFLOAT, 1 = kHALF, 2 = kINT8), format 0 = kLINEAR.
+TensorRT's numbering (0 = kFLOAT, 1 = kHALF, 2 = kINT8, 3 = kINT32, 4 = kBOOL, 7 = kBF16), format 0 = kLINEAR.
 """
 from __future__ import annotations
 
@@ -36,11 +42,15 @@ from dataclasses import dataclass, field
 from . import lib
 
 __all__ = ["TensorDesc", "CorrVolumePlugin", "CostStem3DPlugin", "CorrCostStem3DPlugin", "Nv12DecodePlugin",
-           "DisparityRegressionPlugin", "PluginCreator", "get_plugin_creator", "registered_creators"]
+           "DisparityRegressionPlugin", "CrossAttentionPlugin", "QkNormRopePlugin", "PluginCreator", "get_plugin_creator", "registered_creators"]
 
 DTYPE_FLOAT = 0
 DTYPE_HALF = 1
 DTYPE_INT8 = 2
+DTYPE_INT32 = 3
+DTYPE_BOOL = 4
+DTYPE_BF16 = 7
+ATTENTION_WORKSPACE = 64 << 20
 FORMAT_LINEAR = 0
 
 
@@ -71,10 +81,11 @@ class TensorDesc:
 
     @staticmethod
     def of(t) -> "TensorDesc":
-        """Descriptor of a torch tensor (fp16 or fp32)."""
+        """Descriptor of a torch tensor."""
         import torch
         dt = {torch.float16: DTYPE_HALF, torch.float32: DTYPE_FLOAT, torch.int8: DTYPE_INT8,
-              torch.uint8: DTYPE_INT8}.get(t.dtype, -1)
+              torch.uint8: DTYPE_INT8, torch.int32: DTYPE_INT32, torch.bool: DTYPE_BOOL,
+              torch.bfloat16: DTYPE_BF16}.get(t.dtype, -1)
         return TensorDesc(tuple(t.shape), dt, FORMAT_LINEAR)
 
 
@@ -286,6 +297,84 @@ class DisparityRegressionPlugin(_PluginBase):
                                                             ctypes.c_void_p(_stream(stream)))
 
 
+class CrossAttentionPlugin(_PluginBase):
+    """``CrossAttention`` (extension): inputs q [B, Lq, Hq, D], k, v
+    [B, Lk, Hk, D] fp16/bf16, then k_lens, key_mask and bias_table as the
+    ``use_*`` fields say; one output like q."""
+    NAME = "CrossAttention"
+
+    def __init__(self, use_lens: int = 0, use_mask: int = 0, use_bias: int = 0, max_distance: int = 128,
+                 bidirectional: int = 1, q_offset: int = 0):
+        super().__init__()
+        self.use_lens, self.use_mask, self.use_bias = int(use_lens), int(use_mask), int(use_bias)
+        self.max_distance, self.bidirectional, self.q_offset = int(max_distance), int(bidirectional), int(q_offset)
+
+    @property
+    def _flags(self) -> int:
+        return bool(self.use_lens) | bool(self.use_mask) << 1 | bool(self.use_bias) << 2
+
+    def get_fields_to_serialize(self) -> dict:
+        return {n: getattr(self, n) for n in ("use_lens", "use_mask", "use_bias", "max_distance", "bidirectional",
+                                              "q_offset")}
+
+    def get_output_shapes(self, inputs) -> list:
+        out = _Desc()
+        if lib().ww_plugin_cross_attention_output_dims(self._flags, len(inputs), _descs(inputs), ctypes.byref(out)) != 0:
+            raise ValueError("CrossAttention takes q [B, Lq, Hq, D], k, v [B, Lk, Hk, D] and the inputs its fields name")
+        return [TensorDesc._from_c(out).dims]
+
+    def supports_format_combination(self, pos: int, in_out, nb_inputs: int, nb_outputs: int) -> bool:
+        return bool(lib().ww_plugin_cross_attention_supports_format(self._flags, pos, _descs(in_out), nb_inputs,
+                                                                    nb_outputs))
+
+    def get_workspace_size(self) -> int:
+        return ATTENTION_WORKSPACE
+
+    def enqueue(self, input_desc, inputs, outputs, workspace=None, stream=None) -> int:
+        """workspace: a device buffer of get_workspace_size() bytes or None (slower for few queries)."""
+        ws = None if workspace is None else ctypes.c_void_p(workspace.data_ptr())
+        return lib().ww_plugin_cross_attention_enqueue(self._flags, self.max_distance, self.bidirectional, self.q_offset,
+                                                       _descs(input_desc), _ptrs(inputs), _ptrs(outputs), ws,
+                                                       ctypes.c_void_p(_stream(stream)))
+
+
+class QkNormRopePlugin(_PluginBase):
+    """``QkNormRope`` (extension): inputs q, k, q_weight, k_weight, cos, sin and
+    with ``use_positions`` q_pos, k_pos; outputs like q and k."""
+    NAME = "QkNormRope"
+    NB_OUTPUTS = 2
+
+    def __init__(self, use_positions: int = 0, interleaved: int = 0, eps_nano: int = 1000):
+        super().__init__()
+        self.use_positions, self.interleaved, self.eps_nano = int(use_positions), int(interleaved), int(eps_nano)
+
+    def get_fields_to_serialize(self) -> dict:
+        return {"use_positions": self.use_positions, "interleaved": self.interleaved, "eps_nano": self.eps_nano}
+
+    def get_output_data_types(self, input_types) -> list:
+        return super().get_output_data_types(input_types) * 2
+
+    def get_output_shapes(self, inputs) -> list:
+        shapes = []
+        for which in (0, 1):
+            out = _Desc()
+            if lib().ww_plugin_qk_norm_rope_output_dims(self.use_positions, which, len(inputs), _descs(inputs),
+                                                        ctypes.byref(out)) != 0:
+                raise ValueError("QkNormRope takes q, k [B, L, H, D], two weights [D], cos, sin [P, R / 2] "
+                                 "(and two position tensors with use_positions)")
+            shapes.append(TensorDesc._from_c(out).dims)
+        return shapes
+
+    def supports_format_combination(self, pos: int, in_out, nb_inputs: int, nb_outputs: int) -> bool:
+        return bool(lib().ww_plugin_qk_norm_rope_supports_format(self.use_positions, pos, _descs(in_out), nb_inputs,
+                                                                 nb_outputs))
+
+    def enqueue(self, input_desc, inputs, outputs, stream=None) -> int:
+        return lib().ww_plugin_qk_norm_rope_enqueue(self.use_positions, self.eps_nano, self.interleaved,
+                                                    _descs(input_desc), _ptrs(inputs), _ptrs(outputs),
+                                                    ctypes.c_void_p(_stream(stream)))
+
+
 @dataclass
 class PluginCreator:
     """IPluginCreatorV3One counterpart: name, version, field names, create."""
@@ -319,6 +408,10 @@ _CREATORS = {
     ("CorrCostStem3D", "1"): PluginCreator(CorrCostStem3DPlugin, {"max_disp": 48, "num_groups": 1, "act": 0}),
     ("Nv12Decode", "1"): PluginCreator(Nv12DecodePlugin, {"out_h": 224, "out_w": 288}),
     ("DisparityRegression", "1"): PluginCreator(DisparityRegressionPlugin, {"mode": 0}),
+    ("CrossAttention", "1"): PluginCreator(CrossAttentionPlugin, {"use_lens": 0, "use_mask": 0, "use_bias": 0,
+                                                                  "max_distance": 128, "bidirectional": 1,
+                                                                  "q_offset": 0}),
+    ("QkNormRope", "1"): PluginCreator(QkNormRopePlugin, {"use_positions": 0, "interleaved": 0, "eps_nano": 1000}),
 }
 
 
