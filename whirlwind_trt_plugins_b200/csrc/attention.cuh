@@ -155,7 +155,9 @@ __host__ __device__ __forceinline__ int rel_bucket(const RelBuckets& r, int rel)
     // counted, not searched: every thread reads the same edges in the same
     // order (a search's constant-memory reads differ by thread and serialise)
     int n = 0;
+#ifdef __CUDA_ARCH__
 #pragma unroll 8
+#endif
     for (int t = 0; t < r.n_least; ++t) n += r.least[t] <= d;
     return first + r.exact + n;
 }

@@ -67,7 +67,8 @@ struct FwdParams {
     float* part_lse;  // [item][split][NT * 128], log2
     RelBuckets rel;
     int32_t B, Lq, Lk, Hq, group, D;
-    int32_t q_blocks, whole_items, splits;
+    int32_t q_blocks, per_cta, groups;  // query blocks, those of one CTA, groups of them
+    int32_t whole_items, splits;
     Divisor by_block, by_head, by_group;
     int32_t q_b, q_h, k_b, k_h, v_b, v_h;  // 0 where the tensor is broadcast
     int32_t max_entries;                   // relative positions a CTA keeps
@@ -101,8 +102,8 @@ struct Layout {
 template <int DP, int NT>
 struct Bars {
     static constexpr int kStages = Layout<DP, NT>::kStages;
-    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], p_ready[NT],
-        o_full[NT];
+    uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], p_ready[NT],
+        o_full[NT], o_free[NT];
     uint32_t tmem;
 };
 
@@ -171,15 +172,16 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     Bar* bar = reinterpret_cast<Bar*>(base + L::kBar);
     const auto at = [](const uint64_t& b) { return umma::smem_addr(&b); };
 
-    // items (query block, head, batch item); the last ones are split over their keys
+    // items (group of query blocks, head, batch item); the last ones are split over their keys
     const int blk = blockIdx.x;
     const bool in_parts = blk >= p.whole_items;
     const int split = in_parts ? (blk - p.whole_items) % p.splits : 0, splits = in_parts ? p.splits : 1;
     const int item = in_parts ? p.whole_items + (blk - p.whole_items) / p.splits : blk;
-    const int bh = p.by_block.div(item), qb = item - bh * p.q_blocks, b = p.by_head.div(bh), h = bh - b * p.Hq,
+    const int bh = p.by_block.div(item), qb0 = (item - bh * p.groups) * p.per_cta, b = p.by_head.div(bh), h = bh - b * p.Hq,
               g = p.by_group.div(h);
-    const int q0 = qb * (NT * kTile);
-    const int tiles = NT == 1 || q0 + kTile >= p.Lq ? 1 : 2;  // query tiles with rows
+    const int nq = min(p.per_cta, p.q_blocks - qb0);  // query blocks of this CTA, one after the other
+    const auto q_of = [&](int qi) { return (qb0 + qi) * (NT * kTile); };
+    const auto tiles_of = [&](int qi) { return NT == 1 || q_of(qi) + kTile >= p.Lq ? 1 : 2; };  // query tiles with rows
     const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
     const int n_all = (len + KT - 1) / KT;
     int first, n;
@@ -190,46 +192,53 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     float* limits = reinterpret_cast<float*>(base + L::kLim);
     uint32_t* wholes = reinterpret_cast<uint32_t*>(limits + S * KT);  // tile without a masked key
 
-    const auto load_k = [&](int kt) {
-        const int s = kt % S;
+    // tiles are numbered over all query blocks: number i is key tile i % n of block i / n
+    const auto load_k = [&](int i, int kt) {
+        const int s = i % S;
         umma::mbar_arrive_expect_tx(at(bar->k_full[s]), L::kBytes);
         for (int c = 0; c < L::kChunks; ++c)
             for (int x = 0; x < KT; x += kBox)
                 umma::tma_load_4d(sm + L::kK + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.k, c * L::kCols, g * p.k_h,
                                   (first + kt) * KT + x, b * p.k_b, at(bar->k_full[s]));
     };
+    const auto load_q = [&](int qi) {
+        const int tiles = tiles_of(qi);
+        umma::mbar_arrive_expect_tx(at(bar->q_full), tiles * L::kQBytes);
+        for (int t = 0; t < tiles; ++t)
+            for (int c = 0; c < L::kChunks; ++c)
+                for (int x = 0; x < kTile; x += kBox)  // a box beyond the last row reads zeros
+                    umma::tma_load_4d(sm + t * L::kQBytes + c * L::kQChunk + x * L::kRow, &p.q, c * L::kCols, h * p.q_h,
+                                      min(q_of(qi) + t * kTile + x, p.Lq), b * p.q_b, at(bar->q_full));
+    };
     if (warp == NT * 5 && lane == 0) {
         // this thread alone uses the barriers until the block's first barrier below
         umma::mbar_init(at(bar->q_full), 1);
+        umma::mbar_init(at(bar->q_empty), NT);  // one MMA warp per tile
         for (int s = 0; s < S; ++s) {
             umma::mbar_init(at(bar->k_full[s]), 1);
-            umma::mbar_init(at(bar->k_empty[s]), tiles);  // one MMA warp per tile
+            umma::mbar_init(at(bar->k_empty[s]), NT);
             umma::mbar_init(at(bar->v_full[s]), 1);
-            umma::mbar_init(at(bar->v_empty[s]), tiles);
+            umma::mbar_init(at(bar->v_empty[s]), NT);
         }
         for (int t = 0; t < NT; ++t) {
             umma::mbar_init(at(bar->s_full[t]), 1);
             umma::mbar_init(at(bar->p_ready[t]), 4);  // one arrival per warp
             umma::mbar_init(at(bar->o_full[t]), 1);
+            umma::mbar_init(at(bar->o_free[t]), 4);
         }
         umma::mbar_fence_init();
         umma::fence_proxy_async_smem();
         if (n > 0) {
-            umma::mbar_arrive_expect_tx(at(bar->q_full), tiles * L::kQBytes);
-            for (int t = 0; t < tiles; ++t)
-                for (int c = 0; c < L::kChunks; ++c)
-                    for (int x = 0; x < kTile; x += kBox)  // a box beyond the last row reads zeros
-                        umma::tma_load_4d(sm + t * L::kQBytes + c * L::kQChunk + x * L::kRow, &p.q, c * L::kCols, h * p.q_h,
-                                          min(q0 + t * kTile + x, p.Lq), b * p.q_b, at(bar->q_full));
-            load_k(0);
+            load_q(0);
+            load_k(0, 0);
         }
     }
     RelRange range;  // positions j - i - q_offset of the tiles, padded rows and columns included
     float* values = reinterpret_cast<float*>(base + L::kBias);
     uint8_t* buckets = base + L::kBias + 4 * p.max_entries;
     if (p.rel.per_side != 0 && n > 0) {
-        range = rel_range(p.rel, first * KT - (q0 + NT * kTile - 1) - p.rel.q_offset,
-                          (first + n) * KT - 1 - q0 - p.rel.q_offset);
+        range = rel_range(p.rel, first * KT - (q_of(nq) - 1) - p.rel.q_offset,
+                          (first + n) * KT - 1 - q_of(0) - p.rel.q_offset);
         TableRow<T> table;
         table.load(p.rel, p.table, h, lane);
         for (int e0 = warp * 32; warp < NT * 4 && e0 < range.count(); e0 += NT * 128) {  // the other warps have their own starts
@@ -246,12 +255,17 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
 
     if (warp == NT * 5) {
         bool ok = true;
-        for (int kt = 0; kt < n; ++kt) {
-            const int s = kt % S;
-            const uint32_t ph = (kt / S + 1) & 1;
-            if (kt > 0 && lane == 0) {
+        int kt = 0, qi = 0;
+        for (int i = 0; i < nq * n; ++i) {
+            const int s = i % S;
+            const uint32_t ph = (i / S + 1) & 1;
+            if (i > 0 && lane == 0) {
+                if (kt == 0) {
+                    ok = ok && umma::mbar_poll(at(bar->q_empty), (qi - 1) & 1);
+                    if (ok) load_q(qi);
+                }
                 ok = ok && umma::mbar_poll(at(bar->k_empty[s]), ph);
-                if (ok) load_k(kt);
+                if (ok) load_k(i, kt);
             }
             if (lane == 0) ok = ok && umma::mbar_poll(at(bar->v_empty[s]), ph);
             __syncwarp();
@@ -279,11 +293,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                                           g * p.v_h, k0 + x, b * p.v_b, at(bar->v_full[s]));
             }
             if (!__shfl_sync(~0u, ok, 0)) break;
+            if (++kt == n) {
+                kt = 0;
+                ++qi;
+            }
         }
         if (lane == 0 && !ok) record_device_error(p.err, kErrMbarTimeout | 0x20);
     } else if (warp >= NT * 4) {
         const int t = warp - NT * 4;
-        if (n > 0 && t < tiles) {
+        if (n > 0) {
             // The warp runs the loop as a whole, one elected lane issues; descriptors are
             // formed once and advanced by constants and loops are unrolled, so that all a
             // product needs is in uniform registers (formed per product in one thread
@@ -294,191 +312,216 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             const uint64_t q_desc = umma::smem_desc_swizzled<L::kRow>(sm + t * L::kQBytes, 16);
             const uint64_t k_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kK, 16);
             const uint64_t v_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kV, L::kChunk);
-            const auto qk = [&](int kt) {
-                const int s = kt % S, cols = cols_of(kt);
+            const auto qk = [&](int i, int kt) {
+                const int s = i % S, cols = cols_of(kt);
                 const uint32_t id = cols >= KT ? id_full : umma::idesc_16bit(bf, kTile, (cols + 15) / 16 * 16, false);
                 const uint64_t kd = umma::desc_advance(k_desc, s * L::kBytes);
                 if (umma::elect_one()) {
 #pragma unroll
-                    for (int i = 0; i < DP / 16; ++i)
-                        umma::mma_f16_ss(s_col, umma::desc_advance(q_desc, i * 16 / L::kCols * L::kQChunk + i * 16 % L::kCols * 2),
-                                         umma::desc_advance(kd, i * 16 / L::kCols * L::kChunk + i * 16 % L::kCols * 2), id, i > 0);
+                    for (int j = 0; j < DP / 16; ++j)
+                        umma::mma_f16_ss(s_col, umma::desc_advance(q_desc, j * 16 / L::kCols * L::kQChunk + j * 16 % L::kCols * 2),
+                                         umma::desc_advance(kd, j * 16 / L::kCols * L::kChunk + j * 16 % L::kCols * 2), id, j > 0);
                     umma::mma_commit(at(bar->s_full[t]));
                     umma::mma_commit(at(bar->k_empty[s]));
+                    if (kt == n - 1) umma::mma_commit(at(bar->q_empty));
                 }
                 __syncwarp();
             };
-            bool ok = umma::mbar_poll(at(bar->q_full), 0) && umma::mbar_poll(at(bar->k_full[0]), 0);
-            if (ok) qk(0);
-            for (int kt = 0; kt < n && ok; ++kt) {
-                const int s = kt % S, cols = cols_of(kt);
-                ok = umma::mbar_poll(at(bar->v_full[s]), (kt / S) & 1) && umma::mbar_poll(at(bar->p_ready[t]), kt & 1);
-                if (!ok) break;
-                umma::fence_after_sync();
-                const uint64_t vd = umma::desc_advance(v_desc, s * L::kBytes);
-                if (umma::elect_one()) {
-#pragma unroll
-                    for (int i = 0; i < KT / 16; ++i)
-                        if (i * 16 < cols)
-                            umma::mma_f16_ts(o_col, s_col + i * 8, umma::desc_advance(vd, i * 16 * L::kRow), id_o, kt > 0 || i > 0);
-                    umma::mma_commit(at(bar->v_empty[s]));
-                    if (kt == n - 1) umma::mma_commit(at(bar->o_full[t]));
+            bool ok = true;
+            int i = 0;
+            for (int qi = 0; qi < nq && ok; ++qi) {
+                ok = umma::mbar_poll(at(bar->q_full), qi & 1);
+                if (t >= tiles_of(qi)) {
+                    // a tile without rows: its share of the places is given back as they are filled
+                    if (ok && lane == 0) umma::mbar_arrive(at(bar->q_empty));
+                    for (int kt = 0; kt < n && ok; ++kt, ++i) {
+                        const int s = i % S;
+                        ok = umma::mbar_poll(at(bar->k_full[s]), (i / S) & 1);
+                        if (ok && lane == 0) umma::mbar_arrive(at(bar->k_empty[s]));
+                        ok = ok && umma::mbar_poll(at(bar->v_full[s]), (i / S) & 1);
+                        if (ok && lane == 0) umma::mbar_arrive(at(bar->v_empty[s]));
+                    }
+                    continue;
                 }
-                __syncwarp();
-                if (kt + 1 < n) {
-                    ok = umma::mbar_poll(at(bar->k_full[(kt + 1) % S]), ((kt + 1) / S) & 1);
-                    if (ok) qk(kt + 1);
+                ok = ok && umma::mbar_poll(at(bar->k_full[i % S]), (i / S) & 1);
+                if (ok) qk(i, 0);
+                for (int kt = 0; kt < n && ok; ++kt, ++i) {
+                    const int s = i % S, cols = cols_of(kt);
+                    ok = umma::mbar_poll(at(bar->v_full[s]), (i / S) & 1) && umma::mbar_poll(at(bar->p_ready[t]), i & 1);
+                    // the O before has been read
+                    if (kt == 0 && qi > 0) ok = ok && umma::mbar_poll(at(bar->o_free[t]), (qi - 1) & 1);
+                    if (!ok) break;
+                    umma::fence_after_sync();
+                    const uint64_t vd = umma::desc_advance(v_desc, s * L::kBytes);
+                    if (umma::elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < KT / 16; ++j)
+                            if (j * 16 < cols)
+                                umma::mma_f16_ts(o_col, s_col + j * 8, umma::desc_advance(vd, j * 16 * L::kRow), id_o, kt > 0 || j > 0);
+                        umma::mma_commit(at(bar->v_empty[s]));
+                        if (kt == n - 1) umma::mma_commit(at(bar->o_full[t]));
+                    }
+                    __syncwarp();
+                    if (kt + 1 < n) {
+                        ok = umma::mbar_poll(at(bar->k_full[(i + 1) % S]), ((i + 1) / S) & 1);
+                        if (ok) qk(i + 1, kt + 1);
+                    }
                 }
             }
             if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x21);
         }
-    } else if (warp / 4 < tiles) {
+    } else {
         const int t = warp / 4, r = threadIdx.x % 128;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;  // TMEM lane of this warp's first row
         const uint32_t s_col = tmem + lanes + t * KT, o_col = tmem + lanes + NT * KT + t * DP;
-        const int i = q0 + t * kTile + r;
-        float m = -INFINITY;
-        Pair l2 = pair(0.0f, 0.0f);  // sums of the even and of the odd columns
         bool ok = true;  // once a wait has run out: no more waits, everything else goes on
-        const bool any_row = q0 + t * kTile + warp % 4 * 32 < p.Lq;  // else this warp keeps the barriers only
-        for (int kt = 0; kt < n; ++kt) {
-            const int s = kt % S, k0 = (first + kt) * KT, cols = cols_of(kt);
-            // the bias: one value for the tile, or by j - i from this row's start
-            float flat = 0.0f;
-            const float* mine = nullptr;
-            if (p.rel.per_side != 0) {
-                const int lo = k0 - (q0 + t * kTile + kTile - 1) - p.rel.q_offset;
-                if (bucket_at(range, buckets, lo) == bucket_at(range, buckets, lo + kTile + KT - 2))
-                    flat = values[min(max(lo, range.lo), range.hi) - range.lo];
-                else
-                    mine = values + k0 - i - p.rel.q_offset - range.lo;
-            }
-            bool whole = cols == KT;
-            if (!whole || p.key_mask != nullptr) {
-                ok = ok && umma::mbar_poll(at(bar->v_full[s]), (kt / S) & 1);
-                whole = wholes[s] != 0;
-            }
-            ok = ok && umma::mbar_poll(at(bar->s_full[t]), kt & 1);
-            umma::fence_after_sync();
-            const int chunks = any_row ? (cols + 31) / 32 : 0;
-            // raw scores: scale and constant join the exponential's argument
-            const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f && flat > -INFINITY;
-            float top = -INFINITY;
-            const float* lim = limits + s * KT;
-#pragma unroll 1
-            for (int c = 0; c < chunks; ++c) {
-                uint32_t x[32];
-                umma::tmem_ld32(s_col + c * 32, x);
-                umma::tmem_wait_ld32(x);
-                if (plain) {
-                    float top1 = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        top = max3(top, f32(x[j]), f32(x[j + 1]));
-                        top1 = max3(top1, f32(x[j + 2]), f32(x[j + 3]));
-                    }
-                    top = fmaxf(top, top1);
-                } else {
-                    float tc;
-                    if (mine == nullptr)
-                        tc = whole ? score_pass<false, false>(x, p.scale2, flat, nullptr, nullptr)
-                                   : score_pass<false, true>(x, p.scale2, flat, nullptr, lim + 32 * c);
+        int number = 0;
+        for (int qi = 0; qi < nq && t < tiles_of(qi); ++qi) {
+            const int q0 = q_of(qi), i = q0 + t * kTile + r;
+            float m = -INFINITY;
+            Pair l2 = pair(0.0f, 0.0f);  // sums of the even and of the odd columns
+            const bool any_row = q0 + t * kTile + warp % 4 * 32 < p.Lq;  // else this warp keeps the barriers only
+            for (int kt = 0; kt < n; ++kt, ++number) {
+                const int s = number % S, k0 = (first + kt) * KT, cols = cols_of(kt);
+                // the bias: one value for the tile, or by j - i from this row's start
+                float flat = 0.0f;
+                const float* mine = nullptr;
+                if (p.rel.per_side != 0) {
+                    const int lo = k0 - (q0 + t * kTile + kTile - 1) - p.rel.q_offset;
+                    if (bucket_at(range, buckets, lo) == bucket_at(range, buckets, lo + kTile + KT - 2))
+                        flat = values[min(max(lo, range.lo), range.hi) - range.lo];
                     else
-                        tc = whole ? score_pass<true, false>(x, p.scale2, 0.0f, mine + 32 * c, nullptr)
-                                   : score_pass<true, true>(x, p.scale2, 0.0f, mine + 32 * c, lim + 32 * c);
-                    top = fmaxf(top, tc);
-                    umma::tmem_st32(s_col + c * 32, x);
+                        mine = values + k0 - i - p.rel.q_offset - range.lo;
                 }
-            }
-            if (plain) top = fmaf(top, p.scale2, flat);
-            else umma::tmem_wait_st();
-            // grow the maximum: always on the first tile, then only past kRescale
-            if (__any_sync(~0u, kt == 0 || top > m + kRescale)) {
-                const float mn = fmaxf(m, top);
-                if (kt > 0) {  // the product before is done: its commit came before that of these scores
-                    const float f = exp2_approx(m == -INFINITY ? -INFINITY : m - mn);
-                    l2 = mul2(l2, pair(f, f));
+                bool whole = cols == KT;
+                if (!whole || p.key_mask != nullptr) {
+                    ok = ok && umma::mbar_poll(at(bar->v_full[s]), (number / S) & 1);
+                    whole = wholes[s] != 0;
+                }
+                ok = ok && umma::mbar_poll(at(bar->s_full[t]), number & 1);
+                umma::fence_after_sync();
+                const int chunks = any_row ? (cols + 31) / 32 : 0;
+                // raw scores: scale and constant join the exponential's argument
+                const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f && flat > -INFINITY;
+                float top = -INFINITY;
+                const float* lim = limits + s * KT;
 #pragma unroll 1
-                    for (int c = 0; c < DP; c += 16) {
-                        uint32_t o[16];
-                        umma::tmem_ld16(o_col + c, o);
-                        umma::tmem_wait_ld16(o);
+                for (int c = 0; c < chunks; ++c) {
+                    uint32_t x[32];
+                    umma::tmem_ld32(s_col + c * 32, x);
+                    umma::tmem_wait_ld32(x);
+                    if (plain) {
+                        float top1 = -INFINITY;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(f32(o[j]) * f);
-                        umma::tmem_st16(o_col + c, o);
+                        for (int j = 0; j < 32; j += 4) {
+                            top = max3(top, f32(x[j]), f32(x[j + 1]));
+                            top1 = max3(top1, f32(x[j + 2]), f32(x[j + 3]));
+                        }
+                        top = fmaxf(top, top1);
+                    } else {
+                        float tc;
+                        if (mine == nullptr)
+                            tc = whole ? score_pass<false, false>(x, p.scale2, flat, nullptr, nullptr)
+                                       : score_pass<false, true>(x, p.scale2, flat, nullptr, lim + 32 * c);
+                        else
+                            tc = whole ? score_pass<true, false>(x, p.scale2, 0.0f, mine + 32 * c, nullptr)
+                                       : score_pass<true, true>(x, p.scale2, 0.0f, mine + 32 * c, lim + 32 * c);
+                        top = fmaxf(top, tc);
+                        umma::tmem_st32(s_col + c * 32, x);
                     }
                 }
-                m = mn;
-            }
-            const float add = (plain ? flat : 0.0f) - (m == -INFINITY ? 0.0f : m);
+                if (plain) top = fmaf(top, p.scale2, flat);
+                else umma::tmem_wait_st();
+                // grow the maximum: always on the first tile, then only past kRescale
+                if (__any_sync(~0u, kt == 0 || top > m + kRescale)) {
+                    const float mn = fmaxf(m, top);
+                    if (kt > 0) {  // the product before is done: its commit came before that of these scores
+                        const float f = exp2_approx(m == -INFINITY ? -INFINITY : m - mn);
+                        l2 = mul2(l2, pair(f, f));
 #pragma unroll 1
-            for (int c = 0; c < chunks; ++c) {
-                uint32_t x[32];
-                umma::tmem_ld32(s_col + c * 32, x);
-                umma::tmem_wait_ld32(x);
-                // 16 columns of P over scores that have been read
-                if (plain) exp_pass<T, true>(x, p.scale2, add, l2, s_col + c * 16);
-                else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c * 16);
-            }
-            if (!whole) {
-                // rows of V behind masked keys: 0 in place of whatever they hold
-                if (r < KT && lim[r] < 0.0f) {
-                    for (int c = 0; c < L::kChunks; ++c)
+                        for (int c = 0; c < DP; c += 16) {
+                            uint32_t o[16];
+                            umma::tmem_ld16(o_col + c, o);
+                            umma::tmem_wait_ld16(o);
 #pragma unroll
-                        for (int j = 0; j < L::kRow; j += 16)
-                            umma::st_shared_v4(sm + L::kV + s * L::kBytes + c * L::kChunk + r * L::kRow + j, 0, 0, 0, 0);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(f32(o[j]) * f);
+                            umma::tmem_st16(o_col + c, o);
+                        }
+                    }
+                    m = mn;
                 }
-                umma::fence_proxy_async_smem();
+                const float add = (plain ? flat : 0.0f) - (m == -INFINITY ? 0.0f : m);
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) {
+                    uint32_t x[32];
+                    umma::tmem_ld32(s_col + c * 32, x);
+                    umma::tmem_wait_ld32(x);
+                    // 16 columns of P over scores that have been read
+                    if (plain) exp_pass<T, true>(x, p.scale2, add, l2, s_col + c * 16);
+                    else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c * 16);
+                }
+                if (!whole) {
+                    // rows of V behind masked keys: 0 in place of whatever they hold
+                    if (r < KT && lim[r] < 0.0f) {
+                        for (int c = 0; c < L::kChunks; ++c)
+#pragma unroll
+                            for (int j = 0; j < L::kRow; j += 16)
+                                umma::st_shared_v4(sm + L::kV + s * L::kBytes + c * L::kChunk + r * L::kRow + j, 0, 0, 0, 0);
+                    }
+                    umma::fence_proxy_async_smem();
+                }
+                umma::tmem_wait_st();
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) umma::mbar_arrive(at(bar->p_ready[t]));
             }
-            umma::tmem_wait_st();
+            if (n > 0) ok = ok && umma::mbar_poll(at(bar->o_full[t]), qi & 1);
+            umma::fence_after_sync();
+            float l_even, l_odd;
+            unpair(l2, l_even, l_odd);
+            const float sum = l_even + l_odd;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
+            const int64_t part = (static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (NT * kTile) + t * kTile + r;
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                if (n > 0) {
+                    umma::tmem_ld32(o_col + c, o);
+                    umma::tmem_wait_ld32(o);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = 0;
+                }
+                if (i >= p.Lq) continue;
+                if (in_parts) {
+                    float* to = p.part_o + part * p.D + c;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        if (c + j < p.D)
+                            *reinterpret_cast<float4*>(to + j) =
+                                make_float4(f32(o[j]) * inv, f32(o[j + 1]) * inv, f32(o[j + 2]) * inv, f32(o[j + 3]) * inv);
+                } else {
+                    T* to = static_cast<T*>(p.out) + row * p.D + c;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        if (c + j < p.D)
+                            *reinterpret_cast<uint4*>(to + j) = make_uint4(
+                                pack2<T>(f32(o[j]) * inv, f32(o[j + 1]) * inv), pack2<T>(f32(o[j + 2]) * inv, f32(o[j + 3]) * inv),
+                                pack2<T>(f32(o[j + 4]) * inv, f32(o[j + 5]) * inv),
+                                pack2<T>(f32(o[j + 6]) * inv, f32(o[j + 7]) * inv));
+                }
+            }
+            if (i < p.Lq) {
+                const float lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
+                if (in_parts) p.part_lse[part] = lse2;
+                else if (p.lse != nullptr) p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Lq + i] = lse2 * kLn2F;
+            }
             umma::fence_before_sync();
             __syncwarp();
-            if (lane == 0) umma::mbar_arrive(at(bar->p_ready[t]));
+            if (lane == 0) umma::mbar_arrive(at(bar->o_free[t]));
         }
-        if (n > 0) ok = ok && umma::mbar_poll(at(bar->o_full[t]), 0);
-        umma::fence_after_sync();
         if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x22);
-        float l_even, l_odd;
-        unpair(l2, l_even, l_odd);
-        const float sum = l_even + l_odd;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
-        const int64_t part = (static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (NT * kTile) + t * kTile + r;
-#pragma unroll
-        for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            if (n > 0) {
-                umma::tmem_ld32(o_col + c, o);
-                umma::tmem_wait_ld32(o);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = 0;
-            }
-            if (i >= p.Lq) continue;
-            if (in_parts) {
-                float* to = p.part_o + part * p.D + c;
-#pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    if (c + j < p.D)
-                        *reinterpret_cast<float4*>(to + j) =
-                            make_float4(f32(o[j]) * inv, f32(o[j + 1]) * inv, f32(o[j + 2]) * inv, f32(o[j + 3]) * inv);
-            } else {
-                T* to = static_cast<T*>(p.out) + row * p.D + c;
-#pragma unroll
-                for (int j = 0; j < 32; j += 8)
-                    if (c + j < p.D)
-                        *reinterpret_cast<uint4*>(to + j) = make_uint4(
-                            pack2<T>(f32(o[j]) * inv, f32(o[j + 1]) * inv), pack2<T>(f32(o[j + 2]) * inv, f32(o[j + 3]) * inv),
-                            pack2<T>(f32(o[j + 4]) * inv, f32(o[j + 5]) * inv),
-                            pack2<T>(f32(o[j + 6]) * inv, f32(o[j + 7]) * inv));
-            }
-        }
-        if (i < p.Lq) {
-            const float lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
-            if (in_parts) p.part_lse[part] = lse2;
-            else if (p.lse != nullptr) p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Lq + i] = lse2 * kLn2F;
-        }
-        umma::fence_before_sync();
     }
     __syncthreads();
     if (warp == NT * 4) {
@@ -543,14 +586,14 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o
 // the GPU's CTAs (all of them, where there are few).
 struct Plan {
     bool token;
-    int nt, q_blocks, whole, rest, splits, rows;
+    int nt, q_blocks, per_cta, groups, whole, rest, splits, rows;
     int64_t part_rows() const { return i64(rest) * splits * rows; }
     int64_t part_bytes(int D) const { return part_rows() * (D + 1) * 4; }
     void without_parts(const ww_attention_t& p)
     {
         splits = 1;
         rest = 0;
-        whole = token ? 0 : static_cast<int>(i64(q_blocks) * p.B * p.Hq);
+        whole = token ? 0 : static_cast<int>(i64(groups) * p.B * p.Hq);
     }
 };
 
@@ -559,7 +602,7 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     Plan& r = *plan;
     r.token = token_form(p);
     if (r.token) {
-        r.q_blocks = 0;
+        r.q_blocks = r.groups = r.per_cta = 0;
         r.nt = 0;
         r.rows = p.Hq / p.Hk * p.Lq;
         r.splits = token_splits(p, sms);
@@ -571,11 +614,25 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     r.nt = p.Lq > 1024 ? 2 : 1;
     r.rows = r.nt * kTile;
     r.q_blocks = (p.Lq + r.rows - 1) / r.rows;
-    const int64_t items = i64(r.q_blocks) * p.B * p.Hq, tiles = (p.Lk + 63) / 64;
-    if (items > (1 << 30)) return false;
+    const int64_t heads = i64(p.B) * p.Hq, tiles = (p.Lk + 63) / 64;
+    if (heads * r.q_blocks > (1 << 30)) return false;
     const int slots = sms * (p.D > 64 ? 2 : 4) / r.nt;
+    // query blocks of one CTA, of short rows: a start costs about half a block, so
+    // the count whose rounds end soonest (rows of 312 x 12032 heads: three blocks a CTA)
+    r.per_cta = 1;
+    double least = 1e30;
+    for (int n = 1; n <= (r.nt == 1 ? r.q_blocks : 1); ++n) {
+        const int64_t ctas = heads * ((r.q_blocks + n - 1) / n);
+        const double time = static_cast<double>((ctas + slots - 1) / slots) * (n + 0.5);
+        if (time < least) {
+            least = time;
+            r.per_cta = n;
+        }
+    }
+    r.groups = (r.q_blocks + r.per_cta - 1) / r.per_cta;
+    const int64_t items = heads * r.groups;
     r.rest = static_cast<int>(items % slots);
-    r.splits = tail_splits(r.rest, slots, tiles);
+    r.splits = r.per_cta == 1 ? tail_splits(r.rest, slots, tiles) : 1;  // the join counts blocks
     if (r.splits == 1) r.rest = 0;
     r.whole = static_cast<int>(items - r.rest);
     return true;
@@ -615,7 +672,7 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.max_entries = 0;
     if (p.bias_table != nullptr) {
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
-        const int all = (p.Lk + 127) / 128 * 128 + plan.nt * kTile;
+        const int all = (p.Lk + 127) / 128 * 128 + plan.per_cta * plan.nt * kTile;
         f.max_entries = (std::min(2 * (p.max_distance + kRelMargin) + 1, all) + 15) / 16 * 16;
     }
     f.part_o = part_o;
@@ -627,7 +684,9 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.group = p.Hq / p.Hk;
     f.D = p.D;
     f.q_blocks = plan.q_blocks;
-    f.by_block = make_divisor(plan.q_blocks);
+    f.per_cta = plan.per_cta;
+    f.groups = plan.groups;
+    f.by_block = make_divisor(plan.groups);
     f.by_head = make_divisor(p.Hq);
     f.by_group = make_divisor(p.Hq / p.Hk);
     f.whole_items = plan.whole;
