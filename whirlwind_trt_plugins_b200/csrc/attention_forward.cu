@@ -31,13 +31,14 @@
 //   NT = 2  two CTAs of two query tiles against the same keys: half the reads of
 //           K and V from L2, for long rows
 //
-// Masked keys: their scores meet a limit of -inf (a minimum, which also takes
-// a NaN) and their rows of V are zeroed in shared memory (0 times a NaN would
-// not be 0); tiles without a masked key skip both.
+// Masked keys: the load warp clears their rows of K and V before a tile is used
+// (its products then see zeros, whatever the places held: 0 times a NaN would not
+// be 0) and leaves limits, 0 or -inf, that join the scores; tiles without a masked
+// key skip the limits, calls without one the clearing.
 // The relative bias of a head depends on j - i alone: a CTA puts its values by
 // position into shared memory once, a row reads a tile's at fixed offsets from
-// its own start (neighbouring rows one apart: no bank conflicts); tiles whose
-// positions all lie in one bucket add a constant.
+// its own start (neighbouring rows one apart: no bank conflicts); tiles beyond
+// max_distance add a constant.
 //
 // Few rows against many keys: the keys are split over CTAs, each writes its
 // normalised fp32 rows and log sums, a second kernel joins them in order.
@@ -91,7 +92,7 @@ struct Layout {
     static constexpr int kV = kK + kStages * kBytes;
     static constexpr int kLim = kV + kStages * kBytes;     // [stages][keys] limits, [stages] flags
     static constexpr int kBar = kLim + kStages * (kKeys + 4) * 4;
-    static constexpr int kBias = kBar + 256;               // [entries] values, [entries] buckets
+    static constexpr int kBias = kBar + 256;               // [entries] values
     static constexpr int kTotal = kBias + 1024;            // + alignment of the base, + the bias
     static constexpr int kNeed = NT * (kKeys + DP);
     static constexpr int kColumns = kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
@@ -102,7 +103,8 @@ struct Layout {
 template <int DP, int NT>
 struct Bars {
     static constexpr int kStages = Layout<DP, NT>::kStages;
-    uint64_t q_full, q_empty, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[NT], p_ready[NT],
+    uint64_t q_full, q_empty, k_full[kStages], k_ready[kStages], k_empty[kStages], v_full[kStages], v_ready[kStages],
+        v_empty[kStages], s_full[NT], p_ready[NT],
         o_full[NT], o_free[NT];
     uint32_t tmem;
 };
@@ -116,16 +118,16 @@ __device__ __forceinline__ float score_pass(uint32_t (&x)[32], float scale2, flo
     const Pair scale_2 = pair(scale2, scale2), flat_2 = pair(flat, flat);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-        float y[4];
-        unpair(fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, BIAS ? pair(bias[j], bias[j + 1]) : flat_2), y[0], y[1]);
-        unpair(fma2(pair(f32(x[j + 2]), f32(x[j + 3])), scale_2, BIAS ? pair(bias[j + 2], bias[j + 3]) : flat_2), y[2], y[3]);
+        Pair y0 = fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, BIAS ? pair(bias[j], bias[j + 1]) : flat_2);
+        Pair y1 = fma2(pair(f32(x[j + 2]), f32(x[j + 3])), scale_2, BIAS ? pair(bias[j + 2], bias[j + 3]) : flat_2);
         if (LIMIT) {
             const float4 lim = *reinterpret_cast<const float4*>(limit + j);
-            y[0] = fminf(y[0], lim.x);
-            y[1] = fminf(y[1], lim.y);
-            y[2] = fminf(y[2], lim.z);
-            y[3] = fminf(y[3], lim.w);
+            y0 = add2(y0, pair(lim.x, lim.y));
+            y1 = add2(y1, pair(lim.z, lim.w));
         }
+        float y[4];
+        unpair(y0, y[0], y[1]);
+        unpair(y1, y[2], y[3]);
         top[0] = max3(top[0], y[0], y[1]);
         top[1] = max3(top[1], y[2], y[3]);
 #pragma unroll
@@ -192,6 +194,10 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     float* limits = reinterpret_cast<float*>(base + L::kLim);
     uint32_t* wholes = reinterpret_cast<uint32_t*>(limits + S * KT);  // tile without a masked key
 
+    const bool masks = p.key_mask != nullptr || len % KT != 0;
+    const auto k_bar = [&](int s) { return masks ? at(bar->k_ready[s]) : at(bar->k_full[s]); };
+    const auto v_bar = [&](int s) { return masks ? at(bar->v_ready[s]) : at(bar->v_full[s]); };
+
     // tiles are numbered over all query blocks: number i is key tile i % n of block i / n
     const auto load_k = [&](int i, int kt) {
         const int s = i % S;
@@ -200,6 +206,14 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             for (int x = 0; x < KT; x += kBox)
                 umma::tma_load_4d(sm + L::kK + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.k, c * L::kCols, g * p.k_h,
                                   (first + kt) * KT + x, b * p.k_b, at(bar->k_full[s]));
+    };
+    const auto load_v = [&](int i, int kt) {
+        const int s = i % S;
+        umma::mbar_arrive_expect_tx(at(bar->v_full[s]), L::kBytes);
+        for (int c = 0; c < L::kChunks; ++c)
+            for (int x = 0; x < KT; x += kBox)
+                umma::tma_load_4d(sm + L::kV + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.v, c * L::kCols, g * p.v_h,
+                                  (first + kt) * KT + x, b * p.v_b, at(bar->v_full[s]));
     };
     const auto load_q = [&](int qi) {
         const int tiles = tiles_of(qi);
@@ -216,6 +230,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         umma::mbar_init(at(bar->q_empty), NT);  // one MMA warp per tile
         for (int s = 0; s < S; ++s) {
             umma::mbar_init(at(bar->k_full[s]), 1);
+            umma::mbar_init(at(bar->k_ready[s]), 1);
+            umma::mbar_init(at(bar->v_ready[s]), 1);
             umma::mbar_init(at(bar->k_empty[s]), NT);
             umma::mbar_init(at(bar->v_full[s]), 1);
             umma::mbar_init(at(bar->v_empty[s]), NT);
@@ -231,11 +247,11 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         if (n > 0) {
             load_q(0);
             load_k(0, 0);
+            load_v(0, 0);
         }
     }
     RelRange range;  // positions j - i - q_offset of the tiles, padded rows and columns included
     float* values = reinterpret_cast<float*>(base + L::kBias);
-    uint8_t* buckets = base + L::kBias + 4 * p.max_entries;
     if (p.rel.per_side != 0 && n > 0) {
         range = rel_range(p.rel, first * KT - (q_of(nq) - 1) - p.rel.q_offset,
                           (first + n) * KT - 1 - q_of(0) - p.rel.q_offset);
@@ -243,7 +259,6 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         table.load(p.rel, p.table, h, lane);
         for (int e0 = warp * 32; warp < NT * 4 && e0 < range.count(); e0 += NT * 128) {  // the other warps have their own starts
             const int e = min(e0 + lane, range.count() - 1), bu = rel_bucket(p.rel, range.lo + e);
-            buckets[e] = static_cast<uint8_t>(bu);
             values[e] = table.get(p.rel, bu);
         }
     }
@@ -255,47 +270,79 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
 
     if (warp == NT * 5) {
         bool ok = true;
-        int kt = 0, qi = 0;
-        for (int i = 0; i < nq * n; ++i) {
-            const int s = i % S;
-            const uint32_t ph = (i / S + 1) & 1;
-            if (i > 0 && lane == 0) {
-                if (kt == 0) {
-                    ok = ok && umma::mbar_poll(at(bar->q_empty), (qi - 1) & 1);
-                    if (ok) load_q(qi);
+        int load_kt = 0, load_qi = 0;  // of the next tile to load
+        const auto load = [&](int i) {  // lane 0; tile 0 is on its way already
+            if (i > 0) {
+                const int s = i % S;
+                const uint32_t ph = (i / S + 1) & 1;
+                if (load_kt == 0) {
+                    ok = ok && umma::mbar_poll(at(bar->q_empty), (load_qi - 1) & 1);
+                    if (ok) load_q(load_qi);
                 }
                 ok = ok && umma::mbar_poll(at(bar->k_empty[s]), ph);
-                if (ok) load_k(i, kt);
+                if (ok) load_k(i, load_kt);
+                ok = ok && umma::mbar_poll(at(bar->v_empty[s]), ph);
+                if (ok) load_v(i, load_kt);
             }
-            if (lane == 0) ok = ok && umma::mbar_poll(at(bar->v_empty[s]), ph);
-            __syncwarp();
-            // limits of the tile's keys (read until its P V is done, as V is)
-            const int cols = cols_of(kt), k0 = (first + kt) * KT;
-            if (p.key_mask != nullptr || cols < KT) {
-                bool all = true;
+            if (++load_kt == n) {
+                load_kt = 0;
+                ++load_qi;
+            }
+        };
+        const int total = nq * n;
+        if (!masks) {
+            if (lane == 0)
+                for (int i = 0; i < total && ok; ++i) load(i);
+        } else if (n > 0) {
+            // Tile i - 1 + S is asked for when tile i has been cleared: it waits for the products
+            // of tile i - 1, and, where a query block ends between (one tile of queries, S = 2),
+            // for the scores of tile i.
+            static_assert(NT == 2 || S == 2, "query blocks follow one another");
+            if (lane == 0) load(0);
+            if (lane == 0 && n > 1)
+                for (int i = 1; i < S && i < n; ++i) load(i);
+            int loaded = min(S, n), kt = 0;
+            for (int i = 0; i < total; ++i) {
+                const int s = i % S, k0 = (first + kt) * KT;
+                uint32_t in_mask = 0;
 #pragma unroll
                 for (int c = 0; c < KT; c += 32) {
-                    const bool in = c + lane < cols &&
-                                    (p.key_mask == nullptr ||
-                                     __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + k0 + c + lane) != 0);
-                    limits[s * KT + c + lane] = in ? INFINITY : -INFINITY;
-                    all = all && in;
+                    const int key = k0 + c + lane;
+                    if (key < len && (p.key_mask == nullptr || __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + key) != 0))
+                        in_mask |= 1u << (c / 32);
                 }
-                all = __all_sync(~0u, all);
-                if (lane == 0) wholes[s] = all;
+                ok = __shfl_sync(~0u, ok, 0);
+                bool all = true;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    ok = ok && umma::mbar_poll(kv == 0 ? at(bar->k_full[s]) : at(bar->v_full[s]), (i / S) & 1);
+#pragma unroll
+                    for (int c = 0; c < KT; c += 32) {
+                        const bool in = (in_mask >> (c / 32)) & 1;
+                        all = all && in;
+                        if (kv == 0) limits[s * KT + c + lane] = in ? 0.0f : -INFINITY;
+                        if (!in) {
+                            const uint32_t to = sm + (kv == 0 ? L::kK : L::kV) + s * L::kBytes + (c + lane) * L::kRow;
+                            for (int x = 0; x < L::kChunks; ++x)
+#pragma unroll
+                                for (int j = 0; j < L::kRow; j += 16) umma::st_shared_v4(to + x * L::kChunk + j, 0, 0, 0, 0);
+                        }
+                    }
+                    if (kv == 0) {
+                        all = __all_sync(~0u, all);
+                        if (lane == 0) wholes[s] = all;
+                    }
+                    umma::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) umma::mbar_arrive(kv == 0 ? at(bar->k_ready[s]) : at(bar->v_ready[s]));
+                }
+                // tiles of the next block follow their block's last one (S = 2: tile i + 1)
+                while (loaded < total && loaded <= max(i - 1 + S, i + 1)) {
+                    if (lane == 0) load(loaded);
+                    ++loaded;
+                }
                 __syncwarp();
-            }
-            if (lane == 0 && ok) {
-                umma::mbar_arrive_expect_tx(at(bar->v_full[s]), L::kBytes);
-                for (int c = 0; c < L::kChunks; ++c)
-                    for (int x = 0; x < KT; x += kBox)
-                        umma::tma_load_4d(sm + L::kV + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.v, c * L::kCols,
-                                          g * p.v_h, k0 + x, b * p.v_b, at(bar->v_full[s]));
-            }
-            if (!__shfl_sync(~0u, ok, 0)) break;
-            if (++kt == n) {
-                kt = 0;
-                ++qi;
+                if (++kt == n) kt = 0;
             }
         }
         if (lane == 0 && !ok) record_device_error(p.err, kErrMbarTimeout | 0x20);
@@ -307,20 +354,20 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             // product needs is in uniform registers (formed per product in one thread
             // they took 100 clocks each, more than the products).
             constexpr bool bf = !std::is_same<T, __half>::value;
-            constexpr uint32_t id_full = umma::idesc_16bit(bf, kTile, KT, false), id_o = umma::idesc_16bit(bf, kTile, DP, true);
+            // all columns of a tile: those beyond its keys are products with zeros, not what TMEM held
+            constexpr uint32_t id_s = umma::idesc_16bit(bf, kTile, KT, false), id_o = umma::idesc_16bit(bf, kTile, DP, true);
             const uint32_t s_col = __reduce_or_sync(~0u, tmem) + t * KT, o_col = s_col + (NT - t) * KT + t * DP;
             const uint64_t q_desc = umma::smem_desc_swizzled<L::kRow>(sm + t * L::kQBytes, 16);
             const uint64_t k_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kK, 16);
             const uint64_t v_desc = umma::smem_desc_swizzled<L::kRow>(sm + L::kV, L::kChunk);
             const auto qk = [&](int i, int kt) {
-                const int s = i % S, cols = cols_of(kt);
-                const uint32_t id = cols >= KT ? id_full : umma::idesc_16bit(bf, kTile, (cols + 15) / 16 * 16, false);
+                const int s = i % S;
                 const uint64_t kd = umma::desc_advance(k_desc, s * L::kBytes);
                 if (umma::elect_one()) {
 #pragma unroll
                     for (int j = 0; j < DP / 16; ++j)
                         umma::mma_f16_ss(s_col, umma::desc_advance(q_desc, j * 16 / L::kCols * L::kQChunk + j * 16 % L::kCols * 2),
-                                         umma::desc_advance(kd, j * 16 / L::kCols * L::kChunk + j * 16 % L::kCols * 2), id, j > 0);
+                                         umma::desc_advance(kd, j * 16 / L::kCols * L::kChunk + j * 16 % L::kCols * 2), id_s, j > 0);
                     umma::mma_commit(at(bar->s_full[t]));
                     umma::mma_commit(at(bar->k_empty[s]));
                     if (kt == n - 1) umma::mma_commit(at(bar->q_empty));
@@ -336,18 +383,18 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     if (ok && lane == 0) umma::mbar_arrive(at(bar->q_empty));
                     for (int kt = 0; kt < n && ok; ++kt, ++i) {
                         const int s = i % S;
-                        ok = umma::mbar_poll(at(bar->k_full[s]), (i / S) & 1);
+                        ok = umma::mbar_poll(k_bar(s), (i / S) & 1);
                         if (ok && lane == 0) umma::mbar_arrive(at(bar->k_empty[s]));
-                        ok = ok && umma::mbar_poll(at(bar->v_full[s]), (i / S) & 1);
+                        ok = ok && umma::mbar_poll(v_bar(s), (i / S) & 1);
                         if (ok && lane == 0) umma::mbar_arrive(at(bar->v_empty[s]));
                     }
                     continue;
                 }
-                ok = ok && umma::mbar_poll(at(bar->k_full[i % S]), (i / S) & 1);
+                ok = ok && umma::mbar_poll(k_bar(i % S), (i / S) & 1);
                 if (ok) qk(i, 0);
                 for (int kt = 0; kt < n && ok; ++kt, ++i) {
                     const int s = i % S, cols = cols_of(kt);
-                    ok = umma::mbar_poll(at(bar->v_full[s]), (i / S) & 1) && umma::mbar_poll(at(bar->p_ready[t]), i & 1);
+                    ok = umma::mbar_poll(v_bar(s), (i / S) & 1) && umma::mbar_poll(at(bar->p_ready[t]), i & 1);
                     // the O before has been read
                     if (kt == 0 && qi > 0) ok = ok && umma::mbar_poll(at(bar->o_free[t]), (qi - 1) & 1);
                     if (!ok) break;
@@ -363,7 +410,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     }
                     __syncwarp();
                     if (kt + 1 < n) {
-                        ok = umma::mbar_poll(at(bar->k_full[(i + 1) % S]), ((i + 1) / S) & 1);
+                        ok = umma::mbar_poll(k_bar((i + 1) % S), ((i + 1) / S) & 1);
                         if (ok) qk(i + 1, kt + 1);
                     }
                 }
@@ -387,17 +434,14 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 float flat = 0.0f;
                 const float* mine = nullptr;
                 if (p.rel.per_side != 0) {
-                    const int lo = k0 - (q0 + t * kTile + kTile - 1) - p.rel.q_offset;
-                    if (bucket_at(range, buckets, lo) == bucket_at(range, buckets, lo + kTile + KT - 2))
+                    const int lo = k0 - (q0 + t * kTile + kTile - 1) - p.rel.q_offset, hi = lo + kTile + KT - 2;
+                    if (hi <= -p.rel.max_distance || lo >= p.rel.max_distance || (!p.rel.bidirectional && lo >= 0))
                         flat = values[min(max(lo, range.lo), range.hi) - range.lo];
                     else
                         mine = values + k0 - i - p.rel.q_offset - range.lo;
                 }
-                bool whole = cols == KT;
-                if (!whole || p.key_mask != nullptr) {
-                    ok = ok && umma::mbar_poll(at(bar->v_full[s]), (number / S) & 1);
-                    whole = wholes[s] != 0;
-                }
+                if (masks) ok = ok && umma::mbar_poll(at(bar->k_ready[s]), (number / S) & 1);  // its limits
+                const bool whole = !masks || wholes[s] != 0;
                 ok = ok && umma::mbar_poll(at(bar->s_full[t]), number & 1);
                 umma::fence_after_sync();
                 const int chunks = any_row ? (cols + 31) / 32 : 0;
@@ -459,16 +503,6 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     // 16 columns of P over scores that have been read
                     if (plain) exp_pass<T, true>(x, p.scale2, add, l2, s_col + c * 16);
                     else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c * 16);
-                }
-                if (!whole) {
-                    // rows of V behind masked keys: 0 in place of whatever they hold
-                    if (r < KT && lim[r] < 0.0f) {
-                        for (int c = 0; c < L::kChunks; ++c)
-#pragma unroll
-                            for (int j = 0; j < L::kRow; j += 16)
-                                umma::st_shared_v4(sm + L::kV + s * L::kBytes + c * L::kChunk + r * L::kRow + j, 0, 0, 0, 0);
-                    }
-                    umma::fence_proxy_async_smem();
                 }
                 umma::tmem_wait_st();
                 umma::fence_before_sync();
@@ -643,7 +677,7 @@ int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, NT>;
     const auto kernel = attention_forward_kernel<T, DP, NT>;
-    const int bytes = L::kTotal + 5 * f.max_entries;
+    const int bytes = L::kTotal + 4 * f.max_entries;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
         return launch_status("cross_attention");
     kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
