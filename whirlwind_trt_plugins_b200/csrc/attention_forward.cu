@@ -48,6 +48,7 @@
 #include "umma.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ww {
 namespace {
@@ -109,15 +110,15 @@ struct Bars {
     uint32_t tmem;
 };
 
-// 32 scores in log2 units with bias and limits, and their maximum.
-template <bool BIAS, bool LIMIT>
-__device__ __forceinline__ float score_pass(uint32_t (&x)[32], float scale2, float flat, const float* bias,
+// N scores in log2 units with bias and limits, and their maximum.
+template <bool BIAS, bool LIMIT, int N>
+__device__ __forceinline__ float score_pass(uint32_t (&x)[N], float scale2, float flat, const float* bias,
                                             const float* limit)
 {
     float top[2] = {-INFINITY, -INFINITY};
     const Pair scale_2 = pair(scale2, scale2), flat_2 = pair(flat, flat);
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
+    for (int j = 0; j < N; j += 4) {
         Pair y0 = fma2(pair(f32(x[j]), f32(x[j + 1])), scale_2, BIAS ? pair(bias[j], bias[j + 1]) : flat_2);
         Pair y1 = fma2(pair(f32(x[j + 2]), f32(x[j + 3])), scale_2, BIAS ? pair(bias[j + 2], bias[j + 3]) : flat_2);
         if (LIMIT) {
@@ -136,16 +137,16 @@ __device__ __forceinline__ float score_pass(uint32_t (&x)[32], float scale2, flo
     return fmaxf(top[0], top[1]);
 }
 
-// P = 2^(mul x + add) of 32 columns: summed, rounded and put into 16 columns of
+// P = 2^(mul x + add) of N columns: summed, rounded and put into N / 2 columns of
 // TMEM.  POLY: one pair in kPolyOf on the FMA pipe (whole tiles without a bias
 // of their own: there no argument is -inf).
-template <typename T, bool POLY>
-__device__ __forceinline__ void exp_pass(const uint32_t (&x)[32], float mul, float add, Pair& sum, uint32_t to)
+template <typename T, bool POLY, int N>
+__device__ __forceinline__ void exp_pass(const uint32_t (&x)[N], float mul, float add, Pair& sum, uint32_t to)
 {
-    uint32_t pk[16];
+    uint32_t pk[N / 2];
     const Pair mul_2 = pair(mul, mul), add_2 = pair(add, add);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < N / 2; ++j) {
         const Pair arg = fma2(pair(f32(x[2 * j]), f32(x[2 * j + 1])), mul_2, add_2);
         float a, b;
         if (POLY && j % kPolyOf == kPolyOf - 1) {
@@ -158,7 +159,8 @@ __device__ __forceinline__ void exp_pass(const uint32_t (&x)[32], float mul, flo
         sum = add2(sum, pair(a, b));
         pk[j] = pack2<T>(a, b);
     }
-    umma::tmem_st16(to, pk);
+    if constexpr (N == 32) umma::tmem_st16(to, pk);
+    else umma::tmem_st8(to, pk);
 }
 
 template <typename T, int DP, int NT>
@@ -447,17 +449,14 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 const int chunks = any_row ? (cols + 31) / 32 : 0;
                 // raw scores: scale and constant join the exponential's argument
                 const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f && flat > -INFINITY;
-                float top = -INFINITY;
+                float top = -INFINITY, add;
                 const float* lim = limits + s * KT;
-#pragma unroll 1
-                for (int c = 0; c < chunks; ++c) {
-                    uint32_t x[32];
-                    umma::tmem_ld32(s_col + c * 32, x);
-                    umma::tmem_wait_ld32(x);
-                    if (plain) {
+                const auto largest = [&](auto raw_scores, int c, auto& x) {  // of the N columns from c on
+                    constexpr int N = sizeof(x) / 4;
+                    if (raw_scores) {
                         float top1 = -INFINITY;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
+                        for (int j = 0; j < N; j += 4) {
                             top = max3(top, f32(x[j]), f32(x[j + 1]));
                             top1 = max3(top1, f32(x[j + 2]), f32(x[j + 3]));
                         }
@@ -466,16 +465,54 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                         float tc;
                         if (mine == nullptr)
                             tc = whole ? score_pass<false, false>(x, p.scale2, flat, nullptr, nullptr)
-                                       : score_pass<false, true>(x, p.scale2, flat, nullptr, lim + 32 * c);
+                                       : score_pass<false, true>(x, p.scale2, flat, nullptr, lim + c);
                         else
-                            tc = whole ? score_pass<true, false>(x, p.scale2, 0.0f, mine + 32 * c, nullptr)
-                                       : score_pass<true, true>(x, p.scale2, 0.0f, mine + 32 * c, lim + 32 * c);
+                            tc = whole ? score_pass<true, false>(x, p.scale2, 0.0f, mine + c, nullptr)
+                                       : score_pass<true, true>(x, p.scale2, 0.0f, mine + c, lim + c);
                         top = fmaxf(top, tc);
-                        umma::tmem_st32(s_col + c * 32, x);
+                        if constexpr (N == 32) umma::tmem_st32(s_col + c, x);
+                        else umma::tmem_st16(s_col + c, x);
                     }
-                }
+                };
+                const auto exps = [&](auto raw_scores, int c, const auto& x) {  // P of N columns, over scores that have been read
+                    if (raw_scores) exp_pass<T, true>(x, p.scale2, add, l2, s_col + c / 2);
+                    else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c / 2);
+                };
+                const auto columns = [&](const auto& use, auto raw_scores) {
+                    // Long queries' raw scores, the case without any other work to hide behind:
+                    // 16 at a time, the next ones on their way meanwhile (19200 to 19200, 5 heads of 64: 638 -> 600 us).
+                    // Elsewhere the registers are worth more (rows of 160: 35 us, so 39).
+                    if constexpr (NT == 2 && std::is_same<decltype(raw_scores), std::true_type>::value) {
+                        if (!any_row) return;
+                        uint32_t x[2][16];
+                        umma::tmem_ld16(s_col, x[0]);
+#pragma unroll
+                        for (int c = 0; c < KT; c += 16) {
+                            umma::tmem_wait_ld16(x[c / 16 & 1]);
+                            if (c + 16 < KT) umma::tmem_ld16(s_col + c + 16, x[c / 16 + 1 & 1]);
+                            use(raw_scores, c, x[c / 16 & 1]);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int c = 0; c < chunks; ++c) {
+                            uint32_t x[32];
+                            umma::tmem_ld32(s_col + c * 32, x);
+                            umma::tmem_wait_ld32(x);
+                            use(raw_scores, c * 32, x);
+                        }
+                    }
+                };
+                const auto pass = [&](const auto& use) {
+                    if constexpr (NT == 2) {  // the choice outside the loop, which is unrolled
+                        if (plain) columns(use, std::true_type{});
+                        else columns(use, std::false_type{});
+                    } else {
+                        columns(use, plain);
+                    }
+                };
+                pass(largest);
+                if (!plain) umma::tmem_wait_st();
                 if (plain) top = fmaf(top, p.scale2, flat);
-                else umma::tmem_wait_st();
                 // grow the maximum: always on the first tile, then only past kRescale
                 if (__any_sync(~0u, kt == 0 || top > m + kRescale)) {
                     const float mn = fmaxf(m, top);
@@ -494,16 +531,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     }
                     m = mn;
                 }
-                const float add = (plain ? flat : 0.0f) - (m == -INFINITY ? 0.0f : m);
-#pragma unroll 1
-                for (int c = 0; c < chunks; ++c) {
-                    uint32_t x[32];
-                    umma::tmem_ld32(s_col + c * 32, x);
-                    umma::tmem_wait_ld32(x);
-                    // 16 columns of P over scores that have been read
-                    if (plain) exp_pass<T, true>(x, p.scale2, add, l2, s_col + c * 16);
-                    else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c * 16);
-                }
+                add = (plain ? flat : 0.0f) - (m == -INFINITY ? 0.0f : m);
+                pass(exps);
                 umma::tmem_wait_st();
                 umma::fence_before_sync();
                 __syncwarp();
