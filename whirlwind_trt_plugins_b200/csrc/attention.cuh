@@ -304,6 +304,13 @@ __device__ __forceinline__ void wait_for_launches_before()
     asm volatile("griddepcontrol.wait;" : : : "memory");
 }
 
+// Lets the kernel launched behind this one start wherever CTAs of this grid are
+// none to come any more (it begins once all of them have called this).
+__device__ __forceinline__ void start_launch_behind()
+{
+    asm volatile("griddepcontrol.launch_dependents;" : : : "memory");
+}
+
 // Share [first, first + n) of part `split` of `splits` in `all` steps (a 64-bit
 // division is worth avoiding where there is one part).
 __device__ __forceinline__ void part_of(int all, int split, int splits, int& first, int& n)

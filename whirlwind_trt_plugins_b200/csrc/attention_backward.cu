@@ -35,6 +35,8 @@
 #include "tensor_map.cuh"
 #include "umma.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -137,6 +139,10 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
     const uint32_t sm = umma::smem_addr(base);
     Bar* bar = reinterpret_cast<Bar*>(base + L::kBar);
     const auto at = [](const uint64_t& b) { return umma::smem_addr(&b); };
+
+    // `keys` waits for the deltas; `queries` starts while the last CTAs of `keys` run,
+    // which have seen the deltas complete: it reads them past the L1 caches
+    if (KEYS) wait_for_launches_before();
 
     // items (row block, head, batch item); the last ones are split over their streamed tiles
     const int blk = blockIdx.x;
@@ -257,6 +263,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = bar->tmem;
+    if (KEYS) start_launch_behind();  // this CTA has its TMEM columns
     // queries with masked keys: the load warp clears their rows of K and V before a
     // tile is used (its products then see zeros, whatever the places held) and
     // leaves limits (0 or -inf) that join the scores
@@ -393,7 +400,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         // fp16: f = 2^e, e = 127 - the biased exponent of max |dO|
         float f = 1.0f;
         if (kHalf) {
-            const int top = static_cast<int>(__ldg(p.top) >> 23);
+            const int top = static_cast<int>(__ldcg(p.top) >> 23);
             if (top > 0 && top < 255) f = __int_as_float((254 - top) << 23);
         }
         bool row_ok = row < (KEYS ? len : p.Lq);
@@ -402,8 +409,8 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             if (row_ok && p.key_mask != nullptr) row_ok = __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + row) != 0;
         } else if (row_ok) {
             const int64_t i = (static_cast<int64_t>(b) * p.Hq + h) * p.Lq_pad + row;
-            my_nlse = __ldg(p.nlse2 + i);
-            my_ndelta = __ldg(p.ndelta + i) * f;
+            my_nlse = __ldcg(p.nlse2 + i);
+            my_ndelta = __ldcg(p.ndelta + i) * f;
         }
         const bool any_row = row0 + warp % 4 * 32 < (KEYS ? len : p.Lq);  // else this warp keeps the barriers only
         const Pair scale_2 = pair(p.scale2, p.scale2), f_2 = pair(f, f), ndelta_2 = pair(my_ndelta, my_ndelta);
@@ -619,7 +626,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         const float* plain = values + (1 + kGroups) * entries;
         float back = 1.0f / (1 << kShift);
         if (kHalf) {
-            const int top = static_cast<int>(__ldg(p.top) >> 23);
+            const int top = static_cast<int>(__ldcg(p.top) >> 23);
             if (top > 0 && top < 255) back *= __int_as_float(top << 23);  // 1 / f
         }
         const int sub = lane % 8;
@@ -639,6 +646,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             if (sub == 0 && t0 + lane / 8 < p.rel.total) p.table_part[static_cast<int64_t>(blk) * p.rel.total + t] = sum * back;
         }
     }
+    if (!KEYS) wait_for_launches_before();  // what follows this grid may read what `keys` wrote
 }
 
 // -delta = -rowsum(dO * O) and kShift - lse in log2 units, both laid out
@@ -689,71 +697,94 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
     }
 }
 
-// Joins the parts of the split items in order: kSumRows rows of an item and
-// output per CTA, 4 values per thread and step.
+// Joins the parts of both kernels' split items in order: kSumRows rows of an item
+// and output per CTA, 4 values per thread and step.
 constexpr int kSumRows = 8;
+struct SumParams {
+    const float* part;
+    void *d1, *d2;
+    int32_t count, whole_items, splits, outputs;  // CTAs along x (outputs of split items) and what they join
+    int32_t blocks, heads, L;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) attention_sum_kernel(const float* part, int whole_items, int splits, int outputs,
-                                                            T* d1, T* d2, int blocks, int heads, int L, int D)
+__global__ void __launch_bounds__(256) attention_sum_kernel(const SumParams keys, const SumParams queries, int D)
 {
-    const int k = blockIdx.x / outputs, which = blockIdx.x % outputs, item = whole_items + k;
-    const int row0 = item % blocks * kRows, h = item / blocks % heads;
-    const int64_t b = item / blocks / heads;
-    T* out = which == 0 ? d1 : d2;
+    wait_for_launches_before();
+    const bool second = static_cast<int>(blockIdx.x) >= keys.count;
+    const SumParams& p = second ? queries : keys;
+    const int x = blockIdx.x - (second ? keys.count : 0);
+    const int k = x / p.outputs, which = x % p.outputs, item = p.whole_items + k;
+    const int row0 = item % p.blocks * kRows, h = item / p.blocks % p.heads;
+    const int64_t b = item / p.blocks / p.heads;
+    T* out = static_cast<T*>(which == 0 ? p.d1 : p.d2);
     const int begin = blockIdx.y * kSumRows * D;
     for (int e = begin + threadIdx.x * 4; e < begin + kSumRows * D; e += 256 * 4) {
         const int r = e / D, d = e - r * D;
-        if (row0 + r >= L) break;
+        if (row0 + r >= p.L) break;
         float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll 8
-        for (int n = 0; n < splits; ++n) {
+        for (int n = 0; n < p.splits; ++n) {
             const float4 v = *reinterpret_cast<const float4*>(
-                part + ((static_cast<int64_t>(k) * splits + n) * outputs + which) * kRows * D + e);
+                p.part + ((static_cast<int64_t>(k) * p.splits + n) * p.outputs + which) * kRows * D + e);
             s.x += v.x;
             s.y += v.y;
             s.z += v.z;
             s.w += v.w;
         }
-        *reinterpret_cast<uint2*>(out + ((b * L + row0 + r) * heads + h) * D + d) =
+        *reinterpret_cast<uint2*>(out + ((b * p.L + row0 + r) * p.heads + h) * D + d) =
             make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
     }
 }
 
 // Table gradient of one head: the CTAs' buckets in order.  Items are numbered
 // (batch item, head, block); those from whole_items on have `splits` CTAs each.
-// Each of 32 warps takes every 32nd item of the head (item numbers grow with n),
-// 32 buckets at a time, then the warps' sums in order.
+// Each of the 256 warps of a cluster takes every 256th item of the head (item
+// numbers grow with n), 32 buckets at a time; then the warps' sums in order, and
+// the CTAs'.  1080 items of 3 heads: 12.6 us with one CTA per head.
+constexpr int kTableCtas = 8;
 template <typename T>
-__global__ void __launch_bounds__(1024) attention_table_kernel(const float* part, T* out, int B, int Hq, int blocks,
-                                                               int whole_items, int splits, int total)
+__global__ void __cluster_dims__(kTableCtas, 1, 1) __launch_bounds__(1024)
+    attention_table_kernel(const float* part, T* out, int B, int Hq, int blocks, int whole_items, int splits, int total)
 {
-    __shared__ float sums[32][33];
-    const int h = blockIdx.x, t = blockIdx.y * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
+    __shared__ float sums[32][33], mine[32];
+    wait_for_launches_before();
+    const auto cluster = cooperative_groups::this_cluster();
+    const int rank = blockIdx.x % kTableCtas, h = blockIdx.x / kTableCtas, lane = threadIdx.x % 32,
+              t = blockIdx.y * 32 + lane, w = threadIdx.x / 32;
+    constexpr int kWarps = 32 * kTableCtas;
     float s = 0.0f;
     if (t < total) {
         const auto item_of = [&](int n) { return (static_cast<int64_t>(n / blocks) * Hq + h) * blocks + n % blocks; };
-        int n = w;
-        for (; n + 7 * 32 < B * blocks && item_of(n + 7 * 32) < whole_items; n += 8 * 32) {  // eight loads in flight
-            float v[8];
+        int n = w * kTableCtas + rank;
+        for (; n + 3 * kWarps < B * blocks && item_of(n + 3 * kWarps) < whole_items; n += 4 * kWarps) {  // loads in flight
+            float v[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = part[item_of(n + k * 32) * total + t];
+            for (int k = 0; k < 4; ++k) v[k] = part[item_of(n + k * kWarps) * total + t];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s += v[k];
+            for (int k = 0; k < 4; ++k) s += v[k];
         }
-        for (; n < B * blocks; n += 32) {
+        for (; n < B * blocks; n += kWarps) {
             const int64_t item = item_of(n);
             const bool one = item < whole_items;
             const int64_t at = one ? item : whole_items + (item - whole_items) * splits;
             for (int k = 0; k < (one ? 1 : splits); ++k) s += part[(at + k) * total + t];
         }
     }
-    sums[w][threadIdx.x % 32] = s;
+    sums[w][lane] = s;
     __syncthreads();
-    if (w == 0 && t < total) {
+    if (w == 0) {
         s = 0.0f;
-        for (int n = 0; n < 32; ++n) s += sums[n][threadIdx.x];
+        for (int n = 0; n < 32; ++n) s += sums[n][lane];
+        mine[lane] = s;
+    }
+    cluster.sync();
+    if (rank == 0 && w == 0 && t < total) {
+        s = 0.0f;
+        for (int n = 0; n < kTableCtas; ++n) s += *cluster.map_shared_rank(mine + lane, n);
         out[h * total + t] = from_float<T>(s);
     }
+    cluster.sync();  // until the sums have been read
 }
 
 // How one of the two kernels runs: the items that do not fill a round of the
@@ -778,7 +809,7 @@ Half make_half(int blocks, int64_t items, int64_t tiles, int slots) noexcept
 struct Plan {
     Half q, k;
     int Lq_pad;
-    int64_t nlse2, ndelta, part, table, bytes;  // byte offsets; the maximum of |dO| stands first
+    int64_t nlse2, ndelta, q_part, k_part, table, bytes;  // byte offsets; the maximum of |dO| stands first
 };
 
 bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
@@ -795,51 +826,53 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     const int64_t q_part = i64(r.q.rest) * r.q.splits * kRows * p.D * 4, k_part = i64(r.k.rest) * r.k.splits * 2 * kRows * p.D * 4;
     r.nlse2 = 256;
     r.ndelta = r.nlse2 + rows * 4;
-    r.part = r.ndelta + rows * 4;  // one after the other: both kernels use the same place
-    r.table = r.part + std::max(q_part, k_part);
+    r.q_part = r.ndelta + rows * 4;
+    r.k_part = r.q_part + q_part;
+    r.table = r.k_part + k_part;
     r.bytes = r.table + (p.bias_table != nullptr ? r.q.ctas() * p.num_buckets * 4 : 0);
     return true;
 }
 
 template <typename T, int DP, bool KEYS, bool BIAS>
-int launch_one(const BwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
+int launch_one(const BwdParams& f, int64_t ctas, bool behind, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, KEYS>;
     const auto kernel = attention_backward_kernel<T, DP, KEYS, BIAS>;
     const int bytes = 1024 + L::kBias + (BIAS ? bias_bytes(KEYS, L::kGroups, f.max_entries, f.rel.total) : 0);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
         return launch_status("cross_attention_backward");
-    kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
+    if (behind) launch_behind(kernel, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), bytes, stream, f);
+    else kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
     return launch_status("cross_attention_backward");
 }
 
 template <typename T, bool KEYS>
-int launch(const BwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
+int launch(const BwdParams& f, int64_t ctas, bool behind, cudaStream_t stream) noexcept
 {
     if (ctas == 0) return WW_SUCCESS;
     const int dp = f.D <= 32 ? 32 : f.D <= 64 ? 64 : 128;
     if (f.table != nullptr)
-        return dp == 32 ? launch_one<T, 32, KEYS, true>(f, ctas, stream)
-             : dp == 64 ? launch_one<T, 64, KEYS, true>(f, ctas, stream) : launch_one<T, 128, KEYS, true>(f, ctas, stream);
-    return dp == 32 ? launch_one<T, 32, KEYS, false>(f, ctas, stream)
-         : dp == 64 ? launch_one<T, 64, KEYS, false>(f, ctas, stream) : launch_one<T, 128, KEYS, false>(f, ctas, stream);
+        return dp == 32 ? launch_one<T, 32, KEYS, true>(f, ctas, behind, stream)
+             : dp == 64 ? launch_one<T, 64, KEYS, true>(f, ctas, behind, stream) : launch_one<T, 128, KEYS, true>(f, ctas, behind, stream);
+    return dp == 32 ? launch_one<T, 32, KEYS, false>(f, ctas, behind, stream)
+         : dp == 64 ? launch_one<T, 64, KEYS, false>(f, ctas, behind, stream) : launch_one<T, 128, KEYS, false>(f, ctas, behind, stream);
 }
 
 template <typename T, bool KEYS>
-int run_half(BwdParams& f, const Half& half, cudaStream_t stream) noexcept
+int run_half(BwdParams& f, const Half& half, bool behind, cudaStream_t stream) noexcept
 {
     f.blocks = half.blocks;
     f.by_block = make_divisor(half.blocks > 0 ? half.blocks : 1);
     f.by_head = make_divisor(KEYS ? f.Hk : f.Hq);
     f.whole_items = half.whole;
     f.splits = half.splits;
-    const int st = launch<T, KEYS>(f, half.ctas(), stream);
-    if (st != WW_SUCCESS || half.rest == 0) return st;
-    constexpr int outputs = KEYS ? 2 : 1;
-    attention_sum_kernel<T><<<dim3(half.rest * outputs, kRows / kSumRows), 256, 0, stream>>>(f.part, half.whole, half.splits, outputs,
-                                                                     static_cast<T*>(f.d1), static_cast<T*>(f.d2), half.blocks,
-                                                                     KEYS ? f.Hk : f.Hq, KEYS ? f.Lk : f.Lq, f.D);
-    return launch_status("cross_attention_backward");
+    return launch<T, KEYS>(f, half.ctas(), behind, stream);
+}
+
+SumParams sum_params(const Half& half, bool keys, const float* part, void* d1, void* d2, int heads, int L) noexcept
+{
+    const int outputs = keys ? 2 : 1;
+    return {part, d1, d2, half.rest * outputs, half.whole, half.splits, outputs, half.blocks, heads, L};
 }
 
 template <typename T>
@@ -863,7 +896,6 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     f.top = reinterpret_cast<uint32_t*>(ws);
     f.nlse2 = reinterpret_cast<float*>(ws + plan.nlse2);
     f.ndelta = reinterpret_cast<float*>(ws + plan.ndelta);
-    f.part = reinterpret_cast<float*>(ws + plan.part);
     f.table_part = reinterpret_cast<float*>(ws + plan.table);
     if (p.bias_table != nullptr)
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
@@ -903,6 +935,7 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     }
     const int far = 2 * (p.max_distance + kRelMargin) + 1;
     if (st == WW_SUCCESS && has_k) {
+        f.part = reinterpret_cast<float*>(ws + plan.k_part);
         f.d1 = p.dk;
         f.d2 = p.dv;
         f.r1 = p.k;
@@ -910,9 +943,10 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
         std::copy(p.k_strides, p.k_strides + 3, f.r1_strides);
         std::copy(p.v_strides, p.v_strides + 3, f.r2_strides);
         f.max_entries = std::min(far, plan.Lq_pad + kRows);
-        st = run_half<T, true>(f, plan.k, stream);
+        st = run_half<T, true>(f, plan.k, has_q, stream);
     }
     if (st == WW_SUCCESS && has_q) {
+        f.part = reinterpret_cast<float*>(ws + plan.q_part);
         f.d1 = p.dq;
         f.d2 = nullptr;
         f.r1 = p.q;
@@ -920,12 +954,19 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
         std::copy(p.q_strides, p.q_strides + 3, f.r1_strides);
         std::copy(p.dout_strides, p.dout_strides + 3, f.r2_strides);
         f.max_entries = std::min(far, (p.Lk + kCols - 1) / kCols * kCols + kRows);
-        st = run_half<T, false>(f, plan.q, stream);
+        st = run_half<T, false>(f, plan.q, has_k, stream);
+    }
+    const SumParams keys = sum_params(plan.k, true, reinterpret_cast<const float*>(ws + plan.k_part), p.dk, p.dv, p.Hk, p.Lk);
+    const SumParams queries = sum_params(plan.q, false, reinterpret_cast<const float*>(ws + plan.q_part), p.dq, nullptr, p.Hq, p.Lq);
+    if (st == WW_SUCCESS && keys.count + queries.count > 0) {
+        launch_behind(attention_sum_kernel<T>, dim3(keys.count + queries.count, kRows / kSumRows), dim3(256), 0, stream, keys,
+                      queries, p.D);
+        st = launch_status("cross_attention_backward");
     }
     if (st == WW_SUCCESS && p.bias_table != nullptr) {
-        attention_table_kernel<T><<<dim3(p.Hq, (p.num_buckets + 31) / 32), 1024, 0, stream>>>(
-            f.table_part, static_cast<T*>(p.dbias_table), has_q ? p.B : 0, p.Hq, plan.q.blocks, plan.q.whole, plan.q.splits,
-            p.num_buckets);
+        launch_behind(attention_table_kernel<T>, dim3(p.Hq * kTableCtas, (p.num_buckets + 31) / 32), dim3(1024), 0, stream,
+                      f.table_part, static_cast<T*>(p.dbias_table), has_q ? p.B : 0, p.Hq, plan.q.blocks, plan.q.whole,
+                      plan.q.splits, p.num_buckets);
         st = launch_status("cross_attention_backward");
     }
     return st;
