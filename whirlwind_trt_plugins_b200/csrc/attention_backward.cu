@@ -821,7 +821,11 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     if (q_items > (1 << 30) || k_items > (1 << 30)) return false;
     const int q_slots = sms * (p.D > 64 ? 1 : 2), k_slots = sms * (p.D > 32 ? 1 : 2);  // Layout::kCtas
     r.q = make_half(q_blocks, q_items, (p.Lk + kCols - 1) / kCols, q_slots);
-    r.k = make_half(k_blocks, k_items, i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), k_slots);
+    // `queries` fills what a last round of `keys` leaves free.  Splitting that round is
+    // worth its join only where it is under half full (8 heads of a map of 4800, 8 of 148
+    // CTAs: split 446 us, else 479; 4 x 4 heads of 1777 keys, 76 CTAs: 151 and 144).
+    const bool full = q_items > 0 && k_items % k_slots * 2 >= k_slots;
+    r.k = make_half(k_blocks, k_items, full ? 1 : i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), k_slots);
     const int64_t rows = i64(p.B) * p.Hq * r.Lq_pad;
     const int64_t q_part = i64(r.q.rest) * r.q.splits * kRows * p.D * 4, k_part = i64(r.k.rest) * r.k.splits * 2 * kRows * p.D * 4;
     r.nlse2 = 256;
