@@ -68,26 +68,35 @@ def _is_device(t) -> bool:
     return t.is_cuda
 
 
-def _tensor(t, name: str, like=None, dtype=None, shape=None, contiguous=True):
-    if not isinstance(t, _Torch.Tensor) or not _is_device(t):
+def _tensor(t, name: str, device: int, dtype=None, shape=None, contiguous=True):
+    """A tensor on CUDA device `device`, with these properties where they are given."""
+    if not isinstance(t, _Torch.Tensor):
         raise TypeError(f"{name} must be a CUDA tensor")
-    if like is not None and t.get_device() != like.get_device():
-        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
+    if t.get_device() != device:
+        if not _is_device(t):
+            raise TypeError(f"{name} must be a CUDA tensor")
+        raise ValueError(f"{name} must be on cuda:{device}, got {t.device}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t
 
 
-def _vectors(t, name: str, like=None, shape=None):
+def _first(t, name: str) -> int:
+    """Device of a call's first tensor, which the others share."""
+    if not isinstance(t, _Torch.Tensor) or not _is_device(t):
+        raise TypeError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _vectors(t, name: str, device: int, dtype=None, shape=None):
     """A [B, L, H, D] tensor with strides the kernels take; returns its (b, l, h) strides in elements."""
-    _tensor(t, name, like, None if like is None else like.dtype, shape, False)
-    if t.dim() != 4:
-        raise ValueError(f"{name} must be [B, L, H, D]")
+    _tensor(t, name, device, dtype, shape, False)
     st = t.stride()
+    if len(st) != 4:
+        raise ValueError(f"{name} must be [B, L, H, D]")
     if not t.is_contiguous() and t.numel():
         step = 16 // t.element_size()
         if st[3] != 1 or any(n > 1 and s % step for n, s in zip(t.shape[:3], st[:3])):
@@ -117,10 +126,6 @@ def _place(t, stream):
         yield
 
 
-def _here(t, stream) -> bool:
-    return stream is None and t.get_device() == _Torch.device()
-
-
 def _workspace(n: int, like):
     return _Torch.empty(n, dtype=_Torch.uint8, device=like.device)
 
@@ -131,33 +136,36 @@ def _ptr(t) -> int:
 
 def _rope_args(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos):
     T = _Torch.get()
-    qs = _vectors(q, "q")
-    dt = T.dtypes.get(q.dtype)
+    at = _first(q, "q")
+    dtype = q.dtype
+    qs = _vectors(q, "q", at)
+    dt = T.dtypes.get(dtype)
     if dt is None:
         raise TypeError("q must be float16, bfloat16 or float32")
     B, Lq, Hq, D = q.shape
-    ks = _vectors(k, "k", q)
-    if k.shape[0] != B or k.shape[3] != D:
+    ks = _vectors(k, "k", at, dtype)
+    Bk, Lk, Hk, Dk = k.shape
+    if Bk != B or Dk != D:
         raise ValueError(f"k must be [{B}, Lk, Hk, {D}], got {tuple(k.shape)}")
-    _tensor(q_weight, "q_weight", q, q.dtype, (D,))
-    _tensor(k_weight, "k_weight", q, q.dtype, (D,))
-    _tensor(cos, "cos", q, T.f32)
-    _tensor(sin, "sin", q, T.f32, cos.shape)
-    if cos.dim() != 2 or 2 * cos.shape[1] > D:
+    _tensor(q_weight, "q_weight", at, dtype, (D,))
+    _tensor(k_weight, "k_weight", at, dtype, (D,))
+    table = cos.shape if isinstance(cos, T.Tensor) else ()
+    _tensor(cos, "cos", at, T.f32)
+    _tensor(sin, "sin", at, T.f32, table)
+    if len(table) != 2 or 2 * table[1] > D:
         raise ValueError("cos and sin must be [positions, R / 2] with R <= D")
-    sizes = (_pos_step(q_pos, "q_pos", q, B, Lq), _pos_step(k_pos, "k_pos", q, B, k.shape[1]), dt, B, Lq, k.shape[1], Hq,
-             k.shape[2], D, 2 * cos.shape[1], cos.shape[0])
-    return qs, ks, sizes
+    sizes = (0 if q_pos is None else _pos_step(q_pos, "q_pos", at, B, Lq),
+             0 if k_pos is None else _pos_step(k_pos, "k_pos", at, B, Lk), dt, B, Lq, Lk, Hq, Hk, D, 2 * table[1], table[0])
+    return at, qs, ks, sizes
 
 
-def _pos_step(pos, name: str, like, B: int, L: int) -> int:
+def _pos_step(pos, name: str, device: int, B: int, L: int) -> int:
     """Elements between the batch items of a position tensor."""
-    if pos is None:
+    _tensor(pos, name, device, _Torch.int32)
+    shape = pos.shape
+    if shape == (L,):
         return 0
-    _tensor(pos, name, like, _Torch.int32)
-    if pos.shape == (L,):
-        return 0
-    if pos.shape != (B, L):
+    if shape != (B, L):
         raise ValueError(f"{name} must be [{L}] or [{B}, {L}]")
     return L
 
@@ -173,15 +181,15 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_pos=None, k_pos=None, eps
     (default 0, 1, ...; clamped to the tables).  Pairs (i, i + R / 2), or
     (2i, 2i + 1) with interleaved.  Returns (q, k), contiguous, of the inputs'
     type (fp16, bf16 or fp32)."""
-    qs, ks, sizes = _rope_args(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos)
-    if not _here(q, stream):
+    at, qs, ks, sizes = _rope_args(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos)
+    if stream is not None or at != _Torch.device():
         with _place(q, stream):
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved, q_out, k_out)
     q_out, k_out = _new(q, q_out, "q_out"), _new(k, k_out, "k_out")
     a = _ROPE.pack(q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
                    sin.data_ptr(), _ptr(q_pos), _ptr(k_pos), q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0,
                    0, *qs, *ks, 0, 0, 0, 0, 0, 0, *sizes, bool(interleaved), eps)
-    _check("ww_qk_norm_rope", _lib.ww_qk_norm_rope(a, _Torch.stream(q.get_device())))
+    _check("ww_qk_norm_rope", _lib.ww_qk_norm_rope(a, _Torch.stream(at)))
     return q_out, k_out
 
 
@@ -189,10 +197,10 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, q_
                           eps: float = 1e-6, interleaved: bool = False, stream=None):
     """Gradients of ``qk_norm_rope``: (dq, dk, dq_weight, dk_weight) from those
     of its outputs; the weights' are fp32 sums over all rows, rounded once."""
-    qs, ks, sizes = _rope_args(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos)
-    gqs = _vectors(dq_out, "dq_out", q, q.shape)
-    gks = _vectors(dk_out, "dk_out", q, k.shape)
-    if not _here(q, stream):
+    at, qs, ks, sizes = _rope_args(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos)
+    gqs = _vectors(dq_out, "dq_out", at, q.dtype, q.shape)
+    gks = _vectors(dk_out, "dk_out", at, q.dtype, k.shape)
+    if stream is not None or at != _Torch.device():
         with _place(q, stream):
             return qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps,
                                          interleaved)
@@ -205,40 +213,43 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, q_
     n = _lib.ww_qk_norm_rope_backward_workspace(_ROPE.pack(*ptrs, 0, 0, *rest))
     ws = _workspace(n, q)
     _check("ww_qk_norm_rope_backward", _lib.ww_qk_norm_rope_backward(_ROPE.pack(*ptrs, ws.data_ptr(), n, *rest),
-                                                                     _Torch.stream(q.get_device())))
+                                                                     _Torch.stream(at)))
     return dq, dk, dqw, dkw
 
 
 def _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional, q_offset):
     T = _Torch.get()
-    qs = _vectors(q, "q")
-    dt = T.dtypes.get(q.dtype)
+    at = _first(q, "q")
+    dtype = q.dtype
+    qs = _vectors(q, "q", at)
+    dt = T.dtypes.get(dtype)
     if dt is None or dt == DTYPE_FLOAT:
         raise TypeError("q must be float16 or bfloat16")
     B, Lq, Hq, D = q.shape
-    ks = _vectors(k, "k", q)
-    Lk, Hk = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D:
+    ks = _vectors(k, "k", at, dtype)
+    Bk, Lk, Hk, Dk = k.shape
+    if Bk != B or Dk != D:
         raise ValueError(f"k must be [{B}, Lk, Hk, {D}], got {tuple(k.shape)}")
     if Hk == 0 or Hq % Hk:
         raise ValueError(f"{Hq} query heads cannot share {Hk} key heads evenly")
-    vs = _vectors(v, "v", q, k.shape)
+    vs = _vectors(v, "v", at, dtype, (B, Lk, Hk, D))
     if k_lens is not None:
-        _tensor(k_lens, "k_lens", q, T.int32, (B,))
+        _tensor(k_lens, "k_lens", at, T.int32, (B,))
     if key_mask is not None:
+        _tensor(key_mask, "key_mask", at, None, (B, Lk))
         if key_mask.dtype != T.bool and key_mask.dtype != T.uint8:
             raise TypeError(f"key_mask must be bool or uint8, got {key_mask.dtype}")
-        _tensor(key_mask, "key_mask", q, None, (B, Lk))
     buckets = 0
     if bias_table is not None:
-        _tensor(bias_table, "bias_table", q, q.dtype)
-        if bias_table.dim() != 2 or bias_table.shape[0] != Hq:
-            raise ValueError(f"bias_table must be [{Hq}, buckets], got {tuple(bias_table.shape)}")
-        buckets = bias_table.shape[1]
+        _tensor(bias_table, "bias_table", at, dtype)
+        table = bias_table.shape
+        if len(table) != 2 or table[0] != Hq:
+            raise ValueError(f"bias_table must be [{Hq}, buckets], got {tuple(table)}")
+        buckets = table[1]
     if scale is None:
         scale = 1.0 / math.sqrt(D) if D else 1.0
     sizes = (dt, B, Lq, Lk, Hq, Hk, D, buckets, max_distance, bool(bidirectional), q_offset, scale)
-    return qs, ks, vs, sizes
+    return at, qs, ks, vs, sizes
 
 
 def cross_attention(q, k, v, scale: float | None = None, k_lens=None, key_mask=None, bias_table=None,
@@ -256,8 +267,8 @@ def cross_attention(q, k, v, scale: float | None = None, k_lens=None, key_mask=N
     for keys before the query); q_offset is the key position of query 0.
     scale defaults to 1 / sqrt(D).  Returns out [B, Lq, Hq, D], or
     (out, lse [B, Hq, Lq] fp32) with return_lse."""
-    qs, ks, vs, sizes = _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional, q_offset)
-    if not _here(q, stream):
+    at, qs, ks, vs, sizes = _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional, q_offset)
+    if stream is not None or at != _Torch.device():
         with _place(q, stream):
             return cross_attention(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional,
                                    q_offset, return_lse, out)
@@ -271,7 +282,7 @@ def cross_attention(q, k, v, scale: float | None = None, k_lens=None, key_mask=N
     if n:
         ws = _workspace(n, q)
         a = _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes)
-    _check("ww_cross_attention", _lib.ww_cross_attention(a, _Torch.stream(q.get_device())))
+    _check("ww_cross_attention", _lib.ww_cross_attention(a, _Torch.stream(at)))
     return (out, lse) if return_lse else out
 
 
@@ -282,11 +293,11 @@ def cross_attention_backward(dout, q, k, v, out, lse, scale: float | None = None
     lse it returned: (dq, dk, dv, dbias_table); dbias_table is None without a
     table.  Shared key heads and the table get the sums over all that use
     them, in fp32 and in a fixed order."""
-    qs, ks, vs, sizes = _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional, q_offset)
-    gs = _vectors(dout, "dout", q, q.shape)
-    _tensor(out, "out", q, q.dtype, q.shape)
-    _tensor(lse, "lse", q, _Torch.f32, (q.shape[0], q.shape[2], q.shape[1]))
-    if not _here(q, stream):
+    at, qs, ks, vs, sizes = _attn_args(q, k, v, scale, k_lens, key_mask, bias_table, max_distance, bidirectional, q_offset)
+    gs = _vectors(dout, "dout", at, q.dtype, q.shape)
+    _tensor(out, "out", at, q.dtype, q.shape)
+    _tensor(lse, "lse", at, _Torch.f32, (q.shape[0], q.shape[2], q.shape[1]))
+    if stream is not None or at != _Torch.device():
         with _place(q, stream):
             return cross_attention_backward(dout, q, k, v, out, lse, scale, k_lens, key_mask, bias_table,
                                             max_distance, bidirectional, q_offset)
@@ -298,7 +309,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, scale: float | None = None
     n = _lib.ww_cross_attention_backward_workspace(_ATTN.pack(*ptrs, 0, 0, *strides, *sizes))
     ws = _workspace(n, q)
     _check("ww_cross_attention_backward", _lib.ww_cross_attention_backward(
-        _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes), _Torch.stream(q.get_device())))
+        _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes), _Torch.stream(at)))
     return dq, dk, dv, dtable
 
 
