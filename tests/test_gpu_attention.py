@@ -316,6 +316,17 @@ def test_long_axes(env, shape):
     _run_case(env, shape, "f16", "keys", None, 5)
 
 
+# Both sides of each rule that picks how a call runs: single tokens of many heads that
+# do not share keys, more and fewer than 2048 queries, several query blocks per CTA,
+# last rounds that are split over the streamed axis and ones that are not.
+@pytest.mark.parametrize("shape", [(40, 1, 100, 4, 4, 64), (25, 30, 70, 6, 6, 24), (38, 2, 90, 4, 2, 128),
+                                   (1, 2300, 300, 2, 2, 32), (1, 2100, 200, 3, 1, 64), (1, 2300, 300, 1, 1, 128),
+                                   (100, 300, 140, 3, 3, 32), (1, 300, 1500, 16, 16, 64), (2, 300, 1500, 16, 8, 128)])
+@pytest.mark.parametrize("mask,bias", [("", None), ("lens keys", (16, 100, True, 5))])
+def test_forms(env, shape, mask, bias):
+    _run_case(env, shape, "f16" if shape[1] % 4 else "bf16", mask, bias, 6)
+
+
 @pytest.mark.parametrize("Lq,Lk,B", [(0, 5, 2), (5, 0, 2), (0, 0, 1), (3, 4, 0)])
 def test_lengths_of_zero(env, Lq, Lk, B):
     torch, ww = env

@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         const int t = warp / 4, r = threadIdx.x % 128;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4) << 21;  // TMEM lane of this warp's first row
         const uint32_t s_col = tmem + lanes + t * KT, o_col = tmem + lanes + NT * KT + t * DP;
+        constexpr bool kAhead = NT == 2 || DP == 128;
         bool ok = true;  // once a wait has run out: no more waits, everything else goes on
         int number = 0;
         for (int qi = 0; qi < nq && t < tiles_of(qi); ++qi) {
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     // Long queries' raw scores, the case without any other work to hide behind:
                     // 16 at a time, the next ones on their way meanwhile (19200 to 19200, 5 heads of 64: 638 -> 600 us).
                     // Elsewhere the registers are worth more (rows of 160: 35 us, so 39).
-                    if constexpr (NT == 2 && std::is_same<decltype(raw_scores), std::true_type>::value) {
+                    if constexpr (kAhead && std::is_same<decltype(raw_scores), std::true_type>::value) {
                         if (!any_row) return;
                         uint32_t x[2][16];
                         umma::tmem_ld16(s_col, x[0]);
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     }
                 };
                 const auto pass = [&](const auto& use) {
-                    if constexpr (NT == 2) {  // the choice outside the loop, which is unrolled
+                    if constexpr (kAhead) {  // the choice outside the loop, which is unrolled
                         if (plain) columns(use, std::true_type{});
                         else columns(use, std::false_type{});
                     } else {
@@ -660,10 +661,19 @@ struct Plan {
     }
 };
 
+// Tiles one after the other in `items` CTAs of `tiles` each, the last round split
+// over its tiles where that is sooner (tail_splits).
+double tail_time(int64_t items, int slots, int64_t tiles) noexcept
+{
+    const int rest = static_cast<int>(items % slots), splits = tail_splits(rest, slots, tiles);
+    const double one = tiles + 2.5, last = splits == 1 ? one : static_cast<double>(tiles) * rest / slots + 14.0;
+    return static_cast<double>(items / slots) * one + (rest == 0 ? 0.0 : last);
+}
+
 bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
 {
     Plan& r = *plan;
-    r.token = token_form(p);
+    r.token = token_form(p, sms);
     if (r.token) {
         r.q_blocks = r.groups = r.per_cta = 0;
         r.nt = 0;
@@ -674,19 +684,23 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
         r.rest = r.splits > 1 ? p.B * p.Hk : 0;
         return true;
     }
-    r.nt = p.Lq > 1024 ? 2 : 1;
+    // Two query tiles per CTA for long queries.  fp16, two tiles and one: 8192 to 8192, 8 heads
+    // of 64 209 us and 223, 4096, 16 of 32 108 and 112; 2048, 40 of 64 76 and 75; 4 x 1200 to
+    // 1777 57 and 53; rows of 312 with a bias 1144 and 797; 8192, 8 heads of 128, where both
+    // take all of TMEM, 375 and 334.
+    r.nt = p.Lq > 2048 && p.D <= 64 ? 2 : 1;
     r.rows = r.nt * kTile;
     r.q_blocks = (p.Lq + r.rows - 1) / r.rows;
     const int64_t heads = i64(p.B) * p.Hq, tiles = (p.Lk + 63) / 64;
     if (heads * r.q_blocks > (1 << 30)) return false;
     const int slots = sms * (p.D > 64 ? 2 : 4) / r.nt;
-    // query blocks of one CTA, of short rows: a start costs about half a block, so
-    // the count whose rounds end soonest (rows of 312 x 12032 heads: three blocks a CTA)
+    // query blocks of one CTA: a start costs about 2.5 tiles, so the count whose
+    // rounds end soonest (rows of 312 x 12032 heads: three blocks a CTA)
     r.per_cta = 1;
-    double least = 1e30;
-    for (int n = 1; n <= (r.nt == 1 ? r.q_blocks : 1); ++n) {
+    double least = tail_time(heads * r.q_blocks, slots, tiles);
+    for (int n = 2; n <= (r.nt == 1 ? r.q_blocks : 1); ++n) {
         const int64_t ctas = heads * ((r.q_blocks + n - 1) / n);
-        const double time = static_cast<double>((ctas + slots - 1) / slots) * (n + 0.5);
+        const double time = static_cast<double>((ctas + slots - 1) / slots) * (static_cast<double>(n) * tiles + 2.5);
         if (time < least) {
             least = time;
             r.per_cta = n;
@@ -767,8 +781,7 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     if (plan.nt == 1)
         return dp == 32 ? launch<T, 32, 1>(f, ctas, stream)
              : dp == 64 ? launch<T, 64, 1>(f, ctas, stream) : launch<T, 128, 1>(f, ctas, stream);
-    return dp == 32 ? launch<T, 32, 2>(f, ctas, stream)
-         : dp == 64 ? launch<T, 64, 2>(f, ctas, stream) : launch<T, 128, 2>(f, ctas, stream);
+    return dp == 32 ? launch<T, 32, 2>(f, ctas, stream) : launch<T, 64, 2>(f, ctas, stream);
 }
 
 template <typename T>

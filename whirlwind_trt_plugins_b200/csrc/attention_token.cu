@@ -422,7 +422,16 @@ int tokens(const ww_attention_t& p, int splits, float* part_o, float* part_lse, 
 
 }  // namespace
 
-bool token_form(const ww_attention_t& p) noexcept { return i64(p.Hq / p.Hk) * p.Lq <= 32; }
+// Shared heads read their keys once in this form, and few items are split into
+// shares without a wide tile's start.  Neither: the tiles of attention_forward.cu.
+// fp16, this form and those tiles:
+//   64 x 8 key heads of 64, 1024 keys: one token of a head 40 us and 30, two heads 40 and 51,
+//   four heads 41 and 95; 512 x 8 of 32, 200 keys: 93 and 64, two heads 97 and 122
+//   8 x 8 key heads of 64, 8192 keys, one token 32 us and 36; 1 x 8, 16384 keys 24 and 34
+bool token_form(const ww_attention_t& p, int sms) noexcept
+{
+    return i64(p.Hq / p.Hk) * p.Lq <= 32 && (p.Hq > p.Hk || i64(p.B) * p.Hk <= sms);
+}
 
 int token_splits(const ww_attention_t& p, int sms) noexcept
 {

@@ -7,8 +7,8 @@
 namespace ww {
 
 // Whether a call takes this form: at most 32 rows (query heads of a key head x
-// tokens) share each key.
-bool token_form(const ww_attention_t& p) noexcept;
+// tokens) share each key, and sharing or few items make it pay (attention_token.cu).
+bool token_form(const ww_attention_t& p, int sms) noexcept;
 
 // CTAs that share the keys of one batch item and key head.
 int token_splits(const ww_attention_t& p, int sms) noexcept;
