@@ -27,9 +27,17 @@
 // are read 32 columns at a time in a loop that fits 80 registers -- four tiles on
 // an SM, 16 warps of elementwise work (two tiles at D = 128, where S, P and O of
 // a tile take 192 columns).
-//   NT = 1  four CTAs of one query tile: starts and ends overlap as well
+//   NT = 1  four CTAs of one query tile: starts and ends overlap as well; of short
+//           rows one CTA takes several query blocks of a head
 //   NT = 2  two CTAs of two query tiles against the same keys: half the reads of
-//           K and V from L2, for long rows
+//           K and V from L2, for long rows (make_plan has both sides)
+//
+// Measured, fp16: 19200 queries to 19200 keys, 5 heads of 64: 600 us, 790 TFLOP/s,
+// 3.1e12 exponentials a second (16 per clock: 4.5e12); 8192 to 8192, 8 heads of
+// 128: 297 us, 930 TFLOP/s; 12032 heads of 32 in rows of 312, 5 % of the keys
+// masked, with a bias: 795 us, a third of the exponentials' rate -- a tile's four
+// warps take 1000 to 1500 clocks for each of the two passes over its scores, and
+// five tiles to a row leave the start (tables, first loads) in sight.
 //
 // Masked keys: the load warp clears their rows of K and V before a tile is used
 // (its products then see zeros, whatever the places held: 0 times a NaN would not
