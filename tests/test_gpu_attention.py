@@ -327,6 +327,14 @@ def test_forms(env, shape, mask, bias):
     _run_case(env, shape, "f16" if shape[1] % 4 else "bf16", mask, bias, 6)
 
 
+@pytest.mark.parametrize("shape", [(700, 51, 43, 6, 3, 80), (150, 160, 160, 5, 5, 64), (400, 130, 300, 3, 3, 32),
+                                   (300, 7, 20, 5, 5, 40), (90, 257, 65, 7, 7, 128)])
+@pytest.mark.parametrize("mask,bias", [("", None), ("keys", None), ("", (32, 40, False, 3)), ("keys", (8, 300, True, 0))])
+def test_many_short_rows(env, shape, mask, bias):
+    """Query blocks of several batch items one after the other in a CTA."""
+    _run_case(env, shape, "bf16" if shape[0] % 4 else "f16", mask, bias, 7)
+
+
 @pytest.mark.parametrize("Lq,Lk,B", [(0, 5, 2), (5, 0, 2), (0, 0, 1), (3, 4, 0)])
 def test_lengths_of_zero(env, Lq, Lk, B):
     torch, ww = env

@@ -28,14 +28,14 @@
 // an SM, 16 warps of elementwise work (two tiles at D = 128, where S, P and O of
 // a tile take 192 columns).
 //   NT = 1  four CTAs of one query tile: starts and ends overlap as well; of short
-//           rows one CTA takes several query blocks of a head
+//           rows one CTA takes several query blocks of a head, of several batch items
 //   NT = 2  two CTAs of two query tiles against the same keys: half the reads of
 //           K and V from L2, for long rows (make_plan has both sides)
 //
 // Measured, fp16: 19200 queries to 19200 keys, 5 heads of 64: 600 us, 790 TFLOP/s,
 // 3.1e12 exponentials a second (16 per clock: 4.5e12); 8192 to 8192, 8 heads of
 // 128: 297 us, 930 TFLOP/s; 12032 heads of 32 in rows of 312, 5 % of the keys
-// masked, with a bias: 795 us, a third of the exponentials' rate -- a tile's four
+// masked, with a bias: 753 us, a third of the exponentials' rate -- a tile's four
 // warps take 1000 to 1500 clocks for each of the two passes over its scores, and
 // five tiles to a row leave the start (tables, first loads) in sight.
 //
@@ -78,8 +78,9 @@ struct FwdParams {
     RelBuckets rel;
     int32_t B, Lq, Lk, Hq, group, D;
     int32_t q_blocks, per_cta, groups;  // query blocks, those of one CTA, groups of them
+    int32_t wide, row_blocks;           // groups run over all batch items of a head; the blocks they share out
     int32_t whole_items, splits;
-    Divisor by_block, by_head, by_group;
+    Divisor by_block, by_head, by_group, by_q;
     int32_t q_b, q_h, k_b, k_h, v_b, v_h;  // 0 where the tensor is broadcast
     int32_t max_entries;                   // relative positions a CTA keeps
     float scale2;                          // scale * log2(e)
@@ -189,12 +190,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     const bool in_parts = blk >= p.whole_items;
     const int split = in_parts ? (blk - p.whole_items) % p.splits : 0, splits = in_parts ? p.splits : 1;
     const int item = in_parts ? p.whole_items + (blk - p.whole_items) / p.splits : blk;
-    const int bh = p.by_block.div(item), qb0 = (item - bh * p.groups) * p.per_cta, b = p.by_head.div(bh), h = bh - b * p.Hq,
-              g = p.by_group.div(h);
-    const int nq = min(p.per_cta, p.q_blocks - qb0);  // query blocks of this CTA, one after the other
-    const auto q_of = [&](int qi) { return (qb0 + qi) * (NT * kTile); };
+    // (wide: every batch item has the same number of key tiles, and one group may run over several)
+    const bool wide = NT == 1 && p.wide != 0;
+    const int outer = p.by_block.div(item), u0 = (item - outer * p.groups) * p.per_cta;
+    const int b0 = wide ? 0 : p.by_head.div(outer), h = wide ? outer : outer - b0 * p.Hq, g = p.by_group.div(h);
+    const int nq = min(p.per_cta, p.row_blocks - u0);  // query blocks of this CTA, one after the other
+    const auto batch_of = [&](int qi) { return wide ? p.by_q.div(u0 + qi) : b0; };
+    const auto q_of = [&](int qi) { return (u0 + qi - (wide ? batch_of(qi) * p.q_blocks : 0)) * (NT * kTile); };
     const auto tiles_of = [&](int qi) { return NT == 1 || q_of(qi) + kTile >= p.Lq ? 1 : 2; };  // query tiles with rows
-    const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b), 0), p.Lk);
+    const int len = p.k_lens == nullptr ? p.Lk : min(max(__ldg(p.k_lens + b0), 0), p.Lk);
     const int n_all = (len + KT - 1) / KT;
     int first, n;
     part_of(n_all, split, splits, first, n);
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
     const auto v_bar = [&](int s) { return masks ? at(bar->v_ready[s]) : at(bar->v_full[s]); };
 
     // tiles are numbered over all query blocks: number i is key tile i % n of block i / n
-    const auto load_k = [&](int i, int kt) {
+    const auto load_k = [&](int i, int kt, int b) {
         const int s = i % S;
         umma::mbar_arrive_expect_tx(at(bar->k_full[s]), L::kBytes);
         for (int c = 0; c < L::kChunks; ++c)
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 umma::tma_load_4d(sm + L::kK + s * L::kBytes + c * L::kChunk + x * L::kRow, &p.k, c * L::kCols, g * p.k_h,
                                   (first + kt) * KT + x, b * p.k_b, at(bar->k_full[s]));
     };
-    const auto load_v = [&](int i, int kt) {
+    const auto load_v = [&](int i, int kt, int b) {
         const int s = i % S;
         umma::mbar_arrive_expect_tx(at(bar->v_full[s]), L::kBytes);
         for (int c = 0; c < L::kChunks; ++c)
@@ -226,7 +230,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                                   (first + kt) * KT + x, b * p.v_b, at(bar->v_full[s]));
     };
     const auto load_q = [&](int qi) {
-        const int tiles = tiles_of(qi);
+        const int tiles = tiles_of(qi), b = batch_of(qi);
         umma::mbar_arrive_expect_tx(at(bar->q_full), tiles * L::kQBytes);
         for (int t = 0; t < tiles; ++t)
             for (int c = 0; c < L::kChunks; ++c)
@@ -256,15 +260,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         umma::fence_proxy_async_smem();
         if (n > 0) {
             load_q(0);
-            load_k(0, 0);
-            load_v(0, 0);
+            load_k(0, 0, batch_of(0));
+            load_v(0, 0, batch_of(0));
         }
     }
     RelRange range;  // positions j - i - q_offset of the tiles, padded rows and columns included
     float* values = reinterpret_cast<float*>(base + L::kBias);
     if (p.rel.per_side != 0 && n > 0) {
-        range = rel_range(p.rel, first * KT - (q_of(nq) - 1) - p.rel.q_offset,
-                          (first + n) * KT - 1 - q_of(0) - p.rel.q_offset);
+        const int q_lo = wide ? 0 : q_of(0), q_end = wide ? p.q_blocks * kTile : q_of(nq);
+        range = rel_range(p.rel, first * KT - (q_end - 1) - p.rel.q_offset, (first + n) * KT - 1 - q_lo - p.rel.q_offset);
         TableRow<T> table;
         table.load(p.rel, p.table, h, lane);
         for (int e0 = warp * 32; warp < NT * 4 && e0 < range.count(); e0 += NT * 128) {  // the other warps have their own starts
@@ -290,9 +294,9 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     if (ok) load_q(load_qi);
                 }
                 ok = ok && umma::mbar_poll(at(bar->k_empty[s]), ph);
-                if (ok) load_k(i, load_kt);
+                if (ok) load_k(i, load_kt, batch_of(load_qi));
                 ok = ok && umma::mbar_poll(at(bar->v_empty[s]), ph);
-                if (ok) load_v(i, load_kt);
+                if (ok) load_v(i, load_kt, batch_of(load_qi));
             }
             if (++load_kt == n) {
                 load_kt = 0;
@@ -311,14 +315,15 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             if (lane == 0) load(0);
             if (lane == 0 && n > 1)
                 for (int i = 1; i < S && i < n; ++i) load(i);
-            int loaded = min(S, n), kt = 0;
+            int loaded = min(S, n), kt = 0, qi = 0;
             for (int i = 0; i < total; ++i) {
                 const int s = i % S, k0 = (first + kt) * KT;
+                const uint8_t* mask = p.key_mask + static_cast<int64_t>(batch_of(qi)) * p.Lk;
                 uint32_t in_mask = 0;
 #pragma unroll
                 for (int c = 0; c < KT; c += 32) {
                     const int key = k0 + c + lane;
-                    if (key < len && (p.key_mask == nullptr || __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + key) != 0))
+                    if (key < len && (p.key_mask == nullptr || __ldg(mask + key) != 0))
                         in_mask |= 1u << (c / 32);
                 }
                 ok = __shfl_sync(~0u, ok, 0);
@@ -352,7 +357,10 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     ++loaded;
                 }
                 __syncwarp();
-                if (++kt == n) kt = 0;
+                if (++kt == n) {
+                    kt = 0;
+                    ++qi;
+                }
             }
         }
         if (lane == 0 && !ok) record_device_error(p.err, kErrMbarTimeout | 0x20);
@@ -553,7 +561,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             unpair(l2, l_even, l_odd);
             const float sum = l_even + l_odd;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
+            const int64_t b = batch_of(qi), row = (b * p.Lq + i) * p.Hq + h;
             const int64_t part = (static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (NT * kTile) + t * kTile + r;
 #pragma unroll
             for (int c = 0; c < DP; c += 32) {
@@ -587,7 +595,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             if (i < p.Lq) {
                 const float lse2 = sum == 0.0f ? -INFINITY : m + log2f(sum);
                 if (in_parts) p.part_lse[part] = lse2;
-                else if (p.lse != nullptr) p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Lq + i] = lse2 * kLn2F;
+                else if (p.lse != nullptr) p.lse[(b * p.Hq + h) * p.Lq + i] = lse2 * kLn2F;
             }
             umma::fence_before_sync();
             __syncwarp();
@@ -658,23 +666,24 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o
 // the GPU's CTAs (all of them, where there are few).
 struct Plan {
     bool token;
-    int nt, q_blocks, per_cta, groups, whole, rest, splits, rows;
+    bool wide;
+    int nt, q_blocks, per_cta, row_blocks, outer, groups, whole, rest, splits, rows;
     int64_t part_rows() const { return i64(rest) * splits * rows; }
     int64_t part_bytes(int D) const { return part_rows() * (D + 1) * 4; }
-    void without_parts(const ww_attention_t& p)
+    void without_parts()
     {
         splits = 1;
         rest = 0;
-        whole = token ? 0 : static_cast<int>(i64(groups) * p.B * p.Hq);
+        whole = groups * outer;
     }
 };
 
-// Tiles one after the other in `items` CTAs of `tiles` each, the last round split
-// over its tiles where that is sooner (tail_splits).
-double tail_time(int64_t items, int slots, int64_t tiles) noexcept
+// Tiles one after the other in `items` CTAs of `tiles` each and a start that costs
+// as much as `start` tiles, the last round split where that is sooner (tail_splits).
+double tail_time(int64_t items, int slots, int64_t tiles, double start) noexcept
 {
     const int rest = static_cast<int>(items % slots), splits = tail_splits(rest, slots, tiles);
-    const double one = tiles + 2.5, last = splits == 1 ? one : static_cast<double>(tiles) * rest / slots + 14.0;
+    const double one = tiles + start, last = splits == 1 ? one : static_cast<double>(tiles) * rest / slots + 14.0;
     return static_cast<double>(items / slots) * one + (rest == 0 ? 0.0 : last);
 }
 
@@ -683,7 +692,8 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     Plan& r = *plan;
     r.token = token_form(p, sms);
     if (r.token) {
-        r.q_blocks = r.groups = r.per_cta = 0;
+        r.wide = false;
+        r.q_blocks = r.groups = r.per_cta = r.row_blocks = r.outer = 0;
         r.nt = 0;
         r.rows = p.Hq / p.Hk * p.Lq;
         r.splits = token_splits(p, sms);
@@ -702,20 +712,36 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     const int64_t heads = i64(p.B) * p.Hq, tiles = (p.Lk + 63) / 64;
     if (heads * r.q_blocks > (1 << 30)) return false;
     const int slots = sms * (p.D > 64 ? 2 : 4) / r.nt;
-    // query blocks of one CTA: a start costs about 2.5 tiles, so the count whose
-    // rounds end soonest (rows of 312 x 12032 heads: three blocks a CTA)
+    // Query blocks of one CTA, of one (batch item, head) or, where all items have the same
+    // length, of a head over several items: the count whose rounds end soonest, several
+    // items only where that is clearly sooner (they share no keys).  fp16, one block per
+    // CTA or those of one item, and several items:
+    //   4908 x 6 heads of 80, 51 to 43 tokens, with a bias: 558 us and 364
+    //   2000 x 4 heads of 32, 60 to 60: 68 and 43; 1504 x 8 of 32, 312 to 312: 574 and
+    //   590, masked and with a bias 796 and 753; 360 x 3 of 32, 320 to 320: 83 and 86
+    constexpr double kClearly = 1.15;
+    const double start = p.bias_table != nullptr ? 2.5 : 1.25;
     r.per_cta = 1;
-    double least = tail_time(heads * r.q_blocks, slots, tiles);
-    for (int n = 2; n <= (r.nt == 1 ? r.q_blocks : 1); ++n) {
-        const int64_t ctas = heads * ((r.q_blocks + n - 1) / n);
-        const double time = static_cast<double>((ctas + slots - 1) / slots) * (static_cast<double>(n) * tiles + 2.5);
-        if (time < least) {
-            least = time;
-            r.per_cta = n;
+    r.wide = false;
+    double least = tail_time(heads * r.q_blocks, slots, tiles, start);
+    for (int wide = 0; wide < 2; ++wide) {
+        if (r.nt == 2 || heads == 0 || (wide && p.k_lens != nullptr)) break;
+        const int64_t outer = wide ? p.Hq : heads, blocks = wide ? i64(p.B) * r.q_blocks : r.q_blocks;
+        const int64_t rounds = (outer + slots - 1) / slots;
+        for (int64_t k = rounds; k < rounds + 4; ++k) {  // CTAs for k rounds
+            const int64_t per_outer = k * slots / outer, n = (blocks + per_outer - 1) / per_outer;
+            const double time = static_cast<double>(k) * (static_cast<double>(n) * tiles + start) * (wide ? kClearly : 1.0);
+            if (n > 1 && time < least) {
+                least = time;
+                r.per_cta = static_cast<int>(n);
+                r.wide = wide != 0;
+            }
         }
     }
-    r.groups = (r.q_blocks + r.per_cta - 1) / r.per_cta;
-    const int64_t items = heads * r.groups;
+    r.outer = static_cast<int>(r.wide ? p.Hq : heads);
+    r.row_blocks = r.wide ? p.B * r.q_blocks : r.q_blocks;
+    r.groups = (r.row_blocks + r.per_cta - 1) / r.per_cta;
+    const int64_t items = i64(r.outer) * r.groups;
     r.rest = static_cast<int>(items % slots);
     r.splits = r.per_cta == 1 ? tail_splits(r.rest, slots, tiles) : 1;  // the join counts blocks
     if (r.splits == 1) r.rest = 0;
@@ -757,7 +783,7 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.max_entries = 0;
     if (p.bias_table != nullptr) {
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
-        const int all = (p.Lk + 127) / 128 * 128 + plan.per_cta * plan.nt * kTile;
+        const int all = (p.Lk + 127) / 128 * 128 + (plan.wide ? plan.q_blocks : plan.per_cta) * plan.nt * kTile;
         f.max_entries = (std::min(2 * (p.max_distance + kRelMargin) + 1, all) + 15) / 16 * 16;
     }
     f.part_o = part_o;
@@ -771,8 +797,11 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.q_blocks = plan.q_blocks;
     f.per_cta = plan.per_cta;
     f.groups = plan.groups;
+    f.wide = plan.wide;
+    f.row_blocks = plan.row_blocks;
     f.by_block = make_divisor(plan.groups);
     f.by_head = make_divisor(p.Hq);
+    f.by_q = make_divisor(plan.q_blocks);
     f.by_group = make_divisor(p.Hq / p.Hk);
     f.whole_items = plan.whole;
     f.splits = plan.splits;
@@ -832,7 +861,7 @@ int ww_cross_attention(const ww_attention_t* p, void* stream)
     if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
     ww::Plan plan;
     if (!ww::make_plan(*p, d.sm_count, &plan)) return WW_ERR_UNSUPPORTED;
-    if (p->workspace == nullptr) plan.without_parts(*p);
+    if (p->workspace == nullptr) plan.without_parts();
     else if (plan.part_bytes(p->D) > p->workspace_bytes) return WW_ERR_UNSUPPORTED;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return p->dtype == WW_DTYPE_HALF ? ww::forward<__half>(*p, plan, s) : ww::forward<__nv_bfloat16>(*p, plan, s);
