@@ -776,7 +776,9 @@ __global__ void __cluster_dims__(kTableCtas, 1, 1) __launch_bounds__(1024)
             const int64_t item = item_of(n);
             const bool one = item < whole_items;
             const int64_t at = one ? item : whole_items + (item - whole_items) * splits;
-            for (int k = 0; k < (one ? 1 : splits); ++k) s += part[(at + k) * total + t];
+            const int parts = one ? 1 : splits;
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) s += part[(at + k) * total + t];
         }
     }
     sums[w][lane] = s;

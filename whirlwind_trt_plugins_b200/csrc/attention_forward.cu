@@ -496,9 +496,10 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c / 2);
                 };
                 const auto columns = [&](const auto& use, auto raw_scores) {
-                    // Long queries' raw scores, the case without any other work to hide behind:
-                    // 16 at a time, the next ones on their way meanwhile (19200 to 19200, 5 heads of 64: 638 -> 600 us).
-                    // Elsewhere the registers are worth more (rows of 160: 35 us, so 39).
+                    // Raw scores, with no other work to hide behind, where registers allow (long
+                    // queries, wide heads): 16 at a time, the next ones on their way meanwhile.
+                    // 19200 to 19200, 5 heads of 64: 638 -> 600 us; 8192, 8 of 128: 334 -> 297.
+                    // Elsewhere it spills (rows of 160: 35 us, so 39).
                     if constexpr (kAhead && std::is_same<decltype(raw_scores), std::true_type>::value) {
                         if (!any_row) return;
                         uint32_t x[2][16];
@@ -641,7 +642,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const float* part_o
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) {
         const int64_t at = first + static_cast<int64_t>(s) * rows;
         const float w = exp2_approx(part_lse[at] - base);
