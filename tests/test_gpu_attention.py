@@ -335,6 +335,13 @@ def test_many_short_rows(env, shape, mask, bias):
     _run_case(env, shape, "bf16" if shape[0] % 4 else "f16", mask, bias, 7)
 
 
+@pytest.mark.parametrize("shape", [(1, 200, 2600, 1, 1, 128), (1, 2600, 200, 2, 1, 128), (1, 150, 2600, 2, 2, 64),
+                                   (1, 2600, 150, 1, 1, 32), (1, 4, 2600, 4, 1, 128)])
+def test_widest_tables(env, shape):
+    """The most buckets and the longest distance, every position of a range in use."""
+    _run_case(env, shape, "bf16", "keys", (128, 1024, True, (shape[2] - shape[1]) // 2), 8)
+
+
 @pytest.mark.parametrize("Lq,Lk,B", [(0, 5, 2), (5, 0, 2), (0, 0, 1), (3, 4, 0)])
 def test_lengths_of_zero(env, Lq, Lk, B):
     torch, ww = env

@@ -29,15 +29,16 @@
 // Measured: a map of 4800, 8 heads of 128, bf16 with a bias: 308 us for the
 // gradients, 770 TFLOP/s of the five products (seven are formed); 1200 to 1777
 // tokens, 4 x 16 heads of 64 on 4: 93 us; 1080 heads of 32 in rows of 320, masked,
-// with a bias: 269 us, where a CTA of five tiles spends 4000 of its 17000 clocks
+// with a bias: 283 us, where a CTA of five tiles spends 4000 of its 17000 clocks
 // (5800 of 21600 over queries) before its first tile.
 // The two kernels do not need each other: `queries` is launched behind `keys` and
-// takes the SMs that its last round leaves (rows of 320: 368 us forward and
-// gradients one after the other, 352 so), then one join for both.
+// takes the SMs that its last round leaves (rows of 320, forward and gradients:
+// 16 us less than one after the other), then one join for both.
 //
 // dtable: a tile whose positions all lie in one bucket adds its plain sum.
-// Otherwise dS goes through shared memory, rounded as for its product, 32 columns at a time; a thread sums
-// one diagonal j - i (one read and one add per value, no conflicts), diagonals
+// Otherwise dS goes through shared memory in fp32, 32 columns at a time (rounded as
+// for its product, the errors of dtable are half as large again and rows of 320 take
+// 353 us in place of 367); a thread sums one diagonal j - i (one read and one add per value, no conflicts), diagonals
 // are collected per CTA and joined to buckets, CTAs and warpgroups in order.
 #include "attention.cuh"
 #include "tensor_map.cuh"
@@ -54,8 +55,7 @@ namespace {
 constexpr int kRows = 128;
 constexpr int kCols = 64;
 constexpr int kShift = 6;         // P is kept times 2^kShift
-constexpr int kPitch = 17;        // words (two 16-bit values) of a dS row in shared memory
-constexpr int kTileRows = 160;    // 128, and copies of the first 32
+constexpr int kPitch = 33;        // words of a row of 32 dS in shared memory
 
 struct BwdParams {
     CUtensorMap q, k, v, dout;  // boxes of 64 tokens
@@ -130,7 +130,7 @@ struct Bars {
 __host__ __device__ inline int bias_bytes(bool keys, int groups, int entries, int buckets)
 {
     const int e = (entries + 15) / 16 * 16;
-    return keys ? e + groups * e * 4 : e + (1 + groups) * e * 4 + groups * 4 * buckets * 4 + groups * kTileRows * kPitch * 4;
+    return keys ? e + groups * e * 4 : e + (1 + groups) * e * 4 + groups * 4 * buckets * 4 + groups * kRows * kPitch * 4;
 }
 
 template <typename T, int DP, bool KEYS, bool BIAS>
@@ -425,10 +425,9 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         int built = -1;  // KEYS: head of `values`
         float* diag = values + (1 + wg) * entries;
         float* plain = values + (1 + kGroups) * entries + warp * p.rel.total;
-        uint32_t* tile = reinterpret_cast<uint32_t*>(values + (1 + kGroups) * entries + kGroups * 4 * p.rel.total) +
-                         wg * kTileRows * kPitch;
+        float* tile = values + (1 + kGroups) * entries + kGroups * 4 * p.rel.total + wg * kRows * kPitch;
         if (BIAS && !KEYS && !any_row)
-            for (int j = 0; j < 16; ++j) tile[r * kPitch + j] = 0;  // (never warp 0: its rows exist)
+            for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;
         int ch = h, qt = first + st;  // tile i's head (KEYS) and its place along the streamed axis
         if (KEYS) {
             ch = h * group + (first + st) / p.q_tiles;
@@ -515,18 +514,14 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                         unpair(ds, d0, d1);
                         if (KEYS) pk[j / 2] = pack2<T>(p0, p1);
                         dk[j / 2] = pack2<T>(d0, d1);
+                        if (W && !KEYS) {
+                            tile[r * kPitch + c * 16 + j] = d0;
+                            tile[r * kPitch + c * 16 + j + 1] = d1;
+                        }
                     }
                     // over columns of this half of the tile only: the other half may not have been read
                     if (KEYS) umma::tmem_st8(s_col + half * 32 + c * 8, pk);
                     umma::tmem_st8(dp_col + half * 32 + c * 8, dk);
-                    if (W && !KEYS) {
-                        uint32_t* to = tile + r * kPitch + c * 8;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) to[j] = dk[j];
-                        if (warp % 4 == 0)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) to[128 * kPitch + j] = dk[j];
-                    }
                 }
             };
             if (any_row) {
@@ -551,22 +546,22 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                     for (int o = 16; o > 0; o >>= 1) t0 += __shfl_xor_sync(~0u, t0, o);
                     if (lane == 0) plain[flat_bucket] += t0;
                 } else {
-                    // sums along j - i: each thread a diagonal, column j of row
-                    // j + 127 - r; rows from 128 on are copies of rows 0 ..., so that
-                    // warp 0's threads pass from diagonal r - 127 to r + 1 (r < 31)
+                    // sums along j - i: each thread a diagonal, column j of row j + 127 - r;
+                    // past the last row, warp 0's threads go on from row 0: diagonal
+                    // r - 127 ends, r + 1 begins (r < 31)
                     warpgroup_sync(wg);
-                    const T* at0 = reinterpret_cast<const T*>(tile + (127 - r) * kPitch);
+                    const float* at0 = tile + (127 - r) * kPitch;
                     float* to = diag + col0 - row0 - p.rel.q_offset - range.lo;
                     if (warp % 4 != 0) {
                         float run[2] = {0.0f, 0.0f};
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) run[j & 1] += to_float(at0[j * (2 * kPitch + 1)]);
+                        for (int j = 0; j < 32; ++j) run[j & 1] += at0[j * (kPitch + 1)];
                         to[r - 127] += run[0] + run[1];
                     } else {
                         float before = 0.0f, after = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float v = to_float(at0[j * (2 * kPitch + 1)]);
+                            const float v = at0[j * (kPitch + 1) - (j <= r ? 0 : kRows * kPitch)];
                             before += j <= r ? v : 0.0f;
                             after += j <= r ? 0.0f : v;
                         }
