@@ -42,6 +42,8 @@ _lib.ww_relative_position_bucket.argtypes = [ctypes.c_int] * 4
 # ww_qk_norm_rope_t and ww_attention_t: pointers, workspace bytes, strides, sizes, one float
 _ROPE = struct.Struct("@17Pq12q12if0P")
 _ATTN = struct.Struct("@14Pq12q11if0P")
+_ROPE_WS, _ATTN_WS = 16 * 8, 13 * 8  # where the workspace's address and bytes stand
+_WS = struct.Struct("@Pq")
 
 
 class _Torch:
@@ -126,8 +128,10 @@ def _place(t, stream):
         yield
 
 
-def _workspace(n: int, like):
-    return _Torch.empty(n, dtype=_Torch.uint8, device=like.device)
+def _workspace(n: int, like, args: bytes, at: int):
+    """Scratch memory of n bytes, and the packed parameters with it filled in at their byte `at`."""
+    ws = _Torch.empty(n, dtype=_Torch.uint8, device=like.device)
+    return ws, args[:at] + _WS.pack(ws.data_ptr(), n) + args[at + 16:]
 
 
 def _ptr(t) -> int:
@@ -206,14 +210,12 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, q_
                                          interleaved)
     dq, dk = _new(q, None, "dq"), _new(k, None, "dk")
     dqw, dkw = _Torch.empty_like(q_weight), _Torch.empty_like(k_weight)
-    ptrs = (q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-            _ptr(q_pos), _ptr(k_pos), 0, 0, dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dqw.data_ptr(), dkw.data_ptr())
-    rest = (*qs, *ks, *gqs, *gks, *sizes, bool(interleaved), eps)
-    n = _lib.ww_qk_norm_rope_backward_workspace(_ROPE.pack(*ptrs, 0, 0, *rest))
-    ws = _workspace(n, q)
-    _check("ww_qk_norm_rope_backward", _lib.ww_qk_norm_rope_backward(_ROPE.pack(*ptrs, ws.data_ptr(), n, *rest),
-                                                                     _Torch.stream(at)))
+    a = _ROPE.pack(q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
+                   sin.data_ptr(), _ptr(q_pos), _ptr(k_pos), 0, 0, dq_out.data_ptr(), dk_out.data_ptr(),
+                   dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), 0, 0, *qs, *ks, *gqs, *gks, *sizes,
+                   bool(interleaved), eps)
+    ws, a = _workspace(_lib.ww_qk_norm_rope_backward_workspace(a), q, a, _ROPE_WS)
+    _check("ww_qk_norm_rope_backward", _lib.ww_qk_norm_rope_backward(a, _Torch.stream(at)))
     return dq, dk, dqw, dkw
 
 
@@ -274,14 +276,11 @@ def cross_attention(q, k, v, scale: float | None = None, k_lens=None, key_mask=N
                                    q_offset, return_lse, out)
     out = _new(q, out, "out")
     lse = _Torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=_Torch.f32, device=q.device) if return_lse else None
-    ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(k_lens), _ptr(key_mask),
-            _ptr(bias_table), 0, 0, 0, 0, 0)
-    strides = (*qs, *ks, *vs, 0, 0, 0)
-    a = _ATTN.pack(*ptrs, 0, 0, *strides, *sizes)
+    a = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(k_lens), _ptr(key_mask),
+                   _ptr(bias_table), 0, 0, 0, 0, 0, 0, 0, *qs, *ks, *vs, 0, 0, 0, *sizes)
     n = _lib.ww_cross_attention_workspace(a)
     if n:
-        ws = _workspace(n, q)
-        a = _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes)
+        ws, a = _workspace(n, q, a, _ATTN_WS)
     _check("ww_cross_attention", _lib.ww_cross_attention(a, _Torch.stream(at)))
     return (out, lse) if return_lse else out
 
@@ -303,13 +302,11 @@ def cross_attention_backward(dout, q, k, v, out, lse, scale: float | None = None
                                             max_distance, bidirectional, q_offset)
     dq, dk, dv = _new(q, None, "dq"), _new(k, None, "dk"), _new(v, None, "dv")
     dtable = None if bias_table is None else _Torch.empty_like(bias_table)
-    ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(k_lens), _ptr(key_mask),
-            _ptr(bias_table), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable))
-    strides = (*qs, *ks, *vs, *gs)
-    n = _lib.ww_cross_attention_backward_workspace(_ATTN.pack(*ptrs, 0, 0, *strides, *sizes))
-    ws = _workspace(n, q)
-    _check("ww_cross_attention_backward", _lib.ww_cross_attention_backward(
-        _ATTN.pack(*ptrs, ws.data_ptr(), n, *strides, *sizes), _Torch.stream(at)))
+    a = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(k_lens),
+                   _ptr(key_mask), _ptr(bias_table), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                   _ptr(dtable), 0, 0, *qs, *ks, *vs, *gs, *sizes)
+    ws, a = _workspace(_lib.ww_cross_attention_backward_workspace(a), q, a, _ATTN_WS)
+    _check("ww_cross_attention_backward", _lib.ww_cross_attention_backward(a, _Torch.stream(at)))
     return dq, dk, dv, dtable
 
 
