@@ -658,14 +658,15 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
 // lanes per row, 8 values each.
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ ww_attention_t a, float* nlse2,
-                                                              float* ndelta, uint32_t* top, int Lq_pad)
+                                                              float* ndelta, uint32_t* top, int Lq_pad, Divisor by_blocks,
+                                                              Divisor by_head)
 {
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
-    const int lane = threadIdx.x % kLanes;
-    const int64_t rows = static_cast<int64_t>(a.B) * Lq_pad * a.Hq;
-    const int h = static_cast<int>(item % a.Hq);
-    const int64_t bi = item / a.Hq;
-    const int b = static_cast<int>(bi / Lq_pad), i = static_cast<int>(bi % Lq_pad);
+    const int b = by_blocks.div(blockIdx.x), lane = threadIdx.x % kLanes;
+    const int64_t rows = static_cast<int64_t>(Lq_pad) * a.Hq;  // of a batch item
+    const int64_t item = static_cast<int64_t>(blockIdx.x - b * by_blocks.d) * (256 / kLanes) + threadIdx.x / kLanes;
+    // 64-bit divisions would be most of the kernel
+    const int i = rows <= INT32_MAX - 256 ? by_head.div(static_cast<int>(item)) : static_cast<int>(item / a.Hq);
+    const int h = static_cast<int>(item - static_cast<int64_t>(i) * a.Hq);
     const bool live = item < rows && i < a.Lq;
     float sum = 0.0f, mx = 0.0f;
     if (live && lane * 8 < a.D) {
@@ -932,14 +933,14 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     int st = WW_SUCCESS;
     if (has_q) {
         if (!bf && cudaMemsetAsync(ws, 0, 4, stream) != cudaSuccess) return launch_status("cross_attention_backward");
-        const int64_t rows = i64(p.B) * plan.Lq_pad * p.Hq;
         const int per = p.D <= 32 ? 64 : p.D <= 64 ? 32 : 16;  // rows of a block
-        const int64_t blocks = (rows + per - 1) / per;
+        const int64_t of_item = (i64(plan.Lq_pad) * p.Hq + per - 1) / per, blocks = of_item * p.B;
         if (blocks > 0x7fffffff) return WW_ERR_UNSUPPORTED;
         const auto kernel = per == 64 ? attention_delta_kernel<T, 4> : per == 32 ? attention_delta_kernel<T, 8>
                                                                                  : attention_delta_kernel<T, 16>;
         kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, const_cast<float*>(f.nlse2), const_cast<float*>(f.ndelta),
-                                                                  reinterpret_cast<uint32_t*>(ws), plan.Lq_pad);
+                                                                  reinterpret_cast<uint32_t*>(ws), plan.Lq_pad,
+                                                                  make_divisor(static_cast<int>(of_item)), make_divisor(p.Hq));
         st = launch_status("cross_attention_backward");
     }
     const int far = 2 * (p.max_distance + kRelMargin) + 1;
