@@ -29,7 +29,7 @@
 // Measured: a map of 4800, 8 heads of 128, bf16 with a bias: 308 us for the
 // gradients, 770 TFLOP/s of the five products (seven are formed); 1200 to 1777
 // tokens, 4 x 16 heads of 64 on 4: 93 us; 1080 heads of 32 in rows of 320, masked,
-// with a bias: 283 us, where a CTA of five tiles spends 4000 of its 17000 clocks
+// with a bias: 280 us, where a CTA of five tiles spends 4000 of its 17000 clocks
 // (5800 of 21600 over queries) before its first tile.
 // The two kernels do not need each other: `queries` is launched behind `keys` and
 // takes the SMs that its last round leaves (rows of 320, forward and gradients:
@@ -38,8 +38,9 @@
 // dtable: a tile whose positions all lie in one bucket adds its plain sum.
 // Otherwise dS goes through shared memory in fp32, 32 columns at a time (rounded as
 // for its product, the errors of dtable are half as large again and rows of 320 take
-// 353 us in place of 367); a thread sums one diagonal j - i (one read and one add per value, no conflicts), diagonals
-// are collected per CTA and joined to buckets, CTAs and warpgroups in order.
+// 353 us in place of 367); a thread sums one diagonal j - i (one read and one add per
+// value, no conflicts), diagonals are collected per CTA and joined to buckets, CTAs
+// and warpgroups in order.
 #include "attention.cuh"
 #include "tensor_map.cuh"
 #include "umma.cuh"
