@@ -282,7 +282,7 @@ __device__ __forceinline__ void warpgroup_sync(int w)
 
 // Launch of a kernel that follows another one of the same call: it may be set up
 // while that one still runs, and waits for it (wait_for_launches_before) before
-// it reads anything.
+// it reads what that one writes, at the latest before it ends itself.
 template <typename... P, typename... A>
 inline cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) noexcept
 {
@@ -304,8 +304,8 @@ __device__ __forceinline__ void wait_for_launches_before()
     asm volatile("griddepcontrol.wait;" : : : "memory");
 }
 
-// Lets the kernel launched behind this one start wherever CTAs of this grid are
-// none to come any more (it begins once all of them have called this).
+// Lets the kernel launched behind this one start on what SMs have left, once every
+// CTA of this grid has called this or ended.
 __device__ __forceinline__ void start_launch_behind()
 {
     asm volatile("griddepcontrol.launch_dependents;" : : : "memory");

@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         umma::mbar_init(at(bar->done), 1);
         umma::mbar_fence_init();
         umma::fence_proxy_async_smem();
-            if (n > 0) {
+        if (n > 0) {
             if (!L::kRowsInTmem) {
                 // a half of the row tile that lies beyond the tensor reads as zeros like any other place outside
                 umma::mbar_arrive_expect_tx(at(bar->r_full), 2 * L::kRowBytes);
