@@ -406,9 +406,10 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             __syncwarp();
             if (lane == 0) umma::mbar_arrive(at(bar->r_full));
         }
-        // fp16: f = 2^e, e = 127 - the biased exponent of max |dO|
+        // fp16: f = 2^e, e = 127 - the biased exponent of max |dO|; without tiles nobody may have
+        // written that maximum, and every sum is 0
         float f = 1.0f;
-        if (kHalf) {
+        if (kHalf && n > 0) {
             const int top = static_cast<int>(__ldcg(p.top) >> 23);
             if (top > 0 && top < 255) f = __int_as_float((254 - top) << 23);
         }
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         if (BIAS && !KEYS && !any_row)
             for (int j = 0; j < 32; ++j) tile[r * kPitch + j] = 0.0f;
         int ch = h, qt = first + st;  // tile i's head (KEYS) and its place along the streamed axis
-        if (KEYS) {
+        if (KEYS && n > 0) {
             ch = h * group + (first + st) / p.q_tiles;
             qt = (first + st) % p.q_tiles;
         }
