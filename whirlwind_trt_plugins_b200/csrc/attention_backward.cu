@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                             arg = add2(arg, KEYS ? pair(mine[-k], mine[-k - 1]) : pair(mine[k], mine[k + 1]));
                         }
                         float p0, p1;
-                        if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe: 2^-126 for -inf, times rows of zeros
+                        if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe
                             unpair(exp2_poly(arg), p0, p1);
                         } else {
                             unpair(arg, p0, p1);

@@ -148,7 +148,7 @@ __device__ __forceinline__ float score_pass(uint32_t (&x)[N], float scale2, floa
 
 // P = 2^(mul x + add) of N columns: summed, rounded and put into N / 2 columns of
 // TMEM.  POLY: one pair in kPolyOf on the FMA pipe (whole tiles without a bias
-// of their own: there no argument is -inf).
+// of their own).
 template <typename T, bool POLY, int N>
 __device__ __forceinline__ void exp_pass(const uint32_t (&x)[N], float mul, float add, Pair& sum, uint32_t to)
 {
