@@ -20,9 +20,14 @@
 // its 64 columns each): of two CTAs, whose starts and ends overlap as well, or of
 // one where the accumulators take half of TMEM.
 //
-// 16-bit ranges: P is kept as 2^6 P, and in fp16 dS is formed from dO 2^e with
-// 2^e max|dO| in [1, 2): gradients as small as a mean over a batch leaves
-// them stay in fp16's normal range.  Powers of two, taken out again at the end.
+// 16-bit ranges: P is kept as 2^6 P, dS in fp16 as 2^(6 + e) dS.  delta is a mean of
+// dP, so |dP - delta| <= M = 2 |dO row| max |v row| over the valid keys; e is chosen
+// with 2^8 <= 2^e M < 2^9, which keeps 2^(6 + e) |dS| below 2^15 whatever the values
+// are (P <= 1 up to its rounding) and leaves half of fp16's smallest step at 2^-39 M:
+// neither large values nor gradients as small as a mean over a batch leaves them fall
+// out of its range.  Over queries a row has its own M, over keys M is the batch item's.
+// The row norms come from the kernel that forms delta.  Powers of two, taken out again
+// at the end.
 //
 // Bound: per 128 x 64 tile 512 clocks of exponentials (16 per clock and SM) in
 // each kernel against 8 D (dK, dV) and 6 D (dQ) clocks of products.
@@ -67,7 +72,8 @@ struct BwdParams {
     const void* table;
     const float* nlse2;   // [B * Hq][Lq_pad] kShift - log2 units; -inf: no gradient
     const float* ndelta;  // [B * Hq][Lq_pad]
-    const uint32_t* top;  // bits of max |dO| (fp16)
+    const float* norm2;   // fp16: [B * Hq][Lq_pad] |dO row|^2
+    const uint32_t* tops; // fp16: [B] bits of max |dO row|^2, max |v row|^2
     void* d1;             // keys: dk; queries: dq
     void* d2;             // keys: dv
     float* part;          // split items: [item][split][d1, d2][128][D] fp32
@@ -133,6 +139,16 @@ __host__ __device__ inline int bias_bytes(bool keys, int groups, int entries, in
     const int e = (entries + 15) / 16 * 16;
     return keys ? e + groups * e * 4 : e + (1 + groups) * e * 4 + groups * 4 * buckets * 4 + groups * kRows * kPitch * 4;
 }
+
+// Exponent e with 2^8 <= 2^e M < 2^9 for M = 2 sqrt(g2 v2), from the squared norms of a
+// row of dO and of the largest row of V; 0 where M is 0 (dS is) or not finite.
+__device__ __forceinline__ int ds_exponent(float g2, float v2)
+{
+    const int m = static_cast<int>(__float_as_uint(2.0f * sqrtf(g2 * v2)) >> 23);  // 127 + that of M
+    return m > 0 && m < 255 ? 127 + 8 - m : 0;
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
 template <typename T, int DP, bool KEYS, bool BIAS>
 __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::kCtas)
@@ -406,24 +422,23 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             __syncwarp();
             if (lane == 0) umma::mbar_arrive(at(bar->r_full));
         }
-        // fp16: f = 2^e, e = 127 - the biased exponent of max |dO|; without tiles nobody may have
-        // written that maximum, and every sum is 0
-        float f = 1.0f;
-        if (kHalf && n > 0) {
-            const int top = static_cast<int>(__ldcg(p.top) >> 23);
-            if (top > 0 && top < 255) f = __int_as_float((254 - top) << 23);
-        }
+        // fp16: dS is kept times 2^e too; without tiles nobody may have written the norms, and every
+        // sum is 0
+        int e = 0;
         bool row_ok = row < (KEYS ? len : p.Lq);
         float my_nlse = -INFINITY, my_ndelta = 0.0f;
         if (KEYS) {
             if (row_ok && p.key_mask != nullptr) row_ok = __ldg(p.key_mask + static_cast<int64_t>(b) * p.Lk + row) != 0;
+            if (kHalf && n > 0) e = ds_exponent(f32(__ldcg(p.tops + 2 * b)), f32(__ldcg(p.tops + 2 * b + 1)));
         } else if (row_ok) {
             const int64_t i = (static_cast<int64_t>(b) * p.Hq + h) * p.Lq_pad + row;
-            my_nlse = __ldcg(p.nlse2 + i);
-            my_ndelta = __ldcg(p.ndelta + i) * f;
+            if (kHalf && n > 0) e = ds_exponent(__ldcg(p.norm2 + i), f32(__ldcg(p.tops + 2 * b + 1)));
+            my_nlse = __ldcg(p.nlse2 + i) + e;  // P is not needed without its 2^e here
+            my_ndelta = __ldcg(p.ndelta + i);
         }
+        const float f = power_of_two(e), inv_f = power_of_two(-e);
         const bool any_row = row0 + warp % 4 * 32 < (KEYS ? len : p.Lq);  // else this warp keeps the barriers only
-        const Pair scale_2 = pair(p.scale2, p.scale2), f_2 = pair(f, f), ndelta_2 = pair(my_ndelta, my_ndelta);
+        const Pair scale_2 = pair(p.scale2, p.scale2), f_2 = KEYS ? pair(f, f) : pair(inv_f, inv_f), ndelta_2 = pair(my_ndelta, my_ndelta);
         int built = -1;  // KEYS: head of `values`
         float* diag = values + (1 + wg) * entries;
         float* plain = values + (1 + kGroups) * entries + warp * p.rel.total;
@@ -508,15 +523,15 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                         }
                         const Pair dp = pair(f32(d[j]), f32(d[j + 1]));
                         Pair ds;
-                        if (!kHalf) ds = mul2(pair(p0, p1), add2(dp, nd));
-                        else if (KEYS) ds = mul2(pair(p0, p1), mul2(add2(dp, nd), f_2));
-                        else ds = mul2(pair(p0, p1), fma2(dp, f_2, nd));
+                        if (kHalf && KEYS) ds = mul2(pair(p0, p1), mul2(add2(dp, nd), f_2));
+                        else ds = mul2(pair(p0, p1), add2(dp, nd));
                         if (BIAS && !KEYS && !W) total = add2(total, ds);
                         float d0, d1;
                         unpair(ds, d0, d1);
                         if (KEYS) pk[j / 2] = pack2<T>(p0, p1);
                         dk[j / 2] = pack2<T>(d0, d1);
                         if (W && !KEYS) {
+                            if (kHalf) unpair(mul2(ds, f_2), d0, d1);  // rows meet in the table's sums: without 2^e
                             tile[r * kPitch + c * 16 + j] = d0;
                             tile[r * kPitch + c * 16 + j + 1] = d1;
                         }
@@ -544,7 +559,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                 if (mine == nullptr) {
                     float t0, t1;
                     unpair(total, t0, t1);
-                    t0 += t1;
+                    t0 = (t0 + t1) * inv_f;
                     for (int o = 16; o > 0; o >>= 1) t0 += __shfl_xor_sync(~0u, t0, o);
                     if (lane == 0) plain[flat_bucket] += t0;
                 } else {
@@ -586,7 +601,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         const int rows_of = KEYS ? p.Lk : p.Lq;
         constexpr int kSpan = (KEYS ? 2 : 1) * DP / kGroups;
         const bool second = KEYS && wg >= kGroups / 2;
-        const float mul = second ? 1.0f / (1 << kShift) : p.scale / (1 << kShift) / f;
+        const float mul = second ? 1.0f / (1 << kShift) : p.scale / (1 << kShift) * inv_f;
         const int begin = (KEYS ? wg % (kGroups / 2) : wg) * kSpan;
         const uint32_t acc = tmem + lanes + (second ? L::kAcc2 : L::kAcc1) + begin;
         T* to = static_cast<T*>(second ? p.d2 : p.d1) + ((static_cast<int64_t>(b) * rows_of + row) * heads + h) * p.D;
@@ -629,11 +644,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
         // buckets of this CTA: 8 lanes run over a bucket's positions
         const float* diag = values + entries;
         const float* plain = values + (1 + kGroups) * entries;
-        float back = 1.0f / (1 << kShift);
-        if (kHalf) {
-            const int top = static_cast<int>(__ldcg(p.top) >> 23);
-            if (top > 0 && top < 255) back *= __int_as_float(top << 23);  // 1 / f
-        }
+        constexpr float back = 1.0f / (1 << kShift);
         const int sub = lane % 8;
         for (int t0 = warp * 4; t0 < p.rel.total; t0 += kThreads / 8) {
             const int t = min(t0 + lane / 8, p.rel.total - 1);
@@ -655,51 +666,80 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
 }
 
 // -delta = -rowsum(dO * O) and kShift - lse in log2 units, both laid out
-// [B * Hq][Lq_pad] with rows of no gradient (lse -inf, padding) at nlse2 = -inf; for fp16 also
-// max |dO| (an integer maximum of non-negative floats: no order).  kLanes >= D / 8
-// lanes per row, 8 values each.
+// [B * Hq][Lq_pad] with rows of no gradient (lse -inf, padding) at nlse2 = -inf; for fp16
+// also |dO row|^2, laid out the same, and each batch item's largest of them and of the
+// valid rows of V, which the blocks from first_v on read (an integer maximum of
+// non-negative floats: no order; a NaN is above all).  kLanes >= D / 8 lanes per row,
+// 8 values each.
+struct DeltaParams {
+    float *nlse2, *ndelta, *norm2;
+    uint32_t* tops;
+    int32_t Lq_pad, first_v;
+    Divisor by_q, by_v, by_hq, by_hk;  // blocks of a batch item, heads
+};
+
 template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ ww_attention_t a, float* nlse2,
-                                                              float* ndelta, uint32_t* top, int Lq_pad, Divisor by_blocks,
-                                                              Divisor by_head)
+__global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ ww_attention_t a,
+                                                              const __grid_constant__ DeltaParams p)
 {
-    const int b = by_blocks.div(blockIdx.x), lane = threadIdx.x % kLanes;
-    const int64_t rows = static_cast<int64_t>(Lq_pad) * a.Hq;  // of a batch item
-    const int64_t item = static_cast<int64_t>(blockIdx.x - b * by_blocks.d) * (256 / kLanes) + threadIdx.x / kLanes;
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const bool of_v = kHalf && static_cast<int>(blockIdx.x) >= p.first_v;
+    const Divisor &by_block = of_v ? p.by_v : p.by_q, &by_head = of_v ? p.by_hk : p.by_hq;
+    const int x = blockIdx.x - (of_v ? p.first_v : 0), b = by_block.div(x), lane = threadIdx.x % kLanes;
+    const int64_t rows = static_cast<int64_t>(of_v ? a.Lk : p.Lq_pad) * by_head.d;  // of a batch item
+    const int64_t item = static_cast<int64_t>(x - b * by_block.d) * (256 / kLanes) + threadIdx.x / kLanes;
     // 64-bit divisions would be most of the kernel
-    const int i = rows <= INT32_MAX - 256 ? by_head.div(static_cast<int>(item)) : static_cast<int>(item / a.Hq);
-    const int h = static_cast<int>(item - static_cast<int64_t>(i) * a.Hq);
-    const bool live = item < rows && i < a.Lq;
-    float sum = 0.0f, mx = 0.0f;
-    if (live && lane * 8 < a.D) {
-        const T* g = static_cast<const T*>(a.dout) + b * a.dout_strides[0] + i * a.dout_strides[1] + h * a.dout_strides[2];
-        const T* o = static_cast<const T*>(a.out) + ((static_cast<int64_t>(b) * a.Lq + i) * a.Hq + h) * a.D;
-        const uint4 gu = *reinterpret_cast<const uint4*>(g + lane * 8);
-        const uint4 ou = *reinterpret_cast<const uint4*>(o + lane * 8);
-        const T* ge = reinterpret_cast<const T*>(&gu);
-        const T* oe = reinterpret_cast<const T*>(&ou);
+    const int i = rows <= INT32_MAX - 256 ? by_head.div(static_cast<int>(item)) : static_cast<int>(item / by_head.d);
+    const int h = static_cast<int>(item - static_cast<int64_t>(i) * by_head.d);
+    float sum = 0.0f, square = 0.0f;
+    if (!of_v) {
+        const bool live = item < rows && i < a.Lq;
+        if (live && lane * 8 < a.D) {
+            const T* g = static_cast<const T*>(a.dout) + b * a.dout_strides[0] + i * a.dout_strides[1] + h * a.dout_strides[2];
+            const T* o = static_cast<const T*>(a.out) + ((static_cast<int64_t>(b) * a.Lq + i) * a.Hq + h) * a.D;
+            const uint4 gu = *reinterpret_cast<const uint4*>(g + lane * 8);
+            const uint4 ou = *reinterpret_cast<const uint4*>(o + lane * 8);
+            const T* ge = reinterpret_cast<const T*>(&gu);
+            const T* oe = reinterpret_cast<const T*>(&ou);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            sum = fmaf(to_float(ge[j]), to_float(oe[j]), sum);
-            mx = fmaxf(mx, fabsf(to_float(ge[j])));
+            for (int j = 0; j < 8; ++j) {
+                sum = fmaf(to_float(ge[j]), to_float(oe[j]), sum);
+                if (kHalf) square = fmaf(to_float(ge[j]), to_float(ge[j]), square);
+            }
         }
-    }
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (item < rows && lane == 0) {
-        const int64_t to = (static_cast<int64_t>(b) * a.Hq + h) * Lq_pad + i;
-        const float l = live ? a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Lq + i] : -INFINITY;
-        nlse2[to] = l == -INFINITY ? -INFINITY : kShift - l * kLog2eF;
-        ndelta[to] = -sum;
+        for (int o = kLanes / 2; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(~0u, sum, o);
+            if (kHalf) square += __shfl_xor_sync(~0u, square, o);
+        }
+        if (item < rows && lane == 0) {
+            const int64_t to = (static_cast<int64_t>(b) * a.Hq + h) * p.Lq_pad + i;
+            const float l = live ? a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Lq + i] : -INFINITY;
+            p.nlse2[to] = l == -INFINITY ? -INFINITY : kShift - l * kLog2eF;
+            p.ndelta[to] = -sum;
+            if (kHalf) p.norm2[to] = square;
+        }
+    } else {
+        const int64_t key = static_cast<int64_t>(b) * a.Lk + i;
+        if (item < rows && i < (a.k_lens == nullptr ? a.Lk : a.k_lens[b]) && (a.key_mask == nullptr || a.key_mask[key] != 0) &&
+            lane * 8 < a.D) {
+            const T* v = static_cast<const T*>(a.v) + b * a.v_strides[0] + i * a.v_strides[1] + h * a.v_strides[2];
+            const uint4 u = *reinterpret_cast<const uint4*>(v + lane * 8);
+            const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) square = fmaf(to_float(e[j]), to_float(e[j]), square);
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
     }
-    if (std::is_same<T, __half>::value) {
+    if (kHalf) {
         __shared__ uint32_t block_top;
         if (threadIdx.x == 0) block_top = 0;
         __syncthreads();
-        const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(mx));
+        const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(square) & 0x7fffffffu);
         if (threadIdx.x % 32 == 0) atomicMax(&block_top, m);
         __syncthreads();
-        if (threadIdx.x == 0 && block_top > 0) atomicMax(top, block_top);
+        if (threadIdx.x == 0 && block_top > 0) atomicMax(p.tops + 2 * b + of_v, block_top);
     }
 }
 
@@ -817,7 +857,7 @@ Half make_half(int blocks, int64_t items, int64_t tiles, int slots) noexcept
 struct Plan {
     Half q, k;
     int Lq_pad;
-    int64_t nlse2, ndelta, q_part, k_part, table, bytes;  // byte offsets; the maximum of |dO| stands first
+    int64_t nlse2, ndelta, norm2, q_part, k_part, table, bytes;  // byte offsets; fp16's largest norms stand first
 };
 
 bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
@@ -836,9 +876,10 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     r.k = make_half(k_blocks, k_items, full ? 1 : i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), k_slots);
     const int64_t rows = i64(p.B) * p.Hq * r.Lq_pad;
     const int64_t q_part = i64(r.q.rest) * r.q.splits * kRows * p.D * 4, k_part = i64(r.k.rest) * r.k.splits * 2 * kRows * p.D * 4;
-    r.nlse2 = 256;
+    r.nlse2 = (i64(p.B) * 8 + 255) / 256 * 256;
     r.ndelta = r.nlse2 + rows * 4;
-    r.q_part = r.ndelta + rows * 4;
+    r.norm2 = r.ndelta + rows * 4;
+    r.q_part = r.norm2 + (p.dtype == WW_DTYPE_HALF ? rows * 4 : 0);
     r.k_part = r.q_part + q_part;
     r.table = r.k_part + k_part;
     r.bytes = r.table + (p.bias_table != nullptr ? r.q.ctas() * p.num_buckets * 4 : 0);
@@ -905,7 +946,8 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     f.k_lens = p.k_lens;
     f.key_mask = p.key_mask;
     f.table = p.bias_table;
-    f.top = reinterpret_cast<uint32_t*>(ws);
+    f.tops = reinterpret_cast<uint32_t*>(ws);
+    f.norm2 = reinterpret_cast<float*>(ws + plan.norm2);
     f.nlse2 = reinterpret_cast<float*>(ws + plan.nlse2);
     f.ndelta = reinterpret_cast<float*>(ws + plan.ndelta);
     f.table_part = reinterpret_cast<float*>(ws + plan.table);
@@ -934,15 +976,18 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
 
     int st = WW_SUCCESS;
     if (has_q) {
-        if (!bf && cudaMemsetAsync(ws, 0, 4, stream) != cudaSuccess) return launch_status("cross_attention_backward");
+        if (!bf && cudaMemsetAsync(ws, 0, static_cast<size_t>(p.B) * 8, stream) != cudaSuccess)
+            return launch_status("cross_attention_backward");
         const int per = p.D <= 32 ? 64 : p.D <= 64 ? 32 : 16;  // rows of a block
-        const int64_t of_item = (i64(plan.Lq_pad) * p.Hq + per - 1) / per, blocks = of_item * p.B;
-        if (blocks > 0x7fffffff) return WW_ERR_UNSUPPORTED;
+        const int64_t of_q = (i64(plan.Lq_pad) * p.Hq + per - 1) / per, of_v = bf ? 0 : (i64(p.Lk) * p.Hk + per - 1) / per;
+        if ((of_q + of_v) * p.B > 0x7fffffff) return WW_ERR_UNSUPPORTED;
+        const DeltaParams delta = {const_cast<float*>(f.nlse2), const_cast<float*>(f.ndelta), const_cast<float*>(f.norm2),
+                                   reinterpret_cast<uint32_t*>(ws), plan.Lq_pad, static_cast<int>(of_q * p.B),
+                                   make_divisor(static_cast<int>(of_q)), make_divisor(of_v > 0 ? static_cast<int>(of_v) : 1),
+                                   make_divisor(p.Hq), make_divisor(p.Hk)};
         const auto kernel = per == 64 ? attention_delta_kernel<T, 4> : per == 32 ? attention_delta_kernel<T, 8>
                                                                                  : attention_delta_kernel<T, 16>;
-        kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, const_cast<float*>(f.nlse2), const_cast<float*>(f.ndelta),
-                                                                  reinterpret_cast<uint32_t*>(ws), plan.Lq_pad,
-                                                                  make_divisor(static_cast<int>(of_item)), make_divisor(p.Hq));
+        kernel<<<static_cast<unsigned>((of_q + of_v) * p.B), 256, 0, stream>>>(p, delta);
         st = launch_status("cross_attention_backward");
     }
     const int far = 2 * (p.max_distance + kRelMargin) + 1;
