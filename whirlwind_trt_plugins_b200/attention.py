@@ -7,7 +7,7 @@ with their gradients.  (The reference library has none; the formulas stand in
 * ``qk_norm_rope`` / ``qk_norm_rope_backward``
 * ``cross_attention`` / ``cross_attention_backward``
 * ``qk_norm_rope_autograd``, ``cross_attention_autograd`` -- the same as
-  differentiable torch functions
+  differentiable torch functions (first derivatives; a second raises)
 * ``relative_position_bucket`` -- the bucket of one distance (host)
 
 Vectors are ``[B, L, H, D]`` CUDA tensors with unit stride along D; the other
@@ -328,6 +328,7 @@ def _strided(g):
 @functools.cache
 def _functions():
     torch = _torch()
+    from torch.autograd.function import once_differentiable  # a second derivative raises instead of being dropped
 
     class QkNormRope(torch.autograd.Function):
         @staticmethod
@@ -337,6 +338,7 @@ def _functions():
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved)
 
         @staticmethod
+        @once_differentiable
         def backward(ctx, dq_out, dk_out):
             got = qk_norm_rope_backward(_strided(dq_out), _strided(dk_out), *ctx.saved_tensors, *ctx.more)
             return (*got, None, None, None, None, None, None)
@@ -351,6 +353,7 @@ def _functions():
             return out
 
         @staticmethod
+        @once_differentiable
         def backward(ctx, dout):
             q, k, v, out, lse, k_lens, key_mask, bias_table = ctx.saved_tensors
             scale, *more = ctx.more
@@ -363,11 +366,11 @@ def _functions():
 
 def qk_norm_rope_autograd(q, k, q_weight, k_weight, cos, sin, q_pos=None, k_pos=None, eps: float = 1e-6,
                           interleaved: bool = False):
-    """``qk_norm_rope`` as a differentiable torch function of q, k and the weights."""
+    """``qk_norm_rope`` as a torch function of q, k and the weights that can be differentiated once."""
     return _functions()[0].apply(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved)
 
 
 def cross_attention_autograd(q, k, v, bias_table=None, k_lens=None, key_mask=None, scale: float | None = None,
                              max_distance: int = 128, bidirectional: bool = True, q_offset: int = 0):
-    """``cross_attention`` as a differentiable torch function of q, k, v and bias_table."""
+    """``cross_attention`` as a torch function of q, k, v and bias_table that can be differentiated once."""
     return _functions()[1].apply(q, k, v, bias_table, k_lens, key_mask, scale, max_distance, bidirectional, q_offset)
