@@ -6,6 +6,7 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace ww {
@@ -288,6 +289,22 @@ __device__ __forceinline__ void warpgroup_sync(int w)
     else if (w == 1) asm volatile("bar.sync 2, 128;" : : : "memory");
     else if (w == 2) asm volatile("bar.sync 3, 128;" : : : "memory");
     else asm volatile("bar.sync 4, 128;" : : : "memory");
+}
+
+// Lets a kernel be launched with any dynamic shared memory that the current device has.
+// The limit belongs to the kernel, not to a call: set to every call's own size, one host
+// thread could lower it between another's setting and its launch.  So it is raised once,
+// to the most; `raised` is the kernel's, a bit per device.
+inline bool allow_shared_memory(const void* kernel, std::atomic<uint64_t>& raised) noexcept
+{
+    int dev = 0;
+    DeviceInfo d;
+    if (cudaGetDevice(&dev) != cudaSuccess || current_device_info(&d) != WW_SUCCESS) return false;
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if ((raised.load(std::memory_order_acquire) & bit) != 0) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, d.smem_optin) != cudaSuccess) return false;
+    raised.fetch_or(bit, std::memory_order_release);
+    return true;
 }
 
 // Launch of a kernel that follows another one of the same call: it may be set up

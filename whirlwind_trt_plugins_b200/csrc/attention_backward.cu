@@ -892,8 +892,8 @@ int launch_one(const BwdParams& f, int64_t ctas, bool behind, cudaStream_t strea
     using L = Layout<DP, KEYS>;
     const auto kernel = attention_backward_kernel<T, DP, KEYS, BIAS>;
     const int bytes = 1024 + L::kBias + (BIAS ? bias_bytes(KEYS, L::kGroups, f.max_entries, f.rel.total) : 0);
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-        return launch_status("cross_attention_backward");
+    static std::atomic<uint64_t> raised{0};
+    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention_backward");
     if (behind) launch_behind(kernel, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), bytes, stream, f);
     else kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
     return launch_status("cross_attention_backward");

@@ -756,8 +756,8 @@ int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
     using L = Layout<DP, NT>;
     const auto kernel = attention_forward_kernel<T, DP, NT>;
     const int bytes = L::kTotal + 4 * f.max_entries;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-        return launch_status("cross_attention");
+    static std::atomic<uint64_t> raised{0};
+    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention");
     kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
     return launch_status("cross_attention");
 }

@@ -371,8 +371,8 @@ int launch(const TokenParams& f, int64_t ctas, cudaStream_t stream) noexcept
     using L = Layout<DP, MB>;
     const auto kernel = attention_token_kernel<T, DP, MB>;
     const int bytes = L::kBytes + (f.table != nullptr ? f.Hq / f.Hk * f.rel.total * 4 + f.max_entries : 0);
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-        return launch_status("cross_attention");
+    static std::atomic<uint64_t> raised{0};
+    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention");
     kernel<<<static_cast<unsigned>(ctas), kWarps * 32, bytes, stream>>>(f);
     return launch_status("cross_attention");
 }
