@@ -26,6 +26,21 @@ EncodeTiledFn encode_fn() noexcept
     return fn;
 }
 
+// Encodes a tiled map.  The driver's function wants a current context, which a host
+// thread gets from the runtime only at its first call that works on the device (asking
+// for the current device is none): a thread that starts with one of this library's
+// calls is given it here, where the first attempt fails.
+template <typename... A>
+bool encode(EncodeTiledFn fn, A... args) noexcept
+{
+    if (fn(args...) == CUDA_SUCCESS) return true;
+    if (cudaFree(nullptr) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return fn(args...) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 bool encode_feature_map(CUtensorMap* out, const void* base, int B, int C, int rows, int W, int box_x, int box_z,
@@ -43,11 +58,10 @@ bool encode_feature_map(CUtensorMap* out, const void* base, int B, int C, int ro
     const cuuint64_t strides[3] = {row_b, row_b * rows, row_b * rows * C};
     const cuuint32_t box[4] = {static_cast<cuuint32_t>(box_x), 1u, static_cast<cuuint32_t>(box_z), 1u};
     const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS;
+    return encode(fn, out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 bool encode_volume_map(CUtensorMap* out, const void* base, int B, int G, int D, int H, int W, int box_x, int box_d,
@@ -67,10 +81,9 @@ bool encode_volume_map(CUtensorMap* out, const void* base, int B, int G, int D, 
     const cuuint32_t box[5] = {static_cast<cuuint32_t>(box_x), 1u, static_cast<cuuint32_t>(box_d),
                                static_cast<cuuint32_t>(box_g), 1u};
     const cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
-    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS;
+    return encode(fn, out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 bool encode_vectors_map(CUtensorMap* out, bool bf16, const void* base, int D, const int (&n)[3],
@@ -95,11 +108,10 @@ bool encode_vectors_map(CUtensorMap* out, bool bf16, const void* base, int D, co
     }
     const cuuint32_t box[4] = {static_cast<cuuint32_t>(box_cols), 1u, static_cast<cuuint32_t>(box_rows), 1u};
     const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-    const CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                          const_cast<void*>(base), dims, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS;
+    return encode(fn, out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<void*>(base), dims, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 }  // namespace ww
