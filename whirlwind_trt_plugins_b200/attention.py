@@ -322,7 +322,9 @@ def _strided(g):
     """An incoming gradient in a layout the kernels take (autograd hands over any)."""
     st, step = g.stride(), 16 // g.element_size()
     ok = g.data_ptr() % 16 == 0 and st[3] == 1 and all(n <= 1 or s % step == 0 for n, s in zip(g.shape[:3], st[:3]))
-    return g if ok and (g.shape[1] <= 1 or st[1]) else g.contiguous()
+    if ok and (g.shape[1] <= 1 or st[1]):
+        return g
+    return g.clone(memory_format=_torch().contiguous_format)  # contiguous() keeps a view that starts off the grid
 
 
 @functools.cache
