@@ -472,7 +472,7 @@ int ww_plugin_disparity_regression_enqueue(int mode, const ww_tensor_desc_t* in_
 
 /* "CrossAttention" v"1" (extension): ww_cross_attention with scale 1 / sqrt(D).
  * Inputs q [B, Lq, Hq, D], k, v [B, Lk, Hk, D] (fp16 or bf16), then those that
- * `flags` names, in this order: k_lens [B] int32, key_mask [B, Lk] bool or uint8,
+ * `flags` names, in this order: k_lens [B] int32, key_mask [B, Lk] bool, uint8 or INT8 bytes,
  * bias_table [Hq, num_buckets] (the type of q); output like q.  Fields
  * use_lens, use_mask, use_bias (0), max_distance (128), bidirectional (1),
  * q_offset (0).  `workspace` is NULL or WW_PLUGIN_ATTENTION_WORKSPACE bytes,

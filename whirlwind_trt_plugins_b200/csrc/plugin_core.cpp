@@ -437,7 +437,9 @@ int ww_plugin_cross_attention_supports_format(int flags, int pos, const ww_tenso
     if (pos >= 3 && pos < nb_inputs) {
         const int role = attention_role(flags, pos);
         if (role == WW_PLUGIN_ATTENTION_LENS) return d.dtype == WW_DTYPE_INT32;
-        if (role == WW_PLUGIN_ATTENTION_MASK) return d.dtype == WW_DTYPE_BOOL || d.dtype == WW_DTYPE_UINT8;
+        // bytes, 0 or not; declared INT8 as NV12's are, too
+        if (role == WW_PLUGIN_ATTENTION_MASK)
+            return d.dtype == WW_DTYPE_BOOL || d.dtype == WW_DTYPE_UINT8 || d.dtype == WW_DTYPE_INT8;
     }
     return d.dtype == in_out[0].dtype;
 }
