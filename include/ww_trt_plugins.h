@@ -236,6 +236,11 @@ int ww_multi_inject_copy_failure(int after_n_copies);
  * from the IEEE rounded a / divisor (1 <= divisor <= 1024; synchronises). */
 int ww_selftest_int_division(int divisor, unsigned long long* mismatches);
 
+/* Test hook: one device thread waits, with the bounded wait of the attention
+ * kernels, for a barrier that nothing completes; `ns` gets the time until it
+ * gave up (about a second; synchronises).  WW_ERR_LAUNCH if it did not. */
+int ww_selftest_bounded_wait(unsigned long long* ns);
+
 /* ---------------------------------------------------------------------------
  * CorrVolume (G = 1) fused with the reference's 3-stage CostStem3D, the pair
  * the reference runs at its native shape ([1, 1, 48, 32, 40]):

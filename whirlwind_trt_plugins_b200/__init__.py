@@ -99,6 +99,7 @@ def _load() -> ctypes.CDLL:
     L.ww_clear_device_error.argtypes = []
     L.ww_set_fused_corr_engine.argtypes = [i]
     L.ww_selftest_int_division.argtypes = [i, ctypes.POINTER(ctypes.c_ulonglong)]
+    L.ww_selftest_bounded_wait.argtypes = [ctypes.POINTER(ctypes.c_ulonglong)]
     L.ww_get_fused_corr_engine.argtypes = []
     del f
     return L

@@ -1,6 +1,8 @@
 // attention_host.cu -- host side that the attention entry points share:
-// argument checks and the relative-position bucket edges.
+// argument checks and the relative-position bucket edges; the test hook of their
+// device waits.
 #include "attention.cuh"
+#include "umma.cuh"
 
 #include <cmath>
 
@@ -98,7 +100,40 @@ int check_attention_backward(const ww_attention_t& p, int64_t need) noexcept
     return WW_SUCCESS;
 }
 
+namespace {
+
+// Time until the wait for a barrier that nothing completes gave up; 0 if it did not.
+__device__ unsigned long long g_bounded_wait_ns;
+
+__global__ void bounded_wait_kernel()
+{
+    __shared__ uint64_t bar;
+    const auto now = [] {
+        unsigned long long t;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+        return t;
+    };
+    umma::mbar_init(umma::smem_addr(&bar), 1);
+    umma::mbar_fence_init();
+    const unsigned long long start = now();
+    const bool done = umma::mbar_poll(umma::smem_addr(&bar), 0);
+    g_bounded_wait_ns = done ? 0 : now() - start;
+}
+
+}  // namespace
 }  // namespace ww
+
+extern "C" int ww_selftest_bounded_wait(unsigned long long* ns)
+{
+    if (ns == nullptr) return WW_ERR_NULL_POINTER;
+    ww::DeviceInfo d;
+    const int st = ww::current_device_info(&d);
+    if (st != WW_SUCCESS) return st;
+    ww::bounded_wait_kernel<<<1, 1>>>();
+    if (cudaMemcpyFromSymbol(ns, ww::g_bounded_wait_ns, sizeof(*ns)) != cudaSuccess)
+        return ww::launch_status("ww_selftest_bounded_wait");
+    return *ns != 0 ? WW_SUCCESS : WW_ERR_LAUNCH;
+}
 
 extern "C" int ww_relative_position_bucket(int rel, int num_buckets, int max_distance, int bidirectional)
 {

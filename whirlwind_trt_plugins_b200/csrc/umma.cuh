@@ -266,9 +266,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t saddr, uint32_t parity)
     return false;
 }
 
-// The same bound by count of non-blocking polls, for waits of a few hundred
-// clocks between warps that all have work.
-constexpr uint32_t kPollRounds = 1u << 26;
+// The same for waits of a few hundred clocks between warps that all have work: no
+// polls before the first try_wait.  Without a time of its own a try_wait holds the
+// thread for up to 4 us, so the bound is about a second; copies that were issued
+// before the wait have had that long to land when it runs out.
+constexpr uint32_t kPollRounds = 1u << 18;
 __device__ __forceinline__ bool mbar_poll(uint32_t saddr, uint32_t parity)
 {
     for (uint32_t i = 0; i < kPollRounds; ++i)
