@@ -338,6 +338,23 @@ __device__ __forceinline__ void start_launch_behind()
     asm volatile("griddepcontrol.launch_dependents;" : : : "memory");
 }
 
+__device__ __forceinline__ void store_release(uint32_t* to, uint32_t v)
+{
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" : : "l"(to), "r"(v) : "memory");
+}
+
+// Waits until *from is v: what the thread that released it had seen, this one sees too.
+// Bounded (about half a second); false if it ran out.
+__device__ __forceinline__ bool wait_acquire(const uint32_t* from, uint32_t v)
+{
+    for (int i = 0; i < 1 << 20; ++i) {
+        uint32_t x;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(x) : "l"(from) : "memory");
+        if (x == v) return true;
+    }
+    return false;
+}
+
 // Share [first, first + n) of part `split` of `splits` in `all` steps (a 64-bit
 // division is worth avoiding where there is one part).
 __device__ __forceinline__ void part_of(int all, int split, int splits, int& first, int& n)

@@ -74,6 +74,7 @@ struct BwdParams {
     const float* ndelta;  // [B * Hq][Lq_pad]
     const float* norm2;   // fp16: [B * Hq][Lq_pad] |dO row|^2
     const uint32_t* tops; // fp16: [B] bits of max |dO row|^2, max |v row|^2
+    uint32_t* seen;       // set by `keys` once it has seen the three above; null where `queries` runs alone
     void* d1;             // keys: dk; queries: dq
     void* d2;             // keys: dv
     float* part;          // split items: [item][split][d1, d2][128][D] fp32
@@ -165,8 +166,9 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
     Bar* bar = reinterpret_cast<Bar*>(base + L::kBar);
     const auto at = [](const uint64_t& b) { return umma::smem_addr(&b); };
 
-    // `keys` waits for the deltas; `queries` starts while the last CTAs of `keys` run,
-    // which have seen the deltas complete: it reads them past the L1 caches
+    // `keys` waits for the grid of the deltas.  `queries` starts while the last CTAs of `keys`
+    // run and is not ordered behind that grid by its launch: `keys` passes the order on, by a
+    // word that it releases after its wait and `queries` acquires before it reads them
     if (KEYS) wait_for_launches_before();
 
     // items (row block, head, batch item); the last ones are split over their streamed tiles
@@ -283,7 +285,13 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
             for (int e = threadIdx.x; wg < kGroups && e < kGroups * entries + kGroups * 4 * p.rel.total; e += kGroups * 128)
                 values[entries + e] = 0.0f;
     }
-    if (warp == kMmaWarp) umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
+    if (KEYS && blk == 0 && threadIdx.x == 0 && p.seen != nullptr) store_release(p.seen, 1);
+    if (warp == kMmaWarp) {
+        // set before `queries` can start, so the first look finds it
+        if (!KEYS && p.seen != nullptr && !wait_acquire(p.seen, 1) && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x33);
+        __syncwarp();
+        umma::tmem_alloc(umma::smem_addr(&bar->tmem), L::kColumns);
+    }
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
@@ -673,7 +681,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
 // 8 values each.
 struct DeltaParams {
     float *nlse2, *ndelta, *norm2;
-    uint32_t* tops;
+    uint32_t *tops, *seen;
     int32_t Lq_pad, first_v;
     Divisor by_q, by_v, by_hq, by_hk;  // blocks of a batch item, heads
 };
@@ -683,6 +691,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
                                                               const __grid_constant__ DeltaParams p)
 {
     constexpr bool kHalf = std::is_same<T, __half>::value;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.seen = 0;  // what an earlier call left
     const bool of_v = kHalf && static_cast<int>(blockIdx.x) >= p.first_v;
     const Divisor &by_block = of_v ? p.by_v : p.by_q, &by_head = of_v ? p.by_hk : p.by_hq;
     const int x = blockIdx.x - (of_v ? p.first_v : 0), b = by_block.div(x), lane = threadIdx.x % kLanes;
@@ -857,7 +866,7 @@ Half make_half(int blocks, int64_t items, int64_t tiles, int slots) noexcept
 struct Plan {
     Half q, k;
     int Lq_pad;
-    int64_t nlse2, ndelta, norm2, q_part, k_part, table, bytes;  // byte offsets; fp16's largest norms stand first
+    int64_t seen, nlse2, ndelta, norm2, q_part, k_part, table, bytes;  // byte offsets; fp16's largest norms stand first
 };
 
 bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
@@ -876,7 +885,8 @@ bool make_plan(const ww_attention_t& p, int sms, Plan* plan) noexcept
     r.k = make_half(k_blocks, k_items, full ? 1 : i64(r.Lq_pad / kCols) * (p.Hq / p.Hk), k_slots);
     const int64_t rows = i64(p.B) * p.Hq * r.Lq_pad;
     const int64_t q_part = i64(r.q.rest) * r.q.splits * kRows * p.D * 4, k_part = i64(r.k.rest) * r.k.splits * 2 * kRows * p.D * 4;
-    r.nlse2 = (i64(p.B) * 8 + 255) / 256 * 256;
+    r.seen = i64(p.B) * 8;
+    r.nlse2 = (r.seen + 4 + 255) / 256 * 256;
     r.ndelta = r.nlse2 + rows * 4;
     r.norm2 = r.ndelta + rows * 4;
     r.q_part = r.norm2 + (p.dtype == WW_DTYPE_HALF ? rows * 4 : 0);
@@ -948,6 +958,7 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
     f.table = p.bias_table;
     f.tops = reinterpret_cast<uint32_t*>(ws);
     f.norm2 = reinterpret_cast<float*>(ws + plan.norm2);
+    f.seen = has_q && has_k ? reinterpret_cast<uint32_t*>(ws + plan.seen) : nullptr;
     f.nlse2 = reinterpret_cast<float*>(ws + plan.nlse2);
     f.ndelta = reinterpret_cast<float*>(ws + plan.ndelta);
     f.table_part = reinterpret_cast<float*>(ws + plan.table);
@@ -982,7 +993,8 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
         const int64_t of_q = (i64(plan.Lq_pad) * p.Hq + per - 1) / per, of_v = bf ? 0 : (i64(p.Lk) * p.Hk + per - 1) / per;
         if ((of_q + of_v) * p.B > 0x7fffffff) return WW_ERR_UNSUPPORTED;
         const DeltaParams delta = {const_cast<float*>(f.nlse2), const_cast<float*>(f.ndelta), const_cast<float*>(f.norm2),
-                                   reinterpret_cast<uint32_t*>(ws), plan.Lq_pad, static_cast<int>(of_q * p.B),
+                                   reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + plan.seen),
+                                   plan.Lq_pad, static_cast<int>(of_q * p.B),
                                    make_divisor(static_cast<int>(of_q)), make_divisor(of_v > 0 ? static_cast<int>(of_v) : 1),
                                    make_divisor(p.Hq), make_divisor(p.Hk)};
         const auto kernel = per == 64 ? attention_delta_kernel<T, 4> : per == 32 ? attention_delta_kernel<T, 8>
