@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import unittest
 
 import numpy as np
 
@@ -79,6 +80,11 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+class ReferenceUnavailable(RuntimeError, unittest.SkipTest):
+    """The reference's kernels are not built here: a test that needs them is skipped, as those that look for the
+    library first are."""
+
+
 def ref_lib() -> ctypes.CDLL:
     """The reference's CUDA kernels (GPU box or a machine with a GPU)."""
     global _ref
@@ -86,8 +92,8 @@ def ref_lib() -> ctypes.CDLL:
         if not os.path.exists(REF_SO):
             build_ref()
         if not os.path.exists(REF_SO):
-            raise RuntimeError("oracle/_ref/libww_ref.so is missing; run `make -C oracle ref` "
-                               "where the reference sources are available")
+            raise ReferenceUnavailable("oracle/_ref/libww_ref.so is missing; run `make -C oracle ref` "
+                                       "where the reference sources are available")
         R = ctypes.CDLL(REF_SO)
         p, i = ctypes.c_void_p, ctypes.c_int
         R.wwref_corr_volume_f16.argtypes = [p, p, p] + [i] * 5 + [p]
