@@ -197,6 +197,10 @@ __device__ __forceinline__ float bias_value<__nv_bfloat16>(__nv_bfloat16 b)
 // memory; entry e stands for rel = lo + e.
 constexpr int kRelMargin = 256;
 constexpr int kMaxDistance = 1024;  // what fits beside the operands of the widest heads
+// positions that a CTA keeps at most
+__host__ __device__ constexpr int rel_positions(int max_distance) { return 2 * (max_distance + kRelMargin) + 1; }
+constexpr int kMaxPositions = rel_positions(kMaxDistance);
+constexpr int kMaxShared = 232448;  // dynamic shared memory of a CTA, bytes
 
 struct RelRange {
     int lo = 0, hi = -1;
@@ -307,9 +311,11 @@ inline bool allow_shared_memory(const void* kernel, std::atomic<uint64_t>& raise
     return true;
 }
 
-// Launch of a kernel that follows another one of the same call: it may be set up
-// while that one still runs, and waits for it (wait_for_launches_before) before
-// it reads what that one writes, at the latest before it ends itself.
+// Launch of a kernel that follows another one of the same call, and waits for it
+// (wait_for_launches_before) before it reads what that one writes, at the latest
+// before it ends itself.  Where that one calls start_launch_behind (the gradient's pass
+// over keys does), this kernel runs beside its last CTAs; else it starts when they have
+// ended, without the gap of a launch that waits for their writes first.
 template <typename... P, typename... A>
 inline cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) noexcept
 {

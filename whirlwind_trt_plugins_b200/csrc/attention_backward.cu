@@ -134,8 +134,8 @@ struct Bars {
 //   buckets  [E] bytes
 //   KEYS:    values [W][E] floats, rebuilt when the head changes
 //   queries: values [E], with the gradient's diagonals [W][E], plain sums
-//            [4 W warps][buckets] and dS [W][160][17] words
-__host__ __device__ inline int bias_bytes(bool keys, int groups, int entries, int buckets)
+//            [4 W warps][buckets] and dS [W][128][33] floats
+__host__ __device__ constexpr int bias_bytes(bool keys, int groups, int entries, int buckets)
 {
     const int e = (entries + 15) / 16 * 16;
     return keys ? e + groups * e * 4 : e + (1 + groups) * e * 4 + groups * 4 * buckets * 4 + groups * kRows * kPitch * 4;
@@ -901,6 +901,7 @@ int launch_one(const BwdParams& f, int64_t ctas, bool behind, cudaStream_t strea
 {
     using L = Layout<DP, KEYS>;
     const auto kernel = attention_backward_kernel<T, DP, KEYS, BIAS>;
+    static_assert(!BIAS || 1024 + L::kBias + bias_bytes(KEYS, L::kGroups, kMaxPositions, kMaxBuckets) <= kMaxShared, "shared memory");
     const int bytes = 1024 + L::kBias + (BIAS ? bias_bytes(KEYS, L::kGroups, f.max_entries, f.rel.total) : 0);
     static std::atomic<uint64_t> raised{0};
     if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention_backward");
@@ -1002,7 +1003,7 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
         kernel<<<static_cast<unsigned>((of_q + of_v) * p.B), 256, 0, stream>>>(p, delta);
         st = launch_status("cross_attention_backward");
     }
-    const int far = 2 * (p.max_distance + kRelMargin) + 1;
+    const int far = rel_positions(p.max_distance);
     if (st == WW_SUCCESS && has_k) {
         f.part = reinterpret_cast<float*>(ws + plan.k_part);
         f.d1 = p.dk;

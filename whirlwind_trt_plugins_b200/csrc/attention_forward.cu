@@ -755,6 +755,7 @@ int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, NT>;
     const auto kernel = attention_forward_kernel<T, DP, NT>;
+    static_assert(L::kTotal + 4 * ((kMaxPositions + 15) / 16 * 16) <= kMaxShared, "shared memory");
     const int bytes = L::kTotal + 4 * f.max_entries;
     static std::atomic<uint64_t> raised{0};
     if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention");
@@ -785,7 +786,7 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     if (p.bias_table != nullptr) {
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
         const int all = (p.Lk + 127) / 128 * 128 + (plan.wide ? plan.q_blocks : plan.per_cta) * plan.nt * kTile;
-        f.max_entries = (std::min(2 * (p.max_distance + kRelMargin) + 1, all) + 15) / 16 * 16;
+        f.max_entries = (std::min(rel_positions(p.max_distance), all) + 15) / 16 * 16;
     }
     f.part_o = part_o;
     f.part_lse = part_lse;

@@ -370,6 +370,7 @@ int launch(const TokenParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, MB>;
     const auto kernel = attention_token_kernel<T, DP, MB>;
+    static_assert(L::kBytes + MB * 16 * kMaxBuckets * 4 + kMaxPositions <= kMaxShared, "shared memory");
     const int bytes = L::kBytes + (f.table != nullptr ? f.Hq / f.Hk * f.rel.total * 4 + f.max_entries : 0);
     static std::atomic<uint64_t> raised{0};
     if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention");
@@ -397,7 +398,7 @@ int tokens(const ww_attention_t& p, int splits, float* part_o, float* part_lse, 
         make_buckets(p.num_buckets, p.max_distance, p.bidirectional, p.q_offset, &f.rel);
     f.max_entries = 0;
     if (p.bias_table != nullptr)
-        f.max_entries = static_cast<int>(std::min<int64_t>(2 * (p.max_distance + kRelMargin) + 1, i64(p.Lk) + 64 + p.Lq));
+        f.max_entries = static_cast<int>(std::min<int64_t>(rel_positions(p.max_distance), i64(p.Lk) + 64 + p.Lq));
     f.part_o = part_o;
     f.part_lse = part_lse;
     for (int i = 0; i < 3; ++i) f.q_strides[i] = p.q_strides[i];

@@ -413,7 +413,7 @@ int check(const ww_qk_norm_rope_t& p, bool backward) noexcept
     return WW_SUCCESS;
 }
 
-// Values of a lane's piece: 16 bytes where both halves split into them, else 4.
+// Values of a lane's piece: 8 of 16 bits where both halves split into them, else 4.
 int piece_values(const ww_qk_norm_rope_t& p)
 {
     if (p.dtype == WW_DTYPE_FLOAT) return 4;
