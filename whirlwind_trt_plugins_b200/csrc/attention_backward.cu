@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
 // also |dO row|^2, laid out the same, and each batch item's largest of them and of the
 // valid rows of V, which the blocks from first_v on read (an integer maximum of
 // non-negative floats: no order; a NaN is above all).  kLanes >= D / 8 lanes per row,
-// 8 values each.
+// 8 values each (of V 16).
 struct DeltaParams {
     float *nlse2, *ndelta, *norm2;
     uint32_t *tops, *seen;
@@ -686,60 +686,94 @@ struct DeltaParams {
     Divisor by_q, by_v, by_hq, by_hk;  // blocks of a batch item, heads
 };
 
+// 8 values as pairs of fp32.
+template <typename T>
+__device__ __forceinline__ void to_pairs(const uint4& u, Pair (&f)[4])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const T* e = reinterpret_cast<const T*>(&w[j]);
+        f[j] = pair(to_float(e[0]), to_float(e[1]));
+    }
+}
+
 template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ ww_attention_t a,
                                                               const __grid_constant__ DeltaParams p)
 {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.seen = 0;  // what an earlier call left
+    // token of row `row` of a batch item (64-bit divisions would be most of the kernel)
+    const auto token_of = [](int64_t row, int64_t rows, const Divisor& heads) {
+        return rows <= INT32_MAX - 512 ? heads.div(static_cast<int>(row)) : static_cast<int>(row / heads.d);
+    };
     const bool of_v = kHalf && static_cast<int>(blockIdx.x) >= p.first_v;
-    const Divisor &by_block = of_v ? p.by_v : p.by_q, &by_head = of_v ? p.by_hk : p.by_hq;
-    const int x = blockIdx.x - (of_v ? p.first_v : 0), b = by_block.div(x), lane = threadIdx.x % kLanes;
-    const int64_t rows = static_cast<int64_t>(of_v ? a.Lk : p.Lq_pad) * by_head.d;  // of a batch item
-    const int64_t item = static_cast<int64_t>(x - b * by_block.d) * (256 / kLanes) + threadIdx.x / kLanes;
-    // 64-bit divisions would be most of the kernel
-    const int i = rows <= INT32_MAX - 256 ? by_head.div(static_cast<int>(item)) : static_cast<int>(item / by_head.d);
-    const int h = static_cast<int>(item - static_cast<int64_t>(i) * by_head.d);
-    float sum = 0.0f, square = 0.0f;
+    float square;
+    int b;
     if (!of_v) {
-        const bool live = item < rows && i < a.Lq;
+        b = p.by_q.div(blockIdx.x);
+        const int lane = threadIdx.x % kLanes;
+        const int64_t rows = static_cast<int64_t>(p.Lq_pad) * a.Hq;
+        const int64_t row = static_cast<int64_t>(blockIdx.x - b * p.by_q.d) * (256 / kLanes) + threadIdx.x / kLanes;
+        const int i = token_of(row, rows, p.by_hq), h = static_cast<int>(row - static_cast<int64_t>(i) * a.Hq);
+        const bool live = row < rows && i < a.Lq;
+        Pair sums = pair(0.0f, 0.0f), squares = sums;
         if (live && lane * 8 < a.D) {
             const T* g = static_cast<const T*>(a.dout) + b * a.dout_strides[0] + i * a.dout_strides[1] + h * a.dout_strides[2];
-            const T* o = static_cast<const T*>(a.out) + ((static_cast<int64_t>(b) * a.Lq + i) * a.Hq + h) * a.D;
-            const uint4 gu = *reinterpret_cast<const uint4*>(g + lane * 8);
-            const uint4 ou = *reinterpret_cast<const uint4*>(o + lane * 8);
-            const T* ge = reinterpret_cast<const T*>(&gu);
-            const T* oe = reinterpret_cast<const T*>(&ou);
+            const T* o = static_cast<const T*>(a.out) + (static_cast<int64_t>(b) * a.Lq * a.Hq + row) * a.D;
+            Pair gp[4], op[4];
+            to_pairs<T>(*reinterpret_cast<const uint4*>(g + lane * 8), gp);
+            to_pairs<T>(*reinterpret_cast<const uint4*>(o + lane * 8), op);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sum = fmaf(to_float(ge[j]), to_float(oe[j]), sum);
-                if (kHalf) square = fmaf(to_float(ge[j]), to_float(ge[j]), square);
+            for (int j = 0; j < 4; ++j) {
+                sums = fma2(gp[j], op[j], sums);
+                if (kHalf) squares = fma2(gp[j], gp[j], squares);
             }
         }
+        float sum, other;
+        unpair(sums, sum, other);
+        sum += other;
+        unpair(squares, square, other);
+        square += other;
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) {
             sum += __shfl_xor_sync(~0u, sum, o);
             if (kHalf) square += __shfl_xor_sync(~0u, square, o);
         }
-        if (item < rows && lane == 0) {
-            const int64_t to = (static_cast<int64_t>(b) * a.Hq + h) * p.Lq_pad + i;
-            const float l = live ? a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Lq + i] : -INFINITY;
+        if (row < rows && lane == 0) {
+            const int64_t bh = static_cast<int64_t>(b) * a.Hq + h, to = bh * p.Lq_pad + i;
+            const float l = live ? a.lse[bh * a.Lq + i] : -INFINITY;
             p.nlse2[to] = l == -INFINITY ? -INFINITY : kShift - l * kLog2eF;
             p.ndelta[to] = -sum;
             if (kHalf) p.norm2[to] = square;
         }
     } else {
-        const int64_t key = static_cast<int64_t>(b) * a.Lk + i;
-        if (item < rows && i < (a.k_lens == nullptr ? a.Lk : a.k_lens[b]) && (a.key_mask == nullptr || a.key_mask[key] != 0) &&
-            lane * 8 < a.D) {
-            const T* v = static_cast<const T*>(a.v) + b * a.v_strides[0] + i * a.v_strides[1] + h * a.v_strides[2];
-            const uint4 u = *reinterpret_cast<const uint4*>(v + lane * 8);
-            const T* e = reinterpret_cast<const T*>(&u);
+        constexpr int kPer = kLanes / 2;  // lanes of a row: 16 values each
+        const int x = blockIdx.x - p.first_v, lane = threadIdx.x % kPer;
+        b = p.by_v.div(x);
+        const int64_t rows = static_cast<int64_t>(a.Lk) * a.Hk;
+        const int64_t row = static_cast<int64_t>(x - b * p.by_v.d) * (256 / kPer) + threadIdx.x / kPer;
+        const int j = token_of(row, rows, p.by_hk), h = static_cast<int>(row - static_cast<int64_t>(j) * a.Hk);
+        Pair squares = pair(0.0f, 0.0f);
+        if (row < rows && j < (a.k_lens == nullptr ? a.Lk : a.k_lens[b]) &&
+            (a.key_mask == nullptr || a.key_mask[static_cast<int64_t>(b) * a.Lk + j] != 0)) {
+            const T* v = static_cast<const T*>(a.v) + b * a.v_strides[0] + j * a.v_strides[1] + h * a.v_strides[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) square = fmaf(to_float(e[j]), to_float(e[j]), square);
+            for (int c = 0; c < 2; ++c) {
+                const int d = lane * 16 + c * 8;
+                if (d >= a.D) break;
+                Pair vp[4];
+                to_pairs<T>(*reinterpret_cast<const uint4*>(v + d), vp);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) squares = fma2(vp[k], vp[k], squares);
+            }
         }
+        float other;
+        unpair(squares, square, other);
+        square += other;
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+        for (int o = kPer / 2; o > 0; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
     }
     if (kHalf) {
         __shared__ uint32_t block_top;
@@ -991,7 +1025,7 @@ int backward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noe
         if (!bf && cudaMemsetAsync(ws, 0, static_cast<size_t>(p.B) * 8, stream) != cudaSuccess)
             return launch_status("cross_attention_backward");
         const int per = p.D <= 32 ? 64 : p.D <= 64 ? 32 : 16;  // rows of a block
-        const int64_t of_q = (i64(plan.Lq_pad) * p.Hq + per - 1) / per, of_v = bf ? 0 : (i64(p.Lk) * p.Hk + per - 1) / per;
+        const int64_t of_q = (i64(plan.Lq_pad) * p.Hq + per - 1) / per, of_v = bf ? 0 : (i64(p.Lk) * p.Hk + 2 * per - 1) / (2 * per);
         if ((of_q + of_v) * p.B > 0x7fffffff) return WW_ERR_UNSUPPORTED;
         const DeltaParams delta = {const_cast<float*>(f.nlse2), const_cast<float*>(f.ndelta), const_cast<float*>(f.norm2),
                                    reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + plan.seen),
