@@ -101,7 +101,7 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
-// The larger of a and b; NaN if either is (fmaxf drops it).
+// The largest; NaN if one is (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b)
 {
     float r;
@@ -109,20 +109,31 @@ __device__ __forceinline__ float max_nan(float a, float b)
     return r;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // 2^x of two values on the FMA pipe, for x <= 127: x = n + f with n the nearest
 // whole number (read off the low bits after adding 1.5 * 2^23), 2^f on
 // [-1/2, 1/2] by a polynomial of degree 4 fitted to its relative error (2.6e-6,
-// a hundredth of what rounding P to 16 bits costs), times 2^n formed as a float.
-// Below 2^-126.5: 0, so -inf gives 0 as in the exponential unit; NaN and +inf give
-// NaN: the clamp keeps a NaN, inf - inf makes one, and the product carries it
-// (adding n to the exponent field would turn its bits into a finite number).
-// The exponential unit does 16 values per clock and SM against 128 here, so a share
-// of a tile's exponentials is done this way.
+// a hundredth of what rounding P to 16 bits costs), times 2^n.  The exponential unit
+// does 16 values per clock and SM against 128 here, so a share of a tile's
+// exponentials is done this way.
+// SPECIALS: 2^n is a factor, formed as a float.  Below 2^-126.5 the result is 0, so -inf
+// gives 0 as in the exponential unit; NaN and +inf give NaN: the clamp keeps a NaN,
+// inf - inf makes one, the product carries it.
+// Else n is added to the exponent field, an instruction less (8192 to 8192, 8 heads of
+// 128: 335 us and 347): below 2^-126 and for NaN 2^-126, nothing for +inf; for callers
+// that look at their arguments' maximum.
+template <bool SPECIALS>
 __device__ __forceinline__ Pair exp2_poly(Pair x)
 {
     float a, b;
     unpair(x, a, b);
-    x = pair(max_nan(a, -127.0f), max_nan(b, -127.0f));
+    x = SPECIALS ? pair(max_nan(a, -127.0f), max_nan(b, -127.0f)) : pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
     constexpr float kMagic = 12582912.0f;
     const Pair t = add2(x, pair(kMagic, kMagic));
     const Pair n = add2(t, pair(-kMagic, -kMagic));
@@ -132,10 +143,15 @@ __device__ __forceinline__ Pair exp2_poly(Pair x)
     p = fma2(p, f, pair(0.24024744f, 0.24024744f));
     p = fma2(p, f, pair(0.6931218f, 0.6931218f));
     p = fma2(p, f, pair(0.9999993f, 0.9999993f));
-    unpair(t, a, b);
-    // (n + 127) << 23; n = -127 is 0
-    const auto power = [](float v) { return __uint_as_float((__float_as_uint(v) << 23) + 0x3f800000u); };
-    return mul2(p, pair(power(a), power(b)));
+    float ta, tb;
+    unpair(t, ta, tb);
+    const uint32_t na = __float_as_uint(ta) << 23, nb = __float_as_uint(tb) << 23;
+    if constexpr (SPECIALS) {  // (n + 127) << 23; n = -127 is 0
+        return mul2(p, pair(__uint_as_float(na + 0x3f800000u), __uint_as_float(nb + 0x3f800000u)));
+    } else {
+        unpair(p, a, b);
+        return pair(__uint_as_float(__float_as_uint(a) + na), __uint_as_float(__float_as_uint(b) + nb));
+    }
 }
 
 // Relative-position buckets.  Distance d >= exact is in bucket

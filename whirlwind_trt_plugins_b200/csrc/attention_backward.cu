@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(Layout<DP, KEYS>::kThreads, Layout<DP, KEYS>::
                         }
                         float p0, p1;
                         if (!BIAS && j % 8 == 6) {  // a quarter on the FMA pipe
-                            unpair(exp2_poly(arg), p0, p1);
+                            unpair(exp2_poly<true>(arg), p0, p1);
                         } else {
                             unpair(arg, p0, p1);
                             p0 = exp2_approx(p0);

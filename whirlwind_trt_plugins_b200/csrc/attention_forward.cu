@@ -148,7 +148,8 @@ __device__ __forceinline__ float score_pass(uint32_t (&x)[N], float scale2, floa
 
 // P = 2^(mul x + add) of N columns: summed, rounded and put into N / 2 columns of
 // TMEM.  POLY: one pair in kPolyOf on the FMA pipe (whole tiles without a bias
-// of their own).
+// of their own; a NaN or +inf among their scores has made `add` NaN, and -inf gives
+// 2^-126 in place of 0).
 template <typename T, bool POLY, int N>
 __device__ __forceinline__ void exp_pass(const uint32_t (&x)[N], float mul, float add, Pair& sum, uint32_t to)
 {
@@ -159,7 +160,7 @@ __device__ __forceinline__ void exp_pass(const uint32_t (&x)[N], float mul, floa
         const Pair arg = fma2(pair(f32(x[2 * j]), f32(x[2 * j + 1])), mul_2, add_2);
         float a, b;
         if (POLY && j % kPolyOf == kPolyOf - 1) {
-            unpair(exp2_poly(arg), a, b);
+            unpair(exp2_poly<false>(arg), a, b);
         } else {
             unpair(arg, a, b);
             a = exp2_approx(a);
@@ -474,10 +475,10 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                         float top1 = -INFINITY;
 #pragma unroll
                         for (int j = 0; j < N; j += 4) {
-                            top = max3(top, f32(x[j]), f32(x[j + 1]));
-                            top1 = max3(top1, f32(x[j + 2]), f32(x[j + 3]));
+                            top = max3_nan(top, f32(x[j]), f32(x[j + 1]));
+                            top1 = max3_nan(top1, f32(x[j + 2]), f32(x[j + 3]));
                         }
-                        top = fmaxf(top, top1);
+                        top = max_nan(top, top1);
                     } else {
                         float tc;
                         if (mine == nullptr)
@@ -531,9 +532,11 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 pass(largest);
                 if (!plain) umma::tmem_wait_st();
                 if (plain) top = fmaf(top, p.scale2, flat);
-                // grow the maximum: always on the first tile, then only past kRescale
-                if (__any_sync(~0u, kt == 0 || top > m + kRescale)) {
-                    const float mn = fmaxf(m, top);
+                // grow the maximum: always on the first tile, then only past kRescale.  A NaN score (of
+                // raw ones; others keep it to the sum) or one of +inf makes it NaN, and with it the row.
+                if (__any_sync(~0u, kt == 0 || !(top <= m + kRescale))) {
+                    float mn = max_nan(m, top);
+                    if (mn == INFINITY) mn = NAN;
                     if (kt > 0) {  // the product before is done: its commit came before that of these scores
                         const float f = exp2_approx(m == -INFINITY ? -INFINITY : m - mn);
                         l2 = mul2(l2, pair(f, f));
@@ -560,7 +563,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             umma::fence_after_sync();
             float l_even, l_odd;
             unpair(l2, l_even, l_odd);
-            const float sum = l_even + l_odd;
+            float sum = l_even + l_odd;
+            if (m == -INFINITY && sum < 1.0f) sum = 0.0f;  // scores of -inf alone: an empty row
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const int64_t b = batch_of(qi), row = (b * p.Lq + i) * p.Hq + h;
             const int64_t part = (static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (NT * kTile) + t * kTile + r;
