@@ -343,7 +343,8 @@ int64_t ww_qk_norm_rope_backward_workspace(const ww_qk_norm_rope_t* p);
  *   out[b, i, h] = sum_j P v[b, j, h / (Hq / Hk)],   lse[b, h, i] = log sum_j exp S
  * A row without a valid key gives out = 0, lse = -inf and no gradient.  What
  * masked places of k and v hold does not matter (NaN included); their
- * gradients are 0.  P is rounded to the inputs' 16-bit type before the second
+ * gradients are 0.  In valid places a NaN or +inf score makes its row's out
+ * and lse NaN, one of -inf is a weight of 0.  P is rounded to the inputs' 16-bit type before the second
  * product (as are P and dS in the backward pass); sums are fp32.
  * bucket(r): with n = num_buckets (half of them, the upper half for r > 0, if
  * bidirectional), d = |r| (max(0, -r) if not), e = n / 2: d below e is its own

@@ -31,14 +31,16 @@
 //
 // Bound: per 128 x 64 tile 512 clocks of exponentials (16 per clock and SM) in
 // each kernel against 8 D (dK, dV) and 6 D (dQ) clocks of products.
-// Measured: a map of 4800, 8 heads of 128, bf16 with a bias: 308 us for the
-// gradients, 770 TFLOP/s of the five products (seven are formed); 1200 to 1777
-// tokens, 4 x 16 heads of 64 on 4: 93 us; 1080 heads of 32 in rows of 320, masked,
-// with a bias: 280 us, where a CTA of five tiles spends 4000 of its 17000 clocks
-// (5800 of 21600 over queries) before its first tile.
+// Measured: a map of 4800, 8 heads of 128, bf16 with a bias: 340 us for the
+// gradients, 690 TFLOP/s of the five products (seven are formed; 311 us in short
+// runs); 1200 to 1777 tokens, 4 x 16 heads of 64 on 4: 100 us; 1080 heads of 32 in
+// rows of 320, fp16, masked, with a bias: 296 us, of them 20 for deltas and norms; a
+// CTA of five tiles spends 4000 of its 17000 clocks (5800 of 21600 over queries) before
+// its first tile.
 // The two kernels do not need each other: `queries` is launched behind `keys` and
 // takes the SMs that its last round leaves (rows of 320, forward and gradients:
-// 16 us less than one after the other), then one join for both.
+// 16 us less than one after the other; the order that it then needs by hand, see `seen`,
+// takes 4 of them), then one join for both.
 //
 // dtable: a tile whose positions all lie in one bucket adds its plain sum.
 // Otherwise dS goes through shared memory in fp32, 32 columns at a time (rounded as

@@ -32,9 +32,10 @@
 //   NT = 2  two CTAs of two query tiles against the same keys: half the reads of
 //           K and V from L2, for long rows (make_plan has both sides)
 //
-// Measured, fp16: 19200 queries to 19200 keys, 5 heads of 64: 600 us, 790 TFLOP/s,
-// 3.1e12 exponentials a second (16 per clock: 4.5e12); 8192 to 8192, 8 heads of
-// 128: 297 us, 930 TFLOP/s; 12032 heads of 32 in rows of 312, 5 % of the keys
+// Measured, fp16: 19200 queries to 19200 keys, 5 heads of 64: 665 us in long runs, where
+// the power cap lowers the clock, 710 TFLOP/s, 2.8e12 exponentials a second (16 per
+// clock: 4.5e12), 605 us in short ones; 8192 to 8192, 8 heads of 128: 320 us, 860
+// TFLOP/s, 305 in short runs; 12032 heads of 32 in rows of 312, 5 % of the keys
 // masked, with a bias: 753 us, a third of the exponentials' rate -- a tile's four
 // warps take 1000 to 1500 clocks for each of the two passes over its scores, and
 // five tiles to a row leave the start (tables, first loads) in sight.
