@@ -253,8 +253,9 @@ __device__ __forceinline__ bool mbar_try_wait_hint(uint32_t saddr, uint32_t pari
 }
 
 // Bounded wait for the phase with the given parity to complete: at most
-// kWaitRounds suspended polls of <= 1 ms each (seconds in total, orders of
-// magnitude above any legitimate wait in these kernels).
+// kWaitRounds suspended polls.  The hint is an upper limit; measured, a poll that
+// nothing ends holds the thread for 4 us, 16 ms in total, orders of magnitude above
+// any legitimate wait in these kernels.
 constexpr uint32_t kWaitRounds = 4000;
 constexpr uint32_t kSpinPolls = 4;   // non-blocking polls before suspending (64 polling warps slowed config 3 by 8 %)
 __device__ __forceinline__ bool mbar_wait(uint32_t saddr, uint32_t parity)
