@@ -386,6 +386,125 @@ int64_t ww_cross_attention_backward_workspace(const ww_attention_t* p);
  * that the operators reject (host only). */
 int ww_relative_position_bucket(int rel, int num_buckets, int max_distance, int bidirectional);
 
+/* ---------------------------------------------------------------------------
+ * Operators of a matching layer around the attention, in part in 8 bits
+ * (extensions; the formulas are their specification).
+ *
+ * A row in 8 bits: a = max |x|, scale = a / 127, q = rint(x * (127 / a)), ties
+ * to even, the quotients in fp32, the product exact; so q is in [-127, 127].  A row with a NaN or an
+ * infinity has scale NaN (what is computed from it is NaN), one with a < 2^-119
+ * scale 0 and zeros.
+ * fp32 arithmetic, one rounding to a result's type; the same call gives the
+ * same bits again.  Outputs do not overlap inputs.
+ * ------------------------------------------------------------------------- */
+
+/* Layer norm of rows of N values (x and residual: any stride between rows).
+ *   h = x + residual, rounded to its type;  m = mean h;  v = mean (h - m)^2
+ *   y = (h - m) / sqrt(v + eps) * weight + bias
+ * Either y or, in 8 bits, y_q and y_scale is written; sum gets h, mean and rstd
+ * what the backward pass needs.  weight (and with it bias), residual, sum, mean
+ * and rstd may be NULL.
+ * Backward: x is the normalised input (the sum, where there was a residual):
+ *   g = dy * weight;  dx = rstd (g - mean g - xh mean(g xh)) + dsum
+ *   dweight = sum over rows of dy xh;  dbias = sum of dy       (both or neither)
+ * with dsum (or NULL) the gradient that reaches the sum itself; dweight and dbias
+ * need workspace_bytes of scratch memory.  No rows: their gradients are 0. */
+typedef struct ww_layer_norm {
+    const void* x; /* [rows, N] */
+    const void* residual;
+    const void* weight; /* [N], the type of x */
+    const void* bias;
+    void* y;        /* [rows, N] contiguous */
+    void* sum;      /* [rows, N] contiguous */
+    int8_t* y_q;    /* [rows, N] */
+    float* y_scale; /* [rows] */
+    float* mean;    /* [rows] */
+    float* rstd;
+    const void* dy; /* backward */
+    const void* dsum;
+    void* dx; /* contiguous */
+    void* dweight;
+    void* dbias;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t x_stride, residual_stride, y_q_stride, dy_stride, dsum_stride; /* elements between rows */
+    int32_t dtype, rows, N; /* WW_DTYPE_HALF, WW_DTYPE_BF16 or WW_DTYPE_FLOAT */
+    float eps;
+} ww_layer_norm_t;
+
+int ww_layer_norm(const ww_layer_norm_t* p, void* stream);
+int ww_layer_norm_backward(const ww_layer_norm_t* p, void* stream);
+int64_t ww_layer_norm_backward_workspace(const ww_layer_norm_t* p);
+/* The 8-bit form of the rows of x: y_q and y_scale. */
+int ww_quantize_tokens(const ww_layer_norm_t* p, void* stream);
+
+/* Product in 8-bit integers with a scale for each token and channel:
+ *   out[m, n] = (x_scale[m] * sum_k x_q[m, k] w_q[n, k]) * w_scale[n] + bias[n]
+ * the sums exact in 32 bits.  Either x_q and x_scale are given or x, activations of
+ * the output's type that are brought to 8 bits first, row by row.
+ * x_q and w_q start on 16 bytes, their rows are a multiple of 16 bytes apart; what
+ * stands between a row's K values and the next row does not matter.  K < 2^17. */
+typedef struct ww_int8_matmul {
+    const void* x;        /* [M, K] of dtype, or NULL */
+    const int8_t* x_q;    /* [M, K], or NULL */
+    const float* x_scale; /* [M], with x_q */
+    const int8_t* w_q;    /* [N, K] */
+    const float* w_scale; /* [N] */
+    const void* bias;     /* [N] of dtype, or NULL */
+    void* out;            /* [M, N] of dtype, contiguous */
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t x_stride, x_q_stride, w_stride; /* elements between rows */
+    int32_t dtype, M, K, N;                 /* WW_DTYPE_HALF, WW_DTYPE_BF16 or WW_DTYPE_FLOAT */
+} ww_int8_matmul_t;
+
+int ww_int8_matmul(const ww_int8_matmul_t* p, void* stream);
+int64_t ww_int8_matmul_workspace(const ww_int8_matmul_t* p);
+
+/* Keys and values kept in 8 bits, a row (token, head) at a time:
+ *   k_cache, v_cache [B, places, H, D] int8, strides like those of vectors;
+ *   k_scale, v_scale [B, H, places] fp32, unit stride along the places.
+ * ww_quantize_kv writes token l < lens[b] (all L without lens) of item b of k and v
+ * [B, L, H, D] to place start[b] + l (start: 0 without); tokens whose place lies
+ * outside [0, places) are skipped, other places stay as they are.
+ * ww_dequantize_kv reads places p < lens[b] (all without lens) back: k_out, v_out
+ * [B, places, H, D] contiguous = q * scale, zeros behind the lens.
+ * D a multiple of 16, up to 128. */
+typedef struct ww_kv_cache {
+    const void* k; /* [B, L, H, D] of dtype, strides of whole 16 bytes */
+    const void* v;
+    int8_t* k_cache;
+    int8_t* v_cache;
+    float* k_scale;
+    float* v_scale;
+    const int32_t* start; /* [B] or NULL */
+    const int32_t* lens;  /* [B] or NULL */
+    void* k_out;
+    void* v_out;
+    int64_t k_strides[3], v_strides[3], k_cache_strides[3], v_cache_strides[3]; /* {b, l, h} */
+    int64_t k_scale_strides[2], v_scale_strides[2];                             /* {b, h} */
+    int32_t dtype, B, L, places, H, D; /* WW_DTYPE_HALF or WW_DTYPE_BF16 */
+} ww_kv_cache_t;
+
+int ww_quantize_kv(const ww_kv_cache_t* p, void* stream);
+int ww_dequantize_kv(const ww_kv_cache_t* p, void* stream);
+
+/* ww_cross_attention with keys and values in 8 bits: k and v of `attention` are the
+ * int8 caches [B, Lk, Hk, D], with k_scale and v_scale.  Scales of masked places
+ * do not matter either; those of valid places are >= 0 or NaN.  Up to 128 rows (query heads of
+ * a key head x tokens) the values are used as they stand, P in fp16 with the values'
+ * scales in it; beyond, keys and values are rounded to q's type in the workspace.
+ * No gradients.  D a multiple of 16. */
+typedef struct ww_attention_int8 {
+    ww_attention_t attention;
+    const float* k_scale; /* [B, Hk, Lk], unit stride along Lk */
+    const float* v_scale;
+    int64_t k_scale_strides[2], v_scale_strides[2]; /* {b, h} */
+} ww_attention_int8_t;
+
+int ww_cross_attention_int8(const ww_attention_int8_t* p, void* stream);
+int64_t ww_cross_attention_int8_workspace(const ww_attention_int8_t* p);
+
 /* BatchNorm folding on the host: w16[o, :] = fp16(w[o, :] * scale[o]) computed in
  * fp32, b16[o] = fp16(bias[o]); k = Cin * 27.  Host memory only. */
 int ww_fold_bn_f16(const float* w, const float* scale, const float* bias, int cout, int k,

@@ -27,6 +27,10 @@ reference project):
 * ``qk_norm_rope(...)``, ``cross_attention(...)`` and their gradients -- attention
   of a matching network on the features (``whirlwind_trt_plugins_b200.attention``;
   no reference counterpart)
+* ``layer_norm(...)`` and its gradient, ``int8_linear(...)``, ``quantize_kv(...)``,
+  ``cross_attention_int8(...)`` and what belongs to them -- norm, projections and
+  attention of such a network in 8 bits (``whirlwind_trt_plugins_b200.layers``; no
+  reference counterpart)
 
 The plugin-level classes mirroring the reference's IPluginV3 plugins live in
 ``whirlwind_trt_plugins_b200.plugins``; row-band sharding over several GPUs in
@@ -44,7 +48,9 @@ __all__ = [
     "MULTI_BATCH", "MULTI_ROWS", "multi_split", "corr_cost_stem3d_multi", "CORR_ENGINE_TENSOR",
     "CORR_ENGINE_CUDA_CORES", "set_fused_corr_engine", "fused_corr_engine", "DTYPE_BF16", "qk_norm_rope",
     "qk_norm_rope_backward", "cross_attention", "cross_attention_backward", "qk_norm_rope_autograd",
-    "cross_attention_autograd", "relative_position_bucket",
+    "cross_attention_autograd", "relative_position_bucket", "layer_norm", "layer_norm_backward", "layer_norm_autograd",
+    "layer_norm_int8", "quantize_tokens", "int8_matmul", "int8_linear", "quantize_kv", "dequantize_kv",
+    "cross_attention_int8",
 ]
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libww_trt_plugins.so")
@@ -443,3 +449,5 @@ def clear_device_error() -> None:
 
 from .attention import (DTYPE_BF16, cross_attention, cross_attention_autograd, cross_attention_backward,  # noqa: E402
                         qk_norm_rope, qk_norm_rope_autograd, qk_norm_rope_backward, relative_position_bucket)
+from .layers import (cross_attention_int8, dequantize_kv, int8_linear, int8_matmul, layer_norm,  # noqa: E402
+                     layer_norm_autograd, layer_norm_backward, layer_norm_int8, quantize_kv, quantize_tokens)

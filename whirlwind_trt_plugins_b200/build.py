@@ -42,6 +42,10 @@ SOURCES = [
     "attention_forward.cu",
     "attention_token.cu",
     "attention_backward.cu",
+    "attention_int8.cu",
+    "kv_cache.cu",
+    "layer_norm.cu",
+    "int8_matmul.cu",
     "multi.cu",
     "plugin_core.cpp",
 ]

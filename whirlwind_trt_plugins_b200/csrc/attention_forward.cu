@@ -848,6 +848,19 @@ int sm_count() noexcept
 }
 
 }  // namespace
+
+int attention_join_launch(const ww_attention_t& p, int items, int splits, int rows, const float* part_o, const float* part_lse,
+                          const char* name, cudaStream_t stream) noexcept
+{
+    const auto go = [&](auto kernel) {
+        launch_behind(kernel, dim3(items, (rows + 3) / 4), dim3(128), 0, stream, part_o, part_lse, p.out, p.lse, 0, splits, rows, 0,
+                      p.Lq, p.Hq, p.Hk, p.D);
+    };
+    if (p.dtype == WW_DTYPE_HALF) go(attention_join_kernel<__half>);
+    else go(attention_join_kernel<__nv_bfloat16>);
+    return launch_status(name);
+}
+
 }  // namespace ww
 
 extern "C" {

@@ -19,4 +19,9 @@ int token_splits(const ww_attention_t& p, int sms) noexcept;
 int attention_token_launch(const ww_attention_t& p, int splits, float* part_o, float* part_lse,
                            cudaStream_t stream) noexcept;
 
+// Joins such parts into out and lse; launched behind the kernel that writes them
+// (attention_forward.cu).
+int attention_join_launch(const ww_attention_t& p, int items, int splits, int rows, const float* part_o, const float* part_lse,
+                          const char* name, cudaStream_t stream) noexcept;
+
 }  // namespace ww

@@ -1,0 +1,685 @@
+// int8_matmul.cu -- products in 8-bit integers with a scale for each token and
+// each channel, and the 8-bit form of 16- or 32-bit activations in front of them.
+//
+//   out[m, n] = xs[m] ws[n] sum_k xq[m, k] wq[n, k] + bias[n]
+//
+// The sums are whole numbers in 32 bits, exact (K < 2^17), so that neither tiles nor
+// shares of K change a result; (sum xs) ws + bias in fp32, one rounding to the output's type.
+//
+// Tiles: tcgen05 kind::i8, accumulators in TMEM, operands by TMA in swizzled rows
+// of 128 bytes.  One producer warp, one warp that issues, eight that write out: each
+// takes 32 rows and half the columns of a tile, from TMEM through shared memory to a TMA
+// store, while the next tile's products run into the other half of TMEM.
+// Blocks are persistent; tiles go in bands of rows so that operands are read from L2.
+// Large products take two SMs for a 256 x 256 tile (cta_group::2): each holds half
+// the rows and half the channels and reads each operand once.
+// Few tokens: the weights' bytes are the bound.  A block takes 16 channels, its warps
+// shares of K; each lane loads 16 bytes of a row, which are its fragments of two
+// mma.sync m16n8k32 (k is summed, so any order of it serves that both operands
+// share), and all of a warp's loads are under way before the tokens have been
+// brought to 8 bits in shared memory.
+#include "rows.cuh"
+#include "tensor_map.cuh"
+#include "umma.cuh"
+
+#include <algorithm>
+
+namespace ww {
+
+int quantise_rows(const ww_layer_norm_t& p, const char* name, void* stream) noexcept;  // layer_norm.cu
+
+namespace {
+
+constexpr int kBlockK = 128;  // bytes of a row of a stage
+constexpr int kTileM = 128;   // rows of an SM's tile
+constexpr int kThreads = 384;
+constexpr int kEpilogueWarps = 8;
+
+struct MatmulParams {
+    CUtensorMap a, b, c;
+    const float *xs, *ws;
+    const void* bias;
+    void* out;
+    int32_t M, N, k_blocks;
+    int32_t m_tiles, n_tiles, band;
+    int32_t behind;  // the operands are written by the launch before
+    int32_t stored;  // the output is stored by TMA
+    int* err;
+};
+
+template <int BN, bool PAIR, typename O>
+struct Tiles {
+    static constexpr int kA = kTileM * kBlockK;
+    static constexpr int kB = (PAIR ? BN / 2 : BN) * kBlockK;
+    static constexpr int kStage = kA + kB;
+    static constexpr int kStages = 5;
+    static constexpr int kColumns = BN / 2;  // of an epilogue warp
+    static constexpr int kChunk = kColumns < 128 / static_cast<int>(sizeof(O)) ? kColumns : 128 / static_cast<int>(sizeof(O));
+    static constexpr int kChunkRow = kChunk * static_cast<int>(sizeof(O));  // 64 or 128 bytes
+    static constexpr int kStaging = 32 * kChunkRow;
+    static constexpr int kOut = kStages * kStage;
+    static constexpr int kScales = kOut + kEpilogueWarps * kStaging;
+    static constexpr int kBar = kScales + kEpilogueWarps * kColumns * 8;
+    static constexpr int kBytes = kBar + (2 * kStages + 4) * 8 + 16 + 1024;
+    static constexpr int kTmem = 2 * BN;
+    static_assert(kBytes <= kMaxShared, "shared memory");
+    static_assert(kChunkRow == 64 || kChunkRow == 128, "rows of a swizzle");
+};
+
+// ---- instructions of a pair of SMs ----
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// Address of `saddr` in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t saddr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" : : : "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" : : "r"(bar) : "memory");
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void load_tile(uint32_t dst, const void* map, int x, int y, uint32_t bar)
+{
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                     "[%0], [%1, {%2, %3}], [%4];\n"
+                     : : "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                     "[%0], [%1, {%2, %3}], [%4];\n"
+                     : : "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void store_tile(const void* map, uint32_t src, int x, int y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+                 : : "l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+    asm volatile("cp.async.bulk.commit_group;\n" : : : "memory");
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+                     : : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+                     : : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+// Arrive on the barrier (of both SMs) when the products issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+                     : : "r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+    else
+        umma::mma_commit(bar);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tmem_get(uint32_t to, uint32_t columns)
+{
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" : : "r"(to), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" : : : "memory");
+    } else {
+        umma::tmem_alloc(to, columns);
+    }
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns)
+{
+    if constexpr (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" : : "r"(at), "r"(columns) : "memory");
+    else
+        umma::tmem_dealloc(at, columns);
+}
+
+// Bounded wait of a warp, the same answer in every lane.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity)
+{
+    return __all_sync(~0u, umma::mbar_poll(bar, parity));
+}
+
+// Instruction descriptor of kind::i8: signed operands, K-major both, 32-bit sums.
+__host__ __device__ constexpr uint32_t idesc_i8(int M, int N)
+{
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// Tile t: bands of `band` tiles of rows, the rows of a band first.
+__device__ __forceinline__ void tile_at(const MatmulParams& p, int t, int& m, int& n)
+{
+    const int whole = p.band * p.n_tiles, first = t / whole * p.band, rows = min(p.band, p.m_tiles - first);
+    t %= whole;
+    m = first + t % rows;
+    n = t / rows;
+}
+
+template <typename O>
+__device__ __forceinline__ void pack_row(const Pair (&v)[4], uint32_t to0, uint32_t to1)
+{
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpair(v[i], f[2 * i], f[2 * i + 1]);
+    if constexpr (sizeof(O) == 4) {
+        umma::st_shared_v4(to0, __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        umma::st_shared_v4(to1, __float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+    } else {
+        umma::st_shared_v4(to0, pack2<O>(f[0], f[1]), pack2<O>(f[2], f[3]), pack2<O>(f[4], f[5]), pack2<O>(f[6], f[7]));
+    }
+}
+
+template <int BN, bool PAIR, typename O>
+__global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_constant__ MatmulParams p)
+{
+    using L = Tiles<BN, PAIR, O>;
+    constexpr int S = L::kStages;
+    extern __shared__ uint8_t raw[];
+    uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
+    const uint32_t sm = umma::smem_addr(base);
+    const uint32_t full = sm + L::kBar, empty = full + S * 8, done = empty + S * 8, freed = done + 16, slot = freed + 16;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            umma::mbar_init(full + s * 8, 1);
+            umma::mbar_init(empty + s * 8, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            umma::mbar_init(done + i * 8, 1);
+            umma::mbar_init(freed + i * 8, kEpilogueWarps * (PAIR ? 2 : 1));
+        }
+        umma::mbar_fence_init();
+        umma::tma_prefetch_desc(&p.a);
+        umma::tma_prefetch_desc(&p.b);
+    }
+    if (warp == 2) tmem_get<PAIR>(slot, L::kTmem);
+    umma::fence_before_sync();
+    __syncthreads();
+    if (PAIR) cluster_sync();
+    umma::fence_after_sync();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot) : "memory");
+    if (p.behind) wait_for_launches_before();
+    const int tiles = p.m_tiles * p.n_tiles, step = PAIR ? gridDim.x / 2 : gridDim.x, start = PAIR ? blockIdx.x / 2 : blockIdx.x;
+    bool ok = true;
+
+    if (warp == 0) {  // loads
+        const bool leader = umma::elect_one();
+        int s = 0;
+        uint32_t parity = 1;
+        for (int t = start; t < tiles && ok; t += step) {
+            int m, n;
+            tile_at(p, t, m, n);
+            const int row = (m * (PAIR ? 2 : 1) + static_cast<int>(rank)) * kTileM, channel = n * BN + static_cast<int>(rank) * (BN / 2);
+            for (int k = 0; k < p.k_blocks && ok; ++k) {
+                ok = wait(empty + s * 8, parity);
+                if (ok && leader) {
+                    const uint32_t to = sm + s * L::kStage;
+                    const uint32_t bar = PAIR ? in_block(full + s * 8, 0) : full + s * 8;
+                    if (rank == 0) umma::mbar_arrive_expect_tx(full + s * 8, L::kStage * (PAIR ? 2 : 1));
+                    load_tile<PAIR>(to, &p.a, k * kBlockK, row, bar);
+                    load_tile<PAIR>(to + L::kA, &p.b, k * kBlockK, channel, bar);
+                }
+                __syncwarp();
+                if (++s == S) {
+                    s = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1 && rank == 0) {  // products
+        constexpr uint32_t idesc = idesc_i8(PAIR ? 2 * kTileM : kTileM, BN);
+        const bool leader = umma::elect_one();
+        const uint64_t a0 = umma::smem_desc_swizzled<128>(sm, 1024), b0 = umma::smem_desc_swizzled<128>(sm + L::kA, 1024);
+        int s = 0, i = 0;
+        uint32_t parity = 0;
+        for (int t = start; t < tiles && ok; t += step, ++i) {
+            ok = wait(freed + (i & 1) * 8, ((i >> 1) & 1) ^ 1);
+            umma::fence_after_sync();
+            const uint32_t d = tmem + (i & 1) * BN;
+            for (int k = 0; k < p.k_blocks && ok; ++k) {
+                ok = wait(full + s * 8, parity);
+                umma::fence_after_sync();
+                if (ok && leader) {
+                    const uint64_t a = umma::desc_advance(a0, s * L::kStage), b = umma::desc_advance(b0, s * L::kStage);
+#pragma unroll
+                    for (int j = 0; j < kBlockK / 32; ++j)
+                        mma_i8<PAIR>(d, umma::desc_advance(a, j * 32), umma::desc_advance(b, j * 32), idesc, k > 0 || j > 0);
+                    commit<PAIR>(empty + s * 8);
+                    if (k == p.k_blocks - 1) commit<PAIR>(done + (i & 1) * 8);
+                }
+                __syncwarp();
+                if (++s == S) {
+                    s = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+    } else if (warp >= 4) {  // results
+        const int quarter = warp % 4, half = warp / 4 - 1, w = warp - 4;
+        const uint32_t staging = sm + L::kOut + w * L::kStaging;
+        const uint32_t bar = PAIR ? in_block(freed, 0) : freed;
+        float* scales = reinterpret_cast<float*>(base + L::kScales) + w * 2 * L::kColumns;  // [columns] of ws, of the bias
+        int i = 0;
+        for (int t = start; t < tiles && ok; t += step, ++i) {
+            int m, n;
+            tile_at(p, t, m, n);
+            const int row0 = (m * (PAIR ? 2 : 1) + static_cast<int>(rank)) * kTileM + quarter * 32, column0 = n * BN + half * L::kColumns;
+            __syncwarp();  // the scales before have been read
+            for (int c = lane; c < L::kColumns; c += 32) {
+                const bool in = column0 + c < p.N;
+                scales[c] = in ? __ldg(p.ws + column0 + c) : 0.0f;
+                scales[L::kColumns + c] = in && p.bias != nullptr ? to_float(static_cast<const O*>(p.bias)[column0 + c]) : 0.0f;
+            }
+            const float xs = row0 + lane < p.M ? __ldg(p.xs + row0 + lane) : 0.0f;
+            const Pair x2 = pair(xs, xs);
+            __syncwarp();
+            ok = wait(done + (i & 1) * 8, (i >> 1) & 1);
+            umma::fence_after_sync();
+            if (!ok) break;
+            const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * BN + half * L::kColumns;
+#pragma unroll 1
+            for (int c = 0; c < L::kColumns; c += L::kChunk) {
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" : : : "memory");
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < L::kChunk; e += 32) {
+                    uint32_t v[32];
+                    umma::tmem_ld32(from + c + e, v);
+                    umma::tmem_wait_ld32(v);
+                    if (c + e + 32 == L::kColumns) {  // TMEM has been read
+                        umma::fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (PAIR) arrive_cluster(bar + (i & 1) * 8);
+                            else umma::mbar_arrive(bar + (i & 1) * 8);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        Pair f[4];
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            const float4 sw = *reinterpret_cast<const float4*>(scales + c + e + j + 4 * z);
+                            const float4 sb = *reinterpret_cast<const float4*>(scales + L::kColumns + c + e + j + 4 * z);
+                            const uint32_t* q = v + j + 4 * z;
+                            f[2 * z] = fma2(mul2(pair(__int2float_rn(q[0]), __int2float_rn(q[1])), x2), pair(sw.x, sw.y), pair(sb.x, sb.y));
+                            f[2 * z + 1] = fma2(mul2(pair(__int2float_rn(q[2]), __int2float_rn(q[3])), x2), pair(sw.z, sw.w), pair(sb.z, sb.w));
+                        }
+                        // 16-byte piece of the row, swizzled as the TMA store reads it
+                        const int piece = (e + j) * static_cast<int>(sizeof(O)) / 16;
+                        const int turn = L::kChunkRow == 128 ? lane & 7 : (lane >> 1) & 3;
+                        const uint32_t at = staging + lane * L::kChunkRow;
+                        pack_row<O>(f, at + ((piece ^ turn) << 4), at + (((piece + 1) ^ turn) << 4));
+                    }
+                }
+                const int x = column0 + c;
+                if (p.stored) {
+                    umma::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && x < p.N && row0 < p.M) store_tile(&p.c, staging, x, row0);
+                } else {  // rows that do not start on 16 bytes
+                    __syncwarp();
+                    for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+                        const int turn = L::kChunkRow == 128 ? r & 7 : (r >> 1) & 3;
+                        for (int e = lane; e < L::kChunk && x + e < p.N; e += 32) {
+                            const int byte = e * static_cast<int>(sizeof(O));
+                            const uint8_t* v = base + L::kOut + w * L::kStaging + r * L::kChunkRow + (((byte >> 4) ^ turn) << 4) + (byte & 15);
+                            static_cast<O*>(p.out)[static_cast<int64_t>(row0 + r) * p.N + x + e] = *reinterpret_cast<const O*>(v);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" : : : "memory");
+    }
+    if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x50);
+    umma::fence_before_sync();
+    __syncthreads();
+    if (PAIR) cluster_sync();  // until neither SM's barriers or TMEM are used by the other
+    umma::fence_after_sync();
+    if (warp == 2) tmem_free<PAIR>(tmem, L::kTmem);
+}
+
+// ---- few tokens ----
+
+constexpr int kFewTokens = 16;
+constexpr int kFewChannels = 16;
+constexpr int kFewWarps = 8;
+constexpr int kFewShared = 96 * 1024;  // bytes of the tokens in 8 bits
+
+struct FewParams {
+    const void* x;  // activations, or
+    const int8_t* xq;
+    const float *xs, *ws;
+    const int8_t* wq;
+    const void* bias;
+    void* out;
+    int64_t x_stride, xq_stride, w_stride;
+    int32_t M, K, N, pitch;  // pitch: bytes between the tokens in shared memory
+    int32_t x_pieces;        // x can be read 16 bytes at a time
+};
+
+// 16 bytes of a row at k; what lies beyond K is 0.
+__device__ __forceinline__ uint4 load_row(const int8_t* row, int k, int K)
+{
+    if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    uint32_t u[4] = {0, 0, 0, 0};
+    for (int j = 0; k + j < K; ++j) u[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + j])) << (j % 4 * 8);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+__device__ __forceinline__ void mma_i8_warp(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename O, int NT>  // NT: groups of 8 tokens
+__global__ void __launch_bounds__(kFewWarps * 32) int8_few_kernel(const __grid_constant__ FewParams p)
+{
+    constexpr int kAhead = 4;  // steps of 64 bytes of K under way
+    extern __shared__ __align__(16) uint8_t tokens[];  // [M][pitch], then
+    auto part = reinterpret_cast<int(*)[NT * 8][kFewChannels + 1]>(tokens + p.M * p.pitch);  // [warps], the shares' sums
+    float* scale = reinterpret_cast<float*>(part + kFewWarps);
+    uint32_t* top = reinterpret_cast<uint32_t*>(scale + kFewTokens);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const int n0 = blockIdx.x * kFewChannels;
+    const int steps = (p.K + 63) / 64, share = (steps + kFewWarps - 1) / kFewWarps;
+    const int first = min(warp * share, steps), last = min(first + share, steps);
+    const int8_t* lo = p.wq + min(n0 + g, p.N - 1) * p.w_stride;
+    const int8_t* hi = p.wq + min(n0 + g + 8, p.N - 1) * p.w_stride;
+    uint4 wl[kAhead], wh[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (first + i < last) {
+            wl[i] = load_row(lo, (first + i) * 64 + t * 16, p.K);
+            wh[i] = load_row(hi, (first + i) * 64 + t * 16, p.K);
+        }
+    const int end = steps * 64;
+    if (p.x != nullptr) {
+        // the tokens in 8 bits: each token's largest magnitude (its bits order like the
+        // values, NaN above all), then its whole numbers, from L1 again
+        constexpr int V = 16 / static_cast<int>(sizeof(O));
+        if (threadIdx.x < kFewTokens) top[threadIdx.x] = 0;
+        __syncthreads();
+        for (int m = 0; m < p.M; ++m) {
+            const O* x = static_cast<const O*>(p.x) + m * p.x_stride;
+            float a = 0.0f;
+            if (p.x_pieces) {
+                for (int k = threadIdx.x * V; k < p.K; k += kFewWarps * 32 * V) {
+                    Piece<O, V> r[1];
+                    Pair f[V / 2];
+                    r[0].load(x + k);
+                    values_of<O, V, 1>(r, f);
+                    a = max_nan(a, largest(f));
+                }
+            } else {
+#pragma unroll 8
+                for (int k = threadIdx.x; k < p.K; k += kFewWarps * 32) a = max_nan(a, fabsf(to_float(x[k])));
+            }
+            const uint32_t u = __reduce_max_sync(~0u, __float_as_uint(a) & 0x7fffffffu);
+            if (lane == 0) atomicMax(top + m, u);
+        }
+        __syncthreads();
+        for (int m = 0; m < p.M; ++m) {
+            const O* x = static_cast<const O*>(p.x) + m * p.x_stride;
+            int8_t* to = reinterpret_cast<int8_t*>(tokens) + m * p.pitch;
+            const RowScale r = row_scale(__uint_as_float(top[m]));
+            if (threadIdx.x == 0) scale[m] = r.scale;
+            if (p.x_pieces) {
+                for (int k = threadIdx.x * V; k < end; k += kFewWarps * 32 * V) {
+                    Piece<O, V> v[1];
+                    Pair f[V / 2];
+                    if (k < p.K) v[0].load(x + k);
+                    else v[0].clear();
+                    values_of<O, V, 1>(v, f);
+                    store_piece_int8<V>(to + k, f, r.inv, 0);
+                }
+            } else {
+#pragma unroll 8
+                for (int k = threadIdx.x; k < end; k += kFewWarps * 32)
+                    to[k] = k < p.K ? quantise(to_float(x[k]), r.inv) : 0;
+            }
+        }
+    } else {
+        for (int e = threadIdx.x; e < p.M * (end / 16); e += kFewWarps * 32) {
+            const int m = e / (end / 16), k = e % (end / 16) * 16;
+            *reinterpret_cast<uint4*>(tokens + m * p.pitch + k) = load_row(p.xq + m * p.xq_stride, k, p.K);
+        }
+        if (threadIdx.x < p.M) scale[threadIdx.x] = __ldg(p.xs + threadIdx.x);
+    }
+    __syncthreads();
+    int d[NT][4] = {};
+    for (int i0 = first; i0 < last; i0 += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i >= last) break;
+            const uint4 a = wl[i], b = wh[i];
+            if (i0 + i + kAhead < last) {
+                wl[i] = load_row(lo, (i0 + i + kAhead) * 64 + t * 16, p.K);
+                wh[i] = load_row(hi, (i0 + i + kAhead) * 64 + t * 16, p.K);
+            }
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (c * 8 + g < p.M) x = *reinterpret_cast<const uint4*>(tokens + (c * 8 + g) * p.pitch + (i0 + i) * 64 + t * 16);
+                mma_i8_warp(d[c], a.x, b.x, a.y, b.y, x.x, x.y);
+                mma_i8_warp(d[c], a.z, b.z, a.w, b.w, x.z, x.w);
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[warp][c * 8 + 2 * t + e % 2][g + e / 2 * 8] = d[c][e];
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.M * kFewChannels; e += kFewWarps * 32) {
+        const int m = e / kFewChannels, c = e % kFewChannels;
+        if (n0 + c >= p.N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) sum += part[w][m][c];
+        const float b = p.bias == nullptr ? 0.0f : to_float(static_cast<const O*>(p.bias)[n0 + c]);
+        static_cast<O*>(p.out)[static_cast<int64_t>(m) * p.N + n0 + c] = from_float<O>(fmaf(__int2float_rn(sum) * scale[m], __ldg(p.ws + n0 + c), b));
+    }
+}
+
+// ---- host ----
+
+int pitch_of(int k) noexcept { return (k + 15) / 16 * 16; }
+
+// Shared memory behind the tokens.
+int few_rest(int tokens) noexcept { return kFewWarps * tokens * (kFewChannels + 1) * 4 + kFewTokens * 8; }
+
+// Bytes between tokens in shared memory: half a line of banks apart from line to line.
+int few_pitch(int k) noexcept
+{
+    const int n = (k + 63) / 64 * 64;
+    return n % 128 == 64 ? n : n + 64;
+}
+
+bool few_form(const ww_int8_matmul_t& p) noexcept { return p.M <= kFewTokens && i64(p.M) * few_pitch(p.K) <= kFewShared; }
+
+template <int BN, bool PAIR, typename O>
+int launch_tiles(MatmulParams& f, int tiles, int sms, cudaStream_t stream) noexcept
+{
+    using L = Tiles<BN, PAIR, O>;
+    const auto kernel = int8_matmul_kernel<BN, PAIR, O>;
+    static std::atomic<uint64_t> raised{0};
+    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("int8_matmul");
+    cudaLaunchAttribute attr[2]{};
+    cudaLaunchConfig_t cfg{};
+    if (f.behind) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (PAIR) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = 2;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    cfg.gridDim = PAIR ? 2 * std::min(tiles, sms / 2) : std::min(tiles, sms);
+    cfg.blockDim = kThreads;
+    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cudaLaunchKernelEx(&cfg, kernel, f);
+    return launch_status("int8_matmul");
+}
+
+template <int BN, bool PAIR, typename O>
+int run_tiles(const ww_int8_matmul_t& p, const int8_t* xq, const float* xs, int64_t xq_stride, bool behind, int sms, int* err,
+              cudaStream_t stream) noexcept
+{
+    using L = Tiles<BN, PAIR, O>;
+    MatmulParams f;
+    if (!encode_rows_map(&f.a, WW_DTYPE_INT8, xq, p.M, p.K, xq_stride, kBlockK, kTileM) ||
+        !encode_rows_map(&f.b, WW_DTYPE_INT8, p.w_q, p.N, p.K, p.w_stride, kBlockK, PAIR ? BN / 2 : BN))
+        return WW_ERR_UNSUPPORTED;
+    f.stored = i64(p.N) * static_cast<int>(sizeof(O)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+    if (f.stored && !encode_rows_map(&f.c, p.dtype, p.out, p.M, p.N, p.N, L::kChunk, 32)) return WW_ERR_UNSUPPORTED;
+    f.xs = xs;
+    f.ws = p.w_scale;
+    f.bias = p.bias;
+    f.out = p.out;
+    f.M = p.M;
+    f.N = p.N;
+    f.k_blocks = (p.K + kBlockK - 1) / kBlockK;
+    const int rows = PAIR ? 2 * kTileM : kTileM;
+    f.m_tiles = (p.M + rows - 1) / rows;
+    f.n_tiles = (p.N + BN - 1) / BN;
+    f.band = 8;
+    f.behind = behind;
+    f.err = err;
+    const int64_t tiles = i64(f.m_tiles) * f.n_tiles;
+    if (tiles > INT_MAX / 2) return WW_ERR_UNSUPPORTED;
+    return launch_tiles<BN, PAIR, O>(f, static_cast<int>(tiles), sms, stream);
+}
+
+template <typename O>
+int few(const ww_int8_matmul_t& p, cudaStream_t stream) noexcept
+{
+    FewParams f{p.x, p.x_q, p.x_scale, p.w_scale, p.w_q, p.bias, p.out, p.x_stride, p.x_q_stride, p.w_stride, p.M, p.K, p.N, few_pitch(p.K), 0};
+    constexpr int V = 16 / static_cast<int>(sizeof(O));
+    f.x_pieces = p.K % V == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && (p.M == 1 || p.x_stride % V == 0);
+    const auto kernel = p.M <= 8 ? int8_few_kernel<O, 1> : int8_few_kernel<O, 2>;
+    static std::atomic<uint64_t> raised[2];
+    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised[p.M <= 8 ? 0 : 1])) return launch_status("int8_matmul");
+    kernel<<<(p.N + kFewChannels - 1) / kFewChannels, kFewWarps * 32, p.M * f.pitch + few_rest(p.M <= 8 ? 8 : 16), stream>>>(f);
+    return launch_status("int8_matmul");
+}
+
+template <typename O>
+int matmul(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
+{
+    if (few_form(p)) return few<O>(p, stream);
+    int* err = device_error_slot();
+    if (err == nullptr) return WW_ERR_DEVICE;
+    const int8_t* xq = p.x_q;
+    const float* xs = p.x_scale;
+    int64_t stride = p.x_q_stride;
+    if (p.x != nullptr) {
+        stride = pitch_of(p.K);
+        int8_t* q = static_cast<int8_t*>(p.workspace);
+        float* scale = reinterpret_cast<float*>(q + i64(p.M) * stride);
+        ww_layer_norm_t r{};
+        r.x = p.x;
+        r.x_stride = p.x_stride;
+        r.y_q = q;
+        r.y_scale = scale;
+        r.y_q_stride = stride;
+        r.dtype = p.dtype;
+        r.rows = p.M;
+        r.N = p.K;
+        const int st = quantise_rows(r, "int8_matmul", stream);
+        if (st != WW_SUCCESS) return st;
+        xq = q;
+        xs = scale;
+    }
+    const int64_t rows = (p.M + 127) / 128;
+    if (rows * ((p.N + 255) / 256) >= sms && p.N > 128)
+        return run_tiles<256, true, O>(p, xq, xs, stride, p.x != nullptr, sms, err, stream);
+    if (rows * ((p.N + 127) / 128) >= sms / 2 && p.N > 64)
+        return run_tiles<128, false, O>(p, xq, xs, stride, p.x != nullptr, sms, err, stream);
+    return run_tiles<64, false, O>(p, xq, xs, stride, p.x != nullptr, sms, err, stream);
+}
+
+int check(const ww_int8_matmul_t& p) noexcept
+{
+    if (p.dtype != WW_DTYPE_HALF && p.dtype != WW_DTYPE_BF16 && p.dtype != WW_DTYPE_FLOAT) return WW_ERR_INVALID_DTYPE;
+    if (p.M < 0 || p.N < 0 || p.K <= 0) return WW_ERR_INVALID_SHAPE;
+    if (p.K >= (1 << 17)) return WW_ERR_UNSUPPORTED;
+    if (p.M == 0 || p.N == 0) return WW_SUCCESS;
+    if (p.w_q == nullptr || p.w_scale == nullptr || p.out == nullptr) return WW_ERR_NULL_POINTER;
+    if ((p.x == nullptr) == (p.x_q == nullptr) || (p.x_q != nullptr && p.x_scale == nullptr)) return WW_ERR_NULL_POINTER;
+    const int bytes = p.dtype == WW_DTYPE_FLOAT ? 4 : 2;
+    const auto off = [](const void* q, int by) { return reinterpret_cast<uintptr_t>(q) % by != 0; };
+    if (p.w_stride < p.K || (p.x_q != nullptr && p.x_q_stride < p.K && p.M > 1) || (p.x != nullptr && p.x_stride < 0)) return WW_ERR_INVALID_SHAPE;
+    if (off(p.w_q, 16) || p.w_stride % 16 != 0 || off(p.x_q, 16) || (p.x_q != nullptr && p.M > 1 && p.x_q_stride % 16 != 0)) return WW_ERR_MISALIGNED;
+    if (off(p.x, bytes) || off(p.bias, bytes) || off(p.out, bytes) || off(p.x_scale, 4) || off(p.w_scale, 4)) return WW_ERR_MISALIGNED;
+    return WW_SUCCESS;
+}
+
+int64_t workspace(const ww_int8_matmul_t& p) noexcept
+{
+    if (p.x == nullptr || p.M == 0 || p.N == 0 || few_form(p)) return 0;
+    return i64(p.M) * pitch_of(p.K) + i64(p.M) * 4;
+}
+
+}  // namespace
+}  // namespace ww
+
+extern "C" {
+
+int64_t ww_int8_matmul_workspace(const ww_int8_matmul_t* p)
+{
+    return p == nullptr || ww::check(*p) != WW_SUCCESS ? 0 : ww::workspace(*p);
+}
+
+int ww_int8_matmul(const ww_int8_matmul_t* p, void* stream)
+{
+    if (p == nullptr) return WW_ERR_NULL_POINTER;
+    int st = ww::check(*p);
+    if (st != WW_SUCCESS || p->M == 0 || p->N == 0) return st;
+    const int64_t need = ww::workspace(*p);
+    if (need > 0) {
+        if (p->workspace == nullptr) return WW_ERR_NULL_POINTER;
+        if (reinterpret_cast<uintptr_t>(p->workspace) % 16 != 0) return WW_ERR_MISALIGNED;
+        if (p->workspace_bytes < need) return WW_ERR_UNSUPPORTED;
+    }
+    ww::DeviceInfo d;
+    if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return p->dtype == WW_DTYPE_HALF ? ww::matmul<__half>(*p, d.sm_count, s)
+         : p->dtype == WW_DTYPE_BF16 ? ww::matmul<__nv_bfloat16>(*p, d.sm_count, s) : ww::matmul<float>(*p, d.sm_count, s);
+}
+
+}  // extern "C"

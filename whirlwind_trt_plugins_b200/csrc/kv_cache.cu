@@ -1,0 +1,213 @@
+// kv_cache.cu -- keys and values kept in 8 bits: rows (token, head) written with
+// a scale each, and read back.
+//
+// Bound: HBM (writing: 2 bytes a value read, 1 written, and 4 a row; reading the
+// reverse).  A row is held by a group of lanes with 16 bytes each of the 16-bit side,
+// so that both sides of a warp lie side by side; the row's largest magnitude takes
+// log2(lanes) shuffles.  A group has kRows rows under way.  Scales stand by head, so
+// that attention reads those of a head's keys as a run.
+#include "rows.cuh"
+
+#include <algorithm>
+
+namespace ww {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kRows = 2;  // rows of a group
+
+struct CacheSide {
+    const void* x;
+    int8_t* q;
+    float* scale;
+    void* out;
+    int64_t xb, xl, xh, qb, ql, qh, sb, sh;
+};
+
+struct CacheParams {
+    CacheSide side[2];  // keys, values
+    const int32_t *start, *lens;
+    Divisor L, H;  // tokens (reading: places) of an item, heads
+    int32_t rows, places, D, keep;  // keep: what lies behind the lens is not written (reading)
+};
+
+struct CacheRow {
+    int b, l, h;
+    __device__ __forceinline__ CacheRow(const CacheParams& p, int row)
+    {
+        const int token = p.H.div(row);
+        h = row - token * p.H.d;
+        b = p.L.div(token);
+        l = token - b * p.L.d;
+    }
+};
+
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(kBlock) quantize_kv_kernel(const __grid_constant__ CacheParams p)
+{
+    const CacheSide& s = p.side[blockIdx.y];
+    const int lane = threadIdx.x % GROUP, d = lane * 8;
+    constexpr int kStep = kBlock / GROUP;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kStep * kRows + threadIdx.x / GROUP;
+    Piece<T, 8> raw[kRows][1];
+    int64_t to[kRows], scale_at[kRows];
+    bool put[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int64_t row = first + i * kStep;
+        put[i] = false;
+        raw[i][0].clear();
+        if (row >= p.rows) continue;
+        const CacheRow at(p, static_cast<int>(row));
+        const int64_t place = (p.start == nullptr ? int64_t{0} : static_cast<int64_t>(__ldg(p.start + at.b))) + at.l;
+        put[i] = place >= 0 && place < p.places && (p.lens == nullptr || at.l < __ldg(p.lens + at.b));
+        to[i] = at.b * s.qb + place * s.ql + at.h * s.qh + d;
+        scale_at[i] = at.b * s.sb + at.h * s.sh + place;
+        if (put[i] && d < p.D) raw[i][0].load(static_cast<const T*>(s.x) + at.b * s.xb + at.l * s.xl + at.h * s.xh + d);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        Pair f[4];
+        values_of<T, 8, 1>(raw[i], f);
+        const RowScale k = row_scale(row_max<GROUP>(largest(f), nullptr));
+        if (!put[i]) continue;
+        if (d < p.D) store_piece_int8<8>(s.q + to[i], f, k.inv, 0);
+        if (lane == 0) s.scale[scale_at[i]] = k.scale;
+    }
+}
+
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(kBlock) dequantize_kv_kernel(const __grid_constant__ CacheParams p)
+{
+    const CacheSide& s = p.side[blockIdx.y];
+    const int lane = threadIdx.x % GROUP, d = lane * 8;
+    constexpr int kStep = kBlock / GROUP;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kStep * kRows + threadIdx.x / GROUP;
+    if (d >= p.D) return;
+    uint2 q[kRows];
+    float scale[kRows];
+    bool put[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int64_t row = first + i * kStep;
+        put[i] = row < p.rows;
+        q[i] = make_uint2(0, 0);
+        scale[i] = 0.0f;
+        if (!put[i]) continue;
+        const CacheRow at(p, static_cast<int>(row));
+        if (p.lens == nullptr || at.l < __ldg(p.lens + at.b)) {
+            q[i] = __ldg(reinterpret_cast<const uint2*>(s.q + at.b * s.qb + at.l * s.ql + at.h * s.qh + d));
+            scale[i] = __ldg(s.scale + at.b * s.sb + at.h * s.sh + at.l);
+        } else if (p.keep) {
+            put[i] = false;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        if (!put[i]) continue;
+        uint32_t r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w = j < 2 ? q[i].x : q[i].y;
+            const float a = static_cast<float>(static_cast<int8_t>(w >> (j % 2 * 16))), b = static_cast<float>(static_cast<int8_t>(w >> (j % 2 * 16 + 8)));
+            r[j] = pack2<T>(a * scale[i], b * scale[i]);
+        }
+        *reinterpret_cast<uint4*>(static_cast<T*>(s.out) + (first + i * kStep) * p.D + d) = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+}
+
+CacheParams params(const ww_kv_cache_t& p, int tokens) noexcept
+{
+    CacheParams f{};
+    const auto side = [&](CacheSide& s, const void* x, int8_t* q, float* scale, void* out, const int64_t (&xs)[3], const int64_t (&qs)[3],
+                          const int64_t (&ss)[2]) {
+        s = {x, q, scale, out, xs[0], xs[1], xs[2], qs[0], qs[1], qs[2], ss[0], ss[1]};
+    };
+    side(f.side[0], p.k, p.k_cache, p.k_scale, p.k_out, p.k_strides, p.k_cache_strides, p.k_scale_strides);
+    side(f.side[1], p.v, p.v_cache, p.v_scale, p.v_out, p.v_strides, p.v_cache_strides, p.v_scale_strides);
+    f.start = p.start;
+    f.lens = p.lens;
+    f.L = make_divisor(std::max(tokens, 1));
+    f.H = make_divisor(p.H);
+    f.rows = p.B * tokens * p.H;
+    f.places = p.places;
+    f.D = p.D;
+    return f;
+}
+
+template <bool WRITE, typename T>
+int launch(const CacheParams& f, const char* name, cudaStream_t stream) noexcept
+{
+    const int group = f.D <= 32 ? 4 : f.D <= 64 ? 8 : 16, step = kBlock / group * kRows;
+    const dim3 grid(static_cast<unsigned>((i64(f.rows) + step - 1) / step), 2);
+    const auto go = [&](auto kernel) { kernel<<<grid, kBlock, 0, stream>>>(f); };
+    if constexpr (WRITE) {
+        if (group == 4) go(quantize_kv_kernel<T, 4>);
+        else if (group == 8) go(quantize_kv_kernel<T, 8>);
+        else go(quantize_kv_kernel<T, 16>);
+    } else {
+        if (group == 4) go(dequantize_kv_kernel<T, 4>);
+        else if (group == 8) go(dequantize_kv_kernel<T, 8>);
+        else go(dequantize_kv_kernel<T, 16>);
+    }
+    return launch_status(name);
+}
+
+int check(const ww_kv_cache_t& p, bool write) noexcept
+{
+    if (p.dtype != WW_DTYPE_HALF && p.dtype != WW_DTYPE_BF16) return WW_ERR_INVALID_DTYPE;
+    const int tokens = write ? p.L : p.places;
+    if (p.B < 0 || p.L < 0 || p.places < 0 || p.H <= 0 || p.D <= 0) return WW_ERR_INVALID_SHAPE;
+    if (p.D % 16 != 0 || p.D > 128) return WW_ERR_UNSUPPORTED;
+    if (i64(p.B) * tokens >= INT32_MAX || i64(p.B) * tokens * p.H >= INT32_MAX) return WW_ERR_UNSUPPORTED;
+    if (p.B == 0 || tokens == 0 || p.places == 0) return WW_SUCCESS;
+    if (p.k_cache == nullptr || p.v_cache == nullptr || p.k_scale == nullptr || p.v_scale == nullptr) return WW_ERR_NULL_POINTER;
+    if (write ? p.k == nullptr || p.v == nullptr : p.k_out == nullptr || p.v_out == nullptr) return WW_ERR_NULL_POINTER;
+    for (const int64_t(*s)[3] : {&p.k_cache_strides, &p.v_cache_strides}) {
+        const int n[3] = {p.B, p.places, p.H};
+        for (int i = 0; i < 3; ++i) {
+            if (n[i] <= 1) continue;
+            if (write && (*s)[i] == 0) return WW_ERR_INVALID_SHAPE;  // two places in one
+            if ((*s)[i] < 0 || (*s)[i] % 16 != 0) return WW_ERR_MISALIGNED;
+        }
+    }
+    for (const int64_t(*s)[2] : {&p.k_scale_strides, &p.v_scale_strides})
+        for (int i = 0; i < 2; ++i)
+            if ((i ? p.H : p.B) > 1 && ((*s)[i] < 0 || (write && (*s)[i] < p.places))) return WW_ERR_INVALID_SHAPE;  // two in one
+    const auto off = [](const void* q, int by) { return reinterpret_cast<uintptr_t>(q) % by != 0; };
+    if (off(p.k_cache, 16) || off(p.v_cache, 16) || off(p.k_scale, 4) || off(p.v_scale, 4) || off(p.start, 4) || off(p.lens, 4))
+        return WW_ERR_MISALIGNED;
+    if (write ? !vectors_ok(p.k, p.k_strides, p.B, p.L, p.H, 2) || !vectors_ok(p.v, p.v_strides, p.B, p.L, p.H, 2)
+              : off(p.k_out, 16) || off(p.v_out, 16))
+        return WW_ERR_MISALIGNED;
+    return WW_SUCCESS;
+}
+
+template <bool WRITE>
+int run(const ww_kv_cache_t* p, bool keep, const char* name, void* stream) noexcept
+{
+    if (p == nullptr) return WW_ERR_NULL_POINTER;
+    int st = check(*p, WRITE);
+    const int tokens = WRITE ? p->L : p->places;
+    if (st != WW_SUCCESS || p->B == 0 || tokens == 0 || p->places == 0) return st;
+    DeviceInfo d;
+    if ((st = current_device_info(&d)) != WW_SUCCESS) return st;
+    CacheParams f = params(*p, tokens);
+    f.keep = keep;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return p->dtype == WW_DTYPE_HALF ? launch<WRITE, __half>(f, name, s) : launch<WRITE, __nv_bfloat16>(f, name, s);
+}
+
+}  // namespace
+
+// ww_dequantize_kv that leaves what lies behind the lens unwritten.
+int dequantise_valid(const ww_kv_cache_t& p, const char* name, void* stream) noexcept { return run<false>(&p, true, name, stream); }
+
+}  // namespace ww
+
+extern "C" {
+
+int ww_quantize_kv(const ww_kv_cache_t* p, void* stream) { return ww::run<true>(p, false, "quantize_kv", stream); }
+int ww_dequantize_kv(const ww_kv_cache_t* p, void* stream) { return ww::run<false>(p, false, "dequantize_kv", stream); }
+
+}  // extern "C"

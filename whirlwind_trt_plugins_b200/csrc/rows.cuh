@@ -1,0 +1,231 @@
+// rows.cuh -- what the kernels over rows of values share: pieces of a row in
+// registers as pairs of fp32, sums over the lanes of a row, and the 8-bit form
+// of a row.
+#pragma once
+
+#include "attention.cuh"
+
+#include <climits>
+
+namespace ww {
+
+// ---- a row in 8 bits ----
+//
+// a = max |x|,  scale = a / 127,  q = rint(x * (127 / a)), the product not rounded
+// before: whole numbers in [-127, 127], x = scale q within half a step.  A row with a NaN or an infinity
+// has scale NaN, so that what is computed from it is NaN; one whose largest
+// magnitude is below 2^-119 (the scale would leave fp32's normal range) has
+// scale 0 and zeros.
+struct RowScale {
+    float inv, scale;
+};
+
+__device__ __forceinline__ RowScale row_scale(float top)  // top: max_nan over |x|
+{
+    RowScale r{0.0f, 0.0f};
+    if (!(top < INFINITY)) r.scale = __int_as_float(0x7fffffff);
+    else if (top >= 0x1p-119f) {
+        r.inv = __fdiv_rn(127.0f, top);
+        r.scale = __fdiv_rn(top, 127.0f);
+    }
+    return r;
+}
+
+// rint of a product in [-127, 127] in the low byte: adding 1.5 * 2^23 in the same
+// instruction leaves the whole number, ties to even, in the low bits.
+constexpr float kRintMagic = 12582912.0f;
+
+__device__ __forceinline__ int8_t quantise(float x, float inv)
+{
+    return static_cast<int8_t>(__float_as_uint(__fmaf_rn(x, inv, kRintMagic)));
+}
+
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)  // low bytes
+{
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// Two values to whole numbers in the low bytes.
+__device__ __forceinline__ void quantise2(Pair x, Pair inv, uint32_t& lo, uint32_t& hi)
+{
+    float a, b;
+    unpair(fma2(x, inv, pair(kRintMagic, kRintMagic)), a, b);
+    lo = __float_as_uint(a);
+    hi = __float_as_uint(b);
+}
+
+// ---- pieces of V values of T, as they are loaded ----
+
+template <typename T, int V>
+struct Piece {
+    static constexpr int kBytes = V * static_cast<int>(sizeof(T));
+    static constexpr int kWords = kBytes >= 4 ? kBytes / 4 : 1;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const T* p)
+    {
+        if constexpr (kBytes == 16) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = u.x;
+            w[1] = u.y;
+            w[2] = u.z;
+            w[3] = u.w;
+        } else if constexpr (kBytes == 4) {
+            w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        } else {
+            static_assert(kBytes == 2, "16, 4 or 2 bytes");
+            w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+        }
+    }
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float get(int i) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t u = i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu;
+        if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(static_cast<unsigned short>(u)));
+        return i % 2 ? __uint_as_float(w[i / 2] & 0xffff0000u) : __uint_as_float(w[i / 2] << 16);
+    }
+};
+
+// E values of a row as E / 2 pairs; value e of the lane is value e % V of its piece e / V.
+template <typename T, int V, int P>
+__device__ __forceinline__ void values_of(const Piece<T, V> (&raw)[P], Pair (&f)[P * V / 2])
+{
+#pragma unroll
+    for (int i = 0; i < P * V / 2; ++i) {
+        const int e = 2 * i;
+        if constexpr (std::is_same<T, __half>::value && V > 1) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&raw[e / V].w[e % V / 2]));
+            f[i] = pair(v.x, v.y);
+        } else {
+            f[i] = pair(raw[e / V].get(e % V), raw[(e + 1) / V].get((e + 1) % V));
+        }
+    }
+}
+
+// Piece i of a lane's values to memory.
+template <typename T, int V, int E>
+__device__ __forceinline__ void store_piece(T* p, const Pair (&f)[E], int i)
+{
+    if constexpr (V == 1) {
+        float v[2];
+        unpair(f[i / 2], v[0], v[1]);
+        *p = from_float<T>(i % 2 ? v[1] : v[0]);
+    } else {
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) unpair(f[i * V / 2 + j], v[2 * j], v[2 * j + 1]);
+        if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    }
+}
+
+// Piece i in 8 bits to memory.
+template <int V, int E>
+__device__ __forceinline__ void store_piece_int8(int8_t* p, const Pair (&f)[E], float inv, int i)
+{
+    const Pair k = pair(inv, inv);
+    if constexpr (V == 1) {
+        uint32_t q[2];
+        quantise2(f[i / 2], k, q[0], q[1]);
+        *p = static_cast<int8_t>(i % 2 ? q[1] : q[0]);
+    } else {
+        uint32_t q[V];
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) quantise2(f[i * V / 2 + j], k, q[2 * j], q[2 * j + 1]);
+        if constexpr (V == 4)
+            *reinterpret_cast<uint32_t*>(p) = pack4(q[0], q[1], q[2], q[3]);
+        else
+            *reinterpret_cast<uint2*>(p) = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+    }
+}
+
+__device__ __forceinline__ float both(Pair p)
+{
+    float a, b;
+    unpair(p, a, b);
+    return a + b;
+}
+
+// Sum over the GROUP lanes of a row; GROUP 0: over the block, in a fixed order (`red`: 32
+// floats of shared memory that no other sum under way uses; one barrier).
+template <int GROUP>
+__device__ __forceinline__ float row_sum(float v, float* red)
+{
+#pragma unroll
+    for (int o = (GROUP ? GROUP : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if constexpr (GROUP == 0) {
+        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+        __syncthreads();
+        v = threadIdx.x % 32 < blockDim.x / 32 ? red[threadIdx.x % 32] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    }
+    return v;
+}
+
+// Largest magnitude of a row's values, NaN if there is one.
+template <int GROUP>
+__device__ __forceinline__ float row_max(float v, float* red)
+{
+#pragma unroll
+    for (int o = (GROUP ? GROUP : 32) / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+    if constexpr (GROUP == 0) {
+        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+        __syncthreads();
+        v = threadIdx.x % 32 < blockDim.x / 32 ? red[threadIdx.x % 32] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+    }
+    return v;
+}
+
+template <int E>
+__device__ __forceinline__ float largest(const Pair (&f)[E])
+{
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        float a, b;
+        unpair(f[i], a, b);
+        top = max3_nan(top, fabsf(a), fabsf(b));
+    }
+    return top;
+}
+
+// How a row of n values lies on lanes: `group` lanes a row (0: `threads` of a block),
+// `pieces` pieces of V values each; group and pieces both 0: too long for registers.
+struct RowForm {
+    int group, pieces, threads;
+};
+
+// Pieces of 16 bytes (v > 1): the form with the fewest idle lanes, and of those the one
+// with the fewest pieces a lane (at most `most`).  Single values (v == 1, rows that do
+// not start on 16 bytes): 4 or 16 a lane.  Rows that a warp does not hold: a block of up
+// to `threads` threads.
+inline RowForm row_form(int n, int v, int most, int threads)
+{
+    const int all = (n + v - 1) / v;
+    const auto block = [&](int p) { return RowForm{0, p, ((all + p - 1) / p + 31) / 32 * 32}; };
+    if (v > 1) {
+        static constexpr int kForms[][2] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {16, 3}, {32, 2}, {32, 3}, {32, 4}};
+        for (const auto& f : kForms)  // ascending lanes x pieces
+            if (f[0] * f[1] >= all && f[1] <= most) return {f[0], f[1], 256};
+        for (int p = 2; p <= most && p <= 4; p *= 2)
+            if (all <= threads * p) return block(p);
+    } else {
+        if (n <= 128) return {32, 4, 256};
+        if (n <= 512) return {32, 16, 256};
+        for (int p = 4; p <= 16; p *= 4)
+            if (all <= threads * p) return block(p);
+    }
+    return {0, 0, 0};
+}
+
+}  // namespace ww

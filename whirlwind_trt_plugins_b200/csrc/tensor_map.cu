@@ -1,6 +1,8 @@
 // tensor_map.cu -- see tensor_map.cuh.
 #include "tensor_map.cuh"
 
+#include "../../include/ww_trt_plugins.h"
+
 #include <mutex>
 
 namespace ww {
@@ -111,6 +113,55 @@ bool encode_vectors_map(CUtensorMap* out, bool bf16, const void* base, int D, co
     return encode(fn, out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                   const_cast<void*>(base), dims, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+bool encode_rows_map(CUtensorMap* out, int dtype, const void* base, int rows, int cols, int64_t stride, int box_cols,
+                     int box_rows) noexcept
+{
+    if (out == nullptr || base == nullptr || reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+    const int bytes = dtype == WW_DTYPE_INT8 ? 1 : dtype == WW_DTYPE_FLOAT ? 4 : 2, box_bytes = box_cols * bytes;
+    if (rows <= 0 || cols <= 0 || box_rows <= 0 || box_rows > 256) return false;
+    if (box_bytes != 32 && box_bytes != 64 && box_bytes != 128) return false;
+    if (rows == 1) stride = (cols + 15) / 16 * 16;
+    if (stride < cols || stride * bytes % 16 != 0 || stride * bytes >= (int64_t{1} << 40)) return false;
+    const EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t st[1] = {static_cast<cuuint64_t>(stride * bytes)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2] = {1u, 1u};
+    const CUtensorMapDataType type = dtype == WW_DTYPE_INT8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : dtype == WW_DTYPE_HALF ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : dtype == WW_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    return encode(fn, out, type, 2, const_cast<void*>(base), dims, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+bool encode_bytes_map(CUtensorMap* out, const void* base, int D, const int (&n)[3], const int64_t (&strides)[3],
+                      int box_cols, int box_rows) noexcept
+{
+    if (out == nullptr || base == nullptr || reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+    if (D <= 0 || (box_cols != 32 && box_cols != 64 && box_cols != 128) || box_rows <= 0 || box_rows > 256) return false;
+    const EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), 1, 1, 1};
+    cuuint64_t st[3] = {16, 16, 16};
+    constexpr int from[3] = {2, 1, 0};  // as in encode_vectors_map
+    for (int i = 0; i < 3; ++i) {
+        const int a = from[i];
+        if (n[a] <= 0) return false;
+        if (n[a] == 1 || strides[a] == 0) continue;
+        if (strides[a] < 0 || strides[a] % 16 != 0 || strides[a] >= (int64_t{1} << 40)) return false;
+        dims[i + 1] = static_cast<cuuint64_t>(n[a]);
+        st[i] = static_cast<cuuint64_t>(strides[a]);
+    }
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(box_cols), 1u, static_cast<cuuint32_t>(box_rows), 1u};
+    const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+    return encode(fn, out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, st, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 

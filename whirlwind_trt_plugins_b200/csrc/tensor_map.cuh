@@ -31,4 +31,14 @@ bool encode_volume_map(CUtensorMap* out, const void* base, int B, int G, int D, 
 bool encode_vectors_map(CUtensorMap* out, bool bf16, const void* base, int D, const int (&n)[3],
                         const int64_t (&strides)[3], int box_cols, int box_rows) noexcept;
 
+// [rows, cols] of a ww_dtype_t (`stride` elements between rows, a multiple of 16
+// bytes); box = box_rows rows of 32, 64 or 128 bytes, swizzled over them.  Places
+// outside read 0 and are not written.
+bool encode_rows_map(CUtensorMap* out, int dtype, const void* base, int rows, int cols, int64_t stride, int box_cols,
+                     int box_rows) noexcept;
+
+// encode_vectors_map for 8-bit values: boxes of 32, 64 or 128 values.
+bool encode_bytes_map(CUtensorMap* out, const void* base, int D, const int (&n)[3], const int64_t (&strides)[3],
+                      int box_cols, int box_rows) noexcept;
+
 }  // namespace ww
