@@ -679,7 +679,7 @@ def test_refusals(env):
             (ww.WWError, lambda: ww.quantize_kv(k, k, *[c[:1].expand(2, *c.shape[1:]) for c in kept])),
             (TypeError, lambda: ww.dequantize_kv(*kept, dtype=f32)), (TypeError, lambda: ww.dequantize_kv(kept[0].short(), *kept[1:])),
             (ValueError, lambda: ww.cross_attention_int8(k[..., :16].contiguous(), *kept)), (TypeError, lambda: ww.cross_attention_int8(k.float(), *kept)),
-            (ValueError, lambda: ww.cross_attention_int8(k[:, :, :3].contiguous(), *kept)), (TypeError, lambda: ww.cross_attention_int8(k, *kept, key_mask=s4)),
+            (ValueError, lambda: ww.cross_attention_int8(k[:, :, :3].contiguous(), *kept)), (ValueError, lambda: ww.cross_attention_int8(k, *kept, key_mask=s4)),
             (ValueError, lambda: ww.cross_attention_int8(k, *kept, bias_table=w[None]))]:
         with pytest.raises(error):
             call()

@@ -569,11 +569,11 @@ int ww_cross_attention_int8(const ww_attention_int8_t* a, void* stream)
     const ww_attention_t& p = a->attention;
     int st = ww::check(*a);
     if (st != WW_SUCCESS || p.B == 0 || p.Lq == 0) return st;
-    ww::DeviceInfo d;
-    if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
-    const int64_t need = ww::workspace(*a, d.sm_count);
+    const int64_t need = ww::workspace(*a, ww::sm_count());
     if (need > 0 && p.workspace == nullptr) return WW_ERR_NULL_POINTER;
     if (need > p.workspace_bytes) return WW_ERR_UNSUPPORTED;
+    ww::DeviceInfo d;
+    if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const ww::Plan plan = ww::make_plan(p, d.sm_count);
     if (plan.few) return p.dtype == WW_DTYPE_HALF ? ww::few_rows<__half>(*a, plan, s) : ww::few_rows<__nv_bfloat16>(*a, plan, s);
