@@ -8,7 +8,7 @@ roundoff:
 * layer norm: one rounding of the result (u |y|) and fp32 arithmetic, 2^-20 of the
   magnitudes that enter a value, a normalised value's being (|x| + mean |x|) rstd; sums
   over rows: 2^-18 of the magnitudes (up to 60 additions in a row at 2^-24);
-* 8 bits: whole numbers and scales of rows are compared with the same operations
+* 8 bits: whole numbers and scales of rows are compared with the same fp32 operations
   on the host, bit for bit; a normalised row is within half a step of its exact value
   and the fp32 term above;
 * products: three fp32 roundings and the result's: 2^-22 (|sum xs ws| + |b|) + u |y|;
@@ -193,13 +193,13 @@ def test_layer_norm_autograd(env):
 # ---------------------------------------------------------------- 8 bits
 
 def _int8_host(x):
-    """Whole numbers and scales of rows on the host: fp32 quotients, the products exact in 64 bits."""
+    """Whole numbers and scales of rows by the same fp32 operations on the host."""
     x = x.float().cpu().numpy()
     top = np.abs(x).max(-1, keepdims=True).astype(np.float32)
     with np.errstate(all="ignore"):
         small, bad = top < np.float32(2.0 ** -119), ~np.isfinite(top)
         inv = np.where(small | bad, np.float32(0), np.float32(127) / top).astype(np.float32)
-        q = np.rint(np.where(np.isfinite(x), x, 0).astype(np.float64) * inv).astype(np.int8)
+        q = np.rint((np.where(np.isfinite(x), x, 0) * inv).astype(np.float32)).astype(np.int8)
         scale = np.where(small, np.float32(0), np.where(bad, np.float32(np.nan), top / np.float32(127)))
     return q, scale[..., 0].astype(np.float32), bad[..., 0]
 

@@ -11,8 +11,8 @@ namespace ww {
 
 // ---- a row in 8 bits ----
 //
-// a = max |x|,  scale = a / 127,  q = rint(x * (127 / a)), the product not rounded
-// before: whole numbers in [-127, 127], x = scale q within half a step.  A row with a NaN or an infinity
+// a = max |x|,  scale = a / 127,  q = rint(x * (127 / a)) in fp32: whole numbers in
+// [-127, 127], x = scale q within half a step.  A row with a NaN or an infinity
 // has scale NaN, so that what is computed from it is NaN; one whose largest
 // magnitude is below 2^-119 (the scale would leave fp32's normal range) has
 // scale 0 and zeros.
@@ -31,13 +31,15 @@ __device__ __forceinline__ RowScale row_scale(float top)  // top: max_nan over |
     return r;
 }
 
-// rint of a product in [-127, 127] in the low byte: adding 1.5 * 2^23 in the same
-// instruction leaves the whole number, ties to even, in the low bits.
+// rint of a product in [-127, 127] in the low byte: adding 1.5 * 2^23 leaves the whole
+// number, ties to even, in the low bits.  The product is rounded before, so that values of
+// few bits that lie half way between two steps are met as ties in spite of the
+// quotient's rounding (packed forms of the two would be fused by the compiler).
 constexpr float kRintMagic = 12582912.0f;
 
 __device__ __forceinline__ int8_t quantise(float x, float inv)
 {
-    return static_cast<int8_t>(__float_as_uint(__fmaf_rn(x, inv, kRintMagic)));
+    return static_cast<int8_t>(__float_as_uint(__fadd_rn(__fmul_rn(x, inv), kRintMagic)));
 }
 
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)  // low bytes
@@ -49,9 +51,9 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 __device__ __forceinline__ void quantise2(Pair x, Pair inv, uint32_t& lo, uint32_t& hi)
 {
     float a, b;
-    unpair(fma2(x, inv, pair(kRintMagic, kRintMagic)), a, b);
-    lo = __float_as_uint(a);
-    hi = __float_as_uint(b);
+    unpair(mul2(x, inv), a, b);
+    lo = __float_as_uint(__fadd_rn(a, kRintMagic));
+    hi = __float_as_uint(__fadd_rn(b, kRintMagic));
 }
 
 // ---- pieces of V values of T, as they are loaded ----
