@@ -14,7 +14,10 @@ namespace ww {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kRows = 2;  // rows of a group
+#ifndef WW_WROWS
+#define WW_WROWS 4
+#endif
+constexpr int kRows = 2, kWriteRows = WW_WROWS;  // rows of a group, reading and writing
 
 struct CacheSide {
     const void* x;
@@ -45,34 +48,46 @@ struct CacheRow {
 template <typename T, int GROUP>
 __global__ void __launch_bounds__(kBlock) quantize_kv_kernel(const __grid_constant__ CacheParams p)
 {
+    constexpr int R = kWriteRows, kStep = kBlock / GROUP;
+    // where the block's rows come from and go, worked out by a thread each
+    __shared__ int64_t from[kStep * R], to[kStep * R], scale_to[kStep * R];  // from < 0: not written
     const CacheSide& s = p.side[blockIdx.y];
-    const int lane = threadIdx.x % GROUP, d = lane * 8;
-    constexpr int kStep = kBlock / GROUP;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kStep * kRows + threadIdx.x / GROUP;
-    Piece<T, 8> raw[kRows][1];
-    int64_t to[kRows], scale_at[kRows];
-    bool put[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int64_t row = first + i * kStep;
-        put[i] = false;
-        raw[i][0].clear();
+    const int lane = threadIdx.x % GROUP, d = lane * 8, first = threadIdx.x / GROUP;
+    for (int i = threadIdx.x; i < kStep * R; i += kBlock) {
+        const int64_t row = static_cast<int64_t>(blockIdx.x) * (kStep * R) + i;
+        from[i] = -1;
         if (row >= p.rows) continue;
         const CacheRow at(p, static_cast<int>(row));
         const int64_t place = (p.start == nullptr ? int64_t{0} : static_cast<int64_t>(__ldg(p.start + at.b))) + at.l;
-        put[i] = place >= 0 && place < p.places && (p.lens == nullptr || at.l < __ldg(p.lens + at.b));
-        to[i] = at.b * s.qb + place * s.ql + at.h * s.qh + d;
-        scale_at[i] = at.b * s.sb + at.h * s.sh + place;
-        if (put[i] && d < p.D) raw[i][0].load(static_cast<const T*>(s.x) + at.b * s.xb + at.l * s.xl + at.h * s.xh + d);
+        if (place < 0 || place >= p.places || (p.lens != nullptr && at.l >= __ldg(p.lens + at.b))) continue;
+        from[i] = at.b * s.xb + at.l * s.xl + at.h * s.xh;
+        to[i] = at.b * s.qb + place * s.ql + at.h * s.qh;
+        scale_to[i] = at.b * s.sb + at.h * s.sh + place;
     }
+    __syncthreads();
+    Piece<T, 8> raw[R][1];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        Pair f[4];
-        values_of<T, 8, 1>(raw[i], f);
-        const RowScale k = row_scale(row_max<GROUP>(largest(f), nullptr));
-        if (!put[i]) continue;
-        if (d < p.D) store_piece_int8<8>(s.q + to[i], f, k.inv, 0);
-        if (lane == 0) s.scale[scale_at[i]] = k.scale;
+    for (int i = 0; i < R; ++i) {
+        raw[i][0].clear();
+        const int64_t at = from[first + i * kStep];
+        if (at >= 0 && d < p.D) raw[i][0].load(static_cast<const T*>(s.x) + at + d);
+    }
+    Pair f[R][4];
+    float top[R];
+    RowScale k[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        values_of<T, 8, 1>(raw[i], f[i]);
+        top[i] = largest(f[i]);
+    }
+    row_maxima<GROUP>(top, nullptr);
+    row_scales<GROUP>(top, k);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = first + i * kStep;
+        if (from[r] < 0) continue;
+        if (d < p.D) store_piece_int8<8>(s.q + to[r] + d, f[i], k[i].inv, 0);
+        if (lane == 0) s.scale[scale_to[r]] = k[i].scale;
     }
 }
 
@@ -138,7 +153,7 @@ CacheParams params(const ww_kv_cache_t& p, int tokens) noexcept
 template <bool WRITE, typename T>
 int launch(const CacheParams& f, const char* name, cudaStream_t stream) noexcept
 {
-    const int group = f.D <= 32 ? 4 : f.D <= 64 ? 8 : 16, step = kBlock / group * kRows;
+    const int group = f.D <= 32 ? 4 : f.D <= 64 ? 8 : 16, step = kBlock / group * (WRITE ? kWriteRows : kRows);
     const dim3 grid(static_cast<unsigned>((i64(f.rows) + step - 1) / step), 2);
     const auto go = [&](auto kernel) { kernel<<<grid, kBlock, 0, stream>>>(f); };
     if constexpr (WRITE) {

@@ -28,8 +28,25 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kLongBlock = 1024;
-constexpr int kForwardThreads = 1024;  // of a block that holds a row
-__host__ __device__ constexpr int backward_threads(int v) { return v > 1 ? 512 : 640; }
+#ifndef WW_ROWS
+#define WW_ROWS 2
+#endif
+#ifndef WW_BROWS
+#define WW_BROWS 2
+#endif
+#ifndef WW_RES
+#define WW_RES 768
+#endif
+#ifndef WW_B8
+#define WW_B8 3
+#endif
+#ifndef WW_BBLOCKS
+#define WW_BBLOCKS 2
+#endif
+constexpr int kForwardRows = WW_ROWS, kBackwardRows = WW_BROWS;
+// Rows of a group under way in the gradient's kernel, and resident blocks of it.
+__host__ __device__ constexpr int backward_rows(int v, int pieces, int group) { return v > 1 && pieces == 1 && group > 0 ? kBackwardRows : 1; }
+__host__ __device__ constexpr int backward_blocks(int pieces) { return pieces == 1 ? WW_BBLOCKS : 2; }
 
 struct NormParams {
     const void *x, *r, *w, *b;
@@ -44,134 +61,139 @@ struct NormParams {
     float eps, inv_n;
 };
 
-template <typename T, int V, int P, int GROUP>
-__global__ void __launch_bounds__(GROUP ? kBlock : kForwardThreads) layer_norm_kernel(const __grid_constant__ NormParams p)
+// R rows of a group of lanes are under way at a time.
+template <typename T, int V, int P, int GROUP, int R>
+__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), 1) layer_norm_kernel(const __grid_constant__ NormParams p)
 {
-    __shared__ float red[3][32];
+    __shared__ float red[GROUP ? 1 : 3][32 * R];
     constexpr int E = P * V / 2;
-    const int lanes = GROUP ? GROUP : static_cast<int>(blockDim.x), lane = GROUP ? threadIdx.x % GROUP : threadIdx.x;
-    const int64_t row = GROUP ? static_cast<int64_t>(blockIdx.x) * (kBlock / (GROUP ? GROUP : 1)) + threadIdx.x / (GROUP ? GROUP : 1) : blockIdx.x;
-    const int64_t known = min(row, static_cast<int64_t>(p.rows) - 1);
-    const T* x = static_cast<const T*>(p.x) + known * p.xs;
-    Piece<T, V> raw[P];
+    constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block side by side
+    const int lane = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
+    const Columns<V, P, GROUP> column;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + (GROUP ? threadIdx.x / (GROUP ? GROUP : 1) : 0);
+    const auto row_of = [&](int j) { return row0 + j * kGroups; };
+    const auto known = [&](int j) { return min(row_of(j), static_cast<int64_t>(p.rows) - 1); };
+    Pair f[R][E];
+    {
+        Piece<T, V> raw[R][P];
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int c = (i * lanes + lane) * V;
-        if (c < p.N) raw[i].load(x + c);
-        else raw[i].clear();
-    }
-    Pair f[E];
-    values_of<T, V, P>(raw, f);
-    if (p.r != nullptr) {
-        const T* r = static_cast<const T*>(p.r) + known * p.rs;
+        for (int j = 0; j < R; ++j) {
+            const T* x = static_cast<const T*>(p.x) + known(j) * p.xs;
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int c = (i * lanes + lane) * V;
-            if (c < p.N) raw[i].load(r + c);
+            for (int i = 0; i < P; ++i)
+                if (column(i) < p.N) raw[j][i].load(x + column(i));
+                else raw[j][i].clear();
         }
-        Pair g[E];
-        values_of<T, V, P>(raw, g);
+        if (p.r == nullptr) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            float a, b;
-            unpair(add2(f[i], g[i]), a, b);
-            f[i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(b)));
-        }
-        if (p.sum != nullptr && row < p.rows) {
-            T* to = static_cast<T*>(p.sum) + row * p.N;
+            for (int j = 0; j < R; ++j) values_of<T, V, P>(raw[j], f[j]);
+        } else {
+            Piece<T, V> more[R][P];
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int c = (i * lanes + lane) * V;
-                if (c < p.N) store_piece<T, V>(to + c, f, i);
+            for (int j = 0; j < R; ++j) {
+                const T* r = static_cast<const T*>(p.r) + known(j) * p.rs;
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    if (column(i) < p.N) more[j][i].load(r + column(i));
+                    else more[j][i].clear();
+            }
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                values_of<T, V, P>(raw[j], f[j]);
+                Pair g[E];
+                values_of<T, V, P>(more[j], g);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    float a, b;
+                    unpair(add2(f[j][i], g[i]), a, b);
+                    f[j][i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(b)));
+                }
+                if (p.sum != nullptr && row_of(j) < p.rows) {
+                    T* to = static_cast<T*>(p.sum) + row_of(j) * p.N;
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        if (column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < P; ++i)  // beyond the row: zeros again
-            if ((i * lanes + lane) * V >= p.N)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float a, b;
-                    unpair(f[(i * V + e) / 2], a, b);
-                    f[(i * V + e) / 2] = (i * V + e) % 2 ? pair(a, 0.0f) : pair(0.0f, b);
-                }
     }
     if (p.norm) {
-        Pair s = f[0];
+        float v[R];
 #pragma unroll
-        for (int i = 1; i < E; ++i) s = add2(s, f[i]);
-        const float mean = row_sum<GROUP>(both(s), red[0]) * p.inv_n;
-        const Pair nm = pair(-mean, -mean);
-        s = pair(0.0f, 0.0f);
+        for (int j = 0; j < R; ++j) {
+            Pair s = f[j][0];
 #pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = add2(f[i], nm);
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            if ((i * lanes + lane) * V >= p.N) continue;
-            if constexpr (V == 1) {
-                float a, b;
-                unpair(f[i / 2], a, b);
-                const float d = i % 2 ? b : a;
-                s = fma2(pair(d, 0.0f), pair(d, 0.0f), s);
-            } else {
-#pragma unroll
-                for (int j = i * V / 2; j < (i + 1) * V / 2; ++j) s = fma2(f[j], f[j], s);
-            }
+            for (int i = 1; i < E; ++i) s = add2(s, f[j][i]);
+            v[j] = both(s);
         }
-        const float rstd = rsqrtf(fmaf(row_sum<GROUP>(both(s), red[1]), p.inv_n, p.eps));
-        if (lane == 0 && row < p.rows) {
-            if (p.mean != nullptr) p.mean[row] = mean;
-            if (p.rstd != nullptr) p.rstd[row] = rstd;
-        }
-        const Pair r2 = pair(rstd, rstd);
+        row_sums<GROUP>(v, red[0]);
 #pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = mul2(f[i], r2);
+        for (int j = 0; j < R; ++j) {
+            const float mean = v[j] * p.inv_n;
+            if (lane == 0 && p.mean != nullptr && row_of(j) < p.rows) p.mean[row_of(j)] = mean;
+            const Pair nm = pair(-mean, -mean);
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[j][i] = add2(f[j][i], nm);
+            clear_beyond(f[j], p.N, column);
+            Pair s = mul2(f[j][0], f[j][0]);
+#pragma unroll
+            for (int i = 1; i < E; ++i) s = fma2(f[j][i], f[j][i], s);
+            v[j] = both(s);
+        }
+        row_sums<GROUP>(v, red[GROUP ? 0 : 1]);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const float rstd = rsqrtf(fmaf(v[j], p.inv_n, p.eps));
+            if (lane == 0 && p.rstd != nullptr && row_of(j) < p.rows) p.rstd[row_of(j)] = rstd;
+            const Pair r2 = pair(rstd, rstd);
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[j][i] = mul2(f[j][i], r2);
+        }
         if (p.w != nullptr) {
             Piece<T, V> wr[P], br[P];
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const int c = (i * lanes + lane) * V;
                 wr[i].clear();
                 br[i].clear();
-                if (c < p.N) {
-                    wr[i].load(static_cast<const T*>(p.w) + c);
-                    if (p.b != nullptr) br[i].load(static_cast<const T*>(p.b) + c);
+                if (column(i) < p.N) {
+                    wr[i].load(static_cast<const T*>(p.w) + column(i));
+                    if (p.b != nullptr) br[i].load(static_cast<const T*>(p.b) + column(i));
                 }
             }
             Pair w[E], b[E];
             values_of<T, V, P>(wr, w);
             values_of<T, V, P>(br, b);
 #pragma unroll
-            for (int i = 0; i < E; ++i) f[i] = fma2(f[i], w[i], b[i]);
-        } else {
+            for (int j = 0; j < R; ++j)
 #pragma unroll
-            for (int i = 0; i < P; ++i)  // without weights what lies beyond the row is not 0 yet
-                if ((i * lanes + lane) * V >= p.N)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        float a, b;
-                        unpair(f[(i * V + e) / 2], a, b);
-                        f[(i * V + e) / 2] = (i * V + e) % 2 ? pair(a, 0.0f) : pair(0.0f, b);
-                    }
+                for (int i = 0; i < E; ++i) f[j][i] = fma2(f[j][i], w[i], b[i]);
         }
     }
     if (p.q != nullptr) {
-        const RowScale k = row_scale(row_max<GROUP>(largest(f), red[2]));
-        if (row >= p.rows) return;
-        if (lane == 0) p.scale[row] = k.scale;
-        int8_t* to = p.q + row * p.qs;
+        float top[R];
+        RowScale k[R];
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int c = (i * lanes + lane) * V;
-            if (c < p.N) store_piece_int8<V>(to + c, f, k.inv, i);
+        for (int j = 0; j < R; ++j) top[j] = largest(f[j]);
+        row_maxima<GROUP>(top, red[GROUP ? 0 : 2]);
+        row_scales<GROUP>(top, k);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (row_of(j) >= p.rows) continue;
+            if (lane == 0) p.scale[row_of(j)] = k[j].scale;
+            int8_t* to = p.q + row_of(j) * p.qs;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (column(i) < p.N) store_piece_int8<V>(to + column(i), f[j], k[j].inv, i);
         }
         return;
     }
-    if (row >= p.rows) return;
-    T* to = static_cast<T*>(p.y) + row * p.N;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int c = (i * lanes + lane) * V;
-        if (c < p.N) store_piece<T, V>(to + c, f, i);
+    for (int j = 0; j < R; ++j) {
+        if (row_of(j) >= p.rows) continue;
+        T* to = static_cast<T*>(p.y) + row_of(j) * p.N;
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            if (column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
     }
 }
 
@@ -221,24 +243,24 @@ __global__ void __launch_bounds__(kLongBlock) layer_norm_long_kernel(const __gri
         p.q[row * p.qs + c] = quantise(value(c), k.inv);
 }
 
-template <typename T, int V, int P, int GROUP>
-__global__ void __launch_bounds__(GROUP ? kBlock : backward_threads(V)) layer_norm_backward_kernel(const __grid_constant__ NormParams p)
+template <typename T, int V, int P, int GROUP, int R, bool DSUM>
+__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROUP ? backward_blocks(P) : V == 1 && P == 8 ? WW_B8 : 1) layer_norm_backward_kernel(const __grid_constant__ NormParams p)
 {
     constexpr int E = P * V / 2;
-    constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block at a time
+    constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block side by side
     constexpr int kJoin = GROUP ? kBlock * P * V : 1;                  // values of a block's rows
     __shared__ float joined[kJoin];
-    __shared__ float red[2][2][32];
-    const int lanes = GROUP ? GROUP : static_cast<int>(blockDim.x), lane = GROUP ? threadIdx.x % GROUP : threadIdx.x;
+    __shared__ float red[2][GROUP ? 1 : 64 * R];
+    const int lane = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
     const int group = GROUP ? threadIdx.x / (GROUP ? GROUP : 1) : 0;
+    const Columns<V, P, GROUP> column;
     Pair w[E], dw[E], db[E];
     {
         Piece<T, V> raw[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int c = (i * lanes + lane) * V;
             raw[i].clear();
-            if (p.w != nullptr && c < p.N) raw[i].load(static_cast<const T*>(p.w) + c);
+            if (p.w != nullptr && column(i) < p.N) raw[i].load(static_cast<const T*>(p.w) + column(i));
         }
         values_of<T, V, P>(raw, w);
     }
@@ -247,87 +269,101 @@ __global__ void __launch_bounds__(GROUP ? kBlock : backward_threads(V)) layer_no
         dw[i] = db[i] = pair(0.0f, 0.0f);
         if (p.w == nullptr) w[i] = pair(1.0f, 1.0f);
     }
-    // what lies beyond the row stays 0 in x and dy, and with it in every sum but xh (-mean rstd), which only meets zeros
-    Piece<T, V> xr[P], gr[P];
-    float mean = 0.0f, rstd = 0.0f;
-    const auto load = [&](int64_t row) {
+    // what lies beyond the row stays 0 in x and dy, and with it in every sum but xh (-mean rstd), which only meets zeros;
+    // so do rows beyond the last
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kGroups * R);
+    int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + group;
+    const T* xp = static_cast<const T*>(p.x) + row0 * p.xs + column.first;
+    const T* gp = static_cast<const T*>(p.dy) + row0 * p.gs + column.first;
+    const T* sp = DSUM ? static_cast<const T*>(p.dsum) + row0 * p.ds + column.first : nullptr;
+    T* to = static_cast<T*>(p.dx) + row0 * p.N + column.first;
+    const int64_t x_step = step * p.xs, g_step = step * p.gs, s_step = step * p.ds, to_step = step * p.N;
+    Piece<T, V> xr[R][P], gr[R][P], sr[DSUM ? R : 1][P];
+    float mean[R], rstd[R];
+    const auto load = [&](int64_t at) {  // rows at + j kGroups, from the pointers
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int c = (i * lanes + lane) * V;
-            if (c < p.N) {
-                xr[i].load(static_cast<const T*>(p.x) + row * p.xs + c);
-                gr[i].load(static_cast<const T*>(p.dy) + row * p.gs + c);
-            } else {
-                xr[i].clear();
-                gr[i].clear();
+        for (int j = 0; j < R; ++j) {
+            const bool real = at + j * kGroups < p.rows;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                if (real && column(i) < p.N) {
+                    xr[j][i].load(xp + j * kGroups * p.xs + i * column.kNext);
+                    gr[j][i].load(gp + j * kGroups * p.gs + i * column.kNext);
+                    if constexpr (DSUM) sr[j][i].load(sp + j * kGroups * p.ds + i * column.kNext);
+                } else {
+                    xr[j][i].clear();
+                    gr[j][i].clear();
+                    if constexpr (DSUM) sr[j][i].clear();
+                }
             }
+            mean[j] = real ? __ldg(p.mean + at + j * kGroups) : 0.0f;
+            rstd[j] = real ? __ldg(p.rstd + at + j * kGroups) : 0.0f;
         }
-        mean = __ldg(p.mean + row);
-        rstd = __ldg(p.rstd + row);
     };
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups, last = p.rows - 1;
-    load(min(static_cast<int64_t>(blockIdx.x) * kGroups + group, last));
+    load(row0);
     int turn = 0;
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups; base < p.rows; base += step, turn ^= 1) {
-        const int64_t row = base + group;
-        Pair xh[E], g[E];
-        values_of<T, V, P>(xr, xh);
-        values_of<T, V, P>(gr, g);
-        const float rs = rstd;
-        const Pair nm = pair(-mean, -mean), r2 = pair(rs, rs);
-        if (base + step < p.rows) load(min(row + step, last));
-        const bool real = row < p.rows;
-        Pair s1 = pair(0.0f, 0.0f), s2 = s1;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kGroups * R); base < p.rows; base += step, row0 += step, to += to_step, turn ^= 1) {
+        Pair xh[R][E], g[R][E], d[DSUM ? R : 1][E];
+        float rs[R], v[2 * R];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            xh[i] = mul2(add2(xh[i], nm), r2);
-            if (GROUP == 0 || real) {
-                dw[i] = fma2(g[i], xh[i], dw[i]);
-                db[i] = add2(db[i], g[i]);
-            }
-            g[i] = mul2(g[i], w[i]);
-            s1 = add2(s1, g[i]);
-            s2 = fma2(g[i], xh[i], s2);
+        for (int j = 0; j < R; ++j) {
+            values_of<T, V, P>(xr[j], xh[j]);
+            values_of<T, V, P>(gr[j], g[j]);
+            if constexpr (DSUM) values_of<T, V, P>(sr[j], d[j]);
+            rs[j] = rstd[j];
+            const Pair nm = pair(-mean[j], -mean[j]), r2 = pair(rs[j], rs[j]);
+#pragma unroll
+            for (int i = 0; i < E; ++i) xh[j][i] = mul2(add2(xh[j][i], nm), r2);
         }
-        const float m1 = row_sum<GROUP>(both(s1), red[turn][0]) * p.inv_n, m2 = row_sum<GROUP>(both(s2), red[turn][1]) * p.inv_n;
-        const Pair a = pair(-m1, -m1), b = pair(-m2, -m2);
-#pragma unroll
-        for (int i = 0; i < E; ++i) g[i] = mul2(fma2(xh[i], b, add2(g[i], a)), r2);
-        if (p.dsum != nullptr) {
-            Piece<T, V> raw[P];
-            Pair d[E];
-            const T* from = static_cast<const T*>(p.dsum) + min(row, last) * p.ds;
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int c = (i * lanes + lane) * V;
-                raw[i].clear();
-                if (c < p.N) raw[i].load(from + c);
-            }
-            values_of<T, V, P>(raw, d);
-#pragma unroll
-            for (int i = 0; i < E; ++i) g[i] = add2(g[i], d[i]);
+        if (base + step < p.rows) {
+            xp += x_step;
+            gp += g_step;
+            if constexpr (DSUM) sp += s_step;
+            load(row0 + step);
         }
-        if (real) {
-            T* to = static_cast<T*>(p.dx) + row * p.N;
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int c = (i * lanes + lane) * V;
-                if (c < p.N) store_piece<T, V>(to + c, g, i);
+        for (int j = 0; j < R; ++j) {
+            Pair s1 = pair(0.0f, 0.0f), s2 = s1;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                dw[i] = fma2(g[j][i], xh[j][i], dw[i]);
+                db[i] = add2(db[i], g[j][i]);
+                g[j][i] = mul2(g[j][i], w[i]);
+                s1 = add2(s1, g[j][i]);
+                s2 = fma2(g[j][i], xh[j][i], s2);
             }
+            v[2 * j] = both(s1);
+            v[2 * j + 1] = both(s2);
+        }
+        row_sums<GROUP>(v, red[turn]);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const float m1 = v[2 * j] * p.inv_n, m2 = v[2 * j + 1] * p.inv_n;
+            const Pair a = pair(-m1, -m1), b = pair(-m2, -m2), r2 = pair(rs[j], rs[j]);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const Pair u = fma2(xh[j][i], b, add2(g[j][i], a));
+                if constexpr (DSUM) g[j][i] = fma2(u, r2, d[j][i]);
+                else g[j][i] = mul2(u, r2);
+            }
+            if (row0 + j * kGroups < p.rows)
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    if (column(i) < p.N) store_piece<T, V>(to + static_cast<int64_t>(j * kGroups) * p.N + i * column.kNext, g[j], i);
         }
     }
     if (p.part == nullptr) return;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        float* to = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + which) * p.N;
+        float* sums = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + which) * p.N;
         float v[2 * E];
 #pragma unroll
         for (int i = 0; i < E; ++i) unpair(which ? db[i] : dw[i], v[2 * i], v[2 * i + 1]);
         if constexpr (GROUP == 0) {
 #pragma unroll
             for (int e = 0; e < 2 * E; ++e) {
-                const int c = (e / V * lanes + lane) * V + e % V;
-                if (c < p.N) to[c] = v[e];
+                const int c = column(e / V) + e % V;
+                if (c < p.N) sums[c] = v[e];
             }
         } else {
             constexpr int kRow = GROUP * P * V;  // columns kept of a row
@@ -339,7 +375,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : backward_threads(V)) layer_no
                 float s = 0.0f;
 #pragma unroll 8
                 for (int k = 0; k < kGroups; ++k) s += joined[k * kRow + c];
-                to[c] = s;
+                sums[c] = s;
             }
         }
     }
@@ -387,24 +423,30 @@ __global__ void __launch_bounds__(kBlock) layer_norm_columns_kernel(const __grid
     p.part[(static_cast<int64_t>(blockIdx.y) * 2 + 1) * p.N + c] = db;
 }
 
-// Joins the blocks' sums: 32 columns a block, 32 warps over the parts.
+// Joins the blocks' sums: 8 columns a block (a sector of each part), 128 threads of each
+// over the parts.
+constexpr int kJoinColumns = 8, kJoinLanes = 128;
 template <typename T>
-__global__ void __launch_bounds__(1024) layer_norm_join_kernel(const float* part, int parts, int N, T* dw, T* db)
+__global__ void __launch_bounds__(kJoinColumns * kJoinLanes) layer_norm_join_kernel(const float* part, int parts, int N, T* dw, T* db)
 {
-    __shared__ float sums[32][33];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // of the 2 N
+    __shared__ float sums[kJoinLanes][kJoinColumns + 1];
+    const int at = threadIdx.x % kJoinColumns, lane = threadIdx.x / kJoinColumns;
+    const int64_t all = 2 * static_cast<int64_t>(N), c = static_cast<int64_t>(blockIdx.x) * kJoinColumns + at;
     wait_for_launches_before();
     float s = 0.0f;
-    if (c < 2 * static_cast<int64_t>(N))
-#pragma unroll 4
-        for (int k = warp; k < parts; k += 32) s += part[static_cast<int64_t>(k) * 2 * N + c];
-    sums[warp][lane] = s;
+    if (c < all)
+#pragma unroll 8
+        for (int k = lane; k < parts; k += kJoinLanes) s += part[k * all + c];
+    sums[lane][at] = s;
     __syncthreads();
-    s = sums[lane][warp];
+    if (threadIdx.x >= 32 * kJoinColumns) return;
+    const int column = threadIdx.x / 32;
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoinLanes / 32; ++k) s += sums[threadIdx.x % 32 + 32 * k][column];
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    const int64_t to = static_cast<int64_t>(blockIdx.x) * 32 + warp;
-    if (lane == 0 && to < 2 * static_cast<int64_t>(N)) {
+    const int64_t to = static_cast<int64_t>(blockIdx.x) * kJoinColumns + column;
+    if (threadIdx.x % 32 == 0 && to < all) {
         if (to < N) dw[to] = from_float<T>(s);
         else db[to - N] = from_float<T>(s);
     }
@@ -460,32 +502,34 @@ int forward(const ww_layer_norm_t& p, bool norm, const char* name, cudaStream_t 
     const NormParams f = params(p, norm);
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     const bool pieces = in_pieces(p, sizeof(T));
-    const RowForm form = row_form(p.N, pieces ? V : 1, 16, kForwardThreads);
-    const unsigned groups = form.group ? kBlock / form.group : 1;
-    const unsigned grid = static_cast<unsigned>((i64(p.rows) + groups - 1) / groups);
-    const auto go = [&](auto kernel) { kernel<<<grid, form.threads, 0, stream>>>(f); };
+    const RowForm form = row_form(p.N, pieces ? V : 1, 4, false);
+    const auto go = [&](auto kernel, int r) {
+        const int groups = (form.group ? kBlock / form.group : 1) * r;
+        kernel<<<static_cast<unsigned>((i64(p.rows) + groups - 1) / groups), form.threads, 0, stream>>>(f);
+    };
+#define WW_NORM(V, P, GROUP, R) go(layer_norm_kernel<T, V, P, GROUP, R>, R)
     const int id = form.group * 100 + form.pieces;
     if (form.threads == 0) layer_norm_long_kernel<T><<<p.rows, kLongBlock, 0, stream>>>(f);
     else if (!pieces)
         switch (id) {
-        case 3204: go(layer_norm_kernel<T, 1, 4, 32>); break;
-        case 3216: go(layer_norm_kernel<T, 1, 16, 32>); break;
-        case 4: go(layer_norm_kernel<T, 1, 4, 0>); break;
-        default: go(layer_norm_kernel<T, 1, 16, 0>); break;
+        case 3204: WW_NORM(1, 4, 32, 2); break;
+        case 3216: WW_NORM(1, 16, 32, 1); break;
+        case 8: WW_NORM(1, 8, 0, 1); break;
+        default: WW_NORM(1, 16, 0, 1); break;
         }
     else
         switch (id) {
-        case 401: go(layer_norm_kernel<T, V, 1, 4>); break;
-        case 801: go(layer_norm_kernel<T, V, 1, 8>); break;
-        case 1601: go(layer_norm_kernel<T, V, 1, 16>); break;
-        case 1603: go(layer_norm_kernel<T, V, 3, 16>); break;
-        case 3201: go(layer_norm_kernel<T, V, 1, 32>); break;
-        case 3202: go(layer_norm_kernel<T, V, 2, 32>); break;
-        case 3203: go(layer_norm_kernel<T, V, 3, 32>); break;
-        case 3204: go(layer_norm_kernel<T, V, 4, 32>); break;
-        case 2: go(layer_norm_kernel<T, V, 2, 0>); break;
-        default: go(layer_norm_kernel<T, V, 4, 0>); break;
+        case 401: WW_NORM(V, 1, 4, kForwardRows); break;
+        case 801: WW_NORM(V, 1, 8, kForwardRows); break;
+        case 1601: WW_NORM(V, 1, 16, kForwardRows); break;
+        case 1603: WW_NORM(V, 3, 16, 1); break;
+        case 3201: WW_NORM(V, 1, 32, kForwardRows); break;
+        case 3202: WW_NORM(V, 2, 32, kForwardRows / 2); break;
+        case 3203: WW_NORM(V, 3, 32, 1); break;
+        case 3204: WW_NORM(V, 4, 32, 1); break;
+        default: WW_NORM(V, 2, 0, 1); break;
         }
+#undef WW_NORM
     return launch_status(name);
 }
 
@@ -503,10 +547,12 @@ BackwardPlan backward_plan(const ww_layer_norm_t& p, int sms) noexcept
     BackwardPlan r;
     r.pieces = in_pieces(p, bytes);
     const int v = r.pieces ? 16 / bytes : 1;
-    r.form = row_form(p.N, v, r.pieces ? 3 : 16, backward_threads(v));
+    r.form = row_form(p.N, v, 2, true);
     const int groups = r.form.group ? kBlock / r.form.group : 1;
-    const int resident = r.form.threads == 0 ? 1 : std::max(1, (r.form.pieces > 4 ? 768 : 1024) / r.form.threads);
-    r.blocks = static_cast<int>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + groups - 1) / groups));
+    int resident = backward_blocks(r.form.pieces);
+    if (r.form.group == 0 && r.form.threads > 0) resident = std::max(1, (r.form.pieces == 8 ? WW_RES : 512) / r.form.threads);
+    const int at_once = groups * backward_rows(v, r.form.pieces, r.form.group);
+    r.blocks = static_cast<int>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + at_once - 1) / at_once));
     const int columns = (p.N + kBlock - 1) / kBlock;
     r.splits = std::max(1, std::min(p.rows, 4 * sms / columns));
     return r;
@@ -520,33 +566,38 @@ int backward(const ww_layer_norm_t& p, const BackwardPlan& plan, cudaStream_t st
     f.part = sums ? static_cast<float*>(p.workspace) : nullptr;
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     const RowForm& form = plan.form;
-    const auto go = [&](auto kernel) { kernel<<<plan.blocks, form.threads, 0, stream>>>(f); };
+    const auto go = [&](auto kernel, auto with_sum) {
+        if (p.dsum == nullptr) kernel<<<plan.blocks, form.threads, 0, stream>>>(f);
+        else with_sum<<<plan.blocks, form.threads, 0, stream>>>(f);
+    };
+#define WW_NORM(V, P, GROUP) \
+    go(layer_norm_backward_kernel<T, V, P, GROUP, backward_rows(V, P, GROUP), false>, \
+       layer_norm_backward_kernel<T, V, P, GROUP, backward_rows(V, P, GROUP), true>)
     const int id = form.group * 100 + form.pieces;
     if (form.threads == 0) {
         layer_norm_backward_long_kernel<T><<<p.rows, kLongBlock, 0, stream>>>(f);
         if (sums) layer_norm_columns_kernel<T><<<dim3((p.N + kBlock - 1) / kBlock, plan.splits), kBlock, 0, stream>>>(f);
     } else if (!plan.pieces) {
         switch (id) {
-        case 3204: go(layer_norm_backward_kernel<T, 1, 4, 32>); break;
-        case 3216: go(layer_norm_backward_kernel<T, 1, 16, 32>); break;
-        case 4: go(layer_norm_backward_kernel<T, 1, 4, 0>); break;
-        default: go(layer_norm_backward_kernel<T, 1, 16, 0>); break;
+        case 3204: WW_NORM(1, 4, 32); break;
+        case 3216: WW_NORM(1, 16, 32); break;
+        case 8: WW_NORM(1, 8, 0); break;
+        default: WW_NORM(1, 16, 0); break;
         }
     } else {
         switch (id) {
-        case 401: go(layer_norm_backward_kernel<T, V, 1, 4>); break;
-        case 801: go(layer_norm_backward_kernel<T, V, 1, 8>); break;
-        case 1601: go(layer_norm_backward_kernel<T, V, 1, 16>); break;
-        case 1603: go(layer_norm_backward_kernel<T, V, 3, 16>); break;
-        case 3201: go(layer_norm_backward_kernel<T, V, 1, 32>); break;
-        case 3202: go(layer_norm_backward_kernel<T, V, 2, 32>); break;
-        case 3203: go(layer_norm_backward_kernel<T, V, 3, 32>); break;
-        default: go(layer_norm_backward_kernel<T, V, 2, 0>); break;
+        case 401: WW_NORM(V, 1, 4); break;
+        case 801: WW_NORM(V, 1, 8); break;
+        case 1601: WW_NORM(V, 1, 16); break;
+        case 3201: WW_NORM(V, 1, 32); break;
+        case 3202: WW_NORM(V, 2, 32); break;
+        default: WW_NORM(V, 2, 0); break;
         }
     }
+#undef WW_NORM
     const int st = launch_status("layer_norm_backward");
     if (st != WW_SUCCESS || !sums) return st;
-    launch_behind(layer_norm_join_kernel<T>, dim3((2u * p.N + 31) / 32), dim3(1024), 0, stream, f.part, plan.parts(), p.N,
+    launch_behind(layer_norm_join_kernel<T>, dim3((2u * p.N + kJoinColumns - 1) / kJoinColumns), dim3(kJoinColumns * kJoinLanes), 0, stream, f.part, plan.parts(), p.N,
                   static_cast<T*>(p.dweight), static_cast<T*>(p.dbias));
     return launch_status("layer_norm_backward");
 }

@@ -109,6 +109,32 @@ __device__ __forceinline__ void values_of(const Piece<T, V> (&raw)[P], Pair (&f)
     }
 }
 
+// Columns of a lane's pieces: piece i begins at `first` + i kNext, side by side over the lanes
+// of a group or, where a block holds the row, of a warp (whose pieces follow one another).
+template <int V, int P, int GROUP>
+struct Columns {
+    static constexpr int kNext = (GROUP ? GROUP : 32) * V;
+    int first;
+    __device__ __forceinline__ Columns()
+        : first(GROUP ? threadIdx.x % (GROUP ? GROUP : 1) * V : threadIdx.x / 32 * (P * kNext) + threadIdx.x % 32 * V) {}
+    __device__ __forceinline__ int operator()(int i) const { return first + i * kNext; }
+};
+
+// What a lane holds beyond the n values of its row becomes 0.
+template <int V, int P, int GROUP>
+__device__ __forceinline__ void clear_beyond(Pair (&f)[P * V / 2], int n, const Columns<V, P, GROUP>& column)
+{
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+        if (column(i) >= n)
+#pragma unroll
+            for (int e = i * V; e < (i + 1) * V; ++e) {
+                float a, b;
+                unpair(f[e / 2], a, b);
+                f[e / 2] = e % 2 ? pair(a, 0.0f) : pair(0.0f, b);
+            }
+}
+
 // Piece i of a lane's values to memory.
 template <typename T, int V, int E>
 __device__ __forceinline__ void store_piece(T* p, const Pair (&f)[E], int i)
@@ -155,37 +181,81 @@ __device__ __forceinline__ float both(Pair p)
     return a + b;
 }
 
-// Sum over the GROUP lanes of a row; GROUP 0: over the block, in a fixed order (`red`: 32
-// floats of shared memory that no other sum under way uses; one barrier).
+// K sums, or largest values (NaN above all), over the GROUP lanes of a row; GROUP 0: over
+// the block, in a fixed order (`red`: 32 K floats of shared memory that no other call
+// under way uses; one barrier).
+template <int GROUP, bool MAX, int K>
+__device__ __forceinline__ void row_joins(float (&v)[K], float* red)
+{
+    const auto join = [](float a, float b) { return MAX ? max_nan(a, b) : a + b; };
+#pragma unroll
+    for (int o = (GROUP ? GROUP : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = join(v[k], __shfl_xor_sync(~0u, v[k], o));
+    if constexpr (GROUP == 0) {
+        if (threadIdx.x % 32 == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[k * 32 + threadIdx.x / 32] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = threadIdx.x % 32 < blockDim.x / 32 ? red[k * 32 + threadIdx.x % 32] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] = join(v[k], __shfl_xor_sync(~0u, v[k], o));
+    }
+}
+
+template <int GROUP, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float* red)
+{
+    row_joins<GROUP, false, K>(v, red);
+}
+
+template <int GROUP, int K>
+__device__ __forceinline__ void row_maxima(float (&v)[K], float* red)
+{
+    row_joins<GROUP, true, K>(v, red);
+}
+
 template <int GROUP>
 __device__ __forceinline__ float row_sum(float v, float* red)
 {
-#pragma unroll
-    for (int o = (GROUP ? GROUP : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    if constexpr (GROUP == 0) {
-        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-        __syncthreads();
-        v = threadIdx.x % 32 < blockDim.x / 32 ? red[threadIdx.x % 32] : 0.0f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    }
-    return v;
+    float x[1] = {v};
+    row_sums<GROUP>(x, red);
+    return x[0];
 }
 
-// Largest magnitude of a row's values, NaN if there is one.
 template <int GROUP>
 __device__ __forceinline__ float row_max(float v, float* red)
 {
+    float x[1] = {v};
+    row_maxima<GROUP>(x, red);
+    return x[0];
+}
+
+// Scales of the K <= GROUP rows that a group of lanes holds (GROUP 0: of a block's warp), whose
+// largest magnitudes every lane has: lane k divides for row k (a division costs as much as
+// bringing several values to 8 bits), the others get its quotients.
+template <int GROUP, int K>
+__device__ __forceinline__ void row_scales(const float (&top)[K], RowScale (&r)[K])
+{
+    if constexpr (K == 1) {
+        r[0] = row_scale(top[0]);
+    } else {
+        constexpr int kLanes = GROUP ? GROUP : 32;
+        static_assert(K <= kLanes, "a lane for each row");
+        const int lane = threadIdx.x % kLanes;
+        float mine = top[0];
 #pragma unroll
-    for (int o = (GROUP ? GROUP : 32) / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
-    if constexpr (GROUP == 0) {
-        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-        __syncthreads();
-        v = threadIdx.x % 32 < blockDim.x / 32 ? red[threadIdx.x % 32] : 0.0f;
+        for (int k = 1; k < K; ++k) mine = lane == k ? top[k] : mine;
+        const RowScale own = row_scale(mine);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+        for (int k = 0; k < K; ++k) {
+            r[k].inv = __shfl_sync(~0u, own.inv, k, kLanes);
+            r[k].scale = __shfl_sync(~0u, own.scale, k, kLanes);
+        }
     }
-    return v;
 }
 
 template <int E>
@@ -207,25 +277,27 @@ struct RowForm {
     int group, pieces, threads;
 };
 
+// Most threads of a block that holds a row, P pieces of V values a lane.
+__host__ __device__ constexpr int row_threads(int v, int p, bool backward) { return v > 1 ? (backward ? 512 : 1024) : p == 8 ? 256 : 640; }
+
 // Pieces of 16 bytes (v > 1): the form with the fewest idle lanes, and of those the one
-// with the fewest pieces a lane (at most `most`).  Single values (v == 1, rows that do
-// not start on 16 bytes): 4 or 16 a lane.  Rows that a warp does not hold: a block of up
-// to `threads` threads.
-inline RowForm row_form(int n, int v, int most, int threads)
+// with the fewest pieces a lane (at most `most` in a warp).  Single values (v == 1, rows that
+// do not start on 16 bytes): 4, 8 or 16 a lane.  Rows that a warp does not hold: a block.
+inline RowForm row_form(int n, int v, int most, bool backward)
 {
     const int all = (n + v - 1) / v;
+    const auto fits = [&](int p) { return all <= row_threads(v, p, backward) * p; };
     const auto block = [&](int p) { return RowForm{0, p, ((all + p - 1) / p + 31) / 32 * 32}; };
     if (v > 1) {
-        static constexpr int kForms[][2] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {16, 3}, {32, 2}, {32, 3}, {32, 4}};
+        constexpr int kForms[][2] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {16, 3}, {32, 2}, {32, 3}, {32, 4}};
         for (const auto& f : kForms)  // ascending lanes x pieces
             if (f[0] * f[1] >= all && f[1] <= most) return {f[0], f[1], 256};
-        for (int p = 2; p <= most && p <= 4; p *= 2)
-            if (all <= threads * p) return block(p);
+        if (fits(2)) return block(2);
     } else {
         if (n <= 128) return {32, 4, 256};
         if (n <= 512) return {32, 16, 256};
-        for (int p = 4; p <= 16; p *= 4)
-            if (all <= threads * p) return block(p);
+        for (int p : {8, 16})
+            if (fits(p)) return block(p);
     }
     return {0, 0, 0};
 }
