@@ -52,13 +52,13 @@ struct Tiles {
     static constexpr int kA = kTileM * kBlockK;
     static constexpr int kB = (PAIR ? BN / 2 : BN) * kBlockK;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = 5;
+    static constexpr int kStages = BN == 64 ? 5 : 4;
     static constexpr int kColumns = BN / 2;  // of an epilogue warp
     static constexpr int kChunk = kColumns < 128 / static_cast<int>(sizeof(O)) ? kColumns : 128 / static_cast<int>(sizeof(O));
     static constexpr int kChunkRow = kChunk * static_cast<int>(sizeof(O));  // 64 or 128 bytes
-    static constexpr int kStaging = 32 * kChunkRow;
+    static constexpr int kStaging = 32 * kChunkRow;  // of a warp, twice
     static constexpr int kOut = kStages * kStage;
-    static constexpr int kScales = kOut + kEpilogueWarps * kStaging;
+    static constexpr int kScales = kOut + kEpilogueWarps * 2 * kStaging;
     static constexpr int kBar = kScales + kEpilogueWarps * kColumns * 8;
     static constexpr int kBytes = kBar + (2 * kStages + 4) * 8 + 16 + 1024;
     static constexpr int kTmem = 2 * BN;
@@ -281,30 +281,45 @@ __global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_c
         }
     } else if (warp >= 4) {  // results
         const int quarter = warp % 4, half = warp / 4 - 1, w = warp - 4;
-        const uint32_t staging = sm + L::kOut + w * L::kStaging;
+        constexpr int kMine = L::kColumns / 32;  // columns of a lane whose scales it brings
         const uint32_t bar = PAIR ? in_block(freed, 0) : freed;
         float* scales = reinterpret_cast<float*>(base + L::kScales) + w * 2 * L::kColumns;  // [columns] of ws, of the bias
-        int i = 0;
-        for (int t = start; t < tiles && ok; t += step, ++i) {
+        int row0, column0, buffer = 0;
+        float ws[kMine], bs[kMine], xs;
+        const auto ahead = [&](int t) {
             int m, n;
             tile_at(p, t, m, n);
-            const int row0 = (m * (PAIR ? 2 : 1) + static_cast<int>(rank)) * kTileM + quarter * 32, column0 = n * BN + half * L::kColumns;
-            __syncwarp();  // the scales before have been read
-            for (int c = lane; c < L::kColumns; c += 32) {
-                const bool in = column0 + c < p.N;
-                scales[c] = in ? __ldg(p.ws + column0 + c) : 0.0f;
-                scales[L::kColumns + c] = in && p.bias != nullptr ? to_float(static_cast<const O*>(p.bias)[column0 + c]) : 0.0f;
+            row0 = (m * (PAIR ? 2 : 1) + static_cast<int>(rank)) * kTileM + quarter * 32;
+            column0 = n * BN + half * L::kColumns;
+#pragma unroll
+            for (int c = 0; c < kMine; ++c) {
+                const int x = column0 + c * 32 + lane;
+                ws[c] = x < p.N ? __ldg(p.ws + x) : 0.0f;
+                bs[c] = x < p.N && p.bias != nullptr ? to_float(static_cast<const O*>(p.bias)[x]) : 0.0f;
             }
-            const float xs = row0 + lane < p.M ? __ldg(p.xs + row0 + lane) : 0.0f;
-            const Pair x2 = pair(xs, xs);
+            xs = row0 + lane < p.M ? __ldg(p.xs + row0 + lane) : 0.0f;
+        };
+        if (start < tiles) ahead(start);
+        int i = 0;
+        for (int t = start; t < tiles && ok; t += step, ++i) {
+            __syncwarp();  // the scales before have been read
+#pragma unroll
+            for (int c = 0; c < kMine; ++c) {
+                scales[c * 32 + lane] = ws[c];
+                scales[L::kColumns + c * 32 + lane] = bs[c];
+            }
             __syncwarp();
+            const Pair x2 = pair(xs, xs);
+            const int my_row0 = row0, my_column0 = column0;
+            if (t + step < tiles) ahead(t + step);
             ok = wait(done + (i & 1) * 8, (i >> 1) & 1);
             umma::fence_after_sync();
             if (!ok) break;
             const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * BN + half * L::kColumns;
 #pragma unroll 1
-            for (int c = 0; c < L::kColumns; c += L::kChunk) {
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" : : : "memory");
+            for (int c = 0; c < L::kColumns; c += L::kChunk, buffer ^= 1) {
+                const int my_out = L::kOut + (w * 2 + buffer) * L::kStaging;
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" : : : "memory");
                 __syncwarp();
 #pragma unroll
                 for (int e = 0; e < L::kChunk; e += 32) {
@@ -333,23 +348,23 @@ __global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_c
                         // 16-byte piece of the row, swizzled as the TMA store reads it
                         const int piece = (e + j) * static_cast<int>(sizeof(O)) / 16;
                         const int turn = L::kChunkRow == 128 ? lane & 7 : (lane >> 1) & 3;
-                        const uint32_t at = staging + lane * L::kChunkRow;
+                        const uint32_t at = sm + my_out + lane * L::kChunkRow;
                         pack_row<O>(f, at + ((piece ^ turn) << 4), at + (((piece + 1) ^ turn) << 4));
                     }
                 }
-                const int x = column0 + c;
+                const int x = my_column0 + c;
                 if (p.stored) {
                     umma::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0 && x < p.N && row0 < p.M) store_tile(&p.c, staging, x, row0);
+                    if (lane == 0 && x < p.N && my_row0 < p.M) store_tile(&p.c, sm + my_out, x, my_row0);
                 } else {  // rows that do not start on 16 bytes
                     __syncwarp();
-                    for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+                    for (int r = 0; r < 32 && my_row0 + r < p.M; ++r) {
                         const int turn = L::kChunkRow == 128 ? r & 7 : (r >> 1) & 3;
                         for (int e = lane; e < L::kChunk && x + e < p.N; e += 32) {
                             const int byte = e * static_cast<int>(sizeof(O));
-                            const uint8_t* v = base + L::kOut + w * L::kStaging + r * L::kChunkRow + (((byte >> 4) ^ turn) << 4) + (byte & 15);
-                            static_cast<O*>(p.out)[static_cast<int64_t>(row0 + r) * p.N + x + e] = *reinterpret_cast<const O*>(v);
+                            const uint8_t* v = base + my_out + r * L::kChunkRow + (((byte >> 4) ^ turn) << 4) + (byte & 15);
+                            static_cast<O*>(p.out)[static_cast<int64_t>(my_row0 + r) * p.N + x + e] = *reinterpret_cast<const O*>(v);
                         }
                     }
                     __syncwarp();

@@ -43,7 +43,12 @@ constexpr int kLongBlock = 1024;
 #ifndef WW_BBLOCKS
 #define WW_BBLOCKS 2
 #endif
+#ifndef WW_FBLOCKS
+#define WW_FBLOCKS 4
+#endif
 constexpr int kForwardRows = WW_ROWS, kBackwardRows = WW_BROWS;
+__host__ __device__ constexpr int forward_rows(int v, int pieces, int group) { return v > 1 && pieces == 1 && group > 0 ? kForwardRows : 1; }
+__host__ __device__ constexpr int forward_blocks(int pieces) { return pieces == 1 ? WW_FBLOCKS : pieces < 4 ? 3 : 2; }
 // Rows of a group under way in the gradient's kernel, and resident blocks of it.
 __host__ __device__ constexpr int backward_rows(int v, int pieces, int group) { return v > 1 && pieces == 1 && group > 0 ? kBackwardRows : 1; }
 __host__ __device__ constexpr int backward_blocks(int pieces) { return pieces == 1 ? WW_BBLOCKS : 2; }
@@ -61,139 +66,147 @@ struct NormParams {
     float eps, inv_n;
 };
 
-// R rows of a group of lanes are under way at a time.
-template <typename T, int V, int P, int GROUP, int R>
-__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), 1) layer_norm_kernel(const __grid_constant__ NormParams p)
+// R rows of a group of lanes at a time, those of the block's next step loaded ahead.
+template <typename T, int V, int P, int GROUP, int R, bool RES>
+__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GROUP ? forward_blocks(P) : 1)
+    layer_norm_kernel(const __grid_constant__ NormParams p)
 {
-    __shared__ float red[GROUP ? 1 : 3][32 * R];
+    __shared__ float red[2][GROUP ? 1 : 3][32 * R];
     constexpr int E = P * V / 2;
     constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block side by side
     const int lane = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
     const Columns<V, P, GROUP> column;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + (GROUP ? threadIdx.x / (GROUP ? GROUP : 1) : 0);
-    const auto row_of = [&](int j) { return row0 + j * kGroups; };
-    const auto known = [&](int j) { return min(row_of(j), static_cast<int64_t>(p.rows) - 1); };
-    Pair f[R][E];
-    {
-        Piece<T, V> raw[R][P];
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kGroups * R);
+    int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + (GROUP ? threadIdx.x / (GROUP ? GROUP : 1) : 0);
+    const T* xp = static_cast<const T*>(p.x) + row0 * p.xs + column.first;
+    const T* rp = RES ? static_cast<const T*>(p.r) + row0 * p.rs + column.first : nullptr;
+    // weights: kept where they are few, else from L1 for each row
+    constexpr bool kKeep = E <= 4;
+    Pair w[E], b[E];
+    const auto weights = [&] {
+        Piece<T, V> wr[P], br[P];
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const T* x = static_cast<const T*>(p.x) + known(j) * p.xs;
+        for (int i = 0; i < P; ++i) {
+            wr[i].clear();
+            br[i].clear();
+            if (p.w != nullptr && column(i) < p.N) {
+                wr[i].load(static_cast<const T*>(p.w) + column(i));
+                if (p.b != nullptr) br[i].load(static_cast<const T*>(p.b) + column(i));
+            }
+        }
+        values_of<T, V, P>(wr, w);
+        values_of<T, V, P>(br, b);
+        if (p.w == nullptr)
+#pragma unroll
+            for (int i = 0; i < E; ++i) w[i] = pair(1.0f, 1.0f);
+    };
+    if (kKeep) weights();
+    // what lies beyond a row, and rows beyond the last, are zeros
+    Piece<T, V> xr[R][P], rr[RES ? R : 1][P];
+    const auto load = [&](int64_t at) {
+#pragma unroll
+        for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (column(i) < p.N) raw[j][i].load(x + column(i));
-                else raw[j][i].clear();
-        }
-        if (p.r == nullptr) {
+                if (at + j * kGroups < p.rows && column(i) < p.N) {
+                    xr[j][i].load(xp + j * kGroups * p.xs + i * column.kNext);
+                    if constexpr (RES) rr[j][i].load(rp + j * kGroups * p.rs + i * column.kNext);
+                } else {
+                    xr[j][i].clear();
+                    if constexpr (RES) rr[j][i].clear();
+                }
+    };
+    load(row0);
+    int turn = 0;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kGroups * R); base < p.rows; base += step, row0 += step, turn ^= 1) {
+        Pair f[R][E];
+        const auto real = [&](int j) { return row0 + j * kGroups < p.rows; };
 #pragma unroll
-            for (int j = 0; j < R; ++j) values_of<T, V, P>(raw[j], f[j]);
-        } else {
-            Piece<T, V> more[R][P];
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                const T* r = static_cast<const T*>(p.r) + known(j) * p.rs;
-#pragma unroll
-                for (int i = 0; i < P; ++i)
-                    if (column(i) < p.N) more[j][i].load(r + column(i));
-                    else more[j][i].clear();
-            }
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                values_of<T, V, P>(raw[j], f[j]);
+        for (int j = 0; j < R; ++j) {
+            values_of<T, V, P>(xr[j], f[j]);
+            if constexpr (RES) {
                 Pair g[E];
-                values_of<T, V, P>(more[j], g);
+                values_of<T, V, P>(rr[j], g);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    float a, b;
-                    unpair(add2(f[j][i], g[i]), a, b);
-                    f[j][i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(b)));
-                }
-                if (p.sum != nullptr && row_of(j) < p.rows) {
-                    T* to = static_cast<T*>(p.sum) + row_of(j) * p.N;
-#pragma unroll
-                    for (int i = 0; i < P; ++i)
-                        if (column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
+                    float a, c;
+                    unpair(add2(f[j][i], g[i]), a, c);
+                    f[j][i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(c)));
                 }
             }
         }
-    }
-    if (p.norm) {
-        float v[R];
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            Pair s = f[j][0];
-#pragma unroll
-            for (int i = 1; i < E; ++i) s = add2(s, f[j][i]);
-            v[j] = both(s);
+        if (base + step < p.rows) {
+            xp += step * p.xs;
+            if constexpr (RES) rp += step * p.rs;
+            load(row0 + step);
         }
-        row_sums<GROUP>(v, red[0]);
+        if (RES && p.sum != nullptr)
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const float mean = v[j] * p.inv_n;
-            if (lane == 0 && p.mean != nullptr && row_of(j) < p.rows) p.mean[row_of(j)] = mean;
-            const Pair nm = pair(-mean, -mean);
+            for (int j = 0; j < R; ++j) {
+                T* to = static_cast<T*>(p.sum) + (row0 + j * kGroups) * p.N;
 #pragma unroll
-            for (int i = 0; i < E; ++i) f[j][i] = add2(f[j][i], nm);
-            clear_beyond(f[j], p.N, column);
-            Pair s = mul2(f[j][0], f[j][0]);
-#pragma unroll
-            for (int i = 1; i < E; ++i) s = fma2(f[j][i], f[j][i], s);
-            v[j] = both(s);
-        }
-        row_sums<GROUP>(v, red[GROUP ? 0 : 1]);
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const float rstd = rsqrtf(fmaf(v[j], p.inv_n, p.eps));
-            if (lane == 0 && p.rstd != nullptr && row_of(j) < p.rows) p.rstd[row_of(j)] = rstd;
-            const Pair r2 = pair(rstd, rstd);
-#pragma unroll
-            for (int i = 0; i < E; ++i) f[j][i] = mul2(f[j][i], r2);
-        }
-        if (p.w != nullptr) {
-            Piece<T, V> wr[P], br[P];
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                wr[i].clear();
-                br[i].clear();
-                if (column(i) < p.N) {
-                    wr[i].load(static_cast<const T*>(p.w) + column(i));
-                    if (p.b != nullptr) br[i].load(static_cast<const T*>(p.b) + column(i));
-                }
+                for (int i = 0; i < P; ++i)
+                    if (real(j) && column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
             }
-            Pair w[E], b[E];
-            values_of<T, V, P>(wr, w);
-            values_of<T, V, P>(br, b);
+        if (p.norm) {
+            float v[R];
 #pragma unroll
-            for (int j = 0; j < R; ++j)
+            for (int j = 0; j < R; ++j) {
+                Pair s = f[j][0];
 #pragma unroll
-                for (int i = 0; i < E; ++i) f[j][i] = fma2(f[j][i], w[i], b[i]);
+                for (int i = 1; i < E; ++i) s = add2(s, f[j][i]);
+                v[j] = both(s);
+            }
+            row_sums<GROUP>(v, red[turn][0]);
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const float mean = v[j] * p.inv_n;
+                if (lane == 0 && p.mean != nullptr && real(j)) p.mean[row0 + j * kGroups] = mean;
+                const Pair nm = pair(-mean, -mean);
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[j][i] = add2(f[j][i], nm);
+                clear_beyond(f[j], p.N, column);
+                Pair s = mul2(f[j][0], f[j][0]);
+#pragma unroll
+                for (int i = 1; i < E; ++i) s = fma2(f[j][i], f[j][i], s);
+                v[j] = both(s);
+            }
+            row_sums<GROUP>(v, red[turn][GROUP ? 0 : 1]);
+            if (!kKeep) weights();
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const float rstd = rsqrtf(fmaf(v[j], p.inv_n, p.eps));
+                if (lane == 0 && p.rstd != nullptr && real(j)) p.rstd[row0 + j * kGroups] = rstd;
+                const Pair r2 = pair(rstd, rstd);
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[j][i] = fma2(mul2(f[j][i], r2), w[i], b[i]);
+            }
         }
-    }
-    if (p.q != nullptr) {
-        float top[R];
-        RowScale k[R];
+        if (p.q != nullptr) {
+            float top[R];
+            RowScale k[R];
 #pragma unroll
-        for (int j = 0; j < R; ++j) top[j] = largest(f[j]);
-        row_maxima<GROUP>(top, red[GROUP ? 0 : 2]);
-        row_scales<GROUP>(top, k);
+            for (int j = 0; j < R; ++j) top[j] = largest(f[j]);
+            row_maxima<GROUP>(top, red[turn][GROUP ? 0 : 2]);
+            row_scales<GROUP>(top, k);
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            if (row_of(j) >= p.rows) continue;
-            if (lane == 0) p.scale[row_of(j)] = k[j].scale;
-            int8_t* to = p.q + row_of(j) * p.qs;
+            for (int j = 0; j < R; ++j) {
+                if (!real(j)) continue;
+                if (lane == 0) p.scale[row0 + j * kGroups] = k[j].scale;
+                int8_t* to = p.q + (row0 + j * kGroups) * p.qs;
 #pragma unroll
-            for (int i = 0; i < P; ++i)
-                if (column(i) < p.N) store_piece_int8<V>(to + column(i), f[j], k[j].inv, i);
+                for (int i = 0; i < P; ++i)
+                    if (column(i) < p.N) store_piece_int8<V>(to + column(i), f[j], k[j].inv, i);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                T* to = static_cast<T*>(p.y) + (row0 + j * kGroups) * p.N;
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    if (real(j) && column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
+            }
         }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        if (row_of(j) >= p.rows) continue;
-        T* to = static_cast<T*>(p.y) + row_of(j) * p.N;
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
     }
 }
 
@@ -497,37 +510,42 @@ NormParams params(const ww_layer_norm_t& p, bool norm) noexcept
 }
 
 template <typename T>
-int forward(const ww_layer_norm_t& p, bool norm, const char* name, cudaStream_t stream) noexcept
+int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cudaStream_t stream) noexcept
 {
     const NormParams f = params(p, norm);
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     const bool pieces = in_pieces(p, sizeof(T));
     const RowForm form = row_form(p.N, pieces ? V : 1, 4, false);
-    const auto go = [&](auto kernel, int r) {
+    const auto go = [&](auto kernel, auto with_residual, int r) {
         const int groups = (form.group ? kBlock / form.group : 1) * r;
-        kernel<<<static_cast<unsigned>((i64(p.rows) + groups - 1) / groups), form.threads, 0, stream>>>(f);
+        const int resident = form.group ? forward_blocks(form.pieces) : std::max(1, (pieces ? 1024 : 768) / form.threads);
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + groups - 1) / groups));
+        if (p.residual == nullptr) kernel<<<grid, form.threads, 0, stream>>>(f);
+        else with_residual<<<grid, form.threads, 0, stream>>>(f);
     };
-#define WW_NORM(V, P, GROUP, R) go(layer_norm_kernel<T, V, P, GROUP, R>, R)
+#define WW_NORM(V, P, GROUP) \
+    go(layer_norm_kernel<T, V, P, GROUP, forward_rows(V, P, GROUP), false>, layer_norm_kernel<T, V, P, GROUP, forward_rows(V, P, GROUP), true>, \
+       forward_rows(V, P, GROUP))
     const int id = form.group * 100 + form.pieces;
     if (form.threads == 0) layer_norm_long_kernel<T><<<p.rows, kLongBlock, 0, stream>>>(f);
     else if (!pieces)
         switch (id) {
-        case 3204: WW_NORM(1, 4, 32, 2); break;
-        case 3216: WW_NORM(1, 16, 32, 1); break;
-        case 8: WW_NORM(1, 8, 0, 1); break;
-        default: WW_NORM(1, 16, 0, 1); break;
+        case 3204: WW_NORM(1, 4, 32); break;
+        case 3216: WW_NORM(1, 16, 32); break;
+        case 8: WW_NORM(1, 8, 0); break;
+        default: WW_NORM(1, 16, 0); break;
         }
     else
         switch (id) {
-        case 401: WW_NORM(V, 1, 4, kForwardRows); break;
-        case 801: WW_NORM(V, 1, 8, kForwardRows); break;
-        case 1601: WW_NORM(V, 1, 16, kForwardRows); break;
-        case 1603: WW_NORM(V, 3, 16, 1); break;
-        case 3201: WW_NORM(V, 1, 32, kForwardRows); break;
-        case 3202: WW_NORM(V, 2, 32, kForwardRows / 2); break;
-        case 3203: WW_NORM(V, 3, 32, 1); break;
-        case 3204: WW_NORM(V, 4, 32, 1); break;
-        default: WW_NORM(V, 2, 0, 1); break;
+        case 401: WW_NORM(V, 1, 4); break;
+        case 801: WW_NORM(V, 1, 8); break;
+        case 1601: WW_NORM(V, 1, 16); break;
+        case 1603: WW_NORM(V, 3, 16); break;
+        case 3201: WW_NORM(V, 1, 32); break;
+        case 3202: WW_NORM(V, 2, 32); break;
+        case 3203: WW_NORM(V, 3, 32); break;
+        case 3204: WW_NORM(V, 4, 32); break;
+        default: WW_NORM(V, 2, 0); break;
         }
 #undef WW_NORM
     return launch_status(name);
@@ -638,8 +656,8 @@ int run_forward(const ww_layer_norm_t& p, bool norm, const char* name, void* str
     const int st = current_device_info(&d);
     if (st != WW_SUCCESS) return st;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return p.dtype == WW_DTYPE_HALF ? forward<__half>(p, norm, name, s)
-         : p.dtype == WW_DTYPE_BF16 ? forward<__nv_bfloat16>(p, norm, name, s) : forward<float>(p, norm, name, s);
+    return p.dtype == WW_DTYPE_HALF ? forward<__half>(p, norm, d.sm_count, name, s)
+         : p.dtype == WW_DTYPE_BF16 ? forward<__nv_bfloat16>(p, norm, d.sm_count, name, s) : forward<float>(p, norm, d.sm_count, name, s);
 }
 
 int sm_count() noexcept
