@@ -7,8 +7,8 @@
 // shares of K change a result; (sum xs) ws + bias in fp32, one rounding to the output's type.
 //
 // Tiles: tcgen05 kind::i8, accumulators in TMEM, operands by TMA in swizzled rows
-// of 128 bytes.  One producer warp, one warp that issues, eight that write out: each
-// takes 32 rows and half the columns of a tile, from TMEM through shared memory to a TMA
+// of 128 bytes.  One producer warp, one warp that issues, 16 (8 for narrow tiles) that
+// write out: each takes 32 rows and 32 or 64 columns of a tile, from TMEM through shared memory to a TMA
 // store, while the next tile's products run into the other half of TMEM.
 // Blocks are persistent; tiles go in bands of rows so that operands are read from L2.
 // Large products take two SMs for a 256 x 256 tile (cta_group::2): each holds half
@@ -32,8 +32,6 @@ namespace {
 
 constexpr int kBlockK = 128;  // bytes of a row of a stage
 constexpr int kTileM = 128;   // rows of an SM's tile
-constexpr int kThreads = 384;
-constexpr int kEpilogueWarps = 8;
 
 struct MatmulParams {
     CUtensorMap a, b, c;
@@ -52,18 +50,20 @@ struct Tiles {
     static constexpr int kA = kTileM * kBlockK;
     static constexpr int kB = (PAIR ? BN / 2 : BN) * kBlockK;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = BN == 64 ? 5 : 4;
-    static constexpr int kColumns = BN / 2;  // of an epilogue warp
-    static constexpr int kChunk = kColumns < 128 / static_cast<int>(sizeof(O)) ? kColumns : 128 / static_cast<int>(sizeof(O));
-    static constexpr int kChunkRow = kChunk * static_cast<int>(sizeof(O));  // 64 or 128 bytes
-    static constexpr int kStaging = 32 * kChunkRow;  // of a warp, twice
+    static constexpr int kStages = BN == 64 ? 6 : sizeof(O) == 2 ? 5 : 4;
+    static constexpr int kWarps = BN == 64 ? 8 : 16;  // that write out
+    static constexpr int kThreads = 128 + 32 * kWarps;
+    static constexpr int kColumns = BN * 4 / kWarps;  // of such a warp
+    static constexpr int kChunk = 32;                      // of them staged at a time
+    static constexpr int kChunkRow = kChunk * sizeof(O);   // 64 or 128 bytes
+    static constexpr int kStaging = 32 * kChunkRow;
+    static constexpr int kBuffers = BN == 64 ? 2 : 1;  // of a warp
     static constexpr int kOut = kStages * kStage;
-    static constexpr int kScales = kOut + kEpilogueWarps * 2 * kStaging;
-    static constexpr int kBar = kScales + kEpilogueWarps * kColumns * 8;
+    static constexpr int kScales = kOut + kWarps * kBuffers * kStaging;
+    static constexpr int kBar = kScales + kWarps * kColumns * 8;
     static constexpr int kBytes = kBar + (2 * kStages + 4) * 8 + 16 + 1024;
     static constexpr int kTmem = 2 * BN;
     static_assert(kBytes <= kMaxShared, "shared memory");
-    static_assert(kChunkRow == 64 || kChunkRow == 128, "rows of a swizzle");
 };
 
 // ---- instructions of a pair of SMs ----
@@ -88,9 +88,12 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" : : : "memory");
 }
 
+// Tells the other SM that this one's tensor memory has been read.  Relaxed: the reads are in
+// registers (tcgen05.wait::ld), nothing written here is read there; a release would wait
+// for the stores to memory under way (1700 clocks of 5000 a tile).
 __device__ __forceinline__ void arrive_cluster(uint32_t bar)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" : : "r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" : : "r"(bar) : "memory");
 }
 
 template <bool PAIR>
@@ -193,7 +196,7 @@ __device__ __forceinline__ void pack_row(const Pair (&v)[4], uint32_t to0, uint3
 }
 
 template <int BN, bool PAIR, typename O>
-__global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_constant__ MatmulParams p)
+__global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_kernel(const __grid_constant__ MatmulParams p)
 {
     using L = Tiles<BN, PAIR, O>;
     constexpr int S = L::kStages;
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_c
         }
         for (int i = 0; i < 2; ++i) {
             umma::mbar_init(done + i * 8, 1);
-            umma::mbar_init(freed + i * 8, kEpilogueWarps * (PAIR ? 2 : 1));
+            umma::mbar_init(freed + i * 8, L::kWarps * (PAIR ? 2 : 1));
         }
         umma::mbar_fence_init();
         umma::tma_prefetch_desc(&p.a);
@@ -280,22 +283,24 @@ __global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_c
             }
         }
     } else if (warp >= 4) {  // results
-        const int quarter = warp % 4, half = warp / 4 - 1, w = warp - 4;
+        const int quarter = warp % 4, part = warp / 4 - 1, w = warp - 4;
         constexpr int kMine = L::kColumns / 32;  // columns of a lane whose scales it brings
         const uint32_t bar = PAIR ? in_block(freed, 0) : freed;
         float* scales = reinterpret_cast<float*>(base + L::kScales) + w * 2 * L::kColumns;  // [columns] of ws, of the bias
         int row0, column0, buffer = 0;
-        float ws[kMine], bs[kMine], xs;
+        float ws[kMine], xs;
+        O bs[kMine];  // converted when they are used: the loads stay under way
         const auto ahead = [&](int t) {
             int m, n;
             tile_at(p, t, m, n);
             row0 = (m * (PAIR ? 2 : 1) + static_cast<int>(rank)) * kTileM + quarter * 32;
-            column0 = n * BN + half * L::kColumns;
+            column0 = n * BN + part * L::kColumns;
 #pragma unroll
             for (int c = 0; c < kMine; ++c) {
                 const int x = column0 + c * 32 + lane;
                 ws[c] = x < p.N ? __ldg(p.ws + x) : 0.0f;
-                bs[c] = x < p.N && p.bias != nullptr ? to_float(static_cast<const O*>(p.bias)[x]) : 0.0f;
+                bs[c] = from_float<O>(0.0f);
+                if (x < p.N && p.bias != nullptr) bs[c] = static_cast<const O*>(p.bias)[x];
             }
             xs = row0 + lane < p.M ? __ldg(p.xs + row0 + lane) : 0.0f;
         };
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_c
 #pragma unroll
             for (int c = 0; c < kMine; ++c) {
                 scales[c * 32 + lane] = ws[c];
-                scales[L::kColumns + c * 32 + lane] = bs[c];
+                scales[L::kColumns + c * 32 + lane] = to_float(bs[c]);
             }
             __syncwarp();
             const Pair x2 = pair(xs, xs);
@@ -315,42 +320,39 @@ __global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_c
             ok = wait(done + (i & 1) * 8, (i >> 1) & 1);
             umma::fence_after_sync();
             if (!ok) break;
-            const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * BN + half * L::kColumns;
+            const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * BN + part * L::kColumns;
 #pragma unroll 1
-            for (int c = 0; c < L::kColumns; c += L::kChunk, buffer ^= 1) {
-                const int my_out = L::kOut + (w * 2 + buffer) * L::kStaging;
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" : : : "memory");
+            for (int c = 0; c < L::kColumns; c += L::kChunk, buffer = L::kBuffers - 1 - buffer) {
+                const int my_out = L::kOut + (w * L::kBuffers + buffer) * L::kStaging;
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;\n" : : "n"(L::kBuffers - 1) : "memory");
                 __syncwarp();
-#pragma unroll
-                for (int e = 0; e < L::kChunk; e += 32) {
-                    uint32_t v[32];
-                    umma::tmem_ld32(from + c + e, v);
-                    umma::tmem_wait_ld32(v);
-                    if (c + e + 32 == L::kColumns) {  // TMEM has been read
-                        umma::fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (PAIR) arrive_cluster(bar + (i & 1) * 8);
-                            else umma::mbar_arrive(bar + (i & 1) * 8);
-                        }
+                uint32_t v[32];
+                umma::tmem_ld32(from + c, v);
+                umma::tmem_wait_ld32(v);
+                if (c + L::kChunk == L::kColumns) {  // TMEM has been read
+                    umma::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (PAIR) arrive_cluster(bar + (i & 1) * 8);
+                        else umma::mbar_arrive(bar + (i & 1) * 8);
                     }
+                }
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        Pair f[4];
+                for (int j = 0; j < L::kChunk; j += 8) {
+                    Pair f[4];
 #pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            const float4 sw = *reinterpret_cast<const float4*>(scales + c + e + j + 4 * z);
-                            const float4 sb = *reinterpret_cast<const float4*>(scales + L::kColumns + c + e + j + 4 * z);
-                            const uint32_t* q = v + j + 4 * z;
-                            f[2 * z] = fma2(mul2(pair(__int2float_rn(q[0]), __int2float_rn(q[1])), x2), pair(sw.x, sw.y), pair(sb.x, sb.y));
-                            f[2 * z + 1] = fma2(mul2(pair(__int2float_rn(q[2]), __int2float_rn(q[3])), x2), pair(sw.z, sw.w), pair(sb.z, sb.w));
-                        }
-                        // 16-byte piece of the row, swizzled as the TMA store reads it
-                        const int piece = (e + j) * static_cast<int>(sizeof(O)) / 16;
-                        const int turn = L::kChunkRow == 128 ? lane & 7 : (lane >> 1) & 3;
-                        const uint32_t at = sm + my_out + lane * L::kChunkRow;
-                        pack_row<O>(f, at + ((piece ^ turn) << 4), at + (((piece + 1) ^ turn) << 4));
+                    for (int z = 0; z < 2; ++z) {
+                        const float4 m = *reinterpret_cast<const float4*>(scales + c + j + 4 * z);
+                        const float4 a = *reinterpret_cast<const float4*>(scales + L::kColumns + c + j + 4 * z);
+                        const uint32_t* q = v + j + 4 * z;
+                        f[2 * z] = fma2(mul2(pair(__int2float_rn(q[0]), __int2float_rn(q[1])), x2), pair(m.x, m.y), pair(a.x, a.y));
+                        f[2 * z + 1] = fma2(mul2(pair(__int2float_rn(q[2]), __int2float_rn(q[3])), x2), pair(m.z, m.w), pair(a.z, a.w));
                     }
+                    // 16-byte piece of the row, swizzled as the TMA store reads it
+                    const int piece = j * static_cast<int>(sizeof(O)) / 16;
+                    const int turn = L::kChunkRow == 128 ? lane & 7 : (lane >> 1) & 3;
+                    const uint32_t at = sm + my_out + lane * L::kChunkRow;
+                    pack_row<O>(f, at + ((piece ^ turn) << 4), at + (((piece + 1) ^ turn) << 4));
                 }
                 const int x = my_column0 + c;
                 if (p.stored) {
@@ -361,11 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1) int8_matmul_kernel(const __grid_c
                     __syncwarp();
                     for (int r = 0; r < 32 && my_row0 + r < p.M; ++r) {
                         const int turn = L::kChunkRow == 128 ? r & 7 : (r >> 1) & 3;
-                        for (int e = lane; e < L::kChunk && x + e < p.N; e += 32) {
-                            const int byte = e * static_cast<int>(sizeof(O));
-                            const uint8_t* v = base + my_out + r * L::kChunkRow + (((byte >> 4) ^ turn) << 4) + (byte & 15);
-                            static_cast<O*>(p.out)[static_cast<int64_t>(my_row0 + r) * p.N + x + e] = *reinterpret_cast<const O*>(v);
-                        }
+                        const int byte = lane * static_cast<int>(sizeof(O));
+                        const uint8_t* from_row = base + my_out + r * L::kChunkRow + (((byte >> 4) ^ turn) << 4) + (byte & 15);
+                        if (x + lane < p.N)
+                            static_cast<O*>(p.out)[static_cast<int64_t>(my_row0 + r) * p.N + x + lane] = *reinterpret_cast<const O*>(from_row);
                     }
                     __syncwarp();
                 }
@@ -562,7 +563,7 @@ int launch_tiles(MatmulParams& f, int tiles, int sms, cudaStream_t stream) noexc
         attr[cfg.numAttrs++].val.clusterDim.z = 1;
     }
     cfg.gridDim = PAIR ? 2 * std::min(tiles, sms / 2) : std::min(tiles, sms);
-    cfg.blockDim = kThreads;
+    cfg.blockDim = L::kThreads;
     cfg.dynamicSmemBytes = L::kBytes;
     cfg.stream = stream;
     cfg.attrs = attr;
