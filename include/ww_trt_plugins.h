@@ -442,8 +442,9 @@ int ww_quantize_tokens(const ww_layer_norm_t* p, void* stream);
  *   out[m, n] = (x_scale[m] * sum_k x_q[m, k] w_q[n, k]) * w_scale[n] + bias[n]
  * the sums exact in 32 bits.  Either x_q and x_scale are given or x, activations of
  * the output's type that are brought to 8 bits first, row by row.
- * x_q and w_q start on 16 bytes, their rows are a multiple of 16 bytes apart; what
- * stands between a row's K values and the next row does not matter.  K < 2^17. */
+ * x_q and w_q start on 16 bytes, their rows are a multiple of 16 bytes apart and are
+ * read in whole 16 bytes, the last ones too; what stands behind a row's K values does
+ * not matter.  K < 2^17. */
 typedef struct ww_int8_matmul {
     const void* x;        /* [M, K] of dtype, or NULL */
     const int8_t* x_q;    /* [M, K], or NULL */

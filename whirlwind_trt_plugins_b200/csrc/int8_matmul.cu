@@ -13,11 +13,11 @@
 // Blocks are persistent; tiles go in bands of rows so that operands are read from L2.
 // Large products take two SMs for a 256 x 256 tile (cta_group::2): each holds half
 // the rows and half the channels and reads each operand once.
-// Few tokens: the weights' bytes are the bound.  A block takes 16 channels, its warps
-// shares of K; each lane loads 16 bytes of a row, which are its fragments of two
-// mma.sync m16n8k32 (k is summed, so any order of it serves that both operands
-// share), and all of a warp's loads are under way before the tokens have been
-// brought to 8 bits in shared memory.
+// Up to 8 tokens: the weights' bytes are the bound.  One round of blocks shares the
+// channels; a warp's load is 512 bytes of a channel, so that a lane's 16 bytes of the
+// tokens stay in registers over all channels; dp4a, and eight integer sums at a time joined
+// over the warp.  The weights' loads are under way before the tokens have been brought to
+// 8 bits.
 #include "rows.cuh"
 #include "tensor_map.cuh"
 #include "umma.cuh"
@@ -30,6 +30,9 @@ int quantise_rows(const ww_layer_norm_t& p, const char* name, void* stream) noex
 
 namespace {
 
+#ifndef WW_ALONE
+#define WW_ALONE 16384
+#endif
 constexpr int kBlockK = 128;  // bytes of a row of a stage
 constexpr int kTileM = 128;   // rows of an SM's tile
 
@@ -384,10 +387,12 @@ __global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_k
 
 // ---- few tokens ----
 
-constexpr int kFewTokens = 16;
-constexpr int kFewChannels = 16;
-constexpr int kFewWarps = 8;
-constexpr int kFewShared = 96 * 1024;  // bytes of the tokens in 8 bits
+constexpr int kFewTokens = 8;
+constexpr int kFewWarps = 16;
+constexpr int kFewThreads = kFewWarps * 32;
+constexpr int kSlice = 512;             // bytes of K of a warp's load
+constexpr int kFewShared = 160 * 1024;  // bytes of the tokens in 8 bits
+constexpr int kFewAhead = 8;            // loads that a warp has under way
 
 struct FewParams {
     const void* x;  // activations, or
@@ -398,132 +403,188 @@ struct FewParams {
     void* out;
     int64_t x_stride, xq_stride, w_stride;
     int32_t M, K, N, pitch;  // pitch: bytes between the tokens in shared memory
+    int32_t channels;        // of a block
     int32_t x_pieces;        // x can be read 16 bytes at a time
+    int32_t behind;          // xq is written by the launch before
 };
 
-// 16 bytes of a row at k; what lies beyond K is 0.
+// 16 bytes of a row at k < K; what lies beyond K is 0.
 __device__ __forceinline__ uint4 load_row(const int8_t* row, int k, int K)
 {
-    if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
-    uint32_t u[4] = {0, 0, 0, 0};
-    for (int j = 0; k + j < K; ++j) u[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + j])) << (j % 4 * 8);
-    return make_uint4(u[0], u[1], u[2], u[3]);
+    uint4 u = __ldg(reinterpret_cast<const uint4*>(row + k));
+    const auto keep = [&](uint32_t& w, int at) {  // the word's bytes before K
+        const int n = K - k - at;
+        if (n < 4) w = n <= 0 ? 0 : w & (0xffffffffu >> (32 - 8 * n));
+    };
+    if (k + 16 > K) {
+        keep(u.x, 0);
+        keep(u.y, 4);
+        keep(u.z, 8);
+        keep(u.w, 12);
+    }
+    return u;
 }
 
-__device__ __forceinline__ void mma_i8_warp(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+template <typename O, int TOKENS>
+__global__ void __launch_bounds__(kFewThreads, 1) int8_few_kernel(const __grid_constant__ FewParams p)
 {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
-                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-template <typename O, int NT>  // NT: groups of 8 tokens
-__global__ void __launch_bounds__(kFewWarps * 32) int8_few_kernel(const __grid_constant__ FewParams p)
-{
-    constexpr int kAhead = 4;  // steps of 64 bytes of K under way
-    extern __shared__ __align__(16) uint8_t tokens[];  // [M][pitch], then
-    auto part = reinterpret_cast<int(*)[NT * 8][kFewChannels + 1]>(tokens + p.M * p.pitch);  // [warps], the shares' sums
-    float* scale = reinterpret_cast<float*>(part + kFewWarps);
-    uint32_t* top = reinterpret_cast<uint32_t*>(scale + kFewTokens);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    const int n0 = blockIdx.x * kFewChannels;
-    const int steps = (p.K + 63) / 64, share = (steps + kFewWarps - 1) / kFewWarps;
-    const int first = min(warp * share, steps), last = min(first + share, steps);
-    const int8_t* lo = p.wq + min(n0 + g, p.N - 1) * p.w_stride;
-    const int8_t* hi = p.wq + min(n0 + g + 8, p.N - 1) * p.w_stride;
-    uint4 wl[kAhead], wh[kAhead];
+    constexpr int kAhead = kFewAhead;
+    extern __shared__ __align__(16) uint8_t tokens[];  // [M][pitch], then the sums [channels][tokens], then
+    int* sums = reinterpret_cast<int*>(tokens + p.M * p.pitch);
+    float* scale = reinterpret_cast<float*>(sums + p.channels * TOKENS);
+    uint32_t* top = reinterpret_cast<uint32_t*>(scale + TOKENS);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int n0 = blockIdx.x * p.channels, channels = min(p.channels, p.N - n0);
+    const int slices = (p.K + kSlice - 1) / kSlice, end = slices * kSlice;
+    // This warp's rows: [row0, channels) in steps of `by`, of slices slice0, slice0 + 16, ..., kAhead
+    // rows (places beyond the channels included) at a time.  The first loads are under way before
+    // the tokens are there.  Bytes beyond K meet zeros of the tokens.
+    const int by = slices < kFewWarps ? kFewWarps / slices : 1, row0 = slices < kFewWarps ? warp / slices : 0;
+    const int slice0 = slices < kFewWarps ? warp % slices : warp;
+    const int turns = row0 < by && row0 < channels ? (channels - row0 + by * kAhead - 1) / (by * kAhead) : 0;
+    const int count = slice0 < slices ? turns * ((slices - slice0 + kFewWarps - 1) / kFewWarps) : 0;
+    uint4 w[kAhead];
+    const auto load = [&](int i, int slice, int r0) {  // row i of those from r0 on
+        const int row = r0 + i * by, k = slice * kSlice + lane * 16;
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (row < channels && k < p.K) w[i] = __ldg(reinterpret_cast<const uint4*>(p.wq + (n0 + row) * p.w_stride + k));
+    };
+    if (count > 0)
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-        if (first + i < last) {
-            wl[i] = load_row(lo, (first + i) * 64 + t * 16, p.K);
-            wh[i] = load_row(hi, (first + i) * 64 + t * 16, p.K);
-        }
-    const int end = steps * 64;
+        for (int i = 0; i < kAhead; ++i) load(i, slice0, row0);
+    for (int e = threadIdx.x; e < p.channels * TOKENS; e += kFewThreads) sums[e] = 0;
+    if (threadIdx.x < TOKENS) top[threadIdx.x] = 0;
+    if (p.behind) wait_for_launches_before();
+    constexpr int kBatch = TOKENS < 4 ? TOKENS : 4;  // tokens whose loads are under way together
     if (p.x != nullptr) {
         // the tokens in 8 bits: each token's largest magnitude (its bits order like the
         // values, NaN above all), then its whole numbers, from L1 again
         constexpr int V = 16 / static_cast<int>(sizeof(O));
-        if (threadIdx.x < kFewTokens) top[threadIdx.x] = 0;
         __syncthreads();
-        for (int m = 0; m < p.M; ++m) {
-            const O* x = static_cast<const O*>(p.x) + m * p.x_stride;
-            float a = 0.0f;
+        for (int m0 = 0; m0 < p.M; m0 += kBatch) {
+            float a[kBatch] = {};
             if (p.x_pieces) {
-                for (int k = threadIdx.x * V; k < p.K; k += kFewWarps * 32 * V) {
-                    Piece<O, V> r[1];
+                for (int k = threadIdx.x * V; k < p.K; k += kFewThreads * V) {
+                    Piece<O, V> r[kBatch][1];
                     Pair f[V / 2];
-                    r[0].load(x + k);
-                    values_of<O, V, 1>(r, f);
-                    a = max_nan(a, largest(f));
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j)
+                        if (m0 + j < p.M) r[j][0].load(static_cast<const O*>(p.x) + (m0 + j) * p.x_stride + k);
+                        else r[j][0].clear();
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        values_of<O, V, 1>(r[j], f);
+                        a[j] = max_nan(a[j], largest(f));
+                    }
                 }
             } else {
-#pragma unroll 8
-                for (int k = threadIdx.x; k < p.K; k += kFewWarps * 32) a = max_nan(a, fabsf(to_float(x[k])));
+#pragma unroll 4
+                for (int k = threadIdx.x; k < p.K; k += kFewThreads)
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j)
+                        if (m0 + j < p.M) a[j] = max_nan(a[j], fabsf(to_float(static_cast<const O*>(p.x)[(m0 + j) * p.x_stride + k])));
             }
-            const uint32_t u = __reduce_max_sync(~0u, __float_as_uint(a) & 0x7fffffffu);
-            if (lane == 0) atomicMax(top + m, u);
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const uint32_t u = __reduce_max_sync(~0u, __float_as_uint(a[j]) & 0x7fffffffu);
+                if (lane == 0 && m0 + j < p.M) atomicMax(top + m0 + j, u);
+            }
         }
         __syncthreads();
-        for (int m = 0; m < p.M; ++m) {
-            const O* x = static_cast<const O*>(p.x) + m * p.x_stride;
-            int8_t* to = reinterpret_cast<int8_t*>(tokens) + m * p.pitch;
-            const RowScale r = row_scale(__uint_as_float(top[m]));
-            if (threadIdx.x == 0) scale[m] = r.scale;
+        if (threadIdx.x < p.M) scale[threadIdx.x] = row_scale(__uint_as_float(top[threadIdx.x])).scale;
+        for (int m0 = 0; m0 < p.M; m0 += kBatch) {
+            float inv[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) inv[j] = row_scale(__uint_as_float(top[min(m0 + j, p.M - 1)])).inv;
+            int8_t* to = reinterpret_cast<int8_t*>(tokens) + m0 * p.pitch;
             if (p.x_pieces) {
-                for (int k = threadIdx.x * V; k < end; k += kFewWarps * 32 * V) {
-                    Piece<O, V> v[1];
+                for (int k = threadIdx.x * V; k < end; k += kFewThreads * V) {
+                    Piece<O, V> r[kBatch][1];
                     Pair f[V / 2];
-                    if (k < p.K) v[0].load(x + k);
-                    else v[0].clear();
-                    values_of<O, V, 1>(v, f);
-                    store_piece_int8<V>(to + k, f, r.inv, 0);
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j)
+                        if (m0 + j < p.M && k < p.K) r[j][0].load(static_cast<const O*>(p.x) + (m0 + j) * p.x_stride + k);
+                        else r[j][0].clear();
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        if (m0 + j >= p.M) continue;
+                        values_of<O, V, 1>(r[j], f);
+                        store_piece_int8<V>(to + j * p.pitch + k, f, inv[j], 0);
+                    }
                 }
             } else {
-#pragma unroll 8
-                for (int k = threadIdx.x; k < end; k += kFewWarps * 32)
-                    to[k] = k < p.K ? quantise(to_float(x[k]), r.inv) : 0;
+#pragma unroll 4
+                for (int k = threadIdx.x; k < end; k += kFewThreads)
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j)
+                        if (m0 + j < p.M)
+                            to[j * p.pitch + k] = k < p.K ? quantise(to_float(static_cast<const O*>(p.x)[(m0 + j) * p.x_stride + k]), inv[j]) : 0;
             }
         }
     } else {
-        for (int e = threadIdx.x; e < p.M * (end / 16); e += kFewWarps * 32) {
-            const int m = e / (end / 16), k = e % (end / 16) * 16;
-            *reinterpret_cast<uint4*>(tokens + m * p.pitch + k) = load_row(p.xq + m * p.xq_stride, k, p.K);
-        }
         if (threadIdx.x < p.M) scale[threadIdx.x] = __ldg(p.xs + threadIdx.x);
+        for (int m0 = 0; m0 < p.M; m0 += kBatch)
+            for (int k = threadIdx.x * 16; k < end; k += kFewThreads * 16) {
+                uint4 u[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j)
+                    u[j] = m0 + j < p.M && k < p.K ? load_row(p.xq + (m0 + j) * p.xq_stride, k, p.K) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j)
+                    if (m0 + j < p.M) *reinterpret_cast<uint4*>(tokens + (m0 + j) * p.pitch + k) = u[j];
+            }
     }
     __syncthreads();
-    int d[NT][4] = {};
-    for (int i0 = first; i0 < last; i0 += kAhead) {
+    uint4 x[TOKENS];
+    constexpr int kAtOnce = 8 / TOKENS;  // rows whose eight sums are joined over the warp together
+    int slice = slice0, r0 = row0;
+    for (int n = 0; n < count; ++n) {
+        if (r0 == row0)
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (i0 + i >= last) break;
-            const uint4 a = wl[i], b = wh[i];
-            if (i0 + i + kAhead < last) {
-                wl[i] = load_row(lo, (i0 + i + kAhead) * 64 + t * 16, p.K);
-                wh[i] = load_row(hi, (i0 + i + kAhead) * 64 + t * 16, p.K);
-            }
+            for (int m = 0; m < TOKENS; ++m)
+                x[m] = m < p.M ? *reinterpret_cast<const uint4*>(tokens + m * p.pitch + slice * kSlice + lane * 16) : make_uint4(0, 0, 0, 0);
+        const bool wraps = r0 + by * kAhead >= channels;
+        const int next_slice = wraps ? slice + kFewWarps : slice, next_r0 = wraps ? row0 : r0 + by * kAhead;
 #pragma unroll
-            for (int c = 0; c < NT; ++c) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (c * 8 + g < p.M) x = *reinterpret_cast<const uint4*>(tokens + (c * 8 + g) * p.pitch + (i0 + i) * 64 + t * 16);
-                mma_i8_warp(d[c], a.x, b.x, a.y, b.y, x.x, x.y);
-                mma_i8_warp(d[c], a.z, b.z, a.w, b.w, x.z, x.w);
+        for (int i = 0; i < kAhead; i += kAtOnce) {
+            int v[8];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                const uint4 a = w[i + j];
+                if (n + 1 < count) load(i + j, next_slice, next_r0);
+#pragma unroll
+                for (int m = 0; m < TOKENS; ++m) {
+                    int d = __dp4a(static_cast<int>(a.x), static_cast<int>(x[m].x), 0);
+                    d = __dp4a(static_cast<int>(a.y), static_cast<int>(x[m].y), d);
+                    d = __dp4a(static_cast<int>(a.z), static_cast<int>(x[m].z), d);
+                    v[j * TOKENS + m] = __dp4a(static_cast<int>(a.w), static_cast<int>(x[m].w), d);
+                }
             }
+            // eight sums over 32 lanes: half of them change sides at each of three steps
+#pragma unroll
+            for (int half = 4; half > 0; half /= 2) {
+                const bool upper = lane & (half * 4);
+#pragma unroll
+                for (int j = 0; j < half; ++j) {
+                    const int give = upper ? v[j] : v[j + half];
+                    v[j] = (upper ? v[j + half] : v[j]) + __shfl_xor_sync(~0u, give, half * 4);
+                }
+            }
+            v[0] += __shfl_xor_sync(~0u, v[0], 2);
+            v[0] += __shfl_xor_sync(~0u, v[0], 1);
+            // value lane / 4; the slices' sums are whole numbers, so that their order does not matter
+            const int row = r0 + (i + lane / 4 / TOKENS) * by, m = lane / 4 % TOKENS;
+            if (lane % 4 == 0 && row < channels && m < p.M) atomicAdd(sums + row * TOKENS + m, v[0]);
         }
+        slice = next_slice;
+        r0 = next_r0;
     }
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) part[warp][c * 8 + 2 * t + e % 2][g + e / 2 * 8] = d[c][e];
     __syncthreads();
-    for (int e = threadIdx.x; e < p.M * kFewChannels; e += kFewWarps * 32) {
-        const int m = e / kFewChannels, c = e % kFewChannels;
-        if (n0 + c >= p.N) continue;
-        int sum = 0;
-#pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) sum += part[w][m][c];
+    for (int e = threadIdx.x; e < p.M * channels; e += kFewThreads) {
+        const int m = e / channels, c = e - m * channels;
         const float b = p.bias == nullptr ? 0.0f : to_float(static_cast<const O*>(p.bias)[n0 + c]);
-        static_cast<O*>(p.out)[static_cast<int64_t>(m) * p.N + n0 + c] = from_float<O>(fmaf(__int2float_rn(sum) * scale[m], __ldg(p.ws + n0 + c), b));
+        static_cast<O*>(p.out)[static_cast<int64_t>(m) * p.N + n0 + c] =
+            from_float<O>(fmaf(__int2float_rn(sums[c * TOKENS + m]) * scale[m], __ldg(p.ws + n0 + c), b));
     }
 }
 
@@ -531,17 +592,16 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_kernel(const __grid_c
 
 int pitch_of(int k) noexcept { return (k + 15) / 16 * 16; }
 
-// Shared memory behind the tokens.
-int few_rest(int tokens) noexcept { return kFewWarps * tokens * (kFewChannels + 1) * 4 + kFewTokens * 8; }
+// Bytes between tokens in shared memory: whole slices.
+int few_pitch(int k) noexcept { return (k + kSlice - 1) / kSlice * kSlice; }
 
-// Bytes between tokens in shared memory: half a line of banks apart from line to line.
-int few_pitch(int k) noexcept
+bool few_form(const ww_int8_matmul_t& p) noexcept
 {
-    const int n = (k + 63) / 64 * 64;
-    return n % 128 == 64 ? n : n + 64;
+    return p.M <= kFewTokens && i64(p.M) * few_pitch(p.K) <= kFewShared && p.N <= (1 << 16);
 }
 
-bool few_form(const ww_int8_matmul_t& p) noexcept { return p.M <= kFewTokens && i64(p.M) * few_pitch(p.K) <= kFewShared; }
+// Few tokens that every block brings to 8 bits by itself; more are brought there once.
+bool few_alone(const ww_int8_matmul_t& p) noexcept { return p.x == nullptr || i64(p.M) * p.K <= WW_ALONE; }
 
 template <int BN, bool PAIR, typename O>
 int launch_tiles(MatmulParams& f, int tiles, int sms, cudaStream_t stream) noexcept
@@ -572,17 +632,16 @@ int launch_tiles(MatmulParams& f, int tiles, int sms, cudaStream_t stream) noexc
 }
 
 template <int BN, bool PAIR, typename O>
-int run_tiles(const ww_int8_matmul_t& p, const int8_t* xq, const float* xs, int64_t xq_stride, bool behind, int sms, int* err,
-              cudaStream_t stream) noexcept
+int run_tiles(const ww_int8_matmul_t& p, bool behind, int sms, int* err, cudaStream_t stream) noexcept
 {
     using L = Tiles<BN, PAIR, O>;
     MatmulParams f;
-    if (!encode_rows_map(&f.a, WW_DTYPE_INT8, xq, p.M, p.K, xq_stride, kBlockK, kTileM) ||
+    if (!encode_rows_map(&f.a, WW_DTYPE_INT8, p.x_q, p.M, p.K, p.x_q_stride, kBlockK, kTileM) ||
         !encode_rows_map(&f.b, WW_DTYPE_INT8, p.w_q, p.N, p.K, p.w_stride, kBlockK, PAIR ? BN / 2 : BN))
         return WW_ERR_UNSUPPORTED;
     f.stored = i64(p.N) * static_cast<int>(sizeof(O)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
     if (f.stored && !encode_rows_map(&f.c, p.dtype, p.out, p.M, p.N, p.N, L::kChunk, 32)) return WW_ERR_UNSUPPORTED;
-    f.xs = xs;
+    f.xs = p.x_scale;
     f.ws = p.w_scale;
     f.bias = p.bias;
     f.out = p.out;
@@ -600,52 +659,57 @@ int run_tiles(const ww_int8_matmul_t& p, const int8_t* xq, const float* xs, int6
     return launch_tiles<BN, PAIR, O>(f, static_cast<int>(tiles), sms, stream);
 }
 
+// Channels of a block in the form for few tokens: one round of blocks, at least 4 channels each.
+int few_channels(int n, int sms) noexcept { return std::max(4, (n + sms - 1) / sms); }
+
 template <typename O>
-int few(const ww_int8_matmul_t& p, cudaStream_t stream) noexcept
+int few(const ww_int8_matmul_t& p, bool behind, int sms, cudaStream_t stream) noexcept
 {
-    FewParams f{p.x, p.x_q, p.x_scale, p.w_scale, p.w_q, p.bias, p.out, p.x_stride, p.x_q_stride, p.w_stride, p.M, p.K, p.N, few_pitch(p.K), 0};
+    FewParams f{p.x, p.x_q, p.x_scale, p.w_scale, p.w_q, p.bias, p.out, p.x_stride, p.x_q_stride, p.w_stride, p.M, p.K, p.N, few_pitch(p.K),
+                few_channels(p.N, sms), 0, behind};
     constexpr int V = 16 / static_cast<int>(sizeof(O));
     f.x_pieces = p.K % V == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && (p.M == 1 || p.x_stride % V == 0);
-    const auto kernel = p.M <= 8 ? int8_few_kernel<O, 1> : int8_few_kernel<O, 2>;
-    static std::atomic<uint64_t> raised[2];
-    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised[p.M <= 8 ? 0 : 1])) return launch_status("int8_matmul");
-    kernel<<<(p.N + kFewChannels - 1) / kFewChannels, kFewWarps * 32, p.M * f.pitch + few_rest(p.M <= 8 ? 8 : 16), stream>>>(f);
+    const int form = p.M == 1 ? 0 : p.M <= 4 ? 1 : 2, tokens = form == 0 ? 1 : 4 * form;
+    const auto kernel = form == 0 ? int8_few_kernel<O, 1> : form == 1 ? int8_few_kernel<O, 4> : int8_few_kernel<O, 8>;
+    static std::atomic<uint64_t> raised[3];
+    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised[form])) return launch_status("int8_matmul");
+    const int bytes = p.M * f.pitch + f.channels * tokens * 4 + tokens * 8;
+    const dim3 grid((p.N + f.channels - 1) / f.channels);
+    if (behind) launch_behind(kernel, grid, dim3(kFewThreads), bytes, stream, f);
+    else kernel<<<grid, kFewThreads, bytes, stream>>>(f);
     return launch_status("int8_matmul");
 }
 
 template <typename O>
 int matmul(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
 {
-    if (few_form(p)) return few<O>(p, stream);
-    int* err = device_error_slot();
-    if (err == nullptr) return WW_ERR_DEVICE;
-    const int8_t* xq = p.x_q;
-    const float* xs = p.x_scale;
-    int64_t stride = p.x_q_stride;
+    const bool is_few = few_form(p);
+    if (is_few && few_alone(p)) return few<O>(p, false, sms, stream);
+    ww_int8_matmul_t c = p;
     if (p.x != nullptr) {
-        stride = pitch_of(p.K);
-        int8_t* q = static_cast<int8_t*>(p.workspace);
-        float* scale = reinterpret_cast<float*>(q + i64(p.M) * stride);
         ww_layer_norm_t r{};
+        c.x = nullptr;
+        c.x_q_stride = r.y_q_stride = pitch_of(p.K);
+        c.x_q = r.y_q = static_cast<int8_t*>(p.workspace);
+        c.x_scale = r.y_scale = reinterpret_cast<float*>(r.y_q + i64(p.M) * r.y_q_stride);
         r.x = p.x;
         r.x_stride = p.x_stride;
-        r.y_q = q;
-        r.y_scale = scale;
-        r.y_q_stride = stride;
         r.dtype = p.dtype;
         r.rows = p.M;
         r.N = p.K;
         const int st = quantise_rows(r, "int8_matmul", stream);
         if (st != WW_SUCCESS) return st;
-        xq = q;
-        xs = scale;
     }
+    const bool behind = p.x != nullptr;
+    if (is_few) return few<O>(c, behind, sms, stream);
+    int* err = device_error_slot();
+    if (err == nullptr) return WW_ERR_DEVICE;
     const int64_t rows = (p.M + 127) / 128;
     if (rows * ((p.N + 255) / 256) >= sms && p.N > 128)
-        return run_tiles<256, true, O>(p, xq, xs, stride, p.x != nullptr, sms, err, stream);
+        return run_tiles<256, true, O>(c, behind, sms, err, stream);
     if (rows * ((p.N + 127) / 128) >= sms / 2 && p.N > 64)
-        return run_tiles<128, false, O>(p, xq, xs, stride, p.x != nullptr, sms, err, stream);
-    return run_tiles<64, false, O>(p, xq, xs, stride, p.x != nullptr, sms, err, stream);
+        return run_tiles<128, false, O>(c, behind, sms, err, stream);
+    return run_tiles<64, false, O>(c, behind, sms, err, stream);
 }
 
 int check(const ww_int8_matmul_t& p) noexcept
@@ -666,7 +730,7 @@ int check(const ww_int8_matmul_t& p) noexcept
 
 int64_t workspace(const ww_int8_matmul_t& p) noexcept
 {
-    if (p.x == nullptr || p.M == 0 || p.N == 0 || few_form(p)) return 0;
+    if (p.x == nullptr || p.M == 0 || p.N == 0 || (few_form(p) && few_alone(p))) return 0;
     return i64(p.M) * pitch_of(p.K) + i64(p.M) * 4;
 }
 

@@ -207,6 +207,12 @@ def quantize_tokens(x, stream=None):
     return q, scale
 
 
+def _whole_pieces(t, name: str, rows: int, k: int, stride: int):
+    """Rows of K bytes that the kernels read in whole 16 bytes: so far the memory of the last one must go."""
+    if k % 16 and rows and t.untyped_storage().nbytes() - t.storage_offset() < (rows - 1) * stride + (k + 15) // 16 * 16:
+        raise ValueError(f"{name}'s last row must be followed by memory up to whole 16 bytes: see quantize_tokens")
+
+
 def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
     T = _Torch.get()
     at = _first(x, "x" if x_scale is None else "x_q")
@@ -222,6 +228,7 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
         _tensor(x_scale, "x_scale", at, T.f32, x.shape[:-1])
         if rows > 1 and xs % 16:
             raise ValueError("rows of x_q must start on 16 bytes: see quantize_tokens")
+        _whole_pieces(x, "x_q", rows, k, xs)
     channels, kw, ws = _rows(w_q, "w_q", at, int8)
     if len(w_q.shape) != 2 or kw != k:
         raise ValueError(f"w_q must be [N, {k}], got {tuple(w_q.shape)}")
@@ -229,6 +236,7 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
         ws = (k + 15) // 16 * 16
     if ws % 16:
         raise ValueError("rows of w_q must start on 16 bytes: see quantize_tokens")
+    _whole_pieces(w_q, "w_q", channels, k, ws)
     _tensor(w_scale, "w_scale", at, T.f32, (channels,))
     if bias is not None:
         _tensor(bias, "bias", at, dtype, (channels,))
