@@ -24,7 +24,7 @@ import math
 import struct
 
 from . import _check, _lib, _out, _torch
-from .attention import _ATTN, _P, _Torch, _first, _new, _place, _ptr, _tensor, _vectors, _workspace
+from .attention import _ATTN, _P, _Torch, _empty, _first, _new, _place, _ptr, _tensor, _vectors, _workspace
 
 __all__ = ["layer_norm", "layer_norm_backward", "layer_norm_autograd", "layer_norm_int8", "quantize_tokens",
            "int8_matmul", "int8_linear", "quantize_kv", "dequantize_kv", "cross_attention_int8"]
@@ -81,13 +81,13 @@ def _dtype(t, name: str):
     return dt
 
 
-def _int8_rows(shape, device):
+def _int8_rows(shape):
     """An int8 tensor whose rows start on 16 bytes, and their stride."""
     n = shape[-1]
+    if n % 16 == 0:
+        return _empty(shape, _Torch.int8), n
     pitch = (n + 15) // 16 * 16
-    torch = _Torch.torch
-    t = torch.empty((*shape[:-1], pitch), dtype=torch.int8, device=device)
-    return (t if pitch == n else t[..., :n]), pitch
+    return _empty((*shape[:-1], pitch), _Torch.int8)[..., :n], pitch
 
 
 def _norm_args(x, weight, bias, eps, residual):
@@ -128,7 +128,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, residual=None, retu
         total = got[1].data_ptr()
     mean = rstd = 0
     if return_stats:
-        stats = [T.empty(x.shape[:-1], dtype=T.f32, device=x.device) for _ in range(2)]
+        stats = [_empty(x.shape[:-1], T.f32) for _ in range(2)]
         got += (*stats,)
         mean, rstd = stats[0].data_ptr(), stats[1].data_ptr()
     a = _NORM.pack(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), y.data_ptr(), total, 0, 0, mean, rstd, 0, 0,
@@ -144,8 +144,8 @@ def layer_norm_int8(x, weight=None, bias=None, eps: float = 1e-5, residual=None,
     if stream is not None or at != T.device():
         with _place(x, stream):
             return layer_norm_int8(x, weight, bias, eps, residual)
-    q, pitch = _int8_rows(x.shape, x.device)
-    scale = T.empty(x.shape[:-1], dtype=T.f32, device=x.device)
+    q, pitch = _int8_rows(x.shape)
+    scale = _empty(x.shape[:-1], T.f32)
     total = None if residual is None else _new(x, None, "sum")
     a = _NORM.pack(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), 0, _ptr(total), q.data_ptr(),
                    scale.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, xs, rs, pitch, 0, 0, dt, rows, n, eps)
@@ -177,12 +177,12 @@ def layer_norm_backward(dy, x, weight, mean, rstd, dsum=None, stream=None):
     dx = _new(x, None, "dx")
     dw = db = None
     if weight is not None:
-        dw, db = T.empty_like(weight), T.empty_like(weight)
+        dw, db = _new(weight, None, "dweight"), _new(weight, None, "dbias")
     a = _NORM.pack(x.data_ptr(), 0, _ptr(weight), 0, 0, 0, 0, 0, mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(),
                    _ptr(dsum), dx.data_ptr(), _ptr(dw), _ptr(db), 0, 0, xs, 0, 0, gs, ds, dt, rows, n, 0.0)
     need = _lib.ww_layer_norm_backward_workspace(a)
     if need:
-        ws, a = _workspace(need, x, a, _NORM_WS)
+        ws, a = _workspace(need, a, _NORM_WS)
     _check("ww_layer_norm_backward", _lib.ww_layer_norm_backward(a, T.stream(at)))
     return dx, dw, db
 
@@ -199,8 +199,8 @@ def quantize_tokens(x, stream=None):
     if stream is not None or at != T.device():
         with _place(x, stream):
             return quantize_tokens(x)
-    q, pitch = _int8_rows(x.shape, x.device)
-    scale = T.empty(x.shape[:-1], dtype=T.f32, device=x.device)
+    q, pitch = _int8_rows(x.shape)
+    scale = _empty(x.shape[:-1], T.f32)
     a = _NORM.pack(x.data_ptr(), 0, 0, 0, 0, 0, q.data_ptr(), scale.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, xs, 0,
                    pitch, 0, 0, dt, rows, n, 0.0)
     _check("ww_quantize_tokens", _lib.ww_quantize_tokens(a, T.stream(at)))
@@ -216,7 +216,7 @@ def _whole_pieces(t, name: str, rows: int, k: int, stride: int):
 def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
     T = _Torch.get()
     at = _first(x, "x" if x_scale is None else "x_q")
-    int8 = T.torch.int8
+    int8 = T.int8
     if x_scale is None:
         dt, dtype = _dtype(x, "x"), x.dtype
         rows, k, xs = _rows(x, "x", at)
@@ -244,13 +244,13 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
         with _place(x, stream):
             return _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, None)
     shape = (*x.shape[:-1], channels)
-    out = T.empty(shape, dtype=dtype, device=x.device) if out is None else _out(out, shape, dtype, x.device, "out")
+    out = _empty(shape, dtype) if out is None else _out(out, shape, dtype, x.device, "out")
     p = x.data_ptr()
     a = _MATMUL.pack(p if x_scale is None else 0, 0 if x_scale is None else p, _ptr(x_scale), w_q.data_ptr(),
                      w_scale.data_ptr(), _ptr(bias), out.data_ptr(), 0, 0, xs, xs, ws, dt, rows, k, channels)
     need = _lib.ww_int8_matmul_workspace(a) if x_scale is None else 0
     if need:
-        scratch, a = _workspace(need, x, a, _MATMUL_WS)
+        scratch, a = _workspace(need, a, _MATMUL_WS)
     _check("ww_int8_matmul", _lib.ww_int8_matmul(a, T.stream(at)))
     return out
 
@@ -273,7 +273,7 @@ def int8_linear(x, w_q, w_scale, bias=None, out=None, stream=None):
 
 def _kept(k_cache, v_cache, k_scale, v_scale, at: int):
     """Checks keys and values in 8 bits; returns (B, places, H, D) and the packed strides' values."""
-    int8 = _Torch.torch.int8
+    int8 = _Torch.int8
     ks = _vectors(k_cache, "k_cache", at, int8)
     shape = k_cache.shape
     vs = _vectors(v_cache, "v_cache", at, int8, shape)
@@ -336,7 +336,7 @@ def dequantize_kv(k_cache, v_cache, k_scale, v_scale, lens=None, dtype=None, str
     if stream is not None or at != T.device():
         with _place(k_cache, stream):
             return dequantize_kv(k_cache, v_cache, k_scale, v_scale, lens, dtype)
-    k, v = (T.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+    k, v = _empty(shape, dtype), _empty(shape, dtype)
     B, places, H, D = shape
     a = _CACHE.pack(0, 0, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), 0, _ptr(lens),
                     k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 0, 0, *kc, *vc, *ss, dt, B, 0, places, H, D)
@@ -385,14 +385,14 @@ def cross_attention_int8(q, k_cache, v_cache, k_scale, v_scale, scale: float | N
     if scale is None:
         scale = 1.0 / math.sqrt(D) if D else 1.0
     out = _new(q, out, "out")
-    lse = T.empty((B, Hq, Lq), dtype=T.f32, device=q.device) if return_lse else None
+    lse = _empty((B, Hq, Lq), T.f32) if return_lse else None
     a = _ATTN.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(k_lens),
                    _ptr(key_mask), _ptr(bias_table), 0, 0, 0, 0, 0, 0, 0, *qs, *ks, *vs, 0, 0, 0, dt, B, Lq, Lk, Hq, Hk,
                    D, buckets, max_distance, bool(bidirectional), q_offset, scale)
     a += _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), *ss)
     need = _lib.ww_cross_attention_int8_workspace(a)
     if need:
-        ws, a = _workspace(need, q, a, _ATTN_WS)
+        ws, a = _workspace(need, a, _ATTN_WS)
     _check("ww_cross_attention_int8", _lib.ww_cross_attention_int8(a, T.stream(at)))
     return (out, lse) if return_lse else out
 
