@@ -13,17 +13,27 @@
 // side and 8 rows (query heads of the key head x tokens) as its N side: what lanes
 // convert is used once for all rows.  Queries are scaled by a power of two to fp16's
 // upper range, whatever their type.
-// Each of 8 warps runs alone over every 8th tile of 32 keys of its block's share: one
-// lane keeps a ring of TMA loads in flight (swizzled rows, read back by ldmatrix), and no
-// barrier joins the warps before the end.  Sums of scores belong to a lane until then;
-// O is rescaled only when n has grown by 2^8.  The keys are split over blocks until
-// the GPU is full; attention_join_kernel joins the parts in order.
+// Two blocks of 6 warps (4 for more than 8 rows) per SM.  Each warp runs alone over every 6th tile
+// of 32 keys of its block's share: one lane keeps a ring of TMA loads in flight (swizzled rows, read back by
+// ldmatrix), and no barrier joins the warps before the end.  Sums of scores belong to a
+// lane until then; O is rescaled only when n has grown by 2^8.  The keys are split over
+// blocks until the GPU is full: up to 4 are a cluster that joins its parts through shared
+// memory, more are joined by attention_join_kernel, in order either way.
 #include "attention_token.cuh"
 #include "rows.cuh"
 #include "tensor_map.cuh"
 #include "umma.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
+
+#ifndef WW_CLUSTER
+#define WW_CLUSTER 4
+#endif
+#ifndef WW_SHORT
+#define WW_SHORT 32
+#endif
 
 namespace ww {
 
@@ -31,8 +41,8 @@ int dequantise_valid(const ww_kv_cache_t& p, const char* name, void* stream) noe
 
 namespace {
 
-constexpr int kWarps = 8;
 constexpr int kKeys = 32;          // of a warp's tile
+constexpr int kCluster = WW_CLUSTER;  // splits that join themselves
 constexpr int kMostRows = 128;     // of a key head, in blocks of up to 32
 constexpr float kRescale = 8.0f;   // log2 growth of a maximum that is left in P
 constexpr float kHead = 6.0f;      // P times 2^6
@@ -54,6 +64,7 @@ struct Int8Params {
     int32_t splits;
     int32_t k_b, k_h, v_b, v_h;
     int32_t max_entries;
+    int32_t joined;  // the splits are a cluster
     float scale2;
     int* err;
 };
@@ -61,7 +72,8 @@ struct Int8Params {
 template <int DP, int NB>
 struct Layout {
     static constexpr int kTile = kKeys * DP;
-    static constexpr int kStages = DP == 128 ? 3 : DP == 64 ? 4 : 6;
+    static constexpr int kWarps = NB == 1 ? 6 : 4;  // as registers allow two blocks per SM
+    static constexpr int kStages = DP == 128 ? (NB == 1 ? 2 : 3) : DP == 64 ? 4 : 6;
     static constexpr int kRows = NB * 8;
     static constexpr int kRing = (kStages * 2 * kTile > kRows * DP * 4 ? kStages * 2 * kTile : kRows * DP * 4);  // of a warp; its rows at the end
     static constexpr int kQPitch = DP * 2 + 16;  // bytes
@@ -71,7 +83,9 @@ struct Layout {
     static constexpr int kMl = kBar + kWarps * kStages * 8;     // n, maximum and sum of [warp][row]
     static constexpr int kBias = kMl + kWarps * kRows * 12;     // [heads][buckets] values, [entries] buckets
     static constexpr int kBytes = kBias + 1024;
+    static constexpr int kItems = (kRows * (DP / 8) + kWarps * 32 - 1) / (kWarps * 32);  // 8 values of a row, of a thread at the end
     static_assert(kRing % 1024 == 0, "swizzled tiles");
+    static_assert(kRows * DP * 4 + kRows * 8 <= kWarps * kRing, "a block's rows for its cluster");
 };
 
 // 16-byte piece j of row r of a swizzled tile of rows of DP bytes.
@@ -108,16 +122,17 @@ __device__ __forceinline__ uint32_t to_half2(uint32_t w)
 }
 
 template <typename T, int DP, int NB>
-__global__ void __launch_bounds__(kWarps * 32, 1) attention_int8_kernel(const __grid_constant__ Int8Params p)
+__global__ void __launch_bounds__(Layout<DP, NB>::kWarps * 32, 2) attention_int8_kernel(const __grid_constant__ Int8Params p)
 {
     using L = Layout<DP, NB>;
-    constexpr int S = L::kStages, kRows = L::kRows;
+    constexpr int S = L::kStages, kRows = L::kRows, kWarps = L::kWarps;
     extern __shared__ uint8_t raw[];
     uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
     const uint32_t sm = umma::smem_addr(base);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
     const uint32_t ring = sm + warp * L::kRing, bars = sm + L::kBar + warp * S * 8;
 
+    if (p.splits > 1 && !p.joined) start_launch_behind();  // the join, which waits for this grid's end
     const int split = blockIdx.x % p.splits;
     const int g = blockIdx.x / p.splits % p.Hk, b = blockIdx.x / p.splits / p.Hk;
     const int row0 = blockIdx.y * kRows, rows = min(kRows, p.rows - row0);
@@ -268,30 +283,45 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attention_int8_kernel(const __
             float kk[4], vv[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int key = c * 8 + g8;
-                kk[c] = __shfl_sync(~0u, my_k, key);
-                vv[c] = __shfl_sync(~0u, my_v, key);
+                kk[c] = __shfl_sync(~0u, my_k, c * 8 + g8);
+                vv[c] = __shfl_sync(~0u, my_v, c * 8 + g8);
             }
 #pragma unroll
             for (int x = 0; x < NB; ++x) {
-                float w[4][2];
+                float w[4][2], v[2][4];
+                if (one) {  // a tile's bias is one value a row, or none
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const float flat = biased ? tables[x][z][bucket] : 0.0f;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) v[z][c] = fmaf(sc[x][c / 2][c % 2 * 2 + z], kk[c] * rscale[x][z], flat);
+                    }
+                } else {
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const uint8_t* by = buckets + rel0 + g8 - token[x][z] - range.lo;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            v[z][c] = fmaf(sc[x][c / 2][c % 2 * 2 + z], kk[c] * rscale[x][z], tables[x][z][by[c * 8]]);
+                    }
+                }
+                if (keep != ~0u) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (!((keep >> (c * 8 + g8)) & 1)) {
+                            v[0][c] = v[1][c] = -INFINITY;
+                            vv[c] = 0.0f;  // whatever the place holds
+                        }
+                }
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    const float flat = biased ? tables[x][z][bucket] : 0.0f;
-                    float top = -INFINITY, v[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int key = c * 8 + g8;
-                        const float bias = !one ? tables[x][z][buckets[rel0 + key - token[x][z] - range.lo]] : flat;
-                        const float y = fmaf(sc[x][c / 2][c % 2 * 2 + z], kk[c] * rscale[x][z], bias);
-                        v[c] = (keep >> key) & 1 ? y : -INFINITY;
-                        w[c][z] = (keep >> key) & 1 ? y + vv[c] : -INFINITY;
-                        top = fmaxf(top, v[c]);
-                    }
-                    const float m = fmaxf(top_m[x][z], top), ms = m == -INFINITY ? 0.0f : m;
+                    const float m = fmaxf(fmaxf(fmaxf(v[z][0], v[z][1]), fmaxf(v[z][2], v[z][3])), top_m[x][z]), ms = m == -INFINITY ? 0.0f : m;
                     float add = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) add += exp2_approx(v[c] - ms);
+                    for (int c = 0; c < 4; ++c) {
+                        add += exp2_approx(v[z][c] - ms);
+                        w[c][z] = v[z][c] + vv[c];
+                    }
                     sum[x][z] = fmaf(sum[x][z], exp2_approx(top_m[x][z] - ms), add);
                     top_m[x][z] = m;
                 }
@@ -368,37 +398,95 @@ __global__ void __launch_bounds__(kWarps * 32, 1) attention_int8_kernel(const __
                 *reinterpret_cast<float2*>(mine + r * DP + e * 16 + 2 * g8) = make_float2(o[x][e][z], o[x][e][2 + z]);
         }
     __syncthreads();
-    for (int e = threadIdx.x; e < rows * (p.D / 8); e += kWarps * 32) {
-        const int r = e / (p.D / 8), d = e % (p.D / 8) * 8;
-        float top = -INFINITY;
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[(w * kRows + r) * 3 + 1]);
-        const float ms = top == -INFINITY ? 0.0f : top;
-        float total = 0.0f, v[8] = {};
+    // the warps' rows joined: unnormalised values, the maximum and the sum
+    float v[L::kItems][8], tops[L::kItems], totals[L::kItems];
+    const int pieces = p.D / 8, items = rows * pieces;
+#pragma unroll
+    for (int n = 0; n < L::kItems; ++n) {
+        const int e = threadIdx.x + n * kWarps * 32;
+        tops[n] = -INFINITY;
+        totals[n] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[n][j] = 0.0f;
+        if (e >= items) continue;
+        const int r = e / pieces, d = e % pieces * 8;
+        for (int w = 0; w < kWarps; ++w) tops[n] = fmaxf(tops[n], ml[(w * kRows + r) * 3 + 1]);
+        const float ms = tops[n] == -INFINITY ? 0.0f : tops[n];
         for (int w = 0; w < kWarps; ++w) {
             const float* x = ml + (w * kRows + r) * 3;
-            total += x[1] == -INFINITY ? x[2] : exp2_approx(x[1] - ms) * x[2];  // a NaN sum has no maximum
+            totals[n] += x[1] == -INFINITY ? x[2] : exp2_approx(x[1] - ms) * x[2];  // a NaN sum has no maximum
             // a warp without keys, or whose values are all 0, has n = -inf and zeros
             const float f = x[0] == -INFINITY ? 1.0f : exp2_approx(x[0] - kHead - ms);
             const float* from = reinterpret_cast<const float*>(base + w * L::kRing) + r * DP + d;
-            for (int j = 0; j < 8; ++j) v[j] += f * from[j];
+            for (int j = 0; j < 8; ++j) v[n][j] += f * from[j];
         }
+    }
+    const auto finish = [&](int r, int d, float top, float total, const float (&o)[8]) {
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         const int h = g * group + (row0 + r) / p.Lq, i = (row0 + r) % p.Lq;
         const int64_t row = (static_cast<int64_t>(b) * p.Lq + i) * p.Hq + h;
-        const float lse2 = total == 0.0f ? -INFINITY : ms + log2f(total);
-        if (p.splits > 1) {
+        const float lse2 = total == 0.0f ? -INFINITY : (top == -INFINITY ? 0.0f : top) + log2f(total);
+        if (p.splits > 1 && !p.joined) {
             const int64_t part = static_cast<int64_t>(blockIdx.x) * p.rows + row0 + r;  // [item][split][row]
             float* to = p.part_o + part * p.D + d;
-            *reinterpret_cast<float4*>(to) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-            *reinterpret_cast<float4*>(to + 4) = make_float4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+            *reinterpret_cast<float4*>(to) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            *reinterpret_cast<float4*>(to + 4) = make_float4(o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv);
             if (d == 0) p.part_lse[part] = lse2;
         } else {
             *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.D + d) =
-                make_uint4(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv),
-                           pack2<T>(v[4] * inv, v[5] * inv), pack2<T>(v[6] * inv, v[7] * inv));
+                make_uint4(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv),
+                           pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv));
             if (d == 0 && p.lse != nullptr) p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Lq + i] = lse2 * kLn2F;
         }
+    };
+    if (!p.joined) {
+#pragma unroll
+        for (int n = 0; n < L::kItems; ++n) {
+            const int e = threadIdx.x + n * kWarps * 32;
+            if (e < items) finish(e / pieces, e % pieces * 8, tops[n], totals[n], v[n]);
+        }
+        return;
     }
+    // the cluster's blocks put theirs into their shared memory; each joins a share of the rows
+    // from all of them, in order
+    float* block_o = reinterpret_cast<float*>(base);
+    float2* block_ml = reinterpret_cast<float2*>(base + kRows * DP * 4);
+    __syncthreads();  // the warps' rows have been read
+#pragma unroll
+    for (int n = 0; n < L::kItems; ++n) {
+        const int e = threadIdx.x + n * kWarps * 32;
+        if (e >= items) continue;
+        float4* to = reinterpret_cast<float4*>(block_o + e * 8);
+        to[0] = make_float4(v[n][0], v[n][1], v[n][2], v[n][3]);
+        to[1] = make_float4(v[n][4], v[n][5], v[n][6], v[n][7]);
+        if (e % pieces == 0) block_ml[e / pieces] = make_float2(tops[n], totals[n]);
+    }
+    const auto cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    const int e0 = items * split / p.splits, e1 = items * (split + 1) / p.splits;
+    for (int e = e0 + threadIdx.x; e < e1; e += kWarps * 32) {
+        const int r = e / pieces;
+        float top = -INFINITY, total = 0.0f, o[8] = {};
+        for (int c = 0; c < p.splits; ++c) top = fmaxf(top, cluster.map_shared_rank(block_ml, c)[r].x);
+        const float ms = top == -INFINITY ? 0.0f : top;
+        for (int c = 0; c < p.splits; ++c) {
+            const float2 x = cluster.map_shared_rank(block_ml, c)[r];
+            const float4* from = reinterpret_cast<const float4*>(cluster.map_shared_rank(block_o, c) + e * 8);
+            const float f = x.x == -INFINITY ? 1.0f : exp2_approx(x.x - ms);  // zeros, or a NaN sum
+            const float4 lo = from[0], hi = from[1];
+            total += f * x.y;
+            o[0] += f * lo.x;
+            o[1] += f * lo.y;
+            o[2] += f * lo.z;
+            o[3] += f * lo.w;
+            o[4] += f * hi.x;
+            o[5] += f * hi.y;
+            o[6] += f * hi.z;
+            o[7] += f * hi.w;
+        }
+        finish(r, e % pieces * 8, top, total, o);
+    }
+    cluster.sync();  // until the others have read this block's
 }
 
 template <typename T, int DP, int NB>
@@ -410,7 +498,18 @@ int launch(const Int8Params& f, int64_t items, cudaStream_t stream) noexcept
     const int bytes = L::kBytes + (f.table != nullptr ? std::min(L::kRows, f.Hq / f.Hk) * f.rel.total * 4 + f.max_entries : 0);
     static std::atomic<uint64_t> raised{0};
     if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention_int8");
-    kernel<<<dim3(static_cast<unsigned>(items * f.splits), (f.rows + L::kRows - 1) / L::kRows), kWarps * 32, bytes, stream>>>(f);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(f.splits);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(items * f.splits), (f.rows + L::kRows - 1) / L::kRows);
+    cfg.blockDim = L::kWarps * 32;
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = f.joined ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kernel, f);
     return launch_status("cross_attention_int8");
 }
 
@@ -423,9 +522,9 @@ int launch_rows(const Int8Params& f, int64_t items, cudaStream_t stream) noexcep
 // How a call runs: rows against the 8-bit values, keys split over blocks; or 16-bit
 // copies in the workspace and the kernels of ww_cross_attention.
 struct Plan {
-    bool few;
+    bool few, joined;  // joined: the splits are a cluster, which joins them itself
     int rows, row_blocks, splits;
-    int64_t part_rows(const ww_attention_t& p) const { return splits > 1 ? i64(p.B) * p.Hk * splits * rows : 0; }
+    int64_t part_rows(const ww_attention_t& p) const { return splits > 1 && !joined ? i64(p.B) * p.Hk * splits * rows : 0; }
 };
 
 Plan make_plan(const ww_attention_t& p, int sms) noexcept
@@ -437,7 +536,12 @@ Plan make_plan(const ww_attention_t& p, int sms) noexcept
     r.rows = static_cast<int>(rows);
     r.row_blocks = (r.rows + 31) / 32;
     const int64_t items = i64(p.B) * p.Hk * r.row_blocks, tiles = (p.Lk + kKeys - 1) / kKeys;
-    r.splits = items <= 0 || items >= sms ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({sms / items, tiles / kWarps, 128})));
+    // two blocks per SM; a block has a tile for each of its warps at least
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>({items > 0 ? 2 * sms / items : 1, tiles / 6, 128}));
+    r.splits = static_cast<int>(most);
+    // short keys: a cluster, which saves a launch
+    if (most > kCluster && tiles <= kCluster * WW_SHORT) r.splits = kCluster;
+    r.joined = r.splits > 1 && r.splits <= kCluster;
     return r;
 }
 
@@ -534,6 +638,7 @@ int few_rows(const ww_attention_int8_t& a, const Plan& plan, cudaStream_t stream
     f.D = p.D;
     f.rows = plan.rows;
     f.splits = plan.splits;
+    f.joined = plan.joined;
     f.k_b = p.k_strides[0] != 0;
     f.k_h = p.k_strides[2] != 0;
     f.v_b = p.v_strides[0] != 0;
@@ -543,7 +648,7 @@ int few_rows(const ww_attention_int8_t& a, const Plan& plan, cudaStream_t stream
     if (f.err == nullptr) return WW_ERR_DEVICE;
     const int64_t items = i64(p.B) * p.Hk;
     const int st = dp == 32 ? launch_rows<T, 32>(f, items, stream) : dp == 64 ? launch_rows<T, 64>(f, items, stream) : launch_rows<T, 128>(f, items, stream);
-    if (st != WW_SUCCESS || plan.splits == 1) return st;
+    if (st != WW_SUCCESS || plan.splits == 1 || plan.joined) return st;
     return attention_join_launch(p, static_cast<int>(items), plan.splits, plan.rows, f.part_o, f.part_lse, "cross_attention_int8", stream);
 }
 
