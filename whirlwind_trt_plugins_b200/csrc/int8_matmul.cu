@@ -57,7 +57,9 @@ struct Tiles {
     static constexpr int kWarps = BN == 64 ? 8 : 16;  // that write out
     static constexpr int kThreads = 128 + 32 * kWarps;
     static constexpr int kColumns = BN * 4 / kWarps;  // of such a warp
-    static constexpr int kStaging = 32 * 32 * sizeof(O);  // 32 rows x 32 columns
+    static constexpr int kChunk = 32;                      // of them staged at a time
+    static constexpr int kChunkRow = kChunk * sizeof(O);   // 64 or 128 bytes
+    static constexpr int kStaging = 32 * kChunkRow;
     static constexpr int kBuffers = BN == 64 ? 2 : 1;  // of a warp
     static constexpr int kOut = kStages * kStage;
     static constexpr int kScales = kOut + kWarps * kBuffers * kStaging;
@@ -196,56 +198,6 @@ __device__ __forceinline__ void pack_row(const Pair (&v)[4], uint32_t to0, uint3
     }
 }
 
-constexpr int kChunk = 32;  // columns of a tile that a warp stages at a time, rows of 64 or 128 bytes
-
-// 16-byte piece j of row r of a staged chunk, swizzled as a TMA store reads it.
-template <typename O>
-__device__ __forceinline__ uint32_t staged(int r, int j)
-{
-    constexpr int kRow = kChunk * sizeof(O);
-    return r * kRow + ((j ^ (kRow == 128 ? r & 7 : (r >> 1) & 3)) << 4);
-}
-
-// 32 sums of a lane's row into its staged chunk: times the row's scale x2, times the columns'
-// ws, plus their bias bs.
-template <typename O>
-__device__ __forceinline__ void stage_chunk(const uint32_t (&v)[32], Pair x2, const float* ws, const float* bs, uint32_t to, int lane)
-{
-#pragma unroll
-    for (int j = 0; j < kChunk; j += 8) {
-        Pair f[4];
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const float4 m = *reinterpret_cast<const float4*>(ws + j + 4 * z);
-            const float4 a = *reinterpret_cast<const float4*>(bs + j + 4 * z);
-            const uint32_t* q = v + j + 4 * z;
-            f[2 * z] = fma2(mul2(pair(__int2float_rn(q[0]), __int2float_rn(q[1])), x2), pair(m.x, m.y), pair(a.x, a.y));
-            f[2 * z + 1] = fma2(mul2(pair(__int2float_rn(q[2]), __int2float_rn(q[3])), x2), pair(m.z, m.w), pair(a.z, a.w));
-        }
-        const int piece = j * static_cast<int>(sizeof(O)) / 16;
-        pack_row<O>(f, to + staged<O>(lane, piece), to + staged<O>(lane, piece + 1));
-    }
-}
-
-// A warp's staged chunk to rows row0 .. and columns x .. of the output.
-template <typename O>
-__device__ __forceinline__ void store_chunk(const CUtensorMap& map, bool stored, void* out, int M, int N, const uint8_t* from, int x, int row0, int lane)
-{
-    if (stored) {
-        umma::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && x < N && row0 < M) store_tile(&map, umma::smem_addr(from), x, row0);
-    } else {  // rows that do not start on 16 bytes
-        __syncwarp();
-        const int byte = lane * static_cast<int>(sizeof(O));
-        for (int r = 0; r < 32 && row0 + r < M; ++r)
-            if (x + lane < N)
-                static_cast<O*>(out)[static_cast<int64_t>(row0 + r) * N + x + lane] =
-                    *reinterpret_cast<const O*>(from + staged<O>(r, byte >> 4) + (byte & 15));
-        __syncwarp();
-    }
-}
-
 template <int BN, bool PAIR, typename O>
 __global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_kernel(const __grid_constant__ MatmulParams p)
 {
@@ -373,14 +325,14 @@ __global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_k
             if (!ok) break;
             const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * BN + part * L::kColumns;
 #pragma unroll 1
-            for (int c = 0; c < L::kColumns; c += kChunk, buffer = L::kBuffers - 1 - buffer) {
+            for (int c = 0; c < L::kColumns; c += L::kChunk, buffer = L::kBuffers - 1 - buffer) {
                 const int my_out = L::kOut + (w * L::kBuffers + buffer) * L::kStaging;
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;\n" : : "n"(L::kBuffers - 1) : "memory");
                 __syncwarp();
                 uint32_t v[32];
                 umma::tmem_ld32(from + c, v);
                 umma::tmem_wait_ld32(v);
-                if (c + kChunk == L::kColumns) {  // TMEM has been read
+                if (c + L::kChunk == L::kColumns) {  // TMEM has been read
                     umma::fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
@@ -388,8 +340,39 @@ __global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_k
                         else umma::mbar_arrive(bar + (i & 1) * 8);
                     }
                 }
-                stage_chunk<O>(v, x2, scales + c, scales + L::kColumns + c, sm + my_out, lane);
-                store_chunk<O>(p.c, p.stored, p.out, p.M, p.N, base + my_out, my_column0 + c, my_row0, lane);
+#pragma unroll
+                for (int j = 0; j < L::kChunk; j += 8) {
+                    Pair f[4];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const float4 m = *reinterpret_cast<const float4*>(scales + c + j + 4 * z);
+                        const float4 a = *reinterpret_cast<const float4*>(scales + L::kColumns + c + j + 4 * z);
+                        const uint32_t* q = v + j + 4 * z;
+                        f[2 * z] = fma2(mul2(pair(__int2float_rn(q[0]), __int2float_rn(q[1])), x2), pair(m.x, m.y), pair(a.x, a.y));
+                        f[2 * z + 1] = fma2(mul2(pair(__int2float_rn(q[2]), __int2float_rn(q[3])), x2), pair(m.z, m.w), pair(a.z, a.w));
+                    }
+                    // 16-byte piece of the row, swizzled as the TMA store reads it
+                    const int piece = j * static_cast<int>(sizeof(O)) / 16;
+                    const int turn = L::kChunkRow == 128 ? lane & 7 : (lane >> 1) & 3;
+                    const uint32_t at = sm + my_out + lane * L::kChunkRow;
+                    pack_row<O>(f, at + ((piece ^ turn) << 4), at + (((piece + 1) ^ turn) << 4));
+                }
+                const int x = my_column0 + c;
+                if (p.stored) {
+                    umma::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && x < p.N && my_row0 < p.M) store_tile(&p.c, sm + my_out, x, my_row0);
+                } else {  // rows that do not start on 16 bytes
+                    __syncwarp();
+                    for (int r = 0; r < 32 && my_row0 + r < p.M; ++r) {
+                        const int turn = L::kChunkRow == 128 ? r & 7 : (r >> 1) & 3;
+                        const int byte = lane * static_cast<int>(sizeof(O));
+                        const uint8_t* from_row = base + my_out + r * L::kChunkRow + (((byte >> 4) ^ turn) << 4) + (byte & 15);
+                        if (x + lane < p.N)
+                            static_cast<O*>(p.out)[static_cast<int64_t>(my_row0 + r) * p.N + x + lane] = *reinterpret_cast<const O*>(from_row);
+                    }
+                    __syncwarp();
+                }
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" : : : "memory");
@@ -400,239 +383,6 @@ __global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_k
     if (PAIR) cluster_sync();  // until neither SM's barriers or TMEM are used by the other
     umma::fence_after_sync();
     if (warp == 2) tmem_free<PAIR>(tmem, L::kTmem);
-}
-
-// ---- rows brought to 8 bits on their way ----
-//
-// Many rows of few values: their bytes, in and out, are the bound, so they are
-// brought to 8 bits in the blocks that multiply them.  A block takes 128 rows at a time:
-// four warps load them, 16 bytes a lane, and put them as an operand of all their
-// channels into shared memory (two such places, so that the next rows are loaded
-// meanwhile); the weights come from L2 through a ring, 128 channels at a time.
-struct RowsParams {
-    CUtensorMap b, c;
-    const void* x;
-    const float* ws;
-    const void* bias;
-    void* out;
-    int64_t x_stride;
-    int32_t M, N, K, k_blocks, stages;
-    int32_t m_tiles, n_tiles;
-    int32_t stored;
-    int* err;
-};
-
-template <typename O, int P>  // P: 16-byte pieces of a lane of a row
-struct Rows {
-    static constexpr int BN = 128;
-    static constexpr int kMakers = 8;   // warps that bring rows to 8 bits
-    static constexpr int kWarps = 16;   // warps that write out, 32 rows and 32 columns each
-    static constexpr int kThreads = 128 + 32 * (kMakers + kWarps);
-    static constexpr int kAhead = P == 1 ? 4 : 2;  // rows of a maker under way
-    static constexpr int kStage = BN * kBlockK;
-    static constexpr int kStaging = 32 * 32 * sizeof(O);
-    static constexpr int kMostStages = 8;
-    // bytes: staging, scales of the columns and rows, barriers; then the rows, the ring
-    static constexpr int kScales = kWarps * kStaging;
-    static constexpr int kRowScales = kScales + kWarps * 64 * 4;
-    static constexpr int kBar = kRowScales + 2 * kTileM * 4;
-    static constexpr int kRows = (kBar + (2 * kMostStages + 8) * 8 + 16 + 1023) / 1024 * 1024;
-    static int stages(int k_blocks) { return std::min(kMostStages, (kMaxShared - 1024 - kRows - 2 * k_blocks * kTileM * kBlockK) / kStage); }
-    static int bytes(int k_blocks) { return 1024 + kRows + 2 * k_blocks * kTileM * kBlockK + stages(k_blocks) * kStage; }
-};
-
-template <typename O, int P>
-__global__ void __launch_bounds__(Rows<O, P>::kThreads, 1) int8_rows_kernel(const __grid_constant__ RowsParams p)
-{
-    using L = Rows<O, P>;
-    constexpr int BN = L::BN;
-    extern __shared__ uint8_t raw[];
-    uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
-    const uint32_t sm = umma::smem_addr(base);
-    const uint32_t full = sm + L::kBar, empty = full + L::kMostStages * 8, made = empty + L::kMostStages * 8, used = made + 16, done = used + 16,
-                   freed = done + 16, slot = freed + 16;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int row_bytes = p.k_blocks * kTileM * kBlockK;  // of 128 rows
-    const uint32_t rows = sm + L::kRows, ring = rows + 2 * row_bytes;
-    float* xscales = reinterpret_cast<float*>(base + L::kRowScales);
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            umma::mbar_init(full + s * 8, 1);
-            umma::mbar_init(empty + s * 8, 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            umma::mbar_init(made + i * 8, L::kMakers);
-            umma::mbar_init(used + i * 8, 1 + L::kWarps);
-            umma::mbar_init(done + i * 8, 1);
-            umma::mbar_init(freed + i * 8, L::kWarps);
-        }
-        umma::mbar_fence_init();
-        umma::tma_prefetch_desc(&p.b);
-    }
-    if (warp == 2) tmem_get<false>(slot, 2 * BN);
-    umma::fence_before_sync();
-    __syncthreads();
-    umma::fence_after_sync();
-    uint32_t tmem;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot) : "memory");
-    bool ok = true;
-
-    if (warp == 0) {  // loads of the weights
-        const bool leader = umma::elect_one();
-        int s = 0;
-        uint32_t parity = 1;
-        for (int m = blockIdx.x; m < p.m_tiles && ok; m += gridDim.x)
-            for (int n = 0; n < p.n_tiles && ok; ++n)
-                for (int k = 0; k < p.k_blocks && ok; ++k) {
-                    ok = wait(empty + s * 8, parity);
-                    if (ok && leader) {
-                        umma::mbar_arrive_expect_tx(full + s * 8, L::kStage);
-                        load_tile<false>(ring + s * L::kStage, &p.b, k * kBlockK, n * BN, full + s * 8);
-                    }
-                    __syncwarp();
-                    if (++s == p.stages) {
-                        s = 0;
-                        parity ^= 1;
-                    }
-                }
-    } else if (warp == 1) {  // products
-        constexpr uint32_t idesc = idesc_i8(kTileM, BN);
-        const bool leader = umma::elect_one();
-        const uint64_t a0 = umma::smem_desc_swizzled<128>(rows, 1024), b0 = umma::smem_desc_swizzled<128>(ring, 1024);
-        int s = 0, i = 0, turn = 0;
-        uint32_t parity = 0;
-        for (int m = blockIdx.x; m < p.m_tiles && ok; m += gridDim.x, ++turn) {
-            ok = wait(made + (turn & 1) * 8, (turn >> 1) & 1);
-            umma::fence_after_sync();
-            for (int n = 0; n < p.n_tiles && ok; ++n, ++i) {
-                ok = wait(freed + (i & 1) * 8, ((i >> 1) & 1) ^ 1);
-                umma::fence_after_sync();
-                for (int k = 0; k < p.k_blocks && ok; ++k) {
-                    ok = wait(full + s * 8, parity);
-                    umma::fence_after_sync();
-                    if (ok && leader) {
-                        const uint64_t a = umma::desc_advance(a0, (turn & 1) * row_bytes + k * kTileM * kBlockK), b = umma::desc_advance(b0, s * L::kStage);
-#pragma unroll
-                        for (int j = 0; j < kBlockK / 32; ++j)
-                            mma_i8<false>(tmem + (i & 1) * BN, umma::desc_advance(a, j * 32), umma::desc_advance(b, j * 32), idesc, k > 0 || j > 0);
-                        commit<false>(empty + s * 8);
-                        if (k == p.k_blocks - 1) {
-                            commit<false>(done + (i & 1) * 8);
-                            if (n == p.n_tiles - 1) commit<false>(used + (turn & 1) * 8);
-                        }
-                    }
-                    __syncwarp();
-                    if (++s == p.stages) {
-                        s = 0;
-                        parity ^= 1;
-                    }
-                }
-            }
-        }
-    } else if (warp >= 4 && warp < 4 + L::kMakers) {  // rows to 8 bits: this warp's share of the 128
-        constexpr int V = 16 / static_cast<int>(sizeof(O)), R = L::kAhead, kMine = kTileM / L::kMakers;
-        const int mine = (warp - 4) * kMine;
-        Piece<O, V> xr[R][P];
-        const auto load = [&](int m, int r0) {
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                const int64_t row = static_cast<int64_t>(m) * kTileM + mine + r0 + j;
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const int k = (i * 32 + lane) * V;
-                    if (row < p.M && k < p.K) xr[j][i].load(static_cast<const O*>(p.x) + row * p.x_stride + k);
-                    else xr[j][i].clear();
-                }
-            }
-        };
-        load(blockIdx.x, 0);  // there are no more blocks than tiles
-        int turn = 0;
-        for (int m = blockIdx.x; m < p.m_tiles && ok; m += gridDim.x, ++turn) {
-            ok = wait(used + (turn & 1) * 8, ((turn >> 1) & 1) ^ 1);
-            if (!ok) break;
-            uint8_t* to = base + L::kRows + (turn & 1) * row_bytes;
-            for (int r0 = 0; r0 < kMine; r0 += R) {
-                Pair f[R][P * V / 2];
-                float top[R];
-                RowScale scale[R];
-#pragma unroll
-                for (int j = 0; j < R; ++j) {
-                    values_of<O, V, P>(xr[j], f[j]);
-                    top[j] = largest(f[j]);
-                }
-                if (r0 + R < kMine) load(m, r0 + R);
-                else if (m + static_cast<int>(gridDim.x) < p.m_tiles) load(m + gridDim.x, 0);
-                row_maxima<32>(top, nullptr);
-                row_scales<32>(top, scale);
-#pragma unroll
-                for (int j = 0; j < R; ++j) {
-                    const int r = mine + r0 + j;
-                    if (lane == 0) xscales[(turn & 1) * kTileM + r] = scale[j].scale;
-#pragma unroll
-                    for (int i = 0; i < P; ++i) {
-                        const int k = (i * 32 + lane) * V;
-                        if (k < p.k_blocks * kBlockK)
-                            store_piece_int8<V>(reinterpret_cast<int8_t*>(to + k / kBlockK * (kTileM * kBlockK) + r * kBlockK +
-                                                                          ((((k & (kBlockK - 1)) >> 4) ^ (r & 7)) << 4) + (k & 15)),
-                                                f[j], scale[j].inv, i);
-                    }
-                }
-            }
-            umma::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) umma::mbar_arrive(made + (turn & 1) * 8);
-        }
-    } else if (warp >= 4 + L::kMakers) {  // results
-        const int w = warp - 4 - L::kMakers, quarter = warp % 4, part = w / 4;
-        float* scales = reinterpret_cast<float*>(base + L::kScales) + w * 64;  // [32] of ws, of the bias
-        const uint32_t staging = sm + w * L::kStaging;
-        float ws;
-        O bs;  // converted when it is used: the load stays under way
-        const auto ahead = [&](int n) {
-            const int x = n * BN + part * kChunk + lane;
-            ws = x < p.N ? __ldg(p.ws + x) : 0.0f;
-            bs = from_float<O>(0.0f);
-            if (x < p.N && p.bias != nullptr) bs = static_cast<const O*>(p.bias)[x];
-        };
-        ahead(0);
-        int i = 0, turn = 0;
-        for (int m = blockIdx.x; m < p.m_tiles && ok; m += gridDim.x, ++turn) {
-            float xs = 0.0f;
-            for (int n = 0; n < p.n_tiles && ok; ++n, ++i) {
-                __syncwarp();  // the scales before have been read
-                scales[lane] = ws;
-                scales[32 + lane] = to_float(bs);
-                __syncwarp();
-                ahead(n + 1 < p.n_tiles ? n + 1 : 0);
-                ok = wait(done + (i & 1) * 8, (i >> 1) & 1);
-                if (n == 0) {
-                    // the makers' scales of these rows: their barrier, so that they are seen
-                    ok = ok && wait(made + (turn & 1) * 8, (turn >> 1) & 1);
-                    xs = xscales[(turn & 1) * kTileM + quarter * 32 + lane];
-                    __syncwarp();
-                    if (lane == 0) umma::mbar_arrive(used + (turn & 1) * 8);
-                }
-                umma::fence_after_sync();
-                if (!ok) break;
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" : : : "memory");
-                __syncwarp();
-                uint32_t v[32];
-                umma::tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * BN + part * kChunk, v);
-                umma::tmem_wait_ld32(v);
-                umma::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) umma::mbar_arrive(freed + (i & 1) * 8);
-                stage_chunk<O>(v, pair(xs, xs), scales, scales + 32, staging, lane);
-                store_chunk<O>(p.c, p.stored, p.out, p.M, p.N, base + w * L::kStaging, n * BN + part * kChunk, m * kTileM + quarter * 32, lane);
-            }
-        }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" : : : "memory");
-    }
-    if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x51);
-    umma::fence_before_sync();
-    __syncthreads();
-    umma::fence_after_sync();
-    if (warp == 2) tmem_free<false>(tmem, 2 * BN);
 }
 
 // ---- few tokens ----
@@ -890,7 +640,7 @@ int run_tiles(const ww_int8_matmul_t& p, bool behind, int sms, int* err, cudaStr
         !encode_rows_map(&f.b, WW_DTYPE_INT8, p.w_q, p.N, p.K, p.w_stride, kBlockK, PAIR ? BN / 2 : BN))
         return WW_ERR_UNSUPPORTED;
     f.stored = i64(p.N) * static_cast<int>(sizeof(O)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-    if (f.stored && !encode_rows_map(&f.c, p.dtype, p.out, p.M, p.N, p.N, kChunk, 32)) return WW_ERR_UNSUPPORTED;
+    if (f.stored && !encode_rows_map(&f.c, p.dtype, p.out, p.M, p.N, p.N, L::kChunk, 32)) return WW_ERR_UNSUPPORTED;
     f.xs = p.x_scale;
     f.ws = p.w_scale;
     f.bias = p.bias;
@@ -930,47 +680,9 @@ int few(const ww_int8_matmul_t& p, bool behind, int sms, cudaStream_t stream) no
     return launch_status("int8_matmul");
 }
 
-// Many rows of few values, in pieces of 16 bytes, are brought to 8 bits on their way.
-bool rows_form(const ww_int8_matmul_t& p, int sms) noexcept
-{
-    const int bytes = p.dtype == WW_DTYPE_FLOAT ? 4 : 2;
-    if (p.x == nullptr || few_form(p) || p.K * bytes > 1024 || p.M < i64(sms) * kTileM || p.N < 64) return false;
-    return p.K * bytes % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.x_stride * bytes % 16 == 0;
-}
-
-template <typename O, int P>
-int run_rows(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
-{
-    using L = Rows<O, P>;
-    RowsParams f{};
-    if (!encode_rows_map(&f.b, WW_DTYPE_INT8, p.w_q, p.N, p.K, p.w_stride, kBlockK, L::BN)) return WW_ERR_UNSUPPORTED;
-    f.stored = i64(p.N) * static_cast<int>(sizeof(O)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-    if (f.stored && !encode_rows_map(&f.c, p.dtype, p.out, p.M, p.N, p.N, kChunk, 32)) return WW_ERR_UNSUPPORTED;
-    f.x = p.x;
-    f.ws = p.w_scale;
-    f.bias = p.bias;
-    f.out = p.out;
-    f.x_stride = p.x_stride;
-    f.M = p.M;
-    f.N = p.N;
-    f.K = p.K;
-    f.k_blocks = (p.K + kBlockK - 1) / kBlockK;
-    f.stages = L::stages(f.k_blocks);
-    f.m_tiles = (p.M + kTileM - 1) / kTileM;
-    f.n_tiles = (p.N + L::BN - 1) / L::BN;
-    f.err = device_error_slot();
-    if (f.err == nullptr) return WW_ERR_DEVICE;
-    const auto kernel = int8_rows_kernel<O, P>;
-    static std::atomic<uint64_t> raised{0};
-    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("int8_matmul");
-    kernel<<<std::min(f.m_tiles, sms), L::kThreads, L::bytes(f.k_blocks), stream>>>(f);
-    return launch_status("int8_matmul");
-}
-
 template <typename O>
 int matmul(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
 {
-    if (rows_form(p, sms)) return p.K * static_cast<int>(sizeof(O)) <= 512 ? run_rows<O, 1>(p, sms, stream) : run_rows<O, 2>(p, sms, stream);
     const bool is_few = few_form(p);
     if (is_few && few_alone(p)) return few<O>(p, false, sms, stream);
     ww_int8_matmul_t c = p;
@@ -1016,15 +728,9 @@ int check(const ww_int8_matmul_t& p) noexcept
     return WW_SUCCESS;
 }
 
-int sm_count() noexcept
-{
-    DeviceInfo d;
-    return current_device_info(&d) == WW_SUCCESS ? d.sm_count : 148;
-}
-
 int64_t workspace(const ww_int8_matmul_t& p) noexcept
 {
-    if (p.x == nullptr || p.M == 0 || p.N == 0 || (few_form(p) && few_alone(p)) || rows_form(p, sm_count())) return 0;
+    if (p.x == nullptr || p.M == 0 || p.N == 0 || (few_form(p) && few_alone(p))) return 0;
     return i64(p.M) * pitch_of(p.K) + i64(p.M) * 4;
 }
 
