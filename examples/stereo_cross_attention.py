@@ -6,8 +6,9 @@ volume and the disparity regression.
 
 The layer runs ``qk_norm_rope`` (norm and column rotation of queries and keys),
 ``cross_attention`` with a learned bias by column distance and invalid right
-pixels masked, and in training their gradients.  The data are synthetic: random
-left rows and right rows shifted by a per-row disparity, with noise.
+pixels masked, and in training their gradients.  The trained layer also runs in 8
+bits (``int8_linear``, ``quantize_kv``, ``cross_attention_int8``).  The data are
+synthetic: random left rows and right rows shifted by a per-row disparity, with noise.
 """
 from __future__ import annotations
 
@@ -59,6 +60,29 @@ class RowCrossAttention(nn.Module):
         return out.reshape(B, H, W, C).permute(0, 3, 1, 2)
 
 
+class Int8RowCrossAttention:
+    """A trained layer for inference in 8 bits: weights with a scale for each channel, tokens
+    with one each, keys and values with one for each token and head."""
+
+    def __init__(self, layer: RowCrossAttention):
+        self.layer = layer
+        self.to_q, self.to_kv = ww.quantize_tokens(layer.to_q.weight.detach()), ww.quantize_tokens(layer.to_kv.weight.detach())
+
+    @torch.no_grad()
+    def __call__(self, left, right, right_valid=None):
+        n, (B, C, H, W) = self.layer, left.shape
+        rows = lambda x: x.permute(0, 2, 3, 1).reshape(B * H, W, C).contiguous()  # noqa: E731
+        q = ww.int8_linear(rows(left), *self.to_q).view(B * H, W, n.heads, -1)
+        kv = ww.int8_linear(rows(right), *self.to_kv).view(B * H, W, 2, n.heads, -1)
+        q, k = ww.qk_norm_rope(q, kv[:, :, 0], n.q_weight, n.k_weight, n.cos, n.sin)
+        kept = [torch.empty(k.shape, device=k.device, dtype=torch.int8) for _ in range(2)]
+        kept += [torch.empty((B * H, n.heads, W), device=k.device) for _ in range(2)]
+        ww.quantize_kv(k, kv[:, :, 1], *kept)
+        mask = None if right_valid is None else right_valid.reshape(B * H, W)
+        out = ww.cross_attention_int8(q, *kept, bias_table=n.bias_table, key_mask=mask, max_distance=n.max_distance)
+        return out.reshape(B, H, W, C).permute(0, 3, 1, 2)
+
+
 def pair(B, C, H, W, max_disp, generator):
     """Left and right features, the disparity of each row and the valid right pixels."""
     wide = torch.randn((B, C, H, W + max_disp), generator=generator, device="cuda")
@@ -99,11 +123,14 @@ def main(steps: int = 150, verbose: bool = True):
     with torch.no_grad():
         left, right, disp, valid = pair(B, C, H, W, D, g)
         fetched = layer(left.bfloat16(), right.bfloat16(), valid)
+        in_8_bits = Int8RowCrossAttention(layer)(left.bfloat16(), right.bfloat16(), valid)
+        apart = (in_8_bits.float() - fetched.float()).norm() / fetched.float().norm()
         volume = ww.corr_volume((left + fetched.float()).half().contiguous(), right.half().contiguous(), D)
         estimate = ww.disparity_regression(volume * 16, ww.DISP_SOFTARGMAX, dtype=torch.float32)[:, 0]
         error = (estimate - disp[..., None]).abs()[..., D:].mean().item()
     if verbose:
-        print(f"loss {losses[0]:.4f} -> {losses[-1]:.4f}; mean disparity error {error:.3f} of {D}")
+        print(f"loss {losses[0]:.4f} -> {losses[-1]:.4f}; mean disparity error {error:.3f} of {D}; "
+              f"features in 8 bits {apart:.3f} apart")
     assert ww.device_error() == 0
     return losses, error
 

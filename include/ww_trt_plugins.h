@@ -30,6 +30,10 @@
  *   ww_qk_norm_rope           per-head norm and rotation of queries and keys, and its gradient
  *   ww_cross_attention        attention to states of another length with a bucketed relative
  *                             position bias, and its gradient
+ *   ww_layer_norm             layer norm of token rows, also into 8 bits, and its gradient
+ *   ww_int8_matmul            products in 8-bit integers, scales by token and channel
+ *   ww_quantize_kv            keys and values in 8 bits, written and read back
+ *   ww_cross_attention_int8   attention over keys and values in 8 bits
  *
  * Status codes: 0 on success.  The plugin-level ww_plugin_*_enqueue calls
  * return exactly what IPluginV3OneRuntime::enqueue returns in the reference
@@ -495,6 +499,8 @@ int ww_dequantize_kv(const ww_kv_cache_t* p, void* stream);
  * do not matter either; those of valid places are >= 0 or NaN.  Up to 128 rows (query heads of
  * a key head x tokens) the values are used as they stand, P in fp16 with the values'
  * scales in it; beyond, keys and values are rounded to q's type in the workspace.
+ * The former runs without a workspace too (fewer blocks share long keys then), the
+ * latter needs B * Lk * Hk * D * 4 bytes, rounded up to 512, at least.
  * No gradients.  D a multiple of 16. */
 typedef struct ww_attention_int8 {
     ww_attention_t attention;
@@ -626,6 +632,51 @@ int ww_plugin_qk_norm_rope_supports_format(int use_positions, int pos, const ww_
                                            int nb_outputs);
 int ww_plugin_qk_norm_rope_enqueue(int use_positions, int eps_nano, int interleaved, const ww_tensor_desc_t* in_desc,
                                    const void* const* inputs, void* const* outputs, void* stream);
+
+/* "LayerNorm" v"1" (extension): ww_layer_norm.  Inputs x [..., N], weight [N], bias [N] and
+ * with use_residual residual like x (one type: fp16, bf16 or fp32); outputs y and with
+ * use_residual the sum, like x.  Fields use_residual (0), eps_nano (eps in 1e-9, default
+ * 10000). */
+int ww_plugin_layer_norm_output_dims(int use_residual, int which, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                     ww_tensor_desc_t* out);
+int ww_plugin_layer_norm_supports_format(int use_residual, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                         int nb_outputs);
+int ww_plugin_layer_norm_enqueue(int use_residual, int eps_nano, const ww_tensor_desc_t* in_desc,
+                                 const void* const* inputs, void* const* outputs, void* stream);
+
+/* "Int8Linear" v"1" (extension): ww_int8_matmul of activations.  Inputs x [..., K] (fp16, bf16 or
+ * fp32), w_q [N, K] INT8 with K a multiple of 16, w_scale [N] fp32 and with use_bias bias [N] of
+ * x's type; output [..., N] of x's type.  Field use_bias (0).  `workspace` holds
+ * ww_plugin_int8_linear_workspace bytes (-1: no such inputs), which grow with the rows of x. */
+int ww_plugin_int8_linear_output_dims(int use_bias, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                      ww_tensor_desc_t* out);
+int ww_plugin_int8_linear_supports_format(int use_bias, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                          int nb_outputs);
+int64_t ww_plugin_int8_linear_workspace(int use_bias, const ww_tensor_desc_t* in_desc);
+int ww_plugin_int8_linear_enqueue(int use_bias, const ww_tensor_desc_t* in_desc, const void* const* inputs,
+                                  void* const* outputs, void* workspace, void* stream);
+
+/* "QuantizeKv" v"1" (extension): ww_quantize_kv of whole tensors.  Inputs k, v [B, L, H, D] (fp16 or
+ * bf16, D a multiple of 16 up to 128); outputs k_q, v_q [B, L, H, D] INT8 and k_scale, v_scale
+ * [B, H, L] fp32, as "CrossAttentionInt8" takes them.  No fields. */
+int ww_plugin_quantize_kv_output_dims(int which, int nb_inputs, const ww_tensor_desc_t* inputs, ww_tensor_desc_t* out);
+int ww_plugin_quantize_kv_supports_format(int pos, const ww_tensor_desc_t* in_out, int nb_inputs, int nb_outputs);
+int ww_plugin_quantize_kv_enqueue(const ww_tensor_desc_t* in_desc, const void* const* inputs, void* const* outputs,
+                                  void* stream);
+
+/* "CrossAttentionInt8" v"1" (extension): ww_cross_attention_int8 with scale 1 / sqrt(D).  Inputs q
+ * [B, Lq, Hq, D] (fp16 or bf16), k, v [B, Lk, Hk, D] INT8, k_scale, v_scale [B, Hk, Lk] fp32, then
+ * those that `flags` names as for "CrossAttention", whose fields it has; output like q.
+ * `workspace` holds ww_plugin_cross_attention_int8_workspace bytes for inputs of at least
+ * these sizes (-1: no such inputs). */
+int ww_plugin_cross_attention_int8_output_dims(int flags, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                               ww_tensor_desc_t* out);
+int ww_plugin_cross_attention_int8_supports_format(int flags, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                                   int nb_outputs);
+int64_t ww_plugin_cross_attention_int8_workspace(int flags, const ww_tensor_desc_t* in_desc);
+int ww_plugin_cross_attention_int8_enqueue(int flags, int max_distance, int bidirectional, int q_offset,
+                                           const ww_tensor_desc_t* in_desc, const void* const* inputs,
+                                           void* const* outputs, void* workspace, void* stream);
 
 /* Device error word written by bounded waits inside the tensor-core kernels
  * (0 = none).  There is ONE word per device, shared by every call, stream and

@@ -683,3 +683,83 @@ def test_refusals(env):
             (ValueError, lambda: ww.cross_attention_int8(k, *kept, bias_table=w[None]))]:
         with pytest.raises(error):
             call()
+
+
+def test_plugins_give_the_functions_bits(env):
+    torch, ww = env
+    from whirlwind_trt_plugins_b200 import plugins as pl
+    T = pl.TensorDesc.of
+
+    def run(p, ins, outs, *ws):
+        assert p.enqueue([T(t) for t in ins], ins, outs, *ws) == 0
+        return outs
+
+    like = torch.empty_like
+    x, r = _randn(torch, (3, 40, 64), 1, torch.float16), _randn(torch, (3, 40, 64), 2, torch.float16)
+    w, b = _randn(torch, (64,), 3, torch.float16), _randn(torch, (64,), 4, torch.float16)
+    got = run(pl.LayerNormPlugin(use_residual=1, eps_nano=2000), [x, w, b, r], [like(x), like(x)])
+    assert all(torch.equal(a, c) for a, c in zip(got, ww.layer_norm(x, w, b, 2e-6, residual=r)))
+    assert torch.equal(run(pl.LayerNormPlugin(), [x, w, b], [like(x)])[0], ww.layer_norm(x, w, b))
+    wq, ws = ww.quantize_tokens(_randn(torch, (128, 64), 5, torch.float16))
+    bias = _randn(torch, (128,), 6, torch.float16)
+    for rows in (x, x[:, :1].contiguous()):
+        p = pl.Int8LinearPlugin(use_bias=1)
+        ins = [rows, wq, ws, bias]
+        scratch = torch.empty(max(16, p.get_workspace_size([T(t) for t in ins])), device="cuda", dtype=torch.uint8)
+        out = torch.empty((*rows.shape[:2], 128), device="cuda", dtype=torch.float16)
+        assert torch.equal(run(p, ins, [out], scratch)[0], ww.int8_linear(*ins))
+    k, v = _randn(torch, (2, 900, 2, 64), 7, torch.bfloat16), _randn(torch, (2, 900, 2, 64), 8, torch.bfloat16)
+    kept = [torch.empty(k.shape, device="cuda", dtype=torch.int8) for _ in range(2)] + [torch.empty((2, 2, 900), device="cuda") for _ in range(2)]
+    want = [like(c) for c in kept]
+    run(pl.QuantizeKvPlugin(), [k, v], kept)
+    ww.quantize_kv(k, v, *want)
+    assert all(torch.equal(a, c) for a, c in zip(kept, want))
+    lens, table = torch.tensor([900, 333], device="cuda", dtype=torch.int32), _randn(torch, (8, 32), 9, torch.bfloat16)
+    mask = torch.rand((2, 900), device="cuda") >= 0.1
+    for Lq in (1, 3, 50):
+        q = _randn(torch, (2, Lq, 8, 64), 10, torch.bfloat16)
+        p = pl.CrossAttentionInt8Plugin(1, 1, 1, max_distance=64, q_offset=5)
+        ins = [q, *kept, lens, mask, table]
+        scratch = torch.empty(p.get_workspace_size([T(t) for t in ins]), device="cuda", dtype=torch.uint8)
+        ref = ww.cross_attention_int8(q, *kept, k_lens=lens, key_mask=mask, bias_table=table, max_distance=64, q_offset=5)
+        assert torch.equal(run(p, ins, [like(q)], scratch)[0], ref)
+        if Lq < 50:  # few rows also without a workspace: in other parts, so not to the bit
+            plain = run(p, ins, [like(q)])[0]
+            assert (plain.float() - ref.float()).abs().max() <= 2.0 ** -7 * ref.float().abs().max()
+    assert ww.device_error() == 0
+
+
+def test_example_layer_in_8_bits(env):
+    """The example's layer in 8 bits beside itself: 8-bit steps of 1/254 of a row's largest value."""
+    import importlib.util
+    import os
+
+    from conftest import ROOT
+    torch, ww = env
+    spec = importlib.util.spec_from_file_location("example", os.path.join(ROOT, "examples", "stereo_cross_attention.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    torch.manual_seed(0)
+    layer = m.RowCrossAttention(64, heads=2).cuda().bfloat16()
+    left, right, _, valid = m.pair(1, 64, 6, 160, 24, torch.Generator(device="cuda").manual_seed(0))
+    with torch.no_grad():
+        full = layer(left.bfloat16(), right.bfloat16(), valid).float()
+    got = m.Int8RowCrossAttention(layer)(left.bfloat16(), right.bfloat16(), valid).float()
+    assert torch.isfinite(got).all() and (got - full).norm() <= 0.05 * full.norm()
+
+
+def test_long_rows_without_workspace(env):
+    """Up to 128 rows a key head run without scratch memory through the C call."""
+    torch, ww = env
+    from whirlwind_trt_plugins_b200 import attention, layers
+    q = _randn(torch, (1, 1, 4, 64), 1, torch.float16)
+    kept = _caches(torch, 1, 9000, 2, 64, 2)
+    ref = ww.cross_attention_int8(q, *kept)
+    out = torch.empty_like(q)
+    st = [9000 * 128, 128, 64]
+    a = attention._ATTN.pack(q.data_ptr(), kept[0].data_ptr(), kept[1].data_ptr(), out.data_ptr(), *[0] * 10, 0, 256, 256, 64, *st, *st, 0, 0, 0,
+                             1, 1, 1, 9000, 4, 2, 64, 0, 128, 1, 0, 0.125) + layers._SCALES.pack(kept[2].data_ptr(), kept[3].data_ptr(), 18000, 9000, 18000, 9000)
+    assert layers._lib.ww_cross_attention_int8_workspace(a) > 0
+    assert layers._lib.ww_cross_attention_int8(a, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert (out.float() - ref.float()).abs().max() <= 2.0 ** -9 * ref.float().abs().max()

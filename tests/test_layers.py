@@ -155,3 +155,90 @@ def test_wrappers_refuse():
                  lambda: ww.cross_attention_int8(x, x, x, x, x), lambda: ww.layer_norm(None)):
         with pytest.raises(TypeError, match="CUDA tensor"):
             call()
+
+
+@pytest.fixture(scope="module")
+def pl():
+    from whirlwind_trt_plugins_b200 import plugins
+    return plugins
+
+
+def test_struct_layouts(tmp_path):
+    import shutil
+    import subprocess
+
+    from conftest import ROOT
+    layers, _ = _layers()
+    if shutil.which("gcc") is None:
+        pytest.skip("needs gcc")
+    src, exe = tmp_path / "s.c", tmp_path / "s"
+    names = "ww_layer_norm_t ww_int8_matmul_t ww_kv_cache_t ww_attention_int8_t".split()
+    at = "ww_layer_norm_t, workspace|ww_int8_matmul_t, workspace|ww_attention_t, workspace|ww_attention_int8_t, k_scale".split("|")
+    values = ", ".join([f"sizeof({n})" for n in names] + [f"offsetof({n})" for n in at])
+    src.write_text(f'#include "ww_trt_plugins.h"\n#include <stdio.h>\nint main(void) {{ size_t v[] = {{{values}}}; '
+                   'for (int i = 0; i < 8; ++i) printf("%zu ", v[i]); return 0; }\n')
+    subprocess.run(["gcc", f"-I{ROOT}/include", str(src), "-o", str(exe)], check=True)
+    got = list(map(int, subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()))
+    from whirlwind_trt_plugins_b200.attention import _ATTN
+    assert got == [layers._NORM.size, layers._MATMUL.size, layers._CACHE.size, _ATTN.size + layers._SCALES.size,
+                   layers._NORM_WS, layers._MATMUL_WS, layers._ATTN_WS, _ATTN.size]
+
+
+def test_plugin_shapes_and_formats(pl):
+    T = pl.TensorDesc
+    H, I8, F = pl.DTYPE_HALF, pl.DTYPE_INT8, pl.DTYPE_FLOAT
+    norm = pl.get_plugin_creator("LayerNorm").create_plugin({"use_residual": 1})
+    x, w = T((2, 5, 64)), T((64,))
+    assert norm.get_nb_outputs() == 2 and norm.eps_nano == 10000 and norm.clone().use_residual == 1
+    assert norm.get_output_shapes([x, w, w, x]) == [(2, 5, 64)] * 2 and norm.get_output_data_types([H] * 4) == [H, H]
+    assert all(norm.supports_format_combination(i, [x, w, w, x, x, x], 4, 2) for i in range(6))
+    assert not norm.supports_format_combination(1, [x, T((64,), F), w, x, x, x], 4, 2)
+    assert not norm.supports_format_combination(0, [T((2, 64), I8)] * 6, 4, 2) and not norm.supports_format_combination(6, [x] * 6, 4, 2)
+    for bad in ([x, w, w], [x, T((32,)), w, x], [x, w, w, T((2, 4, 64))], [T(()), w, w, T(())]):
+        with pytest.raises(ValueError):
+            norm.get_output_shapes(bad)
+    lin = pl.get_plugin_creator("Int8Linear").create_plugin({"use_bias": 1})
+    ins = [x, T((33, 64), I8), T((33,), F), T((33,))]
+    assert lin.get_output_shapes(ins) == [(2, 5, 33)]
+    assert all(lin.supports_format_combination(i, ins + [T((2, 5, 33))], 4, 1) for i in range(5))
+    assert not lin.supports_format_combination(1, [x, T((33, 64)), *ins[2:], x], 4, 1)
+    assert lin.get_workspace_size([T((700, 64)), *ins[1:]]) == 700 * 64 + 700 * 4 and lin.get_workspace_size(ins[:1] * 4) == -1
+    for bad in ([x, T((33, 72), I8), *ins[2:]], [T((2, 24)), T((33, 24), I8), *ins[2:]], ins[:3], [*ins[:3], T((32,))]):
+        with pytest.raises(ValueError):
+            lin.get_output_shapes(bad)
+    quant = pl.get_plugin_creator("QuantizeKv").create_plugin()
+    k = T((2, 7, 3, 32))
+    assert quant.get_output_shapes([k, k]) == [(2, 7, 3, 32)] * 2 + [(2, 3, 7)] * 2 and quant.get_output_data_types([H, H]) == [I8, I8, F, F]
+    outs = [T((2, 7, 3, 32), I8)] * 2 + [T((2, 3, 7), F)] * 2
+    assert all(quant.supports_format_combination(i, [k, k, *outs], 2, 4) for i in range(6))
+    for bad in ([k], [k, T((2, 7, 3, 16))], [T((2, 7, 3, 40))] * 2, [T((2, 7, 96))] * 2):
+        with pytest.raises(ValueError):
+            quant.get_output_shapes(bad)
+    attn = pl.get_plugin_creator("CrossAttentionInt8").create_plugin({"use_lens": 1, "use_bias": 1})
+    q = T((2, 1, 6, 32))
+    ins = [q, *outs, T((2,), pl.DTYPE_INT32), T((6, 16))]
+    assert attn.get_output_shapes(ins) == [(2, 1, 6, 32)] and attn.clone().use_bias == 1
+    assert all(attn.supports_format_combination(i, ins + [q], 7, 1) for i in range(8))
+    assert not attn.supports_format_combination(1, [q, k, *ins[2:], q], 7, 1) and not attn.supports_format_combination(3, ins[:3] + [q] * 5, 7, 1)
+    assert attn.get_workspace_size(ins) >= 2 * 2 * 7 * 3 * 32 * 2 and attn.get_workspace_size([q] * 7) == -1
+    for bad in (ins[:5], [q, *outs[:2], T((2, 7, 3), F), *ins[4:]], [T((2, 1, 6, 16)), *ins[1:]]):
+        with pytest.raises(ValueError):
+            attn.get_output_shapes(bad)
+
+
+def test_plugin_enqueue_refuses(pl):
+    """A rejected request gives 1, as IPluginV3OneRuntime::enqueue does, before any GPU work."""
+    T = pl.TensorDesc
+    x, w = T((4, 64)), T((64,))
+    norm = pl.LayerNormPlugin()
+    assert norm.enqueue([x, w, T((32,))], [0x1000] * 3, [0x2000], stream=0) == 1
+    assert norm.enqueue([x, w, w], [0x1000, 0x1000, 0], [0x2000], stream=0) == 1
+    lin = pl.Int8LinearPlugin()
+    ins = [T((400, 64)), T((33, 64), pl.DTYPE_INT8), T((33,), pl.DTYPE_FLOAT)]
+    assert lin.enqueue(ins, [0x1000] * 3, [0x2000], stream=0) == 1  # its workspace is missing
+    k = T((2, 7, 3, 32))
+    assert pl.QuantizeKvPlugin().enqueue([k, T((2, 7, 3, 32), pl.DTYPE_FLOAT)], [0x1000] * 2, [0x2000] * 4, stream=0) == 1
+    attn = pl.CrossAttentionInt8Plugin()
+    i8, sc = T((2, 7, 3, 32), pl.DTYPE_INT8), T((2, 3, 7), pl.DTYPE_FLOAT)
+    assert attn.enqueue([T((2, 200, 6, 32)), i8, i8, sc, sc], [0x1000] * 5, [0x2000], stream=0) == 1  # copies need their memory
+    assert attn.enqueue([T((2, 1, 6, 32)), i8, i8, sc, k], [0x1000] * 5, [0x2000], stream=0) == 1

@@ -525,6 +525,11 @@ struct Plan {
     bool few, joined;  // joined: the splits are a cluster, which joins them itself
     int rows, row_blocks, splits;
     int64_t part_rows(const ww_attention_t& p) const { return splits > 1 && !joined ? i64(p.B) * p.Hk * splits * rows : 0; }
+    void without_parts()
+    {
+        splits = std::min(splits, kCluster);
+        joined = splits > 1;
+    }
 };
 
 Plan make_plan(const ww_attention_t& p, int sms) noexcept
@@ -568,11 +573,10 @@ ww_attention_t of_copies(const ww_attention_int8_t& a) noexcept
     return p;
 }
 
-int64_t workspace(const ww_attention_int8_t& a, int sms) noexcept
+int64_t workspace(const ww_attention_int8_t& a, const Plan& plan) noexcept
 {
     const ww_attention_t& p = a.attention;
     if (p.B == 0 || p.Lq == 0) return 0;
-    const Plan plan = make_plan(p, sms);
     if (plan.few) return plan.part_rows(p) * (p.D + 1) * 4;
     const ww_attention_t q = of_copies(a);
     return 2 * copy_bytes(p) + ww_cross_attention_workspace(&q);
@@ -665,7 +669,7 @@ extern "C" {
 
 int64_t ww_cross_attention_int8_workspace(const ww_attention_int8_t* p)
 {
-    return p == nullptr || ww::check(*p) != WW_SUCCESS ? 0 : ww::workspace(*p, ww::sm_count());
+    return p == nullptr || ww::check(*p) != WW_SUCCESS ? 0 : ww::workspace(*p, ww::make_plan(p->attention, ww::sm_count()));
 }
 
 int ww_cross_attention_int8(const ww_attention_int8_t* a, void* stream)
@@ -674,15 +678,20 @@ int ww_cross_attention_int8(const ww_attention_int8_t* a, void* stream)
     const ww_attention_t& p = a->attention;
     int st = ww::check(*a);
     if (st != WW_SUCCESS || p.B == 0 || p.Lq == 0) return st;
-    const int64_t need = ww::workspace(*a, ww::sm_count());
-    if (need > 0 && p.workspace == nullptr) return WW_ERR_NULL_POINTER;
-    if (need > p.workspace_bytes) return WW_ERR_UNSUPPORTED;
+    ww::Plan plan = ww::make_plan(p, ww::sm_count());
+    if (plan.few) {
+        if (p.workspace == nullptr) plan.without_parts();
+        else if (ww::workspace(*a, plan) > p.workspace_bytes) return WW_ERR_UNSUPPORTED;
+    } else {
+        if (p.Lk > 0 && p.workspace == nullptr) return WW_ERR_NULL_POINTER;
+        if (2 * ww::copy_bytes(p) > p.workspace_bytes) return WW_ERR_UNSUPPORTED;
+    }
     ww::DeviceInfo d;
     if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const ww::Plan plan = ww::make_plan(p, d.sm_count);
     if (plan.few) return p.dtype == WW_DTYPE_HALF ? ww::few_rows<__half>(*a, plan, s) : ww::few_rows<__nv_bfloat16>(*a, plan, s);
-    const ww_attention_t q = ww::of_copies(*a);
+    ww_attention_t q = ww::of_copies(*a);
+    if (ww_cross_attention_workspace(&q) > q.workspace_bytes) q.workspace = nullptr;  // keys are not split then
     ww_kv_cache_t c{};
     c.k_cache = static_cast<int8_t*>(const_cast<void*>(p.k));
     c.v_cache = static_cast<int8_t*>(const_cast<void*>(p.v));

@@ -60,6 +60,85 @@ void contiguous_strides(const ww_tensor_desc_t& d, int64_t (&s)[3])
     s[0] = s[1] * d.dims[1];
 }
 
+bool is_float_type(int32_t t) { return t == WW_DTYPE_HALF || t == WW_DTYPE_BF16 || t == WW_DTYPE_FLOAT; }
+
+// Rows (all dims but the last) and their length; false where they do not fit.
+bool rows_of(const ww_tensor_desc_t& d, int32_t* rows, int32_t* n)
+{
+    const int64_t all = numel(d);
+    if (d.nb_dims < 1 || all < 0) return false;
+    const int64_t last = d.dims[d.nb_dims - 1], count = last > 0 ? all / last : 0;
+    if (!fits_int(last) || !fits_int(count)) return false;
+    *rows = static_cast<int32_t>(count);
+    *n = static_cast<int32_t>(last);
+    return true;
+}
+
+// Sizes of an Int8Linear call, pointers that are there (not these) for the workspace's size.
+bool int8_linear(int use_bias, const ww_tensor_desc_t* in, ww_int8_matmul_t* p)
+{
+    ww_tensor_desc_t out;
+    const int n = use_bias ? 4 : 3;
+    if (in == nullptr || ww_plugin_int8_linear_output_dims(use_bias, n, in, &out) != 0) return false;
+    for (int i = 0; i < n; ++i)
+        if (!ww_plugin_int8_linear_supports_format(use_bias, i, in, n, 1)) return false;
+    std::memset(p, 0, sizeof(*p));
+    if (!rows_of(in[0], &p->M, &p->K) || !fits_int(in[1].dims[0])) return false;
+    p->N = static_cast<int32_t>(in[1].dims[0]);
+    p->x_stride = p->w_stride = p->K;
+    p->dtype = in[0].dtype;
+    static const uint64_t kThere[2] = {};
+    p->x = p->w_scale = reinterpret_cast<const float*>(kThere);
+    p->w_q = reinterpret_cast<const int8_t*>((reinterpret_cast<uintptr_t>(kThere) + 15) / 16 * 16);
+    p->out = const_cast<uint64_t*>(kThere);
+    return true;
+}
+
+// Descriptors without the two scales behind v.
+void without_scales(const ww_tensor_desc_t* in, int n, ww_tensor_desc_t* out)
+{
+    for (int i = 0; i < n; ++i)
+        if (i < 3) out[i] = in[i];
+        else if (i >= 5) out[i - 2] = in[i];
+}
+
+// Sizes and strides of a CrossAttentionInt8 call.
+bool attention_int8(int flags, const ww_tensor_desc_t* in, ww_attention_int8_t* p)
+{
+    ww_tensor_desc_t out;
+    const int n = attention_inputs(flags) + 2;
+    if (in == nullptr || ww_plugin_cross_attention_int8_output_dims(flags, n, in, &out) != 0) return false;
+    for (int i = 0; i < n; ++i) {
+        if (!ww_plugin_cross_attention_int8_supports_format(flags, i, in, n, 1)) return false;
+        for (int j = 0; j < in[i].nb_dims; ++j)
+            if (!fits_int(in[i].dims[j])) return false;
+    }
+    std::memset(p, 0, sizeof(*p));
+    ww_attention_t& a = p->attention;
+    const ww_tensor_desc_t &q = in[0], &k = in[1];
+    a.dtype = q.dtype;
+    a.B = static_cast<int32_t>(q.dims[0]);
+    a.Lq = static_cast<int32_t>(q.dims[1]);
+    a.Hq = static_cast<int32_t>(q.dims[2]);
+    a.D = static_cast<int32_t>(q.dims[3]);
+    a.Lk = static_cast<int32_t>(k.dims[1]);
+    a.Hk = static_cast<int32_t>(k.dims[2]);
+    contiguous_strides(q, a.q_strides);
+    contiguous_strides(k, a.k_strides);
+    contiguous_strides(k, a.v_strides);
+    p->k_scale_strides[0] = p->v_scale_strides[0] = k.dims[1] * k.dims[2];
+    p->k_scale_strides[1] = p->v_scale_strides[1] = k.dims[1];
+    a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(a.D)));
+    return true;
+}
+
+// Bytes of the 16-bit copies that ww_cross_attention_int8 makes for many rows.
+int64_t attention_copies(const ww_attention_t& a)
+{
+    const int64_t one = static_cast<int64_t>(a.B) * a.Lk * a.Hk * a.D * 2;
+    return 2 * ((one + 255) / 256 * 256);
+}
+
 }  // namespace
 
 extern "C" {
@@ -571,6 +650,240 @@ int ww_plugin_qk_norm_rope_enqueue(int use_positions, int eps_nano, int interlea
     p.interleaved = interleaved;
     p.eps = static_cast<float>(eps_nano * 1e-9);
     return ww_qk_norm_rope(&p, stream) == WW_SUCCESS ? 0 : 1;
+}
+
+// ---------------------------------------------------------------- LayerNorm
+
+int ww_plugin_layer_norm_output_dims(int use_residual, int which, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                     ww_tensor_desc_t* out)
+{
+    if (inputs == nullptr || out == nullptr || nb_inputs != (use_residual ? 4 : 3) || which < 0 || which > (use_residual ? 1 : 0)) return 1;
+    const ww_tensor_desc_t& x = inputs[0];
+    if (x.nb_dims < 1 || x.nb_dims > 8) return 1;
+    for (int i = 1; i < 3; ++i)
+        if (inputs[i].nb_dims != 1 || inputs[i].dims[0] != x.dims[x.nb_dims - 1]) return 1;
+    if (use_residual && !same_shape(inputs[3], x)) return 1;
+    *out = x;
+    return 0;
+}
+
+int ww_plugin_layer_norm_supports_format(int use_residual, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                         int nb_outputs)
+{
+    if (in_out == nullptr || nb_inputs != (use_residual ? 4 : 3) || nb_outputs != (use_residual ? 2 : 1)) return 0;
+    if (pos < 0 || pos >= nb_inputs + nb_outputs || in_out[pos].format != WW_FORMAT_LINEAR) return 0;
+    if (pos == 0) return is_float_type(in_out[0].dtype);
+    return in_out[pos].dtype == in_out[0].dtype;
+}
+
+int ww_plugin_layer_norm_enqueue(int use_residual, int eps_nano, const ww_tensor_desc_t* in_desc,
+                                 const void* const* inputs, void* const* outputs, void* stream)
+{
+    if (in_desc == nullptr || inputs == nullptr || outputs == nullptr) return 1;
+    const int n = use_residual ? 4 : 3;
+    ww_tensor_desc_t out;
+    if (ww_plugin_layer_norm_output_dims(use_residual, 0, n, in_desc, &out) != 0) return 1;
+    for (int i = 0; i < n; ++i)
+        if (!ww_plugin_layer_norm_supports_format(use_residual, i, in_desc, n, use_residual ? 2 : 1)) return 1;
+    ww_layer_norm_t p;
+    std::memset(&p, 0, sizeof(p));
+    if (!rows_of(in_desc[0], &p.rows, &p.N)) return 1;
+    p.x = inputs[0];
+    p.weight = inputs[1];
+    p.bias = inputs[2];
+    p.y = outputs[0];
+    if (use_residual) {
+        p.residual = inputs[3];
+        p.sum = outputs[1];
+        if (p.rows > 0 && (p.residual == nullptr || p.sum == nullptr)) return 1;
+    }
+    if (p.weight == nullptr || p.bias == nullptr) return 1;
+    p.x_stride = p.residual_stride = p.N;
+    p.dtype = in_desc[0].dtype;
+    p.eps = static_cast<float>(eps_nano * 1e-9);
+    return ww_layer_norm(&p, stream) == WW_SUCCESS ? 0 : 1;
+}
+
+// --------------------------------------------------------------- Int8Linear
+
+int ww_plugin_int8_linear_output_dims(int use_bias, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                      ww_tensor_desc_t* out)
+{
+    if (inputs == nullptr || out == nullptr || nb_inputs != (use_bias ? 4 : 3)) return 1;
+    const ww_tensor_desc_t &x = inputs[0], &w = inputs[1];
+    if (x.nb_dims < 1 || x.nb_dims > 8 || w.nb_dims != 2 || w.dims[1] != x.dims[x.nb_dims - 1] || w.dims[1] % 16 != 0) return 1;
+    for (int i = 2; i < nb_inputs; ++i)
+        if (inputs[i].nb_dims != 1 || inputs[i].dims[0] != w.dims[0]) return 1;
+    *out = x;
+    out->dims[x.nb_dims - 1] = w.dims[0];
+    return 0;
+}
+
+int ww_plugin_int8_linear_supports_format(int use_bias, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                          int nb_outputs)
+{
+    if (in_out == nullptr || nb_inputs != (use_bias ? 4 : 3) || nb_outputs != 1) return 0;
+    if (pos < 0 || pos >= nb_inputs + nb_outputs || in_out[pos].format != WW_FORMAT_LINEAR) return 0;
+    if (pos == 0) return is_float_type(in_out[0].dtype);
+    if (pos == 1) return in_out[1].dtype == WW_DTYPE_INT8;
+    if (pos == 2) return in_out[2].dtype == WW_DTYPE_FLOAT;
+    return in_out[pos].dtype == in_out[0].dtype;
+}
+
+int64_t ww_plugin_int8_linear_workspace(int use_bias, const ww_tensor_desc_t* in_desc)
+{
+    ww_int8_matmul_t p;
+    return int8_linear(use_bias, in_desc, &p) ? ww_int8_matmul_workspace(&p) : -1;
+}
+
+int ww_plugin_int8_linear_enqueue(int use_bias, const ww_tensor_desc_t* in_desc, const void* const* inputs,
+                                  void* const* outputs, void* workspace, void* stream)
+{
+    ww_int8_matmul_t p;
+    if (inputs == nullptr || outputs == nullptr || !int8_linear(use_bias, in_desc, &p)) return 1;
+    const int64_t need = ww_int8_matmul_workspace(&p);
+    p.x = inputs[0];
+    p.w_q = static_cast<const int8_t*>(inputs[1]);
+    p.w_scale = static_cast<const float*>(inputs[2]);
+    p.bias = use_bias ? inputs[3] : nullptr;
+    if (use_bias && p.bias == nullptr) return 1;
+    p.out = outputs[0];
+    p.workspace = workspace;
+    p.workspace_bytes = workspace == nullptr ? 0 : need;
+    return ww_int8_matmul(&p, stream) == WW_SUCCESS ? 0 : 1;
+}
+
+// --------------------------------------------------------------- QuantizeKv
+
+int ww_plugin_quantize_kv_output_dims(int which, int nb_inputs, const ww_tensor_desc_t* inputs, ww_tensor_desc_t* out)
+{
+    if (inputs == nullptr || out == nullptr || nb_inputs != 2 || which < 0 || which > 3) return 1;
+    const ww_tensor_desc_t& k = inputs[0];
+    if (k.nb_dims != 4 || !same_shape(k, inputs[1]) || k.dims[3] <= 0 || k.dims[3] % 16 != 0 || k.dims[3] > 128) return 1;
+    *out = k;
+    out->dtype = WW_DTYPE_INT8;
+    if (which >= 2) {
+        out->dtype = WW_DTYPE_FLOAT;
+        out->nb_dims = 3;
+        out->dims[1] = k.dims[2];
+        out->dims[2] = k.dims[1];
+        out->dims[3] = 0;
+    }
+    return 0;
+}
+
+int ww_plugin_quantize_kv_supports_format(int pos, const ww_tensor_desc_t* in_out, int nb_inputs, int nb_outputs)
+{
+    if (in_out == nullptr || nb_inputs != 2 || nb_outputs != 4) return 0;
+    if (pos < 0 || pos >= 6 || in_out[pos].format != WW_FORMAT_LINEAR) return 0;
+    const int32_t t = in_out[pos].dtype;
+    if (pos == 0) return t == WW_DTYPE_HALF || t == WW_DTYPE_BF16;
+    return t == (pos == 1 ? in_out[0].dtype : pos < 4 ? WW_DTYPE_INT8 : WW_DTYPE_FLOAT);
+}
+
+int ww_plugin_quantize_kv_enqueue(const ww_tensor_desc_t* in_desc, const void* const* inputs, void* const* outputs,
+                                  void* stream)
+{
+    if (in_desc == nullptr || inputs == nullptr || outputs == nullptr) return 1;
+    ww_tensor_desc_t out;
+    if (ww_plugin_quantize_kv_output_dims(0, 2, in_desc, &out) != 0) return 1;
+    for (int i = 0; i < 2; ++i)
+        if (!ww_plugin_quantize_kv_supports_format(i, in_desc, 2, 4)) return 1;
+    const ww_tensor_desc_t& k = in_desc[0];
+    for (int i = 0; i < 4; ++i)
+        if (!fits_int(k.dims[i])) return 1;
+    ww_kv_cache_t p;
+    std::memset(&p, 0, sizeof(p));
+    p.k = inputs[0];
+    p.v = inputs[1];
+    p.k_cache = static_cast<int8_t*>(outputs[0]);
+    p.v_cache = static_cast<int8_t*>(outputs[1]);
+    p.k_scale = static_cast<float*>(outputs[2]);
+    p.v_scale = static_cast<float*>(outputs[3]);
+    contiguous_strides(k, p.k_strides);
+    contiguous_strides(k, p.v_strides);
+    contiguous_strides(k, p.k_cache_strides);
+    contiguous_strides(k, p.v_cache_strides);
+    p.k_scale_strides[1] = p.v_scale_strides[1] = k.dims[1];
+    p.k_scale_strides[0] = p.v_scale_strides[0] = k.dims[1] * k.dims[2];
+    p.dtype = k.dtype;
+    p.B = static_cast<int32_t>(k.dims[0]);
+    p.L = p.places = static_cast<int32_t>(k.dims[1]);
+    p.H = static_cast<int32_t>(k.dims[2]);
+    p.D = static_cast<int32_t>(k.dims[3]);
+    return ww_quantize_kv(&p, stream) == WW_SUCCESS ? 0 : 1;
+}
+
+// ------------------------------------------------------- CrossAttentionInt8
+// CrossAttention with two scales behind v.
+
+int ww_plugin_cross_attention_int8_output_dims(int flags, int nb_inputs, const ww_tensor_desc_t* inputs,
+                                               ww_tensor_desc_t* out)
+{
+    if (inputs == nullptr || nb_inputs != attention_inputs(flags) + 2) return 1;
+    ww_tensor_desc_t d[6];
+    without_scales(inputs, nb_inputs, d);
+    if (ww_plugin_cross_attention_output_dims(flags, nb_inputs - 2, d, out) != 0 || d[0].dims[3] % 16 != 0) return 1;
+    for (int i = 3; i < 5; ++i) {
+        const ww_tensor_desc_t& s = inputs[i];
+        if (s.nb_dims != 3 || s.dims[0] != d[1].dims[0] || s.dims[1] != d[1].dims[2] || s.dims[2] != d[1].dims[1]) return 1;
+    }
+    return 0;
+}
+
+int ww_plugin_cross_attention_int8_supports_format(int flags, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,
+                                                   int nb_outputs)
+{
+    if (in_out == nullptr || nb_outputs != 1 || nb_inputs != attention_inputs(flags) + 2) return 0;
+    if (pos < 0 || pos > nb_inputs || in_out[pos].format != WW_FORMAT_LINEAR) return 0;
+    if (pos == 1 || pos == 2) return in_out[pos].dtype == WW_DTYPE_INT8;
+    if (pos == 3 || pos == 4) return in_out[pos].dtype == WW_DTYPE_FLOAT;
+    ww_tensor_desc_t d[7];
+    without_scales(in_out, nb_inputs + 1, d);
+    return ww_plugin_cross_attention_supports_format(flags, pos < 3 ? pos : pos - 2, d, nb_inputs - 2, 1);
+}
+
+int64_t ww_plugin_cross_attention_int8_workspace(int flags, const ww_tensor_desc_t* in_desc)
+{
+    ww_attention_int8_t p;
+    // the 16-bit copies, and what smaller calls may want to split their keys
+    return attention_int8(flags, in_desc, &p) ? attention_copies(p.attention) + WW_PLUGIN_ATTENTION_WORKSPACE : -1;
+}
+
+int ww_plugin_cross_attention_int8_enqueue(int flags, int max_distance, int bidirectional, int q_offset,
+                                           const ww_tensor_desc_t* in_desc, const void* const* inputs,
+                                           void* const* outputs, void* workspace, void* stream)
+{
+    ww_attention_int8_t p;
+    if (inputs == nullptr || outputs == nullptr || !attention_int8(flags, in_desc, &p)) return 1;
+    ww_attention_t& a = p.attention;
+    a.q = inputs[0];
+    a.k = inputs[1];
+    a.v = inputs[2];
+    p.k_scale = static_cast<const float*>(inputs[3]);
+    p.v_scale = static_cast<const float*>(inputs[4]);
+    a.out = outputs[0];
+    const int n = attention_inputs(flags);
+    for (int i = 3; i < n; ++i) {
+        const void* in = inputs[i + 2];
+        switch (attention_role(flags, i)) {
+            case WW_PLUGIN_ATTENTION_LENS: a.k_lens = static_cast<const int32_t*>(in); break;
+            case WW_PLUGIN_ATTENTION_MASK: a.key_mask = static_cast<const uint8_t*>(in); break;
+            default:
+                a.bias_table = in;
+                a.num_buckets = static_cast<int32_t>(in_desc[i + 2].dims[1]);
+        }
+        if (in == nullptr && numel(in_desc[i + 2]) != 0) return 1;
+    }
+    a.max_distance = max_distance;
+    a.bidirectional = bidirectional;
+    a.q_offset = q_offset;
+    const int64_t have = attention_copies(a) + WW_PLUGIN_ATTENTION_WORKSPACE;
+    a.workspace_bytes = have;
+    a.workspace = workspace;
+    // parts of few rows that do not fit: without them
+    if (workspace != nullptr && static_cast<int64_t>(a.Hq / a.Hk) * a.Lq <= 128 && ww_cross_attention_int8_workspace(&p) > have) a.workspace = nullptr;
+    return ww_cross_attention_int8(&p, stream) == WW_SUCCESS ? 0 : 1;
 }
 
 }  // extern "C"

@@ -10,8 +10,8 @@
 // under the same names and version -- "CorrVolume" v"1" with field max_disp
 // (default 48), "CostStem3D" v"1" with no required field, "Nv12Decode" v"1"
 // with fields out_h / out_w (224 / 288) -- plus the fused "CorrCostStem3D" and
-// "DisparityRegression" (field mode), "CrossAttention" and "QkNormRope", which have
-// no reference counterpart.  Every method is
+// "DisparityRegression" (field mode), "CrossAttention", "QkNormRope", "LayerNorm",
+// "Int8Linear", "QuantizeKv" and "CrossAttentionInt8", which have no reference counterpart.  Every method is
 // a thin forwarder to the ww_plugin_* functions of the C ABI (plugin_core.cpp),
 // which carry the logic of the reference's IPluginV3 methods
 // (src/plugins/corr_volume/corr_volume.cpp:23-139,
@@ -41,7 +41,11 @@ enum class Op {
     kNv12Decode,
     kDisparityRegression,
     kCrossAttention,
-    kQkNormRope
+    kQkNormRope,
+    kLayerNorm,
+    kInt8Linear,
+    kQuantizeKv,
+    kCrossAttentionInt8
 };
 
 // Integer fields an op carries; every op stores all three, serialises its own.
@@ -61,6 +65,7 @@ struct Fields {
     int32_t use_positions = 0;
     int32_t interleaved = 0;
     int32_t eps_nano = 1000;
+    int32_t use_residual = 0;
 
     int attention_flags() const noexcept
     {
@@ -81,6 +86,10 @@ char const* op_name(Op op) noexcept
         case Op::kDisparityRegression: return "DisparityRegression";
         case Op::kCrossAttention: return "CrossAttention";
         case Op::kQkNormRope: return "QkNormRope";
+        case Op::kLayerNorm: return "LayerNorm";
+        case Op::kInt8Linear: return "Int8Linear";
+        case Op::kQuantizeKv: return "QuantizeKv";
+        case Op::kCrossAttentionInt8: return "CrossAttentionInt8";
     }
     return "";
 }
@@ -95,8 +104,12 @@ std::vector<char const*> op_fields(Op op)
         case Op::kNv12Decode: return {"out_h", "out_w"};
         case Op::kDisparityRegression: return {"mode"};
         case Op::kCrossAttention:
+        case Op::kCrossAttentionInt8:
             return {"use_lens", "use_mask", "use_bias", "max_distance", "bidirectional", "q_offset"};
         case Op::kQkNormRope: return {"use_positions", "interleaved", "eps_nano"};
+        case Op::kLayerNorm: return {"use_residual", "eps_nano"};
+        case Op::kInt8Linear: return {"use_bias"};
+        case Op::kQuantizeKv: return {};
     }
     return {};
 }
@@ -118,6 +131,7 @@ int32_t* field_slot(Fields& f, char const* name) noexcept
     if (std::strcmp(name, "use_positions") == 0) return &f.use_positions;
     if (std::strcmp(name, "interleaved") == 0) return &f.interleaved;
     if (std::strcmp(name, "eps_nano") == 0) return &f.eps_nano;
+    if (std::strcmp(name, "use_residual") == 0) return &f.use_residual;
     return nullptr;
 }
 
@@ -160,7 +174,11 @@ public:
     AsciiChar const* getPluginNamespace() const noexcept override { return mNamespace.c_str(); }
 
     // IPluginV3OneBuild
-    int32_t getNbOutputs() const noexcept override { return mOp == Op::kQkNormRope ? 2 : 1; }
+    int32_t getNbOutputs() const noexcept override
+    {
+        if (mOp == Op::kQuantizeKv) return 4;
+        return mOp == Op::kQkNormRope || (mOp == Op::kLayerNorm && mFields.use_residual != 0) ? 2 : 1;
+    }
 
     int32_t configurePlugin(DynamicPluginTensorDesc const*, int32_t nbInputs, DynamicPluginTensorDesc const*,
                             int32_t) noexcept override
@@ -175,7 +193,10 @@ public:
         if (nbOutputs < 1 || nbInputs < 1) return 1;
         // Nv12Decode declares fp32 and lets the format choice pick fp16 or
         // fp32 (nv12_decode.cpp:26-39); the others follow input 0.
-        for (int32_t i = 0; i < nbOutputs; ++i) out[i] = mOp == Op::kNv12Decode ? DataType::kFLOAT : in[0];
+        for (int32_t i = 0; i < nbOutputs; ++i) {
+            out[i] = mOp == Op::kNv12Decode ? DataType::kFLOAT : in[0];
+            if (mOp == Op::kQuantizeKv) out[i] = i < 2 ? DataType::kINT8 : DataType::kFLOAT;
+        }
         return 0;
     }
 
@@ -235,6 +256,28 @@ public:
                 out[0] = in[0];
                 out[1] = in[1];
                 return 0;
+            case Op::kLayerNorm:  // like x
+                if (nbInputs < 3 || in[0].nbDims < 1) return 1;
+                for (int32_t i = 0; i < nbOutputs; ++i) out[i] = in[0];
+                return 0;
+            case Op::kInt8Linear:  // [..., K] -> [..., N]
+                if (nbInputs < 3 || in[0].nbDims < 1 || in[1].nbDims != 2) return 1;
+                out[0] = in[0];
+                out[0].d[in[0].nbDims - 1] = in[1].d[0];
+                return 0;
+            case Op::kQuantizeKv:  // like k and v; [B, H, L] of each
+                if (nbInputs != 2 || in[0].nbDims != 4) return 1;
+                for (int32_t i = 0; i < 4; ++i) out[i] = in[i & 1];
+                for (int32_t i = 2; i < 4; ++i) {
+                    out[i].nbDims = 3;
+                    out[i].d[1] = in[0].d[2];
+                    out[i].d[2] = in[0].d[1];
+                }
+                return 0;
+            case Op::kCrossAttentionInt8:  // like q
+                if (nbInputs < 5 || in[0].nbDims != 4 || in[1].nbDims != 4) return 1;
+                out[0] = in[0];
+                return 0;
             case Op::kCorrCostStem3D:  // [B, Cout, D, H, W]; 8 inputs (3-stage stem): Cout = 1
                 if ((nbInputs != 4 && nbInputs != 8) || in[0].nbDims != 4) return 1;
                 if (nbInputs == 4 && in[2].nbDims != 5) return 1;
@@ -273,13 +316,35 @@ public:
             case Op::kQkNormRope:
                 return ww_plugin_qk_norm_rope_supports_format(mFields.use_positions, pos, d.data(), nbInputs,
                                                               nbOutputs) != 0;
+            case Op::kLayerNorm:
+                return ww_plugin_layer_norm_supports_format(mFields.use_residual, pos, d.data(), nbInputs,
+                                                            nbOutputs) != 0;
+            case Op::kInt8Linear:
+                return ww_plugin_int8_linear_supports_format(mFields.use_bias, pos, d.data(), nbInputs, nbOutputs) != 0;
+            case Op::kQuantizeKv:
+                return ww_plugin_quantize_kv_supports_format(pos, d.data(), nbInputs, nbOutputs) != 0;
+            case Op::kCrossAttentionInt8:
+                return ww_plugin_cross_attention_int8_supports_format(mFields.attention_flags(), pos, d.data(),
+                                                                      nbInputs, nbOutputs) != 0;
         }
         return false;
     }
 
-    size_t getWorkspaceSize(DynamicPluginTensorDesc const*, int32_t, DynamicPluginTensorDesc const*,
+    size_t getWorkspaceSize(DynamicPluginTensorDesc const* in, int32_t nbInputs, DynamicPluginTensorDesc const*,
                             int32_t) const noexcept override
     {
+        if ((mOp == Op::kInt8Linear || mOp == Op::kCrossAttentionInt8) && in != nullptr && nbInputs <= 8) {
+            // of the largest shapes; the smaller ones need no more
+            std::array<ww_tensor_desc_t, 8> d{};
+            for (int i = 0; i < nbInputs; ++i) {
+                d[i] = to_ww(in[i].desc);
+                for (int j = 0; j < d[i].nb_dims && j < 8; ++j) d[i].dims[j] = in[i].max.d[j];
+            }
+            const int64_t n = mOp == Op::kInt8Linear
+                                  ? ww_plugin_int8_linear_workspace(mFields.use_bias, d.data())
+                                  : ww_plugin_cross_attention_int8_workspace(mFields.attention_flags(), d.data());
+            return n > 0 ? static_cast<size_t>(n) : 0;
+        }
         // the others use no scratch memory
         return mOp == Op::kCrossAttention ? WW_PLUGIN_ATTENTION_WORKSPACE : 0;
     }
@@ -296,7 +361,8 @@ public:
                     void* const* outputs, void* workspace, cudaStream_t stream) noexcept override
     {
         // Descriptors of the inputs: 2 (CorrVolume), 7 or 3 (CostStem3D), 4 or 8 (fused),
-        // 3 to 6 (CrossAttention), 6 or 8 (QkNormRope).
+        // 3 to 6 (CrossAttention), 6 or 8 (QkNormRope), 3 or 4 (LayerNorm, Int8Linear), 2 (QuantizeKv),
+        // 5 to 8 (CrossAttentionInt8).
         std::array<ww_tensor_desc_t, 8> d{};
         const int nin = mNbInputs;
         if (nin < 1 || nin > 8) return 1;
@@ -328,6 +394,17 @@ public:
             case Op::kQkNormRope:
                 return ww_plugin_qk_norm_rope_enqueue(mFields.use_positions, mFields.eps_nano, mFields.interleaved,
                                                       d.data(), inputs, outputs, stream);
+            case Op::kLayerNorm:
+                return ww_plugin_layer_norm_enqueue(mFields.use_residual, mFields.eps_nano, d.data(), inputs, outputs,
+                                                    stream);
+            case Op::kInt8Linear:
+                return ww_plugin_int8_linear_enqueue(mFields.use_bias, d.data(), inputs, outputs, workspace, stream);
+            case Op::kQuantizeKv:
+                return ww_plugin_quantize_kv_enqueue(d.data(), inputs, outputs, stream);
+            case Op::kCrossAttentionInt8:
+                return ww_plugin_cross_attention_int8_enqueue(mFields.attention_flags(), mFields.max_distance,
+                                                              mFields.bidirectional, mFields.q_offset, d.data(), inputs,
+                                                              outputs, workspace, stream);
         }
         return 1;
     }
@@ -370,6 +447,7 @@ public:
     IPluginV3* createPlugin(AsciiChar const*, PluginFieldCollection const* fc, TensorRTPhase) noexcept override
     {
         Fields f;
+        if (mOp == Op::kLayerNorm) f.eps_nano = 10000;
         if (fc != nullptr && fc->fields != nullptr) {
             // First field of a name with data wins; absent or empty keeps the default.
             std::vector<char const*> names(fc->nbFields);
@@ -423,6 +501,18 @@ struct CrossAttentionCreator final : WwCreator {
 struct QkNormRopeCreator final : WwCreator {
     QkNormRopeCreator() : WwCreator(Op::kQkNormRope) {}
 };
+struct LayerNormCreator final : WwCreator {
+    LayerNormCreator() : WwCreator(Op::kLayerNorm) {}
+};
+struct Int8LinearCreator final : WwCreator {
+    Int8LinearCreator() : WwCreator(Op::kInt8Linear) {}
+};
+struct QuantizeKvCreator final : WwCreator {
+    QuantizeKvCreator() : WwCreator(Op::kQuantizeKv) {}
+};
+struct CrossAttentionInt8Creator final : WwCreator {
+    CrossAttentionInt8Creator() : WwCreator(Op::kCrossAttentionInt8) {}
+};
 
 }  // namespace ww_trt
 
@@ -432,9 +522,13 @@ using ww_trt::CorrCostStem3DCreator;
 using ww_trt::CorrVolumeCreator;
 using ww_trt::CostStem3DCreator;
 using ww_trt::CrossAttentionCreator;
+using ww_trt::CrossAttentionInt8Creator;
 using ww_trt::DisparityRegressionCreator;
+using ww_trt::Int8LinearCreator;
+using ww_trt::LayerNormCreator;
 using ww_trt::Nv12DecodeCreator;
 using ww_trt::QkNormRopeCreator;
+using ww_trt::QuantizeKvCreator;
 
 REGISTER_TENSORRT_PLUGIN(CorrVolumeCreator);
 REGISTER_TENSORRT_PLUGIN(CostStem3DCreator);
@@ -443,3 +537,7 @@ REGISTER_TENSORRT_PLUGIN(Nv12DecodeCreator);
 REGISTER_TENSORRT_PLUGIN(DisparityRegressionCreator);
 REGISTER_TENSORRT_PLUGIN(CrossAttentionCreator);
 REGISTER_TENSORRT_PLUGIN(QkNormRopeCreator);
+REGISTER_TENSORRT_PLUGIN(LayerNormCreator);
+REGISTER_TENSORRT_PLUGIN(Int8LinearCreator);
+REGISTER_TENSORRT_PLUGIN(QuantizeKvCreator);
+REGISTER_TENSORRT_PLUGIN(CrossAttentionInt8Creator);

@@ -30,6 +30,11 @@ Reference plugins (paths relative to the reference project):
   ``bidirectional`` (1), ``q_offset`` (0).
 * ``QkNormRope`` v1 (extension, two outputs): fields ``use_positions``,
   ``interleaved``, ``eps_nano`` (eps in 1e-9, 1000).
+* ``LayerNorm`` v1 (extension; two outputs with a residual): fields
+  ``use_residual``, ``eps_nano`` (10000).
+* ``Int8Linear`` v1 (extension): field ``use_bias``.
+* ``QuantizeKv`` v1 (extension, four outputs): no fields.
+* ``CrossAttentionInt8`` v1 (extension): the fields of ``CrossAttention``.
 
 Descriptors are :class:`TensorDesc` (dims, dtype, format); dtypes use
 TensorRT's numbering (0 = kFLOAT, 1 = kHALF, 2 = kINT8, 3 = kINT32, 4 = kBOOL, 7 = kBF16), format 0 = kLINEAR.
@@ -42,7 +47,8 @@ from dataclasses import dataclass, field
 from . import lib
 
 __all__ = ["TensorDesc", "CorrVolumePlugin", "CostStem3DPlugin", "CorrCostStem3DPlugin", "Nv12DecodePlugin",
-           "DisparityRegressionPlugin", "CrossAttentionPlugin", "QkNormRopePlugin", "PluginCreator", "get_plugin_creator", "registered_creators"]
+           "DisparityRegressionPlugin", "CrossAttentionPlugin", "QkNormRopePlugin",
+           "LayerNormPlugin", "Int8LinearPlugin", "QuantizeKvPlugin", "CrossAttentionInt8Plugin", "PluginCreator", "get_plugin_creator", "registered_creators"]
 
 DTYPE_FLOAT = 0
 DTYPE_HALF = 1
@@ -375,6 +381,134 @@ class QkNormRopePlugin(_PluginBase):
                                                     ctypes.c_void_p(_stream(stream)))
 
 
+class LayerNormPlugin(_PluginBase):
+    """``LayerNorm`` (extension): inputs x [..., N], weight, bias [N] and with
+    ``use_residual`` residual; outputs y and with ``use_residual`` the sum."""
+    NAME = "LayerNorm"
+
+    def __init__(self, use_residual: int = 0, eps_nano: int = 10000):
+        super().__init__()
+        self.use_residual, self.eps_nano = int(use_residual), int(eps_nano)
+
+    @property
+    def NB_OUTPUTS(self) -> int:
+        return 2 if self.use_residual else 1
+
+    def get_fields_to_serialize(self) -> dict:
+        return {"use_residual": self.use_residual, "eps_nano": self.eps_nano}
+
+    def get_output_data_types(self, input_types) -> list:
+        return super().get_output_data_types(input_types) * self.NB_OUTPUTS
+
+    def get_output_shapes(self, inputs) -> list:
+        shapes = []
+        for which in range(self.NB_OUTPUTS):
+            out = _Desc()
+            if lib().ww_plugin_layer_norm_output_dims(self.use_residual, which, len(inputs), _descs(inputs),
+                                                      ctypes.byref(out)) != 0:
+                raise ValueError("LayerNorm takes x [..., N], weight [N], bias [N] (and a residual with use_residual)")
+            shapes.append(TensorDesc._from_c(out).dims)
+        return shapes
+
+    def supports_format_combination(self, pos: int, in_out, nb_inputs: int, nb_outputs: int) -> bool:
+        return bool(lib().ww_plugin_layer_norm_supports_format(self.use_residual, pos, _descs(in_out), nb_inputs,
+                                                               nb_outputs))
+
+    def enqueue(self, input_desc, inputs, outputs, stream=None) -> int:
+        return lib().ww_plugin_layer_norm_enqueue(self.use_residual, self.eps_nano, _descs(input_desc), _ptrs(inputs),
+                                                  _ptrs(outputs), ctypes.c_void_p(_stream(stream)))
+
+
+class Int8LinearPlugin(_PluginBase):
+    """``Int8Linear`` (extension): inputs x [..., K], w_q [N, K] int8, w_scale [N] fp32
+    and with ``use_bias`` bias [N]; output [..., N]."""
+    NAME = "Int8Linear"
+
+    def __init__(self, use_bias: int = 0):
+        super().__init__()
+        self.use_bias = int(use_bias)
+
+    def get_fields_to_serialize(self) -> dict:
+        return {"use_bias": self.use_bias}
+
+    def get_output_shapes(self, inputs) -> list:
+        out = _Desc()
+        if lib().ww_plugin_int8_linear_output_dims(self.use_bias, len(inputs), _descs(inputs), ctypes.byref(out)) != 0:
+            raise ValueError("Int8Linear takes x [..., K], w_q [N, K] with K % 16 == 0, w_scale [N] (and bias [N])")
+        return [TensorDesc._from_c(out).dims]
+
+    def supports_format_combination(self, pos: int, in_out, nb_inputs: int, nb_outputs: int) -> bool:
+        return bool(lib().ww_plugin_int8_linear_supports_format(self.use_bias, pos, _descs(in_out), nb_inputs,
+                                                                nb_outputs))
+
+    def get_workspace_size(self, inputs) -> int:
+        """Bytes for inputs of these descriptors (of the largest ones, for a range)."""
+        return lib().ww_plugin_int8_linear_workspace(self.use_bias, _descs(inputs))
+
+    def enqueue(self, input_desc, inputs, outputs, workspace=None, stream=None) -> int:
+        ws = None if workspace is None else ctypes.c_void_p(workspace.data_ptr())
+        return lib().ww_plugin_int8_linear_enqueue(self.use_bias, _descs(input_desc), _ptrs(inputs), _ptrs(outputs), ws,
+                                                   ctypes.c_void_p(_stream(stream)))
+
+
+class QuantizeKvPlugin(_PluginBase):
+    """``QuantizeKv`` (extension): inputs k, v [B, L, H, D]; outputs k_q, v_q int8 like
+    them and k_scale, v_scale [B, H, L] fp32."""
+    NAME = "QuantizeKv"
+    NB_OUTPUTS = 4
+
+    def get_fields_to_serialize(self) -> dict:
+        return {}
+
+    def get_output_data_types(self, input_types) -> list:
+        return [DTYPE_INT8, DTYPE_INT8, DTYPE_FLOAT, DTYPE_FLOAT]
+
+    def get_output_shapes(self, inputs) -> list:
+        shapes = []
+        for which in range(4):
+            out = _Desc()
+            if lib().ww_plugin_quantize_kv_output_dims(which, len(inputs), _descs(inputs), ctypes.byref(out)) != 0:
+                raise ValueError("QuantizeKv takes k and v [B, L, H, D], D a multiple of 16 up to 128")
+            shapes.append(TensorDesc._from_c(out).dims)
+        return shapes
+
+    def supports_format_combination(self, pos: int, in_out, nb_inputs: int, nb_outputs: int) -> bool:
+        return bool(lib().ww_plugin_quantize_kv_supports_format(pos, _descs(in_out), nb_inputs, nb_outputs))
+
+    def enqueue(self, input_desc, inputs, outputs, stream=None) -> int:
+        return lib().ww_plugin_quantize_kv_enqueue(_descs(input_desc), _ptrs(inputs), _ptrs(outputs),
+                                                   ctypes.c_void_p(_stream(stream)))
+
+
+class CrossAttentionInt8Plugin(CrossAttentionPlugin):
+    """``CrossAttentionInt8`` (extension): ``CrossAttention`` with k, v in int8 and k_scale,
+    v_scale [B, Hk, Lk] fp32 behind them."""
+    NAME = "CrossAttentionInt8"
+
+    def get_output_shapes(self, inputs) -> list:
+        out = _Desc()
+        if lib().ww_plugin_cross_attention_int8_output_dims(self._flags, len(inputs), _descs(inputs),
+                                                            ctypes.byref(out)) != 0:
+            raise ValueError("CrossAttentionInt8 takes q [B, Lq, Hq, D], k, v [B, Lk, Hk, D], k_scale, v_scale "
+                             "[B, Hk, Lk] and the inputs its fields name")
+        return [TensorDesc._from_c(out).dims]
+
+    def supports_format_combination(self, pos: int, in_out, nb_inputs: int, nb_outputs: int) -> bool:
+        return bool(lib().ww_plugin_cross_attention_int8_supports_format(self._flags, pos, _descs(in_out), nb_inputs,
+                                                                         nb_outputs))
+
+    def get_workspace_size(self, inputs) -> int:
+        """Bytes for inputs of these descriptors (of the largest ones, for a range)."""
+        return lib().ww_plugin_cross_attention_int8_workspace(self._flags, _descs(inputs))
+
+    def enqueue(self, input_desc, inputs, outputs, workspace=None, stream=None) -> int:
+        """workspace: a device buffer of get_workspace_size() bytes, or None for up to 128 queries a key head."""
+        ws = None if workspace is None else ctypes.c_void_p(workspace.data_ptr())
+        return lib().ww_plugin_cross_attention_int8_enqueue(
+            self._flags, self.max_distance, self.bidirectional, self.q_offset, _descs(input_desc), _ptrs(inputs),
+            _ptrs(outputs), ws, ctypes.c_void_p(_stream(stream)))
+
+
 @dataclass
 class PluginCreator:
     """IPluginCreatorV3One counterpart: name, version, field names, create."""
@@ -412,7 +546,17 @@ _CREATORS = {
                                                                   "max_distance": 128, "bidirectional": 1,
                                                                   "q_offset": 0}),
     ("QkNormRope", "1"): PluginCreator(QkNormRopePlugin, {"use_positions": 0, "interleaved": 0, "eps_nano": 1000}),
+    ("LayerNorm", "1"): PluginCreator(LayerNormPlugin, {"use_residual": 0, "eps_nano": 10000}),
+    ("Int8Linear", "1"): PluginCreator(Int8LinearPlugin, {"use_bias": 0}),
+    ("QuantizeKv", "1"): PluginCreator(QuantizeKvPlugin, {}),
+    ("CrossAttentionInt8", "1"): PluginCreator(CrossAttentionInt8Plugin, {"use_lens": 0, "use_mask": 0, "use_bias": 0,
+                                                                          "max_distance": 128, "bidirectional": 1,
+                                                                          "q_offset": 0}),
 }
+
+
+for _name in ("ww_plugin_int8_linear_workspace", "ww_plugin_cross_attention_int8_workspace"):
+    getattr(lib(), _name).restype = ctypes.c_int64
 
 
 def get_plugin_creator(name: str, version: str = "1") -> PluginCreator:
