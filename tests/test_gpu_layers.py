@@ -58,7 +58,7 @@ def _within(got, ref, bound, what):
 # widths), rows beyond a block's registers; one row and one value
 NORMS = [(1, 8), (3, 32), (1000, 64), (77, 128), (513, 256), (40, 320), (33, 512), (9, 704), (2000, 1024), (5, 1032), (6, 4096),
          (4, 8192), (3, 9000), (2, 20000), (3, 32776), (1, 1), (7, 2), (50, 17), (300, 129), (6, 511), (129, 1337), (3, 5001),
-         (2, 16389), (1, 40001), (0, 64)]
+         (2, 16389), (1, 40001), (0, 64), (3001, 33), (1999, 251), (700, 505), (2500, 1001), (900, 2047), (301, 8191)]
 
 
 def _norm_reference(torch, h, w, b, eps):
@@ -148,6 +148,30 @@ def test_layer_norm_strides_and_empty_sums(env, n):
     dx, dw, db = ww.layer_norm_backward(none, none, w, mean[:0].contiguous(), rstd[:0].contiguous())
     assert dx.shape == none.shape and not dw.any() and not db.any()
     assert ww.layer_norm(none, w, b).shape == none.shape
+
+
+@pytest.mark.parametrize("off", [1, 3, 8])
+@pytest.mark.parametrize("n", [100, 600, 1336])
+def test_layer_norm_rows_that_begin_anywhere(env, n, off):
+    """Rows off 16 bytes by themselves, or all tensors alike, have the bits of the same rows elsewhere."""
+    torch, ww = env
+    rows = 700
+    x, dy, r = (_randn(torch, (rows, n), s, torch.float16) for s in (1, 2, 3))
+    w, b = _randn(torch, (n,), 4, torch.float16), _randn(torch, (n,), 5, torch.float16)
+
+    def moved(t):
+        m = torch.empty(t.numel() + off, device="cuda", dtype=t.dtype)[off:].view(t.shape)
+        return m.copy_(t)
+
+    y, h, mean, rstd = ww.layer_norm(x, w, b, residual=r, return_stats=True)
+    got = ww.layer_norm(moved(x), moved(w), moved(b), residual=moved(r), return_stats=True)
+    assert torch.equal(got[1], h)
+    ref, mag, *_ = _norm_reference(torch, h, w, b, 1e-5)
+    _within(got[0], ref, U["f16"] * ref.abs() + F * mag + TINY["f16"], "y")
+    one = ww.layer_norm_backward(dy, h, w, mean, rstd, dsum=r)
+    two = ww.layer_norm_backward(moved(dy), moved(h), moved(w), mean, rstd, dsum=moved(r))
+    for a, c in zip(one, two):  # in another order of the sums
+        assert (a.float() - c.float()).abs().max() <= 2.0 ** -8 * a.float().abs().max()
 
 
 def test_layer_norm_large_mean_and_nonfinite(env):

@@ -4,8 +4,12 @@
 // Bound: HBM (writing: 2 bytes a value read, 1 written, and 4 a row; reading the
 // reverse).  A row is held by a group of lanes with 16 bytes each of the 16-bit side,
 // so that both sides of a warp lie side by side; the row's largest magnitude takes
-// log2(lanes) shuffles.  A group has kRows rows under way.  Scales stand by head, so
-// that attention reads those of a head's keys as a run.
+// log2(lanes) shuffles, and a lane divides for each row of the group.  Where rows come
+// from and go is worked out by a thread each and kept in shared memory.  Scales stand
+// by head, so that attention reads those of a head's keys as a run.
+//
+// Measured, 2 x 40001 tokens of 8 heads of 128, fp16, keys and values: written (492 MB) in
+// 88 us, read back (492 MB) in 83: 5.6 and 5.9 TB/s.
 #include "rows.cuh"
 
 #include <algorithm>
@@ -14,10 +18,9 @@ namespace ww {
 namespace {
 
 constexpr int kBlock = 256;
-#ifndef WW_WROWS
-#define WW_WROWS 4
-#endif
-constexpr int kRows = 2, kWriteRows = WW_WROWS;  // rows of a group, reading and writing
+// Rows of a group under way, reading and writing (2 x 40001 x 8 rows of 128 written and read
+// back: 4 rows written at a time 171 us, 2 185).
+constexpr int kRows = 2, kWriteRows = 4;
 
 struct CacheSide {
     const void* x;

@@ -13,11 +13,16 @@
 // variance from the deviations, so that a large mean costs nothing), held by a
 // group of 4 to 32 lanes or, where a warp's registers do not hold it, by a block;
 // loads are 16 bytes a lane where rows start on 16 bytes, else single values.
-// The gradient runs one resident round of blocks: a lane owns the same columns of
-// all its rows, so the weight's and bias's sums stay in registers; the next row's
-// loads are under way while a row is computed.  Sums are joined per block in shared
-// memory and over blocks by a second kernel, both in a fixed order.
+// Both directions run one resident round of blocks, the next rows' loads under way
+// while rows are computed.  In the gradient a lane owns the same columns of all its
+// rows, so the weight's and bias's sums stay in registers; they are joined per
+// block in shared memory and over blocks by a second kernel, both in a fixed order.
 // Rows beyond a block's registers are read again from L2 for each step.
+//
+// Measured: 469248 rows of 256, fp16, 480 MB: 78 us, 6.1 TB/s; their gradient with dsum,
+// bf16, 961 MB: 153 us with the join, 6.3 TB/s.  Gradient of 9001 rows of 1337, fp32, 144 MB:
+// 33.5 us (single loads; pieces of 16 bytes with the rows' ends masked took 52).
+// 40000 rows of 1337 in fp16, single loads of 2 bytes: 98 us for 214 MB, instructions.
 #include "rows.cuh"
 
 #include <algorithm>
@@ -28,30 +33,21 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kLongBlock = 1024;
-#ifndef WW_ROWS
-#define WW_ROWS 2
-#endif
-#ifndef WW_BROWS
-#define WW_BROWS 2
-#endif
-#ifndef WW_RES
-#define WW_RES 768
-#endif
-#ifndef WW_B8
-#define WW_B8 3
-#endif
-#ifndef WW_BBLOCKS
-#define WW_BBLOCKS 2
-#endif
-#ifndef WW_FBLOCKS
-#define WW_FBLOCKS 4
-#endif
-constexpr int kForwardRows = WW_ROWS, kBackwardRows = WW_BROWS;
-__host__ __device__ constexpr int forward_rows(int v, int pieces, int group) { return v > 1 && pieces == 1 && group > 0 ? kForwardRows : 1; }
-__host__ __device__ constexpr int forward_blocks(int pieces) { return pieces == 1 ? WW_FBLOCKS : pieces < 4 ? 3 : 2; }
-// Rows of a group under way in the gradient's kernel, and resident blocks of it.
-__host__ __device__ constexpr int backward_rows(int v, int pieces, int group) { return v > 1 && pieces == 1 && group > 0 ? kBackwardRows : 1; }
-__host__ __device__ constexpr int backward_blocks(int pieces) { return pieces == 1 ? WW_BBLOCKS : 2; }
+// Rows of a group that are under way at a time, and blocks of a resident round, by V (values
+// of a piece), pieces a lane and lanes a row.
+// Rows of 256 in fp16, forward: 2 rows and 4 blocks 78 us; 3 blocks 85, 4 rows and 2 blocks 81,
+// 1 row and 6 blocks 89.  Their gradient with dsum, bf16: 2 rows and 2 blocks 153 us; 1 row and
+// 3 blocks 194.
+__host__ __device__ constexpr int rows_at_once(int v, int pieces, int group) { return v > 1 && pieces == 1 && group > 0 ? 2 : 1; }
+__host__ __device__ constexpr int forward_blocks(int pieces) { return pieces == 1 ? 4 : pieces < 4 ? 3 : 2; }
+constexpr int kBackwardBlocks = 2;
+// Threads of an SM's blocks where a block holds a row.  Gradient of 9001 rows of 1337 in
+// fp32 (8 single values a lane): 768 threads 33.5 us; 512 and 1024, which spills, 40 and 38.
+// Forward, the same rows: 768 20.9 us, 1024, of which not all are resident, 27.
+int forward_threads(bool pieces) { return pieces ? 1024 : 768; }
+int backward_threads(bool pieces, int bytes, int per_lane) { return per_lane == 8 ? 768 : pieces && bytes == 4 ? 1024 : 512; }
+// Blocks of a row that the compiler keeps registers for, so that these threads fit.
+__host__ __device__ constexpr int backward_row_blocks(int v, int pieces) { return v == 1 && pieces == 8 ? 3 : v == 4 ? 2 : 1; }
 
 struct NormParams {
     const void *x, *r, *w, *b;
@@ -257,7 +253,7 @@ __global__ void __launch_bounds__(kLongBlock) layer_norm_long_kernel(const __gri
 }
 
 template <typename T, int V, int P, int GROUP, int R, bool DSUM>
-__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROUP ? backward_blocks(P) : V == 1 && P == 8 ? WW_B8 : 1) layer_norm_backward_kernel(const __grid_constant__ NormParams p)
+__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROUP ? kBackwardBlocks : backward_row_blocks(V, P)) layer_norm_backward_kernel(const __grid_constant__ NormParams p)
 {
     constexpr int E = P * V / 2;
     constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block side by side
@@ -518,14 +514,14 @@ int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cuda
     const RowForm form = row_form(p.N, pieces ? V : 1, 4, false);
     const auto go = [&](auto kernel, auto with_residual, int r) {
         const int groups = (form.group ? kBlock / form.group : 1) * r;
-        const int resident = form.group ? forward_blocks(form.pieces) : std::max(1, (pieces ? 1024 : 768) / form.threads);
+        const int resident = form.group ? forward_blocks(form.pieces) : std::max(1, forward_threads(pieces) / form.threads);
         const unsigned grid = static_cast<unsigned>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + groups - 1) / groups));
         if (p.residual == nullptr) kernel<<<grid, form.threads, 0, stream>>>(f);
         else with_residual<<<grid, form.threads, 0, stream>>>(f);
     };
 #define WW_NORM(V, P, GROUP) \
-    go(layer_norm_kernel<T, V, P, GROUP, forward_rows(V, P, GROUP), false>, layer_norm_kernel<T, V, P, GROUP, forward_rows(V, P, GROUP), true>, \
-       forward_rows(V, P, GROUP))
+    go(layer_norm_kernel<T, V, P, GROUP, rows_at_once(V, P, GROUP), false>, layer_norm_kernel<T, V, P, GROUP, rows_at_once(V, P, GROUP), true>, \
+       rows_at_once(V, P, GROUP))
     const int id = form.group * 100 + form.pieces;
     if (form.threads == 0) layer_norm_long_kernel<T><<<p.rows, kLongBlock, 0, stream>>>(f);
     else if (!pieces)
@@ -567,9 +563,9 @@ BackwardPlan backward_plan(const ww_layer_norm_t& p, int sms) noexcept
     const int v = r.pieces ? 16 / bytes : 1;
     r.form = row_form(p.N, v, 2, true);
     const int groups = r.form.group ? kBlock / r.form.group : 1;
-    int resident = backward_blocks(r.form.pieces);
-    if (r.form.group == 0 && r.form.threads > 0) resident = std::max(1, (r.form.pieces == 8 ? WW_RES : 512) / r.form.threads);
-    const int at_once = groups * backward_rows(v, r.form.pieces, r.form.group);
+    int resident = kBackwardBlocks;
+    if (r.form.group == 0 && r.form.threads > 0) resident = std::max(1, backward_threads(r.pieces, bytes, r.form.pieces) / r.form.threads);
+    const int at_once = groups * rows_at_once(v, r.form.pieces, r.form.group);
     r.blocks = static_cast<int>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + at_once - 1) / at_once));
     const int columns = (p.N + kBlock - 1) / kBlock;
     r.splits = std::max(1, std::min(p.rows, 4 * sms / columns));
@@ -589,8 +585,8 @@ int backward(const ww_layer_norm_t& p, const BackwardPlan& plan, cudaStream_t st
         else with_sum<<<plan.blocks, form.threads, 0, stream>>>(f);
     };
 #define WW_NORM(V, P, GROUP) \
-    go(layer_norm_backward_kernel<T, V, P, GROUP, backward_rows(V, P, GROUP), false>, \
-       layer_norm_backward_kernel<T, V, P, GROUP, backward_rows(V, P, GROUP), true>)
+    go(layer_norm_backward_kernel<T, V, P, GROUP, rows_at_once(V, P, GROUP), false>, \
+       layer_norm_backward_kernel<T, V, P, GROUP, rows_at_once(V, P, GROUP), true>)
     const int id = form.group * 100 + form.pieces;
     if (form.threads == 0) {
         layer_norm_backward_long_kernel<T><<<p.rows, kLongBlock, 0, stream>>>(f);
