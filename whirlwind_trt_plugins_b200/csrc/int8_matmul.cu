@@ -679,6 +679,23 @@ int few(const ww_int8_matmul_t& p, bool behind, int sms, cudaStream_t stream) no
     return launch_status("int8_matmul");
 }
 
+// Channels of a tile: 64 or 128 on an SM, 256 x 256 on a pair; the form whose rounds end
+// soonest, by clocks of a stage of K and of a round's start and end (fitted to the times below).
+// us with 64, 128, 256 channels: 64 x 4096 x 4096 11.6, 12.9, 15.3; 300 x 4096 x 4096 19.2, 13.2,
+// 15.6; 1777 x 1000 x 1111 10.1, 8.7, 12.5; 1024 x 4096 x 4096 34.6, 22.4, 16.5; 2048^3 19.2, 13.3,
+// 11.0; 19200 x 320 x 320 9.5, 9.0, 10.5; 4096 x 512 x 1024 8.5, 7.3, 7.7.
+int tile_form(const ww_int8_matmul_t& p, int sms) noexcept
+{
+    const int64_t k_blocks = (p.K + kBlockK - 1) / kBlockK;
+    const auto time = [&](int rows, int channels, int slots, int stage, int round) {
+        const int64_t tiles = ((i64(p.M) + rows - 1) / rows) * ((p.N + channels - 1) / channels);
+        return (tiles + slots - 1) / slots * (k_blocks * stage + round);
+    };
+    const int64_t narrow = time(kTileM, 64, sms, 510, 600), one = time(kTileM, 128, sms, 660, 1000),
+                  two = time(2 * kTileM, 256, sms / 2, 700, 2900);
+    return two <= narrow && two <= one ? 256 : one <= narrow ? 128 : 64;
+}
+
 template <typename O>
 int matmul(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
 {
@@ -703,12 +720,11 @@ int matmul(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
     if (is_few) return few<O>(c, behind, sms, stream);
     int* err = device_error_slot();
     if (err == nullptr) return WW_ERR_DEVICE;
-    const int64_t rows = (p.M + 127) / 128;
-    if (rows * ((p.N + 255) / 256) >= sms && p.N > 128)
-        return run_tiles<256, true, O>(c, behind, sms, err, stream);
-    if (rows * ((p.N + 127) / 128) >= sms / 2 && p.N > 64)
-        return run_tiles<128, false, O>(c, behind, sms, err, stream);
-    return run_tiles<64, false, O>(c, behind, sms, err, stream);
+    switch (tile_form(c, sms)) {
+    case 256: return run_tiles<256, true, O>(c, behind, sms, err, stream);
+    case 128: return run_tiles<128, false, O>(c, behind, sms, err, stream);
+    default: return run_tiles<64, false, O>(c, behind, sms, err, stream);
+    }
 }
 
 int check(const ww_int8_matmul_t& p) noexcept
