@@ -276,7 +276,7 @@ def test_layer_norm_int8(env, shape, dt, residual):
 
 # (M, K, N): few tokens (to 16, within shared memory and beyond), tiles of 64, 128 and 256 channels, partial tiles in every
 # direction, K below and off a stage, rows of the output off 16 bytes, several tiles a block
-PRODUCTS = [(1, 1, 1), (1, 64, 16), (1, 4096, 100), (3, 100, 33), (8, 1000, 257), (9, 130, 48), (16, 4096, 64), (16, 8192, 40), (17, 64, 8), (2, 9000, 700), (5, 20000, 30),
+PRODUCTS = [(1, 1, 1), (1, 64, 16), (1, 4096, 100), (3, 100, 33), (8, 1000, 257), (9, 130, 48), (16, 4096, 64), (16, 8192, 40), (17, 64, 8), (2, 9000, 700), (5, 20000, 30), (12, 4096, 1000), (30, 1000, 4099), (64, 512, 520), (65, 3000, 128), (128, 8192, 264), (20, 131, 20000), (9, 20000, 136),
             (100, 33, 200), (128, 128, 64), (129, 129, 65), (300, 1000, 1111), (1000, 256, 768), (2500, 300, 520), (5000, 144, 513),
             (4096, 512, 1024), (700, 2048, 4104), (0, 64, 64), (5, 64, 0)]
 
