@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
         }
     }
     if (p.part == nullptr) return;
+    start_launch_behind();  // the join, which waits for this grid's end
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float* sums = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + which) * p.N;
@@ -432,27 +433,24 @@ __global__ void __launch_bounds__(kBlock) layer_norm_columns_kernel(const __grid
     p.part[(static_cast<int64_t>(blockIdx.y) * 2 + 1) * p.N + c] = db;
 }
 
-// Joins the blocks' sums: 8 columns a block (a sector of each part), 128 threads of each
+// Joins the blocks' sums: 8 columns a block (a sector of each part), 32 threads of each
 // over the parts.
-constexpr int kJoinColumns = 8, kJoinLanes = 128;
+constexpr int kJoinColumns = 8;
 template <typename T>
-__global__ void __launch_bounds__(kJoinColumns * kJoinLanes) layer_norm_join_kernel(const float* part, int parts, int N, T* dw, T* db)
+__global__ void __launch_bounds__(kJoinColumns * 32) layer_norm_join_kernel(const float* part, int parts, int N, T* dw, T* db)
 {
-    __shared__ float sums[kJoinLanes][kJoinColumns + 1];
+    __shared__ float sums[32][kJoinColumns + 1];
     const int at = threadIdx.x % kJoinColumns, lane = threadIdx.x / kJoinColumns;
     const int64_t all = 2 * static_cast<int64_t>(N), c = static_cast<int64_t>(blockIdx.x) * kJoinColumns + at;
     wait_for_launches_before();
     float s = 0.0f;
     if (c < all)
-#pragma unroll 8
-        for (int k = lane; k < parts; k += kJoinLanes) s += part[k * all + c];
+#pragma unroll 10
+        for (int k = lane; k < parts; k += 32) s += part[k * all + c];
     sums[lane][at] = s;
     __syncthreads();
-    if (threadIdx.x >= 32 * kJoinColumns) return;
     const int column = threadIdx.x / 32;
-    s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kJoinLanes / 32; ++k) s += sums[threadIdx.x % 32 + 32 * k][column];
+    s = sums[threadIdx.x % 32][column];
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     const int64_t to = static_cast<int64_t>(blockIdx.x) * kJoinColumns + column;
     if (threadIdx.x % 32 == 0 && to < all) {
@@ -611,7 +609,7 @@ int backward(const ww_layer_norm_t& p, const BackwardPlan& plan, cudaStream_t st
 #undef WW_NORM
     const int st = launch_status("layer_norm_backward");
     if (st != WW_SUCCESS || !sums) return st;
-    launch_behind(layer_norm_join_kernel<T>, dim3((2u * p.N + kJoinColumns - 1) / kJoinColumns), dim3(kJoinColumns * kJoinLanes), 0, stream, f.part, plan.parts(), p.N,
+    launch_behind(layer_norm_join_kernel<T>, dim3((2u * p.N + kJoinColumns - 1) / kJoinColumns), dim3(kJoinColumns * 32), 0, stream, f.part, plan.parts(), p.N,
                   static_cast<T*>(p.dweight), static_cast<T*>(p.dbias));
     return launch_status("layer_norm_backward");
 }
