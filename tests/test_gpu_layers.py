@@ -214,6 +214,51 @@ def test_layer_norm_autograd(env):
         torch.autograd.grad(g.sum(), x)
 
 
+def test_layer_norm_autograd_of_one_result(env):
+    """Gradients where only the sum or only the normed rows are used: zeros for what does not reach the loss."""
+    torch, ww = env
+    x, r = (_randn(torch, (5, 40), s, torch.float32).requires_grad_(True) for s in (1, 2))
+    w, b = (_randn(torch, (40,), s, torch.float32).requires_grad_(True) for s in (3, 4))
+    e = _randn(torch, (5, 40), 5, torch.float32)
+    got = torch.autograd.grad((ww.layer_norm_autograd(x, w, b, 1e-5, r)[1] * e).sum(), (x, r, w, b))
+    assert torch.equal(got[0], e) and torch.equal(got[1], e) and not got[2].any() and not got[3].any()
+    y, h = ww.layer_norm_autograd(x, w, b, 1e-5, r)
+    got = torch.autograd.grad((y * e).sum(), (x, r, w, b))
+    _, mean, rstd = ww.layer_norm(h.detach(), w.detach(), b.detach(), return_stats=True)
+    ref = ww.layer_norm_backward(e, h.detach(), w.detach(), mean, rstd)
+    assert all(torch.equal(g, f) for g, f in zip(got, (ref[0], *ref)))
+
+
+@pytest.mark.parametrize("n", [24, 40, 60])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_layer_norm_gradient_of_large_equal_values(env, n, dt):
+    """Rows of one large value: xh is 0 although mean rstd passes fp32's range, and so it is in lanes beyond a row."""
+    torch, ww = env
+    t = _type(torch, dt)
+    x, w, dy = torch.full((9, n), 2.0 ** 122, device="cuda", dtype=t), _randn(torch, (n,), 1, t), _randn(torch, (9, n), 2, t)
+    mean, rstd = torch.full((9,), 2.0 ** 122, device="cuda"), torch.full((9,), 316.0, device="cuda")
+    dx, dw, db = ww.layer_norm_backward(dy, x, w, mean, rstd)
+    g = dy.double() * w.double()
+    ref = 316 * (g - g.mean(-1, keepdim=True))
+    _within(dx, ref, U[dt] * ref.abs() + 316 * 2.0 ** -18 * (g.abs() + g.abs().mean(-1, keepdim=True)), "dx")
+    assert not dw.any()
+    _within(db, dy.double().sum(0), U[dt] * dy.double().sum(0).abs() + 2.0 ** -18 * dy.double().abs().sum(0), "dbias")
+
+
+def test_outputs_apart_from_inputs(env):
+    torch, ww = env
+    x = torch.zeros((8, 64), device="cuda", dtype=torch.float16)
+    wq, ws = ww.quantize_tokens(torch.ones((64, 64), device="cuda"))
+    kept = [torch.zeros((1, 4, 2, 32), device="cuda", dtype=torch.int8)] * 2 + [torch.zeros((1, 2, 4), device="cuda")] * 2
+    q = x.view(1, 8, 2, 32)
+    both = torch.zeros((16, 64), device="cuda", dtype=torch.float16)
+    for call in (lambda: ww.layer_norm(x, out=x), lambda: ww.layer_norm(both[:8], residual=both[4:12], out=both[8:]),
+                 lambda: ww.int8_linear(x, wq, ws, out=x), lambda: ww.cross_attention_int8(q, *kept, out=q)):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    assert ww.layer_norm(both[:8], out=both[8:]).data_ptr() == both[8:].data_ptr()
+
+
 # ---------------------------------------------------------------- 8 bits
 
 def _int8_host(x):
@@ -277,6 +322,7 @@ def test_layer_norm_int8(env, shape, dt, residual):
 # (M, K, N): few tokens (to 16, within shared memory and beyond), tiles of 64, 128 and 256 channels, partial tiles in every
 # direction, K below and off a stage, rows of the output off 16 bytes, several tiles a block
 PRODUCTS = [(1, 1, 1), (1, 64, 16), (1, 4096, 100), (3, 100, 33), (8, 1000, 257), (9, 130, 48), (16, 4096, 64), (16, 8192, 40), (17, 64, 8), (2, 9000, 700), (5, 20000, 30), (12, 4096, 1000), (30, 1000, 4099), (64, 512, 520), (65, 3000, 128), (128, 8192, 264), (20, 131, 20000), (9, 20000, 136),
+            (1, 64, 70001), (4, 33, 70000), (1, 16, 263000), (20, 128, 64), (24, 640, 100), (32, 1025, 72), (33, 384, 96), (40, 900, 130),
             (100, 33, 200), (128, 128, 64), (129, 129, 65), (300, 1000, 1111), (1000, 256, 768), (2500, 300, 520), (5000, 144, 513),
             (4096, 512, 1024), (700, 2048, 4104), (0, 64, 64), (5, 64, 0)]
 

@@ -278,8 +278,10 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
         dw[i] = db[i] = pair(0.0f, 0.0f);
         if (p.w == nullptr) w[i] = pair(1.0f, 1.0f);
     }
-    // what lies beyond the row stays 0 in x and dy, and with it in every sum but xh (-mean rstd), which only meets zeros;
-    // so do rows beyond the last
+    // What lies beyond the row stays 0 in dy, and with it in every sum; so do rows beyond the last.  x is 0 there as well,
+    // with a mean of 0 (-mean rstd times 0 is NaN where it passes fp32's range); few single values, where that is a
+    // select each, take the row's last value instead (rows of 1337 in fp32 31 us and 32.4; 16 values a lane would spill).
+    constexpr bool kLast = V == 1 && P <= 8;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (kGroups * R);
     int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + group;
     const T* xp = static_cast<const T*>(p.x) + row0 * p.xs + column.first;
@@ -295,12 +297,16 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
             const bool real = at + j * kGroups < p.rows;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
+                if constexpr (kLast) {
+                    xr[j][i].clear();
+                    if (real) xr[j][i].load(xp + j * kGroups * p.xs + (min(column(i), p.N - 1) - column.first));
+                }
                 if (real && column(i) < p.N) {
-                    xr[j][i].load(xp + j * kGroups * p.xs + i * column.kNext);
+                    if constexpr (!kLast) xr[j][i].load(xp + j * kGroups * p.xs + i * column.kNext);
                     gr[j][i].load(gp + j * kGroups * p.gs + i * column.kNext);
                     if constexpr (DSUM) sr[j][i].load(sp + j * kGroups * p.ds + i * column.kNext);
                 } else {
-                    xr[j][i].clear();
+                    if constexpr (!kLast) xr[j][i].clear();
                     gr[j][i].clear();
                     if constexpr (DSUM) sr[j][i].clear();
                 }
@@ -320,9 +326,12 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
             values_of<T, V, P>(gr[j], g[j]);
             if constexpr (DSUM) values_of<T, V, P>(sr[j], d[j]);
             rs[j] = rstd[j];
-            const Pair nm = pair(-mean[j], -mean[j]), r2 = pair(rs[j], rs[j]);
+            const Pair r2 = pair(rs[j], rs[j]);
 #pragma unroll
-            for (int i = 0; i < E; ++i) xh[j][i] = mul2(add2(xh[j][i], nm), r2);
+            for (int i = 0; i < E; ++i) {
+                const bool out0 = !kLast && column(2 * i / V) >= p.N, out1 = !kLast && column((2 * i + 1) / V) >= p.N;
+                xh[j][i] = mul2(add2(xh[j][i], pair(out0 ? 0.0f : -mean[j], out1 ? 0.0f : -mean[j])), r2);
+            }
         }
         if (base + step < p.rows) {
             xp += x_step;

@@ -13,7 +13,8 @@ them.  (The reference library has none; the formulas stand in
 * ``cross_attention_int8`` -- ``cross_attention`` over such keys and values
 
 Rows are the last dim of a tensor, with unit stride; the dims before it must
-collapse to one stride.  Results do not overlap inputs.  All functions are also
+collapse to one stride.  Results do not overlap inputs (an ``out`` that does is
+refused).  All functions are also
 names of the package itself.
 """
 from __future__ import annotations
@@ -90,6 +91,18 @@ def _int8_rows(shape):
     return _empty((*shape[:-1], pitch), _Torch.int8)[..., :n], pitch
 
 
+def _apart(out, **inputs):
+    """A caller's output shares no memory with what the call reads."""
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for name, t in inputs.items():
+        if t is not None and t.numel():
+            size = t.element_size()
+            end = t.data_ptr() + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+            if lo < end and t.data_ptr() < hi:
+                raise ValueError(f"out shares memory with {name}")
+
+
 def _norm_args(x, weight, bias, eps, residual):
     T = _Torch.get()
     at = _first(x, "x")
@@ -121,6 +134,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, residual=None, retu
         with _place(x, stream):
             return layer_norm(x, weight, bias, eps, residual, return_stats, out)
     y = _new(x, out, "out")
+    if out is not None:
+        _apart(out, x=x, residual=residual, weight=weight, bias=bias)
     got = (y,)
     total = 0
     if residual is not None:
@@ -244,7 +259,10 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
         with _place(x, stream):
             return _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, None)
     shape = (*x.shape[:-1], channels)
-    out = _empty(shape, dtype) if out is None else _out(out, shape, dtype, x.device, "out")
+    if out is None:
+        out = _empty(shape, dtype)
+    else:
+        _apart(_out(out, shape, dtype, x.device, "out"), x=x, x_scale=x_scale, w_q=w_q, w_scale=w_scale, bias=bias)
     p = x.data_ptr()
     a = _MATMUL.pack(p if x_scale is None else 0, 0 if x_scale is None else p, _ptr(x_scale), w_q.data_ptr(),
                      w_scale.data_ptr(), _ptr(bias), out.data_ptr(), 0, 0, xs, xs, ws, dt, rows, k, channels)
@@ -384,6 +402,9 @@ def cross_attention_int8(q, k_cache, v_cache, k_scale, v_scale, scale: float | N
                                         max_distance, bidirectional, q_offset, return_lse, out)
     if scale is None:
         scale = 1.0 / math.sqrt(D) if D else 1.0
+    if out is not None:
+        _apart(_new(q, out, "out"), q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, k_lens=k_lens,
+               key_mask=key_mask, bias_table=bias_table)
     out = _new(q, out, "out")
     lse = _empty((B, Hq, Lq), T.f32) if return_lse else None
     a = _ATTN.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(k_lens),
@@ -414,6 +435,7 @@ def _functions():
     class LayerNorm(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, weight, bias, residual, eps):
+            ctx.set_materialize_grads(False)  # a result that nothing reads costs nothing
             got = layer_norm(x, weight, bias, eps, residual, return_stats=True)
             ctx.save_for_backward(x if residual is None else got[1], weight, got[-2], got[-1])
             ctx.more = bias is not None, residual is not None
@@ -424,6 +446,9 @@ def _functions():
         def backward(ctx, dy, dsum=None):
             x, weight, mean, rstd = ctx.saved_tensors
             bias, residual = ctx.more
+            if dy is None:
+                dw = None if weight is None else torch.zeros_like(weight)
+                return dsum, dw, dw if bias else None, dsum if residual else None, None
             dx, dw, db = layer_norm_backward(_regular(dy), x, weight, mean, rstd, None if dsum is None else _regular(dsum))
             return dx, dw, db if bias else None, dx if residual else None, None
 
@@ -432,5 +457,7 @@ def _functions():
 
 def layer_norm_autograd(x, weight=None, bias=None, eps: float = 1e-5, residual=None):
     """``layer_norm`` as a torch function of x, weight, bias and residual that can be
-    differentiated once: y, with a residual (y, sum)."""
+    differentiated once: y, with a residual (y, sum).  (A backward pass can be captured into
+    a CUDA graph as any of torch's: no eager graph of the same leaves may be alive, since
+    torch runs a leaf's accumulation on the stream where it was first used.)"""
     return _functions().apply(x, weight, bias, residual, eps)
