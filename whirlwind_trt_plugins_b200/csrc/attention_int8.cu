@@ -44,7 +44,7 @@ constexpr int kKeys = 32;          // of a warp's tile
 // SM each do not all find room at once: 2 x 8 key heads of 128, 40001 keys, 60 us and 37.
 constexpr int kCluster = 4;
 constexpr int kShort = 32;          // tiles of a cluster's block up to which a call takes no more splits
-constexpr int kMostRows = 128;     // of a key head, in blocks of up to 32
+constexpr int kMostRows = 128;     // of a key head, in blocks of up to 32, that run without copies
 constexpr float kRescale = 8.0f;   // log2 growth of a maximum that is left in P
 constexpr float kHead = 6.0f;      // P times 2^6
 
@@ -161,17 +161,25 @@ __global__ void __launch_bounds__(Layout<DP, NB>::kWarps * 32, 2) attention_int8
     // query rows, a warp a row: row r is head g * group + r / Lq, token r % Lq; the rest zeros.
     // A row is multiplied by a power of two that brings its largest value to [2^14, 2^15).
     float* row_scales = reinterpret_cast<float*>(base + L::kRowScale);
-    for (int r = warp; r < kRows; r += kWarps) {
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int d = lane * 4;
-        if (r < rows && d < p.D) {
-            const T* from = static_cast<const T*>(p.q) + b * p.q_strides[0] + ((row0 + r) % p.Lq) * p.q_strides[1] +
-                            (g * group + (row0 + r) / p.Lq) * p.q_strides[2] + d;
-            const uint2 u = __ldg(reinterpret_cast<const uint2*>(from));
-            const T* t = reinterpret_cast<const T*>(&u);
+    constexpr int kQueries = (kRows + kWarps - 1) / kWarps;  // of a warp, their loads under way together
+    uint2 raw_q[kQueries];
+    const int d = lane * 4;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = to_float(t[j]);
-        }
+    for (int i = 0; i < kQueries; ++i) {
+        const int r = warp + i * kWarps;
+        raw_q[i] = make_uint2(0, 0);
+        if (r < rows && d < p.D)
+            raw_q[i] = __ldg(reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + b * p.q_strides[0] + ((row0 + r) % p.Lq) * p.q_strides[1] +
+                                                            (g * group + (row0 + r) / p.Lq) * p.q_strides[2] + d));
+    }
+#pragma unroll
+    for (int i = 0; i < kQueries; ++i) {
+        const int r = warp + i * kWarps;
+        if (r >= kRows) break;
+        const T* t = reinterpret_cast<const T*>(&raw_q[i]);
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = to_float(t[j]);
         const float top = row_max<32>(max_nan(max_nan(fabsf(x[0]), fabsf(x[1])), max_nan(fabsf(x[2]), fabsf(x[3]))), nullptr);
         int e = 0;  // 0 for rows that hold NaN, infinities or nothing
         if (top > 0.0f && top < INFINITY) e = 14 - max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);
@@ -533,11 +541,25 @@ struct Plan {
     }
 };
 
-Plan make_plan(const ww_attention_t& p, int sms) noexcept
+// Copies cost 5 bytes a value and two launches, but are converted once for all rows.  us in 8 bits and by copies:
+// more than 64 rows (converted 3 or 4 times), 8 x 8 key heads of 64 and 128, 1500 keys, 128 rows 31 and 29, 45 and 38,
+// 1 x 8, 40001 keys 77 and 64, 117 and 93 -- but 1 x 4, 300 keys 12 both; 64 rows 22 and 24, 30 and 33, 47 and 57, 69 and 89.
+// Short keys of more blocks than are resident (a block's start and end): 64 x 8 of 64 and 128, 100 keys, 32 rows 20 and
+// 15, 25 and 22, 48 rows 34 and 15, 44 and 22; 16 rows 12 and 15, 16 and 22; 1250 keys, 32 rows 53 and 84, 81 and 160.
+constexpr int64_t kManyKeys = 1 << 16;  // of all items and key heads
+constexpr int kShortKeys = 512;
+bool by_copies(const ww_attention_t& p, int64_t rows, int sms) noexcept
+{
+    if (rows > kMostRows) return true;
+    const int64_t heads = i64(p.B) * p.Hk, row_blocks = (rows + 31) / 32;
+    return (rows > 64 && heads * p.Lk >= kManyKeys) || (rows > 16 && p.Lk < kShortKeys && p.Lk > 0 && heads * row_blocks > 2 * sms);
+}
+
+Plan make_plan(const ww_attention_t& p, int sms, bool copies_fit = true) noexcept
 {
     Plan r{};
     const int64_t rows = i64(p.Hq / p.Hk) * p.Lq;
-    r.few = rows <= kMostRows;
+    r.few = rows <= kMostRows && !(copies_fit && by_copies(p, rows, sms));
     if (!r.few) return r;
     r.rows = static_cast<int>(rows);
     r.row_blocks = (r.rows + 31) / 32;
@@ -679,7 +701,7 @@ int ww_cross_attention_int8(const ww_attention_int8_t* a, void* stream)
     const ww_attention_t& p = a->attention;
     int st = ww::check(*a);
     if (st != WW_SUCCESS || p.B == 0 || p.Lq == 0) return st;
-    ww::Plan plan = ww::make_plan(p, ww::sm_count());
+    ww::Plan plan = ww::make_plan(p, ww::sm_count(), p.workspace != nullptr);
     if (plan.few) {
         if (p.workspace == nullptr) plan.without_parts();
         else if (ww::workspace(*a, plan) > p.workspace_bytes) return WW_ERR_UNSUPPORTED;
