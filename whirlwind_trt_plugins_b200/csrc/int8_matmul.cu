@@ -42,15 +42,22 @@ struct MatmulParams {
     int32_t m_tiles, n_tiles, band;
     int32_t behind;  // the operands are written by the launch before
     int32_t stored;  // the output is stored by TMA
+    int32_t a_bytes, block, stages;  // bytes of a block of K: of the tokens, in all; stages of the ring
     int* err;
 };
 
-template <int BN, bool PAIR, typename O>
+// U: blocks of K of a stage.  A stage costs its two barriers (waits, arrivals) whatever it holds, 150 ns next to the 95 of a
+// block's products in tiles of 64 channels: those take 2 at a time, 4 where the tokens leave room for three stages.
+// One round of 8 tiles, 16 tokens, K = 8192: 18.1 us with 1, 14.7 with 2, 12.3 with 4.
+constexpr int kFewRows = 32;  // of a tile, up to which 4 blocks are a stage
+template <int BN, bool PAIR, int U, typename O>
 struct Tiles {
+    static constexpr int kUnit = U;
     static constexpr int kA = kTileM * kBlockK;
     static constexpr int kB = (PAIR ? BN / 2 : BN) * kBlockK;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = BN == 64 ? 6 : sizeof(O) == 2 ? 5 : 4;
+    static constexpr int kRing = (BN == 64 ? 6 : sizeof(O) == 2 ? 5 : 4) * kStage;
+    static constexpr int kMostStages = 16;  // where the tokens do not fill a tile
     static constexpr int kWarps = BN == 64 ? 8 : 16;  // that write out
     static constexpr int kThreads = 128 + 32 * kWarps;
     static constexpr int kColumns = BN * 4 / kWarps;  // of such a warp
@@ -58,12 +65,14 @@ struct Tiles {
     static constexpr int kChunkRow = kChunk * sizeof(O);   // 64 or 128 bytes
     static constexpr int kStaging = 32 * kChunkRow;
     static constexpr int kBuffers = BN == 64 ? 2 : 1;  // of a warp
-    static constexpr int kOut = kStages * kStage;
+    static constexpr int kOut = kRing;
     static constexpr int kScales = kOut + kWarps * kBuffers * kStaging;
     static constexpr int kBar = kScales + kWarps * kColumns * 8;
-    static constexpr int kBytes = kBar + (2 * kStages + 4) * 8 + 16 + 1024;
+    static constexpr int kBytes = kBar + (2 * kMostStages + 4) * 8 + 16 + 1024;
     static constexpr int kTmem = 2 * BN;
     static_assert(kBytes <= kMaxShared, "shared memory");
+    static_assert(kRing + kA <= kBytes, "products may read a whole tile from the last stage on");
+    static_assert(kRing >= 2 * U * (U == 4 ? kFewRows * kBlockK + kB : kStage), "two stages");
 };
 
 // ---- instructions of a pair of SMs ----
@@ -195,15 +204,15 @@ __device__ __forceinline__ void pack_row(const Pair (&v)[4], uint32_t to0, uint3
     }
 }
 
-template <int BN, bool PAIR, typename O>
-__global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_kernel(const __grid_constant__ MatmulParams p)
+template <int BN, bool PAIR, int U, typename O>
+__global__ void __launch_bounds__(Tiles<BN, PAIR, U, O>::kThreads, 1) int8_matmul_kernel(const __grid_constant__ MatmulParams p)
 {
-    using L = Tiles<BN, PAIR, O>;
-    constexpr int S = L::kStages;
+    using L = Tiles<BN, PAIR, U, O>;
+    const int S = p.stages;
     extern __shared__ uint8_t raw[];
     uint8_t* base = raw + ((1024 - (umma::smem_addr(raw) & 1023)) & 1023);
     const uint32_t sm = umma::smem_addr(base);
-    const uint32_t full = sm + L::kBar, empty = full + S * 8, done = empty + S * 8, freed = done + 16, slot = freed + 16;
+    const uint32_t full = sm + L::kBar, empty = full + L::kMostStages * 8, done = empty + L::kMostStages * 8, freed = done + 16, slot = freed + 16;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = PAIR ? cluster_rank() : 0;
     if (threadIdx.x == 0) {
@@ -230,54 +239,58 @@ __global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_k
     const int tiles = p.m_tiles * p.n_tiles, step = PAIR ? gridDim.x / 2 : gridDim.x, start = PAIR ? blockIdx.x / 2 : blockIdx.x;
     bool ok = true;
 
-    if (warp == 0) {  // loads
-        const bool leader = umma::elect_one();
+    if (warp == 0 && umma::elect_one()) {  // loads
         int s = 0;
-        uint32_t parity = 1;
+        uint32_t parity = 1, to = sm;
         for (int t = start; t < tiles && ok; t += step) {
             int m, n;
             tile_at(p, t, m, n);
             const int row = (m * (PAIR ? 2 : 1) + static_cast<int>(rank)) * kTileM, channel = n * BN + static_cast<int>(rank) * (BN / 2);
-            for (int k = 0; k < p.k_blocks && ok; ++k) {
-                ok = wait(empty + s * 8, parity);
-                if (ok && leader) {
-                    const uint32_t to = sm + s * L::kStage;
+            for (int k = 0; k < p.k_blocks && ok; k += L::kUnit) {  // blocks beyond the last are zeros
+                ok = umma::mbar_poll(empty + s * 8, parity);
+                if (ok) {
                     const uint32_t bar = PAIR ? in_block(full + s * 8, 0) : full + s * 8;
-                    if (rank == 0) umma::mbar_arrive_expect_tx(full + s * 8, L::kStage * (PAIR ? 2 : 1));
-                    load_tile<PAIR>(to, &p.a, k * kBlockK, row, bar);
-                    load_tile<PAIR>(to + L::kA, &p.b, k * kBlockK, channel, bar);
+                    if (rank == 0) umma::mbar_arrive_expect_tx(full + s * 8, L::kUnit * p.block * (PAIR ? 2 : 1));
+#pragma unroll
+                    for (int u = 0; u < L::kUnit; ++u) {
+                        load_tile<PAIR>(to + u * p.block, &p.a, (k + u) * kBlockK, row, bar);
+                        load_tile<PAIR>(to + u * p.block + p.a_bytes, &p.b, (k + u) * kBlockK, channel, bar);
+                    }
                 }
-                __syncwarp();
+                to += L::kUnit * p.block;
                 if (++s == S) {
                     s = 0;
+                    to = sm;
                     parity ^= 1;
                 }
             }
         }
-    } else if (warp == 1 && rank == 0) {  // products
+    } else if (warp == 1 && rank == 0 && umma::elect_one()) {  // products
         constexpr uint32_t idesc = idesc_i8(PAIR ? 2 * kTileM : kTileM, BN);
-        const bool leader = umma::elect_one();
-        const uint64_t a0 = umma::smem_desc_swizzled<128>(sm, 1024), b0 = umma::smem_desc_swizzled<128>(sm + L::kA, 1024);
-        int s = 0, i = 0;
+        const uint64_t a0 = umma::smem_desc_swizzled<128>(sm, 1024), b0 = umma::smem_desc_swizzled<128>(sm + p.a_bytes, 1024);
+        int s = 0, i = 0, at = 0;
         uint32_t parity = 0;
         for (int t = start; t < tiles && ok; t += step, ++i) {
-            ok = wait(freed + (i & 1) * 8, ((i >> 1) & 1) ^ 1);
+            ok = umma::mbar_poll(freed + (i & 1) * 8, ((i >> 1) & 1) ^ 1);
             umma::fence_after_sync();
             const uint32_t d = tmem + (i & 1) * BN;
-            for (int k = 0; k < p.k_blocks && ok; ++k) {
-                ok = wait(full + s * 8, parity);
+            for (int k = 0; k < p.k_blocks && ok; k += L::kUnit) {
+                ok = umma::mbar_poll(full + s * 8, parity);
                 umma::fence_after_sync();
-                if (ok && leader) {
-                    const uint64_t a = umma::desc_advance(a0, s * L::kStage), b = umma::desc_advance(b0, s * L::kStage);
+                if (ok) {
 #pragma unroll
-                    for (int j = 0; j < kBlockK / 32; ++j)
-                        mma_i8<PAIR>(d, umma::desc_advance(a, j * 32), umma::desc_advance(b, j * 32), idesc, k > 0 || j > 0);
+                    for (int u = 0; u < L::kUnit; ++u) {
+                        const uint64_t a = umma::desc_advance(a0, at + u * p.block), b = umma::desc_advance(b0, at + u * p.block);
+#pragma unroll
+                        for (int j = 0; j < kBlockK / 32; ++j)
+                            mma_i8<PAIR>(d, umma::desc_advance(a, j * 32), umma::desc_advance(b, j * 32), idesc, k > 0 || u > 0 || j > 0);
+                    }
                     commit<PAIR>(empty + s * 8);
-                    if (k == p.k_blocks - 1) commit<PAIR>(done + (i & 1) * 8);
+                    if (k + L::kUnit >= p.k_blocks) commit<PAIR>(done + (i & 1) * 8);
                 }
-                __syncwarp();
+                at += L::kUnit * p.block;
                 if (++s == S) {
-                    s = 0;
+                    s = at = 0;
                     parity ^= 1;
                 }
             }
@@ -374,7 +387,8 @@ __global__ void __launch_bounds__(Tiles<BN, PAIR, O>::kThreads, 1) int8_matmul_k
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" : : : "memory");
     }
-    if (!ok && lane == 0) record_device_error(p.err, kErrMbarTimeout | 0x50);
+    if (!ok && (warp < 4 || lane == 0)) record_device_error(p.err, kErrMbarTimeout | 0x50);
+    __syncwarp();
     umma::fence_before_sync();
     __syncthreads();
     if (PAIR) cluster_sync();  // until neither SM's barriers or TMEM are used by the other
@@ -389,6 +403,7 @@ constexpr int kFewWarps = 16;
 constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kSlice = 512;             // bytes of K of a warp's load
 constexpr int kFewShared = 160 * 1024;  // bytes of the tokens in 8 bits
+constexpr int kFewChannels = 1 << 18;   // whose sums fit beside them
 constexpr int kFewAhead = 8;            // loads that a warp has under way
 
 struct FewParams {
@@ -592,21 +607,16 @@ int pitch_of(int k) noexcept { return (k + 15) / 16 * 16; }
 // Bytes between tokens in shared memory: whole slices.
 int few_pitch(int k) noexcept { return (k + kSlice - 1) / kSlice * kSlice; }
 
-bool few_form(const ww_int8_matmul_t& p) noexcept
-{
-    return p.M <= kFewTokens && i64(p.M) * few_pitch(p.K) <= kFewShared && p.N <= (1 << 16);
-}
-
 // Few tokens that every block brings to 8 bits by itself; more are brought there once.  4096 values
 // a token against 4096 channels, in the blocks and before them: one token 7.2 us and 8.9, 4
 // tokens 9.2 and 11.2, 8 tokens 14.9 and 12.1.
 bool few_alone(const ww_int8_matmul_t& p) noexcept { return p.x == nullptr || i64(p.M) * p.K <= 16384; }
 
-template <int BN, bool PAIR, typename O>
+template <int BN, bool PAIR, int U, typename O>
 int launch_tiles(MatmulParams& f, int tiles, int sms, cudaStream_t stream) noexcept
 {
-    using L = Tiles<BN, PAIR, O>;
-    const auto kernel = int8_matmul_kernel<BN, PAIR, O>;
+    using L = Tiles<BN, PAIR, U, O>;
+    const auto kernel = int8_matmul_kernel<BN, PAIR, U, O>;
     static std::atomic<uint64_t> raised{0};
     if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("int8_matmul");
     cudaLaunchAttribute attr[2]{};
@@ -630,12 +640,56 @@ int launch_tiles(MatmulParams& f, int tiles, int sms, cudaStream_t stream) noexc
     return launch_status("int8_matmul");
 }
 
-template <int BN, bool PAIR, typename O>
+// Channels of a tile: 64 or 128 on an SM, 256 x 256 on a pair; the form whose rounds end
+// soonest, by clocks of a block of K and of a round's start and end (fitted to the times below).
+// us with 64, 128, 256 channels: 16 x 4096 x 14336 15.5, 14.6, 16.9; 64 x 8192 x 8192 17.3, 21.5, 24.9; 300 x 4096 x 4096
+// 16.6, 13.3, 15.6; 1777 x 1000 x 1111 10.8, 9.4, 12.5; 1024 x 4096 x 4096 29.9, 23.3, 17.1; 2048^3 17.3, 14.3, 11.9;
+// 19200 x 320 x 320 10.0, 9.0, 10.3; 500 x 2048 x 700 8.2, 9.8, 13.4; 469248 x 256 x 768 -, 184, 149.
+struct TileForm {
+    int channels;
+    int64_t clocks;
+};
+
+TileForm tile_form(const ww_int8_matmul_t& p, int sms) noexcept
+{
+    const int64_t k_blocks = (p.K + kBlockK - 1) / kBlockK;
+    const auto time = [&](int rows, int channels, int slots, int block, int round) {
+        const int64_t tiles = ((i64(p.M) + rows - 1) / rows) * ((i64(p.N) + channels - 1) / channels);
+        return (tiles + slots - 1) / slots * (k_blocks * block + round);
+    };
+    const int64_t narrow = time(kTileM, 64, sms, p.M <= kFewRows ? 290 : 360, 800), one = time(kTileM, 128, sms, 540, 1000),
+                  two = time(2 * kTileM, 256, sms / 2, 690, 2400);
+    if (two <= narrow && two <= one) return {256, two};
+    return one <= narrow ? TileForm{128, one} : TileForm{64, narrow};
+}
+
+// Whether up to 8 tokens take the form of their own: one always does; more where it is expected to end before the tiles
+// do (dp4a costs 0.2 or 0.3 ps a weight with 4 or 8 tokens), the 8-bit form of the tokens in a launch before them included.
+// us in their own form and in tiles, 4 tokens: 4096 x 4096 8.1 and 9.3, 8192 x 8192 17.6 and 15.8, 1024 x 131072 32 and 25;
+// 8 tokens: 4096 x 512 6.3 and 7.8, 1024 x 1024 6.1 and 4.6, 4096 x 4096 10.6 and 9.4, 8192 x 8192 24 and 16.  One: 4096 x 131072 85 and 138.
+bool few_form(const ww_int8_matmul_t& p, int sms) noexcept
+{
+    if (p.M > kFewTokens || i64(p.M) * few_pitch(p.K) > kFewShared || p.N > kFewChannels) return false;
+    if (p.M == 1) return true;
+    const int64_t own = (p.M <= 4 ? 700'000 : 1'900'000) + i64(p.N) * p.K * (p.M <= 4 ? 200 : 300) / 1000;   // ps
+    const int64_t tiles = tile_form(p, sms).clocks * 526 + (p.x != nullptr && few_alone(p) ? 1'700'000 : 0);  // at 1.9 GHz
+    return own <= tiles;
+}
+
+// Rows of a tile of tokens that are loaded: of a tile that the tokens do not fill, only those.
+// The products then read on into what lies behind them, in shared memory, for rows that are not written out.
+int loaded_rows(int m) noexcept { return std::min(kTileM, (m + 7) / 8 * 8); }
+
+template <int BN, bool PAIR, int U, typename O>
 int run_tiles(const ww_int8_matmul_t& p, bool behind, int sms, int* err, cudaStream_t stream) noexcept
 {
-    using L = Tiles<BN, PAIR, O>;
+    using L = Tiles<BN, PAIR, U, O>;
     MatmulParams f;
-    if (!encode_rows_map(&f.a, WW_DTYPE_INT8, p.x_q, p.M, p.K, p.x_q_stride, kBlockK, kTileM) ||
+    const int a_rows = loaded_rows(p.M);
+    f.a_bytes = a_rows * kBlockK;
+    f.block = f.a_bytes + L::kB;
+    f.stages = std::min(L::kMostStages, L::kRing / (L::kUnit * f.block));
+    if (!encode_rows_map(&f.a, WW_DTYPE_INT8, p.x_q, p.M, p.K, p.x_q_stride, kBlockK, a_rows) ||
         !encode_rows_map(&f.b, WW_DTYPE_INT8, p.w_q, p.N, p.K, p.w_stride, kBlockK, PAIR ? BN / 2 : BN))
         return WW_ERR_UNSUPPORTED;
     f.stored = i64(p.N) * static_cast<int>(sizeof(O)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
@@ -655,7 +709,7 @@ int run_tiles(const ww_int8_matmul_t& p, bool behind, int sms, int* err, cudaStr
     f.err = err;
     const int64_t tiles = i64(f.m_tiles) * f.n_tiles;
     if (tiles > INT_MAX / 2) return WW_ERR_UNSUPPORTED;
-    return launch_tiles<BN, PAIR, O>(f, static_cast<int>(tiles), sms, stream);
+    return launch_tiles<BN, PAIR, U, O>(f, static_cast<int>(tiles), sms, stream);
 }
 
 // Channels of a block in the form for few tokens: one round of blocks, at least 4 channels each.
@@ -679,27 +733,10 @@ int few(const ww_int8_matmul_t& p, bool behind, int sms, cudaStream_t stream) no
     return launch_status("int8_matmul");
 }
 
-// Channels of a tile: 64 or 128 on an SM, 256 x 256 on a pair; the form whose rounds end
-// soonest, by clocks of a stage of K and of a round's start and end (fitted to the times below).
-// us with 64, 128, 256 channels: 64 x 4096 x 4096 11.6, 12.9, 15.3; 300 x 4096 x 4096 19.2, 13.2,
-// 15.6; 1777 x 1000 x 1111 10.1, 8.7, 12.5; 1024 x 4096 x 4096 34.6, 22.4, 16.5; 2048^3 19.2, 13.3,
-// 11.0; 19200 x 320 x 320 9.5, 9.0, 10.5; 4096 x 512 x 1024 8.5, 7.3, 7.7.
-int tile_form(const ww_int8_matmul_t& p, int sms) noexcept
-{
-    const int64_t k_blocks = (p.K + kBlockK - 1) / kBlockK;
-    const auto time = [&](int rows, int channels, int slots, int stage, int round) {
-        const int64_t tiles = ((i64(p.M) + rows - 1) / rows) * ((p.N + channels - 1) / channels);
-        return (tiles + slots - 1) / slots * (k_blocks * stage + round);
-    };
-    const int64_t narrow = time(kTileM, 64, sms, 510, 600), one = time(kTileM, 128, sms, 660, 1000),
-                  two = time(2 * kTileM, 256, sms / 2, 700, 2900);
-    return two <= narrow && two <= one ? 256 : one <= narrow ? 128 : 64;
-}
-
 template <typename O>
 int matmul(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
 {
-    const bool is_few = few_form(p);
+    const bool is_few = few_form(p, sms);
     if (is_few && few_alone(p)) return few<O>(p, false, sms, stream);
     ww_int8_matmul_t c = p;
     if (p.x != nullptr) {
@@ -720,10 +757,12 @@ int matmul(const ww_int8_matmul_t& p, int sms, cudaStream_t stream) noexcept
     if (is_few) return few<O>(c, behind, sms, stream);
     int* err = device_error_slot();
     if (err == nullptr) return WW_ERR_DEVICE;
-    switch (tile_form(c, sms)) {
-    case 256: return run_tiles<256, true, O>(c, behind, sms, err, stream);
-    case 128: return run_tiles<128, false, O>(c, behind, sms, err, stream);
-    default: return run_tiles<64, false, O>(c, behind, sms, err, stream);
+    switch (tile_form(c, sms).channels) {
+    case 256: return run_tiles<256, true, 1, O>(c, behind, sms, err, stream);
+    case 128: return run_tiles<128, false, 1, O>(c, behind, sms, err, stream);
+    default:
+        return loaded_rows(c.M) <= kFewRows ? run_tiles<64, false, 4, O>(c, behind, sms, err, stream)
+                                            : run_tiles<64, false, 2, O>(c, behind, sms, err, stream);
     }
 }
 
@@ -743,9 +782,15 @@ int check(const ww_int8_matmul_t& p) noexcept
     return WW_SUCCESS;
 }
 
-int64_t workspace(const ww_int8_matmul_t& p) noexcept
+int sm_count() noexcept
 {
-    if (p.x == nullptr || p.M == 0 || p.N == 0 || (few_form(p) && few_alone(p))) return 0;
+    DeviceInfo d;
+    return current_device_info(&d) == WW_SUCCESS ? d.sm_count : 148;
+}
+
+int64_t workspace(const ww_int8_matmul_t& p, int sms) noexcept
+{
+    if (p.x == nullptr || p.M == 0 || p.N == 0 || (few_form(p, sms) && few_alone(p))) return 0;
     return i64(p.M) * pitch_of(p.K) + i64(p.M) * 4;
 }
 
@@ -756,7 +801,7 @@ extern "C" {
 
 int64_t ww_int8_matmul_workspace(const ww_int8_matmul_t* p)
 {
-    return p == nullptr || ww::check(*p) != WW_SUCCESS ? 0 : ww::workspace(*p);
+    return p == nullptr || ww::check(*p) != WW_SUCCESS ? 0 : ww::workspace(*p, ww::sm_count());
 }
 
 int ww_int8_matmul(const ww_int8_matmul_t* p, void* stream)
@@ -764,7 +809,7 @@ int ww_int8_matmul(const ww_int8_matmul_t* p, void* stream)
     if (p == nullptr) return WW_ERR_NULL_POINTER;
     int st = ww::check(*p);
     if (st != WW_SUCCESS || p->M == 0 || p->N == 0) return st;
-    const int64_t need = ww::workspace(*p);
+    const int64_t need = ww::workspace(*p, ww::sm_count());
     if (need > 0) {
         if (p->workspace == nullptr) return WW_ERR_NULL_POINTER;
         if (reinterpret_cast<uintptr_t>(p->workspace) % 16 != 0) return WW_ERR_MISALIGNED;
