@@ -1,5 +1,5 @@
 // attention_int8.cu -- ww_cross_attention with keys and values in 8 bits, for few
-// query rows per key head; more rows: keys and values brought to 16 bits first.
+// query rows per key head; more rows: keys and values brought to 16 bits first (by_copies).
 //
 //   s_ij = (q_i . kq_j) ks_j scale log2(e) + bias,   l_i = sum_j 2^(s_ij - m_i)
 //   o_i = sum_j 2^(s_ij + log2(vs_j) - n_i) vq_j,    out_i = o_i 2^(n_i - m_i) / l_i
