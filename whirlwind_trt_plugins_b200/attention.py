@@ -117,6 +117,8 @@ def _empty(shape, dtype):
     shape = tuple(shape)
     if len(shape) == 2:
         return _Torch.alloc(shape, (shape[1], 1), dtype)
+    if len(shape) == 1:
+        return _Torch.alloc(shape, (1,), dtype)
     strides, n = (), 1
     for m in reversed(shape):
         strides = (n, *strides)

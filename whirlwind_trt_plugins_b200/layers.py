@@ -42,6 +42,7 @@ _NORM = struct.Struct("@16Pq5q3if0P")
 _MATMUL = struct.Struct("@8Pq3q4i0P")
 _CACHE = struct.Struct("@10P16q6i0P")
 _SCALES = struct.Struct("@2P4q")
+_ATTN_INT8 = struct.Struct("@14Pq12q11if0P2P4q0P")
 _NORM_WS, _MATMUL_WS, _ATTN_WS = 15 * 8, 7 * 8, 13 * 8  # where the workspace's address and bytes stand
 _INT_MAX = 2 ** 31 - 1
 
@@ -55,12 +56,14 @@ def _rows(t, name: str, device: int, dtype=None, shape=None):
     n = size[-1]
     if n == 0:
         raise ValueError(f"{name} has rows without values")
-    rows = t.numel() // n
+    rows = size[0] if len(size) == 2 else t.numel() // n
     if rows > _INT_MAX:
         raise ValueError(f"{name} has more than 2^31 - 1 rows")
     if t.is_contiguous():
         return rows, n, n
     st = t.stride()
+    if len(st) == 2 and (st[1] == 1 or n == 1):
+        return rows, n, st[0] if rows > 1 else n
     if rows and (n > 1 and st[-1] != 1):
         raise ValueError(f"{name} needs unit stride along its last dim, got {st}")
     step, length = None, 1  # stride of the collapsed dims, rows in them
@@ -146,7 +149,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, residual=None, retu
         stats = [_empty(x.shape[:-1], T.f32) for _ in range(2)]
         got += (*stats,)
         mean, rstd = stats[0].data_ptr(), stats[1].data_ptr()
-    a = _NORM.pack(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), y.data_ptr(), total, 0, 0, mean, rstd, 0, 0,
+    a = _NORM.pack(x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
+                   0 if bias is None else bias.data_ptr(), y.data_ptr(), total, 0, 0, mean, rstd, 0, 0,
                    0, 0, 0, 0, 0, xs, rs, 0, 0, 0, dt, rows, n, eps)
     _check("ww_layer_norm", _lib.ww_layer_norm(a, T.stream(at)))
     return got if len(got) > 1 else y
@@ -162,7 +166,8 @@ def layer_norm_int8(x, weight=None, bias=None, eps: float = 1e-5, residual=None,
     q, pitch = _int8_rows(x.shape)
     scale = _empty(x.shape[:-1], T.f32)
     total = None if residual is None else _new(x, None, "sum")
-    a = _NORM.pack(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), 0, _ptr(total), q.data_ptr(),
+    a = _NORM.pack(x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
+                   0 if bias is None else bias.data_ptr(), 0, 0 if total is None else total.data_ptr(), q.data_ptr(),
                    scale.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, xs, rs, pitch, 0, 0, dt, rows, n, eps)
     _check("ww_layer_norm", _lib.ww_layer_norm(a, T.stream(at)))
     return (q, scale) if total is None else (q, scale, total)
@@ -224,8 +229,15 @@ def quantize_tokens(x, stream=None):
 
 def _whole_pieces(t, name: str, rows: int, k: int, stride: int):
     """Rows of K bytes that the kernels read in whole 16 bytes: so far the memory of the last one must go."""
-    if k % 16 and rows and t.untyped_storage().nbytes() - t.storage_offset() < (rows - 1) * stride + (k + 15) // 16 * 16:
+    if rows and t.untyped_storage().nbytes() - t.storage_offset() < (rows - 1) * stride + (k + 15) // 16 * 16:
         raise ValueError(f"{name}'s last row must be followed by memory up to whole 16 bytes: see quantize_tokens")
+
+
+@functools.lru_cache(maxsize=4096)
+def _matmul_need(device: int, dt: int, rows: int, k: int, channels: int) -> int:
+    """Bytes of scratch memory of ``int8_linear``, a function of its sizes (the pointers say what there is)."""
+    step = (k + 15) // 16 * 16
+    return _lib.ww_int8_matmul_workspace(_MATMUL.pack(16, 0, 0, 16, 16, 0, 16, 0, 0, k, k, step, dt, rows, k, channels))
 
 
 def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
@@ -235,6 +247,7 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
     if x_scale is None:
         dt, dtype = _dtype(x, "x"), x.dtype
         rows, k, xs = _rows(x, "x", at)
+        x_at, xq_at, xs_at = x.data_ptr(), 0, 0
     else:
         dt = T.dtypes.get(dtype)
         if dt is None:
@@ -243,7 +256,9 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
         _tensor(x_scale, "x_scale", at, T.f32, x.shape[:-1])
         if rows > 1 and xs % 16:
             raise ValueError("rows of x_q must start on 16 bytes: see quantize_tokens")
-        _whole_pieces(x, "x_q", rows, k, xs)
+        if k % 16:
+            _whole_pieces(x, "x_q", rows, k, xs)
+        x_at, xq_at, xs_at = 0, x.data_ptr(), x_scale.data_ptr()
     channels, kw, ws = _rows(w_q, "w_q", at, int8)
     if len(w_q.shape) != 2 or kw != k:
         raise ValueError(f"w_q must be [N, {k}], got {tuple(w_q.shape)}")
@@ -251,7 +266,8 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
         ws = (k + 15) // 16 * 16
     if ws % 16:
         raise ValueError("rows of w_q must start on 16 bytes: see quantize_tokens")
-    _whole_pieces(w_q, "w_q", channels, k, ws)
+    if k % 16:
+        _whole_pieces(w_q, "w_q", channels, k, ws)
     _tensor(w_scale, "w_scale", at, T.f32, (channels,))
     if bias is not None:
         _tensor(bias, "bias", at, dtype, (channels,))
@@ -263,12 +279,14 @@ def _matmul(x, x_scale, w_q, w_scale, bias, dtype, out, stream):
         out = _empty(shape, dtype)
     else:
         _apart(_out(out, shape, dtype, x.device, "out"), x=x, x_scale=x_scale, w_q=w_q, w_scale=w_scale, bias=bias)
-    p = x.data_ptr()
-    a = _MATMUL.pack(p if x_scale is None else 0, 0 if x_scale is None else p, _ptr(x_scale), w_q.data_ptr(),
-                     w_scale.data_ptr(), _ptr(bias), out.data_ptr(), 0, 0, xs, xs, ws, dt, rows, k, channels)
-    need = _lib.ww_int8_matmul_workspace(a) if x_scale is None else 0
-    if need:
-        scratch, a = _workspace(need, a, _MATMUL_WS)
+    scratch_at = need = 0
+    if x_at:
+        need = _matmul_need(at, dt, rows, k, channels)
+        if need:
+            scratch = T.alloc((need,), (1,), T.uint8)
+            scratch_at = scratch.data_ptr()
+    a = _MATMUL.pack(x_at, xq_at, xs_at, w_q.data_ptr(), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                     out.data_ptr(), scratch_at, need, xs, xs, ws, dt, rows, k, channels)
     _check("ww_int8_matmul", _lib.ww_int8_matmul(a, T.stream(at)))
     return out
 
@@ -296,14 +314,17 @@ def _kept(k_cache, v_cache, k_scale, v_scale, at: int):
     shape = k_cache.shape
     vs = _vectors(v_cache, "v_cache", at, int8, shape)
     B, places, H, D = shape
-    strides = []
-    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        _tensor(t, name, at, _Torch.f32, (B, H, places), False)
-        st = t.stride()
-        if places > 1 and st[2] != 1:
-            raise ValueError(f"{name} needs unit stride along its places, got {st}")
-        strides += st[:2]
-    return shape, ks, vs, strides
+    return shape, ks, vs, _scales(k_scale, "k_scale", at, (B, H, places)) + _scales(v_scale, "v_scale", at, (B, H, places))
+
+
+def _scales(t, name: str, at: int, shape):
+    _tensor(t, name, at, _Torch.f32, shape, False)
+    if t.is_contiguous():
+        return shape[1] * shape[2], shape[2]
+    st = t.stride()
+    if shape[2] > 1 and st[2] != 1:
+        raise ValueError(f"{name} needs unit stride along its places, got {st}")
+    return st[:2]
 
 
 def _items(t, name: str, at: int, B: int):
@@ -408,10 +429,11 @@ def cross_attention_int8(q, k_cache, v_cache, k_scale, v_scale, scale: float | N
                key_mask=key_mask, bias_table=bias_table)
     out = _new(q, out, "out")
     lse = _empty((B, Hq, Lq), T.f32) if return_lse else None
-    a = _ATTN.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(k_lens),
-                   _ptr(key_mask), _ptr(bias_table), 0, 0, 0, 0, 0, 0, 0, *qs, *ks, *vs, 0, 0, 0, dt, B, Lq, Lk, Hq, Hk,
-                   D, buckets, max_distance, bool(bidirectional), q_offset, scale)
-    a += _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), *ss)
+    a = _ATTN_INT8.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+                        0 if lse is None else lse.data_ptr(), 0 if k_lens is None else k_lens.data_ptr(),
+                        0 if key_mask is None else key_mask.data_ptr(), 0 if bias_table is None else bias_table.data_ptr(),
+                        0, 0, 0, 0, 0, 0, 0, *qs, *ks, *vs, 0, 0, 0, dt, B, Lq, Lk, Hq, Hk, D, buckets, max_distance,
+                        bool(bidirectional), q_offset, scale, k_scale.data_ptr(), v_scale.data_ptr(), *ss)
     need = _lib.ww_cross_attention_int8_workspace(a)
     if need:
         ws, a = _workspace(need, a, _ATTN_WS)
