@@ -229,6 +229,33 @@ def test_layer_norm_autograd_of_one_result(env):
     assert all(torch.equal(g, f) for g, f in zip(got, (ref[0], *ref)))
 
 
+@pytest.mark.parametrize("shape", [(15000, 320), (4000, 504), (13001, 712), (9000, 1024), (9001, 1048), (2500, 4096), (1500, 8192)])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("dsum", [False, True])
+def test_layer_norm_gradient_of_many_rows(env, shape, dt, dsum):
+    """Many rows for each lane and block, of strided inputs: their own sums, and the same bits on every run."""
+    torch, ww = env
+    rows, n = shape
+    t, u = _type(torch, dt), U[dt]
+    w, dy = _randn(torch, (n,), 1, t), _randn(torch, (rows, n), 2, t)
+    x = _randn(torch, (rows, n + 16), 3, t)[:, :n]
+    ds = _randn(torch, (rows, 2 * n), 4, t)[:, n:] if dsum else None
+    _, mean, rstd = ww.layer_norm(x, w, return_stats=True)
+    got = ww.layer_norm_backward(dy, x, w, mean, rstd, dsum=ds)
+    assert all(torch.equal(a, b) for a, b in zip(got, ww.layer_norm_backward(dy, x, w, mean, rstd, dsum=ds)))
+    xh = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    g = dy.double() * w.double()
+    s2 = (g * xh).mean(-1, keepdim=True)
+    ref = rstd.double()[:, None] * (g - g.mean(-1, keepdim=True) - xh * s2)
+    mag = rstd.double()[:, None] * (g.abs() + g.abs().mean(-1, keepdim=True) + xh.abs() * (g * xh).abs().mean(-1, keepdim=True))
+    if dsum:
+        ref, mag = ref + ds.double(), mag + ds.double().abs()
+    _within(got[0], ref, u * ref.abs() + 2.0 ** -18 * mag, "dx")
+    for a, terms in ((got[1], dy.double() * xh), (got[2], dy.double())):
+        _within(a, terms.sum(0), u * terms.sum(0).abs() + 2.0 ** -18 * terms.abs().sum(0), "sums")
+    assert ww.device_error() == 0
+
+
 @pytest.mark.parametrize("n", [24, 40, 60])
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_layer_norm_gradient_of_large_equal_values(env, n, dt):

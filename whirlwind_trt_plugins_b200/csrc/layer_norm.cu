@@ -14,7 +14,8 @@
 // group of 4 to 32 lanes or, where a warp's registers do not hold it, by a block;
 // loads are 16 bytes a lane where rows start on 16 bytes, else single values.
 // Both directions run one resident round of blocks, the next rows' loads under way
-// while rows are computed.  In the gradient a lane owns the same columns of all its
+// while rows are computed: in registers, or for the gradient of rows of more than a piece a
+// lane in rings in shared memory.  In the gradient a lane owns the same columns of all its
 // rows, so the weight's and bias's sums stay in registers; they are joined per
 // block in shared memory and over blocks by a second kernel, both in a fixed order.
 // Rows beyond a block's registers are read again from L2 for each step.
@@ -24,6 +25,7 @@
 // 33.5 us (single loads; pieces of 16 bytes with the rows' ends masked took 52).
 // 40000 rows of 1337 in fp16, single loads of 2 bytes: 98 us for 214 MB, instructions.
 #include "rows.cuh"
+#include "umma.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -45,9 +47,9 @@ constexpr int kBackwardBlocks = 2;
 // fp32 (8 single values a lane): 768 threads 33.5 us; 512 and 1024, which spills, 40 and 38.
 // Forward, the same rows: 768 20.9 us, 1024, of which not all are resident, 27.
 int forward_threads(bool pieces) { return pieces ? 1024 : 768; }
-int backward_threads(bool pieces, int bytes, int per_lane) { return per_lane == 8 ? 768 : pieces && bytes == 4 ? 1024 : 512; }
+int backward_threads(int per_lane) { return per_lane == 8 ? 768 : 512; }
 // Blocks of a row that the compiler keeps registers for, so that these threads fit.
-__host__ __device__ constexpr int backward_row_blocks(int v, int pieces) { return v == 1 && pieces == 8 ? 3 : v == 4 ? 2 : 1; }
+__host__ __device__ constexpr int backward_row_blocks(int v, int pieces) { return v == 1 && pieces == 8 ? 3 : 1; }
 
 struct NormParams {
     const void *x, *r, *w, *b;
@@ -60,6 +62,8 @@ struct NormParams {
     int64_t xs, rs, qs, gs, ds;  // elements between rows
     int32_t rows, N, norm;
     float eps, inv_n;
+    int32_t stages;  // of a ring
+    int* err;
 };
 
 // R rows of a group of lanes at a time, those of the block's next step loaded ahead.
@@ -400,6 +404,204 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
     }
 }
 
+// The same for rows of more than a piece a lane: registers hold the weights and their sums, the rows to come lie in a ring in
+// shared memory, a ring for each warp (GROUP) or block, filled by bulk copies of whole rows.
+// us with a row under way in registers (longer rows than 512 in blocks), and so: 153600 rows of 320, fp16, 72 and 59; 60000 of 768 68 and
+// 51, with dsum 84 and 61; 100000 of 1024, bf16, 118 and 104 (614 MB, 5.9 TB/s); 20000 of 4096 101 and 87, with dsum 120 and 105
+// (6.2 TB/s); 10000 of 4096, fp32, with dsum 134 and 98; 300 of 4096 19 and 10.8; 64 of 1024 3.9 and 4.2.
+constexpr int ring_threads(int pieces) { return pieces == 3 ? 384 : 256; }  // of a block of warps, as registers allow
+constexpr int ring_blocks(int pieces) { return pieces == 2 ? 2 : 1; }
+constexpr int kRingRowThreads = 512;  // of an SM's blocks that hold a row each
+
+template <typename T, int V, int P, int GROUP, bool DSUM>
+__global__ void __launch_bounds__(GROUP ? ring_threads(P) : kRingRowThreads, GROUP ? ring_blocks(P) : 1)
+    layer_norm_backward_ring_kernel(const __grid_constant__ NormParams p)
+{
+    constexpr int E = P * V / 2, kTensors = DSUM ? 3 : 2;
+    constexpr int kRows = GROUP ? 32 / (GROUP ? GROUP : 1) : 1;  // of a warp side by side
+    extern __shared__ __align__(16) uint8_t ring[];
+    const int owners = GROUP ? blockDim.x / 32 : 1, owner = GROUP ? threadIdx.x / 32 : 0, S = p.stages;
+    const int sub = GROUP ? threadIdx.x % 32 / (GROUP ? GROUP : 1) : 0;
+    const bool leader = GROUP ? threadIdx.x % 32 == 0 : threadIdx.x == 0;
+    const Columns<V, P, GROUP> column;
+    const uint32_t row_bytes = p.N * static_cast<uint32_t>(sizeof(T)), stage = kTensors * kRows * row_bytes;
+    float* const red = reinterpret_cast<float*>(ring + static_cast<uint32_t>(owners * S) * (stage + 8));  // [2][64] of a block that holds a row
+    uint8_t* const mine = ring + static_cast<uint32_t>(owner * S) * stage;
+    const uint32_t to_mine = umma::smem_addr(mine), bars = umma::smem_addr(ring) + static_cast<uint32_t>(owners * S) * stage + owner * S * 8;
+    // few rows go to many blocks: an owner of each before the second of any
+    const int64_t step = static_cast<int64_t>(gridDim.x) * owners * kRows;
+    int64_t row0 = (static_cast<int64_t>(owner) * gridDim.x + blockIdx.x) * kRows;
+    // the leader's: rows to come, and where they are
+    int64_t ahead = row0;
+    const T* xp = static_cast<const T*>(p.x) + row0 * p.xs;
+    const T* gp = static_cast<const T*>(p.dy) + row0 * p.gs;
+    const T* sp = DSUM ? static_cast<const T*>(p.dsum) + row0 * p.ds : nullptr;
+    const int64_t x_step = step * p.xs, g_step = step * p.gs, s_step = step * p.ds;
+    const auto rows_in = [&](const T* from, int64_t stride, uint32_t to, int n, uint32_t bar) {
+        if (kRows == 1 || stride == p.N) {
+            umma::bulk_g2s(to, from, n * row_bytes, bar);
+        } else {
+            for (int j = 0; j < n; ++j) umma::bulk_g2s(to + j * row_bytes, from + j * stride, row_bytes, bar);
+        }
+    };
+    const auto fill = [&](int s) {
+        if (ahead >= p.rows) return;
+        const int n = kRows == 1 ? 1 : static_cast<int>(min(static_cast<int64_t>(kRows), p.rows - ahead));
+        const uint32_t bar = bars + s * 8, to = to_mine + s * stage;
+        umma::mbar_arrive_expect_tx(bar, n * kTensors * row_bytes);
+        rows_in(xp, p.xs, to, n, bar);
+        rows_in(gp, p.gs, to + kRows * row_bytes, n, bar);
+        if constexpr (DSUM) rows_in(sp, p.ds, to + 2 * kRows * row_bytes, n, bar);
+        ahead += step;
+        xp += x_step;
+        gp += g_step;
+        if constexpr (DSUM) sp += s_step;
+    };
+    if (leader) {
+        for (int s = 0; s < S; ++s) umma::mbar_init(bars + s * 8, 1);
+        umma::mbar_fence_init();
+        for (int s = 0; s < S; ++s) fill(s);
+    }
+    Pair w[E], dw[E], db[E];
+    {
+        Piece<T, V> raw[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            raw[i].clear();
+            if (p.w != nullptr && column(i) < p.N) raw[i].load(static_cast<const T*>(p.w) + column(i));
+        }
+        values_of<T, V, P>(raw, w);
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        dw[i] = db[i] = pair(0.0f, 0.0f);
+        if (p.w == nullptr) w[i] = pair(1.0f, 1.0f);
+    }
+    float mean = 0.0f, rstd = 0.0f;
+    const auto stats = [&](int64_t row) {
+        mean = row < p.rows ? __ldg(p.mean + row) : 0.0f;
+        rstd = row < p.rows ? __ldg(p.rstd + row) : 0.0f;
+    };
+    stats(row0 + sub);
+    __syncthreads();  // the barriers are there
+    int s = 0, turn = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (; row0 < p.rows; row0 += step, turn ^= 1) {
+        ok = ok && umma::mbar_poll(bars + s * 8, parity);  // once given up, no wait and no copy follows
+        const bool real = row0 + sub < p.rows;
+        Pair xh[E], g[E];
+        const float rs = rstd;
+        const T* from = reinterpret_cast<const T*>(mine + s * stage + sub * row_bytes);
+        const uint32_t next = kRows * p.N;
+        {
+            // what lies beyond the row, and rows beyond the last, are zeros, with a mean of 0
+            Piece<T, V> x[P], y[P];
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                x[i].clear();
+                y[i].clear();
+                if (real && column(i) < p.N) {
+                    x[i].load_shared(from + column(i));
+                    y[i].load_shared(from + next + column(i));
+                }
+            }
+            values_of<T, V, P>(x, xh);
+            values_of<T, V, P>(y, g);
+        }
+        const Pair r2 = pair(rs, rs);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float m = column(2 * i / V) < p.N ? -mean : 0.0f;
+            xh[i] = mul2(add2(xh[i], pair(m, m)), r2);
+        }
+        stats(row0 + step + sub);
+        if constexpr (GROUP != 0 && !DSUM) {
+            __syncwarp();  // the stage has been read
+            if (leader && ok) fill(s);
+        }
+        Pair s1 = pair(0.0f, 0.0f), s2 = s1;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            dw[i] = fma2(g[i], xh[i], dw[i]);
+            db[i] = add2(db[i], g[i]);
+            g[i] = mul2(g[i], w[i]);
+            s1 = add2(s1, g[i]);
+            s2 = fma2(g[i], xh[i], s2);
+        }
+        float v[2] = {both(s1), both(s2)};
+        row_sums<GROUP>(v, red + turn * 64);
+        if constexpr (GROUP == 0) {  // row_sums' barrier: the stage has been read, or with dsum the one before
+            if (!DSUM && leader && ok) fill(s);
+            if (DSUM && leader && ok && row0 >= gridDim.x) fill(s == 0 ? S - 1 : s - 1);
+        }
+        const float m1 = v[0] * p.inv_n, m2 = v[1] * p.inv_n;
+        const Pair a = pair(-m1, -m1), b = pair(-m2, -m2);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const Pair u = fma2(xh[i], b, add2(g[i], a));
+            if constexpr (DSUM) g[i] = u;
+            else g[i] = mul2(u, r2);
+        }
+        if (real) {
+            T* to = static_cast<T*>(p.dx) + (row0 + sub) * p.N;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                if (column(i) >= p.N) continue;
+                if constexpr (DSUM) {
+                    Piece<T, V> z[1];
+                    Pair d[V / 2];
+                    z[0].load_shared(from + 2 * next + column(i));
+                    values_of<T, V, 1>(z, d);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) g[i * V / 2 + e] = fma2(g[i * V / 2 + e], r2, d[e]);
+                }
+                store_piece<T, V>(to + column(i), g, i);
+            }
+        }
+        if constexpr (GROUP != 0 && DSUM) {
+            __syncwarp();
+            if (leader && ok) fill(s);
+        }
+        if (++s == S) {
+            s = 0;
+            parity ^= 1;
+        }
+    }
+    if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x60);
+    if (p.part == nullptr) return;
+    start_launch_behind();  // the join, which waits for this grid's end
+    float* joined = reinterpret_cast<float*>(ring);
+    const int lane = threadIdx.x % (GROUP ? GROUP : 1), group = threadIdx.x / (GROUP ? GROUP : 1), groups = blockDim.x / (GROUP ? GROUP : 1);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float* sums = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + which) * p.N;
+        float v[2 * E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) unpair(which ? db[i] : dw[i], v[2 * i], v[2 * i + 1]);
+        if (GROUP == 0 || groups == 1) {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (column(i) < p.N)
+#pragma unroll
+                    for (int e = i * V; e < (i + 1) * V; e += 4)
+                        *reinterpret_cast<float4*>(sums + column(i) + e % V) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        } else {
+            constexpr int kRow = GROUP * P * V;  // columns kept of a row
+            __syncthreads();                     // the rings, or the sums before, have been read
+#pragma unroll
+            for (int e = 0; e < 2 * E; ++e) joined[group * kRow + (e / V * GROUP + lane) * V + e % V] = v[e];
+            __syncthreads();
+            for (int c = threadIdx.x; c < p.N; c += blockDim.x) {
+                float t = 0.0f;
+#pragma unroll 8
+                for (int k = 0; k < groups; ++k) t += joined[k * kRow + c];
+                sums[c] = t;
+            }
+        }
+    }
+}
+
 // Rows of any length: dx by a block for each row, the weight's and bias's sums by columns.
 template <typename T>
 __global__ void __launch_bounds__(kLongBlock) layer_norm_backward_long_kernel(const __grid_constant__ NormParams p)
@@ -556,27 +758,61 @@ int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cuda
 
 // Blocks of the gradient: one resident round, as far as there are rows for it.
 struct BackwardPlan {
-    bool pieces;
+    bool pieces, ring;
     RowForm form;
     int blocks, splits;  // splits: of the rows, for the sums by columns (long rows)
+    int stages, shared;  // of a ring, bytes of its block
     int parts() const { return form.threads == 0 ? splits : blocks; }
 };
 
 BackwardPlan backward_plan(const ww_layer_norm_t& p, int sms) noexcept
 {
     const int bytes = p.dtype == WW_DTYPE_FLOAT ? 4 : 2;
-    BackwardPlan r;
+    BackwardPlan r{};
     r.pieces = in_pieces(p, bytes);
     const int v = r.pieces ? 16 / bytes : 1;
-    r.form = row_form(p.N, v, 2, true);
+    r.form = row_form(p.N, v, 4, true);
+    r.ring = r.pieces && r.form.pieces > 1;
+    if (r.ring) {
+        // an owner of rows in each block before the second of any, and as many stages as fit and are needed (2 or more fit: rows
+        // of 16 KB of three tensors 4)
+        const int resident = r.form.group ? ring_blocks(r.form.pieces) : std::max(1, kRingRowThreads / r.form.threads);
+        const int at_once = r.form.group ? 32 / r.form.group : 1;
+        const int64_t turns = (i64(p.rows) + at_once - 1) / at_once;
+        r.blocks = static_cast<int>(std::min<int64_t>(i64(sms) * resident, turns));
+        int owners = 1;
+        if (r.form.group) {
+            owners = static_cast<int>(std::min<int64_t>(ring_threads(r.form.pieces) / 32, (turns + r.blocks - 1) / r.blocks));
+            r.form.threads = 32 * owners;
+        }
+        const int stage = owners * at_once * p.N * bytes * (p.dsum == nullptr ? 2 : 3) + 8 * owners;
+        const int64_t needed = (turns + r.blocks * owners - 1) / (r.blocks * owners);
+        r.stages = static_cast<int>(std::min<int64_t>({8, needed, (kMaxShared / resident - 2048) / stage}));
+        r.shared = std::max(r.stages * stage + 512, r.form.group ? r.form.threads * r.form.pieces * v * 4 : 0);
+        return r;
+    }
     const int groups = r.form.group ? kBlock / r.form.group : 1;
     int resident = kBackwardBlocks;
-    if (r.form.group == 0 && r.form.threads > 0) resident = std::max(1, backward_threads(r.pieces, bytes, r.form.pieces) / r.form.threads);
+    if (r.form.group == 0 && r.form.threads > 0) resident = std::max(1, backward_threads(r.form.pieces) / r.form.threads);
     const int at_once = groups * rows_at_once(v, r.form.pieces, r.form.group);
     r.blocks = static_cast<int>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + at_once - 1) / at_once));
     const int columns = (p.N + kBlock - 1) / kBlock;
     r.splits = std::max(1, std::min(p.rows, 4 * sms / columns));
     return r;
+}
+
+template <typename T, int P, int GROUP>
+bool launch_ring(NormParams& f, const BackwardPlan& plan, cudaStream_t stream) noexcept
+{
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    const bool sum = f.dsum != nullptr;
+    const auto kernel = sum ? layer_norm_backward_ring_kernel<T, V, P, GROUP, true> : layer_norm_backward_ring_kernel<T, V, P, GROUP, false>;
+    static std::atomic<uint64_t> raised[2];
+    f.stages = plan.stages;
+    f.err = device_error_slot();
+    if (f.err == nullptr || !allow_shared_memory(reinterpret_cast<const void*>(kernel), raised[sum])) return false;
+    kernel<<<plan.blocks, plan.form.threads, plan.shared, stream>>>(f);
+    return true;
 }
 
 template <typename T>
@@ -587,6 +823,7 @@ int backward(const ww_layer_norm_t& p, const BackwardPlan& plan, cudaStream_t st
     f.part = sums ? static_cast<float*>(p.workspace) : nullptr;
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     const RowForm& form = plan.form;
+    bool ready = true;
     const auto go = [&](auto kernel, auto with_sum) {
         if (p.dsum == nullptr) kernel<<<plan.blocks, form.threads, 0, stream>>>(f);
         else with_sum<<<plan.blocks, form.threads, 0, stream>>>(f);
@@ -611,12 +848,16 @@ int backward(const ww_layer_norm_t& p, const BackwardPlan& plan, cudaStream_t st
         case 801: WW_NORM(V, 1, 8); break;
         case 1601: WW_NORM(V, 1, 16); break;
         case 3201: WW_NORM(V, 1, 32); break;
-        case 3202: WW_NORM(V, 2, 32); break;
-        default: WW_NORM(V, 2, 0); break;
+        case 1603: ready = launch_ring<T, 3, 16>(f, plan, stream); break;
+        case 3202: ready = launch_ring<T, 2, 32>(f, plan, stream); break;
+        case 3203: ready = launch_ring<T, 3, 32>(f, plan, stream); break;
+        case 3204: ready = launch_ring<T, 4, 32>(f, plan, stream); break;
+        default: ready = launch_ring<T, 2, 0>(f, plan, stream); break;
         }
     }
 #undef WW_NORM
     const int st = launch_status("layer_norm_backward");
+    if (!ready) return st != WW_SUCCESS ? st : WW_ERR_DEVICE;
     if (st != WW_SUCCESS || !sums) return st;
     launch_behind(layer_norm_join_kernel<T>, dim3((2u * p.N + kJoinColumns - 1) / kJoinColumns), dim3(kJoinColumns * 32), 0, stream, f.part, plan.parts(), p.N,
                   static_cast<T*>(p.dweight), static_cast<T*>(p.dbias));

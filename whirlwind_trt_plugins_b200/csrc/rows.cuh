@@ -62,7 +62,7 @@ template <typename T, int V>
 struct Piece {
     static constexpr int kBytes = V * static_cast<int>(sizeof(T));
     static constexpr int kWords = kBytes >= 4 ? kBytes / 4 : 1;
-    uint32_t w[kWords];
+    alignas(kBytes >= 4 ? kBytes : 4) uint32_t w[kWords];
 
     __device__ __forceinline__ void load(const T* p)
     {
@@ -78,6 +78,11 @@ struct Piece {
             static_assert(kBytes == 2, "16, 4 or 2 bytes");
             w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
         }
+    }
+    __device__ __forceinline__ void load_shared(const T* p)
+    {
+        static_assert(kBytes == 16, "16 bytes");
+        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
     }
     __device__ __forceinline__ void clear()
     {
