@@ -256,6 +256,32 @@ def test_layer_norm_gradient_of_many_rows(env, shape, dt, dsum):
     assert ww.device_error() == 0
 
 
+@pytest.mark.parametrize("shape", [(9001, 1048), (2500, 4096), (1500, 8200), (700, 16384)])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("affine", [False, True])
+def test_layer_norm_of_many_long_sums(env, shape, dt, affine):
+    """Many long rows of strided inputs and their residuals: the sums, the result and its 8-bit form row by row."""
+    torch, ww = env
+    rows, n = shape
+    if dt == "f32" and n > 8192:
+        n //= 2
+    t, u = _type(torch, dt), U[dt]
+    x, r = _randn(torch, (rows, n + 8), 1, t)[:, 8:], _randn(torch, (rows, n), 2, t)
+    w, b = (_randn(torch, (n,), 3, t) + 1, _randn(torch, (n,), 4, t)) if affine else (None, None)
+    y, h, mean, rstd = ww.layer_norm(x, w, b, residual=r, return_stats=True)
+    assert torch.equal(h, x + r)
+    ref, mag, m, rs, *_ = _norm_reference(torch, h, w, b, 1e-5)
+    _within(y, ref, u * ref.abs() + F * mag, "y")
+    _within(mean, m[:, 0], F * h.double().abs().mean(-1), "mean")
+    _within(rstd, rs[:, 0], F * rs[:, 0] * (1 + h.double().abs().mean(-1) * rs[:, 0]), "rstd")
+    q, scale, total = ww.layer_norm_int8(x, w, b, residual=r)
+    assert torch.equal(total, h)
+    _within(q.double() * scale.double()[:, None], ref, 0.5 * scale.double()[:, None] * (1 + F) + 2 * F * mag.amax(-1, keepdim=True), "8 bits")
+    few = ww.layer_norm(x[:40], w, b, residual=r[:40])
+    assert (few[0].double() - y[:40].double()).abs().max() <= 2 * u * y[:40].double().abs().max()
+    assert ww.device_error() == 0
+
+
 @pytest.mark.parametrize("n", [24, 40, 60])
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_layer_norm_gradient_of_large_equal_values(env, n, dt):

@@ -210,6 +210,119 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
     }
 }
 
+// Rows of a residual sum, each held by a block: the rows to come lie in a ring in shared memory, filled by bulk copies.
+// us with the next row in registers, and so: 10000 rows of 8192, bf16, 133 and 108 (655 MB, 6.1 TB/s); 10000 of 4096, fp32, 115 and 104.
+// Not for rows without a residual (20000 of 4096 61 and 74), nor for those that warps hold (100000 of 1024 141 and 148).
+template <typename T, int V>
+__global__ void __launch_bounds__(row_threads(V, 2, false), 1) layer_norm_ring_kernel(const __grid_constant__ NormParams p)
+{
+    constexpr int P = 2, E = P * V / 2;
+    extern __shared__ __align__(16) uint8_t ring[];  // stages of a row of x and one of the residual, their barriers, the sums
+    const int S = p.stages;
+    const bool leader = threadIdx.x == 0;
+    const Columns<V, P, 0> column;
+    const uint32_t row_bytes = p.N * static_cast<uint32_t>(sizeof(T)), stage = 2 * row_bytes;
+    const uint32_t to = umma::smem_addr(ring), bars = to + S * stage;
+    float* const red = reinterpret_cast<float*>(ring + static_cast<uint32_t>(S) * (stage + 8));  // [2][3][32]
+    int64_t ahead = blockIdx.x;
+    const auto fill = [&](int s) {  // the leader
+        if (ahead >= p.rows) return;
+        umma::mbar_arrive_expect_tx(bars + s * 8, stage);
+        umma::bulk_g2s(to + s * stage, static_cast<const T*>(p.x) + ahead * p.xs, row_bytes, bars + s * 8);
+        umma::bulk_g2s(to + s * stage + row_bytes, static_cast<const T*>(p.r) + ahead * p.rs, row_bytes, bars + s * 8);
+        ahead += gridDim.x;
+    };
+    if (leader) {
+        for (int s = 0; s < S; ++s) umma::mbar_init(bars + s * 8, 1);
+        umma::mbar_fence_init();
+        for (int s = 0; s < S; ++s) fill(s);
+    }
+    __syncthreads();  // the barriers are there
+    int s = 0, turn = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 96) {
+        ok = ok && umma::mbar_poll(bars + s * 8, parity);  // once given up, no wait and no copy follows
+        Pair f[E];
+        {
+            Piece<T, V> x[P], y[P];  // zeros beyond the row
+            const T* from = reinterpret_cast<const T*>(ring + static_cast<uint32_t>(s) * stage);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                x[i].clear();
+                y[i].clear();
+                if (column(i) < p.N) {
+                    x[i].load_shared(from + column(i));
+                    y[i].load_shared(from + p.N + column(i));
+                }
+            }
+            Pair g[E];
+            values_of<T, V, P>(x, f);
+            values_of<T, V, P>(y, g);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                float a, c;
+                unpair(add2(f[i], g[i]), a, c);
+                f[i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(c)));
+            }
+        }
+        if (p.sum != nullptr)
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (column(i) < p.N) store_piece<T, V>(static_cast<T*>(p.sum) + row * p.N + column(i), f, i);
+        Pair t = f[0];
+#pragma unroll
+        for (int i = 1; i < E; ++i) t = add2(t, f[i]);
+        const float mean = row_sum<0>(both(t), red + turn) * p.inv_n;
+        if (leader) {
+            if (ok) fill(s);  // the sum's barrier: the stage has been read
+            if (p.mean != nullptr) p.mean[row] = mean;
+        }
+        const Pair nm = pair(-mean, -mean);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = add2(f[i], nm);
+        clear_beyond(f, p.N, column);
+        t = mul2(f[0], f[0]);
+#pragma unroll
+        for (int i = 1; i < E; ++i) t = fma2(f[i], f[i], t);
+        const float rstd = rsqrtf(fmaf(row_sum<0>(both(t), red + turn + 32), p.inv_n, p.eps));
+        if (leader && p.rstd != nullptr) p.rstd[row] = rstd;
+        const Pair r2 = pair(rstd, rstd);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (column(i) >= p.N) continue;
+            Piece<T, V> raw[2][1];
+            Pair w[V / 2], b[V / 2];
+            raw[1][0].clear();
+            if (p.w != nullptr) raw[0][0].load(static_cast<const T*>(p.w) + column(i));
+            if (p.b != nullptr) raw[1][0].load(static_cast<const T*>(p.b) + column(i));
+            values_of<T, V, 1>(raw[0], w);
+            values_of<T, V, 1>(raw[1], b);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) {
+                if (p.w == nullptr) w[e] = pair(1.0f, 1.0f);
+                f[i * V / 2 + e] = fma2(mul2(f[i * V / 2 + e], r2), w[e], b[e]);
+            }
+        }
+        if (p.q != nullptr) {
+            const RowScale k = row_scale(row_max<0>(largest(f), red + turn + 64));
+            if (leader) p.scale[row] = k.scale;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (column(i) < p.N) store_piece_int8<V>(p.q + row * p.qs + column(i), f, k.inv, i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (column(i) < p.N) store_piece<T, V>(static_cast<T*>(p.y) + row * p.N + column(i), f, i);
+        }
+        if (++s == S) {
+            s = 0;
+            parity ^= 1;
+        }
+    }
+    if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x61);
+}
+
 // Rows of any length: a block each, read again for each step.
 template <typename T>
 __global__ void __launch_bounds__(kLongBlock) layer_norm_long_kernel(const __grid_constant__ NormParams p)
@@ -715,9 +828,23 @@ NormParams params(const ww_layer_norm_t& p, bool norm) noexcept
 }
 
 template <typename T>
+bool launch_ring(NormParams& f, int threads, int sms, cudaStream_t stream) noexcept
+{
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    const auto kernel = layer_norm_ring_kernel<T, V>;
+    static std::atomic<uint64_t> raised{0};
+    f.err = device_error_slot();
+    if (f.err == nullptr || !allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return false;
+    const int resident = std::max(1, forward_threads(true) / threads), stage = 2 * f.N * static_cast<int>(sizeof(T)) + 8;
+    f.stages = std::min(8, (kMaxShared / resident - 2048) / stage);  // 3 of the longest rows, 2 x 32 KB
+    kernel<<<std::min(sms * resident, f.rows), threads, f.stages * stage + 768, stream>>>(f);
+    return true;
+}
+
+template <typename T>
 int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cudaStream_t stream) noexcept
 {
-    const NormParams f = params(p, norm);
+    NormParams f = params(p, norm);
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     const bool pieces = in_pieces(p, sizeof(T));
     const RowForm form = row_form(p.N, pieces ? V : 1, 4, false);
@@ -750,7 +877,17 @@ int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cuda
         case 3202: WW_NORM(V, 2, 32); break;
         case 3203: WW_NORM(V, 3, 32); break;
         case 3204: WW_NORM(V, 4, 32); break;
-        default: WW_NORM(V, 2, 0); break;
+        default:
+            // rings start later: for rows of several turns
+            if (norm && p.residual != nullptr && p.rows > 2 * sms * std::max(1, forward_threads(true) / form.threads)) {
+                if (!launch_ring<T>(f, form.threads, sms, stream)) {
+                    const int st = launch_status(name);
+                    return st != WW_SUCCESS ? st : WW_ERR_DEVICE;
+                }
+            } else {
+                WW_NORM(V, 2, 0);
+            }
+            break;
         }
 #undef WW_NORM
     return launch_status(name);
