@@ -282,6 +282,42 @@ def test_layer_norm_of_many_long_sums(env, shape, dt, affine):
     assert ww.device_error() == 0
 
 
+@pytest.mark.parametrize("n", [2049, 2050, 5001, 8191, 10239, 10240])
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+def test_layer_norm_of_many_long_odd_rows(env, n, off, dt):
+    """Rows in pairs: every other one begins off their grid, all with `off`; several rows a block; what lies next to them counts for nothing."""
+    torch, ww = env
+    t, u, rows = _type(torch, dt), U[dt], 700
+
+    def make(seed, pitch=n):  # rows `off` values behind 16 bytes, NaN around them
+        flat = torch.full((rows * pitch + 16,), math.nan, device="cuda", dtype=t)
+        x = flat[off:off + rows * pitch].view(rows, pitch)[:, :n]
+        return x.copy_(_randn(torch, (rows, n), seed, t))
+
+    x, dy, ds, w, b = make(1), make(2), make(3, n + 2 * (n % 3)), _randn(torch, (n + 1,), 4, t)[1:], _randn(torch, (n + 1,), 5, t)[1:]
+    y = torch.full((rows * n + 16,), 7.0, device="cuda", dtype=t)
+    out = y[off:off + rows * n].view(rows, n)
+    got, mean, rstd = ww.layer_norm(x, w, b, return_stats=True, out=out)
+    ref, mag, m, rs, xh, xa = _norm_reference(torch, x, w, b, 1e-5)
+    _within(got, ref, u * ref.abs() + F * mag + TINY[dt], "y")
+    assert torch.equal(y[:off], torch.full_like(y[:off], 7)) and torch.equal(y[off + rows * n:], torch.full_like(y[off + rows * n:], 7))
+    q, scale = ww.layer_norm_int8(x, w, b)
+    _within(q.double() * scale.double()[:, None], ref, 0.5 * scale.double()[:, None] * (1 + F) + 2 * F * mag.amax(-1, keepdim=True), "8 bits")
+    qx, sx = ww.quantize_tokens(x)
+    hq, hs, _ = _int8_host(x)
+    assert np.array_equal(qx.cpu().numpy(), hq) and np.array_equal(sx.cpu().numpy(), hs)
+    dx, dw, db = ww.layer_norm_backward(dy, x, w, mean, rstd, dsum=ds)
+    g = dy.double() * w.double()
+    dref = rs * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True)) + ds.double()
+    dmag = rs * (g.abs() + g.abs().mean(-1, keepdim=True) + xa * (g.abs() * xa).mean(-1, keepdim=True)) + ds.double().abs()
+    _within(dx, dref, u * dref.abs() + F * dmag + TINY[dt], "dx")
+    for a, terms, size in ((dw, dy.double() * xh, dy.double().abs() * xa), (db, dy.double(), dy.double().abs())):
+        _within(a, terms.sum(0), u * terms.sum(0).abs() + 4 * F * size.sum(0) + TINY[dt], "sums")
+    again = ww.layer_norm_backward(dy, x, w, mean, rstd, dsum=ds)
+    assert all(torch.equal(p, r) for p, r in zip((dx, dw, db), again))
+
+
 @pytest.mark.parametrize("n", [24, 40, 60])
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_layer_norm_gradient_of_large_equal_values(env, n, dt):

@@ -12,7 +12,7 @@
 // 4 with dsum; about 10 flops).  A row stays in registers between its sums (the
 // variance from the deviations, so that a large mean costs nothing), held by a
 // group of 4 to 32 lanes or, where a warp's registers do not hold it, by a block;
-// loads are 16 bytes a lane where rows start on 16 bytes, else single values.
+// loads are 16 bytes a lane where rows start on 16 bytes, else single values, or pairs for long rows.
 // Both directions run one resident round of blocks, the next rows' loads under way
 // while rows are computed: in registers, or for the gradient of rows of more than a piece a
 // lane in rings in shared memory.  In the gradient a lane owns the same columns of all its
@@ -22,8 +22,8 @@
 //
 // Measured: 469248 rows of 256, fp16, 480 MB: 78 us, 6.1 TB/s; their gradient with dsum,
 // bf16, 961 MB: 153 us with the join, 6.3 TB/s.  Gradient of 9001 rows of 1337, fp32, 144 MB:
-// 33.5 us (single loads; pieces of 16 bytes with the rows' ends masked took 52).
-// 40000 rows of 1337 in fp16, single loads of 2 bytes: 98 us for 214 MB, instructions.
+// 31 us (single loads; pieces of 16 bytes with the rows' ends masked took 52).
+// 40000 rows of 1337 in fp16, single loads of 2 bytes: 77 us for 214 MB, instructions.
 #include "rows.cuh"
 #include "umma.cuh"
 
@@ -62,9 +62,17 @@ struct NormParams {
     int64_t xs, rs, qs, gs, ds;  // elements between rows
     int32_t rows, N, norm;
     float eps, inv_n;
-    int32_t stages;  // of a ring
+    int32_t shift, odd;  // pairs: whether row 0 begins off their grid, whether every other row does
+    int32_t stages;      // of a ring
     int* err;
 };
+
+// Columns by which the pairs of a group's rows are shifted (rows a step apart begin alike).
+template <int V>
+__device__ __forceinline__ int pair_shift(const NormParams& p, int64_t row)
+{
+    return V == 2 ? (p.shift + static_cast<int>(row & 1) * p.odd) & 1 : 0;
+}
 
 // R rows of a group of lanes at a time, those of the block's next step loaded ahead.
 template <typename T, int V, int P, int GROUP, int R, bool RES>
@@ -75,25 +83,18 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
     constexpr int E = P * V / 2;
     constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block side by side
     const int lane = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
-    const Columns<V, P, GROUP> column;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (kGroups * R);
     int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + (GROUP ? threadIdx.x / (GROUP ? GROUP : 1) : 0);
+    const Columns<V, P, GROUP> column(pair_shift<V>(p, row0));
     const T* xp = static_cast<const T*>(p.x) + row0 * p.xs + column.first;
     const T* rp = RES ? static_cast<const T*>(p.r) + row0 * p.rs + column.first : nullptr;
     // weights: kept where they are few, else from L1 for each row
-    constexpr bool kKeep = E <= 4;
+    constexpr bool kKeep = E <= 4 || V == 2;
     Pair w[E], b[E];
     const auto weights = [&] {
         Piece<T, V> wr[P], br[P];
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            wr[i].clear();
-            br[i].clear();
-            if (p.w != nullptr && column(i) < p.N) {
-                wr[i].load(static_cast<const T*>(p.w) + column(i));
-                if (p.b != nullptr) br[i].load(static_cast<const T*>(p.b) + column(i));
-            }
-        }
+        load_weights(wr, static_cast<const T*>(p.w), p.N, column);
+        load_weights(br, static_cast<const T*>(p.b), p.N, column);
         values_of<T, V, P>(wr, w);
         values_of<T, V, P>(br, b);
         if (p.w == nullptr)
@@ -107,14 +108,11 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
 #pragma unroll
         for (int j = 0; j < R; ++j)
 #pragma unroll
-            for (int i = 0; i < P; ++i)
-                if (at + j * kGroups < p.rows && column(i) < p.N) {
-                    xr[j][i].load(xp + j * kGroups * p.xs + i * column.kNext);
-                    if constexpr (RES) rr[j][i].load(rp + j * kGroups * p.rs + i * column.kNext);
-                } else {
-                    xr[j][i].clear();
-                    if constexpr (RES) rr[j][i].clear();
-                }
+            for (int i = 0; i < P; ++i) {
+                const bool is = at + j * kGroups < p.rows;
+                load_piece<true>(xr[j][i], xp + j * kGroups * p.xs + i * column.kNext, i, p.N, is, column);
+                if constexpr (RES) load_piece<true>(rr[j][i], rp + j * kGroups * p.rs + i * column.kNext, i, p.N, is, column);
+            }
     };
     load(row0);
     int turn = 0;
@@ -146,7 +144,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
                 T* to = static_cast<T*>(p.sum) + (row0 + j * kGroups) * p.N;
 #pragma unroll
                 for (int i = 0; i < P; ++i)
-                    if (real(j) && column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
+                    if (real(j)) store_row_piece(to + column(i), f[j], i, p.N, column);
             }
         if (p.norm) {
             float v[R];
@@ -196,7 +194,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
                 int8_t* to = p.q + (row0 + j * kGroups) * p.qs;
 #pragma unroll
                 for (int i = 0; i < P; ++i)
-                    if (column(i) < p.N) store_piece_int8<V>(to + column(i), f[j], k[j].inv, i);
+                    if (column(i) < p.N) store_piece_int8<V>(to + column(i), f[j], k[j].inv, i, column.has(i, 0, p.N), column.has(i, 1, p.N));
             }
         } else {
 #pragma unroll
@@ -204,7 +202,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
                 T* to = static_cast<T*>(p.y) + (row0 + j * kGroups) * p.N;
 #pragma unroll
                 for (int i = 0; i < P; ++i)
-                    if (real(j) && column(i) < p.N) store_piece<T, V>(to + column(i), f[j], i);
+                    if (real(j)) store_row_piece(to + column(i), f[j], i, p.N, column);
             }
         }
     }
@@ -379,15 +377,13 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
     __shared__ float red[2][GROUP ? 1 : 64 * R];
     const int lane = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
     const int group = GROUP ? threadIdx.x / (GROUP ? GROUP : 1) : 0;
-    const Columns<V, P, GROUP> column;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kGroups * R);
+    int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + group;
+    const Columns<V, P, GROUP> column(pair_shift<V>(p, row0));
     Pair w[E], dw[E], db[E];
     {
         Piece<T, V> raw[P];
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            raw[i].clear();
-            if (p.w != nullptr && column(i) < p.N) raw[i].load(static_cast<const T*>(p.w) + column(i));
-        }
+        load_weights(raw, static_cast<const T*>(p.w), p.N, column);
         values_of<T, V, P>(raw, w);
     }
 #pragma unroll
@@ -399,8 +395,8 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
     // with a mean of 0 (-mean rstd times 0 is NaN where it passes fp32's range); few single values, where that is a
     // select each, take the row's last value instead (rows of 1337 in fp32 31 us and 32.4; 16 values a lane would spill).
     constexpr bool kLast = V == 1 && P <= 8;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kGroups * R);
-    int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kGroups * R) + group;
+    // one condition for a piece of all tensors, or each its own (300000 rows of 101, fp16, 115 and 95 us; 100000 of 401 74 and 83)
+    constexpr bool kTogether = V > 2 || P == 16;
     const T* xp = static_cast<const T*>(p.x) + row0 * p.xs + column.first;
     const T* gp = static_cast<const T*>(p.dy) + row0 * p.gs + column.first;
     const T* sp = DSUM ? static_cast<const T*>(p.dsum) + row0 * p.ds + column.first : nullptr;
@@ -414,19 +410,26 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
             const bool real = at + j * kGroups < p.rows;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
+                if constexpr (kTogether) {
+                    if (real && column(i) < p.N) {
+                        xr[j][i].load(xp + j * kGroups * p.xs + i * column.kNext);
+                        gr[j][i].load(gp + j * kGroups * p.gs + i * column.kNext);
+                        if constexpr (DSUM) sr[j][i].load(sp + j * kGroups * p.ds + i * column.kNext);
+                    } else {
+                        xr[j][i].clear();
+                        gr[j][i].clear();
+                        if constexpr (DSUM) sr[j][i].clear();
+                    }
+                    continue;
+                }
                 if constexpr (kLast) {
                     xr[j][i].clear();
                     if (real) xr[j][i].load(xp + j * kGroups * p.xs + (min(column(i), p.N - 1) - column.first));
-                }
-                if (real && column(i) < p.N) {
-                    if constexpr (!kLast) xr[j][i].load(xp + j * kGroups * p.xs + i * column.kNext);
-                    gr[j][i].load(gp + j * kGroups * p.gs + i * column.kNext);
-                    if constexpr (DSUM) sr[j][i].load(sp + j * kGroups * p.ds + i * column.kNext);
                 } else {
-                    if constexpr (!kLast) xr[j][i].clear();
-                    gr[j][i].clear();
-                    if constexpr (DSUM) sr[j][i].clear();
+                    load_piece<false>(xr[j][i], xp + j * kGroups * p.xs + i * column.kNext, i, p.N, real, column);
                 }
+                load_piece<false>(gr[j][i], gp + j * kGroups * p.gs + i * column.kNext, i, p.N, real, column);
+                if constexpr (DSUM) load_piece<false>(sr[j][i], sp + j * kGroups * p.ds + i * column.kNext, i, p.N, real, column);
             }
             mean[j] = real ? __ldg(p.mean + at + j * kGroups) : 0.0f;
             rstd[j] = real ? __ldg(p.rstd + at + j * kGroups) : 0.0f;
@@ -446,7 +449,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
             const Pair r2 = pair(rs[j], rs[j]);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const bool out0 = !kLast && column(2 * i / V) >= p.N, out1 = !kLast && column((2 * i + 1) / V) >= p.N;
+                const bool out0 = !kLast && !column.has(2 * i / V, 2 * i % V, p.N), out1 = !kLast && !column.has((2 * i + 1) / V, (2 * i + 1) % V, p.N);
                 xh[j][i] = mul2(add2(xh[j][i], pair(out0 ? 0.0f : -mean[j], out1 ? 0.0f : -mean[j])), r2);
             }
         }
@@ -484,7 +487,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
             if (row0 + j * kGroups < p.rows)
 #pragma unroll
                 for (int i = 0; i < P; ++i)
-                    if (column(i) < p.N) store_piece<T, V>(to + static_cast<int64_t>(j * kGroups) * p.N + i * column.kNext, g[j], i);
+                    store_row_piece(to + static_cast<int64_t>(j * kGroups) * p.N + i * column.kNext, g[j], i, p.N, column);
         }
     }
     if (p.part == nullptr) return;
@@ -498,8 +501,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROU
         if constexpr (GROUP == 0) {
 #pragma unroll
             for (int e = 0; e < 2 * E; ++e) {
-                const int c = column(e / V) + e % V;
-                if (c < p.N) sums[c] = v[e];
+                if (column.has(e / V, e % V, p.N) && column(e / V) + e % V < p.N) sums[column(e / V) + e % V] = v[e];
             }
         } else {
             constexpr int kRow = GROUP * P * V;  // columns kept of a row
@@ -798,9 +800,25 @@ bool in_pieces(const ww_layer_norm_t& p, int bytes) noexcept
     return p.y_q == nullptr || (reinterpret_cast<uintptr_t>(p.y_q) % 8 == 0 && p.y_q_stride % v == 0);
 }
 
+// Rows of pairs: every tensor's row begins on the grid of two values, or every one off it.  For rows of which a lane
+// holds 16 values; us by single values and by pairs: 8000 rows of 5001, fp16, 75 and 64, 4000 in fp32 38 and 30, gradients
+// of 6000 198 and 123, of 3000 in fp32 124 and 88; but 40000 of 1337, fp16, 77 and 113, gradients of 401 74 and 78, of 1337 70 and 76.
+constexpr int kPairs = 2048;
+bool in_pairs(const ww_layer_norm_t& p, int bytes) noexcept
+{
+    if (p.N <= kPairs) return false;
+    const auto off = [&](const void* q) { return reinterpret_cast<uintptr_t>(q) / bytes % 2; };
+    for (const void* q : {p.residual, static_cast<const void*>(p.y), static_cast<const void*>(p.sum), p.dy, p.dsum, static_cast<const void*>(p.dx)})
+        if (q != nullptr && off(q) != off(p.x)) return false;
+    const auto like = [&](const void* q, int64_t stride) { return q == nullptr || p.rows == 1 || (stride - p.N) % 2 == 0; };
+    return like(p.x, p.x_stride) && like(p.residual, p.residual_stride) && like(p.dy, p.dy_stride) && like(p.dsum, p.dsum_stride);
+}
+
 NormParams params(const ww_layer_norm_t& p, bool norm) noexcept
 {
     NormParams f{};
+    f.shift = static_cast<int>(reinterpret_cast<uintptr_t>(p.x) / (p.dtype == WW_DTYPE_FLOAT ? 4 : 2) % 2);
+    f.odd = p.N % 2;
     f.x = p.x;
     f.r = p.residual;
     f.w = p.weight;
@@ -827,6 +845,12 @@ NormParams params(const ww_layer_norm_t& p, bool norm) noexcept
     return f;
 }
 
+// Blocks, an even number where each takes rows of pairs one after another.
+int even_step(int64_t blocks, int64_t rows, const RowForm& form, bool pairs) noexcept
+{
+    return static_cast<int>(pairs && form.group == 0 && blocks < rows ? std::max<int64_t>(2, blocks & ~int64_t{1}) : blocks);
+}
+
 template <typename T>
 bool launch_ring(NormParams& f, int threads, int sms, cudaStream_t stream) noexcept
 {
@@ -846,12 +870,12 @@ int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cuda
 {
     NormParams f = params(p, norm);
     constexpr int V = 16 / static_cast<int>(sizeof(T));
-    const bool pieces = in_pieces(p, sizeof(T));
-    const RowForm form = row_form(p.N, pieces ? V : 1, 4, false);
+    const bool pieces = in_pieces(p, sizeof(T)), pairs = !pieces && in_pairs(p, sizeof(T));
+    const RowForm form = row_form(p.N, pieces ? V : pairs ? 2 : 1, 4, false);
     const auto go = [&](auto kernel, auto with_residual, int r) {
         const int groups = (form.group ? kBlock / form.group : 1) * r;
         const int resident = form.group ? forward_blocks(form.pieces) : std::max(1, forward_threads(pieces) / form.threads);
-        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + groups - 1) / groups));
+        const unsigned grid = even_step(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + groups - 1) / groups), i64(p.rows), form, pairs);
         if (p.residual == nullptr) kernel<<<grid, form.threads, 0, stream>>>(f);
         else with_residual<<<grid, form.threads, 0, stream>>>(f);
     };
@@ -860,6 +884,7 @@ int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cuda
        rows_at_once(V, P, GROUP))
     const int id = form.group * 100 + form.pieces;
     if (form.threads == 0) layer_norm_long_kernel<T><<<p.rows, kLongBlock, 0, stream>>>(f);
+    else if (pairs) WW_NORM(2, 8, 0);
     else if (!pieces)
         switch (id) {
         case 3204: WW_NORM(1, 4, 32); break;
@@ -895,7 +920,7 @@ int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cuda
 
 // Blocks of the gradient: one resident round, as far as there are rows for it.
 struct BackwardPlan {
-    bool pieces, ring;
+    bool pieces, pairs, ring;
     RowForm form;
     int blocks, splits;  // splits: of the rows, for the sums by columns (long rows)
     int stages, shared;  // of a ring, bytes of its block
@@ -907,7 +932,8 @@ BackwardPlan backward_plan(const ww_layer_norm_t& p, int sms) noexcept
     const int bytes = p.dtype == WW_DTYPE_FLOAT ? 4 : 2;
     BackwardPlan r{};
     r.pieces = in_pieces(p, bytes);
-    const int v = r.pieces ? 16 / bytes : 1;
+    r.pairs = !r.pieces && in_pairs(p, bytes);
+    const int v = r.pieces ? 16 / bytes : r.pairs ? 2 : 1;
     r.form = row_form(p.N, v, 4, true);
     r.ring = r.pieces && r.form.pieces > 1;
     if (r.ring) {
@@ -930,9 +956,9 @@ BackwardPlan backward_plan(const ww_layer_norm_t& p, int sms) noexcept
     }
     const int groups = r.form.group ? kBlock / r.form.group : 1;
     int resident = kBackwardBlocks;
-    if (r.form.group == 0 && r.form.threads > 0) resident = std::max(1, backward_threads(r.form.pieces) / r.form.threads);
+    if (r.form.group == 0 && r.form.threads > 0) resident = std::max(1, backward_threads(r.pairs ? 16 : r.form.pieces) / r.form.threads);
     const int at_once = groups * rows_at_once(v, r.form.pieces, r.form.group);
-    r.blocks = static_cast<int>(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + at_once - 1) / at_once));
+    r.blocks = even_step(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + at_once - 1) / at_once), p.rows, r.form, r.pairs);
     const int columns = (p.N + kBlock - 1) / kBlock;
     r.splits = std::max(1, std::min(p.rows, 4 * sms / columns));
     return r;
@@ -972,6 +998,8 @@ int backward(const ww_layer_norm_t& p, const BackwardPlan& plan, cudaStream_t st
     if (form.threads == 0) {
         layer_norm_backward_long_kernel<T><<<p.rows, kLongBlock, 0, stream>>>(f);
         if (sums) layer_norm_columns_kernel<T><<<dim3((p.N + kBlock - 1) / kBlock, plan.splits), kBlock, 0, stream>>>(f);
+    } else if (plan.pairs) {
+        WW_NORM(2, 8, 0);
     } else if (!plan.pieces) {
         switch (id) {
         case 3204: WW_NORM(1, 4, 32); break;

@@ -72,11 +72,42 @@ struct Piece {
             w[1] = u.y;
             w[2] = u.z;
             w[3] = u.w;
+        } else if constexpr (kBytes == 8) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+            w[0] = u.x;
+            w[1] = u.y;
         } else if constexpr (kBytes == 4) {
             w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
         } else {
-            static_assert(kBytes == 2, "16, 4 or 2 bytes");
+            static_assert(kBytes == 2, "16, 8, 4 or 2 bytes");
             w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+        }
+    }
+    // Values 0 and 1 of a pair of which one may lie outside the row; outside becomes 0.
+    __device__ __forceinline__ void set_pair(const T* first, bool has0, bool has1)
+    {
+        static_assert(V == 2, "pairs");
+        Piece<T, 1> a, b;
+        a.clear();
+        b.clear();
+        if (has0) a.load(first);
+        if (has1) b.load(first + 1);
+        if constexpr (sizeof(T) == 4) {
+            w[0] = a.w[0];
+            w[1] = b.w[0];
+        } else {
+            w[0] = a.w[0] | b.w[0] << 16;
+        }
+    }
+    // Of a pair at an edge of a row, read whole (its word lies in the row's memory), what lies outside becomes 0.
+    __device__ __forceinline__ void keep(bool has0, bool has1)
+    {
+        static_assert(V == 2, "pairs");
+        if constexpr (sizeof(T) == 4) {
+            w[0] = has0 ? w[0] : 0;
+            w[1] = has1 ? w[1] : 0;
+        } else {
+            w[0] &= (has0 ? 0xffffu : 0u) | (has1 ? 0xffff0000u : 0u);
         }
     }
     __device__ __forceinline__ void load_shared(const T* p)
@@ -116,14 +147,56 @@ __device__ __forceinline__ void values_of(const Piece<T, V> (&raw)[P], Pair (&f)
 
 // Columns of a lane's pieces: piece i begins at `first` + i kNext, side by side over the lanes
 // of a group or, where a block holds the row, of a warp (whose pieces follow one another).
+// Pairs (V == 2) of a row that begins off their grid are shifted by one: the first begins at -1.
 template <int V, int P, int GROUP>
 struct Columns {
     static constexpr int kNext = (GROUP ? GROUP : 32) * V;
     int first;
-    __device__ __forceinline__ Columns()
-        : first(GROUP ? threadIdx.x % (GROUP ? GROUP : 1) * V : threadIdx.x / 32 * (P * kNext) + threadIdx.x % 32 * V) {}
+    __device__ __forceinline__ explicit Columns(int shift = 0)
+        : first((GROUP ? threadIdx.x % (GROUP ? GROUP : 1) * V : threadIdx.x / 32 * (P * kNext) + threadIdx.x % 32 * V) - shift) {}
     __device__ __forceinline__ int operator()(int i) const { return first + i * kNext; }
+    // All of piece i lies within a row of n values; value j of it does.
+    __device__ __forceinline__ bool whole(int i, int n) const
+    {
+        return V == 2 ? static_cast<uint32_t>((*this)(i)) < static_cast<uint32_t>(n - 1) : (*this)(i) < n;
+    }
+    __device__ __forceinline__ bool has(int i, int j, int n) const
+    {
+        return V == 2 ? static_cast<uint32_t>((*this)(i) + j) < static_cast<uint32_t>(n) : (*this)(i) < n;
+    }
 };
+
+// Piece i of a row of n values, from `at`, zeros where it lies outside.  Pairs at an edge: EDGES value by value, else their
+// word or two words, which lie in the memory of the row's edge, with what is outside cleared.
+template <bool EDGES, typename T, int V, int P, int GROUP>
+__device__ __forceinline__ void load_piece(Piece<T, V>& to, const T* at, int i, int n, bool real, const Columns<V, P, GROUP>& column)
+{
+    if constexpr (V == 2 && EDGES) {
+        if (real && column.whole(i, n)) {
+            to.load(at);
+        } else {
+            to.clear();
+            if (real && column(i) < n) to.set_pair(at, column.has(i, 0, n), column.has(i, 1, n));
+        }
+    } else {
+        to.clear();
+        if (real && column(i) < n) to.load(at);
+        if constexpr (V == 2) to.keep(column(i) >= 0, column(i) + 1 < n);
+    }
+}
+
+// Weights of a lane's columns, which may begin anywhere.
+template <typename T, int V, int P, int GROUP>
+__device__ __forceinline__ void load_weights(Piece<T, V> (&to)[P], const T* w, int n, const Columns<V, P, GROUP>& column)
+{
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        to[i].clear();
+        if (w == nullptr) continue;
+        if constexpr (V == 2) to[i].set_pair(w + column(i), column.has(i, 0, n), column.has(i, 1, n));
+        else if (column(i) < n) to[i].load(w + column(i));
+    }
+}
 
 // What a lane holds beyond the n values of its row becomes 0.
 template <int V, int P, int GROUP>
@@ -131,9 +204,10 @@ __device__ __forceinline__ void clear_beyond(Pair (&f)[P * V / 2], int n, const 
 {
 #pragma unroll
     for (int i = 0; i < P; ++i)
-        if (column(i) >= n)
+        if (!column.whole(i, n))
 #pragma unroll
             for (int e = i * V; e < (i + 1) * V; ++e) {
+                if (column.has(i, e % V, n)) continue;
                 float a, b;
                 unpair(f[e / 2], a, b);
                 f[e / 2] = e % 2 ? pair(a, 0.0f) : pair(0.0f, b);
@@ -148,6 +222,11 @@ __device__ __forceinline__ void store_piece(T* p, const Pair (&f)[E], int i)
         float v[2];
         unpair(f[i / 2], v[0], v[1]);
         *p = from_float<T>(i % 2 ? v[1] : v[0]);
+    } else if constexpr (V == 2) {
+        float v[2];
+        unpair(f[i], v[0], v[1]);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+        else *reinterpret_cast<uint32_t*>(p) = pack2<T>(v[0], v[1]);
     } else {
         float v[V];
 #pragma unroll
@@ -159,15 +238,34 @@ __device__ __forceinline__ void store_piece(T* p, const Pair (&f)[E], int i)
     }
 }
 
+// Piece i of a row of n values, as far as it lies within.
+template <typename T, int V, int P, int GROUP, int E>
+__device__ __forceinline__ void store_row_piece(T* p, const Pair (&f)[E], int i, int n, const Columns<V, P, GROUP>& column)
+{
+    if (column.whole(i, n)) {
+        store_piece<T, V>(p, f, i);
+    } else if constexpr (V == 2) {
+        float v[2];
+        unpair(f[i], v[0], v[1]);
+        if (column.has(i, 0, n)) p[0] = from_float<T>(v[0]);
+        if (column.has(i, 1, n)) p[1] = from_float<T>(v[1]);
+    }
+}
+
 // Piece i in 8 bits to memory.
 template <int V, int E>
-__device__ __forceinline__ void store_piece_int8(int8_t* p, const Pair (&f)[E], float inv, int i)
+__device__ __forceinline__ void store_piece_int8(int8_t* p, const Pair (&f)[E], float inv, int i, bool has0 = true, bool has1 = true)
 {
     const Pair k = pair(inv, inv);
     if constexpr (V == 1) {
         uint32_t q[2];
         quantise2(f[i / 2], k, q[0], q[1]);
         *p = static_cast<int8_t>(i % 2 ? q[1] : q[0]);
+    } else if constexpr (V == 2) {
+        uint32_t q[2];
+        quantise2(f[i], k, q[0], q[1]);
+        if (has0) p[0] = static_cast<int8_t>(q[0]);
+        if (has1) p[1] = static_cast<int8_t>(q[1]);
     } else {
         uint32_t q[V];
 #pragma unroll
@@ -283,21 +381,24 @@ struct RowForm {
 };
 
 // Most threads of a block that holds a row, P pieces of V values a lane.
-__host__ __device__ constexpr int row_threads(int v, int p, bool backward) { return v > 1 ? (backward ? 512 : 1024) : p == 8 ? 256 : 640; }
+__host__ __device__ constexpr int row_threads(int v, int p, bool backward) { return v > 2 ? (backward ? 512 : 1024) : v == 1 && p == 8 ? 256 : 640; }
 
 // Pieces of 16 bytes (v > 1): the form with the fewest idle lanes, and of those the one
-// with the fewest pieces a lane (at most `most` in a warp).  Single values (v == 1, rows that
-// do not start on 16 bytes): 4, 8 or 16 a lane.  Rows that a warp does not hold: a block.
+// with the fewest pieces a lane (at most `most` in a warp).  Pairs or single values (v <= 2, rows that
+// do not start on 16 bytes): 4, 8 or 16 values a lane, pairs only where a block's lanes hold 16.  Rows that
+// a warp does not hold: a block.
 inline RowForm row_form(int n, int v, int most, bool backward)
 {
-    const int all = (n + v - 1) / v;
+    const int all = v == 2 ? n / 2 + 1 : (n + v - 1) / v;  // pairs may be shifted by one
     const auto fits = [&](int p) { return all <= row_threads(v, p, backward) * p; };
     const auto block = [&](int p) { return RowForm{0, p, ((all + p - 1) / p + 31) / 32 * 32}; };
-    if (v > 1) {
+    if (v > 2) {
         constexpr int kForms[][2] = {{4, 1}, {8, 1}, {16, 1}, {32, 1}, {16, 3}, {32, 2}, {32, 3}, {32, 4}};
         for (const auto& f : kForms)  // ascending lanes x pieces
             if (f[0] * f[1] >= all && f[1] <= most) return {f[0], f[1], 256};
         if (fits(2)) return block(2);
+    } else if (v == 2) {
+        if (fits(8)) return block(8);
     } else {
         if (n <= 128) return {32, 4, 256};
         if (n <= 512) return {32, 16, 256};
