@@ -395,9 +395,9 @@ int ww_relative_position_bucket(int rel, int num_buckets, int max_distance, int 
  * (extensions; the formulas are their specification).
  *
  * A row in 8 bits: a = max |x|, scale = a / 127, q = rint(x * (127 / a)), ties
- * to even, each step in fp32 (for fp32 rows q is the whole number nearest to
- * 127 x / a); so q is in [-127, 127].  A row with a NaN or an infinity has scale
- * NaN (what is computed from it is NaN), one with a < 2^-119 scale 0 and zeros.
+ * to even, each step in fp32; so q is in [-127, 127].  A row with a NaN or an
+ * infinity has scale NaN (what is computed from it is NaN), one with a < 2^-119
+ * scale 0 and zeros.
  * fp32 arithmetic, one rounding to a result's type; the same call gives the
  * same bits again.  Outputs do not overlap inputs.
  * ------------------------------------------------------------------------- */

@@ -351,44 +351,15 @@ def test_outputs_apart_from_inputs(env):
 # ---------------------------------------------------------------- 8 bits
 
 def _int8_host(x):
-    """Whole numbers and scales of rows by the same fp32 operations on the host; of fp32 rows to the nearest, in 64 bits
-    (127 x is exact there, and a quotient half way between whole numbers too)."""
-    full = x.dtype == x.float().dtype
+    """Whole numbers and scales of rows by the same fp32 operations on the host."""
     x = x.float().cpu().numpy()
     top = np.abs(x).max(-1, keepdims=True).astype(np.float32)
     with np.errstate(all="ignore"):
         small, bad = top < np.float32(2.0 ** -119), ~np.isfinite(top)
         inv = np.where(small | bad, np.float32(0), np.float32(127) / top).astype(np.float32)
-        x = np.where(np.isfinite(x), x, 0)
-        q = np.rint((x * inv).astype(np.float32)).astype(np.int8)
-        if full:
-            q = np.rint(np.where(small | bad, 0, x.astype(np.float64) * 127 / np.where(small | bad, 1, top).astype(np.float64))).astype(np.int8)
+        q = np.rint((np.where(np.isfinite(x), x, 0) * inv).astype(np.float32)).astype(np.int8)
         scale = np.where(small, np.float32(0), np.where(bad, np.float32(np.nan), top / np.float32(127)))
     return q, scale[..., 0].astype(np.float32), bad[..., 0]
-
-
-@pytest.mark.parametrize("n", [256, 1000, 1337, 5001, 40001])
-@pytest.mark.parametrize("scale", [1.0, 2.0 ** 100, 2.0 ** -100])
-def test_fp32_rows_to_the_nearest(env, n, scale):
-    """fp32 values half way between two steps, and next to that: the nearest whole number, ties to the even one."""
-    torch, ww = env
-    tops = torch.tensor([100.0, 254.0, 1000.0, 12345.0, 127.0, 1e6 + 1, 3.0, 0.7], device="cuda")
-    g = torch.Generator(device="cuda").manual_seed(n)
-    k = torch.randint(-127, 127, (8, n), generator=g, device="cuda").double() + 0.5  # the middles
-    x = (k * tops.double()[:, None] / 127).float()
-    x = torch.nextafter(x, torch.where(torch.rand(x.shape, generator=g, device="cuda") < 0.3, x * 2, torch.where(torch.rand(x.shape, generator=g, device="cuda") < 0.4, 0 * x, x)))
-    x[:3, ::2] = torch.randint(-100, 101, x[:3, ::2].shape, generator=g, device="cuda").float()  # whole numbers: exact middles of 254ths
-    x = x.clamp(-tops[:, None], tops[:, None])
-    x[:, 0] = tops
-    x = x * scale
-    q, s = ww.quantize_tokens(x)
-    hq, hs, _ = _int8_host(x)
-    assert np.array_equal(q.cpu().numpy(), hq) and np.array_equal(s.cpu().numpy(), hs)
-    w = torch.eye(n if n < 2000 else 16, (n + 15) // 16 * 16, device="cuda").to(torch.int8)[:, :n]  # the call's own 8-bit form, few rows and one
-    one = torch.ones(w.shape[0], device="cuda")
-    for rows in (1, 8):
-        y = ww.int8_linear(x[:rows], w, one)
-        assert torch.equal(y, q[:rows, :w.shape[0]].float() * s[:rows, None])
 
 
 @pytest.mark.parametrize("shape", [(1, 1), (5, 16), (3, 4, 48), (1000, 256), (7, 1000), (2, 1337), (1, 9001), (3, 40000), (2, 40001)])

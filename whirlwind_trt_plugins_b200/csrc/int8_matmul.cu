@@ -511,9 +511,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) int8_few_kernel(const __grid_c
         __syncthreads();
         if (threadIdx.x < p.M) scale[threadIdx.x] = row_scale(__uint_as_float(top[threadIdx.x])).scale;
         for (int m0 = 0; m0 < p.M; m0 += kBatch) {
-            RowScale of[kBatch];
+            float inv[kBatch];
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) of[j] = row_scale(__uint_as_float(top[min(m0 + j, p.M - 1)]));
+            for (int j = 0; j < kBatch; ++j) inv[j] = row_scale(__uint_as_float(top[min(m0 + j, p.M - 1)])).inv;
             int8_t* to = reinterpret_cast<int8_t*>(tokens) + m0 * p.pitch;
             if (p.x_pieces) {
                 for (int k = threadIdx.x * V; k < end; k += kFewThreads * V) {
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int8_few_kernel(const __grid_c
                     for (int j = 0; j < kBatch; ++j) {
                         if (m0 + j >= p.M) continue;
                         values_of<O, V, 1>(r[j], f);
-                        store_piece_int8<O, V>(to + j * p.pitch + k, f, of[j], 0);
+                        store_piece_int8<V>(to + j * p.pitch + k, f, inv[j], 0);
                     }
                 }
             } else {
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int8_few_kernel(const __grid_c
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j)
                         if (m0 + j < p.M)
-                            to[j * p.pitch + k] = k < p.K ? quantise<O>(to_float(static_cast<const O*>(p.x)[(m0 + j) * p.x_stride + k]), of[j]) : 0;
+                            to[j * p.pitch + k] = k < p.K ? quantise(to_float(static_cast<const O*>(p.x)[(m0 + j) * p.x_stride + k]), inv[j]) : 0;
             }
         }
     } else {

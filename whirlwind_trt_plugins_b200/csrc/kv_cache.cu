@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kBlock) quantize_kv_kernel(const __grid_consta
     for (int i = 0; i < R; ++i) {
         const int r = first + i * kStep;
         if (from[r] < 0) continue;
-        if (d < p.D) store_piece_int8<T, 8>(s.q + to[r] + d, f[i], k[i], 0);
+        if (d < p.D) store_piece_int8<8>(s.q + to[r] + d, f[i], k[i].inv, 0);
         if (lane == 0) s.scale[scale_to[r]] = k[i].scale;
     }
 }

@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
                 int8_t* to = p.q + (row0 + j * kGroups) * p.qs;
 #pragma unroll
                 for (int i = 0; i < P; ++i)
-                    if (column(i) < p.N) store_piece_int8<T, V>(to + column(i), f[j], k[j], i, column.has(i, 0, p.N), column.has(i, 1, p.N));
+                    if (column(i) < p.N) store_piece_int8<V>(to + column(i), f[j], k[j].inv, i, column.has(i, 0, p.N), column.has(i, 1, p.N));
             }
         } else {
 #pragma unroll
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(row_threads(V, 2, false), 1) layer_norm_ring_k
             if (leader) p.scale[row] = k.scale;
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                if (column(i) < p.N) store_piece_int8<T, V>(p.q + row * p.qs + column(i), f, k, i);
+                if (column(i) < p.N) store_piece_int8<V>(p.q + row * p.qs + column(i), f, k.inv, i);
         } else {
 #pragma unroll
             for (int i = 0; i < P; ++i)
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kLongBlock) layer_norm_long_kernel(const __gri
     const RowScale k = row_scale(row_max<0>(top, red[2]));
     if (threadIdx.x == 0) p.scale[row] = k.scale;
     for (int c = threadIdx.x; c < p.N; c += kLongBlock)
-        p.q[row * p.qs + c] = quantise<T>(value(c), k);
+        p.q[row * p.qs + c] = quantise(value(c), k.inv);
 }
 
 template <typename T, int V, int P, int GROUP, int R, bool DSUM>

@@ -12,17 +12,17 @@ namespace ww {
 // ---- a row in 8 bits ----
 //
 // a = max |x|,  scale = a / 127,  q = rint(x * (127 / a)) in fp32: whole numbers in
-// [-127, 127], x = scale q within half a step; of fp32 rows the whole number nearest to 127 x / a itself.  A row with a NaN or an infinity
+// [-127, 127], x = scale q within half a step.  A row with a NaN or an infinity
 // has scale NaN, so that what is computed from it is NaN; one whose largest
 // magnitude is below 2^-119 (the scale would leave fp32's normal range) has
 // scale 0 and zeros.
 struct RowScale {
-    float inv, scale, top;
+    float inv, scale;
 };
 
 __device__ __forceinline__ RowScale row_scale(float top)  // top: max_nan over |x|
 {
-    RowScale r{0.0f, 0.0f, top};
+    RowScale r{0.0f, 0.0f};
     if (!(top < INFINITY)) r.scale = __int_as_float(0x7fffffff);
     else if (top >= 0x1p-119f) {
         r.inv = __fdiv_rn(127.0f, top);
@@ -42,53 +42,16 @@ __device__ __forceinline__ int8_t quantise(float x, float inv)
     return static_cast<int8_t>(__float_as_uint(__fadd_rn(__fmul_rn(x, inv), kRintMagic)));
 }
 
-// The same for 127 x / a to the nearest, ties to even.  fp32's product is off by up to 2^-15 (values of 16 bits keep further
-// from the middle of two steps than that, or meet it); what comes so near to a middle is decided by the sign of
-// 127 x - (q +- 1/2) a, whose large terms cancel and whose roundings are added back.
-inline __device__ __noinline__ uint32_t at_the_middle(float x, float top, float whole)
-{
-    const float s = top > 1.0f ? 0x1p-8f : 1.0f;  // within fp32's range
-    const float c = 127.0f * s, a = top * s;
-    const float h = __fmul_rn(x, c), g = __fmul_rn(whole, a);
-    const float hi = h - g, lo = __fmaf_rn(x, c, -h) - __fmaf_rn(whole, a, -g);
-    const float above = (hi - 0.5f * a) + lo, below = (hi + 0.5f * a) + lo;
-    const bool odd = static_cast<int>(whole) & 1;
-    return (above > 0.0f || (above == 0.0f && odd)) ? 1u : (below < 0.0f || (below == 0.0f && odd)) ? ~0u : 0u;
-}
-
-__device__ __forceinline__ uint32_t quantise_nearest(float x, RowScale k)
-{
-    const float p = __fmul_rn(x, k.inv), m = __fadd_rn(p, kRintMagic), whole = __fsub_rn(m, kRintMagic);
-    uint32_t q = __float_as_uint(m);
-    if (fabsf(p - whole) > 0.4999f) q += at_the_middle(x, k.top, whole);
-    return q;
-}
-
-// A value of a row of T in 8 bits.
-template <typename T>
-__device__ __forceinline__ int8_t quantise(float x, RowScale k)
-{
-    if constexpr (sizeof(T) == 4) return static_cast<int8_t>(quantise_nearest(x, k));
-    else return quantise(x, k.inv);
-}
-
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)  // low bytes
 {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // Two values to whole numbers in the low bytes.
-template <typename T>
-__device__ __forceinline__ void quantise2(Pair x, RowScale k, uint32_t& lo, uint32_t& hi)
+__device__ __forceinline__ void quantise2(Pair x, Pair inv, uint32_t& lo, uint32_t& hi)
 {
     float a, b;
-    if constexpr (sizeof(T) == 4) {
-        unpair(x, a, b);
-        lo = quantise_nearest(a, k);
-        hi = quantise_nearest(b, k);
-        return;
-    }
-    unpair(mul2(x, pair(k.inv, k.inv)), a, b);
+    unpair(mul2(x, inv), a, b);
     lo = __float_as_uint(__fadd_rn(a, kRintMagic));
     hi = __float_as_uint(__fadd_rn(b, kRintMagic));
 }
@@ -290,22 +253,23 @@ __device__ __forceinline__ void store_row_piece(T* p, const Pair (&f)[E], int i,
 }
 
 // Piece i in 8 bits to memory.
-template <typename T, int V, int E>
-__device__ __forceinline__ void store_piece_int8(int8_t* p, const Pair (&f)[E], RowScale k, int i, bool has0 = true, bool has1 = true)
+template <int V, int E>
+__device__ __forceinline__ void store_piece_int8(int8_t* p, const Pair (&f)[E], float inv, int i, bool has0 = true, bool has1 = true)
 {
+    const Pair k = pair(inv, inv);
     if constexpr (V == 1) {
         uint32_t q[2];
-        quantise2<T>(f[i / 2], k, q[0], q[1]);
+        quantise2(f[i / 2], k, q[0], q[1]);
         *p = static_cast<int8_t>(i % 2 ? q[1] : q[0]);
     } else if constexpr (V == 2) {
         uint32_t q[2];
-        quantise2<T>(f[i], k, q[0], q[1]);
+        quantise2(f[i], k, q[0], q[1]);
         if (has0) p[0] = static_cast<int8_t>(q[0]);
         if (has1) p[1] = static_cast<int8_t>(q[1]);
     } else {
         uint32_t q[V];
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) quantise2<T>(f[i * V / 2 + j], k, q[2 * j], q[2 * j + 1]);
+        for (int j = 0; j < V / 2; ++j) quantise2(f[i * V / 2 + j], k, q[2 * j], q[2 * j + 1]);
         if constexpr (V == 4)
             *reinterpret_cast<uint32_t*>(p) = pack4(q[0], q[1], q[2], q[3]);
         else
@@ -391,7 +355,6 @@ __device__ __forceinline__ void row_scales(const float (&top)[K], RowScale (&r)[
         const RowScale own = row_scale(mine);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            r[k].top = top[k];
             r[k].inv = __shfl_sync(~0u, own.inv, k, kLanes);
             r[k].scale = __shfl_sync(~0u, own.scale, k, kLanes);
         }
