@@ -394,7 +394,7 @@ int ww_relative_position_bucket(int rel, int num_buckets, int max_distance, int 
  * Operators of a matching layer around the attention, in part in 8 bits
  * (extensions; the formulas are their specification).
  *
- * A row in 8 bits: a = max |x|, scale = a / 127, q = rint(x * (127 / a)), ties
+ * A row in 8 bits: a = max |x|, scale = a / 127, q = rint(x * (127 * (1 / a))), ties
  * to even, each step in fp32; so q is in [-127, 127].  A row with a NaN or an
  * infinity has scale NaN (what is computed from it is NaN), one with a < 2^-119
  * scale 0 and zeros.

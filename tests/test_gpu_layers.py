@@ -356,7 +356,7 @@ def _int8_host(x):
     top = np.abs(x).max(-1, keepdims=True).astype(np.float32)
     with np.errstate(all="ignore"):
         small, bad = top < np.float32(2.0 ** -119), ~np.isfinite(top)
-        inv = np.where(small | bad, np.float32(0), np.float32(127) / top).astype(np.float32)
+        inv = np.where(small | bad, np.float32(0), np.float32(1) / top * np.float32(127)).astype(np.float32)
         q = np.rint((np.where(np.isfinite(x), x, 0) * inv).astype(np.float32)).astype(np.int8)
         scale = np.where(small, np.float32(0), np.where(bad, np.float32(np.nan), top / np.float32(127)))
     return q, scale[..., 0].astype(np.float32), bad[..., 0]

@@ -11,8 +11,9 @@ namespace ww {
 
 // ---- a row in 8 bits ----
 //
-// a = max |x|,  scale = a / 127,  q = rint(x * (127 / a)) in fp32: whole numbers in
-// [-127, 127], x = scale q within half a step.  A row with a NaN or an infinity
+// a = max |x|,  scale = a / 127,  q = rint(x * (127 * (1 / a))), every operation rounded in
+// fp32, so that tensor operations give the same numbers: whole ones in [-127, 127], x = scale q
+// within half a step and 2^-15 of one (one of 10^5 fp32 values goes to the other side of a middle).  A row with a NaN or an infinity
 // has scale NaN, so that what is computed from it is NaN; one whose largest
 // magnitude is below 2^-119 (the scale would leave fp32's normal range) has
 // scale 0 and zeros.
@@ -25,16 +26,16 @@ __device__ __forceinline__ RowScale row_scale(float top)  // top: max_nan over |
     RowScale r{0.0f, 0.0f};
     if (!(top < INFINITY)) r.scale = __int_as_float(0x7fffffff);
     else if (top >= 0x1p-119f) {
-        r.inv = __fdiv_rn(127.0f, top);
+        r.inv = __fmul_rn(__fdiv_rn(1.0f, top), 127.0f);
         r.scale = __fdiv_rn(top, 127.0f);
     }
     return r;
 }
 
 // rint of a product in [-127, 127] in the low byte: adding 1.5 * 2^23 leaves the whole
-// number, ties to even, in the low bits.  The product is rounded before, so that values of
-// few bits that lie half way between two steps are met as ties in spite of the
-// quotient's rounding (packed forms of the two would be fused by the compiler).
+// number, ties to even, in the low bits.  The product is rounded before, as the formula says, so
+// that most values of few bits that lie half way between two steps are met as ties (packed
+// forms of the two would be fused by the compiler).
 constexpr float kRintMagic = 12582912.0f;
 
 __device__ __forceinline__ int8_t quantise(float x, float inv)
