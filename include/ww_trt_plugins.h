@@ -498,9 +498,9 @@ int ww_dequantize_kv(const ww_kv_cache_t* p, void* stream);
  * int8 caches [B, Lk, Hk, D], with k_scale and v_scale.  Scales of masked places
  * do not matter either; those of valid places are >= 0 or NaN.  Up to 128 rows (query heads of
  * a key head x tokens) the values are used as they stand, P in fp16 with the values'
- * scales in it, unless copies are expected to be faster (more than 64 rows against many keys,
- * more than 16 against short ones of many items); beyond, and then, keys and values are
- * rounded to q's type in the workspace.  Up to 128 rows run without a workspace too, as
+ * scales in it, unless q is fp16 and copies are expected to be faster (more than 64 rows against
+ * many keys, more than 16 against short ones of many items); beyond, and then, keys and values
+ * are rounded to q's type in the workspace.  Up to 128 rows run without a workspace too, as
  * they stand (fewer blocks share long keys then); copies need B * Lk * Hk * D * 4 bytes,
  * rounded up to 512, at least.
  * No gradients.  D a multiple of 16. */

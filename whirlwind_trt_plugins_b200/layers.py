@@ -390,7 +390,7 @@ def cross_attention_int8(q, k_cache, v_cache, k_scale, v_scale, scale: float | N
     (k_cache, v_cache [B, Lk, Hk, D] int8, k_scale, v_scale [B, Hk, Lk] fp32), for q
     [B, Lq, Hq, D] fp16 or bf16, D a multiple of 16 up to 128; the other arguments
     are those of ``cross_attention``.  Places from k_lens on, and masked ones, may
-    hold anything.  Calls of few query rows per key head (up to 16, or 128 where it is
+    hold anything.  Calls of few query rows per key head (up to 128, in fp16 where it is
     faster) read each key and value as a byte; others round them to q's type first.
     No gradients."""
     T = _Torch.get()
