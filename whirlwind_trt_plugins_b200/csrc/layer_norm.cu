@@ -10,7 +10,7 @@
 //
 // Bound: HBM (forward 2 values per element moved, 4 with a residual; backward 3,
 // 4 with dsum; about 10 flops).  A row stays in registers between its sums (the
-// variance from the deviations, so that a large mean costs nothing), held by a
+// variance from the deviations; rows far from zero once more, so that a large mean costs no digits), held by a
 // group of 4 to 32 lanes or, where a warp's registers do not hold it, by a block;
 // loads are 16 bytes a lane where rows start on 16 bytes, else single values, or pairs for long rows.
 // Both directions run one resident round of blocks, the next rows' loads under way
@@ -41,7 +41,12 @@ constexpr int kLongBlock = 1024;
 // 1 row and 6 blocks 89.  Their gradient with dsum, bf16: 2 rows and 2 blocks 153 us; 1 row and
 // 3 blocks 194.
 __host__ __device__ constexpr int rows_at_once(int v, int pieces, int group) { return v > 1 && pieces == 1 && group > 0 ? 2 : 1; }
-__host__ __device__ constexpr int forward_blocks(int pieces) { return pieces == 1 ? 4 : pieces < 4 ? 3 : 2; }
+// Three pieces a lane, 80000 rows of 640: fp16 3 blocks (which spill) 49.7 us and 2 45.6, with a residual 89 and 69.6; 100000 of 320 in
+// fp32 45 and 52, with a residual 90 and 86.
+__host__ __device__ constexpr int forward_blocks(int v, int pieces, bool residual)
+{
+    return pieces == 1 ? 4 : pieces >= 4 || (pieces == 3 && (v == 8 || residual)) ? 2 : 3;
+}
 constexpr int kBackwardBlocks = 2;
 // Threads of an SM's blocks where a block holds a row.  Gradient of 9001 rows of 1337 in
 // fp32 (8 single values a lane): 768 threads 33.5 us; 512 and 1024, which spills, 40 and 38.
@@ -49,7 +54,7 @@ constexpr int kBackwardBlocks = 2;
 int forward_threads(bool pieces) { return pieces ? 1024 : 768; }
 int backward_threads(int per_lane) { return per_lane == 8 ? 768 : 512; }
 // Blocks of a row that the compiler keeps registers for, so that these threads fit.
-__host__ __device__ constexpr int backward_row_blocks(int v, int pieces) { return v == 1 && pieces == 8 ? 3 : 1; }
+__host__ __device__ constexpr int row_blocks(int v, int pieces) { return v == 1 && pieces == 8 ? 3 : 1; }
 
 struct NormParams {
     const void *x, *r, *w, *b;
@@ -74,12 +79,56 @@ __device__ __forceinline__ int pair_shift(const NormParams& p, int64_t row)
     return V == 2 ? (p.shift + static_cast<int>(row & 1) * p.odd) & 1 : 0;
 }
 
-// R rows of a group of lanes at a time, those of the block's next step loaded ahead.
-template <typename T, int V, int P, int GROUP, int R, bool RES>
-__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GROUP ? forward_blocks(P) : 1)
-    layer_norm_kernel(const __grid_constant__ NormParams p)
+template <int E>
+__device__ __forceinline__ float sum_of(const Pair (&f)[E])
 {
-    __shared__ float red[2][GROUP ? 1 : 3][32 * R];
+    Pair s = f[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) s = add2(s, f[i]);
+    return both(s);
+}
+
+// f less the mean, 0 beyond the row; the sum of their squares.
+template <int V, int P, int GROUP, int E>
+__device__ __forceinline__ float deviations(Pair (&f)[E], float mean, int n, const Columns<V, P, GROUP>& column)
+{
+    const Pair nm = pair(-mean, -mean);
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = add2(f[i], nm);
+    clear_beyond(f, n, column);
+    Pair s = mul2(f[0], f[0]);
+#pragma unroll
+    for (int i = 1; i < E; ++i) s = fma2(f[i], f[i], s);
+    return both(s);
+}
+
+// Values of a row and its residual, rounded to their type as they are kept.
+template <typename T, int V, int P>
+__device__ __forceinline__ void add_residual(Pair (&f)[P * V / 2], const Piece<T, V> (&r)[P])
+{
+    Pair g[P * V / 2];
+    values_of<T, V, P>(r, g);
+#pragma unroll
+    for (int i = 0; i < P * V / 2; ++i) {
+        float a, c;
+        unpair(add2(f[i], g[i]), a, c);
+        f[i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(c)));
+    }
+}
+
+// Whether a row's deviations are so far below its mean (32 times) that the mean's own rounding, 2^-24 of it for each
+// addition and for the product with 1 / N, shows in them.
+__device__ __forceinline__ bool mean_far(float mean, float variance) { return mean != 0.0f && variance <= mean * mean * 0x1p-10f; }
+
+// The rows of a block.  R rows of a group of lanes at a time, those of the block's next step loaded ahead.  Returns whether one is far
+// from its deviations; then the block (GROUP: the warp) goes over its rows again, with FAR, and writes those rows anew: their
+// deviations less what these leave of the mean.  Of a row of one value they are a few units in its last place, all equal,
+// whose sum is exact, and so is its quotient by N: what remains is 0.  (Done at once, with the next rows under way in
+// registers, it costs the other rows 3 to 20 % of their time.)  469248 rows of 256, fp16: 78 us without such rows, 147 with one
+// in 1000, 215 where all are.
+template <typename T, int V, int P, int GROUP, int R, bool RES, bool FAR>
+__device__ __forceinline__ bool norm_rows(const NormParams& p, float (&red)[2][GROUP ? 1 : 3][32 * R])
+{
     constexpr int E = P * V / 2;
     constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block side by side
     const int lane = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
@@ -114,31 +163,25 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
                 if constexpr (RES) load_piece<true>(rr[j][i], rp + j * kGroups * p.rs + i * column.kNext, i, p.N, is, column);
             }
     };
-    load(row0);
+    if (!FAR) load(row0);
     int turn = 0;
+    bool any_far = false;
     for (int64_t base = static_cast<int64_t>(blockIdx.x) * (kGroups * R); base < p.rows; base += step, row0 += step, turn ^= 1) {
         Pair f[R][E];
-        const auto real = [&](int j) { return row0 + j * kGroups < p.rows; };
+        bool far[R] = {};
+        if (FAR) load(row0);
+        const auto real = [&](int j) { return row0 + j * kGroups < p.rows && (!FAR || far[j]); };  // written
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             values_of<T, V, P>(xr[j], f[j]);
-            if constexpr (RES) {
-                Pair g[E];
-                values_of<T, V, P>(rr[j], g);
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    float a, c;
-                    unpair(add2(f[j][i], g[i]), a, c);
-                    f[j][i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(c)));
-                }
-            }
+            if constexpr (RES) add_residual<T, V, P>(f[j], rr[j]);
         }
-        if (base + step < p.rows) {
+        if (FAR || base + step < p.rows) {
             xp += step * p.xs;
             if constexpr (RES) rp += step * p.rs;
-            load(row0 + step);
+            if (!FAR) load(row0 + step);
         }
-        if (RES && p.sum != nullptr)
+        if (RES && !FAR && p.sum != nullptr)
 #pragma unroll
             for (int j = 0; j < R; ++j) {
                 T* to = static_cast<T*>(p.sum) + (row0 + j * kGroups) * p.N;
@@ -147,29 +190,34 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
                     if (real(j)) store_row_piece(to + column(i), f[j], i, p.N, column);
             }
         if (p.norm) {
-            float v[R];
+            float v[R], mean[R];
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                Pair s = f[j][0];
-#pragma unroll
-                for (int i = 1; i < E; ++i) s = add2(s, f[j][i]);
-                v[j] = both(s);
-            }
+            for (int j = 0; j < R; ++j) v[j] = sum_of(f[j]);
             row_sums<GROUP>(v, red[turn][0]);
 #pragma unroll
             for (int j = 0; j < R; ++j) {
-                const float mean = v[j] * p.inv_n;
-                if (lane == 0 && p.mean != nullptr && real(j)) p.mean[row0 + j * kGroups] = mean;
-                const Pair nm = pair(-mean, -mean);
-#pragma unroll
-                for (int i = 0; i < E; ++i) f[j][i] = add2(f[j][i], nm);
-                clear_beyond(f[j], p.N, column);
-                Pair s = mul2(f[j][0], f[j][0]);
-#pragma unroll
-                for (int i = 1; i < E; ++i) s = fma2(f[j][i], f[j][i], s);
-                v[j] = both(s);
+                mean[j] = v[j] * p.inv_n;
+                if (!FAR && lane == 0 && p.mean != nullptr && real(j)) p.mean[row0 + j * kGroups] = mean[j];
+                v[j] = deviations(f[j], mean[j], p.N, column);
             }
             row_sums<GROUP>(v, red[turn][GROUP ? 0 : 1]);
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                far[j] = mean_far(mean[j], v[j] * p.inv_n);
+                any_far = any_far || far[j];
+            }
+            if constexpr (FAR) {
+#pragma unroll
+                for (int j = 0; j < R; ++j) v[j] = sum_of(f[j]);
+                row_sums<GROUP>(v, red[turn][0]);
+#pragma unroll
+                for (int j = 0; j < R; ++j) {
+                    const float c = __fdiv_rn(v[j], static_cast<float>(p.N));
+                    if (lane == 0 && p.mean != nullptr && real(j)) p.mean[row0 + j * kGroups] = mean[j] + c;
+                    v[j] = deviations(f[j], c, p.N, column);
+                }
+                row_sums<GROUP>(v, red[turn][GROUP ? 0 : 1]);
+            }
             if (!kKeep) weights();
 #pragma unroll
             for (int j = 0; j < R; ++j) {
@@ -206,6 +254,22 @@ __global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GRO
             }
         }
     }
+    return __any_sync(~0u, any_far);  // a block's threads have the same sums
+}
+
+// At a kernel's end, as a function: nothing is kept across it, and the kernel's registers are its own.
+template <typename T, int V, int P, int GROUP, int R, bool RES>
+__device__ __noinline__ void far_rows(const NormParams& p, float (&red)[2][GROUP ? 1 : 3][32 * R])
+{
+    norm_rows<T, V, P, GROUP, R, RES, true>(p, red);
+}
+
+template <typename T, int V, int P, int GROUP, int R, bool RES>
+__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, false), GROUP ? forward_blocks(V, P, RES) : row_blocks(V, P))
+    layer_norm_kernel(const __grid_constant__ NormParams p)
+{
+    __shared__ float red[2][GROUP ? 1 : 3][32 * R];
+    if (norm_rows<T, V, P, GROUP, R, RES, false>(p, red)) far_rows<T, V, P, GROUP, R, RES>(p, red);
 }
 
 // Rows of a residual sum, each held by a block: the rows to come lie in a ring in shared memory, filled by bulk copies.
@@ -221,7 +285,7 @@ __global__ void __launch_bounds__(row_threads(V, 2, false), 1) layer_norm_ring_k
     const Columns<V, P, 0> column;
     const uint32_t row_bytes = p.N * static_cast<uint32_t>(sizeof(T)), stage = 2 * row_bytes;
     const uint32_t to = umma::smem_addr(ring), bars = to + S * stage;
-    float* const red = reinterpret_cast<float*>(ring + static_cast<uint32_t>(S) * (stage + 8));  // [2][3][32]
+    float (&red)[2][3][32] = *reinterpret_cast<float (*)[2][3][32]>(ring + static_cast<uint32_t>(S) * (stage + 8));
     int64_t ahead = blockIdx.x;
     const auto fill = [&](int s) {  // the leader
         if (ahead >= p.rows) return;
@@ -238,8 +302,8 @@ __global__ void __launch_bounds__(row_threads(V, 2, false), 1) layer_norm_ring_k
     __syncthreads();  // the barriers are there
     int s = 0, turn = 0;
     uint32_t parity = 0;
-    bool ok = true;
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 96) {
+    bool ok = true, far = false;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         ok = ok && umma::mbar_poll(bars + s * 8, parity);  // once given up, no wait and no copy follows
         Pair f[E];
         {
@@ -254,36 +318,21 @@ __global__ void __launch_bounds__(row_threads(V, 2, false), 1) layer_norm_ring_k
                     y[i].load_shared(from + p.N + column(i));
                 }
             }
-            Pair g[E];
             values_of<T, V, P>(x, f);
-            values_of<T, V, P>(y, g);
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                float a, c;
-                unpair(add2(f[i], g[i]), a, c);
-                f[i] = pair(to_float(from_float<T>(a)), to_float(from_float<T>(c)));
-            }
+            add_residual<T, V, P>(f, y);
         }
         if (p.sum != nullptr)
 #pragma unroll
             for (int i = 0; i < P; ++i)
                 if (column(i) < p.N) store_piece<T, V>(static_cast<T*>(p.sum) + row * p.N + column(i), f, i);
-        Pair t = f[0];
-#pragma unroll
-        for (int i = 1; i < E; ++i) t = add2(t, f[i]);
-        const float mean = row_sum<0>(both(t), red + turn) * p.inv_n;
+        const float mean = row_sum<0>(sum_of(f), red[turn][0]) * p.inv_n;
         if (leader) {
             if (ok) fill(s);  // the sum's barrier: the stage has been read
             if (p.mean != nullptr) p.mean[row] = mean;
         }
-        const Pair nm = pair(-mean, -mean);
-#pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = add2(f[i], nm);
-        clear_beyond(f, p.N, column);
-        t = mul2(f[0], f[0]);
-#pragma unroll
-        for (int i = 1; i < E; ++i) t = fma2(f[i], f[i], t);
-        const float rstd = rsqrtf(fmaf(row_sum<0>(both(t), red + turn + 32), p.inv_n, p.eps));
+        const float squares = row_sum<0>(deviations(f, mean, p.N, column), red[turn][1]);
+        const float rstd = rsqrtf(fmaf(squares, p.inv_n, p.eps));
+        far = far || mean_far(mean, squares * p.inv_n);
         if (leader && p.rstd != nullptr) p.rstd[row] = rstd;
         const Pair r2 = pair(rstd, rstd);
 #pragma unroll
@@ -303,7 +352,7 @@ __global__ void __launch_bounds__(row_threads(V, 2, false), 1) layer_norm_ring_k
             }
         }
         if (p.q != nullptr) {
-            const RowScale k = row_scale(row_max<0>(largest(f), red + turn + 64));
+            const RowScale k = row_scale(row_max<0>(largest(f), red[turn][2]));
             if (leader) p.scale[row] = k.scale;
 #pragma unroll
             for (int i = 0; i < P; ++i)
@@ -319,45 +368,54 @@ __global__ void __launch_bounds__(row_threads(V, 2, false), 1) layer_norm_ring_k
         }
     }
     if (!ok) record_device_error(p.err, kErrMbarTimeout | 0x61);
+    if (__any_sync(~0u, far)) far_rows<T, V, P, 0, 1, true>(p, red);  // the same rows, the same lanes
 }
 
-// Rows of any length: a block each, read again for each step.
-template <typename T>
-__global__ void __launch_bounds__(kLongBlock) layer_norm_long_kernel(const __grid_constant__ NormParams p)
+// A row of any length by a block, read again for each step, its mean found (FAR: what that lacks as well); returns
+// whether it is far from its deviations.
+template <typename T, bool FAR>
+__device__ __forceinline__ bool norm_long_row(const NormParams& p, float (&red)[3][32])
 {
-    __shared__ float red[3][32];
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(p.x) + row * p.xs;
     const T* r = p.r == nullptr ? nullptr : static_cast<const T*>(p.r) + row * p.rs;
     const auto at = [&](int c) { return r == nullptr ? to_float(x[c]) : to_float(from_float<T>(to_float(x[c]) + to_float(r[c]))); };
-    float mean = 0.0f, rstd = 1.0f;
+    float mean = 0.0f, rest = 0.0f, rstd = 1.0f;
+    bool far = false;
     if (p.norm) {
         float s = 0.0f;
         for (int c = threadIdx.x; c < p.N; c += kLongBlock) s += at(c);
         mean = row_sum<0>(s, red[0]) * p.inv_n;
+        if constexpr (FAR) {
+            s = 0.0f;
+            for (int c = threadIdx.x; c < p.N; c += kLongBlock) s += at(c) - mean;
+            rest = __fdiv_rn(row_sum<0>(s, red[2]), static_cast<float>(p.N));
+        }
         s = 0.0f;
         for (int c = threadIdx.x; c < p.N; c += kLongBlock) {
-            const float d = at(c) - mean;
+            const float d = FAR ? at(c) - mean - rest : at(c) - mean;
             s = fmaf(d, d, s);
         }
-        rstd = rsqrtf(fmaf(row_sum<0>(s, red[1]), p.inv_n, p.eps));
+        const float variance = row_sum<0>(s, red[1]) * p.inv_n;
+        rstd = rsqrtf(variance + p.eps);
+        far = mean_far(mean, variance);
         if (threadIdx.x == 0) {
-            if (p.mean != nullptr) p.mean[row] = mean;
+            if (p.mean != nullptr) p.mean[row] = mean + rest;
             if (p.rstd != nullptr) p.rstd[row] = rstd;
         }
     }
-    if (p.sum != nullptr)
+    if (!FAR && p.sum != nullptr)
         for (int c = threadIdx.x; c < p.N; c += kLongBlock) static_cast<T*>(p.sum)[row * p.N + c] = from_float<T>(at(c));
     const auto value = [&](int c) {
         float v = at(c);
         if (!p.norm) return v;
-        v = (v - mean) * rstd;
+        v = (FAR ? v - mean - rest : v - mean) * rstd;
         if (p.w == nullptr) return v;
         return fmaf(v, to_float(static_cast<const T*>(p.w)[c]), p.b == nullptr ? 0.0f : to_float(static_cast<const T*>(p.b)[c]));
     };
     if (p.q == nullptr) {
         for (int c = threadIdx.x; c < p.N; c += kLongBlock) static_cast<T*>(p.y)[row * p.N + c] = from_float<T>(value(c));
-        return;
+        return far;
     }
     float top = 0.0f;
     for (int c = threadIdx.x; c < p.N; c += kLongBlock) top = max_nan(top, fabsf(value(c)));
@@ -365,10 +423,25 @@ __global__ void __launch_bounds__(kLongBlock) layer_norm_long_kernel(const __gri
     if (threadIdx.x == 0) p.scale[row] = k.scale;
     for (int c = threadIdx.x; c < p.N; c += kLongBlock)
         p.q[row * p.qs + c] = quantise(value(c), k.inv);
+    return far;
+}
+
+template <typename T>
+__device__ __noinline__ void far_long_row(const NormParams& p, float (&red)[3][32])
+{
+    norm_long_row<T, true>(p, red);
+}
+
+// Rows of any length, a block each.
+template <typename T>
+__global__ void __launch_bounds__(kLongBlock) layer_norm_long_kernel(const __grid_constant__ NormParams p)
+{
+    __shared__ float red[3][32];
+    if (norm_long_row<T, false>(p, red)) far_long_row<T>(p, red);
 }
 
 template <typename T, int V, int P, int GROUP, int R, bool DSUM>
-__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROUP ? kBackwardBlocks : backward_row_blocks(V, P)) layer_norm_backward_kernel(const __grid_constant__ NormParams p)
+__global__ void __launch_bounds__(GROUP ? kBlock : row_threads(V, P, true), GROUP ? kBackwardBlocks : row_blocks(V, P)) layer_norm_backward_kernel(const __grid_constant__ NormParams p)
 {
     constexpr int E = P * V / 2;
     constexpr int kGroups = GROUP ? kBlock / (GROUP ? GROUP : 1) : 1;  // rows of a block side by side
@@ -874,7 +947,7 @@ int forward(const ww_layer_norm_t& p, bool norm, int sms, const char* name, cuda
     const RowForm form = row_form(p.N, pieces ? V : pairs ? 2 : 1, 4, false);
     const auto go = [&](auto kernel, auto with_residual, int r) {
         const int groups = (form.group ? kBlock / form.group : 1) * r;
-        const int resident = form.group ? forward_blocks(form.pieces) : std::max(1, forward_threads(pieces) / form.threads);
+        const int resident = form.group ? forward_blocks(pieces ? V : 1, form.pieces, p.residual != nullptr) : std::max(1, forward_threads(pieces) / form.threads);
         const unsigned grid = even_step(std::min<int64_t>(i64(sms) * resident, (i64(p.rows) + groups - 1) / groups), i64(p.rows), form, pairs);
         if (p.residual == nullptr) kernel<<<grid, form.threads, 0, stream>>>(f);
         else with_residual<<<grid, form.threads, 0, stream>>>(f);
@@ -1029,7 +1102,7 @@ int backward(const ww_layer_norm_t& p, const BackwardPlan& plan, cudaStream_t st
     return launch_status("layer_norm_backward");
 }
 
-// What both directions check; *go = false: nothing to do.
+// What both directions check.
 int check(const ww_layer_norm_t& p, bool norm) noexcept
 {
     if (p.dtype != WW_DTYPE_HALF && p.dtype != WW_DTYPE_BF16 && p.dtype != WW_DTYPE_FLOAT) return WW_ERR_INVALID_DTYPE;
