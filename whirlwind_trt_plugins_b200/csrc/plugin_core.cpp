@@ -94,7 +94,7 @@ bool int8_linear(int use_bias, const ww_tensor_desc_t* in, ww_int8_matmul_t* p)
     return true;
 }
 
-// Descriptors without the two scales behind v.
+// The first n descriptors without the two scales behind v.
 void without_scales(const ww_tensor_desc_t* in, int n, ww_tensor_desc_t* out)
 {
     for (int i = 0; i < n; ++i)
@@ -839,7 +839,7 @@ int ww_plugin_cross_attention_int8_supports_format(int flags, int pos, const ww_
     if (pos == 1 || pos == 2) return in_out[pos].dtype == WW_DTYPE_INT8;
     if (pos == 3 || pos == 4) return in_out[pos].dtype == WW_DTYPE_FLOAT;
     ww_tensor_desc_t d[7];
-    without_scales(in_out, nb_inputs + 1, d);
+    without_scales(in_out, pos + 1, d);  // no further: callers that ask for the inputs alone have no output's descriptor
     return ww_plugin_cross_attention_supports_format(flags, pos < 3 ? pos : pos - 2, d, nb_inputs - 2, 1);
 }
 
