@@ -51,3 +51,20 @@ def test_plugins_read_the_inputs_descriptors_only():
         pytest.skip("mmap")
     r = subprocess.run([sys.executable, "-c", GUARDED], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.strip() == "done", (r.returncode, r.stderr[-500:])
+
+
+def test_linear_plugin_workspace_holds_for_smaller_sizes():
+    """What the plugin asks for its largest sizes is enough for every smaller one, whichever form that takes."""
+    from whirlwind_trt_plugins_b200 import layers, plugins as pl
+    T = pl.TensorDesc
+
+    def needed(M, K, N):
+        return layers._lib.ww_int8_matmul_workspace(layers._MATMUL.pack(16, 0, 0, 16, 16, 0, 16, 0, 0, K, K, K, pl.DTYPE_HALF, M, K, N))
+
+    assert needed(4, 4096, 9473) == 0 and needed(4, 4096, 9472) > 0
+    for M, K, N in ((4, 4096, 9473), (8, 2048, 9473), (1, 4096, 64), (1, 20000, 64), (300, 64, 33)):
+        have = pl.Int8LinearPlugin().get_workspace_size([T((M, K)), T((N, K), pl.DTYPE_INT8), T((N,), pl.DTYPE_FLOAT)])
+        for m in {1, 2, M // 2 or 1, max(1, M - 1), M}:
+            for k in {16, K // 32 * 16, K}:
+                for n in {1, N // 2, N - 1, N}:
+                    assert m > M or needed(m, k, n) <= have, (m, k, n)

@@ -732,8 +732,10 @@ int ww_plugin_int8_linear_supports_format(int use_bias, int pos, const ww_tensor
 
 int64_t ww_plugin_int8_linear_workspace(int use_bias, const ww_tensor_desc_t* in_desc)
 {
+    // An engine asks for its largest sizes: the tokens in 8 bits and their scales, which grow with every size, even where
+    // those sizes take a form without them -- smaller ones may take one with them (4 x 4096 x 9473 does not, 4 x 4096 x 9472 does).
     ww_int8_matmul_t p;
-    return int8_linear(use_bias, in_desc, &p) ? ww_int8_matmul_workspace(&p) : -1;
+    return int8_linear(use_bias, in_desc, &p) ? static_cast<int64_t>(p.M) * (p.K + 4) : -1;
 }
 
 int ww_plugin_int8_linear_enqueue(int use_bias, const ww_tensor_desc_t* in_desc, const void* const* inputs,
