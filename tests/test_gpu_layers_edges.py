@@ -3,7 +3,7 @@ implementations in 64 bits; tolerances count roundings as in test_gpu_layers.py.
 import math
 
 import pytest
-from test_gpu_layers import F, TINY, U, _int8_host, _randn, _type, _within, env  # noqa: F401
+from test_gpu_layers import F, TINY, U, _randn, _type, _weights, _within, env  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,22 @@ def test_layer_norm_far_from_zero(env, n, size):  # noqa: F811
     alone = x.clone()
     alone[~near] = x[near][0]
     assert torch.equal(ww.layer_norm(alone)[near], y[near])
+
+
+# ---------------------------------------------------------------- products
+
+@pytest.mark.parametrize("shape", [(13090, 256, 288), (9600, 256, 416), (4300, 256, 1056)])
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+def test_products_of_tiles_in_part_outside(env, shape, dt):  # noqa: F811
+    """Several narrow tiles a block, between them some whose second half lies outside the result and is not stored: what is
+    staged for the next one does not reach a store that is still under way."""
+    torch, ww = env
+    M, K, N = shape
+    t, u = _type(torch, dt), U[dt]
+    w, ws = _weights(torch, ww, N, K, 1)
+    x = _randn(torch, (M, K), 2, t)
+    xq, xs = ww.quantize_tokens(x)
+    one = (xq.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
+    for _ in range(5):
+        _within(ww.int8_matmul(xq, xs, w, ws, dtype=t), one, u * one.abs() + 2.0 ** -22 * one.abs() + TINY[dt], "out")
+    assert ww.device_error() == 0

@@ -128,8 +128,9 @@ __device__ __forceinline__ void store_tile(const void* map, uint32_t src, int x,
 {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
                  : : "l"(map), "r"(x), "r"(y), "r"(src) : "memory");
-    asm volatile("cp.async.bulk.commit_group;\n" : : : "memory");
 }
+
+__device__ __forceinline__ void commit_store() { asm volatile("cp.async.bulk.commit_group;\n" : : : "memory"); }
 
 template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
@@ -377,7 +378,11 @@ __global__ void __launch_bounds__(Tiles<BN, PAIR, U, O>::kThreads, 1) int8_matmu
                 if (p.stored) {
                     umma::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0 && x < p.N && my_row0 < p.M) store_tile(&p.c, sm + my_out, x, my_row0);
+                    // Of two buffers one is free when all groups but the last have been read, which has to be the other one's: a
+                    // chunk that lies outside the output is an empty group.
+                    const bool within = x < p.N && my_row0 < p.M;
+                    if (lane == 0 && within) store_tile(&p.c, sm + my_out, x, my_row0);
+                    if (lane == 0 && (within || L::kBuffers > 1)) commit_store();
                 } else {  // rows that do not start on 16 bytes
                     __syncwarp();
                     for (int r = 0; r < 32 && my_row0 + r < p.M; ++r) {
