@@ -93,3 +93,40 @@ def test_products_of_tiles_in_part_outside(env, shape, dt):  # noqa: F811
     for _ in range(5):
         _within(ww.int8_matmul(xq, xs, w, ws, dtype=t), one, u * one.abs() + 2.0 ** -22 * one.abs() + TINY[dt], "out")
     assert ww.device_error() == 0
+
+
+# ---------------------------------------------------------------- together
+
+def test_dispatch_modes_see_the_outputs(env):  # noqa: F811
+    """A mode that watches torch's calls (a memory counter, say) sees the tensors that the operators allocate, and the bits are the same."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    torch, ww = env
+    x, w = _randn(torch, (8, 64), 1, torch.float16), _randn(torch, (64,), 2, torch.float16)
+    q = _randn(torch, (1, 4, 2, 64), 3, torch.float16)
+    kv = _randn(torch, (1, 300, 2, 64), 4, torch.float16)
+    wq, ws = ww.quantize_tokens(_randn(torch, (32, 64), 5, torch.float16))
+    kept = [torch.empty((1, 300, 2, 64), device="cuda", dtype=torch.int8) for _ in range(2)] + [torch.empty((1, 2, 300), device="cuda") for _ in range(2)]
+    ww.quantize_kv(kv, kv, *kept)
+    angle = torch.rand((300, 32), device="cuda")
+    calls = [lambda: ww.layer_norm(x, w, return_stats=True), lambda: ww.layer_norm_int8(x, w), lambda: (ww.int8_linear(x, wq, ws),),
+             lambda: ww.cross_attention(q, kv, kv, return_lse=True), lambda: ww.cross_attention_int8(q, *kept, return_lse=True),
+             lambda: ww.qk_norm_rope(q, kv, w, w, angle.cos(), angle.sin()), lambda: ww.dequantize_kv(*kept)]
+
+    class Watch(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if isinstance(out, torch.Tensor):
+                self.seen.append(out)  # alive, so that no other one is in its place
+            return out
+
+    for call in calls:
+        plain = call()
+        with Watch() as watch:
+            got = call()
+        places = {t.untyped_storage().data_ptr() for t in watch.seen}
+        assert all(t.untyped_storage().data_ptr() in places for t in got)
+        assert all(torch.equal(a, b) for a, b in zip(got, plain))
