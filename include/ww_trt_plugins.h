@@ -499,10 +499,12 @@ int ww_dequantize_kv(const ww_kv_cache_t* p, void* stream);
  * do not matter either; those of valid places are >= 0 or NaN.  Up to 128 rows (query heads of
  * a key head x tokens) the values are used as they stand, P in fp16 with the values'
  * scales in it, unless q is fp16 and copies are expected to be faster (more than 64 rows against
- * many keys, more than 16 against short ones of many items); beyond, and then, keys and values
- * are rounded to q's type in the workspace.  Up to 128 rows run without a workspace too, as
- * they stand (fewer blocks share long keys then); copies need B * Lk * Hk * D * 4 bytes,
- * rounded up to 512, at least.
+ * many keys, more than 32 against short ones of many items); beyond, and then, keys and values
+ * are rounded to q's type in the workspace, in fp16 divided by a power of two for each head
+ * where the largest scale of its valid places asks for it, so that scales of any size are as
+ * precise.  Up to 128 rows run without a workspace too, as they stand (fewer blocks share long
+ * keys then); copies need B * Lk * Hk * D * 4 bytes, rounded up to 512, at least, and in fp16
+ * B * Hk * 8, rounded up to 256, for the powers (without them what passes fp16's range is infinite).
  * No gradients.  D a multiple of 16. */
 typedef struct ww_attention_int8 {
     ww_attention_t attention;

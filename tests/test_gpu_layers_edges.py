@@ -3,7 +3,7 @@ implementations in 64 bits; tolerances count roundings as in test_gpu_layers.py.
 import math
 
 import pytest
-from test_gpu_layers import F, TINY, U, _randn, _type, _weights, _within, env  # noqa: F401
+from test_gpu_layers import F, TINY, U, _attention_reference, _caches, _randn, _type, _weights, _within, env  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -93,6 +93,99 @@ def test_products_of_tiles_in_part_outside(env, shape, dt):  # noqa: F811
     for _ in range(5):
         _within(ww.int8_matmul(xq, xs, w, ws, dtype=t), one, u * one.abs() + 2.0 ** -22 * one.abs() + TINY[dt], "out")
     assert ww.device_error() == 0
+
+
+# ---------------------------------------------------------------- attention by 16-bit copies
+
+# (B, Lq, Lk, Hq, Hk, D): more rows a key head than are read from the 8-bit form, and fewer that are faster by copies in fp16
+MANY = [(2, 70, 300, 6, 3, 64), (3, 150, 333, 4, 4, 32), (2, 200, 1000, 2, 2, 128), (3, 45, 77, 12, 2, 48), (64, 1, 100, 160, 8, 64), (40, 48, 130, 8, 8, 32),
+        (8, 100, 1100, 8, 8, 64)]
+# factors of the keys' scales and of the values', and how far scores lie from one another
+SIZES = [(0.05, 0.05, 3.0), (2.0 ** -20, 2.0 ** -12, 3.0), (2.0 ** 10, 0.05, 3.0), (2.0 ** 60, 2.0 ** -20, 3.0), (2.0 ** -90, 2.0 ** 11, 0.5)]
+
+
+@pytest.mark.parametrize("shape", MANY)
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("form", ["plain", "masked", "biased"])
+def test_attention_by_copies(env, shape, sizes, dt, form):  # noqa: F811
+    """Keys and values rounded to 16 bits (u each) against 64 bits, whatever the sizes of their scales.  A score is off by u scale sum |q k|,
+    e for the row's largest, and its weight by exp(2 e) - 1; values by u; P by u and 2^-12 for fp32; the result by u.  In fp16 elements
+    below its normal range are off by 2^-25 where the head's largest is 2^-10 or more: 2^-15 of that; and P, whose largest is 1 or more, by
+    2^-25 a key."""
+    torch, ww = env
+    B, Lq, Lk, Hq, Hk, D = shape
+    t, u = _type(torch, dt), U[dt]
+    q = _randn(torch, (B, Lq, Hq, D), 1, t)
+    kept = _caches(torch, B, Lk, Hk, D, 2)
+    kept[2], kept[3] = kept[2] * 20 * sizes[0], kept[3] * 20 * sizes[1]
+    scale = sizes[2] / (sizes[0] * 42 * math.sqrt(D))
+    keep = torch.ones((B, Lk), device="cuda", dtype=torch.bool)
+    lens = mask = table = None
+    if form != "plain":
+        lens = torch.tensor([(Lk, Lk // 3, 0, 1, Lk + 5)[b % 5] for b in range(B)], device="cuda", dtype=torch.int32)
+        g = torch.Generator(device="cuda").manual_seed(3)
+        mask = torch.rand((B, Lk), generator=g, device="cuda") >= 0.3
+        keep = mask & (torch.arange(Lk, device="cuda")[None] < lens[:, None])
+        other = torch.where(torch.rand((B, 1, Lk), generator=g, device="cuda") < 0.5, math.nan, 1e30)
+        for i in range(2):  # what masked places hold does not matter
+            kept[2 + i] = torch.where(keep[:, None, :], kept[2 + i], other)
+    if form == "biased":
+        table = _randn(torch, (Hq, 32), 4, t)
+    more = dict(k_lens=lens, key_mask=mask, bias_table=table, max_distance=64, q_offset=3)
+    out, lse = ww.cross_attention_int8(q, *kept, scale=scale, return_lse=True, **more)
+    assert torch.equal(out, ww.cross_attention_int8(q, *kept, scale=scale, **more))
+    clean = kept[:2] + [torch.where(keep[:, None, :], c, 0.0) for c in kept[2:]]
+    ref, rl, sums, most = _attention_reference(torch, ww, q, clean, keep, table, 64, True, 3, scale)
+    size = [(clean[i].double() * clean[2 + i].double().transpose(1, 2)[..., None]).abs() for i in range(2)]
+    size = [x.repeat_interleave(Hq // Hk, 2) for x in size]
+    tiny = 2.0 ** -15 if dt == "f16" else 0.0
+    top_k, top_v = (x.amax((1, 3)) for x in size)  # of each head
+    e = scale * (u * torch.einsum("bihd,bjhd->bhij", q.double().abs(), size[0]).amax(-1) + tiny * q.double().abs().sum(-1).transpose(1, 2) * top_k[:, :, None])
+    e = e.transpose(1, 2)[..., None]
+    bound = (torch.expm1(2 * e) + 3 * u + 2.0 ** -12) * (1 + 4 * u) * sums + Lk * 2.0 ** -24 * most + tiny * top_v[:, None, :, None] + TINY[dt]
+    if dt == "f16":  # a result of 65520 or more, half a step above the largest, is an infinity of fp16 (an item of one key: its value, up to 127 x 2048)
+        beyond = (ref.abs() + bound >= 65520) & (out == torch.sign(ref) * math.inf)
+        out = torch.where(beyond, ref, out.double())
+    _within(out, ref, bound, "out")
+    empty = torch.isinf(rl)
+    assert torch.equal(torch.isinf(lse), empty) and not out.transpose(1, 2)[empty].any()
+    if (~empty).any():
+        assert ((lse.double() - rl).abs() - e[..., 0].transpose(1, 2))[~empty].max().item() <= 2.0 ** -11
+    assert ww.device_error() == 0
+
+
+def test_attention_by_copies_keeps_nonfinite_rows_apart(env):  # noqa: F811
+    """A NaN scale in a valid place reaches its head's rows, and no others; scales that are large there do not change the others' bits."""
+    torch, ww = env
+    q = _randn(torch, (2, 140, 4, 64), 1, torch.float16)
+    kept = _caches(torch, 2, 300, 2, 64, 2)
+    plain = ww.cross_attention_int8(q, *kept)
+    for which in (2, 3):
+        changed = [c.clone() for c in kept]
+        changed[which][0, 1, 77] = math.nan
+        changed[which][1, 0, 5] = 3000.0 if which == 2 else 600.0
+        out = ww.cross_attention_int8(q, *changed)
+        assert out[0, :, 2:].isnan().all() and torch.isfinite(out[1]).all()
+        assert torch.equal(out[0, :, :2], plain[0, :, :2]) and torch.equal(out[1, :, 2:], plain[1, :, 2:])
+
+
+def test_attention_by_copies_with_the_least_memory(env):  # noqa: F811
+    """A workspace of the copies alone: the same bits where fp16 holds the values."""
+    torch, ww = env
+    from whirlwind_trt_plugins_b200 import attention, layers
+    q = _randn(torch, (1, 140, 4, 64), 1, torch.float16)
+    kept = _caches(torch, 1, 900, 2, 64, 2)
+    ref = ww.cross_attention_int8(q, *kept)
+    n, st, out = 2 * 900 * 128 * 2, [900 * 128, 128, 64], torch.empty_like(q)
+    ws = torch.empty(n, device="cuda", dtype=torch.uint8)
+    a = attention._ATTN.pack(q.data_ptr(), kept[0].data_ptr(), kept[1].data_ptr(), out.data_ptr(), *[0] * 9, ws.data_ptr(), n, 140 * 256, 256, 64, *st, *st,
+                             0, 0, 0, 1, 1, 140, 900, 4, 2, 64, 0, 128, 1, 0, 0.125)
+    a += layers._SCALES.pack(kept[2].data_ptr(), kept[3].data_ptr(), 1800, 900, 1800, 900)
+    assert layers._lib.ww_cross_attention_int8(a, torch.cuda.current_stream().cuda_stream) == 0
+    # keys in other parts: either result is within P's and its own rounding (u each) and 2^-12 of the values' largest
+    most = (kept[1].double() * kept[3].double().transpose(1, 2)[..., None]).abs().max()
+    assert (out.double() - ref.double()).abs().max() <= 2 * (2 * U["f16"] + 2.0 ** -12) * most
 
 
 # ---------------------------------------------------------------- together

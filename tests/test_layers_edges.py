@@ -68,3 +68,21 @@ def test_linear_plugin_workspace_holds_for_smaller_sizes():
             for k in {16, K // 32 * 16, K}:
                 for n in {1, N // 2, N - 1, N}:
                     assert m > M or needed(m, k, n) <= have, (m, k, n)
+
+
+def test_attention_copies_of_the_least_memory():
+    """Many rows take the copies' bytes alone, as the header says; the size asked for holds the heads' powers in fp16 as well."""
+    import test_layers as t
+    import torch
+    layers, L = t._layers()
+    copies, powers = 2 * 2 * 8 * 4 * 64 * 2, 256
+    assert L.ww_cross_attention_int8_workspace(t._attention(Lq=129)) >= copies + powers
+
+    def status(have):
+        from whirlwind_trt_plugins_b200.attention import _ATTN
+        a = _ATTN.pack(*[0x1000] * 4, *[0] * 9, 0x10000, have, *[4 * 64 * 8, 4 * 64, 64] * 4, 1, 2, 129, 8, 4, 4, 64, 0, 128, 1, 0, 0.125)
+        return L.ww_cross_attention_int8(a + layers._SCALES.pack(0x1000, 0x1000, 32, 8, 32, 8), None)
+
+    assert status(copies - 1) == t.LIMIT
+    if not torch.cuda.is_available():  # past the checks a call asks for its device (the addresses are none: only where there is none)
+        assert status(copies) not in (t.OK, t.LIMIT)

@@ -86,6 +86,8 @@ struct FwdParams {
     int32_t max_entries;                   // relative positions a CTA keeps
     float scale2;                          // scale * log2(e)
     int* err;
+    const float2* powers;                  // of keys and values, [batch item][key head]
+    int32_t Hk;
 };
 
 template <int DP, int NT>
@@ -174,7 +176,8 @@ __device__ __forceinline__ void exp_pass(const uint32_t (&x)[N], float mul, floa
     else umma::tmem_st8(to, pk);
 }
 
-template <typename T, int DP, int NT>
+// POWERS: keys and values come divided by powers of two, which scores and results take back.
+template <typename T, int DP, int NT, bool POWERS>
 __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCtas)
     attention_forward_kernel(const __grid_constant__ FwdParams p)
 {
@@ -446,6 +449,8 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
         int number = 0;
         for (int qi = 0; qi < nq && t < tiles_of(qi); ++qi) {
             const int q0 = q_of(qi), i = q0 + t * kTile + r;
+            const auto power = [&] { return p.powers + static_cast<int64_t>(batch_of(qi)) * p.Hk + p.by_group.div(h); };
+            const float scale2 = POWERS ? p.scale2 * __ldg(&power()->x) : p.scale2;
             float m = -INFINITY;
             Pair l2 = pair(0.0f, 0.0f);  // sums of the even and of the odd columns
             const bool any_row = q0 + t * kTile + warp % 4 * 32 < p.Lq;  // else this warp keeps the barriers only
@@ -467,7 +472,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 umma::fence_after_sync();
                 const int chunks = any_row ? (cols + 31) / 32 : 0;
                 // raw scores: scale and constant join the exponential's argument
-                const bool plain = whole && mine == nullptr && p.scale2 >= 0.0f && flat > -INFINITY;
+                const bool plain = whole && mine == nullptr && scale2 >= 0.0f && flat > -INFINITY;
                 float top = -INFINITY, add;
                 const float* lim = limits + s * KT;
                 const auto largest = [&](auto raw_scores, int c, auto& x) {  // of the N columns from c on
@@ -483,18 +488,18 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                     } else {
                         float tc;
                         if (mine == nullptr)
-                            tc = whole ? score_pass<false, false>(x, p.scale2, flat, nullptr, nullptr)
-                                       : score_pass<false, true>(x, p.scale2, flat, nullptr, lim + c);
+                            tc = whole ? score_pass<false, false>(x, scale2, flat, nullptr, nullptr)
+                                       : score_pass<false, true>(x, scale2, flat, nullptr, lim + c);
                         else
-                            tc = whole ? score_pass<true, false>(x, p.scale2, 0.0f, mine + c, nullptr)
-                                       : score_pass<true, true>(x, p.scale2, 0.0f, mine + c, lim + c);
+                            tc = whole ? score_pass<true, false>(x, scale2, 0.0f, mine + c, nullptr)
+                                       : score_pass<true, true>(x, scale2, 0.0f, mine + c, lim + c);
                         top = fmaxf(top, tc);
                         if constexpr (N == 32) umma::tmem_st32(s_col + c, x);
                         else umma::tmem_st16(s_col + c, x);
                     }
                 };
                 const auto exps = [&](auto raw_scores, int c, const auto& x) {  // P of N columns, over scores that have been read
-                    if (raw_scores) exp_pass<T, true>(x, p.scale2, add, l2, s_col + c / 2);
+                    if (raw_scores) exp_pass<T, true>(x, scale2, add, l2, s_col + c / 2);
                     else exp_pass<T, false>(x, 1.0f, add, l2, s_col + c / 2);
                 };
                 const auto columns = [&](const auto& use, auto raw_scores) {
@@ -532,7 +537,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
                 };
                 pass(largest);
                 if (!plain) umma::tmem_wait_st();
-                if (plain) top = fmaf(top, p.scale2, flat);
+                if (plain) top = fmaf(top, scale2, flat);
                 // grow the maximum: always on the first tile, then only past kRescale.  A NaN score (of
                 // raw ones; others keep it to the sum) or one of +inf makes it NaN, and with it the row.
                 if (__any_sync(~0u, kt == 0 || !(top <= m + kRescale))) {
@@ -566,7 +571,7 @@ __global__ void __launch_bounds__(Layout<DP, NT>::kThreads, Layout<DP, NT>::kCta
             unpair(l2, l_even, l_odd);
             float sum = l_even + l_odd;
             if (m == -INFINITY && sum < 1.0f) sum = 0.0f;  // scores of -inf alone: an empty row
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float inv = (sum == 0.0f ? 0.0f : 1.0f / sum) * (POWERS ? __ldg(&power()->y) : 1.0f);
             const int64_t b = batch_of(qi), row = (b * p.Lq + i) * p.Hq + h;
             const int64_t part = (static_cast<int64_t>(item - p.whole_items) * p.splits + split) * (NT * kTile) + t * kTile + r;
 #pragma unroll
@@ -759,19 +764,23 @@ template <typename T, int DP, int NT>
 int launch(const FwdParams& f, int64_t ctas, cudaStream_t stream) noexcept
 {
     using L = Layout<DP, NT>;
-    const auto kernel = attention_forward_kernel<T, DP, NT>;
+    // only fp16's range is too narrow for some keys and values
+    auto kernel = attention_forward_kernel<T, DP, NT, false>;
+    if constexpr (std::is_same<T, __half>::value)
+        if (f.powers != nullptr) kernel = attention_forward_kernel<T, DP, NT, true>;
     static_assert(L::kTotal + 4 * ((kMaxPositions + 15) / 16 * 16) <= kMaxShared, "shared memory");
     const int bytes = L::kTotal + 4 * f.max_entries;
-    static std::atomic<uint64_t> raised{0};
-    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised)) return launch_status("cross_attention");
+    static std::atomic<uint64_t> raised[2];
+    if (!allow_shared_memory(reinterpret_cast<const void*>(kernel), raised[f.powers != nullptr])) return launch_status("cross_attention");
     kernel<<<static_cast<unsigned>(ctas), L::kThreads, bytes, stream>>>(f);
     return launch_status("cross_attention");
 }
 
 template <typename T>
-int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_lse, cudaStream_t stream) noexcept
+int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_lse, const float2* powers, cudaStream_t stream) noexcept
 {
     FwdParams f;
+    f.powers = powers;
     const int dp = p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128;
     constexpr bool bf = !std::is_same<T, __half>::value;
     const int nq[3] = {p.B, p.Lq, p.Hq}, nk[3] = {p.B, p.Lk, p.Hk};
@@ -799,6 +808,7 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
     f.Lq = p.Lq;
     f.Lk = p.Lk;
     f.Hq = p.Hq;
+    f.Hk = p.Hk;
     f.group = p.Hq / p.Hk;
     f.D = p.D;
     f.q_blocks = plan.q_blocks;
@@ -829,12 +839,12 @@ int tiles(const ww_attention_t& p, const Plan& plan, float* part_o, float* part_
 }
 
 template <typename T>
-int forward(const ww_attention_t& p, const Plan& plan, cudaStream_t stream) noexcept
+int forward(const ww_attention_t& p, const Plan& plan, const float2* powers, cudaStream_t stream) noexcept
 {
     float* part_o = static_cast<float*>(p.workspace);
     float* part_lse = part_o + plan.part_rows() * p.D;
     const int st = plan.token ? attention_token_launch(p, plan.splits, part_o, part_lse, stream)
-                              : tiles<T>(p, plan, part_o, part_lse, stream);
+                              : tiles<T>(p, plan, part_o, part_lse, powers, stream);
     if (st != WW_SUCCESS || plan.rest == 0) return st;
     launch_behind(attention_join_kernel<T>, dim3(plan.rest, (plan.rows + 3) / 4), dim3(128), 0, stream, part_o, part_lse, p.out,
                   p.lse, plan.whole, plan.splits, plan.rows, plan.q_blocks, p.Lq, p.Hq, p.Hk, p.D);
@@ -861,6 +871,20 @@ int attention_join_launch(const ww_attention_t& p, int items, int splits, int ro
     return launch_status(name);
 }
 
+int cross_attention(const ww_attention_t& p, const float2* powers, void* stream) noexcept
+{
+    int st = check_attention(p);
+    if (st != WW_SUCCESS || p.B == 0 || p.Lq == 0) return st;
+    DeviceInfo d;
+    if ((st = current_device_info(&d)) != WW_SUCCESS) return st;
+    Plan plan;
+    if (!make_plan(p, d.sm_count, &plan)) return WW_ERR_UNSUPPORTED;
+    if (p.workspace == nullptr) plan.without_parts();
+    else if (plan.part_bytes(p.D) > p.workspace_bytes) return WW_ERR_UNSUPPORTED;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return p.dtype == WW_DTYPE_HALF ? forward<__half>(p, plan, powers, s) : forward<__nv_bfloat16>(p, plan, nullptr, s);
+}
+
 }  // namespace ww
 
 extern "C" {
@@ -874,17 +898,7 @@ int64_t ww_cross_attention_workspace(const ww_attention_t* p)
 
 int ww_cross_attention(const ww_attention_t* p, void* stream)
 {
-    if (p == nullptr) return WW_ERR_NULL_POINTER;
-    int st = ww::check_attention(*p);
-    if (st != WW_SUCCESS || p->B == 0 || p->Lq == 0) return st;
-    ww::DeviceInfo d;
-    if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
-    ww::Plan plan;
-    if (!ww::make_plan(*p, d.sm_count, &plan)) return WW_ERR_UNSUPPORTED;
-    if (p->workspace == nullptr) plan.without_parts();
-    else if (plan.part_bytes(p->D) > p->workspace_bytes) return WW_ERR_UNSUPPORTED;
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return p->dtype == WW_DTYPE_HALF ? ww::forward<__half>(*p, plan, s) : ww::forward<__nv_bfloat16>(*p, plan, s);
+    return p == nullptr ? WW_ERR_NULL_POINTER : ww::cross_attention(*p, nullptr, stream);
 }
 
 }  // extern "C"

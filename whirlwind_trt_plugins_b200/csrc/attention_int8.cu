@@ -34,7 +34,7 @@
 
 namespace ww {
 
-int dequantise_valid(const ww_kv_cache_t& p, const char* name, void* stream) noexcept;  // kv_cache.cu
+int dequantise_valid(const ww_kv_cache_t& p, const uint8_t* mask, float2* powers, const char* name, void* stream) noexcept;  // kv_cache.cu
 
 namespace {
 
@@ -541,19 +541,18 @@ struct Plan {
     }
 };
 
-// Copies cost 5 bytes a value and two launches, but are converted once for all rows.  us in 8 bits and by copies:
-// more than 64 rows (converted 3 or 4 times), 8 x 8 key heads of 64 and 128, 1500 keys, 128 rows 31 and 29, 45 and 38,
-// 1 x 8, 40001 keys 77 and 64, 117 and 93 -- but 1 x 4, 300 keys 12 both; 64 rows 22 and 24, 30 and 33, 47 and 57, 69 and 89.
-// Short keys of more blocks than are resident (a block's start and end): 64 x 8 of 64 and 128, 100 keys, 32 rows 20 and
-// 15, 25 and 22, 48 rows 34 and 15, 44 and 22; 16 rows 12 and 15, 16 and 22; 1250 keys, 32 rows 53 and 84, 81 and 160.
-constexpr int64_t kManyKeys = 1 << 16;  // of all items and key heads
+// Copies cost 5 bytes a value and three launches, but are converted once for all rows.  us in 8 bits and by copies:
+// more than 64 rows (converted 3 or 4 times), 8 x 8 key heads of 64 and 128, 1500 keys, 128 rows 33 and 38, 48 and 46,
+// 1 x 8, 40001 keys 80 and 76, 120 and 105.
+// Short keys of more blocks than are resident (a block's start and end): 64 x 8, 100 keys, 32 rows of 64 21 and 21, 48 rows of 128 46 and 27.
+constexpr int64_t kManyKeys = 1 << 17;  // of all items and key heads
 constexpr int kShortKeys = 512;
 bool by_copies(const ww_attention_t& p, int64_t rows, int sms) noexcept
 {
     if (rows > kMostRows) return true;
     if (p.dtype == WW_DTYPE_BF16) return false;  // whose rounding of keys and values shows: 0.4 % of the result, 0.17 its own
     const int64_t heads = i64(p.B) * p.Hk, row_blocks = (rows + 31) / 32;
-    return (rows > 64 && heads * p.Lk >= kManyKeys) || (rows > 16 && p.Lk < kShortKeys && p.Lk > 0 && heads * row_blocks > 2 * sms);
+    return (rows > 64 && heads * p.Lk >= kManyKeys) || (rows > 32 && p.Lk < kShortKeys && p.Lk > 0 && heads * row_blocks > 2 * sms);
 }
 
 Plan make_plan(const ww_attention_t& p, int sms, bool copies_fit = true) noexcept
@@ -576,19 +575,25 @@ Plan make_plan(const ww_attention_t& p, int sms, bool copies_fit = true) noexcep
 
 int64_t aligned(int64_t n) noexcept { return (n + 255) / 256 * 256; }
 
-// Workspace of the 16-bit form: keys, values, then that of ww_cross_attention.
+// Workspace of the 16-bit form: (powers,) keys, values, then that of ww_cross_attention.
 int64_t copy_bytes(const ww_attention_t& p) noexcept { return aligned(i64(p.B) * p.Lk * p.Hk * p.D * 2); }
 
-ww_attention_t of_copies(const ww_attention_int8_t& a) noexcept
+// In front of them in fp16, whose range is narrower than the scales': a power of two for each head's keys and values, by which
+// the copies are divided and which scores and results take back.  A workspace of the copies alone does without.
+int64_t power_bytes(const ww_attention_t& p) noexcept { return p.dtype == WW_DTYPE_HALF ? aligned(i64(p.B) * p.Hk * 8) : 0; }
+
+ww_attention_t of_copies(const ww_attention_int8_t& a, bool powers) noexcept
 {
     ww_attention_t p = a.attention;
     char* ws = static_cast<char*>(p.workspace);
     const int64_t n = copy_bytes(p);
     if (ws == nullptr) ws = reinterpret_cast<char*>(static_cast<uintptr_t>(256));  // sizes only
+    const int64_t before = powers ? power_bytes(p) : 0;
+    ws += before;
     p.k = ws;
     p.v = ws + n;
     p.workspace = ws + 2 * n;
-    p.workspace_bytes -= 2 * n;
+    p.workspace_bytes -= 2 * n + before;
     for (int64_t* s : {p.k_strides, p.v_strides}) {
         s[0] = i64(p.Lk) * p.Hk * p.D;
         s[1] = i64(p.Hk) * p.D;
@@ -602,8 +607,8 @@ int64_t workspace(const ww_attention_int8_t& a, const Plan& plan) noexcept
     const ww_attention_t& p = a.attention;
     if (p.B == 0 || p.Lq == 0) return 0;
     if (plan.few) return plan.part_rows(p) * (p.D + 1) * 4;
-    const ww_attention_t q = of_copies(a);
-    return 2 * copy_bytes(p) + ww_cross_attention_workspace(&q);
+    const ww_attention_t q = of_copies(a, true);
+    return power_bytes(p) + 2 * copy_bytes(p) + ww_cross_attention_workspace(&q);
 }
 
 int check(const ww_attention_int8_t& a) noexcept
@@ -714,7 +719,8 @@ int ww_cross_attention_int8(const ww_attention_int8_t* a, void* stream)
     if ((st = ww::current_device_info(&d)) != WW_SUCCESS) return st;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (plan.few) return p.dtype == WW_DTYPE_HALF ? ww::few_rows<__half>(*a, plan, s) : ww::few_rows<__nv_bfloat16>(*a, plan, s);
-    ww_attention_t q = ww::of_copies(*a);
+    const bool has_powers = p.Lk > 0 && ww::power_bytes(p) > 0 && ww::power_bytes(p) + 2 * ww::copy_bytes(p) <= p.workspace_bytes;
+    ww_attention_t q = ww::of_copies(*a, has_powers);
     if (ww_cross_attention_workspace(&q) > q.workspace_bytes) q.workspace = nullptr;  // keys are not split then
     ww_kv_cache_t c{};
     c.k_cache = static_cast<int8_t*>(const_cast<void*>(p.k));
@@ -737,8 +743,9 @@ int ww_cross_attention_int8(const ww_attention_int8_t* a, void* stream)
     c.places = p.Lk;
     c.H = p.Hk;
     c.D = p.D;
-    if (p.Lk > 0 && (st = ww::dequantise_valid(c, "cross_attention_int8", stream)) != WW_SUCCESS) return st;
-    return ww_cross_attention(&q, stream);
+    float2* powers = has_powers ? static_cast<float2*>(p.workspace) : nullptr;
+    if (p.Lk > 0 && (st = ww::dequantise_valid(c, p.key_mask, powers, "cross_attention_int8", stream)) != WW_SUCCESS) return st;
+    return ww::cross_attention(q, powers, stream);
 }
 
 }  // extern "C"

@@ -19,6 +19,11 @@ int token_splits(const ww_attention_t& p, int sms) noexcept;
 int attention_token_launch(const ww_attention_t& p, int splits, float* part_o, float* part_lse,
                            cudaStream_t stream) noexcept;
 
+// ww_cross_attention.  `powers`, not nullptr only for fp16 calls that are not of the token form: keys and values come divided by
+// powers of two, which scores and results take back: what those of each (batch item, key head) are to be multiplied by,
+// [B][Hk] {keys, values}.  (attention_forward.cu)
+int cross_attention(const ww_attention_t& p, const float2* powers, void* stream) noexcept;
+
 // Joins such parts into out and lse; launched behind the kernel that writes them
 // (attention_forward.cu).
 int attention_join_launch(const ww_attention_t& p, int items, int splits, int rows, const float* part_o, const float* part_lse,

@@ -12,6 +12,8 @@
 // 88 us, read back (492 MB) in 83: 5.6 and 5.9 TB/s.
 #include "rows.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 namespace ww {
@@ -35,6 +37,8 @@ struct CacheParams {
     const int32_t *start, *lens;
     Divisor L, H;  // tokens (reading: places) of an item, heads
     int32_t rows, places, D, keep;  // keep: what lies behind the lens is not written (reading)
+    const uint8_t* mask;            // [B][places] of the keys that count, or
+    float2* powers;                 // [B][H] of keys and values that are read back divided by powers of two
 };
 
 struct CacheRow {
@@ -94,6 +98,75 @@ __global__ void __launch_bounds__(kBlock) quantize_kv_kernel(const __grid_consta
     }
 }
 
+// The power of two by which a head's keys or values are divided in fp16, whose range is narrower than the scales': the largest
+// comes to [2^8, 2^9) 127, or stays what it is where fp16 holds it with 5 bits to spare above its subnormal numbers.
+__device__ __forceinline__ float power_of(float top)
+{
+    if (top == 0.0f || (top >= 0x1p-17f && top < 0x1p9f)) return 1.0f;
+    const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 8;
+    return __uint_as_float(static_cast<uint32_t>(127 + min(max(e, -100), 113)) << 23);
+}
+
+// Those of all heads, keys and values in turn (rows [B][H][2]): a warp for each, or where places are many a cluster of blocks.
+// Bound: latency, a few loads after one another: 8 heads of 40001 places 7 us, 12032 of 312 10.5.
+constexpr int kWarpPlaces = 1024, kMostBlocks = 8;
+
+template <bool MANY>
+__global__ void __launch_bounds__(MANY ? 1024 : kBlock) kv_powers_kernel(const __grid_constant__ CacheParams p, int rows)
+{
+    __shared__ float red[32], joined;
+    start_launch_behind();  // reading back waits for this grid's end
+    const auto cluster = cooperative_groups::this_cluster();
+    const int blocks = MANY ? static_cast<int>(cluster.num_blocks()) : 1, rank = MANY ? static_cast<int>(cluster.block_rank()) : 0;
+    const int row = MANY ? blockIdx.x / blocks : blockIdx.x * (kBlock / 32) + threadIdx.x / 32;
+    float top = 0.0f;
+    if (row < rows) {
+        const int b = p.H.div(row / 2), h = row / 2 - b * p.H.d;
+        const CacheSide& s = p.side[row % 2];
+        const float* scale = s.scale + b * s.sb + h * s.sh;
+        const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + static_cast<int64_t>(b) * p.places;
+        const int len = p.lens == nullptr ? p.places : min(__ldg(p.lens + b), p.places);
+#pragma unroll 8
+        for (int at = MANY ? rank * 1024 + threadIdx.x : threadIdx.x % 32; at < len; at += MANY ? blocks * 1024 : 32) {
+            const float x = fabsf(__ldg(scale + at));
+            const bool counts = mask == nullptr || __ldg(mask + at) != 0;
+            top = counts && x < INFINITY ? fmaxf(top, x) : top;
+        }
+    }
+    top = row_max<MANY ? 0 : 32>(top, red);
+    if constexpr (MANY) {
+        if (threadIdx.x == 0) joined = top;
+        cluster.sync();
+        if (rank == 0 && threadIdx.x == 0)
+            for (int i = 1; i < blocks; ++i) top = fmaxf(top, *cluster.map_shared_rank(&joined, i));
+        cluster.sync();  // until it has been read
+    }
+    if (row < rows && rank == 0 && (MANY ? threadIdx.x : threadIdx.x % 32) == 0) reinterpret_cast<float*>(p.powers)[row] = power_of(top);
+}
+
+int launch_powers(const CacheParams& f, const char* name, cudaStream_t stream) noexcept
+{
+    const int rows = f.rows / f.places * 2;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(std::min(kMostBlocks, (f.places + 4095) / 4096));
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.stream = stream;
+    if (f.places > kWarpPlaces) {
+        cfg.gridDim = dim3(static_cast<unsigned>(rows) * attr.val.clusterDim.x);
+        cfg.blockDim = dim3(1024);
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, kv_powers_kernel<true>, f, rows);
+    } else {
+        cfg.gridDim = dim3((rows + kBlock / 32 - 1) / (kBlock / 32));
+        cfg.blockDim = dim3(kBlock);
+        cudaLaunchKernelEx(&cfg, kv_powers_kernel<false>, f, rows);
+    }
+    return launch_status(name);
+}
+
 template <typename T, int GROUP>
 __global__ void __launch_bounds__(kBlock) dequantize_kv_kernel(const __grid_constant__ CacheParams p)
 {
@@ -104,6 +177,7 @@ __global__ void __launch_bounds__(kBlock) dequantize_kv_kernel(const __grid_cons
     if (d >= p.D) return;
     uint2 q[kRows];
     float scale[kRows];
+    int head[kRows];
     bool put[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
@@ -111,13 +185,23 @@ __global__ void __launch_bounds__(kBlock) dequantize_kv_kernel(const __grid_cons
         put[i] = row < p.rows;
         q[i] = make_uint2(0, 0);
         scale[i] = 0.0f;
+        head[i] = 0;
         if (!put[i]) continue;
         const CacheRow at(p, static_cast<int>(row));
+        head[i] = at.b * p.H.d + at.h;
         if (p.lens == nullptr || at.l < __ldg(p.lens + at.b)) {
             q[i] = __ldg(reinterpret_cast<const uint2*>(s.q + at.b * s.qb + at.l * s.ql + at.h * s.qh + d));
             scale[i] = __ldg(s.scale + at.b * s.sb + at.h * s.sh + at.l);
         } else if (p.keep) {
             put[i] = false;
+        }
+    }
+    if (p.powers != nullptr) {
+        wait_for_launches_before();
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const float power = reinterpret_cast<const float*>(p.powers + head[i])[blockIdx.y];
+            scale[i] *= __uint_as_float((254u << 23) - __float_as_uint(power));  // 1 / power
         }
     }
 #pragma unroll
@@ -158,7 +242,13 @@ int launch(const CacheParams& f, const char* name, cudaStream_t stream) noexcept
 {
     const int group = f.D <= 32 ? 4 : f.D <= 64 ? 8 : 16, step = kBlock / group * (WRITE ? kWriteRows : kRows);
     const dim3 grid(static_cast<unsigned>((i64(f.rows) + step - 1) / step), 2);
-    const auto go = [&](auto kernel) { kernel<<<grid, kBlock, 0, stream>>>(f); };
+    if (f.powers != nullptr) {
+        if (const int st = launch_powers(f, name, stream); st != WW_SUCCESS) return st;
+    }
+    const auto go = [&](auto kernel) {
+        if (f.powers != nullptr) launch_behind(kernel, grid, dim3(kBlock), 0, stream, f);
+        else kernel<<<grid, kBlock, 0, stream>>>(f);
+    };
     if constexpr (WRITE) {
         if (group == 4) go(quantize_kv_kernel<T, 4>);
         else if (group == 8) go(quantize_kv_kernel<T, 8>);
@@ -201,8 +291,15 @@ int check(const ww_kv_cache_t& p, bool write) noexcept
     return WW_SUCCESS;
 }
 
+// What reading back for an attention call adds: see dequantise_valid.
+struct Valid {
+    bool keep = false;
+    const uint8_t* mask = nullptr;
+    float2* powers = nullptr;
+};
+
 template <bool WRITE>
-int run(const ww_kv_cache_t* p, bool keep, const char* name, void* stream) noexcept
+int run(const ww_kv_cache_t* p, const Valid& valid, const char* name, void* stream) noexcept
 {
     if (p == nullptr) return WW_ERR_NULL_POINTER;
     int st = check(*p, WRITE);
@@ -211,21 +308,27 @@ int run(const ww_kv_cache_t* p, bool keep, const char* name, void* stream) noexc
     DeviceInfo d;
     if ((st = current_device_info(&d)) != WW_SUCCESS) return st;
     CacheParams f = params(*p, tokens);
-    f.keep = keep;
+    f.keep = valid.keep;
+    f.mask = valid.mask;
+    f.powers = valid.powers;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return p->dtype == WW_DTYPE_HALF ? launch<WRITE, __half>(f, name, s) : launch<WRITE, __nv_bfloat16>(f, name, s);
 }
 
 }  // namespace
 
-// ww_dequantize_kv that leaves what lies behind the lens unwritten.
-int dequantise_valid(const ww_kv_cache_t& p, const char* name, void* stream) noexcept { return run<false>(&p, true, name, stream); }
+// ww_dequantize_kv that leaves what lies behind the lens unwritten.  With `powers` [B][H] it divides the keys and values of each
+// item's head by powers of two, of the scales in valid places (mask [B][places], nullptr for all), and leaves those there.
+int dequantise_valid(const ww_kv_cache_t& p, const uint8_t* mask, float2* powers, const char* name, void* stream) noexcept
+{
+    return run<false>(&p, {true, mask, powers}, name, stream);
+}
 
 }  // namespace ww
 
 extern "C" {
 
-int ww_quantize_kv(const ww_kv_cache_t* p, void* stream) { return ww::run<true>(p, false, "quantize_kv", stream); }
-int ww_dequantize_kv(const ww_kv_cache_t* p, void* stream) { return ww::run<false>(p, false, "dequantize_kv", stream); }
+int ww_quantize_kv(const ww_kv_cache_t* p, void* stream) { return ww::run<true>(p, {}, "quantize_kv", stream); }
+int ww_dequantize_kv(const ww_kv_cache_t* p, void* stream) { return ww::run<false>(p, {}, "dequantize_kv", stream); }
 
 }  // extern "C"

@@ -132,11 +132,11 @@ bool attention_int8(int flags, const ww_tensor_desc_t* in, ww_attention_int8_t* 
     return true;
 }
 
-// Bytes of the 16-bit copies that ww_cross_attention_int8 makes for many rows.
+// Bytes of the 16-bit copies that ww_cross_attention_int8 makes for many rows, with their powers of two.
 int64_t attention_copies(const ww_attention_t& a)
 {
-    const int64_t one = static_cast<int64_t>(a.B) * a.Lk * a.Hk * a.D * 2;
-    return 2 * ((one + 255) / 256 * 256);
+    const int64_t heads = static_cast<int64_t>(a.B) * a.Hk, one = heads * a.Lk * a.D * 2;
+    return 2 * ((one + 255) / 256 * 256) + (heads * 8 + 255) / 256 * 256;
 }
 
 }  // namespace

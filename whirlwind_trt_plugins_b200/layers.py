@@ -303,7 +303,8 @@ def int8_matmul(x_q, x_scale, w_q, w_scale, bias=None, dtype=None, out=None, str
 def int8_linear(x, w_q, w_scale, bias=None, out=None, stream=None):
     """x @ w.T + bias in 8-bit integers: the rows of x [..., K] (fp16, bf16 or fp32) are
     brought to 8 bits as by ``quantize_tokens``, then ``int8_matmul`` with the
-    weights w_q [N, K] and w_scale [N]; the result has x's type."""
+    weights w_q [N, K] and w_scale [N]; the result has x's type.  No gradients: it is
+    not part of autograd's graph, x's or bias's neither."""
     return _matmul(x, None, w_q, w_scale, bias, None, out, stream)
 
 
@@ -391,8 +392,9 @@ def cross_attention_int8(q, k_cache, v_cache, k_scale, v_scale, scale: float | N
     [B, Lq, Hq, D] fp16 or bf16, D a multiple of 16 up to 128; the other arguments
     are those of ``cross_attention``.  Places from k_lens on, and masked ones, may
     hold anything.  Calls of few query rows per key head (up to 128, in fp16 where it is
-    faster) read each key and value as a byte; others round them to q's type first.
-    No gradients."""
+    faster) read each key and value as a byte; others round them to q's type first, in
+    fp16 divided by a power of two for each head where its scales are large or small.
+    No gradients: the result is not part of autograd's graph."""
     T = _Torch.get()
     at = _first(q, "q")
     dtype = q.dtype
