@@ -651,7 +651,7 @@ int ww_plugin_layer_norm_enqueue(int use_residual, int eps_nano, const ww_tensor
 /* "Int8Linear" v"1" (extension): ww_int8_matmul of activations.  Inputs x [..., K] (fp16, bf16 or
  * fp32), w_q [N, K] INT8 with K a multiple of 16, w_scale [N] fp32 and with use_bias bias [N] of
  * x's type; output [..., N] of x's type.  Field use_bias (0).  `workspace` holds
- * ww_plugin_int8_linear_workspace bytes (-1: no such inputs), which grow with the rows of x. */
+ * ww_plugin_int8_linear_workspace bytes for inputs of at least these sizes (-1: no such inputs). */
 int ww_plugin_int8_linear_output_dims(int use_bias, int nb_inputs, const ww_tensor_desc_t* inputs,
                                       ww_tensor_desc_t* out);
 int ww_plugin_int8_linear_supports_format(int use_bias, int pos, const ww_tensor_desc_t* in_out, int nb_inputs,

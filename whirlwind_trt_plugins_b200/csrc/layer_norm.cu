@@ -23,7 +23,7 @@
 // Measured: 469248 rows of 256, fp16, 480 MB: 78 us, 6.1 TB/s; their gradient with dsum,
 // bf16, 961 MB: 153 us with the join, 6.3 TB/s.  Gradient of 9001 rows of 1337, fp32, 144 MB:
 // 31 us (single loads; pieces of 16 bytes with the rows' ends masked took 52).
-// 40000 rows of 1337 in fp16, single loads of 2 bytes: 77 us for 214 MB, instructions.
+// 40000 rows of 1337 in fp16, single loads of 2 bytes: 82 us for 214 MB, instructions.
 #include "rows.cuh"
 #include "umma.cuh"
 
@@ -875,7 +875,7 @@ bool in_pieces(const ww_layer_norm_t& p, int bytes) noexcept
 
 // Rows of pairs: every tensor's row begins on the grid of two values, or every one off it.  For rows of which a lane
 // holds 16 values; us by single values and by pairs: 8000 rows of 5001, fp16, 75 and 64, 4000 in fp32 38 and 30, gradients
-// of 6000 198 and 123, of 3000 in fp32 124 and 88; but 40000 of 1337, fp16, 77 and 113, gradients of 401 74 and 78, of 1337 70 and 76.
+// of 6000 198 and 123, of 3000 in fp32 124 and 88; but 40000 of 1337, fp16, 82 and 113, gradients of 401 74 and 78, of 1337 70 and 76.
 constexpr int kPairs = 2048;
 bool in_pairs(const ww_layer_norm_t& p, int bytes) noexcept
 {
