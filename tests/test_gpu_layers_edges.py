@@ -223,3 +223,38 @@ def test_dispatch_modes_see_the_outputs(env):  # noqa: F811
         places = {t.untyped_storage().data_ptr() for t in watch.seen}
         assert all(t.untyped_storage().data_ptr() in places for t in got)
         assert all(torch.equal(a, b) for a, b in zip(got, plain))
+
+
+def test_copies_and_far_rows_captured(env):  # noqa: F811
+    """Attention by copies (three kernels behind one another) and a norm whose rows turn far from zero, captured twice and replayed at once on
+    two streams on changed inputs: the bits of eager calls."""
+    torch, ww = env
+    x = [_randn(torch, (700, 264), s, torch.float16) for s in (1, 2)]
+    q = [_randn(torch, (2, 140, 4, 64), s, torch.float16) for s in (3, 4)]
+    kept = [_caches(torch, 2, n, 2, 64, n) for n in (900, 3000)]
+    lens = torch.tensor([900, 333], device="cuda", dtype=torch.int32)
+    step = lambda i: (ww.layer_norm(x[i]), ww.cross_attention_int8(q[i], *kept[i], k_lens=lens))  # noqa: E731
+    for i in (0, 1):
+        step(i)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in (0, 1):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i))
+        graphs.append(g)
+    x[0][::3] = 7.0
+    kept[0][2][1] *= 2.0 ** 20
+    kept[1][3][0] *= 2.0 ** -30
+    lens.copy_(torch.tensor([17, 900], dtype=torch.int32))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], step(i)))
+    assert not outs[0][0][::3].any() and all(torch.isfinite(o[1]).all() for o in outs)
+    assert ww.device_error() == 0
